@@ -289,6 +289,65 @@ void k_random_q8(int8_t *q, float *s, int rows, int cols, size_t row0, size_t co
                  unsigned long long seed, unsigned long long tensor, float std, int gs);
 void k_fill(float *x, size_t n, float value);
 
+/* ---- a batch of requests over one prompt (no counterpart in the reference, which serves one sequence) ------------ */
+/* Attention of `batch` requests that share a prefix. q and out are [batch][rows][n_heads * head_dim]; the prefix lies
+ * in one head-major cache [n_kv_heads][prefix_seq_len][head_dim] (one layer of an engine's, say), positions
+ * [0, prefix); each request's own positions in its cache of [batch][n_kv_heads][seq_len][head_dim]. Row r of request b
+ * (its last token and its drafts, say) sees the prefix and own positions [0, starts[b] + r]: starts[b] positions were
+ * stored before this step's rows. counts[b] (NULL: all) says how many of the rows request b uses, 0 .. rows; the other
+ * rows of out are left as they were, and a request that uses none needs no starts[b]. starts and counts are device
+ * memory, so a captured step replays as the requests grow. starts[b] outside [0, seq_len - counts[b]] or counts[b]
+ * outside [0, rows] raises an error (kc_status) and leaves the request's rows as they were. What a row sees must be
+ * finite; what it does not see is never read into it. oq / os (may be NULL): out quantized for Wo as k_quantize does,
+ * gs dividing head_dim. The prefix is read once for the whole batch. head_dim <= 256.
+ * `work` (k_attention_shared_init, released with k_attention_free): partial results for this n_heads and head_dim and
+ * at most what its batch and rows need; `memory` as for k_attention_init_rows (k_attention_shared_bytes bytes, or
+ * NULL). One call in flight per work. */
+size_t k_attention_shared_bytes(int n_heads, int n_kv_heads, int head_dim, int batch, int rows);
+void k_attention_shared_init(AttentionWork *work, int n_heads, int n_kv_heads, int head_dim, int batch, int rows,
+                             void *memory);
+void k_attention_shared_rows(float *out, int8_t *oq, float *os, const float *q, const float *prefix_key,
+                             const float *prefix_value, int prefix_seq_len, int prefix, const float *key_cache,
+                             const float *value_cache, const int *starts, const int *counts, AttentionWork *work,
+                             int n_heads, int n_kv_heads, int head_dim, int seq_len, int batch, int rows, int gs);
+
+/* Low-rank adapters beside a shared projection: out[r] = base[r] + scale * B (A x[r]) for rows r of x [rows][n] (stride
+ * ldx), with the adapter index[r] (device memory; -1: none, out[r] = base[r]) of the device table `adapters` of `count`
+ * entries: a [rank][n] and b [d][rank] row-major, of the type `type`. base (stride ldb) may be out itself, as after the
+ * product of k_gemm_q8 or k_matmul_q8, or NULL for zeros; out must not overlap x. Ranks 0 .. max_rank <= 256; an index
+ * outside [-1, count), a rank outside [0, max_rank] or a missing matrix raises an error (kc_status) and the row gets
+ * its base. Sums are fp32 in a fixed order. 16-byte aligned matrices with n and rank multiples of 8 are read in 16-byte
+ * units, others one value at a time. */
+typedef enum { K_F32, K_BF16, K_F16 } KernelType;
+typedef struct {
+  const void *a, *b;
+  int rank;
+  float scale;
+} LoraAdapter;
+void k_lora_rows(float *out, size_t ldo, const float *base, size_t ldb, const float *x, size_t ldx, const int *index,
+                 const LoraAdapter *adapters, int count, int type, int max_rank, int n, int d, int rows);
+
+/* Verification of drafted tokens (speculative sampling): request b drafted the tokens drafted[b][0 .. counts[b] - 1]
+ * of drafted [batch][rows]; row j of target [batch][rows + 1] (logits, row stride ldt, as engine_forward_batch makes
+ * them) is the target model's after j drafts, row j of draft [batch][rows] (stride ldd) the logits that draft j was
+ * drawn from, or draft is NULL when the drafts came from no distribution (a lookup in the prompt). p_j and q_j are
+ * their softmax at temperature[b] (q_j one at the drafted token without logits). Draft j is accepted when all before
+ * it are and u_j q_j(x_j) < p_j(x_j), with the given random numbers u = uniforms[b] of uniforms [batch][rows + 1], in
+ * [0, 1). Behind the accepted drafts one token is drawn with u_rows: from (p - q)+ at the refused draft, else from p
+ * of row counts[b]; it is the first token whose running sum in vocabulary order exceeds u_rows times the total (where
+ * p - q leaves nothing, p's first maximum). At temperature 0 a draft is accepted when it is the row's first maximum
+ * (sample_argmax, src/sampler.c:9-23), and the last token is one.
+ * accepted[b] is the number of accepted drafts, tokens [batch][rows + 1] the accepted drafts, the drawn token, then -1.
+ * counts (NULL: rows for all) -1: a slot not in use, its outputs stay as they were. A needed row with a NaN, +infinity
+ * or no value above -infinity, a drafted token outside the vocabulary where it is looked at, a count or temperature
+ * outside its range: accepted[b] and tokens[b] are -1, and kc_status reports it. Rows behind the first refused draft
+ * are not looked at. Sums are 64-bit. rows <= 64. `work`: k_verify_bytes bytes of device memory, 16-byte aligned, one
+ * call in flight per work. */
+size_t k_verify_bytes(int vocab, int batch, int rows);
+void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt, const float *draft, size_t ldd,
+                    const int *drafted, const int *counts, const float *uniforms, const float *temperature, int vocab,
+                    int batch, int rows, void *work);
+
 /* ---- test hooks (include/testing.h:67-69) ------------------------------------------------------------------------ */
 /* One named backend; returns 0 when it is not compiled in (the CPU rungs). */
 int k_gemm_q8_backend_test(Q8GemmBackend backend, const int8_t *xq, const float *xs, int m, int k, int gs,

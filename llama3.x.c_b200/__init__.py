@@ -22,6 +22,7 @@ GEMM_STORE, GEMM_ADD, GEMM_SWIGLU, GEMM_PARTIAL = 0, 1, 2, 3  # include/gemm.h:1
 Q8_GEMM_PORTABLE, Q8_GEMM_AVX512, Q8_GEMM_AMX = 0, 1, 2
 Q8_GEMM_GPU_DP4A, Q8_GEMM_GPU_TCGEN05 = 16, 17
 KC_FAIL_EXIT, KC_FAIL_RETURN = 0, 1
+K_F32, K_BF16, K_F16 = 0, 1, 2                              # include/kernels_cuda.h: KernelType
 
 _i8p = ctypes.c_void_p
 _f32p = ctypes.c_void_p
@@ -58,6 +59,11 @@ class AttentionWork(ctypes.Structure):
     _fields_ = [("partial", ctypes.c_void_p), ("max_chunks", ctypes.c_int), ("n_heads", ctypes.c_int),
                 ("head_dim", ctypes.c_int), ("workers", ctypes.c_int), ("external", ctypes.c_int),
                 ("capacity", ctypes.c_size_t)]
+
+
+class LoraAdapter(ctypes.Structure):
+    """include/kernels_cuda.h: one entry of k_lora_rows' device table."""
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("rank", ctypes.c_int), ("scale", ctypes.c_float)]
 
 
 # Every symbol include/kernels_cuda.h declares, with its ctypes signature (restype, argtypes).
@@ -136,6 +142,17 @@ _SIGNATURES = {
     "k_random_q8": (None, [_i8p, _f32p, _c.c_int, _c.c_int, _c.c_size_t, _c.c_size_t, _c.c_size_t, _c.c_ulonglong,
                            _c.c_ulonglong, _c.c_float, _c.c_int]),
     "k_fill": (None, [_f32p, _c.c_size_t, _c.c_float]),
+    "k_attention_shared_bytes": (_c.c_size_t, [_c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int]),
+    "k_attention_shared_init": (None, [_c.POINTER(AttentionWork), _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int,
+                                       _c.c_void_p]),
+    "k_attention_shared_rows": (None, [_f32p, _i8p, _f32p, _f32p, _f32p, _f32p, _c.c_int, _c.c_int, _f32p, _f32p,
+                                       _c.c_void_p, _c.c_void_p, _c.POINTER(AttentionWork), _c.c_int, _c.c_int,
+                                       _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int]),
+    "k_lora_rows": (None, [_f32p, _c.c_size_t, _f32p, _c.c_size_t, _f32p, _c.c_size_t, _c.c_void_p, _c.c_void_p,
+                           _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int]),
+    "k_verify_bytes": (_c.c_size_t, [_c.c_int, _c.c_int, _c.c_int]),
+    "k_verify_draft": (None, [_c.c_void_p, _c.c_void_p, _f32p, _c.c_size_t, _f32p, _c.c_size_t, _c.c_void_p,
+                              _c.c_void_p, _f32p, _f32p, _c.c_int, _c.c_int, _c.c_int, _c.c_void_p]),
 }
 
 
@@ -467,3 +484,70 @@ def k_greedy_advance(out, step, token, position, key):
 
 def k_random_q8(q, s, rows, cols, row0, col0, full_cols, seed, tensor, std, gs):
     _call("k_random_q8", _ptr(q), _ptr(s), rows, cols, row0, col0, full_cols, seed, tensor, std, gs)
+
+
+# ---- a batch of requests over one prompt ------------------------------------------------------------------------------
+
+def _want(dtype, *tensors):
+    """The tensors (None allowed) must be contiguous ones of `dtype` on the current device: their addresses are all
+    that the library sees."""
+    for t in tensors:
+        if t is not None and not (t.dtype is dtype and t.is_cuda and t.is_contiguous()):
+            raise KernelError(f"needs a contiguous {dtype} CUDA tensor, got {t.dtype} on {t.device} with strides "
+                              f"{tuple(t.stride())}")
+
+
+def shared_attention_work(n_heads, n_kv_heads, head_dim, batch, rows):
+    """k_attention_shared_init with library-allocated device memory; release with k_attention_free."""
+    w = AttentionWork()
+    _call("k_attention_shared_init", ctypes.byref(w), n_heads, n_kv_heads, head_dim, batch, rows, None)
+    return w
+
+
+def k_attention_shared_rows(out, oq, os_, q, prefix_key, prefix_value, prefix_seq_len, prefix, kc, vc, starts, counts,
+                            work, n_heads, n_kv_heads, head_dim, seq_len, batch, rows, gs):
+    """Attention of a batch whose requests share a prefix (include/kernels_cuda.h); oq, os_ and counts may be None."""
+    import torch
+    _want(torch.float32, out, q, prefix_key, prefix_value, kc, vc, os_)
+    _want(torch.int32, starts, counts)
+    _want(torch.int8, oq)
+    _call("k_attention_shared_rows", _ptr(out), _ptr(oq), _ptr(os_), _ptr(q), _ptr(prefix_key), _ptr(prefix_value),
+          prefix_seq_len, prefix, _ptr(kc), _ptr(vc), _ptr(starts), _ptr(counts), ctypes.byref(work), n_heads,
+          n_kv_heads, head_dim, seq_len, batch, rows, gs)
+
+
+def lora_table(a, b, scale):
+    """k_lora_rows' device table of the adapters (a[i] [rank_i][n], b[i] [d][rank_i], scale[i]); it keeps the matrices
+    alive. One dtype throughout: float32, bfloat16 or float16."""
+    import torch
+    if not (len(a) == len(b) == len(scale)) or not a:
+        raise KernelError("lora_table needs as many a and b matrices as scales, at least one")
+    for x, y in zip(a, b):
+        _want(a[0].dtype, x, y)
+        if x.shape[0] != y.shape[1] or x.shape[1] != a[0].shape[1] or y.shape[0] != b[0].shape[0]:
+            raise KernelError(f"adapter matrices {tuple(x.shape)} and {tuple(y.shape)} do not fit together")
+    entries = (LoraAdapter * len(a))(*[LoraAdapter(x.data_ptr(), y.data_ptr(), x.shape[0], float(s))
+                                       for x, y, s in zip(a, b, scale)])
+    table = torch.frombuffer(bytearray(entries), dtype=torch.uint8).to(a[0].device)
+    table._tensors = (a, b)  # the table holds raw pointers
+    return table
+
+
+def k_lora_rows(out, ldo, base, ldb, x, ldx, index, table, count, type, max_rank, n, d, rows):
+    """out = base + scale B (A x) with the adapter each row names (include/kernels_cuda.h); table from lora_table."""
+    _call("k_lora_rows", _ptr(out), ldo, _ptr(base), ldb, _ptr(x), ldx, _ptr(index), _ptr(table), count, type, max_rank,
+          n, d, rows)
+
+
+def k_verify_bytes(vocab, batch, rows):
+    return load().k_verify_bytes(vocab, batch, rows)
+
+
+def k_verify_draft(accepted, tokens, target, ldt, draft, ldd, drafted, counts, uniforms, temperature, vocab, batch, rows,
+                   work):
+    """Verification of drafted tokens (include/kernels_cuda.h); draft and counts may be None."""
+    import torch
+    _want(torch.int32, accepted, tokens, drafted, counts)
+    _want(torch.float32, uniforms, temperature)
+    _call("k_verify_draft", _ptr(accepted), _ptr(tokens), _ptr(target), ldt, _ptr(draft), ldd, _ptr(drafted),
+          _ptr(counts), _ptr(uniforms), _ptr(temperature), vocab, batch, rows, _ptr(work))

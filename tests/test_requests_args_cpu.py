@@ -1,0 +1,127 @@
+"""CPU tests of the argument checks of the operators that serve a batch of requests over one prompt
+(k_attention_shared_rows, k_lora_rows, k_verify_draft): refused on the host, nothing queued. The buffers are made-up
+aligned addresses that are never read."""
+import ctypes
+
+import pytest
+
+from conftest import load_package
+
+A = 0x10000
+
+
+@pytest.fixture(scope="module")
+def lib():
+    kc = load_package()
+    L = kc.load()
+    L.kc_set_fail_mode(kc.KC_FAIL_RETURN)
+    return kc, L
+
+
+def rejected(L):
+    msg = L.kc_last_error()
+    L.kc_clear_error()
+    assert msg, "the call was accepted"
+    return msg.decode()
+
+
+def shared(kc, L, work=None, out=A, oq=None, os_=None, q=A, pk=A, pv=A, prefix_seq=64, prefix=32, k=A, v=A, starts=A,
+           counts=A, heads=8, kv=2, hd=64, seq=32, batch=2, rows=3, gs=0):
+    L.k_attention_shared_rows(out, oq, os_, q, pk, pv, prefix_seq, prefix, k, v, starts, counts,
+                              ctypes.byref(work) if work is not None else None, heads, kv, hd, seq, batch, rows, gs)
+    return rejected(L)
+
+
+def made_up_work(kc, L, heads=8, kv=2, hd=64, batch=2, rows=3):
+    w = kc.AttentionWork()
+    L.k_attention_shared_init(ctypes.byref(w), heads, kv, hd, batch, rows, A)
+    assert not L.kc_last_error()
+    assert w.external == 1 and w.capacity * 4 == L.k_attention_shared_bytes(heads, kv, hd, batch, rows)
+    return w
+
+
+@pytest.mark.parametrize("bad", [dict(heads=9), dict(heads=0), dict(kv=0), dict(hd=0), dict(hd=257), dict(batch=-1),
+                                 dict(rows=-1), dict(seq=0), dict(seq=2), dict(prefix=-1), dict(prefix=65)])
+def test_shared_attention_shapes(lib, bad):
+    kc, L = lib
+    assert "k_attention_shared_rows: invalid shape" in shared(kc, L, made_up_work(kc, L), **bad)
+
+
+@pytest.mark.parametrize("missing", ["out", "q", "pk", "pv", "k", "v", "starts"])
+def test_shared_attention_missing_pointers(lib, missing):
+    kc, L = lib
+    assert "missing output, queries, caches or starts" in shared(kc, L, made_up_work(kc, L), **{missing: None})
+
+
+def test_shared_attention_quantizer_and_work(lib):
+    kc, L = lib
+    w = made_up_work(kc, L)
+    assert "missing output" in shared(kc, L, w, oq=A, gs=64)
+    assert "group size 48 does not divide the head's 64 outputs" in shared(kc, L, w, oq=A, os_=A, gs=48)
+    assert "group size 0 does not divide" in shared(kc, L, w, oq=A, os_=A)
+    assert "work is missing or too small" in shared(kc, L)
+    assert "work is missing or too small" in shared(kc, L, w, hd=32)
+    assert "work is missing or too small" in shared(kc, L, w, rows=8)
+    assert "work is missing or too small" in shared(kc, L, kc.AttentionWork())
+
+
+def test_shared_attention_work_arguments(lib):
+    kc, L = lib
+    w = kc.AttentionWork()
+    L.k_attention_shared_init(ctypes.byref(w), 8, 3, 64, 2, 3, A)
+    assert rejected(L) == "k_attention_shared_init: invalid shape"
+    L.k_attention_shared_init(ctypes.byref(w), 8, 2, 64, 2, 3, A + 4)
+    assert "16-byte aligned" in rejected(L)
+    assert L.k_attention_shared_bytes(8, 2, 64, 0, 3) == 0
+
+
+def lora(L, out=A, ldo=32, base=A, ldb=32, x=A, ldx=64, index=A, table=A, count=2, kind=1, max_rank=8, n=64, d=32,
+         rows=4):
+    L.k_lora_rows(out, ldo, base, ldb, x, ldx, index, table, count, kind, max_rank, n, d, rows)
+    return rejected(L)
+
+
+@pytest.mark.parametrize("bad", [dict(rows=-1), dict(n=0), dict(d=0), dict(count=-1), dict(max_rank=0),
+                                 dict(max_rank=257), dict(ldx=63), dict(ldo=31), dict(ldb=31)])
+def test_lora_shapes(lib, bad):
+    assert "k_lora_rows: invalid shape" in lora(lib[1], **bad)
+
+
+def test_lora_type_and_pointers(lib):
+    kc, L = lib
+    assert lora(L, kind=3) == "k_lora_rows: invalid weight type 3"
+    for missing in ("out", "x", "index", "table"):
+        assert "missing output, activations, row indices or adapters" in lora(L, **{missing: None})
+
+
+def verify(L, accepted=A, tokens=A, target=A, ldt=100, draft=A, ldd=100, drafted=A, counts=A, uniforms=A,
+           temperature=A, vocab=100, batch=2, rows=3, work=A):
+    L.k_verify_draft(accepted, tokens, target, ldt, draft, ldd, drafted, counts, uniforms, temperature, vocab, batch, rows,
+                     work)
+    return rejected(L)
+
+
+@pytest.mark.parametrize("bad", [dict(vocab=0), dict(batch=-1), dict(rows=-1), dict(rows=65), dict(ldt=99),
+                                 dict(ldd=99)])
+def test_verify_shapes(lib, bad):
+    assert "k_verify_draft: invalid shape" in verify(lib[1], **bad)
+
+
+def test_verify_pointers_and_work(lib):
+    kc, L = lib
+    for missing in ("accepted", "tokens", "target", "drafted", "uniforms", "temperature", "work"):
+        assert "missing outputs, logits, drafts, numbers or 16-byte aligned work" in verify(L, **{missing: None})
+    assert "aligned work" in verify(L, work=A + 4)
+    assert "too large" in verify(L, vocab=1 << 30, ldt=1 << 30, ldd=1 << 30, batch=1 << 20)
+    assert L.k_verify_bytes(0, 1, 1) == 0 and L.k_verify_bytes(100, 1, 65) == 0
+
+
+def test_python_mirror_refuses_other_layouts():
+    """The mirror passes addresses only: other types, devices or strides raise before any call."""
+    import torch
+    kc = load_package()
+    a = torch.zeros(4, 4)
+    with pytest.raises(kc.KernelError, match="contiguous torch.float32 CUDA tensor"):
+        kc.k_attention_shared_rows(a, None, None, a, a, a, 4, 4, a, a, a, a, kc.AttentionWork(), 1, 1, 4, 4, 1, 4, 0)
+    with pytest.raises(kc.KernelError, match="as many a and b matrices"):
+        kc.lora_table([a], [], [1.0])

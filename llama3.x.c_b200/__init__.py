@@ -498,9 +498,12 @@ def _want(dtype, *tensors):
 
 
 def shared_attention_work(n_heads, n_kv_heads, head_dim, batch, rows):
-    """k_attention_shared_init with library-allocated device memory; release with k_attention_free."""
+    """k_attention_shared_init on torch memory, which lives as long as the work does."""
+    import torch
     w = AttentionWork()
-    _call("k_attention_shared_init", ctypes.byref(w), n_heads, n_kv_heads, head_dim, batch, rows, None)
+    w._memory = torch.empty(max(16, load().k_attention_shared_bytes(n_heads, n_kv_heads, head_dim, batch, rows)),
+                            dtype=torch.uint8, device="cuda")
+    _call("k_attention_shared_init", ctypes.byref(w), n_heads, n_kv_heads, head_dim, batch, rows, _ptr(w._memory))
     return w
 
 

@@ -301,8 +301,9 @@ void k_fill(float *x, size_t n, float value);
  * finite; what it does not see is never read into it. oq / os (may be NULL): out quantized for Wo as k_quantize does,
  * gs dividing head_dim. The prefix is read once for the whole batch. head_dim <= 256.
  * `work` (k_attention_shared_init, released with k_attention_free): partial results for this n_heads and head_dim and
- * at most what its batch and rows need; `memory` as for k_attention_init_rows (k_attention_shared_bytes bytes, or
- * NULL). One call in flight per work. */
+ * up to batch * rows rows (its `workers`; its max_chunks is 0, so that neither kind of work passes for the other), which
+ * may split the positions differently, and so round differently, for works made for different sizes; `memory` as for
+ * k_attention_init_rows (k_attention_shared_bytes bytes, 16-byte aligned, or NULL). One call in flight per work. */
 size_t k_attention_shared_bytes(int n_heads, int n_kv_heads, int head_dim, int batch, int rows);
 void k_attention_shared_init(AttentionWork *work, int n_heads, int n_kv_heads, int head_dim, int batch, int rows,
                              void *memory);

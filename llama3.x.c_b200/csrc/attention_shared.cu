@@ -205,65 +205,79 @@ __global__ void __launch_bounds__(kGenericThreads) shared_generic_kernel(const S
 //
 // fp32 products on half-precision tensor cores: x = 2^-k (hi + lo) with hi and lo fp16, 22 bits of x, and
 // x y = 2^-(k + k') (hi hi' + hi lo' + lo hi') up to 2^-22 of the product (what is dropped, lo lo', is below the
-// rounding of lo). The power 2^k puts the largest magnitude of a query vector, of a tile of keys or of a tile of values
-// just below 2^15, so no finite input overflows and a value 2^-17 of the largest still keeps its 22 bits. k of the
-// keys goes into the scores' scale; k of the values into the probabilities (exact powers of two both).
+// rounding of lo). The power 2^k puts the largest magnitude of a query vector, of eight keys or of eight values just
+// below 2^15, so no finite input overflows and a value 2^-17 of the largest still keeps its 22 bits. k of the keys goes
+// into the scores' scale, k of the values into the probabilities' exponent (exact powers of two both).
 //
-// Warps: 0-3 the softmax, a thread per query vector (TMEM lane); 4 issues the MMAs; 5-12 read keys and values from
-// global memory, split them and store them as the MMA's operands (values transposed, so both are K-major), two stages.
-// The running maximum is a reference m that moves only when a score exceeds it by 8 (a factor of 256): O in TMEM is
-// seldom rescaled.
+// Warps: 0-3 the softmax of the even tiles and 4-7 that of the odd ones, a thread per query vector (TMEM lane), each
+// group with a reference, a sum and an O of its own (joined at the end), so that a group has two tiles' time; 8 issues
+// the MMAs; 9-16 split eight keys and eight values of a tile each and store them as the MMAs' operands (keys K-major,
+// values MN-major, so neither is transposed), two stages. The queries are the A operand in TMEM (from shared memory an
+// MMA of 64 columns would wait for it), and the probabilities take the place of the scores they come from.
+// The running maximum is a whole-number reference m that moves only when a score exceeds it by 8 (a factor of 256): O
+// is seldom rescaled.
 constexpr int kTcVecs = 128, kTcPos = 64;
-constexpr int kSoftWarps = 4, kConvWarps = 8;
+constexpr int kSoftWarps = 8, kConvWarps = 8;
 constexpr int kTcThreads = 32 * (kSoftWarps + 1 + kConvWarps);
-constexpr int kConvThreads = 32 * kConvWarps;
-constexpr uint32_t kTmemS = 0, kTmemP = 128, kTmemO = 256, kTmemCols = 512;
+constexpr uint32_t kTmemQ = 0, kTmemS = 128, kTmemO = 256, kTmemCols = 512;  // S and O: two buffers each
 constexpr int kPShift = 7;  // probabilities are up to 2^8 (the lazy reference) and carry this power of two more
 
 template <int HD>
 struct TcSmem {
-  static constexpr int q_bytes = kTcVecs * HD * 2;  // hi or lo
   static constexpr int kv_bytes = kTcPos * HD * 2;  // hi or lo of K or V
   static constexpr int stage = 4 * kv_bytes;
-  static constexpr int stages_at = 2 * q_bytes;
-  static constexpr int tail_at = stages_at + 2 * stage;
-  static constexpr int total = tail_at + 2048 + 1024;  // the tail, and room to align the start to 1 KiB
+  static constexpr int tail_at = 2 * stage;
+  static constexpr int total = tail_at + 4096 + 1024;  // the tail, and room to align the start to 1 KiB
 };
 
 struct TcTail {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], sempty[2], pfull[2], pvdone[2];
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2];
   uint32_t tmem;
   int abort_flag;
-  int kshift[4], vshift[4];      // powers of two of the keys' and values' tiles
-  unsigned wmax[4][kConvWarps];  // magnitudes while they are agreed on
-  int qshift[kTcVecs];
+  float kscale[4][kConvWarps];  // 2^-k of eight keys, a ring of tiles
+  int vshift[4][kConvWarps];    // k of eight values
+  unsigned qmax[2][kTcVecs];
+  float m[kTcVecs], l[kTcVecs];  // of the odd tiles, and O's power
+  int vref[kTcVecs];
 };
-static_assert(sizeof(TcTail) <= 2048, "the tail's room");
+static_assert(sizeof(TcTail) <= 4096, "the tail's room");
 
 // A whole warp's bounded wait, with one answer for all lanes: false once any wait of the CTA has given up.
 __device__ __forceinline__ bool tc_wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
-  bool ok = *abort_flag == 0;
-  if (ok && !mbar_wait_sleep_bounded(bar, parity)) {
-    *abort_flag = 1;
-    ok = false;
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    ok = *abort_flag == 0;
+    if (ok && !mbar_wait_sleep_bounded(bar, parity)) {
+      *abort_flag = 1;
+      ok = false;
+    }
   }
   return __all_sync(0xffffffffu, ok);
 }
 
-// kind::f16 instruction descriptor: fp16 A and B, both K-major, fp32 accumulators, M x N.
-__host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
 }
 
-__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
+// kind::f16 instruction descriptor: fp16 A and B, A K-major, B K-major or MN-major, fp32 accumulators, M x N.
+__host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n, bool b_mn) {
+  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// A from TMEM: lane = row, a 32-bit column holds two neighbouring elements.
+
+// MN-major operand in the 128-byte swizzle: rows of 64 values along N, 8 rows (K) to an atom of 1 KiB; atoms 1 KiB apart
+// along K, `n_bytes` apart along N.
+__device__ __forceinline__ uint64_t umma_desc_sw128_mn(const void *smem_tile, uint32_t n_bytes) {
+  uint64_t d = (smem_u32(smem_tile) >> 4) & 0x3FFFull;
+  d |= (uint64_t)(n_bytes >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// A from TMEM (lane = row, a 32-bit column holds two neighbouring elements), B from shared memory.
 __device__ __forceinline__ void umma_f16_ta(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -272,31 +286,33 @@ __device__ __forceinline__ void umma_f16_ta(uint32_t d, uint32_t a, uint64_t bde
       "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
-// Writes 32 lanes (this warp's quadrant) x 32 consecutive columns.
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+// Writes 32 lanes (this warp's quadrant) x 16 consecutive columns.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 
-// The power k for a largest magnitude (its bits): magnitudes times 2^k below 2^15. At most 126, so that 2^k is a
-// number; tiny and zero maxima take that.
+// The power k for a largest magnitude (its bits): magnitudes times 2^k below 2^15. At most 100 (zeros, and maxima below
+// 2^-86, which keep fewer bits), so that a scale times 2^-k is a normal number.
 __device__ __forceinline__ int shift_for(unsigned max_bits) {
   const int e = (int)(max_bits >> 23) - 127;
-  return min(14 - e, 126);
+  return min(14 - e, 100);
 }
-__device__ __forceinline__ float pow2(int k) { return ldexpf(1.0f, k); }
+// 2^k for k <= 127, 0 below the normal range.
+__device__ __forceinline__ float pow2(int k) { return k < -126 ? 0.0f : __int_as_float((k + 127) << 23); }
 
-// Two scaled values as packed fp16 high parts and the packed rest.
-__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+// Two values (packed) as packed fp16 high parts and the packed rest.
+__device__ __forceinline__ void split2(uint64_t xy, uint32_t &hi, uint32_t &lo) {
+  float x, y;
+  f2_unpack(xy, x, y);
   const __half2 h = __floats2half2_rn(x, y);
   const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  f2_unpack(f2_fma(f2_pack(f.x, f.y), f2_pack(-1.0f, -1.0f), xy), x, y);  // exact
+  const __half2 l = __floats2half2_rn(x, y);
   hi = *reinterpret_cast<const uint32_t *>(&h);
   lo = *reinterpret_cast<const uint32_t *>(&l);
 }
@@ -307,19 +323,50 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// The largest of the converters' magnitudes (bits), agreed over their warps. `slot` alternates, so that a value is not
-// overwritten while another warp still reads it.
-__device__ __forceinline__ unsigned agree_max(TcTail *t, int slot, unsigned mine, int cw, int lane) {
-  mine = __reduce_max_sync(0xffffffffu, mine);
-  if (lane == 0)
-    t->wmax[slot][cw] = mine;
-  asm volatile("bar.sync 1, %0;" ::"n"(kConvThreads) : "memory");
-  unsigned m = 0;
+__device__ __forceinline__ unsigned abs_max(unsigned m, float x) { return max(m, __float_as_uint(fabsf(x))); }
+
+// Eight rows of a tile in a warp's registers: HD / 4 lanes to a row.
+template <int HD>
+struct Rows8 {
+  static constexpr int kSteps = HD / 16;    // float4 a lane: 8 or 4
+  static constexpr int kAt = 128 / HD;      // rows a step
+  float4 x[kSteps];
+
+  // Rows [row0, row0 + 8) of cache rows of hd floats; rows from `end` on and columns from hd on are zeros.
+  __device__ __forceinline__ void load(const float *cache, int row0, int end, int hd, int lane) {
+    const int col = lane * 4 % HD, r = lane * 4 / HD;
+    const float *src = cache + (size_t)(row0 + r) * hd + col;
 #pragma unroll
-  for (int w = 0; w < kConvWarps; w++)
-    m = max(m, t->wmax[slot][w]);
-  return m;
-}
+    for (int i = 0; i < kSteps; i++) {
+      x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (row0 + r + i * kAt < end && col < hd)
+        x[i] = __ldcg(reinterpret_cast<const float4 *>(src + (size_t)i * kAt * hd));
+    }
+  }
+  // Splits the rows and stores them as rows row .. row + 7 of the operand pair (64 rows of 128 swizzled bytes to 64
+  // columns); returns their power of two.
+  __device__ __forceinline__ int store(uint8_t *hi_at, uint8_t *lo_at, int row, int lane) const {
+    unsigned mx = 0;
+#pragma unroll
+    for (int i = 0; i < kSteps; i++)
+      mx = abs_max(abs_max(abs_max(abs_max(mx, x[i].x), x[i].y), x[i].z), x[i].w);
+    const int k = shift_for(__reduce_max_sync(0xffffffffu, mx));
+    const uint64_t f = f2_pack(pow2(k), pow2(k));
+    const int col = lane * 4 % HD, r = lane * 4 / HD;
+    const uint32_t base = (col >> 6) * (kTcPos * 128) + row * 128 + (col & 7) * 2;
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+      const int rr = r + i * kAt;
+      const uint32_t at = base + rr * 128 + ((((col & 63) >> 3) ^ (rr & 7)) << 4);
+      uint2 hi, lo;
+      split2(f2_mul(f2_pack(x[i].x, x[i].y), f), hi.x, lo.x);
+      split2(f2_mul(f2_pack(x[i].z, x[i].w), f), hi.y, lo.y);
+      *reinterpret_cast<uint2 *>(hi_at + at) = hi;
+      *reinterpret_cast<uint2 *>(lo_at + at) = lo;
+    }
+    return k;
+  }
+};
 
 template <int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedArgs a) {
@@ -347,8 +394,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       mbar_init(&t->kempty[i], 1);
       mbar_init(&t->vempty[i], 1);
       mbar_init(&t->sfull[i], 1);
-      mbar_init(&t->sempty[i], kSoftWarps);
-      mbar_init(&t->pfull[i], kSoftWarps);
+      mbar_init(&t->pfull[i], kSoftWarps / 2);
       mbar_init(&t->pvdone[i], 1);
     }
     t->abort_flag = 0;
@@ -356,153 +402,118 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
   }
   if (warp == kSoftWarps)
     tmem_alloc(&t->tmem, kTmemCols);
-
   const int hd = a.hd;
-  // The queries: a warp per vector, split with the vector's own power of two. Vectors not in use are zeros.
-  for (int i = warp; i < kTcVecs; i += kTcThreads / 32) {
-    constexpr int E = HD / 32;  // 4 or 2 elements a lane
-    float x[E];
-    bool use = i < it.vecs;
-    if (use) {
-      const int flat = it.first + i, row = flat / a.group, b = row / a.rows;
-      const int count = rows_of(a, b);
-      use = row - b * a.rows < count && request_ok(a, b, count);
-    }
-    const float *src = a.q + (size_t)(use ? vector_at(a, it.kv, it.first + i) : 0) * hd;
-    unsigned mx = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      x[e] = use && lane * E + e < hd ? src[lane * E + e] : 0.0f;
-      mx = max(mx, __float_as_uint(fabsf(x[e])));
-    }
-    const int k = shift_for(__reduce_max_sync(0xffffffffu, mx));
-    const float f = pow2(k);
-    if (lane == 0)
-      t->qshift[i] = k;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      uint32_t hi, lo;
-      split2(x[e] * f, x[e + 1] * f, hi, lo);
-      const int c = lane * E + e;
-      const int at = (c >> 6) * (kTcVecs * 128) + i * 128 + ((((c & 63) >> 3) ^ (i & 7)) << 4) + (c & 7) * 2;
-      *reinterpret_cast<uint32_t *>(smem + at) = hi;
-      *reinterpret_cast<uint32_t *>(smem + L::q_bytes + at) = lo;
-    }
-  }
-  fence_proxy_async_smem();
+  Rows8<HD> kx, vx;
+  const int cw = warp - kSoftWarps - 1;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = t->tmem;
 
+  // The queries: group g's threads lay out half g of their vectors' elements. Vectors not in use are zeros.
+  const int g = warp >> 2, vec_i = 32 * (warp & 3) + lane;
+  const uint32_t quadrant = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+  const bool have = vec_i < it.vecs, busy = 32 * (warp & 3) < it.vecs;
+  int qshift = 0;
+  if (warp < kSoftWarps) {
+    constexpr int H = HD / 2;
+    float x[H];
+    bool use = have;
+    if (use) {
+      const int row = (it.first + vec_i) / a.group, b = row / a.rows, count = rows_of(a, b);
+      use = row - b * a.rows < count && request_ok(a, b, count);
+    }
+    unsigned mx = 0;
+    if (busy) {
+      const float *src = a.q + (size_t)(use ? vector_at(a, it.kv, it.first + vec_i) : 0) * hd + g * H;
+      if (((uintptr_t)a.q & 15) == 0) {
+#pragma unroll
+        for (int e = 0; e < H; e += 4) {
+          float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (use && g * H + e < hd)
+            y = *reinterpret_cast<const float4 *>(src + e);
+          x[e] = y.x, x[e + 1] = y.y, x[e + 2] = y.z, x[e + 3] = y.w;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < H; e++)
+          x[e] = use && g * H + e < hd ? src[e] : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < H; e++)
+        mx = abs_max(mx, x[e]);
+    }
+    t->qmax[g][vec_i] = mx;
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
+    qshift = shift_for(max(t->qmax[0][vec_i], t->qmax[1][vec_i]));
+    if (busy) {
+      const uint64_t f = f2_pack(pow2(qshift), pow2(qshift));
+#pragma unroll
+      for (int c = 0; c < H; c += 32) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+          split2(f2_mul(f2_pack(x[c + 2 * e], x[c + 2 * e + 1]), f), hi[e], lo[e]);
+        tmem_st16(quadrant + kTmemQ + (g * H + c) / 2, hi);
+        tmem_st16(quadrant + kTmemQ + 64 + (g * H + c) / 2, lo);
+      }
+      tmem_wait_st();
+    }
+  } else if (cw >= 0) {  // the first tile's keys and values come meanwhile
+    kx.load(it.k, it.p0 + 8 * cw, it.p1, hd, lane);
+    vx.load(it.v, it.p0 + 8 * cw, it.p1, hd, lane);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
   if (warp > kSoftWarps) {
     // ---- converters ----
-    const int ct = threadIdx.x - 32 * (kSoftWarps + 1), cw = warp - kSoftWarps - 1;
-    constexpr int kChunks = kTcPos * HD / 8 / kConvThreads;  // chunks of 8 values per thread: 4 or 2
-    float kx[kChunks][8], vx[kChunks][8];
-    auto load_k = [&](int tile) {
-      const int p0 = it.p0 + tile * kTcPos;
-#pragma unroll
-      for (int i = 0; i < kChunks; i++) {
-        const int c = i * kConvThreads + ct, r = c / (HD / 8), e = c % (HD / 8) * 8;
-        const float *src = it.k + (size_t)(p0 + r) * hd + e;
-        const bool in = p0 + r < it.p1;
-        float4 x = make_float4(0, 0, 0, 0), y = x;
-        if (in && e < hd)
-          x = *reinterpret_cast<const float4 *>(src);
-        if (in && e + 4 < hd)
-          y = *reinterpret_cast<const float4 *>(src + 4);
-        kx[i][0] = x.x, kx[i][1] = x.y, kx[i][2] = x.z, kx[i][3] = x.w;
-        kx[i][4] = y.x, kx[i][5] = y.y, kx[i][6] = y.z, kx[i][7] = y.w;
-      }
-    };
-    auto load_v = [&](int tile) {
-      const int p0 = it.p0 + tile * kTcPos;
-#pragma unroll
-      for (int i = 0; i < kChunks; i++) {
-        const int c = i * kConvThreads + ct, d = c % HD, r = c / HD * 8;
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          vx[i][j] = p0 + r + j < it.p1 && d < hd ? it.v[(size_t)(p0 + r + j) * hd + d] : 0.0f;
-      }
-    };
-    auto largest = [&](const float (&x)[kChunks][8]) {
-      unsigned m = 0;
-#pragma unroll
-      for (int i = 0; i < kChunks; i++)
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          m = max(m, __float_as_uint(fabsf(x[i][j])));
-      return m;
-    };
-    auto store = [&](uint8_t *hi_at, uint8_t *lo_at, const float (&x)[8], float f) {
-      uint4 hi, lo;
-      split2(x[0] * f, x[1] * f, hi.x, lo.x);
-      split2(x[2] * f, x[3] * f, hi.y, lo.y);
-      split2(x[4] * f, x[5] * f, hi.z, lo.z);
-      split2(x[6] * f, x[7] * f, hi.w, lo.w);
-      *reinterpret_cast<uint4 *>(hi_at) = hi;
-      *reinterpret_cast<uint4 *>(lo_at) = lo;
-    };
-    load_k(0);
-    load_v(0);
     for (int j = 0; j < tiles; j++) {
-      const int s = j & 1, use = j >> 1;
-      uint8_t *stage = smem + L::stages_at + s * L::stage;
-      const int ks = shift_for(agree_max(t, 2 * s, largest(kx), cw, lane));
-      const float kf = pow2(ks);
+      const int s = j & 1, use = j >> 1, row0 = it.p0 + (j + 1) * kTcPos + 8 * cw;
+      uint8_t *stage = smem + s * L::stage;
       tc_wait(&t->kempty[s], (use & 1) ^ 1, abort_flag);
-#pragma unroll
-      for (int i = 0; i < kChunks; i++) {
-        const int c = i * kConvThreads + ct, r = c / (HD / 8), e8 = c % (HD / 8);
-        uint8_t *at = stage + (e8 >> 3) * (kTcPos * 128) + r * 128 + (((e8 & 7) ^ (r & 7)) << 4);
-        store(at, at + L::kv_bytes, kx[i], kf);
-      }
-      if (ct == 0)
-        t->kshift[j & 3] = ks;
+      const int ks = kx.store(stage, stage + L::kv_bytes, 8 * cw, lane);
+      if (lane == 0)
+        t->kscale[j & 3][cw] = pow2(-ks);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&t->kfull[s]);
       if (j + 1 < tiles)
-        load_k(j + 1);
-      const int vs = shift_for(agree_max(t, 2 * s + 1, largest(vx), cw, lane));
-      const float vf = pow2(vs);
+        kx.load(it.k, row0, it.p1, hd, lane);
       tc_wait(&t->vempty[s], (use & 1) ^ 1, abort_flag);
-#pragma unroll
-      for (int i = 0; i < kChunks; i++) {
-        const int c = i * kConvThreads + ct, d = c % HD, r8 = c / HD;
-        uint8_t *at = stage + 2 * L::kv_bytes + d * 128 + ((r8 ^ (d & 7)) << 4);
-        store(at, at + L::kv_bytes, vx[i], vf);
-      }
-      if (ct == 0)
-        t->vshift[j & 3] = vs;
+      const int vs = vx.store(stage + 2 * L::kv_bytes, stage + 3 * L::kv_bytes, 8 * cw, lane);
+      if (lane == 0)
+        t->vshift[j & 3][cw] = vs;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&t->vfull[s]);
       if (j + 1 < tiles)
-        load_v(j + 1);
+        vx.load(it.v, row0, it.p1, hd, lane);
     }
   } else if (warp == kSoftWarps) {
-    // ---- MMA issue: the scores of tile j + 1 go out before the sums of tile j, so that they run under its softmax ----
-    const uint32_t idesc_s = umma_idesc_f16(kTcVecs, kTcPos), idesc_o = umma_idesc_f16(kTcVecs, HD);
+    // ---- MMA issue. The scores of tile j + 1 go out before the sums of tile j, so that they run under its softmax; the
+    // MMAs run in the order of issue, so the scores of tile j + 2 never overtake the sums that read their buffer. ----
+    const bool leader = elect_one();
+    const uint32_t idesc_s = umma_idesc_f16(kTcVecs, kTcPos, false), idesc_o = umma_idesc_f16(kTcVecs, HD, true);
+    const uint64_t kdesc = umma_desc_sw128(smem), vdesc = umma_desc_sw128_mn(smem + 2 * L::kv_bytes, kTcPos * 128);
     auto scores = [&](int j) {
       const int s = j & 1, use = j >> 1;
-      if (!tc_wait(&t->kfull[s], use & 1, abort_flag) || !tc_wait(&t->sempty[s], (use & 1) ^ 1, abort_flag))
+      if (!tc_wait(&t->kfull[s], use & 1, abort_flag))
         return;
       tc_fence_after();
-      if (lane == 0) {
-        const uint8_t *k = smem + L::stages_at + s * L::stage;
+      if (leader) {
+        const uint64_t kd = kdesc + (uint64_t)(s * (L::stage >> 4));
         const uint32_t d = tmem + kTmemS + 64 * s;
 #pragma unroll
-        for (int term = 0; term < 3; term++) {  // lo hi, hi lo, hi hi: the small terms first
-          const uint8_t *qa = smem + (term == 0 ? L::q_bytes : 0), *kb = k + (term == 1 ? L::kv_bytes : 0);
+        for (int term = 0; term < 3; term++)  // lo hi, hi lo, hi hi: the small terms first
 #pragma unroll
           for (int c = 0; c < HD / 16; c++)
-            umma_f16(d, umma_desc_sw128(qa + (c >> 2) * (kTcVecs * 128)) + 2 * (c & 3),
-                     umma_desc_sw128(kb + (c >> 2) * (kTcPos * 128)) + 2 * (c & 3), idesc_s, term || c);
-        }
+            umma_f16_ta(d, tmem + kTmemQ + (term == 0 ? 64 : 0) + 8 * c,
+                        kd + ((term == 1 ? L::kv_bytes : 0) + (c >> 2) * (kTcPos * 128) + 32 * (c & 3)) / 16, idesc_s,
+                        term || c);
         umma_commit(&t->sfull[s]);
         umma_commit(&t->kempty[s]);
       }
@@ -516,141 +527,160 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       if (!tc_wait(&t->vfull[s], use & 1, abort_flag) || !tc_wait(&t->pfull[s], use & 1, abort_flag))
         break;
       tc_fence_after();
-      if (lane == 0) {
-        const uint8_t *v = smem + L::stages_at + s * L::stage + 2 * L::kv_bytes;
-        const uint32_t p = tmem + kTmemP + 64 * s;
+      if (leader) {
+        const uint64_t vd = vdesc + (uint64_t)(s * (L::stage >> 4));
+        const uint32_t p = tmem + kTmemS + 64 * s, d = tmem + kTmemO + 128 * s;
 #pragma unroll
-        for (int term = 0; term < 3; term++) {
-          const uint32_t pa = p + (term == 0 ? 32 : 0);
-          const uint8_t *vb = v + (term == 1 ? L::kv_bytes : 0);
+        for (int term = 0; term < 3; term++)
 #pragma unroll
-          for (int c = 0; c < kTcPos / 16; c++)
-            umma_f16_ta(tmem + kTmemO, pa + 8 * c, umma_desc_sw128(vb) + 2 * c, idesc_o, j || term || c);
-        }
+          for (int c = 0; c < kTcPos / 16; c++)  // 32 positions: 16 columns of hi, 16 of lo
+            umma_f16_ta(d, p + 32 * (c >> 1) + 8 * (c & 1) + (term == 0 ? 16 : 0),
+                        vd + ((term == 1 ? L::kv_bytes : 0) + 2048 * c) / 16, idesc_o, j > 1 || term || c);
         umma_commit(&t->pvdone[s]);
         umma_commit(&t->vempty[s]);
       }
       __syncwarp();
     }
   } else {
-    // ---- softmax: a thread per query vector ----
-    const uint32_t quadrant = tmem + ((uint32_t)(32 * warp) << 16);
-    const int i = 32 * warp + lane;
-    const bool have = i < it.vecs, busy = 32 * warp < it.vecs;
-    const int limit = have ? limit_of(a, it, it.first + i) : it.p0;
+    // ---- softmax: a thread per query vector, group g the tiles of its parity ----
+    const uint32_t ts = quadrant + kTmemS + 64 * g, to = quadrant + kTmemO + 128 * g;
+    const int limit = have ? limit_of(a, it, it.first + vec_i) : it.p0;
     const int lowest = __reduce_min_sync(0xffffffffu, have ? limit : 0x7fffffff);
-    const int qs = t->qshift[i];
-    const float scale = rsqrtf((float)hd) * kLog2e;
+    const float scale = rsqrtf((float)hd) * kLog2e * pow2(-qshift);
     float m = -INFINITY, l = 0.0f;
     int vref = 0;  // O holds sums times 2^(kPShift + vref)
-    for (int j = 0; j < tiles; j++) {
-      const int s = j & 1, use = j >> 1;
-      if (!tc_wait(&t->sfull[s], use & 1, abort_flag))
+    for (int j = g; j < tiles; j += 2) {
+      const int use = j >> 1;
+      // The scores; with them the group's previous sums are done, so O can be rescaled. The values' powers.
+      if (!tc_wait(&t->sfull[g], use & 1, abort_flag) || !tc_wait(&t->vfull[g], use & 1, abort_flag))
         break;
       tc_fence_after();
-      uint32_t r0[32], r1[32];
-      if (busy) {
-        tmem_ld32(quadrant + kTmemS + 64 * s, r0);
-        tmem_ld32(quadrant + kTmemS + 64 * s + 32, r1);
-        tmem_wait_ld();
-      }
-      const int ks = t->kshift[j & 3];
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0)
-        mbar_arrive(&t->sempty[s]);
-      // The values' power of two for the probabilities.
-      if (!tc_wait(&t->vfull[s], use & 1, abort_flag))
-        break;
-      const int vs = t->vshift[j & 3];
       if (busy) {
         const int p0 = it.p0 + j * kTcPos;
-        if (p0 + kTcPos > lowest) {
-#pragma unroll
-          for (int c = 0; c < 32; c++) {
-            r0[c] = p0 + c < limit ? r0[c] : 0xff800000u;
-            r1[c] = p0 + 32 + c < limit ? r1[c] : 0xff800000u;
-          }
-        }
-        const float factor = ldexpf(scale, -(qs + ks));
+        const bool masked = p0 + kTcPos > lowest;
+        const float *kscale = t->kscale[j & 3];
+        const int *vshift = t->vshift[j & 3];
+        auto factor = [&](int c8) {  // never 0: a masked score's -infinity has to stay one
+          return fmaxf(scale * kscale[c8], FLT_MIN);
+        };
+        // Two passes over the scores in TMEM, 32 at a time: their maximum, then the probabilities.
         float top = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 32; c++)
-          top = fmaxf(top, fmaxf(__uint_as_float(r0[c]), __uint_as_float(r1[c])));
-        top *= factor;
-        // Move the reference when a score exceeds it by more than 8, and O's power when the values have grown.
-        const bool up = top > m + 8.0f || (m == -INFINITY && top > m);
-        const float m_new = up ? top : m;
-        const int vref_new = j == 0 || vs < vref ? vs - 1 : vref;
-        const float keep = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - m_new);
-        if (j > 0 && (vref_new != vref || __any_sync(0xffffffffu, up))) {
-          if (!tc_wait(&t->pvdone[s ^ 1], ((j - 1) >> 1) & 1, abort_flag))
-            break;
-          tc_fence_after();
-          const float f = keep * pow2(vref_new - vref);
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(quadrant + kTmemO + c, o);
-            tmem_wait_ld();
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(ts + c, r);
+          tmem_wait_ld();
+          if (masked)
 #pragma unroll
             for (int e = 0; e < 32; e++)
+              r[e] = p0 + c + e < limit ? r[e] : 0xff800000u;
+#pragma unroll
+          for (int e8 = 0; e8 < 32; e8 += 8) {
+            float x = __uint_as_float(r[e8]);
+#pragma unroll
+            for (int e = 1; e < 8; e++)
+              x = fmaxf(x, __uint_as_float(r[e8 + e]));
+            top = fmaxf(top, x * factor((c + e8) >> 3));
+          }
+        }
+        int vmin = vshift[0];
+#pragma unroll
+        for (int w = 1; w < kConvWarps; w++)
+          vmin = min(vmin, vshift[w]);
+        // Move the reference when a score exceeds it by more than 8, and O's power when the values have grown.
+        const bool up = top > m + 8.0f || (m == -INFINITY && top > m);
+        const float m_new = up ? ceilf(top) : m;
+        const int vref_new = use == 0 || vmin < vref ? vmin - 1 : vref;
+        const float keep = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - m_new);
+        if (use > 0 && (vref_new != vref || __any_sync(0xffffffffu, up))) {
+          const float f = keep * pow2(vref_new - vref);
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(to + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; e++)
               o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st32(quadrant + kTmemO + c, o);
+            tmem_st16(to + c, o);
           }
         }
         l *= keep;
         m = m_new;
         vref = vref_new;
-        const float base = m == -INFINITY ? 0.0f : m, grow = pow2(kPShift - vs + vref);
-        float sum = 0.0f;
-        uint32_t hi[32], lo[32];
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t r[32], hi[16], lo[16];
+          tmem_ld32(ts + c, r);
+          tmem_wait_ld();
+          if (masked)
 #pragma unroll
-        for (int c = 0; c < 16; c++) {
-          const float x = ex2(fmaf(__uint_as_float(r0[2 * c]), factor, -base));
-          const float y = ex2(fmaf(__uint_as_float(r0[2 * c + 1]), factor, -base));
-          sum += x + y;
-          split2(x * grow, y * grow, hi[c], lo[c]);
-        }
+            for (int e = 0; e < 32; e++)
+              r[e] = p0 + c + e < limit ? r[e] : 0xff800000u;
 #pragma unroll
-        for (int c = 0; c < 16; c++) {
-          const float x = ex2(fmaf(__uint_as_float(r1[2 * c]), factor, -base));
-          const float y = ex2(fmaf(__uint_as_float(r1[2 * c + 1]), factor, -base));
-          sum += x + y;
-          split2(x * grow, y * grow, hi[16 + c], lo[16 + c]);
+          for (int e8 = 0; e8 < 32; e8 += 8) {
+            // 2^(score - m) times 2^grow, the values' power in the exponent: base and grow are whole numbers. Values
+            // 2^-60 of the largest seen (zeros, mostly) count as that at most, which O does not hold.
+            const float f = factor((c + e8) >> 3);
+            const int grow = max(kPShift - vshift[(c + e8) >> 3] + vref, -60);
+            const float from = (float)grow - base;
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = e8; e < e8 + 8; e += 2) {
+              const float x = ex2(fmaf(__uint_as_float(r[e]), f, from));
+              const float y = ex2(fmaf(__uint_as_float(r[e + 1]), f, from));
+              sum += x + y;
+              split2(f2_pack(x, y), hi[e / 2], lo[e / 2]);
+            }
+            l += sum * pow2(-grow);
+          }
+          tmem_st16(ts + c, hi);
+          tmem_st16(ts + c + 16, lo);
         }
-        l += sum;
-        // The probabilities' buffer: free once the sums of two tiles ago are done.
-        if (j > 1 && !tc_wait(&t->pvdone[s], ((j - 2) >> 1) & 1, abort_flag))
-          break;
-        tmem_st32(quadrant + kTmemP + 64 * s, hi);
-        tmem_st32(quadrant + kTmemP + 64 * s + 32, lo);
         tmem_wait_st();
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0)
-        mbar_arrive(&t->pfull[s]);
+        mbar_arrive(&t->pfull[g]);
     }
-    if (busy && tc_wait(&t->pvdone[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, abort_flag)) {
+    // The odd tiles' statistics go to the even group, which joins the two and writes the partial result.
+    if (g == 1) {
+      t->m[vec_i] = m, t->l[vec_i] = l;
+      t->vref[vec_i] = vref;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
+    if (g == 0 && busy && tc_wait(&t->pvdone[0], ((tiles - 1) >> 1) & 1, abort_flag) &&
+        (tiles < 2 || tc_wait(&t->pvdone[1], ((tiles - 2) >> 1) & 1, abort_flag))) {
       tc_fence_after();
-      const size_t at = (size_t)it.split * a.vectors + (have ? vector_at(a, it.kv, it.first + i) : 0);
+      const float m1 = tiles > 1 ? t->m[vec_i] : -INFINITY, both = fmaxf(m, m1);
+      const float w0 = m == -INFINITY ? 0.0f : ex2(m - both), w1 = m1 == -INFINITY ? 0.0f : ex2(m1 - both);
+      const size_t at = (size_t)it.split * a.vectors + (have ? vector_at(a, it.kv, it.first + vec_i) : 0);
       if (have)
-        a.ml[at] = make_float2(m, l);
-      const int down = -(kPShift + vref);
-      const float f0 = pow2(down / 2), f1 = pow2(down - down / 2);  // 2^down itself may not be a number
+        a.ml[at] = make_float2(both, w0 * l + (tiles > 1 ? w1 * t->l[vec_i] : 0.0f));
+      const int d0 = -(kPShift + vref), d1 = -(kPShift + t->vref[vec_i]);
+      const float f0 = w0 * pow2(d0 / 2), f1 = w1 * pow2(d1 / 2);  // 2^d itself may not be a number
+      const float g0 = pow2(d0 - d0 / 2), g1 = pow2(d1 - d1 / 2);
 #pragma unroll 1
-      for (int c = 0; c < HD; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(quadrant + kTmemO + c, o);
+      for (int c = 0; c < HD; c += 16) {
+        uint32_t o[16], p[16];
+        tmem_ld16(to + c, o);
+        if (tiles > 1)
+          tmem_ld16(to + 128 + c, p);
         tmem_wait_ld();
-        if (have)
+        float x[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            if (c + e < hd)
-              *reinterpret_cast<float4 *>(a.acc + at * hd + c + e) =
-                  make_float4(__uint_as_float(o[e]) * f0 * f1, __uint_as_float(o[e + 1]) * f0 * f1,
-                              __uint_as_float(o[e + 2]) * f0 * f1, __uint_as_float(o[e + 3]) * f0 * f1);
+        for (int e = 0; e < 16; e++) {
+          x[e] = __uint_as_float(o[e]) * f0 * g0;
+          if (tiles > 1)
+            x[e] += __uint_as_float(p[e]) * f1 * g1;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          if (have && c + e < hd)
+            *reinterpret_cast<float4 *>(a.acc + at * hd + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        __syncwarp();
       }
       tc_fence_before();
     }
@@ -678,7 +708,8 @@ bool tc_shape(const SharedArgs &a) {
 
 // A warp per output vector: the splits joined in their order, and optionally quantized in gs-groups as k_quantize does.
 __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs a) {
-  __shared__ float weights[8][2 * kMaxSplits], outs[8][kMaxHd];
+  __shared__ float weights[8][2 * kMaxSplits];
+  __shared__ __align__(16) float outs[8][kMaxHd];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -707,14 +738,44 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs a) {
   for (int o = 16; o; o >>= 1)
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
   __syncwarp();
-  for (int e = lane; e < hd; e += 32) {
-    float o = 0.0f;
-    for (int s = 0; s < splits; s++)
-      if (weights[warp][s] != 0.0f)
-        o = fmaf(weights[warp][s], a.acc[((size_t)s * a.vectors + vec) * hd + e], o);
-    o /= sum;
-    a.out[(size_t)vec * hd + e] = o;
-    outs[warp][e] = o;
+  const float inv = 1.0f / sum;
+  const float *acc = a.acc + (size_t)vec * hd;
+  const size_t step = (size_t)a.vectors * hd;
+  if (hd % 4 == 0) {
+    for (int e = 4 * lane; e < hd; e += 128) {
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int s = 0; s < splits; s += 8) {  // eight loads in flight; a split without weight was not written
+        float4 x[8];
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          w[i] = s + i < splits ? weights[warp][s + i] : 0.0f;
+          x[i] = w[i] != 0.0f ? __ldcg(reinterpret_cast<const float4 *>(acc + (s + i) * step + e))
+                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          o.x = fmaf(w[i], x[i].x, o.x), o.y = fmaf(w[i], x[i].y, o.y), o.z = fmaf(w[i], x[i].z, o.z),
+          o.w = fmaf(w[i], x[i].w, o.w);
+      }
+      o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+      if (((uintptr_t)a.out & 15) == 0)
+        *reinterpret_cast<float4 *>(a.out + (size_t)vec * hd + e) = o;
+      else
+        a.out[(size_t)vec * hd + e] = o.x, a.out[(size_t)vec * hd + e + 1] = o.y, a.out[(size_t)vec * hd + e + 2] = o.z,
+                               a.out[(size_t)vec * hd + e + 3] = o.w;
+      *reinterpret_cast<float4 *>(&outs[warp][e]) = o;
+    }
+  } else {
+    for (int e = lane; e < hd; e += 32) {
+      float o = 0.0f;
+      for (int s = 0; s < splits; s++)
+        if (weights[warp][s] != 0.0f)
+          o = fmaf(weights[warp][s], acc[s * step + e], o);
+      o *= inv;
+      a.out[(size_t)vec * hd + e] = o;
+      outs[warp][e] = o;
+    }
   }
   if (!a.oq)
     return;
@@ -743,17 +804,6 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs a) {
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// How many ways a work's partial results split the prefix and each request's own positions at most.
-int most_prefix_splits(int n_kv, int group, int batch, int rows) {
-  const int tiles = ceil_div(batch * rows * group, 128);
-  const int s = 2 * kPlanSms / (n_kv * tiles);
-  return s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s;
-}
-int most_own_splits(int n_kv, int batch) {
-  const int s = 2 * kPlanSms / (n_kv * batch);
-  return s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s;
-}
-
 bool shape_ok(int n_heads, int n_kv, int hd, int batch, int rows) {
   return n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && hd > 0 && hd <= kMaxHd && batch > 0 && rows > 0 &&
          (long long)batch * rows * n_heads <= (1 << 24);
@@ -762,10 +812,30 @@ bool shape_ok(int n_heads, int n_kv, int hd, int batch, int rows) {
 // Floats of n (m, l) pairs, to a whole number of 16-byte units: the accumulators behind them stay aligned.
 size_t pairs_floats(size_t n) { return (2 * n + 3) & ~(size_t)3; }
 
-size_t partial_floats(int n_heads, int n_kv, int hd, int batch, int rows) {
-  const size_t splits = (size_t)most_prefix_splits(n_kv, n_heads / n_kv, batch, rows) + most_own_splits(n_kv, batch);
-  const size_t pairs = splits * ((size_t)batch * rows * n_heads);
-  return pairs_floats(pairs) + pairs * hd;
+// Partial results of up to 2 * kMaxSplits splits as far as 96 MiB hold them, of two at least (one of the prefix, one of
+// the requests' own positions).
+size_t partial_floats(int n_heads, int hd, int batch, int rows) {
+  const size_t vectors = (size_t)batch * rows * n_heads, each = vectors * (hd + 2);
+  size_t splits = ((size_t)96 << 20) / (sizeof(float) * each);
+  splits = splits < 2 ? 2 : splits > 2 * kMaxSplits ? 2 * kMaxSplits : splits;
+  return splits * each + 4;
+}
+
+// How the positions are split. In units of a tile of 64 positions against a query tile: a CTA costs about kStart units
+// before its first, so the splits are as long as an even share of the work over the SMs allows, and at most kLongest
+// tiles: the tensor cores' accumulators truncate, which over more tiles would show in the result.
+constexpr int kStart = 6, kLongest = 16;
+// `most` splits at most, two at least.
+void plan_splits(SharedArgs *a, int most) {
+  const long long prefix_tiles = ceil_div(a->prefix, kTcPos), own_tiles = ceil_div(a->seq, kTcPos);
+  const long long columns = (long long)a->n_kv * a->tiles, own_columns = (long long)a->n_kv * a->batch * a->own_tiles;
+  const long long units = columns * prefix_tiles + own_columns * ((own_tiles + 1) / 2 + kStart);
+  const long long share = units / kPlanSms;
+  auto clamp = [](long long v, long long low, long long high) { return v < low ? low : v > high ? high : v; };
+  const int prefix_length = (int)clamp(share / 2, 2, kLongest), own_length = (int)clamp(share, 4, kLongest);
+  a->own_splits = (int)clamp(ceil_div((int)own_tiles, own_length), 1, kMaxSplits < most / 2 ? kMaxSplits : most / 2);
+  const int rest = most - a->own_splits;
+  a->prefix_splits = (int)clamp(ceil_div((int)prefix_tiles, prefix_length), 0, kMaxSplits < rest ? kMaxSplits : rest);
 }
 
 size_t generic_smem(int hd) { return sizeof(float) * ((size_t)kGenericPos * (2 * hd + 1) + 4 * (size_t)hd); }
@@ -777,7 +847,7 @@ extern "C" {
 size_t k_attention_shared_bytes(int n_heads, int n_kv_heads, int head_dim, int batch, int rows) {
   if (!shape_ok(n_heads, n_kv_heads, head_dim, batch, rows))
     return 0;
-  return sizeof(float) * partial_floats(n_heads, n_kv_heads, head_dim, batch, rows);
+  return sizeof(float) * partial_floats(n_heads, head_dim, batch, rows);
 }
 
 void k_attention_shared_init(AttentionWork *work, int n_heads, int n_kv_heads, int head_dim, int batch, int rows,
@@ -799,11 +869,9 @@ void k_attention_shared_init(AttentionWork *work, int n_heads, int n_kv_heads, i
     return;
   }
   work->partial = static_cast<float *>(base);
-  work->max_chunks = most_prefix_splits(n_kv_heads, n_heads / n_kv_heads, batch, rows) +
-                     most_own_splits(n_kv_heads, batch);
   work->n_heads = n_heads;
   work->head_dim = head_dim;
-  work->workers = 1;
+  work->workers = batch * rows;
   work->external = memory != nullptr;
   work->capacity = bytes / sizeof(float);
 }
@@ -830,8 +898,8 @@ void k_attention_shared_rows(float *out, int8_t *oq, float *os, const float *q, 
     kc_fail("%s: group size %d does not divide the head's %d outputs", name, gs, head_dim);
     return;
   }
-  if (!work || !work->partial || work->n_heads != n_heads || work->head_dim != head_dim ||
-      work->capacity < partial_floats(n_heads, n_kv_heads, head_dim, batch, rows)) {
+  if (!work || !work->partial || work->max_chunks != 0 || work->n_heads != n_heads || work->head_dim != head_dim ||
+      (long long)batch * rows > work->workers) {
     kc_fail("%s: the attention work is missing or too small for this shape", name);
     return;
   }
@@ -842,16 +910,14 @@ void k_attention_shared_rows(float *out, int8_t *oq, float *os, const float *q, 
   a.n_heads = n_heads, a.n_kv = n_kv_heads, a.group = n_heads / n_kv_heads, a.hd = head_dim;
   a.prefix_seq = prefix_seq_len, a.prefix = prefix, a.seq = seq_len, a.batch = batch, a.rows = rows, a.gs = gs;
   a.vectors = batch * rows * n_heads;
-  const int most_p = most_prefix_splits(n_kv_heads, a.group, batch, rows), most_o = most_own_splits(n_kv_heads, batch);
-  a.prefix_splits = prefix ? (ceil_div(prefix, 64) < most_p ? ceil_div(prefix, 64) : most_p) : 0;
-  a.own_splits = ceil_div(seq_len, 64) < most_o ? ceil_div(seq_len, 64) : most_o;
-  const size_t splits = (size_t)a.prefix_splits + a.own_splits;
-  a.ml = reinterpret_cast<float2 *>(work->partial);
-  a.acc = work->partial + pairs_floats(splits * a.vectors);
   const bool tc = tc_shape(a);
   const int tile = tc ? kTcVecs : kGenericVecs;
   a.tiles = ceil_div(batch * rows * a.group, tile);
   a.own_tiles = ceil_div(rows * a.group, tile);
+  plan_splits(&a, (int)((work->capacity - 4) / ((size_t)a.vectors * (head_dim + 2))));
+  const size_t splits = (size_t)a.prefix_splits + a.own_splits;
+  a.ml = reinterpret_cast<float2 *>(work->partial);
+  a.acc = work->partial + pairs_floats(splits * a.vectors);
   const long long items = (long long)n_kv_heads * ((long long)a.tiles * a.prefix_splits +
                                                    (long long)batch * a.own_tiles * a.own_splits);
   if (items > 0x7fffffff) {

@@ -226,9 +226,13 @@ template <int HD>
 struct TcSmem {
   static constexpr int kv_bytes = kTcPos * HD * 2;  // hi or lo of K or V
   static constexpr int stage = 4 * kv_bytes;
-  static constexpr int tail_at = 2 * stage;
-  static constexpr int total = tail_at + 4096 + 1024;  // the tail, and room to align the start to 1 KiB
+  static constexpr int raw_at = 2 * stage;          // the next tile's keys and values as they come, a slot per converter
+  static constexpr int tail_at = raw_at + 2 * kTcPos * HD * 4;
+  static constexpr int total = tail_at + 5120 + 1024;  // the tail, and room to align the start to 1 KiB
+  static constexpr int row = HD + 4;  // floats of a vector's row where queries and results pass through the stages
 };
+static_assert(kTcVecs * TcSmem<64>::row * 4 <= TcSmem<64>::raw_at && kTcVecs * TcSmem<128>::row * 4 <= TcSmem<128>::raw_at,
+              "the stages hold a tile of queries or results");
 
 struct TcTail {
   uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2];
@@ -236,11 +240,11 @@ struct TcTail {
   int abort_flag;
   float kscale[4][kConvWarps];  // 2^-k of eight keys, a ring of tiles
   int vshift[4][kConvWarps];    // k of eight values
-  unsigned qmax[2][kTcVecs];
-  float m[kTcVecs], l[kTcVecs];  // of the odd tiles, and O's power
-  int vref[kTcVecs];
+  float qmax[2][kTcVecs];
+  float m[2][kTcVecs], l[2][kTcVecs];  // of a group's tiles, and the power of its O
+  int vref[2][kTcVecs];
 };
-static_assert(sizeof(TcTail) <= 4096, "the tail's room");
+static_assert(sizeof(TcTail) <= 5120, "the tail's room");
 
 // A whole warp's bounded wait, with one answer for all lanes: false once any wait of the CTA has given up.
 __device__ __forceinline__ bool tc_wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
@@ -323,34 +327,54 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ unsigned abs_max(unsigned m, float x) { return max(m, __float_as_uint(fabsf(x))); }
+__device__ __forceinline__ float abs_max(float m, float4 v) {
+  return fmaxf(fmaxf(fmaxf(m, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+}
 
-// Eight rows of a tile in a warp's registers: HD / 4 lanes to a row.
+// 16 bytes from global to shared memory, asynchronously; zeros without `in`.
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the newest group of this thread's copies are done.
+__device__ __forceinline__ void copy_wait1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+
+// Eight rows of a tile in a warp's registers: HD / 4 lanes to a row. They come by way of a slot of shared memory, where
+// every lane reads what it copied itself.
 template <int HD>
 struct Rows8 {
   static constexpr int kSteps = HD / 16;    // float4 a lane: 8 or 4
   static constexpr int kAt = 128 / HD;      // rows a step
   float4 x[kSteps];
+  float top;
 
-  // Rows [row0, row0 + 8) of cache rows of hd floats; rows from `end` on and columns from hd on are zeros.
-  __device__ __forceinline__ void load(const float *cache, int row0, int end, int hd, int lane) {
+  // Starts the copy of rows [row0, row0 + 8) of cache rows of hd floats; rows from `end` on and columns from hd on are
+  // zeros.
+  static __device__ __forceinline__ void copy(float4 *slot, const float *cache, int row0, int end, int hd, int lane) {
     const int col = lane * 4 % HD, r = lane * 4 / HD;
     const float *src = cache + (size_t)(row0 + r) * hd + col;
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
-      x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (row0 + r + i * kAt < end && col < hd)
-        x[i] = __ldcg(reinterpret_cast<const float4 *>(src + (size_t)i * kAt * hd));
+      const bool in = row0 + r + i * kAt < end && col < hd;
+      copy16(slot + 32 * i + lane, in ? src + (size_t)i * kAt * hd : cache, in);
     }
+  }
+  __device__ __forceinline__ void take(const float4 *slot, int lane) {
+    top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSteps; i++)
+      x[i] = slot[32 * i + lane];
+#pragma unroll
+    for (int i = 0; i < kSteps; i++)
+      top = abs_max(top, x[i]);
+    // The values are here before the slot's next copy starts.
+    asm volatile("" : "+f"(top)::"memory");
   }
   // Splits the rows and stores them as rows row .. row + 7 of the operand pair (64 rows of 128 swizzled bytes to 64
   // columns); returns their power of two.
   __device__ __forceinline__ int store(uint8_t *hi_at, uint8_t *lo_at, int row, int lane) const {
-    unsigned mx = 0;
-#pragma unroll
-    for (int i = 0; i < kSteps; i++)
-      mx = abs_max(abs_max(abs_max(abs_max(mx, x[i].x), x[i].y), x[i].z), x[i].w);
-    const int k = shift_for(__reduce_max_sync(0xffffffffu, mx));
+    const int k = shift_for(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
     const uint64_t f = f2_pack(pow2(k), pow2(k));
     const int col = lane * 4 % HD, r = lane * 4 / HD;
     const uint32_t base = (col >> 6) * (kTcPos * 128) + row * 128 + (col & 7) * 2;
@@ -403,8 +427,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
   if (warp == kSoftWarps)
     tmem_alloc(&t->tmem, kTmemCols);
   const int hd = a.hd;
-  Rows8<HD> kx, vx;
   const int cw = warp - kSoftWarps - 1;
+  float4 *kslot = reinterpret_cast<float4 *>(smem + L::raw_at) + max(cw, 0) * (4 * HD), *vslot = kslot + 2 * HD;
+  if (cw >= 0) {
+    Rows8<HD>::copy(kslot, it.k, it.p0 + 8 * cw, it.p1, hd, lane);
+    copy_commit();
+    Rows8<HD>::copy(vslot, it.v, it.p0 + 8 * cw, it.p1, hd, lane);
+    copy_commit();
+  } else if (warp < kSoftWarps) {
+    // The queries into the stages, a warp per row, eight rows in flight. Vectors not in use are zeros.
+    const bool wide = ((uintptr_t)a.q & 15) == 0;
+    int vec = -1;
+    const int mine = it.first + warp + kSoftWarps * lane;
+    if (warp + kSoftWarps * lane < it.vecs) {
+      const int row = mine / a.group, b = row / a.rows, count = rows_of(a, b);
+      if (row - b * a.rows < count && request_ok(a, b, count))
+        vec = vector_at(a, it.kv, mine);
+    }
+    const int e = 4 * lane;
+    for (int n0 = 0; warp + kSoftWarps * n0 < it.vecs; n0 += 8) {
+      float4 y[8];
+#pragma unroll
+      for (int n = 0; n < 8; n++) {
+        const int v = __shfl_sync(0xffffffffu, vec, n0 + n);
+        const float *src = a.q + (size_t)max(v, 0) * hd + e;
+        y[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (v >= 0 && e < hd)
+          y[n] = wide ? *reinterpret_cast<const float4 *>(src) : make_float4(src[0], src[1], src[2], src[3]);
+      }
+#pragma unroll
+      for (int n = 0; n < 8; n++) {
+        const int i = warp + kSoftWarps * (n0 + n);
+        if (i < it.vecs && e < HD)
+          *reinterpret_cast<float4 *>(smem + ((size_t)i * L::row + e) * 4) = y[n];
+      }
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -418,34 +476,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
   if (warp < kSoftWarps) {
     constexpr int H = HD / 2;
     float x[H];
-    bool use = have;
-    if (use) {
-      const int row = (it.first + vec_i) / a.group, b = row / a.rows, count = rows_of(a, b);
-      use = row - b * a.rows < count && request_ok(a, b, count);
-    }
-    unsigned mx = 0;
+    float mx = 0.0f;
     if (busy) {
-      const float *src = a.q + (size_t)(use ? vector_at(a, it.kv, it.first + vec_i) : 0) * hd + g * H;
-      if (((uintptr_t)a.q & 15) == 0) {
+      const float *src = reinterpret_cast<const float *>(smem) + (size_t)vec_i * L::row + g * H;
 #pragma unroll
-        for (int e = 0; e < H; e += 4) {
-          float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (use && g * H + e < hd)
-            y = *reinterpret_cast<const float4 *>(src + e);
-          x[e] = y.x, x[e + 1] = y.y, x[e + 2] = y.z, x[e + 3] = y.w;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < H; e++)
-          x[e] = use && g * H + e < hd ? src[e] : 0.0f;
+      for (int e = 0; e < H; e += 4) {
+        const float4 y = have ? *reinterpret_cast<const float4 *>(src + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        x[e] = y.x, x[e + 1] = y.y, x[e + 2] = y.z, x[e + 3] = y.w;
+        mx = abs_max(mx, y);
       }
-#pragma unroll
-      for (int e = 0; e < H; e++)
-        mx = abs_max(mx, x[e]);
     }
     t->qmax[g][vec_i] = mx;
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
-    qshift = shift_for(max(t->qmax[0][vec_i], t->qmax[1][vec_i]));
+    qshift = shift_for(__float_as_uint(fmaxf(t->qmax[0][vec_i], t->qmax[1][vec_i])));
     if (busy) {
       const uint64_t f = f2_pack(pow2(qshift), pow2(qshift));
 #pragma unroll
@@ -459,9 +502,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       }
       tmem_wait_st();
     }
-  } else if (cw >= 0) {  // the first tile's keys and values come meanwhile
-    kx.load(it.k, it.p0 + 8 * cw, it.p1, hd, lane);
-    vx.load(it.v, it.p0 + 8 * cw, it.p1, hd, lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -469,8 +509,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
 
   if (warp > kSoftWarps) {
     // ---- converters ----
+    // Registers hold tile j, the slots tile j + 1 as it comes. Every copy is a group of its own, empty past the last.
+    Rows8<HD> kx, vx;
+    auto next = [&](Rows8<HD> &x, float4 *slot, const float *cache, int tile) {
+      copy_wait1();
+      x.take(slot, lane);
+      if (tile < tiles)
+        Rows8<HD>::copy(slot, cache, it.p0 + tile * kTcPos + 8 * cw, it.p1, hd, lane);
+      copy_commit();
+    };
+    next(kx, kslot, it.k, 1);
+    next(vx, vslot, it.v, 1);
     for (int j = 0; j < tiles; j++) {
-      const int s = j & 1, use = j >> 1, row0 = it.p0 + (j + 1) * kTcPos + 8 * cw;
+      const int s = j & 1, use = j >> 1;
       uint8_t *stage = smem + s * L::stage;
       tc_wait(&t->kempty[s], (use & 1) ^ 1, abort_flag);
       const int ks = kx.store(stage, stage + L::kv_bytes, 8 * cw, lane);
@@ -480,8 +531,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&t->kfull[s]);
-      if (j + 1 < tiles)
-        kx.load(it.k, row0, it.p1, hd, lane);
+      next(kx, kslot, it.k, j + 2);
       tc_wait(&t->vempty[s], (use & 1) ^ 1, abort_flag);
       const int vs = vx.store(stage + 2 * L::kv_bytes, stage + 3 * L::kv_bytes, 8 * cw, lane);
       if (lane == 0)
@@ -490,8 +540,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&t->vfull[s]);
-      if (j + 1 < tiles)
-        vx.load(it.v, row0, it.p1, hd, lane);
+      next(vx, vslot, it.v, j + 2);
     }
   } else if (warp == kSoftWarps) {
     // ---- MMA issue. The scores of tile j + 1 go out before the sums of tile j, so that they run under its softmax; the
@@ -551,8 +600,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     int vref = 0;  // O holds sums times 2^(kPShift + vref)
     for (int j = g; j < tiles; j += 2) {
       const int use = j >> 1;
-      // The scores; with them the group's previous sums are done, so O can be rescaled. The values' powers.
-      if (!tc_wait(&t->sfull[g], use & 1, abort_flag) || !tc_wait(&t->vfull[g], use & 1, abort_flag))
+      // The scores, the values' powers, and the group's previous sums: O can be rescaled. (Those are done when the
+      // scores are; the wait keeps step with the barrier's phases.)
+      if (!tc_wait(&t->sfull[g], use & 1, abort_flag) || !tc_wait(&t->vfull[g], use & 1, abort_flag) ||
+          (use > 0 && !tc_wait(&t->pvdone[g], (use - 1) & 1, abort_flag)))
         break;
       tc_fence_after();
       if (busy) {
@@ -645,45 +696,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       if (lane == 0)
         mbar_arrive(&t->pfull[g]);
     }
-    // The odd tiles' statistics go to the even group, which joins the two and writes the partial result.
-    if (g == 1) {
-      t->m[vec_i] = m, t->l[vec_i] = l;
-      t->vref[vec_i] = vref;
-    }
+    // The two groups' results joined, by way of the stages (no MMA reads them any more), into the partial result.
+    t->m[g][vec_i] = m, t->l[g][vec_i] = l, t->vref[g][vec_i] = vref;
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
-    if (g == 0 && busy && tc_wait(&t->pvdone[0], ((tiles - 1) >> 1) & 1, abort_flag) &&
-        (tiles < 2 || tc_wait(&t->pvdone[1], ((tiles - 2) >> 1) & 1, abort_flag))) {
+    const bool done = tc_wait(&t->pvdone[0], ((tiles - 1) >> 1) & 1, abort_flag) &&
+                      (tiles < 2 || tc_wait(&t->pvdone[1], ((tiles - 2) >> 1) & 1, abort_flag));
+    // Group g joins half g of the elements.
+    if (done && busy) {
       tc_fence_after();
-      const float m1 = tiles > 1 ? t->m[vec_i] : -INFINITY, both = fmaxf(m, m1);
-      const float w0 = m == -INFINITY ? 0.0f : ex2(m - both), w1 = m1 == -INFINITY ? 0.0f : ex2(m1 - both);
-      const size_t at = (size_t)it.split * a.vectors + (have ? vector_at(a, it.kv, it.first + vec_i) : 0);
-      if (have)
-        a.ml[at] = make_float2(both, w0 * l + (tiles > 1 ? w1 * t->l[vec_i] : 0.0f));
-      const int d0 = -(kPShift + vref), d1 = -(kPShift + t->vref[vec_i]);
+      const float m0 = t->m[0][vec_i], m1 = t->m[1][vec_i], both = fmaxf(m0, m1);
+      const float w0 = m0 == -INFINITY ? 0.0f : ex2(m0 - both), w1 = m1 == -INFINITY ? 0.0f : ex2(m1 - both);
+      if (have && g == 0)
+        a.ml[(size_t)it.split * a.vectors + vector_at(a, it.kv, it.first + vec_i)] =
+            make_float2(both, w0 * t->l[0][vec_i] + w1 * t->l[1][vec_i]);
+      const int d0 = -(kPShift + t->vref[0][vec_i]), d1 = -(kPShift + t->vref[1][vec_i]);
       const float f0 = w0 * pow2(d0 / 2), f1 = w1 * pow2(d1 / 2);  // 2^d itself may not be a number
       const float g0 = pow2(d0 - d0 / 2), g1 = pow2(d1 - d1 / 2);
+      float *row = reinterpret_cast<float *>(smem) + (size_t)vec_i * L::row;
+      const uint32_t from = quadrant + kTmemO;
 #pragma unroll 1
-      for (int c = 0; c < HD; c += 16) {
+      for (int c = g * (HD / 2); c < (g + 1) * (HD / 2); c += 16) {
         uint32_t o[16], p[16];
-        tmem_ld16(to + c, o);
+        tmem_ld16(from + c, o);
         if (tiles > 1)
-          tmem_ld16(to + 128 + c, p);
+          tmem_ld16(from + 128 + c, p);
         tmem_wait_ld();
-        float x[16];
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          x[e] = __uint_as_float(o[e]) * f0 * g0;
-          if (tiles > 1)
-            x[e] += __uint_as_float(p[e]) * f1 * g1;
+        for (int e = 0; e < 16; e += 4) {
+          float y[4];
+#pragma unroll
+          for (int n = 0; n < 4; n++) {
+            y[n] = __uint_as_float(o[e + n]) * f0 * g0;
+            if (tiles > 1)
+              y[n] += __uint_as_float(p[e + n]) * f1 * g1;
+          }
+          *reinterpret_cast<float4 *>(row + c + e) = make_float4(y[0], y[1], y[2], y[3]);
         }
-#pragma unroll
-        for (int e = 0; e < 16; e += 4)
-          if (have && c + e < hd)
-            *reinterpret_cast<float4 *>(a.acc + at * hd + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-        __syncwarp();
       }
       tc_fence_before();
     }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
+    if (done)
+      for (int i = warp; i < it.vecs; i += kSoftWarps) {
+        float *dst = a.acc + ((size_t)it.split * a.vectors + vector_at(a, it.kv, it.first + i)) * hd;
+        for (int e = 4 * lane; e < hd; e += 128)
+          *reinterpret_cast<float4 *>(dst + e) =
+              *reinterpret_cast<const float4 *>(smem + ((size_t)i * L::row + e) * 4);
+      }
   }
   __syncthreads();
   if (warp == kSoftWarps) {

@@ -46,10 +46,16 @@ struct SharedArgs {
   int tiles, own_tiles;           // query tiles per KV head: of the prefix part, of a request's own part
 };
 
-__device__ __forceinline__ int rows_of(const SharedArgs &a, int b) { return a.counts ? a.counts[b] : a.rows; }
-// A request whose rows the kernels compute: a row count within the call and own positions within the cache.
-__device__ __forceinline__ bool request_ok(const SharedArgs &a, int b, int count) {
-  return count > 0 && count <= a.rows && a.starts[b] >= 0 && a.starts[b] <= a.seq - count;
+// Rows that request b uses and the positions it has stored before them; 0 rows where they are not sound. Both loads go
+// out at once.
+struct Request {
+  int count, start;
+  bool bad;
+};
+__device__ __forceinline__ Request request_of(const SharedArgs &a, int b) {
+  const int count = a.counts ? a.counts[b] : a.rows, start = a.starts[b];
+  const bool ok = count > 0 && count <= a.rows && start >= 0 && start <= a.seq - count;
+  return Request{ok ? count : 0, start, !ok && count != 0};
 }
 
 // One work item: up to a tile of query vectors of one KV head against a range of one cache's positions.
@@ -57,6 +63,7 @@ struct Item {
   const float *k, *v;  // the KV head's rows
   int kv, split;       // split: index of the partial result
   int b;               // the request, or -1: the prefix
+  int start;           // the request's positions before its rows
   int first, vecs;     // tile vectors: the flat (b, r, group member) index of the first, and how many
   int p0, p1;          // positions
 };
@@ -91,20 +98,21 @@ __device__ __forceinline__ bool item_at(const SharedArgs &a, int id, int tile, I
   id /= a.own_tiles;
   it->kv = id % a.n_kv;
   it->b = id / a.n_kv;
-  const int count = rows_of(a, it->b);
-  if (!request_ok(a, it->b, count)) {
-    if (count != 0 && threadIdx.x == 0)
+  const Request r = request_of(a, it->b);
+  if (!r.count) {
+    if (r.bad && threadIdx.x == 0)
       kc_raise(KC_ERR_BAD_ARGS);
     return false;
   }
   it->first = it->b * a.rows * a.group + own_tile;
-  it->vecs = min(tile, count * a.group - own_tile);
+  it->vecs = min(tile, r.count * a.group - own_tile);
   if (it->vecs <= 0)
     return false;
   const size_t head = ((size_t)it->b * a.n_kv + it->kv) * a.seq * a.hd;
   it->k = a.k + head;
   it->v = a.v + head;
-  const int length = a.starts[it->b] + count;
+  it->start = r.start;
+  const int length = r.start + r.count;
   it->p0 = (int)((long long)length * split / a.own_splits);
   it->p1 = (int)((long long)length * (split + 1) / a.own_splits);
   return true;
@@ -114,7 +122,7 @@ __device__ __forceinline__ bool item_at(const SharedArgs &a, int id, int tile, I
 __device__ __forceinline__ int limit_of(const SharedArgs &a, const Item &it, int i) {
   if (it.b < 0)
     return it.p1;
-  return min(it.p1, a.starts[it.b] + (i - it.b * a.rows * a.group) / a.group + 1);
+  return min(it.p1, it.start + (i - it.b * a.rows * a.group) / a.group + 1);
 }
 
 // Any head_dim up to 256 and any alignment, in fp32 FMAs: a warp takes 8 of the tile's 32 vectors in turn, its lanes
@@ -435,29 +443,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     Rows8<HD>::copy(vslot, it.v, it.p0 + 8 * cw, it.p1, hd, lane);
     copy_commit();
   } else if (warp < kSoftWarps) {
-    // The queries into the stages, a warp per row, eight rows in flight. Vectors not in use are zeros.
+    // The queries into the stages, a warp per row, eight rows in flight. Vectors not in use are zeros (what lies there
+    // is read, but not taken).
     const bool wide = ((uintptr_t)a.q & 15) == 0;
-    int vec = -1;
+    int vec = 0, use = 0;
     const int mine = it.first + warp + kSoftWarps * lane;
     if (warp + kSoftWarps * lane < it.vecs) {
-      const int row = mine / a.group, b = row / a.rows, count = rows_of(a, b);
-      if (row - b * a.rows < count && request_ok(a, b, count))
-        vec = vector_at(a, it.kv, mine);
+      const int row = mine / a.group, b = row / a.rows;
+      vec = vector_at(a, it.kv, mine);
+      use = row - b * a.rows < request_of(a, b).count;
     }
     const int e = 4 * lane;
     for (int n0 = 0; warp + kSoftWarps * n0 < it.vecs; n0 += 8) {
       float4 y[8];
 #pragma unroll
       for (int n = 0; n < 8; n++) {
-        const int v = __shfl_sync(0xffffffffu, vec, n0 + n);
-        const float *src = a.q + (size_t)max(v, 0) * hd + e;
+        const float *src = a.q + (size_t)__shfl_sync(0xffffffffu, vec, n0 + n) * hd + e;
         y[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (v >= 0 && e < hd)
+        if (e < hd)
           y[n] = wide ? *reinterpret_cast<const float4 *>(src) : make_float4(src[0], src[1], src[2], src[3]);
       }
 #pragma unroll
       for (int n = 0; n < 8; n++) {
         const int i = warp + kSoftWarps * (n0 + n);
+        if (!__shfl_sync(0xffffffffu, use, n0 + n))
+          y[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (i < it.vecs && e < HD)
           *reinterpret_cast<float4 *>(smem + ((size_t)i * L::row + e) * 4) = y[n];
       }
@@ -776,22 +786,27 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs a) {
   if (vec >= a.vectors)
     return;
   const int row = vec / a.n_heads, b = row / a.rows, r = row - b * a.rows;
-  const int count = rows_of(a, b);
-  if (!request_ok(a, b, count) || r >= count)
-    return;  // rows out of use stay as they were
   const int splits = a.prefix_splits + a.own_splits, hd = a.hd;
-  float top = -INFINITY;
-  for (int s = lane; s < splits; s += 32)
-    top = fmaxf(top, a.ml[(size_t)s * a.vectors + vec].x);
+  const Request request = request_of(a, b);
+  constexpr int kPer = 2 * kMaxSplits / 32;
+  float2 ml[kPer];  // read before the request is looked at: one round trip
+#pragma unroll
+  for (int i = 0; i < kPer; i++)
+    ml[i] = lane + 32 * i < splits ? __ldcg(&a.ml[(size_t)(lane + 32 * i) * a.vectors + vec]) : make_float2(-INFINITY, 0.0f);
+  if (r >= request.count)
+    return;  // rows out of use stay as they were
+  float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPer; i++)
+    top = fmaxf(top, ml[i].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1)
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum = 0.0f;
-  for (int s = lane; s < splits; s += 32) {
-    const float2 ml = a.ml[(size_t)s * a.vectors + vec];
-    const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
-    weights[warp][s] = w;
-    sum += w * ml.y;
+#pragma unroll
+  for (int i = 0; i < kPer; i++) {
+    const float w = ml[i].x == -INFINITY ? 0.0f : exp2f(ml[i].x - top);
+    weights[warp][lane + 32 * i] = w;
+    sum += w * ml[i].y;
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1)

@@ -206,14 +206,17 @@ def _check_host():
 
 def _stream():
     import torch
-    load().kernels_set_stream(ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    if not torch.cuda.is_initialized():
+        torch.cuda.init()
+    _lib.kernels_set_stream(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def _call(name, *args):
-    L = init()
+    L = _lib if _ready else init()
     _stream()
     r = getattr(L, name)(*args)
-    _check_host()
+    if L.kc_last_error():
+        _check_host()
     return r
 
 
@@ -227,7 +230,7 @@ def status():
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _weight(q, s):

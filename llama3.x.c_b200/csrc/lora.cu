@@ -1,9 +1,10 @@
 // Low-rank adapters of many requests beside a shared projection (k_lora_rows): out[r] = base[r] + scale B (A x[r]) with
 // the adapter that row r names, A [rank][n] and B [d][rank] in fp32, bf16 or fp16. Products and sums are fp32.
 //
-// One launch: a cluster of CTAs per row. Each CTA takes a slice of n for A x, the cluster sums the slices' partial
-// vectors through distributed shared memory in CTA order (no atomics: the same bits on every call), and each CTA then
-// takes a slice of d for B. The rank-long vector between the two products never leaves the SMs.
+// One launch: a cluster of CTAs per row, or per tile of up to 64 rows of one adapter. Each CTA takes a slice of n for
+// A x, the cluster sums the slices' partial vectors through distributed shared memory in CTA order (no atomics: the same
+// bits on every call), and each CTA then takes a slice of d for B. The rank-long vectors between the two products never
+// leave the SMs.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -57,7 +58,7 @@ __device__ __forceinline__ void load8(const __half *p, float (&v)[8]) { halves<_
 __device__ __forceinline__ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename W>
-__global__ void __launch_bounds__(kThreads) lora_row_kernel(const LoraArgs a) {
+__global__ void __launch_bounds__(kThreads) lora_row_kernel(const LoraArgs a, int) {
   __shared__ float part[kMaxRank], h[kMaxRank];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
@@ -136,12 +137,348 @@ __global__ void __launch_bounds__(kThreads) lora_row_kernel(const LoraArgs a) {
   }
 }
 
+// ---- tiles of rows ------------------------------------------------------------------------------------------------
+
+// Many rows: tiles of up to 64 rows of one adapter, wherever they lie in the batch, so that a tile reads its adapter
+// once. Every CTA finds its tile in the index array by itself (a histogram of the adapters, then the tile's rows in
+// order): no sorting launch and no workspace. Rows without an adapter form tiles too, which copy their base.
+//
+// Products on mma.sync m16n8k8 tf32 with both operands' 24 bits kept: x = hi + lo with hi its upper 11 bits, bf16 and
+// fp16 weights are exact in tf32, fp32 ones split like x: hi w + lo w (+ hi w_lo), off by 2^-22 of a product. The tensor
+// core's sums truncate, so they run over 32 elements only and are added up in fp32 registers. The k index of a
+// fragment is free as long as both operands agree: a lane's two fragment columns of four steps are eight neighbouring
+// elements, one 16- or 32-byte read, without a pass through shared memory.
+constexpr int kTileRows = 64;
+constexpr int kMaxBins = 2048;       // adapters + 1 of the histogram
+constexpr int kMaxTileRows = 16384;  // rows of a launch: every CTA reads their indices
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t tf32_hi(float x) { return __float_as_uint(x) & 0xffffe000u; }
+__device__ __forceinline__ uint32_t tf32_lo(float x) { return __float_as_uint(x - __uint_as_float(tf32_hi(x))); }
+
+// Eight elements of a row as they lie in memory, so that many can be under way.
 template <typename W>
-cudaError_t launch(const LoraArgs &a) {
+struct Raw8 {
+  uint4 v[sizeof(W) / 2];
+
+  // From element i on, zeros from `end` on. `wide`: whole groups of eight at 16-byte addresses.
+  __device__ __forceinline__ void load(const W *row, int i, int end, bool wide) {
+    if (wide && i + 8 <= end) {
+#pragma unroll
+      for (int j = 0; j < (int)(sizeof(W) / 2); j++)
+        v[j] = __ldg(reinterpret_cast<const uint4 *>(row + i) + j);
+    } else {
+      W *at = reinterpret_cast<W *>(v);
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        at[j] = i + j < end ? row[i + j] : W(0.0f);
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const W *at = reinterpret_cast<const W *>(v);
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      f[j] = to_float(at[j]);
+  }
+};
+
+// 16 rows x 8 columns += 32 elements of the 16 rows (this lane's eight of rows g and g + 8) times those of the 8 columns
+// (this lane's eight of column g). SPLIT: the weights have more bits than tf32.
+template <bool SPLIT>
+__device__ __forceinline__ void product32(float (&sum)[4], const float (&x0)[8], const float (&x1)[8],
+                                          const float (&w)[8]) {
+  float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int s = 0; s < 4; s++) {
+    const uint32_t lo[4] = {tf32_lo(x0[2 * s]), tf32_lo(x1[2 * s]), tf32_lo(x0[2 * s + 1]), tf32_lo(x1[2 * s + 1])};
+    const uint32_t hi[4] = {tf32_hi(x0[2 * s]), tf32_hi(x1[2 * s]), tf32_hi(x0[2 * s + 1]), tf32_hi(x1[2 * s + 1])};
+    const uint32_t b0 = tf32_hi(w[2 * s]), b1 = tf32_hi(w[2 * s + 1]);
+    mma_tf32(d, lo, b0, b1);
+    if (SPLIT)
+      mma_tf32(d, hi, tf32_lo(w[2 * s]), tf32_lo(w[2 * s + 1]));
+    mma_tf32(d, hi, b0, b1);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    sum[i] += d[i];
+}
+
+// The cluster's tile: its adapter (`count`: rows without one) and its rows in order. False: no such tile.
+struct LoraTile {
+  int bins[kMaxBins];
+  int rows[kTileRows];
+  int warp_sums[kWarps];
+  int adapter, part, n;
+};
+
+__device__ bool find_tile(const LoraArgs &a, LoraTile *t, int tile) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bins = a.count + 1;
+  auto bin_of = [&](int r) {
+    const int id = a.index[r];
+    return id >= 0 && id < a.count ? id : a.count;
+  };
+  for (int i = threadIdx.x; i < bins; i += kThreads)
+    t->bins[i] = 0;
+  if (threadIdx.x == 0)
+    t->adapter = -1;
+  __syncthreads();
+  for (int r = threadIdx.x; r < a.rows; r += kThreads)
+    atomicAdd(&t->bins[bin_of(r)], 1);
+  __syncthreads();
+  // The adapter whose tiles hold number `tile`: a running sum over the adapters' tiles.
+  int before = 0;
+  for (int i0 = 0; i0 < bins; i0 += kThreads) {
+    const int i = i0 + threadIdx.x, tiles = i < bins ? (t->bins[i] + kTileRows - 1) / kTileRows : 0;
+    int upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o)
+        upto += other;
+    }
+    if (lane == 31)
+      t->warp_sums[warp] = upto;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < kWarps; w++) {
+      if (w < warp)
+        upto += t->warp_sums[w];
+      all += t->warp_sums[w];
+    }
+    if (tile >= before + upto - tiles && tile < before + upto) {
+      t->adapter = i;
+      t->part = tile - (before + upto - tiles);
+      t->n = min(kTileRows, t->bins[i] - t->part * kTileRows);
+    }
+    before += all;
+    __syncthreads();
+  }
+  if (t->adapter < 0)
+    return false;
+  // Its rows: every thread a run of neighbouring rows, ranked by the matches before it.
+  const int per = (a.rows + kThreads - 1) / kThreads, r0 = min((int)threadIdx.x * per, a.rows), r1 = min(r0 + per, a.rows);
+  int mine = 0;
+  for (int r = r0; r < r1; r++)
+    mine += bin_of(r) == t->adapter;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o)
+      upto += other;
+  }
+  if (lane == 31)
+    t->warp_sums[warp] = upto;
+  __syncthreads();
+  int rank = upto - mine - t->part * kTileRows;
+  for (int w = 0; w < warp; w++)
+    rank += t->warp_sums[w];
+  for (int r = r0; r < r1; r++)
+    if (bin_of(r) == t->adapter) {
+      if (rank >= 0 && rank < kTileRows)
+        t->rows[rank] = r;
+      rank++;
+    }
+  __syncthreads();
+  return true;
+}
+
+// Floats of a row of the tile's vectors: the rank in whole 32s, and 4 so that neighbouring rows lie in other banks.
+__host__ __device__ constexpr int h_stride(int max_rank) { return (max_rank + 31) / 32 * 32 + 4; }
+
+// parts clusters share a tile: each computes its vectors and takes a part of d.
+template <typename W>
+__global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a, int parts) {
+  extern __shared__ __align__(16) float smem[];
+  __shared__ LoraTile t;
+  constexpr bool kSplit = sizeof(W) == 4;
+  constexpr int kFlight = kSplit ? 4 : 8;  // column groups whose weights are under way at once
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = cluster.num_blocks(), rank = cluster.block_rank(), id = blockIdx.x / ctas;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (!find_tile(a, &t, id / parts))
+    return;  // the whole cluster
+  const int part = id % parts, rows = t.n, hs = h_stride(a.max_rank);
+  float *partial = smem, *h = smem + kTileRows * hs;  // [64][hs] each
+  LoraAdapter w = {nullptr, nullptr, 0, 0.0f};
+  bool bad = false;
+  if (t.adapter < a.count) {
+    w = a.adapters[t.adapter];
+    bad = w.rank < 0 || w.rank > a.max_rank || (w.rank > 0 && (!w.a || !w.b));
+  } else if (part == 0 && rank == 0) {
+    for (int i = threadIdx.x; i < rows; i += kThreads)
+      bad |= a.index[t.rows[i]] != -1;
+  }
+  if (bad) {
+    w.rank = 0;
+    if (part == 0 && rank == 0)
+      kc_raise(KC_ERR_BAD_ARGS);
+  }
+  const W *A = static_cast<const W *>(w.a), *B = static_cast<const W *>(w.b);
+  const int rank32 = (w.rank + 31) / 32 * 32;
+  const int rg = warp & 3, half = warp >> 2;  // this warp's 16 rows, and its half of the work along n or d
+  const int i0 = 16 * rg + g, i1 = i0 + 8;
+  const bool busy = 16 * rg < rows;
+
+  // A x: this CTA's slice of n in steps of 32, the two halves of the warps in turn; 64 rows of A at a time.
+  const int n_slice = ((a.n + ctas - 1) / ctas + 31) / 32 * 32;
+  const int n0 = min(rank * n_slice, a.n), n1 = min(n0 + n_slice, a.n);
+  const bool x_wide = aligned16(a.x) && a.ldx % 4 == 0, a_wide = aligned16(A) && a.n % 8 == 0;
+  for (int k0 = 0; k0 < w.rank; k0 += 64) {
+    float sum[8][4];
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        sum[c][i] = 0.0f;
+    if (busy) {
+      const float *x0 = a.x + (long long)t.rows[min(i0, rows - 1)] * a.ldx, *x1 = a.x + (long long)t.rows[min(i1, rows - 1)] * a.ldx;
+      for (int i = n0 + 32 * half; i < n1; i += 64) {
+        Raw8<float> x[2];
+        x[0].load(x0, i + 8 * q, n1, x_wide);
+        x[1].load(x1, i + 8 * q, n1, x_wide);
+        float v0[8], v1[8];
+#pragma unroll
+        for (int c0 = 0; c0 < 8; c0 += kFlight) {
+          Raw8<W> wr[kFlight];
+#pragma unroll
+          for (int c = 0; c < kFlight; c++)
+            if (k0 + 8 * (c0 + c) < w.rank)
+              wr[c].load(A + (long long)min(k0 + 8 * (c0 + c) + g, w.rank - 1) * a.n, i + 8 * q, n1, a_wide);
+          if (c0 == 0) {
+            x[0].get(v0);
+            x[1].get(v1);
+          }
+#pragma unroll
+          for (int c = 0; c < kFlight; c++)
+            if (k0 + 8 * (c0 + c) < w.rank) {
+              float wv[8];
+              wr[c].get(wv);
+              product32<kSplit>(sum[c0 + c], v0, v1, wv);
+            }
+        }
+      }
+    }
+    // The second half's sums, then the first's on top, into this CTA's partial vectors.
+    for (int turn = 1; turn >= 0; turn--) {
+      if (busy && half == turn)
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int k = k0 + 8 * c + 2 * q + (i & 1);
+            float *at = partial + (i < 2 ? i0 : i1) * hs + k;
+            if (k < rank32)
+              *at = k >= w.rank ? 0.0f : turn ? sum[c][i] : *at + sum[c][i];
+          }
+      __syncthreads();
+    }
+  }
+  // The cluster's sums: CTA c adds up its share of the rows from all CTAs in their order, then everyone fetches them.
+  cluster.sync();
+  for (int e = threadIdx.x; e < kTileRows * rank32; e += kThreads) {
+    const int i = e / rank32, k = e - i * rank32;
+    if (i % ctas == rank && i < rows) {
+      float s = 0.0f;
+      for (int c = 0; c < ctas; c++)
+        s += *cluster.map_shared_rank(&partial[i * hs + k], c);
+      h[i * hs + k] = s * w.scale;
+    }
+  }
+  cluster.sync();
+  for (int e = threadIdx.x; e < kTileRows * rank32; e += kThreads) {
+    const int i = e / rank32, k = e - i * rank32;
+    if (i < rows && i % ctas != rank)
+      h[i * hs + k] = *cluster.map_shared_rank(&h[i * hs + k], i % ctas);
+  }
+  cluster.sync();  // everything is fetched: a CTA may leave
+  if (!busy)
+    return;
+
+  // B h: this CTA's slice of d, 32 columns at a time, the two halves of the warps in turn.
+  const int d_all = parts * ctas, d_slice = ((a.d + d_all - 1) / d_all + 31) / 32 * 32;
+  const int d0 = min((part * ctas + rank) * d_slice, a.d), d1 = min(d0 + d_slice, a.d);
+  const bool b_wide = aligned16(B) && w.rank % 8 == 0;
+  const bool pairs = a.ldo % 2 == 0 && ((uintptr_t)a.out & 7) == 0 && (!a.base || (a.ldb % 2 == 0 && ((uintptr_t)a.base & 7) == 0));
+  const long long r0 = t.rows[min(i0, rows - 1)], r1 = t.rows[min(i1, rows - 1)];
+  for (int d = d0 + 32 * half; d < d1; d += 64) {
+    float sum[4][4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) {  // the base first: its reads are under way during the products
+      const int i = d + 8 * c + 2 * q;
+      float2 y0 = make_float2(0.0f, 0.0f), y1 = y0;
+      if (a.base) {
+        const float *b0 = a.base + r0 * a.ldb + i, *b1 = a.base + r1 * a.ldb + i;
+        if (pairs && i + 1 < d1) {
+          y0 = *reinterpret_cast<const float2 *>(b0), y1 = *reinterpret_cast<const float2 *>(b1);
+        } else {
+          if (i < d1)
+            y0.x = b0[0], y1.x = b1[0];
+          if (i + 1 < d1)
+            y0.y = b0[1], y1.y = b1[1];
+        }
+      }
+      sum[c][0] = y0.x, sum[c][1] = y0.y, sum[c][2] = y1.x, sum[c][3] = y1.y;
+    }
+    float prod[4][4];
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        prod[c][i] = 0.0f;
+    for (int k = 0; k < rank32; k += 32) {
+      Raw8<W> wr[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        wr[c].load(B + (long long)min(d + 8 * c + g, a.d - 1) * w.rank, k + 8 * q, w.rank, b_wide);
+      float v0[8], v1[8];
+      load8(h + i0 * hs + k + 8 * q, v0);
+      load8(h + i1 * hs + k + 8 * q, v1);
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        float wv[8];
+        wr[c].get(wv);
+        product32<kSplit>(prod[c], v0, v1, wv);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const int i = d + 8 * c + 2 * q;
+      float *o0 = a.out + r0 * a.ldo + i, *o1 = a.out + r1 * a.ldo + i;
+      const float y[4] = {sum[c][0] + prod[c][0], sum[c][1] + prod[c][1], sum[c][2] + prod[c][2], sum[c][3] + prod[c][3]};
+      if (pairs && i + 1 < d1) {
+        if (i0 < rows)
+          *reinterpret_cast<float2 *>(o0) = make_float2(y[0], y[1]);
+        if (i1 < rows)
+          *reinterpret_cast<float2 *>(o1) = make_float2(y[2], y[3]);
+      } else {
+        if (i < d1 && i0 < rows)
+          o0[0] = y[0];
+        if (i < d1 && i1 < rows)
+          o1[0] = y[2];
+        if (i + 1 < d1 && i0 < rows)
+          o0[1] = y[1];
+        if (i + 1 < d1 && i1 < rows)
+          o1[1] = y[3];
+      }
+    }
+  }
+}
+
+template <typename W>
+cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned clusters, int ctas, int parts, size_t smem) {
   cudaLaunchConfig_t cfg = {};
-  const int ctas = 8;
-  cfg.gridDim = dim3((unsigned)a.rows * ctas);
+  cfg.gridDim = dim3(clusters * ctas);
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = kc_stream();
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -150,7 +487,31 @@ cudaError_t launch(const LoraArgs &a) {
   attr[1].val.clusterDim.x = ctas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, lora_row_kernel<W>, a);
+  return cudaLaunchKernelEx(&cfg, kernel, a, parts);
+}
+
+template <typename W>
+cudaError_t run(const LoraArgs &a) {
+  constexpr int kCtas = 8;
+  if (a.rows < 24 || a.count >= kMaxBins)
+    return launch<W>(lora_row_kernel<W>, a, (unsigned)a.rows, kCtas, 1, 0);
+  const size_t smem = 2 * sizeof(float) * kTileRows * h_stride(a.max_rank);
+  cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(lora_tile_kernel<W>),
+                                (int)(2 * sizeof(float) * kTileRows * h_stride(kMaxRank)));
+  for (int r = 0; r < a.rows && e == cudaSuccess; r += kMaxTileRows) {
+    LoraArgs b = a;
+    b.rows = a.rows - r < kMaxTileRows ? a.rows - r : kMaxTileRows;
+    b.x += (long long)r * a.ldx, b.out += (long long)r * a.ldo, b.index += r;
+    if (b.base)
+      b.base += (long long)r * a.ldb;
+    // At most this many tiles: the full ones, and one more for each adapter and the rows without one.
+    const int some = b.count + 1 < b.rows ? b.count + 1 : b.rows, tiles = (b.rows - some) / kTileRows + some;
+    const int few = kc_device_sms() / (kCtas * tiles), parts = few < 1 ? 1 : few > 4 ? 4 : few;
+    e = launch<W>(lora_tile_kernel<W>, b, (unsigned)(tiles * parts), kCtas, parts, smem);
+    if (e == cudaSuccess && r + kMaxTileRows < a.rows)
+      kc_count_launch();
+  }
+  return e;
 }
 
 }  // namespace
@@ -178,7 +539,7 @@ void k_lora_rows(float *out, size_t ldo, const float *base, size_t ldb, const fl
   }
   const LoraArgs a = {out, base, x, (long long)ldo, (long long)ldb, (long long)ldx, index, adapters, count, max_rank,
                       n, d, rows};
-  const cudaError_t e = type == K_F32 ? launch<float>(a) : type == K_BF16 ? launch<__nv_bfloat16>(a) : launch<__half>(a);
+  const cudaError_t e = type == K_F32 ? run<float>(a) : type == K_BF16 ? run<__nv_bfloat16>(a) : run<__half>(a);
   if (e == cudaSuccess)
     kc_count_launch();
   else

@@ -72,8 +72,31 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// exp of a non-positive argument (or 0).
-__device__ __forceinline__ double weight(float l, float m, double inv_t) { return exp(((double)l - (double)m) * inv_t); }
+// exp((l - m) / T) for l <= m, with k32 = 32 / (T ln 2), to about 2^-43 of itself: 2^(a / 32) with a = (l - m) k32 =
+// k + r, |r| <= 1/2, as a table value 2^((k mod 32) / 32), the exponent k / 32, and a polynomial for 2^(r / 32) (Tang's
+// table-driven scheme; the polynomial is the Taylor sum of degree 5 with its last term economized onto the lower ones by
+// Chebyshev's T5, 8e-14 off at most). Ten 64-bit operations: the sums kernel is as much bound by them (64 a clock and
+// SM) as by its reads; the library's exp made it twice as long.
+struct Weights {
+  const unsigned long long *table;  // kExpfTable in shared memory
+  double k32;
+  __device__ __forceinline__ double operator()(float l, float m) const {
+    constexpr double c = 0.021660849392498290, a2 = c * c / 4;  // ln 2 / 32; the square of |r| c's largest value
+    constexpr double c4 = c * c * c * c / 24, c3 = c * c * c * (1.0 / 6 + a2 * 5 / 4 / 120), c2 = c * c / 2,
+                     c1 = c * (1 - a2 * a2 * 5 / 16 / 120), shift = 0x1.8p+52;
+    const double d = (double)l - (double)m;
+    const double t = __fma_rn(d, k32, shift), kd = t - shift, r = __fma_rn(d, k32, -kd);
+    const unsigned long long k = (unsigned long long)__double_as_longlong(t);
+    const double s = __longlong_as_double((long long)(table[k % 32] + (k << 47)));
+    const double y = __fma_rn(__fma_rn(__fma_rn(__fma_rn(c4, r, c3), r, c2), r, c1), r, 1.0);
+    return kd < -32000.0 ? 0.0 : y * s;  // below 2^-1000; -infinity
+  }
+};
+__device__ __forceinline__ double k32_of(float t) { return 46.166241308446829 / (double)t; }  // 32 / ln 2
+__device__ __forceinline__ void load_table(unsigned long long *table) {
+  if (threadIdx.x < 32)
+    table[threadIdx.x] = kExpfTable[threadIdx.x];
+}
 
 __device__ __forceinline__ int count_of(const VerifyArgs &a, int b) { return a.counts ? a.counts[b] : a.rows; }
 
@@ -96,6 +119,8 @@ __device__ __forceinline__ bool slot_row(const VerifyArgs &a, int b, int slot, c
 __global__ void __launch_bounds__(kSumThreads) verify_sums_kernel(const VerifyArgs a) {
   __shared__ unsigned long long key_s[kSumThreads / 32];
   __shared__ double sum_s[kSumThreads / 32];
+  __shared__ unsigned long long table[32];
+  load_table(table);
   pdl_wait();
   pdl_launch_dependents();
   const int chunk = blockIdx.x % a.chunks, id = blockIdx.x / a.chunks;
@@ -128,10 +153,10 @@ __global__ void __launch_bounds__(kSumThreads) verify_sums_kernel(const VerifyAr
   double sum = 0.0;
   if (t > 0.0f && key_good(key)) {
     const float m = key_value(key);
-    const double inv_t = 1.0 / (double)t;
+    const Weights weight{table, k32_of(t)};
 #pragma unroll
     for (int i = 0; i < 16; i++)
-      sum += weight(v[i], m, inv_t);
+      sum += weight(v[i], m);
   }
   sum = warp_sum(sum);
   if (lane == 0)
@@ -149,47 +174,115 @@ __global__ void __launch_bounds__(kSumThreads) verify_sums_kernel(const VerifyAr
 // The weight of token i when the next token is drawn: p_a(i), less q_a(i) at a refused draft (the drafted token alone
 // has q = 1 where there are no draft logits).
 struct Residual {
+  Weights weight;
   const float *p, *q;
   float pm, qm;
-  double inv_t, p_norm, q_norm;
+  double p_norm, q_norm;
   int without;
   __device__ __forceinline__ double operator()(int i) const {
     // Both products are rounded (no fused multiply-add): where draft and target are the same row nothing is left.
-    double w = __dmul_rn(weight(p[i], pm, inv_t), p_norm);
+    double w = __dmul_rn(weight(p[i], pm), p_norm);
     if (q)
-      w -= __dmul_rn(weight(q[i], qm, inv_t), q_norm);
+      w -= __dmul_rn(weight(q[i], qm), q_norm);
     return i == without ? 0.0 : fmax(w, 0.0);
   }
 };
 
-// A cluster per request: every CTA decides which drafts are accepted, then sums its slice of the vocabulary's weights;
-// the CTA whose slice holds the place of u inverts it.
+// The whole CTA: the first token of [s0, s1) whose running sum, `run` before s0, passes `place`; the last one with
+// weight where rounding leaves none. Every thread a run of neighbouring tokens.
+struct Invert {
+  double warp_sums[kPickWarps];
+  int first, last;
+};
+__device__ int invert(const Residual &w, Invert *t, int s0, int s1, double run, double place) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (s1 - s0 + kPickThreads - 1) / kPickThreads;
+  const int i0 = min(s0 + (int)threadIdx.x * per, s1), i1 = min(i0 + per, s1);
+  double mine = 0.0;
+#pragma unroll 4
+  for (int i = i0; i < i1; i++)
+    mine += w(i);
+  double upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double other = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o)
+      upto += other;
+  }
+  if (lane == 31)
+    t->warp_sums[warp] = upto;
+  if (threadIdx.x == 0)
+    t->first = kPickThreads, t->last = -1;
+  __syncthreads();
+  for (int i = 0; i < warp; i++)
+    run += t->warp_sums[i];
+  upto += run;
+  if (mine > 0.0) {
+    if (upto > place)
+      atomicMin(&t->first, (int)threadIdx.x);
+    atomicMax(&t->last, (int)threadIdx.x);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x != (t->first < kPickThreads ? t->first : t->last))
+    return -1;
+  run = upto - mine;
+  int at = -1;
+  for (int i = i0; i < i1; i++) {
+    const double x = w(i);
+    if (x > 0.0) {
+      at = i;
+      run += x;
+      if (run > place)
+        break;
+    }
+  }
+  return at;
+}
+
+// A cluster per request: every CTA decides which drafts are accepted. Where the weights are p alone the chunks' sums are
+// known, and one CTA inverts one chunk; else every CTA sums its slice of the vocabulary's weights, and the CTA whose
+// slice holds the place of u inverts the part of it that a warp summed.
 __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyArgs a) {
-  __shared__ unsigned long long key_s[kMaxSlots];
+  __shared__ unsigned long long key_s[kMaxSlots], table[32];
   __shared__ double sum_s[kMaxSlots], warp_sums[kPickWarps], slices[kPickCtas];
-  __shared__ int stop_s;
+  __shared__ Invert inv;
+  __shared__ int stop_s, found_s;
   cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();  // every CTA has started before any writes into another's shared memory
+  load_table(table);
   pdl_wait();
   pdl_launch_dependents();
   const int b = blockIdx.x / kPickCtas, rank = blockIdx.x % kPickCtas;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count = count_of(a, b);
-  if (count < 0)
-    return;  // the whole cluster: a slot of the batch that is not in use
   const float t = a.temperature[b];
   const bool greedy = t == 0.0f;
-  int *tokens = a.tokens + (long long)b * (a.rows + 1);
-  const bool valid = count <= a.rows && t >= 0.0f && t < __int_as_float(0x7f800000);
-  const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
+  const bool valid = count >= 0 && count <= a.rows && t >= 0.0f && t < __int_as_float(0x7f800000);
+  // This thread's draft, and its logits.
+  const int j = threadIdx.x;
+  const bool drafts = valid && j < count;
+  const int x = drafts ? a.drafted[(long long)b * a.rows + j] : -1;
+  const bool x_good = x >= 0 && x < a.vocab;
+  float px = 0.0f, qx = 0.0f, u = 0.0f;
+  if (drafts && x_good && !greedy) {
+    px = a.target[((long long)b * (a.rows + 1) + j) * a.ldt + x];
+    qx = a.draft ? a.draft[((long long)b * a.rows + j) * a.ldd + x] : 0.0f;
+    u = a.uniforms[(long long)b * (a.rows + 1) + j];
+  }
+  const float u_last = a.uniforms[(long long)b * (a.rows + 1) + a.rows];
   if (threadIdx.x == 0)
     stop_s = valid ? count : 0;
+  cluster.sync();  // every CTA has started before any writes into another's shared memory; the table is there
+  if (count < 0)
+    return;  // the whole cluster: a slot of the batch that is not in use
+  const Weights weight{table, greedy ? 0.0 : k32_of(t)};
+  int *tokens = a.tokens + (long long)b * (a.rows + 1);
+  const long long base = (long long)b * (2 * a.rows + 1) * a.chunks;
   if (valid)
     for (int slot = warp; slot < 2 * a.rows + 1; slot += kPickWarps) {
       const float *row;
       if (!slot_row(a, b, slot, &row))
         continue;
-      const long long at = ((long long)b * (2 * a.rows + 1) + slot) * a.chunks;
+      const long long at = base + (long long)slot * a.chunks;
       unsigned long long key = 0;
       for (int c = lane; c < a.chunks; c += 32)
         key = max64(key, a.keys[at + c]);
@@ -199,7 +292,7 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
         for (int c = lane; c < a.chunks; c += 32) {
           const unsigned long long k = a.keys[at + c];
           if (key_good(k))
-            sum += a.sums[at + c] * weight(key_value(k), key_value(key), inv_t);
+            sum += a.sums[at + c] * weight(key_value(k), key_value(key));
         }
       sum = warp_sum(sum);
       if (lane == 0)
@@ -207,42 +300,38 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
     }
   __syncthreads();
   // A draft is refused, or its rows have no distribution: the first such place ends the run.
-  if (valid)
-    for (int j = threadIdx.x; j < count; j += kPickThreads) {
-      const int x = a.drafted[(long long)b * a.rows + j], dj = a.rows + 1 + j;
-      const bool rows_good = key_good(key_s[j]) && (greedy || !a.draft || key_good(key_s[dj]));
-      bool good = false;
-      if (rows_good && x >= 0 && x < a.vocab) {
-        if (greedy) {
-          good = key_index(key_s[j]) == x;
-        } else {
-          const float *p = a.target + ((long long)b * (a.rows + 1) + j) * a.ldt;
-          const double px = weight(p[x], key_value(key_s[j]), inv_t) / sum_s[j];
-          double qx = 1.0;
-          if (a.draft)
-            qx = weight(a.draft[((long long)b * a.rows + j) * a.ldd + x], key_value(key_s[dj]), inv_t) / sum_s[dj];
-          good = (double)a.uniforms[(long long)b * (a.rows + 1) + j] * qx < px;
-        }
+  if (drafts) {
+    const int dj = a.rows + 1 + j;
+    bool good = false;
+    if (x_good && key_good(key_s[j]) && (greedy || !a.draft || key_good(key_s[dj]))) {
+      if (greedy) {
+        good = key_index(key_s[j]) == x;
+      } else {
+        const double p = weight(px, key_value(key_s[j])) / sum_s[j];
+        const double q = a.draft ? weight(qx, key_value(key_s[dj])) / sum_s[dj] : 1.0;
+        good = (double)u * q < p;
       }
-      if (!good)
-        atomicMin(&stop_s, j);
     }
+    if (!good)
+      atomicMin(&stop_s, j);
+  }
   __syncthreads();
   const int stop = stop_s;
   const bool refused = stop < count;
-  const int x = valid && refused ? a.drafted[(long long)b * a.rows + stop] : -1;
+  const int at_stop = valid && refused ? a.drafted[(long long)b * a.rows + stop] : -1;
   // No distribution at the place where the run ends (or arguments that mean nothing): no answer.
   unsigned error = 0;
-  if (!valid || (refused && (x < 0 || x >= a.vocab)))
+  if (!valid || (refused && (at_stop < 0 || at_stop >= a.vocab)))
     error = KC_ERR_BAD_ARGS;
   else if (!key_good(key_s[stop]) || (refused && !greedy && a.draft && !key_good(key_s[a.rows + 1 + stop])))
     error = KC_ERR_NONFINITE;
   if (rank == 0) {
-    for (int j = threadIdx.x; j <= a.rows; j += kPickThreads)
+    if (j <= a.rows) {
       if (error || j > stop)
         tokens[j] = -1;
       else if (j < stop)
-        tokens[j] = a.drafted[(long long)b * a.rows + j];
+        tokens[j] = x;
+    }
     if (threadIdx.x == 0) {
       a.accepted[b] = error ? -1 : stop;
       if (error)
@@ -255,83 +344,128 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
     return;  // the whole cluster
 
   Residual w;
+  w.weight = weight;
   w.p = a.target + ((long long)b * (a.rows + 1) + stop) * a.ldt;
-  w.pm = key_value(key_s[stop]), w.p_norm = 1.0 / sum_s[stop], w.inv_t = inv_t;
+  w.pm = key_value(key_s[stop]), w.p_norm = 1.0 / sum_s[stop];
   w.q = refused && a.draft ? a.draft + ((long long)b * a.rows + stop) * a.ldd : nullptr;
   w.qm = w.q ? key_value(key_s[a.rows + 1 + stop]) : 0.0f, w.q_norm = w.q ? 1.0 / sum_s[a.rows + 1 + stop] : 0.0;
-  w.without = refused && !a.draft ? x : -1;
-  // Warp segments of equal length: segment s of kPickCtas * kPickWarps.
-  const int segment = (a.vocab + kPickCtas * kPickWarps - 1) / (kPickCtas * kPickWarps);
-  const int s0 = min((rank * kPickWarps + warp) * segment, a.vocab), s1 = min(s0 + segment, a.vocab);
-  double sum = 0.0;
-  for (int i = s0 + lane; i < s1; i += 32)
-    sum += w(i);
-  sum = warp_sum(sum);
-  if (lane == 0)
-    warp_sums[warp] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double slice = 0.0;
-    for (int i = 0; i < kPickWarps; i++)
-      slice += warp_sums[i];
-    for (int r = 0; r < kPickCtas; r++)
-      *cluster.map_shared_rank(&slices[rank], r) = slice;
-  }
-  cluster.sync();
-  double total = 0.0, before = 0.0;
-  for (int r = 0; r < kPickCtas; r++) {
-    if (r == rank)
-      before = total;
-    total += slices[r];
+  w.without = refused && !a.draft ? at_stop : -1;
+  int s0 = 0, s1 = 0;
+  double before = 0.0, total = 0.0, place = 0.0;
+  auto place_in = [&]() {
+    place = (double)u_last * total;
+    if (!(place < total))
+      place = total * (1.0 - 0x1p-52);
+    place = fmax(place, 0.0);
+  };
+  if (!w.q) {
+    if (rank)
+      return;
+    // p alone: the chunks' sums; the refused token's chunk is summed again without it (a difference would leave rounding
+    // where nothing is left).
+    const long long at = base + (long long)stop * a.chunks;
+    const int again = w.without >= 0 ? w.without / kChunk : -1;
+    if (again >= 0) {
+      double sum = 0.0;
+      for (int i = again * kChunk + threadIdx.x; i < min((again + 1) * kChunk, a.vocab); i += kPickThreads)
+        sum += w(i);
+      sum = warp_sum(sum);
+      if (lane == 0)
+        warp_sums[warp] = sum;
+      __syncthreads();
+    }
+    auto chunk = [&](int c) {
+      if (c == again) {
+        double sum = 0.0;
+        for (int i = 0; i < kPickWarps; i++)
+          sum += warp_sums[i];
+        return sum;
+      }
+      const unsigned long long k = a.keys[at + c];
+      return key_good(k) ? a.sums[at + c] * weight(key_value(k), w.pm) * w.p_norm : 0.0;
+    };
+    if (warp == 0) {
+      double upto = 0.0;
+      for (int c0 = 0; c0 < a.chunks; c0 += 32)
+        upto += warp_sum(c0 + lane < a.chunks ? chunk(c0 + lane) : 0.0);
+      total = upto;
+      place_in();
+      // The chunk whose running sum passes the place; behind the last one with weight, that one.
+      int found = -1;
+      double run = 0.0, at_found = 0.0;
+      for (int c0 = 0; c0 < a.chunks; c0 += 32) {
+        const double mine = c0 + lane < a.chunks ? chunk(c0 + lane) : 0.0;
+        double sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double other = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o)
+            sum += other;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, mine > 0.0 && run + sum > place);
+        const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
+        if (past || some) {
+          const int l = past ? __ffs(past) - 1 : 31 - __clz(some);
+          found = c0 + l;
+          at_found = run + __shfl_sync(0xffffffffu, sum - mine, l);
+        }
+        if (past)
+          break;
+        run += __shfl_sync(0xffffffffu, sum, 31);
+      }
+      if (lane == 0)
+        slices[0] = total, slices[1] = place, slices[2] = at_found, found_s = found;
+    }
+    __syncthreads();
+    total = slices[0], place = slices[1], before = slices[2];
+    s0 = max(found_s, 0) * kChunk, s1 = min(s0 + kChunk, a.vocab);
+  } else {
+    // Warp segments of equal length: segment s of kPickCtas * kPickWarps.
+    const int segment = (a.vocab + kPickCtas * kPickWarps - 1) / (kPickCtas * kPickWarps);
+    const int w0 = min((rank * kPickWarps + warp) * segment, a.vocab), w1 = min(w0 + segment, a.vocab);
+    double sum = 0.0;
+#pragma unroll 4
+    for (int i = w0 + lane; i < w1; i += 32)
+      sum += w(i);
+    sum = warp_sum(sum);
+    if (lane == 0)
+      warp_sums[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x < kPickCtas) {
+      double slice = 0.0;
+      for (int i = 0; i < kPickWarps; i++)
+        slice += warp_sums[i];
+      *cluster.map_shared_rank(&slices[rank], threadIdx.x) = slice;
+    }
+    cluster.sync();
+    for (int r = 0; r < kPickCtas; r++) {
+      if (r == rank)
+        before = total;
+      total += slices[r];
+    }
+    place_in();
+    if (total > 0.0 && (place < before || place >= before + slices[rank]))  // the slices tile [0, total): one CTA goes on
+      return;
+    // The warp whose segment the place falls into; behind the last one with weight, that one.
+    int seg = -1;
+    double run = before;
+    for (int i = 0; i < kPickWarps; i++) {
+      if (warp_sums[i] > 0.0 && (seg < 0 || place >= run)) {
+        seg = i;
+        before = run;
+      }
+      run += warp_sums[i];
+    }
+    s0 = min((rank * kPickWarps + seg) * segment, a.vocab), s1 = min(s0 + segment, a.vocab);
   }
   if (!(total > 0.0)) {  // nothing of the target is left but rounding: its first maximum
     if (rank == 0 && threadIdx.x == 0)
       tokens[stop] = key_index(key_s[stop]);
     return;
   }
-  double place = (double)a.uniforms[(long long)b * (a.rows + 1) + a.rows] * total;
-  if (!(place < total))
-    place = total * (1.0 - 0x1p-52);
-  place = fmax(place, 0.0);
-  if (place < before || place >= before + slices[rank])  // the slices tile [0, total): one CTA goes on
-    return;
-  // The warp whose segment the place falls into; behind the last one with weight, that one.
-  int seg = -1;
-  double seg_before = before;
-  for (int i = 0; i < kPickWarps; i++) {
-    if (warp_sums[i] > 0.0 && (seg < 0 || place >= before)) {
-      seg = i;
-      seg_before = before;
-    }
-    before += warp_sums[i];
-  }
-  if (warp != seg)
-    return;
-  int last = -1;
-  double run = seg_before;
-  for (int i0 = s0; i0 < s1; i0 += 32) {
-    const int i = i0 + lane;
-    const double mine = i < s1 ? w(i) : 0.0;
-    double upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double other = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o)
-        upto += other;
-    }
-    upto += run;
-    const unsigned past = __ballot_sync(0xffffffffu, mine > 0.0 && upto > place);
-    if (past) {
-      last = i0 + __ffs(past) - 1;
-      break;
-    }
-    const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
-    if (some)
-      last = i0 + 31 - __clz(some);
-    run = __shfl_sync(0xffffffffu, upto, 31);
-  }
-  if (lane == 0)
-    tokens[stop] = last;
+  const int token = invert(w, &inv, s0, s1, before, place);
+  if (token >= 0)
+    tokens[stop] = token;
 }
 
 size_t verify_chunks(int vocab) { return ((size_t)vocab + kChunk - 1) / kChunk; }

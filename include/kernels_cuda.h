@@ -332,7 +332,7 @@ void k_lora_rows(float *out, size_t ldo, const float *base, size_t ldb, const fl
  * of drafted [batch][rows]; row j of target [batch][rows + 1] (logits, row stride ldt, as engine_forward_batch makes
  * them) is the target model's after j drafts, row j of draft [batch][rows] (stride ldd) the logits that draft j was
  * drawn from, or draft is NULL when the drafts came from no distribution (a lookup in the prompt). p_j and q_j are
- * their softmax at temperature[b] (q_j one at the drafted token without logits). Draft j is accepted when all before
+ * their softmax at temperature[b], 0 .. 1e30 (q_j one at the drafted token without logits). Draft j is accepted when all before
  * it are and u_j q_j(x_j) < p_j(x_j), with the given random numbers u = uniforms[b] of uniforms [batch][rows + 1], in
  * [0, 1). Behind the accepted drafts one token is drawn with u_rows: from (p - q)+ at the refused draft, else from p
  * of row counts[b]; it is the first token whose running sum in vocabulary order exceeds u_rows times the total (where

@@ -7,6 +7,7 @@
 // move the choice for about one u in a hundred.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "../../include/kernels_cuda.h"
@@ -24,6 +25,7 @@ constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kPickCtas = 8;  // a cluster per request
 constexpr int kMaxRows = 64;
 constexpr int kMaxSlots = 2 * kMaxRows + 1;
+constexpr float kMaxTemperature = 1e30f;  // 700 T is a number
 
 struct VerifyArgs {
   int *accepted, *tokens;
@@ -36,16 +38,13 @@ struct VerifyArgs {
   unsigned long long *keys;  // the same: order-preserving maximum and its first index
 };
 
-// 64-bit key whose unsigned maximum is the first maximum. NaN and +infinity have no place in a distribution: they get
-// the largest key.
-__device__ __forceinline__ unsigned long long row_key(float v, int i) {
-  unsigned b = __float_as_uint(v);
-  if (!(v < __int_as_float(0x7f800000)))
-    return ~0ull;
-  if (v == 0.0f)
-    b = 0;  // the two zeros are one value: the first of them wins
+// 64-bit key whose unsigned maximum is the first maximum; kBad, the largest, where a value is NaN or +infinity, which
+// have no place in a distribution.
+constexpr unsigned long long kBad = ~0ull;
+__device__ __forceinline__ unsigned long long row_key(float v, unsigned i) {
+  unsigned b = v == 0.0f ? 0u : __float_as_uint(v);  // the two zeros are one value
   b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  return ((unsigned long long)b << 32) | (0xFFFFFFFFu - (unsigned)i);
+  return ((unsigned long long)b << 32) | (0xFFFFFFFFu - i);
 }
 __device__ __forceinline__ float key_value(unsigned long long k) {
   unsigned b = (unsigned)(k >> 32);
@@ -55,7 +54,7 @@ __device__ __forceinline__ float key_value(unsigned long long k) {
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)(0xFFFFFFFFu - (unsigned)k); }
 // A maximum that gives a distribution: above -infinity, and no NaN or +infinity in the row.
 __device__ __forceinline__ bool key_good(unsigned long long k) {
-  return k != ~0ull && key_value(k) > __int_as_float(0xff800000);
+  return k != kBad && key_value(k) > __int_as_float(0xff800000);
 }
 __device__ __forceinline__ unsigned long long max64(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 
@@ -72,30 +71,34 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// exp((l - m) / T) for l <= m, with k32 = 32 / (T ln 2), to about 2^-43 of itself: 2^(a / 32) with a = (l - m) k32 =
-// k + r, |r| <= 1/2, as a table value 2^((k mod 32) / 32), the exponent k / 32, and a polynomial for 2^(r / 32) (Tang's
-// table-driven scheme; the polynomial is the Taylor sum of degree 5 with its last term economized onto the lower ones by
-// Chebyshev's T5, 8e-14 off at most). Ten 64-bit operations: the sums kernel is as much bound by them (64 a clock and
-// SM) as by its reads; the library's exp made it twice as long.
+// exp((l - m) / T) for l <= m, to about 2^-43 of itself: 2^(a / 32) with a = (l - m) 32 / (T ln 2) = k + r, |r| <= 1/2,
+// as a table value 2^((k mod 32) / 32), the exponent k / 32, and a polynomial for 2^(r / 32) (Tang's table-driven scheme;
+// the polynomial is the Taylor sum of degree 5 with its last term economized onto the lower ones by Chebyshev's T5,
+// 8e-14 off at most). 0 below `floor`, some 700 T below m. Ten 64-bit operations.
 struct Weights {
-  const unsigned long long *table;  // kExpfTable in shared memory
-  double k32;
-  __device__ __forceinline__ double operator()(float l, float m) const {
+  const uint2 *table;  // kExpfTable in shared memory
+  double k32;          // 32 / (T ln 2)
+  __device__ __forceinline__ double operator()(float l, float m, float floor) const {
     constexpr double c = 0.021660849392498290, a2 = c * c / 4;  // ln 2 / 32; the square of |r| c's largest value
     constexpr double c4 = c * c * c * c / 24, c3 = c * c * c * (1.0 / 6 + a2 * 5 / 4 / 120), c2 = c * c / 2,
                      c1 = c * (1 - a2 * a2 * 5 / 16 / 120), shift = 0x1.8p+52;
-    const double d = (double)l - (double)m;
+    const double d = (double)fmaxf(l, floor) - (double)m;
     const double t = __fma_rn(d, k32, shift), kd = t - shift, r = __fma_rn(d, k32, -kd);
-    const unsigned long long k = (unsigned long long)__double_as_longlong(t);
-    const double s = __longlong_as_double((long long)(table[k % 32] + (k << 47)));
+    const int k = __double2loint(t);
+    const uint2 e = table[k & 31];
+    const double s = __hiloint2double((int)e.y + (k << 15), (int)e.x);
     const double y = __fma_rn(__fma_rn(__fma_rn(__fma_rn(c4, r, c3), r, c2), r, c1), r, 1.0);
-    return kd < -32000.0 ? 0.0 : y * s;  // below 2^-1000; -infinity
+    return l < floor ? 0.0 : y * s;
   }
 };
+// The floor: (l - m) / T is in [-760, 0] above it whatever the roundings, and finite.
+__device__ __forceinline__ float floor_of(float m, float t) { return fmaxf(fmaf(-700.0f, t, m), -FLT_MAX); }
 __device__ __forceinline__ double k32_of(float t) { return 46.166241308446829 / (double)t; }  // 32 / ln 2
-__device__ __forceinline__ void load_table(unsigned long long *table) {
-  if (threadIdx.x < 32)
-    table[threadIdx.x] = kExpfTable[threadIdx.x];
+__device__ __forceinline__ void load_table(uint2 *table) {
+  if (threadIdx.x < 32) {
+    const unsigned long long e = kExpfTable[threadIdx.x];
+    table[threadIdx.x] = make_uint2((unsigned)e, (unsigned)(e >> 32));
+  }
 }
 
 __device__ __forceinline__ int count_of(const VerifyArgs &a, int b) { return a.counts ? a.counts[b] : a.rows; }
@@ -115,59 +118,76 @@ __device__ __forceinline__ bool slot_row(const VerifyArgs &a, int b, int slot, c
   return a.draft && j < count && a.temperature[b] != 0.0f;
 }
 
-// One chunk of one row: its first maximum, and the sum of exp((l - max) / T) over the chunk (T > 0).
-__global__ void __launch_bounds__(kSumThreads) verify_sums_kernel(const VerifyArgs a) {
-  __shared__ unsigned long long key_s[kSumThreads / 32];
+// One chunk of one row: its maximum and the sum of exp((l - max) / T) over the chunk, or (T = 0) its first maximum.
+__global__ void __launch_bounds__(kSumThreads, 4) verify_sums_kernel(const VerifyArgs a) {
+  __shared__ float max_s[kSumThreads / 32];
   __shared__ double sum_s[kSumThreads / 32];
-  __shared__ unsigned long long table[32];
+  __shared__ unsigned first_s[kSumThreads / 32];
+  __shared__ uint2 table[32];
   load_table(table);
   pdl_wait();
   pdl_launch_dependents();
   const int chunk = blockIdx.x % a.chunks, id = blockIdx.x / a.chunks;
   const int b = id / (2 * a.rows + 1), slot = id - b * (2 * a.rows + 1);
+  const float t = a.temperature[b];
   const float *row;
   if (!slot_row(a, b, slot, &row))
     return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = chunk * kChunk;
-  float v[16];
-  unsigned long long key = 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = chunk * kChunk + threadIdx.x;
+  float v[16], m = __int_as_float(0xff800000);
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 16; i++)
+    v[i] = first + i * kSumThreads < a.vocab ? row[first + i * kSumThreads] : __int_as_float(0xff800000);
 #pragma unroll
   for (int i = 0; i < 16; i++) {
-    const int e = first + i * kSumThreads + threadIdx.x;
-    v[i] = e < a.vocab ? row[e] : __int_as_float(0xff800000);
+    m = fmaxf(m, v[i]);
+    bad |= !(v[i] < __int_as_float(0x7f800000));
   }
+  if (bad)
+    m = __int_as_float(0x7f800000);
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
-    const int e = first + i * kSumThreads + threadIdx.x;
-    if (e < a.vocab)
-      key = max64(key, row_key(v[i], e));
-  }
-  key = warp_max(key);
+  for (int o = 16; o; o >>= 1)
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0)
-    key_s[warp] = key;
+    max_s[warp] = m;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kSumThreads / 32; w++)
-    key = max64(key, key_s[w]);
-  const float t = a.temperature[b];
+    m = fmaxf(m, max_s[w]);
+  const bool good = fabsf(m) < __int_as_float(0x7f800000);
   double sum = 0.0;
-  if (t > 0.0f && key_good(key)) {
-    const float m = key_value(key);
+  unsigned at = 0;
+  if (t > 0.0f && good) {
     const Weights weight{table, k32_of(t)};
+    const float floor = floor_of(m, t);
 #pragma unroll
     for (int i = 0; i < 16; i++)
-      sum += weight(v[i], m);
+      sum += weight(v[i], m, floor);
+    sum = warp_sum(sum);
+    if (lane == 0)
+      sum_s[warp] = sum;
+  } else {
+    at = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 15; i >= 0; i--)
+      if (v[i] == m && first + i * kSumThreads < a.vocab)
+        at = first + i * kSumThreads;
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0)
+      first_s[warp] = at;
   }
-  sum = warp_sum(sum);
-  if (lane == 0)
-    sum_s[warp] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     sum = 0.0;
+    at = 0xFFFFFFFFu;
     for (int w = 0; w < kSumThreads / 32; w++)
-      sum += sum_s[w];
+      if (t > 0.0f && good)
+        sum += sum_s[w];
+      else
+        at = min(at, first_s[w]);
     a.sums[(long long)id * a.chunks + chunk] = sum;
-    a.keys[(long long)id * a.chunks + chunk] = key;
+    a.keys[(long long)id * a.chunks + chunk] = m == __int_as_float(0x7f800000) ? kBad : row_key(m, at);
   }
 }
 
@@ -176,14 +196,14 @@ __global__ void __launch_bounds__(kSumThreads) verify_sums_kernel(const VerifyAr
 struct Residual {
   Weights weight;
   const float *p, *q;
-  float pm, qm;
+  float pm, qm, p_floor, q_floor;
   double p_norm, q_norm;
   int without;
   __device__ __forceinline__ double operator()(int i) const {
     // Both products are rounded (no fused multiply-add): where draft and target are the same row nothing is left.
-    double w = __dmul_rn(weight(p[i], pm), p_norm);
+    double w = __dmul_rn(weight(p[i], pm, p_floor), p_norm);
     if (q)
-      w -= __dmul_rn(weight(q[i], qm), q_norm);
+      w -= __dmul_rn(weight(q[i], qm, q_floor), q_norm);
     return i == without ? 0.0 : fmax(w, 0.0);
   }
 };
@@ -242,8 +262,9 @@ __device__ int invert(const Residual &w, Invert *t, int s0, int s1, double run, 
 // A cluster per request: every CTA decides which drafts are accepted. Where the weights are p alone the chunks' sums are
 // known, and one CTA inverts one chunk; else every CTA sums its slice of the vocabulary's weights, and the CTA whose
 // slice holds the place of u inverts the part of it that a warp summed.
-__global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyArgs a) {
-  __shared__ unsigned long long key_s[kMaxSlots], table[32];
+__global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const VerifyArgs a) {
+  __shared__ unsigned long long key_s[kMaxSlots];
+  __shared__ uint2 table[32];
   __shared__ double sum_s[kMaxSlots], warp_sums[kPickWarps], slices[kPickCtas];
   __shared__ Invert inv;
   __shared__ int stop_s, found_s;
@@ -256,7 +277,7 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
   const int count = count_of(a, b);
   const float t = a.temperature[b];
   const bool greedy = t == 0.0f;
-  const bool valid = count >= 0 && count <= a.rows && t >= 0.0f && t < __int_as_float(0x7f800000);
+  const bool valid = count >= 0 && count <= a.rows && t >= 0.0f && t <= kMaxTemperature;
   // This thread's draft, and its logits.
   const int j = threadIdx.x;
   const bool drafts = valid && j < count;
@@ -292,7 +313,7 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
         for (int c = lane; c < a.chunks; c += 32) {
           const unsigned long long k = a.keys[at + c];
           if (key_good(k))
-            sum += a.sums[at + c] * weight(key_value(k), key_value(key));
+            sum += a.sums[at + c] * weight(key_value(k), key_value(key), floor_of(key_value(key), t));
         }
       sum = warp_sum(sum);
       if (lane == 0)
@@ -307,8 +328,9 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
       if (greedy) {
         good = key_index(key_s[j]) == x;
       } else {
-        const double p = weight(px, key_value(key_s[j])) / sum_s[j];
-        const double q = a.draft ? weight(qx, key_value(key_s[dj])) / sum_s[dj] : 1.0;
+        const float pm = key_value(key_s[j]), qm = a.draft ? key_value(key_s[dj]) : 0.0f;
+        const double p = weight(px, pm, floor_of(pm, t)) / sum_s[j];
+        const double q = a.draft ? weight(qx, qm, floor_of(qm, t)) / sum_s[dj] : 1.0;
         good = (double)u * q < p;
       }
     }
@@ -349,6 +371,7 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
   w.pm = key_value(key_s[stop]), w.p_norm = 1.0 / sum_s[stop];
   w.q = refused && a.draft ? a.draft + ((long long)b * a.rows + stop) * a.ldd : nullptr;
   w.qm = w.q ? key_value(key_s[a.rows + 1 + stop]) : 0.0f, w.q_norm = w.q ? 1.0 / sum_s[a.rows + 1 + stop] : 0.0;
+  w.p_floor = floor_of(w.pm, t), w.q_floor = floor_of(w.qm, t);
   w.without = refused && !a.draft ? at_stop : -1;
   int s0 = 0, s1 = 0;
   double before = 0.0, total = 0.0, place = 0.0;
@@ -382,7 +405,7 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
         return sum;
       }
       const unsigned long long k = a.keys[at + c];
-      return key_good(k) ? a.sums[at + c] * weight(key_value(k), w.pm) * w.p_norm : 0.0;
+      return key_good(k) ? a.sums[at + c] * weight(key_value(k), w.pm, w.p_floor) * w.p_norm : 0.0;
     };
     if (warp == 0) {
       double upto = 0.0;
@@ -459,8 +482,20 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
     s0 = min((rank * kPickWarps + seg) * segment, a.vocab), s1 = min(s0 + segment, a.vocab);
   }
   if (!(total > 0.0)) {  // nothing of the target is left but rounding: its first maximum
-    if (rank == 0 && threadIdx.x == 0)
-      tokens[stop] = key_index(key_s[stop]);
+    if (rank)
+      return;
+    __syncthreads();
+    if (threadIdx.x == 0)
+      found_s = a.vocab;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.vocab; i += kPickThreads)
+      if (w.p[i] == w.pm) {
+        atomicMin(&found_s, i);
+        break;
+      }
+    __syncthreads();
+    if (threadIdx.x == 0)
+      tokens[stop] = found_s;
     return;
   }
   const int token = invert(w, &inv, s0, s1, before, place);

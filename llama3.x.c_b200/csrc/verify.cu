@@ -10,6 +10,8 @@
 #include <float.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "../../include/kernels_cuda.h"
 #include "common.cuh"
 #include "kernels_cuda_internal.h"
@@ -22,7 +24,7 @@ constexpr int kSumThreads = 256;
 constexpr int kChunk = 16 * kSumThreads;  // logits of a row per CTA of the sums kernel
 constexpr int kPickThreads = 512;
 constexpr int kPickWarps = kPickThreads / 32;
-constexpr int kPickCtas = 8;  // a cluster per request
+constexpr int kMaxCtas = 16;  // a cluster per request, of 4 to 16 CTAs
 constexpr int kMaxRows = 64;
 constexpr int kMaxSlots = 2 * kMaxRows + 1;
 constexpr float kMaxTemperature = 1e30f;  // 700 T is a number
@@ -78,7 +80,8 @@ __device__ __forceinline__ double warp_sum(double v) {
 struct Weights {
   const uint2 *table;  // kExpfTable in shared memory
   double k32;          // 32 / (T ln 2)
-  __device__ __forceinline__ double operator()(float l, float m, float floor) const {
+  // e^-700 of the largest instead of 0 below the floor: what a sum does not see.
+  __device__ __forceinline__ double above(float l, float m, float floor) const {
     constexpr double c = 0.021660849392498290, a2 = c * c / 4;  // ln 2 / 32; the square of |r| c's largest value
     constexpr double c4 = c * c * c * c / 24, c3 = c * c * c * (1.0 / 6 + a2 * 5 / 4 / 120), c2 = c * c / 2,
                      c1 = c * (1 - a2 * a2 * 5 / 16 / 120), shift = 0x1.8p+52;
@@ -88,7 +91,11 @@ struct Weights {
     const uint2 e = table[k & 31];
     const double s = __hiloint2double((int)e.y + (k << 15), (int)e.x);
     const double y = __fma_rn(__fma_rn(__fma_rn(__fma_rn(c4, r, c3), r, c2), r, c1), r, 1.0);
-    return l < floor ? 0.0 : y * s;
+    return y * s;
+  }
+  __device__ __forceinline__ double operator()(float l, float m, float floor) const {
+    const double w = above(l, m, floor);
+    return l < floor ? 0.0 : w;
   }
 };
 // The floor: (l - m) / T is in [-760, 0] above it whatever the roundings, and finite.
@@ -118,6 +125,12 @@ __device__ __forceinline__ bool slot_row(const VerifyArgs &a, int b, int slot, c
   return a.draft && j < count && a.temperature[b] != 0.0f;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // One chunk of one row: its maximum and the sum of exp((l - max) / T) over the chunk, or (T = 0) its first maximum.
 __global__ void __launch_bounds__(kSumThreads, 4) verify_sums_kernel(const VerifyArgs a) {
   __shared__ float max_s[kSumThreads / 32];
@@ -133,18 +146,28 @@ __global__ void __launch_bounds__(kSumThreads, 4) verify_sums_kernel(const Verif
   const float *row;
   if (!slot_row(a, b, slot, &row))
     return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = chunk * kChunk + threadIdx.x;
-  float v[16], m = __int_as_float(0xff800000);
-  bool bad = false;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = chunk * kChunk;
+  // Sixteen values a thread: four neighbouring ones of each quarter of the chunk where they lie at 16-byte addresses.
+  const bool whole = first + kChunk <= a.vocab && ((uintptr_t)(row + first) & 15) == 0;
+  float v[16];
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < 16; i++)
-    v[i] = first + i * kSumThreads < a.vocab ? row[first + i * kSumThreads] : __int_as_float(0xff800000);
+    for (int i = 0; i < 4; i++) {
+      const float4 x = reinterpret_cast<const float4 *>(row + first)[i * kSumThreads + threadIdx.x];
+      v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+    }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
-    m = fmaxf(m, v[i]);
-    bad |= !(v[i] < __int_as_float(0x7f800000));
+    for (int i = 0; i < 16; i++) {
+      const int e = first + i * kSumThreads + threadIdx.x;
+      v[i] = e < a.vocab ? row[e] : __int_as_float(0xff800000);
+    }
   }
-  if (bad)
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < 16; i++)
+    m = max_nan(m, v[i]);
+  if (!(m < __int_as_float(0x7f800000)))
     m = __int_as_float(0x7f800000);
 #pragma unroll
   for (int o = 16; o; o >>= 1)
@@ -161,18 +184,27 @@ __global__ void __launch_bounds__(kSumThreads, 4) verify_sums_kernel(const Verif
   if (t > 0.0f && good) {
     const Weights weight{table, k32_of(t)};
     const float floor = floor_of(m, t);
+    if ((double)m - (double)floor >= 600.0 * (double)t) {
 #pragma unroll
-    for (int i = 0; i < 16; i++)
-      sum += weight(v[i], m, floor);
+      for (int i = 0; i < 16; i++)
+        sum += weight.above(v[i], m, floor);
+    } else {  // the floor is rounded to the maximum, or ends at the lowest number
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        sum += weight(v[i], m, floor);
+    }
     sum = warp_sum(sum);
     if (lane == 0)
       sum_s[warp] = sum;
   } else {
     at = 0xFFFFFFFFu;
 #pragma unroll
-    for (int i = 15; i >= 0; i--)
-      if (v[i] == m && first + i * kSumThreads < a.vocab)
-        at = first + i * kSumThreads;
+    for (int i = 15; i >= 0; i--) {
+      const int e = whole ? first + 4 * ((i >> 2) * kSumThreads + (int)threadIdx.x) + (i & 3)
+                          : first + i * kSumThreads + (int)threadIdx.x;
+      if (v[i] == m && e < a.vocab)
+        at = e;
+    }
     at = __reduce_min_sync(0xffffffffu, at);
     if (lane == 0)
       first_s[warp] = at;
@@ -199,12 +231,15 @@ struct Residual {
   float pm, qm, p_floor, q_floor;
   double p_norm, q_norm;
   int without;
-  __device__ __forceinline__ double operator()(int i) const {
+  __device__ __forceinline__ double of(float pl, float ql) const {
     // Both products are rounded (no fused multiply-add): where draft and target are the same row nothing is left.
-    double w = __dmul_rn(weight(p[i], pm, p_floor), p_norm);
+    double w = __dmul_rn(weight(pl, pm, p_floor), p_norm);
     if (q)
-      w -= __dmul_rn(weight(q[i], qm, q_floor), q_norm);
-    return i == without ? 0.0 : fmax(w, 0.0);
+      w -= __dmul_rn(weight(ql, qm, q_floor), q_norm);
+    return fmax(w, 0.0);
+  }
+  __device__ __forceinline__ double operator()(int i) const {
+    return i == without ? 0.0 : of(p[i], q ? q[i] : 0.0f);
   }
 };
 
@@ -265,14 +300,14 @@ __device__ int invert(const Residual &w, Invert *t, int s0, int s1, double run, 
 __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const VerifyArgs a) {
   __shared__ unsigned long long key_s[kMaxSlots];
   __shared__ uint2 table[32];
-  __shared__ double sum_s[kMaxSlots], warp_sums[kPickWarps], slices[kPickCtas];
+  __shared__ double sum_s[kMaxSlots], warp_sums[kPickWarps], slices[kMaxCtas];
   __shared__ Invert inv;
   __shared__ int stop_s, found_s;
   cg::cluster_group cluster = cg::this_cluster();
   load_table(table);
   pdl_wait();
   pdl_launch_dependents();
-  const int b = blockIdx.x / kPickCtas, rank = blockIdx.x % kPickCtas;
+  const int ctas = cluster.num_blocks(), b = blockIdx.x / ctas, rank = blockIdx.x % ctas;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count = count_of(a, b);
   const float t = a.temperature[b];
@@ -443,25 +478,34 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
     total = slices[0], place = slices[1], before = slices[2];
     s0 = max(found_s, 0) * kChunk, s1 = min(s0 + kChunk, a.vocab);
   } else {
-    // Warp segments of equal length: segment s of kPickCtas * kPickWarps.
-    const int segment = (a.vocab + kPickCtas * kPickWarps - 1) / (kPickCtas * kPickWarps);
+    // Warp segments of equal length, eight reads of both rows under way a lane.
+    const int segment = (a.vocab + ctas * kPickWarps - 1) / (ctas * kPickWarps);
     const int w0 = min((rank * kPickWarps + warp) * segment, a.vocab), w1 = min(w0 + segment, a.vocab);
     double sum = 0.0;
-#pragma unroll 4
-    for (int i = w0 + lane; i < w1; i += 32)
-      sum += w(i);
+    for (int i0 = w0 + lane; i0 < w1; i0 += 256) {
+      float p[8], q[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int i = i0 + 32 * k;
+        p[k] = i < w1 ? w.p[i] : __int_as_float(0xff800000);
+        q[k] = i < w1 ? w.q[i] : __int_as_float(0xff800000);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        sum += w.of(p[k], q[k]);
+    }
     sum = warp_sum(sum);
     if (lane == 0)
       warp_sums[warp] = sum;
     __syncthreads();
-    if (threadIdx.x < kPickCtas) {
+    if ((int)threadIdx.x < ctas) {
       double slice = 0.0;
       for (int i = 0; i < kPickWarps; i++)
         slice += warp_sums[i];
       *cluster.map_shared_rank(&slices[rank], threadIdx.x) = slice;
     }
     cluster.sync();
-    for (int r = 0; r < kPickCtas; r++) {
+    for (int r = 0; r < ctas; r++) {
       if (r == rank)
         before = total;
       total += slices[r];
@@ -505,6 +549,22 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
 
 size_t verify_chunks(int vocab) { return ((size_t)vocab + kChunk - 1) / kChunk; }
 
+// Clusters of 16 CTAs are above the portable 8: allowed once per device.
+cudaError_t allow_large_clusters() {
+  static std::mutex mu;
+  static bool done[64];
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= 64)
+    return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> hold(mu);
+  if (done[dev])
+    return cudaSuccess;
+  const cudaError_t r = cudaFuncSetAttribute(verify_pick_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  done[dev] = r == cudaSuccess;
+  return r;
+}
+
 }  // namespace
 
 extern "C" {
@@ -533,7 +593,7 @@ void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt,
     return;
   }
   const size_t pairs = (size_t)batch * (2 * rows + 1) * verify_chunks(vocab);
-  if (pairs > 0x7fffffffu || (size_t)batch * kPickCtas > 0x7fffffffu) {
+  if (pairs > 0x7fffffffu || (size_t)batch * kMaxCtas > 0x7fffffffu) {
     kc_fail("%s: batch %d of %d rows is too large", name, batch, rows);
     return;
   }
@@ -548,18 +608,24 @@ void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt,
       kc_launch_pdl(verify_sums_kernel, dim3((unsigned)pairs), dim3(kSumThreads), 0, kc_stream(), a);
   if (e == cudaSuccess) {
     kc_count_launch();
+    // The largest clusters that run in one wave of two CTAs per SM: a request's rows are read by more SMs at once.
+    int ctas = kMaxCtas;
+    while (ctas > 4 && (long long)ctas * batch > 2 * kc_device_sms())
+      ctas /= 2;
+    e = allow_large_clusters();
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)batch * kPickCtas);
+    cfg.gridDim = dim3((unsigned)batch * ctas);
     cfg.blockDim = dim3(kPickThreads);
     cfg.stream = kc_stream();
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = kc_pdl_enabled() ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = kPickCtas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.x = ctas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, verify_pick_kernel, a);
+    if (e == cudaSuccess)
+      e = cudaLaunchKernelEx(&cfg, verify_pick_kernel, a);
     if (e == cudaSuccess)
       kc_count_launch();
   }

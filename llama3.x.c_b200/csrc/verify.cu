@@ -21,7 +21,8 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kSumThreads = 256;
-constexpr int kChunk = 16 * kSumThreads;  // logits of a row per CTA of the sums kernel
+constexpr int kBlock = 16 * kSumThreads;  // logits that a CTA of the sums kernel takes at a time
+constexpr int kLoops = 4;                 // and how often, where there is work enough for every SM all the same
 constexpr int kPickThreads = 512;
 constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kMaxCtas = 16;  // a cluster per request, of 4 to 16 CTAs
@@ -35,7 +36,7 @@ struct VerifyArgs {
   long long ldt, ldd;
   const int *drafted, *counts;
   const float *uniforms, *temperature;
-  int vocab, batch, rows, chunks;
+  int vocab, batch, rows, loops, chunks;  // chunks of loops * kBlock logits a row
   double *sums;              // [batch][2 rows + 1][chunks]
   unsigned long long *keys;  // the same: order-preserving maximum and its first index
 };
@@ -131,7 +132,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// One chunk of one row: its maximum and the sum of exp((l - max) / T) over the chunk, or (T = 0) its first maximum.
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// One chunk of one row (a.loops blocks of 4096): its maximum and the sum of exp((l - max) / T) over the chunk, or
+// (T = 0) its first maximum. A warp keeps a maximum of its own from block to block, to which its lanes' sums refer.
 __global__ void __launch_bounds__(kSumThreads, 4) verify_sums_kernel(const VerifyArgs a) {
   __shared__ float max_s[kSumThreads / 32];
   __shared__ double sum_s[kSumThreads / 32];
@@ -146,45 +154,64 @@ __global__ void __launch_bounds__(kSumThreads, 4) verify_sums_kernel(const Verif
   const float *row;
   if (!slot_row(a, b, slot, &row))
     return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = chunk * kChunk;
-  // Sixteen values a thread: four neighbouring ones of each quarter of the chunk where they lie at 16-byte addresses.
-  const bool whole = first + kChunk <= a.vocab && ((uintptr_t)(row + first) & 15) == 0;
-  float v[16];
-  if (whole) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float4 x = reinterpret_cast<const float4 *>(row + first)[i * kSumThreads + threadIdx.x];
-      v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const int e = first + i * kSumThreads + threadIdx.x;
-      v[i] = e < a.vocab ? row[e] : __int_as_float(0xff800000);
-    }
-  }
-  float m = v[0];
-#pragma unroll
-  for (int i = 1; i < 16; i++)
-    m = max_nan(m, v[i]);
-  if (!(m < __int_as_float(0x7f800000)))
-    m = __int_as_float(0x7f800000);
-#pragma unroll
-  for (int o = 16; o; o >>= 1)
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0)
-    max_s[warp] = m;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kSumThreads / 32; w++)
-    m = fmaxf(m, max_s[w]);
-  const bool good = fabsf(m) < __int_as_float(0x7f800000);
+  constexpr float kInf = __builtin_inff();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Weights weight{table, t > 0.0f ? k32_of(t) : 0.0};
+  float m = -kInf, floor = 0.0f;  // the warp's maximum (the lane's at T = 0)
+  unsigned at = 0xFFFFFFFFu;
   double sum = 0.0;
-  unsigned at = 0;
-  if (t > 0.0f && good) {
-    const Weights weight{table, k32_of(t)};
-    const float floor = floor_of(m, t);
-    if ((double)m - (double)floor >= 600.0 * (double)t) {
+  bool bad = false, deep = false;
+  for (int loop = 0; loop < a.loops; loop++) {
+    const int first = (chunk * a.loops + loop) * kBlock;
+    if (first >= a.vocab)
+      break;
+    // Sixteen values a thread: four neighbouring ones of each quarter of the block where they lie at 16-byte addresses.
+    const bool whole = first + kBlock <= a.vocab && ((uintptr_t)(row + first) & 15) == 0;
+    float v[16];
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float4 x = reinterpret_cast<const float4 *>(row + first)[i * kSumThreads + threadIdx.x];
+        v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int e = first + i * kSumThreads + threadIdx.x;
+        v[i] = e < a.vocab ? row[e] : -kInf;
+      }
+    }
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i < 16; i++)
+      top = max_nan(top, v[i]);
+    if (!(t > 0.0f)) {
+      bad |= !(top < kInf);
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        if (v[i] > m) {
+          m = v[i];
+          at = whole ? first + 4 * ((i >> 2) * kSumThreads + (int)threadIdx.x) + (i & 3)
+                     : first + i * kSumThreads + (int)threadIdx.x;
+        }
+      continue;
+    }
+    top = warp_max_nan(top);
+    if (!(top < kInf)) {
+      bad = true;
+      break;
+    }
+    if (top > m) {
+      floor = floor_of(top, t);
+      deep = (double)top - (double)floor >= 600.0 * (double)t;
+      if (m > -kInf)
+        sum *= weight(m, top, floor);
+      m = top;
+    }
+    if (m == -kInf)
+      continue;
+    if (deep) {
 #pragma unroll
       for (int i = 0; i < 16; i++)
         sum += weight.above(v[i], m, floor);
@@ -193,33 +220,28 @@ __global__ void __launch_bounds__(kSumThreads, 4) verify_sums_kernel(const Verif
       for (int i = 0; i < 16; i++)
         sum += weight(v[i], m, floor);
     }
-    sum = warp_sum(sum);
-    if (lane == 0)
-      sum_s[warp] = sum;
-  } else {
-    at = 0xFFFFFFFFu;
-#pragma unroll
-    for (int i = 15; i >= 0; i--) {
-      const int e = whole ? first + 4 * ((i >> 2) * kSumThreads + (int)threadIdx.x) + (i & 3)
-                          : first + i * kSumThreads + (int)threadIdx.x;
-      if (v[i] == m && e < a.vocab)
-        at = e;
-    }
-    at = __reduce_min_sync(0xffffffffu, at);
-    if (lane == 0)
-      first_s[warp] = at;
   }
+  float top = bad ? kInf : m;
+  top = warp_max_nan(top);
+  if (lane == 0)
+    max_s[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSumThreads / 32; w++)
+    top = fmaxf(top, max_s[w]);
+  if (t > 0.0f && top < kInf && m > -kInf)
+    sum *= weight(m, top, floor_of(top, t));
+  sum = warp_sum(sum);
+  at = __reduce_min_sync(0xffffffffu, m == top ? at : 0xFFFFFFFFu);
+  if (lane == 0)
+    sum_s[warp] = sum, first_s[warp] = at;
   __syncthreads();
   if (threadIdx.x == 0) {
     sum = 0.0;
-    at = 0xFFFFFFFFu;
     for (int w = 0; w < kSumThreads / 32; w++)
-      if (t > 0.0f && good)
-        sum += sum_s[w];
-      else
-        at = min(at, first_s[w]);
+      sum += sum_s[w], at = min(at, first_s[w]);
     a.sums[(long long)id * a.chunks + chunk] = sum;
-    a.keys[(long long)id * a.chunks + chunk] = m == __int_as_float(0x7f800000) ? kBad : row_key(m, at);
+    a.keys[(long long)id * a.chunks + chunk] = top == kInf ? kBad : row_key(top, at);
   }
 }
 
@@ -410,6 +432,42 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
   w.without = refused && !a.draft ? at_stop : -1;
   int s0 = 0, s1 = 0;
   double before = 0.0, total = 0.0, place = 0.0;
+  // The weights of the warps' segments (of `segment` tokens) of [first, last), eight reads of both rows under way a lane.
+  auto segments = [&](int first, int last, int segment) {
+    const int w0 = min(first + warp * segment, last), w1 = min(w0 + segment, last);
+    double sum = 0.0;
+    for (int i0 = w0 + lane; i0 < w1; i0 += 256) {
+      float p[8], q[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int i = i0 + 32 * k;
+        p[k] = i < w1 && i != w.without ? w.p[i] : __int_as_float(0xff800000);
+        q[k] = i < w1 && w.q ? w.q[i] : __int_as_float(0xff800000);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        sum += w.of(p[k], q[k]);
+    }
+    sum = warp_sum(sum);
+    if (lane == 0)
+      warp_sums[warp] = sum;
+    __syncthreads();
+  };
+  // The segment that the place falls into; behind the last one with weight, that one.
+  auto narrow = [&](int first, int last, int segment) {
+    int seg = 0;
+    bool some = false;
+    double run = before;
+    for (int i = 0; i < kPickWarps; i++) {
+      if (warp_sums[i] > 0.0 && (!some || place >= run)) {
+        seg = i;
+        before = run;
+        some = true;
+      }
+      run += warp_sums[i];
+    }
+    s0 = min(first + seg * segment, last), s1 = min(s0 + segment, last);
+  };
   auto place_in = [&]() {
     place = (double)u_last * total;
     if (!(place < total))
@@ -422,15 +480,10 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
     // p alone: the chunks' sums; the refused token's chunk is summed again without it (a difference would leave rounding
     // where nothing is left).
     const long long at = base + (long long)stop * a.chunks;
-    const int again = w.without >= 0 ? w.without / kChunk : -1;
+    const int length = a.loops * kBlock, again = w.without >= 0 ? w.without / length : -1;
     if (again >= 0) {
-      double sum = 0.0;
-      for (int i = again * kChunk + threadIdx.x; i < min((again + 1) * kChunk, a.vocab); i += kPickThreads)
-        sum += w(i);
-      sum = warp_sum(sum);
-      if (lane == 0)
-        warp_sums[warp] = sum;
-      __syncthreads();
+      const int first = again * length;
+      segments(first, min(first + length, a.vocab), length / kPickWarps);
     }
     auto chunk = [&](int c) {
       if (c == again) {
@@ -476,28 +529,13 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
     }
     __syncthreads();
     total = slices[0], place = slices[1], before = slices[2];
-    s0 = max(found_s, 0) * kChunk, s1 = min(s0 + kChunk, a.vocab);
+    const int first = max(found_s, 0) * length, last = min(first + length, a.vocab);
+    segments(first, last, length / kPickWarps);
+    narrow(first, last, length / kPickWarps);
   } else {
-    // Warp segments of equal length, eight reads of both rows under way a lane.
     const int segment = (a.vocab + ctas * kPickWarps - 1) / (ctas * kPickWarps);
-    const int w0 = min((rank * kPickWarps + warp) * segment, a.vocab), w1 = min(w0 + segment, a.vocab);
-    double sum = 0.0;
-    for (int i0 = w0 + lane; i0 < w1; i0 += 256) {
-      float p[8], q[8];
-#pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const int i = i0 + 32 * k;
-        p[k] = i < w1 ? w.p[i] : __int_as_float(0xff800000);
-        q[k] = i < w1 ? w.q[i] : __int_as_float(0xff800000);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; k++)
-        sum += w.of(p[k], q[k]);
-    }
-    sum = warp_sum(sum);
-    if (lane == 0)
-      warp_sums[warp] = sum;
-    __syncthreads();
+    const int first = min(rank * kPickWarps * segment, a.vocab), last = min(first + kPickWarps * segment, a.vocab);
+    segments(first, last, segment);
     if ((int)threadIdx.x < ctas) {
       double slice = 0.0;
       for (int i = 0; i < kPickWarps; i++)
@@ -513,17 +551,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
     place_in();
     if (total > 0.0 && (place < before || place >= before + slices[rank]))  // the slices tile [0, total): one CTA goes on
       return;
-    // The warp whose segment the place falls into; behind the last one with weight, that one.
-    int seg = -1;
-    double run = before;
-    for (int i = 0; i < kPickWarps; i++) {
-      if (warp_sums[i] > 0.0 && (seg < 0 || place >= run)) {
-        seg = i;
-        before = run;
-      }
-      run += warp_sums[i];
-    }
-    s0 = min((rank * kPickWarps + seg) * segment, a.vocab), s1 = min(s0 + segment, a.vocab);
+    narrow(first, last, segment);
   }
   if (!(total > 0.0)) {  // nothing of the target is left but rounding: its first maximum
     if (rank)
@@ -547,7 +575,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
     tokens[stop] = token;
 }
 
-size_t verify_chunks(int vocab) { return ((size_t)vocab + kChunk - 1) / kChunk; }
+size_t verify_blocks(int vocab) { return ((size_t)vocab + kBlock - 1) / kBlock; }
 
 // Clusters of 16 CTAs are above the portable 8: allowed once per device.
 cudaError_t allow_large_clusters() {
@@ -572,14 +600,14 @@ extern "C" {
 size_t k_verify_bytes(int vocab, int batch, int rows) {
   if (vocab <= 0 || batch <= 0 || rows < 0 || rows > kMaxRows)
     return 0;
-  return (size_t)batch * (2 * rows + 1) * verify_chunks(vocab) * (sizeof(double) + sizeof(unsigned long long));
+  return (size_t)batch * (2 * rows + 1) * verify_blocks(vocab) * (sizeof(double) + sizeof(unsigned long long));
 }
 
 void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt, const float *draft, size_t ldd,
                     const int *drafted, const int *counts, const float *uniforms, const float *temperature, int vocab,
                     int batch, int rows, void *work) {
   const char *name = "k_verify_draft";
-  if (vocab <= 0 || batch < 0 || rows < 0 || rows > kMaxRows || ldt < (size_t)vocab ||
+  if (vocab <= 0 || vocab > (1 << 30) || batch < 0 || rows < 0 || rows > kMaxRows || ldt < (size_t)vocab ||
       (draft && rows && ldd < (size_t)vocab)) {
     kc_fail("%s: invalid shape vocab=%d batch=%d rows=%d ldt=%zu ldd=%zu (at most %d rows)", name, vocab, batch, rows,
             ldt, ldd, kMaxRows);
@@ -592,7 +620,8 @@ void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt,
     kc_fail("%s: missing outputs, logits, drafts, numbers or 16-byte aligned work", name);
     return;
   }
-  const size_t pairs = (size_t)batch * (2 * rows + 1) * verify_chunks(vocab);
+  // Longer chunks where they leave every SM some sixteen CTAs (half of which, or more, find nothing to do).
+  size_t blocks = verify_blocks(vocab), pairs = (size_t)batch * (2 * rows + 1) * blocks;
   if (pairs > 0x7fffffffu || (size_t)batch * kMaxCtas > 0x7fffffffu) {
     kc_fail("%s: batch %d of %d rows is too large", name, batch, rows);
     return;
@@ -601,7 +630,9 @@ void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt,
   a.accepted = accepted, a.tokens = tokens, a.target = target, a.draft = rows ? draft : nullptr;
   a.ldt = (long long)ldt, a.ldd = (long long)ldd, a.drafted = drafted, a.counts = counts;
   a.uniforms = uniforms, a.temperature = temperature, a.vocab = vocab, a.batch = batch, a.rows = rows;
-  a.chunks = (int)verify_chunks(vocab);
+  a.loops = pairs >= (size_t)16 * kLoops * kc_device_sms() ? kLoops : 1;
+  a.chunks = (int)((blocks + a.loops - 1) / a.loops);
+  pairs = (size_t)batch * (2 * rows + 1) * a.chunks;
   a.sums = static_cast<double *>(work);
   a.keys = reinterpret_cast<unsigned long long *>(a.sums + pairs);
   cudaError_t e =

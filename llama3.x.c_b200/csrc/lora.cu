@@ -162,6 +162,16 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ uint32_t tf32_hi(float x) { return __float_as_uint(x) & 0xffffe000u; }
 __device__ __forceinline__ uint32_t tf32_lo(float x) { return __float_as_uint(x - __uint_as_float(tf32_hi(x))); }
 
+// This lane's eight elements of rows g and g + 8, split.
+struct Split16 {
+  uint32_t hi[2][8], lo[2][8];
+  __device__ __forceinline__ void set(int r, const float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      hi[r][j] = tf32_hi(v[j]), lo[r][j] = tf32_lo(v[j]);
+  }
+};
+
 // Eight elements of a row as they lie in memory, so that many can be under way.
 template <typename W>
 struct Raw8 {
@@ -188,20 +198,21 @@ struct Raw8 {
   }
 };
 
-// 16 rows x 8 columns += 32 elements of the 16 rows (this lane's eight of rows g and g + 8) times those of the 8 columns
-// (this lane's eight of column g). SPLIT: the weights have more bits than tf32.
+// 16 rows x 8 columns += 32 elements of the 16 rows times those of the 8 columns (this lane's eight of column g).
+// SPLIT: the weights have more bits than tf32.
 template <bool SPLIT>
-__device__ __forceinline__ void product32(float (&sum)[4], const float (&x0)[8], const float (&x1)[8],
-                                          const float (&w)[8]) {
+__device__ __forceinline__ void product32(float (&sum)[4], const Split16 &x, const float (&w)[8]) {
   float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int s = 0; s < 4; s++) {
-    const uint32_t lo[4] = {tf32_lo(x0[2 * s]), tf32_lo(x1[2 * s]), tf32_lo(x0[2 * s + 1]), tf32_lo(x1[2 * s + 1])};
-    const uint32_t hi[4] = {tf32_hi(x0[2 * s]), tf32_hi(x1[2 * s]), tf32_hi(x0[2 * s + 1]), tf32_hi(x1[2 * s + 1])};
-    const uint32_t b0 = tf32_hi(w[2 * s]), b1 = tf32_hi(w[2 * s + 1]);
+    const int e = 2 * s;
+    const uint32_t lo[4] = {x.lo[0][e], x.lo[1][e], x.lo[0][e + 1], x.lo[1][e + 1]};
+    const uint32_t hi[4] = {x.hi[0][e], x.hi[1][e], x.hi[0][e + 1], x.hi[1][e + 1]};
+    const uint32_t b0 = SPLIT ? tf32_hi(w[e]) : __float_as_uint(w[e]);
+    const uint32_t b1 = SPLIT ? tf32_hi(w[e + 1]) : __float_as_uint(w[e + 1]);
     mma_tf32(d, lo, b0, b1);
     if (SPLIT)
-      mma_tf32(d, hi, tf32_lo(w[2 * s]), tf32_lo(w[2 * s + 1]));
+      mma_tf32(d, hi, tf32_lo(w[e]), tf32_lo(w[e + 1]));
     mma_tf32(d, hi, b0, b1);
   }
 #pragma unroll
@@ -307,7 +318,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
   if (!find_tile(a, &t, id / parts))
     return;  // the whole cluster
   const int part = id % parts, rows = t.n, hs = h_stride(a.max_rank);
-  float *partial = smem, *h = smem + kTileRows * hs;  // [64][hs] each
+  // [64][hs] each: this CTA's partial vectors (then the low parts), the vectors, their high parts.
+  float *partial = smem, *h = smem + kTileRows * hs, *high = h + kTileRows * hs, *low = partial;
   LoraAdapter w = {nullptr, nullptr, 0, 0.0f};
   bool bad = false;
   if (t.adapter < a.count) {
@@ -324,11 +336,12 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
   }
   const W *A = static_cast<const W *>(w.a), *B = static_cast<const W *>(w.b);
   const int rank32 = (w.rank + 31) / 32 * 32;
-  const int rg = warp & 3, half = warp >> 2;  // this warp's 16 rows, and its half of the work along n or d
+  // This warp's 16 rows, and its share of the work along n or d: the warps that a small tile leaves over take shares.
+  const int groups = rows > 32 ? 4 : rows > 16 ? 2 : 1, ways = kWarps / groups, rg = warp % groups, way = warp / groups;
   const int i0 = 16 * rg + g, i1 = i0 + 8;
   const bool busy = 16 * rg < rows;
 
-  // A x: this CTA's slice of n in steps of 32, the two halves of the warps in turn; 64 rows of A at a time.
+  // A x: this CTA's slice of n in steps of 32, the ways in turn; 64 rows of A at a time.
   const int n_slice = ((a.n + ctas - 1) / ctas + 31) / 32 * 32;
   const int n0 = min(rank * n_slice, a.n), n1 = min(n0 + n_slice, a.n);
   const bool x_wide = aligned16(a.x) && a.ldx % 4 == 0, a_wide = aligned16(A) && a.n % 8 == 0;
@@ -341,11 +354,11 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         sum[c][i] = 0.0f;
     if (busy) {
       const float *x0 = a.x + (long long)t.rows[min(i0, rows - 1)] * a.ldx, *x1 = a.x + (long long)t.rows[min(i1, rows - 1)] * a.ldx;
-      for (int i = n0 + 32 * half; i < n1; i += 64) {
+      for (int i = n0 + 32 * way; i < n1; i += 32 * ways) {
         Raw8<float> x[2];
         x[0].load(x0, i + 8 * q, n1, x_wide);
         x[1].load(x1, i + 8 * q, n1, x_wide);
-        float v0[8], v1[8];
+        Split16 xs;
 #pragma unroll
         for (int c0 = 0; c0 < 8; c0 += kFlight) {
           Raw8<W> wr[kFlight];
@@ -354,22 +367,25 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
             if (k0 + 8 * (c0 + c) < w.rank)
               wr[c].load(A + (long long)min(k0 + 8 * (c0 + c) + g, w.rank - 1) * a.n, i + 8 * q, n1, a_wide);
           if (c0 == 0) {
-            x[0].get(v0);
-            x[1].get(v1);
+            float v[8];
+            x[0].get(v);
+            xs.set(0, v);
+            x[1].get(v);
+            xs.set(1, v);
           }
 #pragma unroll
           for (int c = 0; c < kFlight; c++)
             if (k0 + 8 * (c0 + c) < w.rank) {
               float wv[8];
               wr[c].get(wv);
-              product32<kSplit>(sum[c0 + c], v0, v1, wv);
+              product32<kSplit>(sum[c0 + c], xs, wv);
             }
         }
       }
     }
-    // The second half's sums, then the first's on top, into this CTA's partial vectors.
-    for (int turn = 1; turn >= 0; turn--) {
-      if (busy && half == turn)
+    // The last way's sums, then the others' on top, into this CTA's partial vectors.
+    for (int turn = ways - 1; turn >= 0; turn--) {
+      if (busy && way == turn)
 #pragma unroll
         for (int c = 0; c < 8; c++)
 #pragma unroll
@@ -377,39 +393,40 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
             const int k = k0 + 8 * c + 2 * q + (i & 1);
             float *at = partial + (i < 2 ? i0 : i1) * hs + k;
             if (k < rank32)
-              *at = k >= w.rank ? 0.0f : turn ? sum[c][i] : *at + sum[c][i];
+              *at = k >= w.rank ? 0.0f : turn == ways - 1 ? sum[c][i] : *at + sum[c][i];
           }
       __syncthreads();
     }
   }
   // The cluster's sums: CTA c adds up its share of the rows from all CTAs in their order, then everyone fetches them.
   cluster.sync();
-  for (int e = threadIdx.x; e < kTileRows * rank32; e += kThreads) {
-    const int i = e / rank32, k = e - i * rank32;
-    if (i % ctas == rank && i < rows) {
-      float s = 0.0f;
-      for (int c = 0; c < ctas; c++)
-        s += *cluster.map_shared_rank(&partial[i * hs + k], c);
-      h[i * hs + k] = s * w.scale;
-    }
+  const int own = (rows - rank + ctas - 1) / ctas;  // rows rank, rank + ctas, ...
+  for (int e = threadIdx.x; e < own * rank32; e += kThreads) {
+    const int n = e / rank32, at = (rank + n * ctas) * hs + e - n * rank32;
+    float s = 0.0f;
+#pragma unroll 8
+    for (int c = 0; c < ctas; c++)
+      s += *cluster.map_shared_rank(&partial[at], c);
+    h[at] = s * w.scale;
   }
   cluster.sync();
-  for (int e = threadIdx.x; e < kTileRows * rank32; e += kThreads) {
-    const int i = e / rank32, k = e - i * rank32;
-    if (i < rows && i % ctas != rank)
-      h[i * hs + k] = *cluster.map_shared_rank(&h[i * hs + k], i % ctas);
+#pragma unroll 4
+  for (int e = threadIdx.x; e < rows * rank32; e += kThreads) {
+    const int i = e / rank32, at = i * hs + e - i * rank32;
+    const float v = *cluster.map_shared_rank(&h[at], i % ctas);
+    high[at] = __uint_as_float(tf32_hi(v)), low[at] = __uint_as_float(tf32_lo(v));
   }
   cluster.sync();  // everything is fetched: a CTA may leave
   if (!busy)
     return;
 
-  // B h: this CTA's slice of d, 32 columns at a time, the two halves of the warps in turn.
+  // B h: this CTA's slice of d, 32 columns at a time, the ways in turn.
   const int d_all = parts * ctas, d_slice = ((a.d + d_all - 1) / d_all + 31) / 32 * 32;
   const int d0 = min((part * ctas + rank) * d_slice, a.d), d1 = min(d0 + d_slice, a.d);
   const bool b_wide = aligned16(B) && w.rank % 8 == 0;
   const bool pairs = a.ldo % 2 == 0 && ((uintptr_t)a.out & 7) == 0 && (!a.base || (a.ldb % 2 == 0 && ((uintptr_t)a.base & 7) == 0));
   const long long r0 = t.rows[min(i0, rows - 1)], r1 = t.rows[min(i1, rows - 1)];
-  for (int d = d0 + 32 * half; d < d1; d += 64) {
+  for (int d = d0 + 32 * way; d < d1; d += 32 * ways) {
     float sum[4][4];
 #pragma unroll
     for (int c = 0; c < 4; c++) {  // the base first: its reads are under way during the products
@@ -439,14 +456,22 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
 #pragma unroll
       for (int c = 0; c < 4; c++)
         wr[c].load(B + (long long)min(d + 8 * c + g, a.d - 1) * w.rank, k + 8 * q, w.rank, b_wide);
-      float v0[8], v1[8];
-      load8(h + i0 * hs + k + 8 * q, v0);
-      load8(h + i1 * hs + k + 8 * q, v1);
+      Split16 hv;
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const int at = (r ? i1 : i0) * hs + k + 8 * q;
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(high + at + j), y = *reinterpret_cast<const uint4 *>(low + at + j);
+          hv.hi[r][j] = x.x, hv.hi[r][j + 1] = x.y, hv.hi[r][j + 2] = x.z, hv.hi[r][j + 3] = x.w;
+          hv.lo[r][j] = y.x, hv.lo[r][j + 1] = y.y, hv.lo[r][j + 2] = y.z, hv.lo[r][j + 3] = y.w;
+        }
+      }
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         float wv[8];
         wr[c].get(wv);
-        product32<kSplit>(prod[c], v0, v1, wv);
+        product32<kSplit>(prod[c], hv, wv);
       }
     }
 #pragma unroll
@@ -493,11 +518,12 @@ cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned cl
 template <typename W>
 cudaError_t run(const LoraArgs &a) {
   constexpr int kCtas = 8;
-  if (a.rows < 24 || a.count >= kMaxBins)
+  // Four rows an adapter make a tile worth its search (measured at d = n = 4096, rank 16).
+  if (a.rows < 16 || a.rows < 4 * a.count || a.count >= kMaxBins)
     return launch<W>(lora_row_kernel<W>, a, (unsigned)a.rows, kCtas, 1, 0);
-  const size_t smem = 2 * sizeof(float) * kTileRows * h_stride(a.max_rank);
+  const size_t smem = 3 * sizeof(float) * kTileRows * h_stride(a.max_rank);
   cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(lora_tile_kernel<W>),
-                                (int)(2 * sizeof(float) * kTileRows * h_stride(kMaxRank)));
+                                (int)(3 * sizeof(float) * kTileRows * h_stride(kMaxRank)));
   for (int r = 0; r < a.rows && e == cudaSuccess; r += kMaxTileRows) {
     LoraArgs b = a;
     b.rows = a.rows - r < kMaxTileRows ? a.rows - r : kMaxTileRows;

@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/kernels_cuda.h"
 #include "common.cuh"
 #include "kernels_cuda_internal.h"
@@ -158,6 +160,12 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_tf32_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 
 __device__ __forceinline__ uint32_t tf32_hi(float x) { return __float_as_uint(x) & 0xffffe000u; }
 __device__ __forceinline__ uint32_t tf32_lo(float x) { return __float_as_uint(x - __uint_as_float(tf32_hi(x))); }
@@ -172,12 +180,31 @@ struct Split16 {
   }
 };
 
+// Values 2 j and 2 j + 1 of words u.
+template <typename W>
+__device__ __forceinline__ void two(const unsigned *u, int j, float &x, float &y) {
+  if constexpr (sizeof(W) == 4) {
+    x = __uint_as_float(u[2 * j]), y = __uint_as_float(u[2 * j + 1]);
+  } else if constexpr (std::is_same_v<W, __nv_bfloat16>) {
+    x = __uint_as_float(u[j] << 16), y = __uint_as_float(u[j] & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[j]));
+    x = f.x, y = f.y;
+  }
+}
+
 // Eight elements of a row as they lie in memory, so that many can be under way.
 template <typename W>
 struct Raw8 {
   uint4 v[sizeof(W) / 2];
 
-  // From element i on, zeros from `end` on. `wide`: whole groups of eight at 16-byte addresses.
+  // Whole groups of eight at 16-byte addresses.
+  __device__ __forceinline__ void load(const W *at) {
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(W) / 2); j++)
+      v[j] = __ldg(reinterpret_cast<const uint4 *>(at) + j);
+  }
+  // From element i on, zeros from `end` on. `wide`: as above.
   __device__ __forceinline__ void load(const W *row, int i, int end, bool wide) {
     if (wide && i + 8 <= end) {
 #pragma unroll
@@ -191,10 +218,10 @@ struct Raw8 {
     }
   }
   __device__ __forceinline__ void get(float (&f)[8]) const {
-    const W *at = reinterpret_cast<const W *>(v);
+    const unsigned *u = reinterpret_cast<const unsigned *>(v);
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-      f[j] = to_float(at[j]);
+    for (int j = 0; j < 4; j++)
+      two<W>(u, j, f[2 * j], f[2 * j + 1]);
   }
 };
 
@@ -202,7 +229,7 @@ struct Raw8 {
 // SPLIT: the weights have more bits than tf32.
 template <bool SPLIT>
 __device__ __forceinline__ void product32(float (&sum)[4], const Split16 &x, const float (&w)[8]) {
-  float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float d[4], small[4];  // two chains of MMAs
 #pragma unroll
   for (int s = 0; s < 4; s++) {
     const int e = 2 * s;
@@ -210,14 +237,19 @@ __device__ __forceinline__ void product32(float (&sum)[4], const Split16 &x, con
     const uint32_t hi[4] = {x.hi[0][e], x.hi[1][e], x.hi[0][e + 1], x.hi[1][e + 1]};
     const uint32_t b0 = SPLIT ? tf32_hi(w[e]) : __float_as_uint(w[e]);
     const uint32_t b1 = SPLIT ? tf32_hi(w[e + 1]) : __float_as_uint(w[e + 1]);
-    mma_tf32(d, lo, b0, b1);
+    if (s == 0) {
+      mma_tf32_first(small, lo, b0, b1);
+      mma_tf32_first(d, hi, b0, b1);
+    } else {
+      mma_tf32(small, lo, b0, b1);
+      mma_tf32(d, hi, b0, b1);
+    }
     if (SPLIT)
-      mma_tf32(d, hi, tf32_lo(w[e]), tf32_lo(w[e + 1]));
-    mma_tf32(d, hi, b0, b1);
+      mma_tf32(small, hi, tf32_lo(w[e]), tf32_lo(w[e + 1]));
   }
 #pragma unroll
   for (int i = 0; i < 4; i++)
-    sum[i] += d[i];
+    sum[i] += d[i] + small[i];
 }
 
 // The cluster's tile: its adapter (`count`: rows without one) and its rows in order. False: no such tile.
@@ -309,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
   extern __shared__ __align__(16) float smem[];
   __shared__ LoraTile t;
   constexpr bool kSplit = sizeof(W) == 4;
-  constexpr int kFlight = kSplit ? 4 : 8;  // column groups whose weights are under way at once
+  constexpr int kFlight = kSplit ? 2 : 4;  // column groups whose weights are under way at once
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank(), id = blockIdx.x / ctas;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
@@ -353,34 +385,64 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
       for (int i = 0; i < 4; i++)
         sum[c][i] = 0.0f;
     if (busy) {
-      const float *x0 = a.x + (long long)t.rows[min(i0, rows - 1)] * a.ldx, *x1 = a.x + (long long)t.rows[min(i1, rows - 1)] * a.ldx;
-      for (int i = n0 + 32 * way; i < n1; i += 32 * ways) {
-        Raw8<float> x[2];
-        x[0].load(x0, i + 8 * q, n1, x_wide);
-        x[1].load(x1, i + 8 * q, n1, x_wide);
+      const float *x0 = a.x + (long long)t.rows[min(i0, rows - 1)] * a.ldx;
+      const float *x1 = a.x + (long long)t.rows[min(i1, rows - 1)] * a.ldx;
+      // Whole steps first: every register is loaded again, for a step or half a step ahead, as soon as its value is
+      // used.
+      const int r1 = w.rank - 1, step = 32 * ways, first = n0 + 32 * way;
+      const int whole = x_wide && a_wide && w.rank % 8 == 0 ? n1 - 31 : 0;  // steps that start below it
+      const W *rows_a = A + (size_t)min(k0 + g, r1) * a.n + 8 * q;
+      const size_t rows8 = (size_t)8 * a.n;
+      auto row_of = [&](int c) { return rows_a + c * rows8; };
+      Raw8<float> x[2];
+      Raw8<W> wr[kFlight];
+      x0 += 8 * q, x1 += 8 * q;
+      if (first < whole) {
+        x[0].load(x0 + first);
+        x[1].load(x1 + first);
+#pragma unroll
+        for (int c = 0; c < kFlight; c++)
+          if (k0 + 8 * c < w.rank)
+            wr[c].load(row_of(c) + first);
+      }
+      int i = first;
+      for (; i < whole; i += step) {
+        const int next = i + step < whole ? i + step : first;  // past the end: any step's, which nothing uses
         Split16 xs;
+        float v[8];
+        x[0].get(v);
+        xs.set(0, v);
+        x[1].get(v);
+        xs.set(1, v);
+        x[0].load(x0 + next);
+        x[1].load(x1 + next);
 #pragma unroll
-        for (int c0 = 0; c0 < 8; c0 += kFlight) {
-          Raw8<W> wr[kFlight];
-#pragma unroll
-          for (int c = 0; c < kFlight; c++)
-            if (k0 + 8 * (c0 + c) < w.rank)
-              wr[c].load(A + (long long)min(k0 + 8 * (c0 + c) + g, w.rank - 1) * a.n, i + 8 * q, n1, a_wide);
-          if (c0 == 0) {
-            float v[8];
-            x[0].get(v);
-            xs.set(0, v);
-            x[1].get(v);
-            xs.set(1, v);
+        for (int c = 0; c < 8; c++) {
+          if (k0 + 8 * c < w.rank) {
+            wr[c % kFlight].get(v);
+            product32<kSplit>(sum[c], xs, v);
           }
-#pragma unroll
-          for (int c = 0; c < kFlight; c++)
-            if (k0 + 8 * (c0 + c) < w.rank) {
-              float wv[8];
-              wr[c].get(wv);
-              product32<kSplit>(sum[c0 + c], xs, wv);
-            }
+          const int ahead = (c + kFlight) % 8;
+          if (k0 + 8 * ahead < w.rank)
+            wr[c % kFlight].load(row_of(ahead) + (c + kFlight < 8 ? i : next));
         }
+      }
+      for (; i < n1; i += step) {
+        Split16 xs;
+        float v[8];
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          x[r].load(r ? x1 : x0, i, n1 - 8 * q, x_wide);
+          x[r].get(v);
+          xs.set(r, v);
+        }
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+          if (k0 + 8 * c < w.rank) {
+            wr[0].load(A + (size_t)min(k0 + 8 * c + g, r1) * a.n + 8 * q, i, n1 - 8 * q, a_wide);
+            wr[0].get(v);
+            product32<kSplit>(sum[c], xs, v);
+          }
       }
     }
     // The last way's sums, then the others' on top, into this CTA's partial vectors.
@@ -426,75 +488,101 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
   const bool b_wide = aligned16(B) && w.rank % 8 == 0;
   const bool pairs = a.ldo % 2 == 0 && ((uintptr_t)a.out & 7) == 0 && (!a.base || (a.ldb % 2 == 0 && ((uintptr_t)a.base & 7) == 0));
   const long long r0 = t.rows[min(i0, rows - 1)], r1 = t.rows[min(i1, rows - 1)];
-  for (int d = d0 + 32 * way; d < d1; d += 32 * ways) {
-    float sum[4][4];
+  float *const out[2] = {a.out + r0 * a.ldo + 2 * q, a.out + r1 * a.ldo + 2 * q};
+  const float *const base[2] = {a.base ? a.base + r0 * a.ldb + 2 * q : nullptr, a.base ? a.base + r1 * a.ldb + 2 * q : nullptr};
+  // As above: the weights of the first kAhead ranks and the base of the next step come during this one.
+  constexpr int kAhead = 1;
+  const int step = 32 * ways;
+  Raw8<W> wr[kAhead][4];
+  float2 y[4][2];
+  const bool b_whole = b_wide && w.rank == rank32;
+  auto load_b = [&](Raw8<W> &r, int d, int c, int k) {
+    const W *row = B + (size_t)min(d + 8 * c + g, a.d - 1) * w.rank;
+    if (b_whole)
+      r.load(row + min(k, rank32 - 32) + 8 * q);
+    else if (k < rank32)
+      r.load(row, k + 8 * q, w.rank, b_wide);
+  };
+  auto load_base = [&](int d) {
+    const bool whole = pairs && d + 32 <= d1;
 #pragma unroll
-    for (int c = 0; c < 4; c++) {  // the base first: its reads are under way during the products
-      const int i = d + 8 * c + 2 * q;
-      float2 y0 = make_float2(0.0f, 0.0f), y1 = y0;
-      if (a.base) {
-        const float *b0 = a.base + r0 * a.ldb + i, *b1 = a.base + r1 * a.ldb + i;
-        if (pairs && i + 1 < d1) {
-          y0 = *reinterpret_cast<const float2 *>(b0), y1 = *reinterpret_cast<const float2 *>(b1);
-        } else {
-          if (i < d1)
-            y0.x = b0[0], y1.x = b1[0];
-          if (i + 1 < d1)
-            y0.y = b0[1], y1.y = b1[1];
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const float *at = base[r] + d + 8 * c;
+        const int left = d1 - (d + 8 * c + 2 * q);
+        y[c][r] = make_float2(0.0f, 0.0f);
+        if (a.base && whole) {
+          y[c][r] = *reinterpret_cast<const float2 *>(at);
+        } else if (a.base) {
+          y[c][r].x = left > 0 ? at[0] : 0.0f;
+          y[c][r].y = left > 1 ? at[1] : 0.0f;
         }
       }
-      sum[c][0] = y0.x, sum[c][1] = y0.y, sum[c][2] = y1.x, sum[c][3] = y1.y;
-    }
+  };
+  const int first = d0 + 32 * way;
+  if (rank32 && first < d1)
+#pragma unroll
+    for (int k = 0; k < kAhead; k++)
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        load_b(wr[k][c], first, c, 32 * k);
+  if (first < d1)
+    load_base(first);
+  for (int d = first; d < d1; d += step) {
     float prod[4][4];
 #pragma unroll
     for (int c = 0; c < 4; c++)
 #pragma unroll
       for (int i = 0; i < 4; i++)
         prod[c][i] = 0.0f;
-    for (int k = 0; k < rank32; k += 32) {
-      Raw8<W> wr[4];
+    for (int k0 = 0; k0 < rank32; k0 += 32 * kAhead) {
+      const bool last = k0 + 32 * kAhead >= rank32;
 #pragma unroll
-      for (int c = 0; c < 4; c++)
-        wr[c].load(B + (long long)min(d + 8 * c + g, a.d - 1) * w.rank, k + 8 * q, w.rank, b_wide);
-      Split16 hv;
+      for (int n = 0; n < kAhead; n++) {
+        const int k = k0 + 32 * n;
+        if (k >= rank32)
+          break;
+        Split16 hv;
 #pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const int at = (r ? i1 : i0) * hs + k + 8 * q;
+        for (int r = 0; r < 2; r++) {
+          const int at = (r ? i1 : i0) * hs + k + 8 * q;
 #pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(high + at + j), y = *reinterpret_cast<const uint4 *>(low + at + j);
-          hv.hi[r][j] = x.x, hv.hi[r][j + 1] = x.y, hv.hi[r][j + 2] = x.z, hv.hi[r][j + 3] = x.w;
-          hv.lo[r][j] = y.x, hv.lo[r][j + 1] = y.y, hv.lo[r][j + 2] = y.z, hv.lo[r][j + 3] = y.w;
+          for (int j = 0; j < 8; j += 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(high + at + j), z = *reinterpret_cast<const uint4 *>(low + at + j);
+            hv.hi[r][j] = x.x, hv.hi[r][j + 1] = x.y, hv.hi[r][j + 2] = x.z, hv.hi[r][j + 3] = x.w;
+            hv.lo[r][j] = z.x, hv.lo[r][j + 1] = z.y, hv.lo[r][j + 2] = z.z, hv.lo[r][j + 3] = z.w;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          float wv[8];
+          wr[n][c].get(wv);
+          product32<kSplit>(prod[c], hv, wv);
+          load_b(wr[n][c], last ? d + step : d, c, last ? 32 * n : k + 32 * kAhead);
         }
       }
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        float wv[8];
-        wr[c].get(wv);
-        product32<kSplit>(prod[c], hv, wv);
-      }
     }
+    const bool whole = pairs && d + 32 <= d1;
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      const int i = d + 8 * c + 2 * q;
-      float *o0 = a.out + r0 * a.ldo + i, *o1 = a.out + r1 * a.ldo + i;
-      const float y[4] = {sum[c][0] + prod[c][0], sum[c][1] + prod[c][1], sum[c][2] + prod[c][2], sum[c][3] + prod[c][3]};
-      if (pairs && i + 1 < d1) {
-        if (i0 < rows)
-          *reinterpret_cast<float2 *>(o0) = make_float2(y[0], y[1]);
-        if (i1 < rows)
-          *reinterpret_cast<float2 *>(o1) = make_float2(y[2], y[3]);
-      } else {
-        if (i < d1 && i0 < rows)
-          o0[0] = y[0];
-        if (i < d1 && i1 < rows)
-          o1[0] = y[2];
-        if (i + 1 < d1 && i0 < rows)
-          o0[1] = y[1];
-        if (i + 1 < d1 && i1 < rows)
-          o1[1] = y[3];
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const float2 o = make_float2(y[c][r].x + prod[c][2 * r], y[c][r].y + prod[c][2 * r + 1]);
+        float *at = out[r] + d + 8 * c;
+        const int left = (r ? i1 : i0) < rows ? d1 - (d + 8 * c + 2 * q) : 0;
+        if (whole) {
+          if (left)
+            *reinterpret_cast<float2 *>(at) = o;
+        } else {
+          if (left > 0)
+            at[0] = o.x;
+          if (left > 1)
+            at[1] = o.y;
+        }
       }
-    }
+    if (d + step < d1)
+      load_base(d + step);
   }
 }
 

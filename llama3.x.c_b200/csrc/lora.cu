@@ -16,6 +16,7 @@
 #include "../../include/kernels_cuda.h"
 #include "common.cuh"
 #include "kernels_cuda_internal.h"
+#include "tcgen05.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -145,139 +146,73 @@ __global__ void __launch_bounds__(kThreads) lora_row_kernel(const LoraArgs a, in
 // once. Every CTA finds its tile in the index array by itself (a histogram of the adapters, then the tile's rows in
 // order): no sorting launch and no workspace. Rows without an adapter form tiles too, which copy their base.
 //
-// Products on mma.sync m16n8k8 tf32 with both operands' 24 bits kept: x = hi + lo with hi its upper 11 bits, bf16 and
-// fp16 weights are exact in tf32, fp32 ones split like x: hi w + lo w (+ hi w_lo), off by 2^-22 of a product. The tensor
-// core's sums truncate, so they run over 32 elements only and are added up in fp32 registers. The k index of a
-// fragment is free as long as both operands agree: a lane's two fragment columns of four steps are eight neighbouring
-// elements, one 16- or 32-byte read, without a pass through shared memory.
+// Both products run on tcgen05 with the weights as the M operand, as they lie in memory for bf16, and the tile's vectors
+// as the N operand: D = A x' is [ranks][rows], then D = B h' [128 outputs][rows], whose lanes are neighbouring outputs
+// of one row for the epilogue's reads and writes. fp32 values are three bf16 parts (24 bits: x = x0 + x1 + x2 with no
+// scaling), fp16 weights two, fp32 weights three; a product is the sum of the parts' products up to 2^-24 of it
+// (x_i w_j with i + j <= 2). The tensor cores' sums truncate: in the first product, whose sums are long, the small
+// parts' sums have an accumulator of their own, so that the large one's is cut once for sixteen elements only.
 constexpr int kTileRows = 64;
+constexpr int kTileRank = 128;       // ranks the tile kernel takes
 constexpr int kMaxBins = 2048;       // adapters + 1 of the histogram
 constexpr int kMaxTileRows = 16384;  // rows of a launch: every CTA reads their indices
+constexpr int kStep = 64;            // elements of n a step: one 128-byte row of bf16
+constexpr uint32_t kTmemCols = 128;  // two accumulators of 64 rows
 
-__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_tf32_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
-}
+// Parts of a weight.
+template <typename W>
+constexpr int kParts = std::is_same_v<W, __nv_bfloat16> ? 1 : sizeof(W) == 2 ? 2 : 3;
 
-__device__ __forceinline__ uint32_t tf32_hi(float x) { return __float_as_uint(x) & 0xffffe000u; }
-__device__ __forceinline__ uint32_t tf32_lo(float x) { return __float_as_uint(x - __uint_as_float(tf32_hi(x))); }
+__host__ __device__ constexpr int rank_rows(int max_rank) { return max_rank <= 64 ? 64 : 128; }
+__host__ __device__ constexpr int h_stride(int max_rank) { return rank_rows(max_rank) + 4; }
 
-// This lane's eight elements of rows g and g + 8, split.
-struct Split16 {
-  uint32_t hi[2][8], lo[2][8];
-  __device__ __forceinline__ void set(int r, const float (&v)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; j++)
-      hi[r][j] = tf32_hi(v[j]), lo[r][j] = tf32_lo(v[j]);
+// Shared memory: `work` holds two stages of the first product (weights, then vectors), then the partial vectors, then
+// one or two weight tiles of the second product; behind it the operand of the vectors h and this CTA's own rows of h.
+template <typename W>
+struct TileSmem {
+  int stage, tile, tiles, work, operand, total;
+  __host__ __device__ explicit TileSmem(int max_rank) {
+    const int r = rank_rows(max_rank);
+    stage = kParts<W> * r * 128 + 3 * kTileRows * 128;
+    tile = kParts<W> * 128 * r * 2;
+    work = 2 * stage;
+    tiles = 2 * tile <= work ? 2 : 1;
+    if (tile > work)
+      work = tile;
+    operand = 3 * kTileRows * r * 2;
+    total = work + operand + kTileRows / 8 * h_stride(max_rank) * 4 + 1024;
   }
 };
 
-// Values 2 j and 2 j + 1 of words u.
-template <typename W>
-__device__ __forceinline__ void two(const unsigned *u, int j, float &x, float &y) {
-  if constexpr (sizeof(W) == 4) {
-    x = __uint_as_float(u[2 * j]), y = __uint_as_float(u[2 * j + 1]);
-  } else if constexpr (std::is_same_v<W, __nv_bfloat16>) {
-    x = __uint_as_float(u[j] << 16), y = __uint_as_float(u[j] & 0xffff0000u);
-  } else {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[j]));
-    x = f.x, y = f.y;
-  }
-}
-
-// Eight elements of a row as they lie in memory, so that many can be under way.
-template <typename W>
-struct Raw8 {
-  uint4 v[sizeof(W) / 2];
-
-  // Whole groups of eight at 16-byte addresses.
-  __device__ __forceinline__ void load(const W *at) {
-#pragma unroll
-    for (int j = 0; j < (int)(sizeof(W) / 2); j++)
-      v[j] = __ldg(reinterpret_cast<const uint4 *>(at) + j);
-  }
-  // From element i on, zeros from `end` on. `wide`: as above.
-  __device__ __forceinline__ void load(const W *row, int i, int end, bool wide) {
-    if (wide && i + 8 <= end) {
-#pragma unroll
-      for (int j = 0; j < (int)(sizeof(W) / 2); j++)
-        v[j] = __ldg(reinterpret_cast<const uint4 *>(row + i) + j);
-    } else {
-      W *at = reinterpret_cast<W *>(v);
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-        at[j] = i + j < end ? row[i + j] : W(0.0f);
-    }
-  }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    const unsigned *u = reinterpret_cast<const unsigned *>(v);
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      two<W>(u, j, f[2 * j], f[2 * j + 1]);
-  }
-};
-
-// 16 rows x 8 columns += 32 elements of the 16 rows times those of the 8 columns (this lane's eight of column g).
-// SPLIT: the weights have more bits than tf32.
-template <bool SPLIT>
-__device__ __forceinline__ void product32(float (&sum)[4], const Split16 &x, const float (&w)[8]) {
-  float d[4], small[4];  // two chains of MMAs
-#pragma unroll
-  for (int s = 0; s < 4; s++) {
-    const int e = 2 * s;
-    const uint32_t lo[4] = {x.lo[0][e], x.lo[1][e], x.lo[0][e + 1], x.lo[1][e + 1]};
-    const uint32_t hi[4] = {x.hi[0][e], x.hi[1][e], x.hi[0][e + 1], x.hi[1][e + 1]};
-    const uint32_t b0 = SPLIT ? tf32_hi(w[e]) : __float_as_uint(w[e]);
-    const uint32_t b1 = SPLIT ? tf32_hi(w[e + 1]) : __float_as_uint(w[e + 1]);
-    if (s == 0) {
-      mma_tf32_first(small, lo, b0, b1);
-      mma_tf32_first(d, hi, b0, b1);
-    } else {
-      mma_tf32(small, lo, b0, b1);
-      mma_tf32(d, hi, b0, b1);
-    }
-    if (SPLIT)
-      mma_tf32(small, hi, tf32_lo(w[e]), tf32_lo(w[e + 1]));
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-    sum[i] += d[i] + small[i];
-}
-
-// The cluster's tile: its adapter (`count`: rows without one) and its rows in order. False: no such tile.
 struct LoraTile {
-  int bins[kMaxBins];
+  uint64_t bar[2];
+  uint32_t tmem;
+  int abort_flag;
   int rows[kTileRows];
   int warp_sums[kWarps];
-  int adapter, part, n;
+  int adapter, part, n;  // the cluster's tile: its adapter (`count`: rows without one) and its rows in order
 };
 
-__device__ bool find_tile(const LoraArgs &a, LoraTile *t, int tile) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bins = a.count + 1;
+// False: no such tile. bins: kMaxBins words.
+__device__ bool find_tile(const LoraArgs &a, LoraTile *t, int *bins, int tile) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, count = a.count + 1;
   auto bin_of = [&](int r) {
     const int id = a.index[r];
     return id >= 0 && id < a.count ? id : a.count;
   };
-  for (int i = threadIdx.x; i < bins; i += kThreads)
-    t->bins[i] = 0;
+  for (int i = threadIdx.x; i < count; i += kThreads)
+    bins[i] = 0;
   if (threadIdx.x == 0)
     t->adapter = -1;
   __syncthreads();
+#pragma unroll 4
   for (int r = threadIdx.x; r < a.rows; r += kThreads)
-    atomicAdd(&t->bins[bin_of(r)], 1);
+    atomicAdd(&bins[bin_of(r)], 1);
   __syncthreads();
   // The adapter whose tiles hold number `tile`: a running sum over the adapters' tiles.
   int before = 0;
-  for (int i0 = 0; i0 < bins; i0 += kThreads) {
-    const int i = i0 + threadIdx.x, tiles = i < bins ? (t->bins[i] + kTileRows - 1) / kTileRows : 0;
+  for (int i0 = 0; i0 < count; i0 += kThreads) {
+    const int i = i0 + threadIdx.x, tiles = i < count ? (bins[i] + kTileRows - 1) / kTileRows : 0;
     int upto = tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -297,7 +232,7 @@ __device__ bool find_tile(const LoraArgs &a, LoraTile *t, int tile) {
     if (tile >= before + upto - tiles && tile < before + upto) {
       t->adapter = i;
       t->part = tile - (before + upto - tiles);
-      t->n = min(kTileRows, t->bins[i] - t->part * kTileRows);
+      t->n = min(kTileRows, bins[i] - t->part * kTileRows);
     }
     before += all;
     __syncthreads();
@@ -307,6 +242,7 @@ __device__ bool find_tile(const LoraArgs &a, LoraTile *t, int tile) {
   // Its rows: every thread a run of neighbouring rows, ranked by the matches before it.
   const int per = (a.rows + kThreads - 1) / kThreads, r0 = min((int)threadIdx.x * per, a.rows), r1 = min(r0 + per, a.rows);
   int mine = 0;
+#pragma unroll 4
   for (int r = r0; r < r1; r++)
     mine += bin_of(r) == t->adapter;
   int upto = mine;
@@ -322,36 +258,130 @@ __device__ bool find_tile(const LoraArgs &a, LoraTile *t, int tile) {
   int rank = upto - mine - t->part * kTileRows;
   for (int w = 0; w < warp; w++)
     rank += t->warp_sums[w];
-  for (int r = r0; r < r1; r++)
-    if (bin_of(r) == t->adapter) {
-      if (rank >= 0 && rank < kTileRows)
-        t->rows[rank] = r;
-      rank++;
-    }
+  if (mine && rank < kTileRows && rank + mine > 0)
+    for (int r = r0; r < r1; r++)
+      if (bin_of(r) == t->adapter) {
+        if (rank >= 0 && rank < kTileRows)
+          t->rows[rank] = r;
+        rank++;
+      }
   __syncthreads();
   return true;
 }
 
-// Floats of a row of the tile's vectors: the rank in whole 32s, and 4 so that neighbouring rows lie in other banks.
-__host__ __device__ constexpr int h_stride(int max_rank) { return (max_rank + 31) / 32 * 32 + 4; }
+// kind::f16 instruction descriptor: bf16 A and B, both K-major, fp32 accumulators, M x N.
+__host__ __device__ constexpr uint32_t umma_idesc_bf16(int m, int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+
+// A CTA's wait for its MMAs, with one answer for a warp's lanes: false once any wait of the CTA has given up.
+__device__ __forceinline__ bool tile_wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    ok = *abort_flag == 0;
+    if (ok && !mbar_wait_bounded(bar, parity)) {
+      *abort_flag = 1;
+      ok = false;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+// Two values as N packed bf16 parts.
+template <int N>
+__device__ __forceinline__ void parts2(float x, float y, uint32_t (&p)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    p[i] = *reinterpret_cast<const uint32_t *>(&h);
+    if (i + 1 < N) {
+      x -= __uint_as_float(p[i] << 16);
+      y -= __uint_as_float(p[i] & 0xffff0000u);
+    }
+  }
+}
+
+// Byte offset of element (row, col) of a K-major operand of 128-byte rows in the 128-byte swizzle, `rows` rows to a
+// block of 64 columns.
+__device__ __forceinline__ uint32_t operand_at(int rows, int row, int col) {
+  return (col >> 6) * rows * 128 + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
+}
+
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Elements [c0, c0 + cols) of rows [0, rows) of a row-major weight matrix (row stride ld) as operand parts of `high`
+// rows, `bytes` apart; zeros from column `end` on. cols a multiple of 8. bf16 rows at 16-byte addresses are copied
+// asynchronously.
+template <typename W>
+__device__ __forceinline__ void weight_operand(uint8_t *at, int bytes, int high, const W *w, size_t ld, int rows, int c0,
+                                               int cols, int end, bool wide) {
+  const int per = cols / 8;
+  for (int id = threadIdx.x; id < rows * per; id += kThreads) {
+    const int row = id / per, c = (id - row * per) * 8;
+    uint8_t *dst = at + operand_at(high, row, c);
+    const W *src = w + row * ld + c0 + c;
+    if constexpr (kParts<W> == 1) {
+      if (wide) {
+        copy16(dst, c0 + c < end ? src : w, c0 + c < end);
+        continue;
+      }
+    }
+    float v[8];
+    if (wide && c0 + c < end) {
+      load8(src, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        v[j] = c0 + c + j < end ? to_float(src[j]) : 0.0f;
+    }
+    uint32_t p[4][kParts<W>];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      parts2(v[2 * j], v[2 * j + 1], p[j]);
+#pragma unroll
+    for (int i = 0; i < kParts<W>; i++)
+      *reinterpret_cast<uint4 *>(dst + i * bytes) = make_uint4(p[0][i], p[1][i], p[2][i], p[3][i]);
+  }
+}
 
 // parts clusters share a tile: each computes its vectors and takes a part of d.
 template <typename W>
 __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a, int parts) {
-  extern __shared__ __align__(16) float smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ LoraTile t;
-  constexpr bool kSplit = sizeof(W) == 4;
-  constexpr int kFlight = kSplit ? 2 : 4;  // column groups whose weights are under way at once
+  constexpr int P = kParts<W>;
+  const TileSmem<W> L(a.max_rank);
+  const int rank_high = rank_rows(a.max_rank), hs = h_stride(a.max_rank);
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank(), id = blockIdx.x / ctas;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int *abort_flag = &t.abort_flag;
+  if (threadIdx.x == 0) {
+    mbar_init(&t.bar[0], 1);
+    mbar_init(&t.bar[1], 1);
+    t.abort_flag = 0;
+    fence_mbar_init();
+  }
   pdl_wait();
   pdl_launch_dependents();
-  if (!find_tile(a, &t, id / parts))
+  if (!find_tile(a, &t, reinterpret_cast<int *>(smem), id / parts))
     return;  // the whole cluster
-  const int part = id % parts, rows = t.n, hs = h_stride(a.max_rank);
-  // [64][hs] each: this CTA's partial vectors (then the low parts), the vectors, their high parts.
-  float *partial = smem, *h = smem + kTileRows * hs, *high = h + kTileRows * hs, *low = partial;
+  if (warp == 0)
+    tmem_alloc(&t.tmem, kTmemCols);
+  const int part = id % parts, rows = t.n, n16 = (rows + 15) / 16 * 16;
   LoraAdapter w = {nullptr, nullptr, 0, 0.0f};
   bool bad = false;
   if (t.adapter < a.count) {
@@ -367,222 +397,236 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
       kc_raise(KC_ERR_BAD_ARGS);
   }
   const W *A = static_cast<const W *>(w.a), *B = static_cast<const W *>(w.b);
-  const int rank32 = (w.rank + 31) / 32 * 32;
-  // This warp's 16 rows, and its share of the work along n or d: the warps that a small tile leaves over take shares.
-  const int groups = rows > 32 ? 4 : rows > 16 ? 2 : 1, ways = kWarps / groups, rg = warp % groups, way = warp / groups;
-  const int i0 = 16 * rg + g, i1 = i0 + 8;
-  const bool busy = 16 * rg < rows;
+  const int rank16 = (w.rank + 15) / 16 * 16;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = t.tmem;
+  uint8_t *operand = smem + L.work;
+  float *partial = reinterpret_cast<float *>(smem), *own_h = reinterpret_cast<float *>(operand + L.operand);
+  int phase[2] = {0, 0};  // of the two barriers, the same in all threads
+  bool ok = true;
 
-  // A x: this CTA's slice of n in steps of 32, the ways in turn; 64 rows of A at a time.
-  const int n_slice = ((a.n + ctas - 1) / ctas + 31) / 32 * 32;
-  const int n0 = min(rank * n_slice, a.n), n1 = min(n0 + n_slice, a.n);
-  const bool x_wide = aligned16(a.x) && a.ldx % 4 == 0, a_wide = aligned16(A) && a.n % 8 == 0;
-  for (int k0 = 0; k0 < w.rank; k0 += 64) {
-    float sum[8][4];
+  // A x over this CTA's slice of n.
+  const int n_slice = ((a.n + ctas - 1) / ctas + kStep - 1) / kStep * kStep;
+  const int n0 = min(rank * n_slice, a.n), n1 = min(n0 + n_slice, a.n), steps = w.rank ? (n1 - n0 + kStep - 1) / kStep : 0;
+  const bool x_wide = aligned16(a.x) && a.ldx % 4 == 0 && a.n % 4 == 0, a_wide = aligned16(A) && a.n % 8 == 0;
+  const int a_bytes = rank_high * 128, x_bytes = kTileRows * 128;
+  if (steps) {
+    // This thread's share of a step's vectors: four neighbouring elements of rows r0, r0 + 16, ...
+    const int r0 = threadIdx.x >> 4, c0 = (threadIdx.x & 15) * 4;
+    const float *src[4];
+    float4 x[2][4];
 #pragma unroll
-    for (int c = 0; c < 8; c++)
+    for (int p = 0; p < 4; p++)
+      src[p] = a.x + (long long)t.rows[min(r0 + 16 * p, rows - 1)] * a.ldx + c0;
+    auto load_x = [&](float4 (&v)[4], int j) {
+      const int c = n0 + j * kStep;
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        sum[c][i] = 0.0f;
-    if (busy) {
-      const float *x0 = a.x + (long long)t.rows[min(i0, rows - 1)] * a.ldx;
-      const float *x1 = a.x + (long long)t.rows[min(i1, rows - 1)] * a.ldx;
-      // Whole steps first: every register is loaded again, for a step or half a step ahead, as soon as its value is
-      // used.
-      const int r1 = w.rank - 1, step = 32 * ways, first = n0 + 32 * way;
-      const int whole = x_wide && a_wide && w.rank % 8 == 0 ? n1 - 31 : 0;  // steps that start below it
-      const W *rows_a = A + (size_t)min(k0 + g, r1) * a.n + 8 * q;
-      const size_t rows8 = (size_t)8 * a.n;
-      auto row_of = [&](int c) { return rows_a + c * rows8; };
-      Raw8<float> x[2];
-      Raw8<W> wr[kFlight];
-      x0 += 8 * q, x1 += 8 * q;
-      if (first < whole) {
-        x[0].load(x0 + first);
-        x[1].load(x1 + first);
-#pragma unroll
-        for (int c = 0; c < kFlight; c++)
-          if (k0 + 8 * c < w.rank)
-            wr[c].load(row_of(c) + first);
-      }
-      int i = first;
-      for (; i < whole; i += step) {
-        const int next = i + step < whole ? i + step : first;  // past the end: any step's, which nothing uses
-        Split16 xs;
-        float v[8];
-        x[0].get(v);
-        xs.set(0, v);
-        x[1].get(v);
-        xs.set(1, v);
-        x[0].load(x0 + next);
-        x[1].load(x1 + next);
-#pragma unroll
-        for (int c = 0; c < 8; c++) {
-          if (k0 + 8 * c < w.rank) {
-            wr[c % kFlight].get(v);
-            product32<kSplit>(sum[c], xs, v);
-          }
-          const int ahead = (c + kFlight) % 8;
-          if (k0 + 8 * ahead < w.rank)
-            wr[c % kFlight].load(row_of(ahead) + (c + kFlight < 8 ? i : next));
+      for (int p = 0; p < 4; p++) {
+        v[p] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (j >= steps || r0 + 16 * p >= rows)
+          continue;
+        if (x_wide) {
+          if (c + c0 < n1)
+            v[p] = __ldcg(reinterpret_cast<const float4 *>(src[p] + c));
+        } else {
+          v[p].x = c + c0 < n1 ? src[p][c] : 0.0f;
+          v[p].y = c + c0 + 1 < n1 ? src[p][c + 1] : 0.0f;
+          v[p].z = c + c0 + 2 < n1 ? src[p][c + 2] : 0.0f;
+          v[p].w = c + c0 + 3 < n1 ? src[p][c + 3] : 0.0f;
         }
       }
-      for (; i < n1; i += step) {
-        Split16 xs;
-        float v[8];
+    };
+    auto weights = [&](int j) {
+      weight_operand(smem + (j & 1) * L.stage, a_bytes, rank_high, A, (size_t)a.n, w.rank, n0 + j * kStep, kStep, n1, a_wide);
+    };
+    const uint32_t idesc = umma_idesc_bf16(128, n16);
+    auto step = [&](float4 (&v)[4], int j) {
+      uint8_t *stage = smem + (j & 1) * L.stage, *xs = stage + P * a_bytes;
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-          x[r].load(r ? x1 : x0, i, n1 - 8 * q, x_wide);
-          x[r].get(v);
-          xs.set(r, v);
+      for (int p = 0; p < 4; p++)
+        if (16 * p < n16) {
+          uint32_t p0[3], p1[3];
+          parts2(v[p].x, v[p].y, p0);
+          parts2(v[p].z, v[p].w, p1);
+          uint8_t *dst = xs + operand_at(kTileRows, r0 + 16 * p, c0);
+#pragma unroll
+          for (int i = 0; i < 3; i++)
+            *reinterpret_cast<uint2 *>(dst + i * x_bytes) = make_uint2(p0[i], p1[i]);
         }
-#pragma unroll
-        for (int c = 0; c < 8; c++)
-          if (k0 + 8 * c < w.rank) {
-            wr[0].load(A + (size_t)min(k0 + 8 * c + g, r1) * a.n + 8 * q, i, n1 - 8 * q, a_wide);
-            wr[0].get(v);
-            product32<kSplit>(sum[c], xs, v);
-          }
-      }
-    }
-    // The last way's sums, then the others' on top, into this CTA's partial vectors.
-    for (int turn = ways - 1; turn >= 0; turn--) {
-      if (busy && way == turn)
-#pragma unroll
-        for (int c = 0; c < 8; c++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int k = k0 + 8 * c + 2 * q + (i & 1);
-            float *at = partial + (i < 2 ? i0 : i1) * hs + k;
-            if (k < rank32)
-              *at = k >= w.rank ? 0.0f : turn == ways - 1 ? sum[c][i] : *at + sum[c][i];
-          }
+      load_x(v, j + 2);
+      copies_done();
+      fence_proxy_async_smem();
       __syncthreads();
+      if (warp == 0 && ok) {
+        if (lane == 0) {
+          const uint64_t ad = umma_desc_sw128(stage), bd = umma_desc_sw128(xs);
+#pragma unroll
+          for (int s = 2; s >= 0; s--)
+#pragma unroll
+            for (int i = 0; i < P; i++) {  // part i of the weights, s - i of the vectors
+              if (i > s)
+                continue;
+#pragma unroll
+              for (int k = 0; k < kStep / 16; k++)
+                umma_bf16(tmem + (s ? 64 : 0), ad + (i * a_bytes + 32 * k) / 16, bd + ((s - i) * x_bytes + 32 * k) / 16,
+                          idesc, j > 0 || k > 0 || (s ? s < 2 || i > 0 : false));
+            }
+          umma_commit(&t.bar[j & 1]);
+        }
+        __syncwarp();
+      }
+      if (j + 1 < steps) {  // the other stage is free once the MMAs of the step before are done
+        if (j > 0) {
+          ok &= tile_wait(&t.bar[(j & 1) ^ 1], phase[(j & 1) ^ 1] & 1, abort_flag);
+          phase[(j & 1) ^ 1]++;
+        }
+        weights(j + 1);
+      }
+    };
+    weights(0);
+    load_x(x[0], 0);
+    load_x(x[1], 1);
+    for (int j = 0; j < steps; j += 2) {
+      step(x[0], j);
+      if (j + 1 < steps)
+        step(x[1], j + 1);
     }
+    // The last two steps' MMAs.
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int uses = (steps + 1 - i) / 2;
+      for (; phase[i] < uses; phase[i]++)
+        ok &= tile_wait(&t.bar[i], phase[i] & 1, abort_flag);
+    }
+    __syncthreads();
+    tc_fence_after();
+    // Lanes are ranks, columns rows: into this CTA's partial vectors, 32 columns for each half of the warps.
+    const int k = 32 * (warp & 3) + lane, column = 32 * (warp >> 2);
+    if (32 * (warp & 3) < rank16 && column < n16) {
+      const uint32_t from = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + column;
+#pragma unroll
+      for (int c = 0; c < 32; c += 16) {
+        uint32_t d[16], e[16];
+        tmem_ld16(from + c, d);
+        tmem_ld16(from + 64 + c, e);
+        tmem_wait_ld();
+        if (k < rank16)
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            partial[(column + c + i) * hs + k] =
+                k < w.rank ? __uint_as_float(d[i]) + __uint_as_float(e[i]) : 0.0f;
+      }
+    }
+    tc_fence_before();
+  } else {
+    for (int e = threadIdx.x; e < rows * rank16; e += kThreads)
+      partial[e / rank16 * hs + e % rank16] = 0.0f;
   }
-  // The cluster's sums: CTA c adds up its share of the rows from all CTAs in their order, then everyone fetches them.
+  // The cluster's sums: CTA c adds up its share of the rows from all CTAs in their order, then everyone fetches them as
+  // the second product's operand.
   cluster.sync();
   const int own = (rows - rank + ctas - 1) / ctas;  // rows rank, rank + ctas, ...
-  for (int e = threadIdx.x; e < own * rank32; e += kThreads) {
-    const int n = e / rank32, at = (rank + n * ctas) * hs + e - n * rank32;
+  for (int e = threadIdx.x; e < own * rank16; e += kThreads) {
+    const int n = e / rank16, k = e - n * rank16;
     float s = 0.0f;
 #pragma unroll 8
     for (int c = 0; c < ctas; c++)
-      s += *cluster.map_shared_rank(&partial[at], c);
-    h[at] = s * w.scale;
+      s += *cluster.map_shared_rank(&partial[(rank + n * ctas) * hs + k], c);
+    own_h[n * hs + k] = s * w.scale;
   }
   cluster.sync();
+  const int h_bytes = kTileRows * rank_high * 2, pairs = rank16 / 2;
 #pragma unroll 4
-  for (int e = threadIdx.x; e < rows * rank32; e += kThreads) {
-    const int i = e / rank32, at = i * hs + e - i * rank32;
-    const float v = *cluster.map_shared_rank(&h[at], i % ctas);
-    high[at] = __uint_as_float(tf32_hi(v)), low[at] = __uint_as_float(tf32_lo(v));
+  for (int e = threadIdx.x; e < n16 * pairs; e += kThreads) {
+    const int i = e / pairs, k = 2 * (e - i * pairs);
+    float2 v = make_float2(0.0f, 0.0f);
+    if (i < rows)
+      v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&own_h[i / ctas * hs + k], i % ctas));
+    uint32_t p[3];
+    parts2(v.x, v.y, p);
+    uint8_t *dst = operand + operand_at(kTileRows, i, k);
+#pragma unroll
+    for (int n = 0; n < 3; n++)
+      *reinterpret_cast<uint32_t *>(dst + n * h_bytes) = p[n];
   }
   cluster.sync();  // everything is fetched: a CTA may leave
-  if (!busy)
-    return;
 
-  // B h: this CTA's slice of d, 32 columns at a time, the ways in turn.
+  // B h over this CTA's slice of d, 128 outputs at a time.
   const int d_all = parts * ctas, d_slice = ((a.d + d_all - 1) / d_all + 31) / 32 * 32;
-  const int d0 = min((part * ctas + rank) * d_slice, a.d), d1 = min(d0 + d_slice, a.d);
+  const int d0 = min((part * ctas + rank) * d_slice, a.d), d1 = min(d0 + d_slice, a.d), tiles = (d1 - d0 + 127) / 128;
   const bool b_wide = aligned16(B) && w.rank % 8 == 0;
-  const bool pairs = a.ldo % 2 == 0 && ((uintptr_t)a.out & 7) == 0 && (!a.base || (a.ldb % 2 == 0 && ((uintptr_t)a.base & 7) == 0));
-  const long long r0 = t.rows[min(i0, rows - 1)], r1 = t.rows[min(i1, rows - 1)];
-  float *const out[2] = {a.out + r0 * a.ldo + 2 * q, a.out + r1 * a.ldo + 2 * q};
-  const float *const base[2] = {a.base ? a.base + r0 * a.ldb + 2 * q : nullptr, a.base ? a.base + r1 * a.ldb + 2 * q : nullptr};
-  // As above: the weights of the first kAhead ranks and the base of the next step come during this one.
-  constexpr int kAhead = 1;
-  const int step = 32 * ways;
-  Raw8<W> wr[kAhead][4];
-  float2 y[4][2];
-  const bool b_whole = b_wide && w.rank == rank32;
-  auto load_b = [&](Raw8<W> &r, int d, int c, int k) {
-    const W *row = B + (size_t)min(d + 8 * c + g, a.d - 1) * w.rank;
-    if (b_whole)
-      r.load(row + min(k, rank32 - 32) + 8 * q);
-    else if (k < rank32)
-      r.load(row, k + 8 * q, w.rank, b_wide);
+  const int b_bytes = 128 * rank_high * 2;
+  const uint32_t idesc = umma_idesc_bf16(128, n16);
+  const int column = 32 * (warp >> 2), lane_d = 32 * (warp & 3) + lane;
+  auto weights = [&](int j) {
+    if (rank16)
+      weight_operand(smem + (j & (L.tiles - 1)) * L.tile, b_bytes, 128, B + (size_t)(d0 + 128 * j) * w.rank, (size_t)w.rank,
+                     min(128, d1 - d0 - 128 * j), 0, rank16, w.rank, b_wide);
   };
-  auto load_base = [&](int d) {
-    const bool whole = pairs && d + 32 <= d1;
+  if (L.tiles == 2 && tiles)
+    weights(0);
+  phase[0] &= 1, phase[1] &= 1;
+  for (int j = 0; j < tiles; j++) {
+    if (L.tiles == 1)
+      weights(j);
+    copies_done();
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0 && rank16 && ok) {
+      if (lane == 0) {
+        tc_fence_after();
+        const uint64_t ad = umma_desc_sw128(smem + (j & (L.tiles - 1)) * L.tile), bd = umma_desc_sw128(operand);
+        bool more = false;
 #pragma unroll
-    for (int c = 0; c < 4; c++)
+        for (int s = 2; s >= 0; s--)
 #pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const float *at = base[r] + d + 8 * c;
-        const int left = d1 - (d + 8 * c + 2 * q);
-        y[c][r] = make_float2(0.0f, 0.0f);
-        if (a.base && whole) {
-          y[c][r] = *reinterpret_cast<const float2 *>(at);
-        } else if (a.base) {
-          y[c][r].x = left > 0 ? at[0] : 0.0f;
-          y[c][r].y = left > 1 ? at[1] : 0.0f;
-        }
-      }
-  };
-  const int first = d0 + 32 * way;
-  if (rank32 && first < d1)
-#pragma unroll
-    for (int k = 0; k < kAhead; k++)
-#pragma unroll
-      for (int c = 0; c < 4; c++)
-        load_b(wr[k][c], first, c, 32 * k);
-  if (first < d1)
-    load_base(first);
-  for (int d = first; d < d1; d += step) {
-    float prod[4][4];
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        prod[c][i] = 0.0f;
-    for (int k0 = 0; k0 < rank32; k0 += 32 * kAhead) {
-      const bool last = k0 + 32 * kAhead >= rank32;
-#pragma unroll
-      for (int n = 0; n < kAhead; n++) {
-        const int k = k0 + 32 * n;
-        if (k >= rank32)
-          break;
-        Split16 hv;
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-          const int at = (r ? i1 : i0) * hs + k + 8 * q;
-#pragma unroll
-          for (int j = 0; j < 8; j += 4) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(high + at + j), z = *reinterpret_cast<const uint4 *>(low + at + j);
-            hv.hi[r][j] = x.x, hv.hi[r][j + 1] = x.y, hv.hi[r][j + 2] = x.z, hv.hi[r][j + 3] = x.w;
-            hv.lo[r][j] = z.x, hv.lo[r][j + 1] = z.y, hv.lo[r][j + 2] = z.z, hv.lo[r][j + 3] = z.w;
+          for (int i = 0; i < P; i++) {
+            if (i > s)
+              continue;
+            for (int k = 0; k < rank16 / 16; k++) {
+              umma_bf16(tmem + 64 * (j & 1), ad + (i * b_bytes + (k >> 2) * 128 * 128 + 32 * (k & 3)) / 16,
+                        bd + ((s - i) * h_bytes + (k >> 2) * kTileRows * 128 + 32 * (k & 3)) / 16, idesc, more);
+              more = true;
+            }
           }
-        }
+        umma_commit(&t.bar[j & 1]);
+      }
+      __syncwarp();
+    }
+    // Under the MMAs: the next tile's weights, and this tile's base.
+    if (L.tiles == 2 && j + 1 < tiles)
+      weights(j + 1);
+    const int d = d0 + 128 * j + lane_d;
+    float y[32];
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          float wv[8];
-          wr[n][c].get(wv);
-          product32<kSplit>(prod[c], hv, wv);
-          load_b(wr[n][c], last ? d + step : d, c, last ? 32 * n : k + 32 * kAhead);
-        }
+    for (int i = 0; i < 32; i++)
+      y[i] = a.base && d < d1 && column + i < rows ? a.base[t.rows[min(column + i, rows - 1)] * a.ldb + d] : 0.0f;
+    if (rank16) {
+      ok &= tile_wait(&t.bar[j & 1], phase[j & 1] & 1, abort_flag);
+      phase[j & 1]++;
+      tc_fence_after();
+      if (column < n16) {
+        uint32_t v[32];
+        tmem_ld32(tmem + 64 * (j & 1) + ((uint32_t)(32 * (warp & 3)) << 16) + column, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i++)
+          y[i] += __uint_as_float(v[i]);
       }
     }
-    const bool whole = pairs && d + 32 <= d1;
 #pragma unroll
-    for (int c = 0; c < 4; c++)
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const float2 o = make_float2(y[c][r].x + prod[c][2 * r], y[c][r].y + prod[c][2 * r + 1]);
-        float *at = out[r] + d + 8 * c;
-        const int left = (r ? i1 : i0) < rows ? d1 - (d + 8 * c + 2 * q) : 0;
-        if (whole) {
-          if (left)
-            *reinterpret_cast<float2 *>(at) = o;
-        } else {
-          if (left > 0)
-            at[0] = o.x;
-          if (left > 1)
-            at[1] = o.y;
-        }
-      }
-    if (d + step < d1)
-      load_base(d + step);
+    for (int i = 0; i < 32; i++)
+      if (d < d1 && column + i < rows)
+        a.out[t.rows[column + i] * a.ldo + d] = y[i];
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
   }
 }
 
@@ -607,11 +651,10 @@ template <typename W>
 cudaError_t run(const LoraArgs &a) {
   constexpr int kCtas = 8;
   // Four rows an adapter make a tile worth its search (measured at d = n = 4096, rank 16).
-  if (a.rows < 16 || a.rows < 4 * a.count || a.count >= kMaxBins)
+  if (a.rows < 16 || a.rows < 4 * a.count || a.count >= kMaxBins || a.max_rank > kTileRank)
     return launch<W>(lora_row_kernel<W>, a, (unsigned)a.rows, kCtas, 1, 0);
-  const size_t smem = 3 * sizeof(float) * kTileRows * h_stride(a.max_rank);
-  cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(lora_tile_kernel<W>),
-                                (int)(3 * sizeof(float) * kTileRows * h_stride(kMaxRank)));
+  const size_t smem = TileSmem<W>(a.max_rank).total;
+  cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(lora_tile_kernel<W>), TileSmem<W>(kTileRank).total);
   for (int r = 0; r < a.rows && e == cudaSuccess; r += kMaxTileRows) {
     LoraArgs b = a;
     b.rows = a.rows - r < kMaxTileRows ? a.rows - r : kMaxTileRows;

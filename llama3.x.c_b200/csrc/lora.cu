@@ -166,19 +166,18 @@ constexpr int kParts = std::is_same_v<W, __nv_bfloat16> ? 1 : sizeof(W) == 2 ? 2
 __host__ __device__ constexpr int rank_rows(int max_rank) { return max_rank <= 64 ? 64 : 128; }
 __host__ __device__ constexpr int h_stride(int max_rank) { return rank_rows(max_rank) + 4; }
 
-// Shared memory: `work` holds two stages of the first product (weights, then vectors), then the partial vectors, then
-// one or two weight tiles of the second product; behind it the operand of the vectors h and this CTA's own rows of h.
+// Shared memory: `work` holds two stages of the first product (weights, then vectors), then the partial vectors, then a
+// weight tile of the second product and a tile of outputs; behind it the operand of the vectors h and this CTA's own
+// rows of h.
+constexpr int kOutBytes = kTileRows * 128 * 4;
 template <typename W>
 struct TileSmem {
-  int stage, tile, tiles, work, operand, total;
+  int stage, tile, work, operand, total;
   __host__ __device__ explicit TileSmem(int max_rank) {
     const int r = rank_rows(max_rank);
     stage = kParts<W> * r * 128 + 3 * kTileRows * 128;
     tile = kParts<W> * 128 * r * 2;
-    work = 2 * stage;
-    tiles = 2 * tile <= work ? 2 : 1;
-    if (tile > work)
-      work = tile;
+    work = 2 * stage > tile + kOutBytes ? 2 * stage : tile + kOutBytes;
     operand = 3 * kTileRows * r * 2;
     total = work + operand + kTileRows / 8 * h_stride(max_rank) * 4 + 1024;
   }
@@ -206,8 +205,12 @@ __device__ bool find_tile(const LoraArgs &a, LoraTile *t, int *bins, int tile) {
     t->adapter = -1;
   __syncthreads();
 #pragma unroll 4
-  for (int r = threadIdx.x; r < a.rows; r += kThreads)
-    atomicAdd(&bins[bin_of(r)], 1);
+  for (int r = threadIdx.x; r < a.rows; r += kThreads) {
+    const int bin = bin_of(r);
+    const unsigned same = __match_any_sync(__activemask(), bin);  // one add for neighbours of one adapter
+    if (lane == __ffs(same) - 1)
+      atomicAdd(&bins[bin], __popc(same));
+  }
   __syncthreads();
   // The adapter whose tiles hold number `tile`: a running sum over the adapters' tiles.
   int before = 0;
@@ -315,45 +318,83 @@ __device__ __forceinline__ uint32_t operand_at(int rows, int row, int col) {
   return (col >> 6) * rows * 128 + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
 }
 
-__device__ __forceinline__ void copy16(void *dst, const void *src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// A thread's share of a weight operand: up to N runs of eight neighbouring elements in registers, read ahead of their
+// use. The operand is columns [c0, c0 + 8 per) of `rows` rows of a row-major matrix (row stride ld); zeros from column
+// `end` on.
+template <typename W, int N>
+struct WeightRuns {
+  uint4 v[N][sizeof(W) / 2];
 
-// Elements [c0, c0 + cols) of rows [0, rows) of a row-major weight matrix (row stride ld) as operand parts of `high`
-// rows, `bytes` apart; zeros from column `end` on. cols a multiple of 8. bf16 rows at 16-byte addresses are copied
-// asynchronously.
-template <typename W>
-__device__ __forceinline__ void weight_operand(uint8_t *at, int bytes, int high, const W *w, size_t ld, int rows, int c0,
-                                               int cols, int end, bool wide) {
-  const int per = cols / 8;
-  for (int id = threadIdx.x; id < rows * per; id += kThreads) {
-    const int row = id / per, c = (id - row * per) * 8;
-    uint8_t *dst = at + operand_at(high, row, c);
-    const W *src = w + row * ld + c0 + c;
-    if constexpr (kParts<W> == 1) {
-      if (wide) {
-        copy16(dst, c0 + c < end ? src : w, c0 + c < end);
-        continue;
+  __device__ __forceinline__ void load(int first, const W *w, size_t ld, int rows, int c0, int per, int end, bool wide) {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const int id = first + n * kThreads + threadIdx.x, row = id / per, c = c0 + (id - row * per) * 8;
+      if (row >= rows)
+        break;
+      const W *src = w + row * ld + c;
+      if (wide && c < end) {
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(W) / 2); j++)
+          v[n][j] = __ldg(reinterpret_cast<const uint4 *>(src) + j);
+      } else {
+        W *at = reinterpret_cast<W *>(v[n]);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          at[j] = c + j < end ? src[j] : W(0.0f);
       }
     }
-    float v[8];
-    if (wide && c0 + c < end) {
-      load8(src, v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-        v[j] = c0 + c + j < end ? to_float(src[j]) : 0.0f;
-    }
-    uint32_t p[4][kParts<W>];
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      parts2(v[2 * j], v[2 * j + 1], p[j]);
-#pragma unroll
-    for (int i = 0; i < kParts<W>; i++)
-      *reinterpret_cast<uint4 *>(dst + i * bytes) = make_uint4(p[0][i], p[1][i], p[2][i], p[3][i]);
   }
+  // As operand parts of blocks of `high` rows, `bytes` apart.
+  __device__ __forceinline__ void store(int first, uint8_t *at, int bytes, int high, int rows, int per) const {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const int id = first + n * kThreads + threadIdx.x, row = id / per;
+      if (row >= rows)
+        break;
+      uint8_t *dst = at + operand_at(high, row, (id - row * per) * 8);
+      if constexpr (kParts<W> == 1) {
+        *reinterpret_cast<uint4 *>(dst) = v[n][0];
+      } else {
+        const unsigned *u = reinterpret_cast<const unsigned *>(v[n]);
+        uint32_t p[4][kParts<W>];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          float x, y;
+          if constexpr (sizeof(W) == 4) {
+            x = __uint_as_float(u[2 * j]), y = __uint_as_float(u[2 * j + 1]);
+          } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[j]));
+            x = f.x, y = f.y;
+          }
+          parts2(x, y, p[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < kParts<W>; i++)
+          *reinterpret_cast<uint4 *>(dst + i * bytes) = make_uint4(p[0][i], p[1][i], p[2][i], p[3][i]);
+      }
+    }
+  }
+};
+
+// Four neighbouring floats of a row, `left` of them inside; 16-byte units where `wide`.
+__device__ __forceinline__ float4 read4(const float *p, int left, bool wide) {
+  if (wide && left >= 4)
+    return *reinterpret_cast<const float4 *>(p);
+  return make_float4(left > 0 ? p[0] : 0.0f, left > 1 ? p[1] : 0.0f, left > 2 ? p[2] : 0.0f, left > 3 ? p[3] : 0.0f);
+}
+__device__ __forceinline__ void write4(float *p, float4 v, int left, bool wide) {
+  if (wide && left >= 4) {
+    *reinterpret_cast<float4 *>(p) = v;
+    return;
+  }
+  if (left > 0)
+    p[0] = v.x;
+  if (left > 1)
+    p[1] = v.y;
+  if (left > 2)
+    p[2] = v.z;
+  if (left > 3)
+    p[3] = v.w;
 }
 
 // parts clusters share a tile: each computes its vectors and takes a part of d.
@@ -438,12 +479,19 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         }
       }
     };
-    auto weights = [&](int j) {
-      weight_operand(smem + (j & 1) * L.stage, a_bytes, rank_high, A, (size_t)a.n, w.rank, n0 + j * kStep, kStep, n1, a_wide);
+    // Its share of the weights: two runs a step up to 64 ranks, read a step ahead; the others as they are needed.
+    WeightRuns<W, 2> runs;
+    auto load_w = [&](WeightRuns<W, 2> &r, int first, int j) {
+      r.load(first, A, (size_t)a.n, w.rank, n0 + j * kStep, kStep / 8, n1, a_wide);
     };
     const uint32_t idesc = umma_idesc_bf16(128, n16);
     auto step = [&](float4 (&v)[4], int j) {
-      uint8_t *stage = smem + (j & 1) * L.stage, *xs = stage + P * a_bytes;
+      const int s = j & 1;
+      uint8_t *stage = smem + s * L.stage, *xs = stage + P * a_bytes;
+      if (j > 1) {  // the stage is free once the MMAs of two steps ago are done
+        ok &= tile_wait(&t.bar[s], phase[s] & 1, abort_flag);
+        phase[s]++;
+      }
 #pragma unroll
       for (int p = 0; p < 4; p++)
         if (16 * p < n16) {
@@ -455,37 +503,36 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
           for (int i = 0; i < 3; i++)
             *reinterpret_cast<uint2 *>(dst + i * x_bytes) = make_uint2(p0[i], p1[i]);
         }
-      load_x(v, j + 2);
-      copies_done();
+      runs.store(0, stage, a_bytes, rank_high, w.rank, kStep / 8);
+      if (w.rank > 64) {
+        load_w(runs, 2 * kThreads, j);
+        runs.store(2 * kThreads, stage, a_bytes, rank_high, w.rank, kStep / 8);
+      }
       fence_proxy_async_smem();
       __syncthreads();
       if (warp == 0 && ok) {
         if (lane == 0) {
           const uint64_t ad = umma_desc_sw128(stage), bd = umma_desc_sw128(xs);
 #pragma unroll
-          for (int s = 2; s >= 0; s--)
+          for (int s2 = 2; s2 >= 0; s2--)
 #pragma unroll
-            for (int i = 0; i < P; i++) {  // part i of the weights, s - i of the vectors
-              if (i > s)
+            for (int i = 0; i < P; i++) {  // part i of the weights, s2 - i of the vectors
+              if (i > s2)
                 continue;
 #pragma unroll
               for (int k = 0; k < kStep / 16; k++)
-                umma_bf16(tmem + (s ? 64 : 0), ad + (i * a_bytes + 32 * k) / 16, bd + ((s - i) * x_bytes + 32 * k) / 16,
-                          idesc, j > 0 || k > 0 || (s ? s < 2 || i > 0 : false));
+                umma_bf16(tmem + (s2 ? 64 : 0), ad + (i * a_bytes + 32 * k) / 16, bd + ((s2 - i) * x_bytes + 32 * k) / 16,
+                          idesc, j > 0 || k > 0 || (s2 ? s2 < 2 || i > 0 : false));
             }
-          umma_commit(&t.bar[j & 1]);
+          umma_commit(&t.bar[s]);
         }
         __syncwarp();
       }
-      if (j + 1 < steps) {  // the other stage is free once the MMAs of the step before are done
-        if (j > 0) {
-          ok &= tile_wait(&t.bar[(j & 1) ^ 1], phase[(j & 1) ^ 1] & 1, abort_flag);
-          phase[(j & 1) ^ 1]++;
-        }
-        weights(j + 1);
-      }
+      load_x(v, j + 2);
+      if (j + 1 < steps)
+        load_w(runs, 0, j + 1);
     };
-    weights(0);
+    load_w(runs, 0, 0);
     load_x(x[0], 0);
     load_x(x[1], 1);
     for (int j = 0; j < steps; j += 2) {
@@ -527,29 +574,33 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
   // The cluster's sums: CTA c adds up its share of the rows from all CTAs in their order, then everyone fetches them as
   // the second product's operand.
   cluster.sync();
-  const int own = (rows - rank + ctas - 1) / ctas;  // rows rank, rank + ctas, ...
-  for (int e = threadIdx.x; e < own * rank16; e += kThreads) {
-    const int n = e / rank16, k = e - n * rank16;
-    float s = 0.0f;
+  const int own = (rows - rank + ctas - 1) / ctas;  // rows rank, rank + ctas, ...: a warp each
+  if (warp < own)
+    for (int k = lane; k < rank16; k += 32) {
+      float s = 0.0f;
 #pragma unroll 8
-    for (int c = 0; c < ctas; c++)
-      s += *cluster.map_shared_rank(&partial[(rank + n * ctas) * hs + k], c);
-    own_h[n * hs + k] = s * w.scale;
-  }
+      for (int c = 0; c < ctas; c++)
+        s += *cluster.map_shared_rank(&partial[(rank + warp * ctas) * hs + k], c);
+      own_h[warp * hs + k] = s * w.scale;
+    }
   cluster.sync();
-  const int h_bytes = kTileRows * rank_high * 2, pairs = rank16 / 2;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < n16 * pairs; e += kThreads) {
-    const int i = e / pairs, k = 2 * (e - i * pairs);
-    float2 v = make_float2(0.0f, 0.0f);
-    if (i < rows)
-      v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&own_h[i / ctas * hs + k], i % ctas));
-    uint32_t p[3];
-    parts2(v.x, v.y, p);
-    uint8_t *dst = operand + operand_at(kTileRows, i, k);
+  const int h_bytes = kTileRows * rank_high * 2;
+  for (int k = 2 * lane; k < rank16; k += 64) {
 #pragma unroll
-    for (int n = 0; n < 3; n++)
-      *reinterpret_cast<uint32_t *>(dst + n * h_bytes) = p[n];
+    for (int n = 0; n < kTileRows / kWarps; n++) {
+      const int i = warp + kWarps * n;
+      if (i >= n16)
+        break;
+      float2 v = make_float2(0.0f, 0.0f);
+      if (i < rows)
+        v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&own_h[i / ctas * hs + k], i % ctas));
+      uint32_t p[3];
+      parts2(v.x, v.y, p);
+      uint8_t *dst = operand + operand_at(kTileRows, i, k);
+#pragma unroll
+      for (int j = 0; j < 3; j++)
+        *reinterpret_cast<uint32_t *>(dst + j * h_bytes) = p[j];
+    }
   }
   cluster.sync();  // everything is fetched: a CTA may leave
 
@@ -557,70 +608,91 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
   const int d_all = parts * ctas, d_slice = ((a.d + d_all - 1) / d_all + 31) / 32 * 32;
   const int d0 = min((part * ctas + rank) * d_slice, a.d), d1 = min(d0 + d_slice, a.d), tiles = (d1 - d0 + 127) / 128;
   const bool b_wide = aligned16(B) && w.rank % 8 == 0;
-  const int b_bytes = 128 * rank_high * 2;
+  const int b_bytes = 128 * rank_high * 2, per = rank16 / 8;
   const uint32_t idesc = umma_idesc_bf16(128, n16);
   const int column = 32 * (warp >> 2), lane_d = 32 * (warp & 3) + lane;
-  auto weights = [&](int j) {
-    if (rank16)
-      weight_operand(smem + (j & (L.tiles - 1)) * L.tile, b_bytes, 128, B + (size_t)(d0 + 128 * j) * w.rank, (size_t)w.rank,
-                     min(128, d1 - d0 - 128 * j), 0, rank16, w.rank, b_wide);
+  const bool base_wide = aligned16(a.base) && a.ldb % 4 == 0, out_wide = aligned16(a.out) && a.ldo % 4 == 0;
+  float *tile_out = reinterpret_cast<float *>(smem + L.tile);  // [64][128]
+  // This thread's share of a weight tile: four runs up to 64 ranks, read a tile ahead.
+  WeightRuns<W, 4> runs;
+  auto load_w = [&](int first, int j) {
+    const int d = d0 + 128 * j;
+    if (per && d < d1)
+      runs.load(first, B + (size_t)d * w.rank, (size_t)w.rank, min(128, d1 - d), 0, per, w.rank, b_wide);
   };
-  if (L.tiles == 2 && tiles)
-    weights(0);
-  phase[0] &= 1, phase[1] &= 1;
+  load_w(0, 0);
   for (int j = 0; j < tiles; j++) {
-    if (L.tiles == 1)
-      weights(j);
-    copies_done();
-    fence_proxy_async_smem();
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 0 && rank16 && ok) {
-      if (lane == 0) {
-        tc_fence_after();
-        const uint64_t ad = umma_desc_sw128(smem + (j & (L.tiles - 1)) * L.tile), bd = umma_desc_sw128(operand);
-        bool more = false;
+    const int d = d0 + 128 * j;
+    if (per) {
+      runs.store(0, smem, b_bytes, 128, min(128, d1 - d), per);
+      if (w.rank > 64) {
+        load_w(4 * kThreads, j);
+        runs.store(4 * kThreads, smem, b_bytes, 128, min(128, d1 - d), per);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncthreads();
+      if (warp == 0 && ok) {
+        if (lane == 0) {
+          tc_fence_after();
+          const uint64_t ad = umma_desc_sw128(smem), bd = umma_desc_sw128(operand);
+          bool more = false;
 #pragma unroll
-        for (int s = 2; s >= 0; s--)
+          for (int s = 2; s >= 0; s--)
 #pragma unroll
-          for (int i = 0; i < P; i++) {
-            if (i > s)
-              continue;
-            for (int k = 0; k < rank16 / 16; k++) {
-              umma_bf16(tmem + 64 * (j & 1), ad + (i * b_bytes + (k >> 2) * 128 * 128 + 32 * (k & 3)) / 16,
-                        bd + ((s - i) * h_bytes + (k >> 2) * kTileRows * 128 + 32 * (k & 3)) / 16, idesc, more);
-              more = true;
+            for (int i = 0; i < P; i++) {
+              if (i > s)
+                continue;
+              for (int k = 0; k < rank16 / 16; k++) {
+                umma_bf16(tmem, ad + (i * b_bytes + (k >> 2) * 128 * 128 + 32 * (k & 3)) / 16,
+                          bd + ((s - i) * h_bytes + (k >> 2) * kTileRows * 128 + 32 * (k & 3)) / 16, idesc, more);
+                more = true;
+              }
             }
-          }
-        umma_commit(&t.bar[j & 1]);
+          umma_commit(&t.bar[0]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      load_w(0, j + 1);
     }
-    // Under the MMAs: the next tile's weights, and this tile's base.
-    if (L.tiles == 2 && j + 1 < tiles)
-      weights(j + 1);
-    const int d = d0 + 128 * j + lane_d;
-    float y[32];
+    // Under the MMAs: this tile's base, a warp per row, four outputs a lane.
+    const int at = d + 4 * lane, left = d1 - at;
+    float4 y[kTileRows / kWarps];
 #pragma unroll
-    for (int i = 0; i < 32; i++)
-      y[i] = a.base && d < d1 && column + i < rows ? a.base[t.rows[min(column + i, rows - 1)] * a.ldb + d] : 0.0f;
-    if (rank16) {
-      ok &= tile_wait(&t.bar[j & 1], phase[j & 1] & 1, abort_flag);
-      phase[j & 1]++;
+    for (int n = 0; n < kTileRows / kWarps; n++) {
+      const int i = warp + kWarps * n;
+      y[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (a.base && i < rows)
+        y[n] = read4(a.base + t.rows[i] * a.ldb + at, left, base_wide);
+    }
+    if (per) {
+      ok &= tile_wait(&t.bar[0], phase[0] & 1, abort_flag);
+      phase[0]++;
       tc_fence_after();
-      if (column < n16) {
-        uint32_t v[32];
-        tmem_ld32(tmem + 64 * (j & 1) + ((uint32_t)(32 * (warp & 3)) << 16) + column, v);
-        tmem_wait_ld();
+      if (column < n16) {  // lanes are outputs, columns rows: by way of shared memory
 #pragma unroll
-        for (int i = 0; i < 32; i++)
-          y[i] += __uint_as_float(v[i]);
+        for (int c = 0; c < 32; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + column + c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            tile_out[(column + c + i) * 128 + lane_d] = __uint_as_float(v[i]);
+        }
       }
+      __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < 32; i++)
-      if (d < d1 && column + i < rows)
-        a.out[t.rows[column + i] * a.ldo + d] = y[i];
+    for (int n = 0; n < kTileRows / kWarps; n++) {
+      const int i = warp + kWarps * n;
+      if (i >= rows)
+        break;
+      if (per) {
+        const float4 v = *reinterpret_cast<const float4 *>(tile_out + i * 128 + 4 * lane);
+        y[n].x += v.x, y[n].y += v.y, y[n].z += v.z, y[n].w += v.w;
+      }
+      write4(a.out + t.rows[i] * a.ldo + at, y[n], left, out_wide);
+    }
   }
   tc_fence_before();
   __syncthreads();

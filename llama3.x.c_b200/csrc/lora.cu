@@ -12,6 +12,7 @@
 #include <stdint.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "../../include/kernels_cuda.h"
 #include "common.cuh"
@@ -25,6 +26,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRank = 256;
+constexpr int kCtas = 8;  // of a cluster
 
 struct LoraArgs {
   float *out;
@@ -64,8 +66,8 @@ template <typename W>
 __global__ void __launch_bounds__(kThreads) lora_row_kernel(const LoraArgs a, int) {
   __shared__ float part[kMaxRank], h[kMaxRank];
   cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
-  const int row = blockIdx.x / ctas;
+  constexpr int ctas = kCtas;
+  const int rank = cluster.block_rank(), row = blockIdx.x / ctas;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
@@ -192,25 +194,40 @@ struct LoraTile {
   int adapter, part, n;  // the cluster's tile: its adapter (`count`: rows without one) and its rows in order
 };
 
-// False: no such tile. bins: kMaxBins words.
+// False: no such tile. bins: kMaxBins words. A thread takes a run of neighbouring rows, whose adapters it keeps as long
+// as there are no more than kKept.
 __device__ bool find_tile(const LoraArgs &a, LoraTile *t, int *bins, int tile) {
+  constexpr int kKept = 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, count = a.count + 1;
-  auto bin_of = [&](int r) {
+  const int per = (a.rows + kThreads - 1) / kThreads, r0 = min((int)threadIdx.x * per, a.rows), r1 = min(r0 + per, a.rows);
+  int kept[kKept];
+  auto read = [&](int r) {
     const int id = a.index[r];
     return id >= 0 && id < a.count ? id : a.count;
   };
+#pragma unroll
+  for (int i = 0; i < kKept; i++)
+    kept[i] = r0 + i < r1 ? read(r0 + i) : -1;
   for (int i = threadIdx.x; i < count; i += kThreads)
     bins[i] = 0;
   if (threadIdx.x == 0)
     t->adapter = -1;
   __syncthreads();
-#pragma unroll 4
-  for (int r = threadIdx.x; r < a.rows; r += kThreads) {
-    const int bin = bin_of(r);
-    const unsigned same = __match_any_sync(__activemask(), bin);  // one add for neighbours of one adapter
-    if (lane == __ffs(same) - 1)
-      atomicAdd(&bins[bin], __popc(same));
-  }
+  int last = -1, run = 0;  // neighbours of one adapter are added at once
+  auto add = [&](int bin) {
+    if (bin != last && run)
+      atomicAdd(&bins[last], run);
+    run = bin == last ? run + 1 : 1;
+    last = bin;
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; i++)
+    if (kept[i] >= 0)
+      add(kept[i]);
+  for (int r = r0 + kKept; r < r1; r++)
+    add(read(r));
+  if (run)
+    atomicAdd(&bins[last], run);
   __syncthreads();
   // The adapter whose tiles hold number `tile`: a running sum over the adapters' tiles.
   int before = 0;
@@ -242,12 +259,13 @@ __device__ bool find_tile(const LoraArgs &a, LoraTile *t, int *bins, int tile) {
   }
   if (t->adapter < 0)
     return false;
-  // Its rows: every thread a run of neighbouring rows, ranked by the matches before it.
-  const int per = (a.rows + kThreads - 1) / kThreads, r0 = min((int)threadIdx.x * per, a.rows), r1 = min(r0 + per, a.rows);
+  // Its rows, ranked by the matches before them.
   int mine = 0;
-#pragma unroll 4
-  for (int r = r0; r < r1; r++)
-    mine += bin_of(r) == t->adapter;
+#pragma unroll
+  for (int i = 0; i < kKept; i++)
+    mine += kept[i] == t->adapter;
+  for (int r = r0 + kKept; r < r1; r++)
+    mine += read(r) == t->adapter;
   int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -261,13 +279,20 @@ __device__ bool find_tile(const LoraArgs &a, LoraTile *t, int *bins, int tile) {
   int rank = upto - mine - t->part * kTileRows;
   for (int w = 0; w < warp; w++)
     rank += t->warp_sums[w];
-  if (mine && rank < kTileRows && rank + mine > 0)
-    for (int r = r0; r < r1; r++)
-      if (bin_of(r) == t->adapter) {
-        if (rank >= 0 && rank < kTileRows)
-          t->rows[rank] = r;
-        rank++;
-      }
+  if (mine && rank < kTileRows && rank + mine > 0) {
+    auto take = [&](int r) {
+      if (rank >= 0 && rank < kTileRows)
+        t->rows[rank] = r;
+      rank++;
+    };
+#pragma unroll
+    for (int i = 0; i < kKept; i++)
+      if (kept[i] == t->adapter)
+        take(r0 + i);
+    for (int r = r0 + kKept; r < r1; r++)
+      if (read(r) == t->adapter)
+        take(r);
+  }
   __syncthreads();
   return true;
 }
@@ -407,7 +432,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
   const TileSmem<W> L(a.max_rank);
   const int rank_high = rank_rows(a.max_rank), hs = h_stride(a.max_rank);
   cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = cluster.num_blocks(), rank = cluster.block_rank(), id = blockIdx.x / ctas;
+  constexpr int ctas = kCtas;
+  const int rank = cluster.block_rank(), id = blockIdx.x / ctas;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int *abort_flag = &t.abort_flag;
   if (threadIdx.x == 0) {
@@ -448,9 +474,22 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
   int phase[2] = {0, 0};  // of the two barriers, the same in all threads
   bool ok = true;
 
-  // A x over this CTA's slice of n.
+  // This CTA's slices of n and d. Its vectors' and its base's lines start on their way to L2 now.
+  const int d_all = parts * ctas, d_slice = ((a.d + d_all - 1) / d_all + 31) / 32 * 32;
+  const int d0 = min((part * ctas + rank) * d_slice, a.d), d1 = min(d0 + d_slice, a.d), tiles = (d1 - d0 + 127) / 128;
   const int n_slice = ((a.n + ctas - 1) / ctas + kStep - 1) / kStep * kStep;
   const int n0 = min(rank * n_slice, a.n), n1 = min(n0 + n_slice, a.n), steps = w.rank ? (n1 - n0 + kStep - 1) / kStep : 0;
+  auto prefetch = [&](const float *from, long long ld, int c0, int c1) {
+    const int lines = (c1 - c0 + 31) / 32;
+    for (int e = threadIdx.x; e < rows * lines; e += kThreads) {
+      const int i = e / lines;
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(from + t.rows[i] * ld + c0 + 32 * (e - i * lines)));
+    }
+  };
+  if (w.rank)
+    prefetch(a.x, a.ldx, n0, n1);
+  if (a.base)
+    prefetch(a.base, a.ldb, d0, d1);
   const bool x_wide = aligned16(a.x) && a.ldx % 4 == 0 && a.n % 4 == 0, a_wide = aligned16(A) && a.n % 8 == 0;
   const int a_bytes = rank_high * 128, x_bytes = kTileRows * 128;
   if (steps) {
@@ -479,13 +518,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         }
       }
     };
-    // Its share of the weights: two runs a step up to 64 ranks, read a step ahead; the others as they are needed.
-    WeightRuns<W, 2> runs;
+    // Its share of the weights: two runs a step up to 64 ranks, read two steps ahead; the others as they are needed.
+    WeightRuns<W, 2> runs2[2];
     auto load_w = [&](WeightRuns<W, 2> &r, int first, int j) {
       r.load(first, A, (size_t)a.n, w.rank, n0 + j * kStep, kStep / 8, n1, a_wide);
     };
     const uint32_t idesc = umma_idesc_bf16(128, n16);
-    auto step = [&](float4 (&v)[4], int j) {
+    auto step = [&](float4 (&v)[4], WeightRuns<W, 2> &runs, int j) {
       const int s = j & 1;
       uint8_t *stage = smem + s * L.stage, *xs = stage + P * a_bytes;
       if (j > 1) {  // the stage is free once the MMAs of two steps ago are done
@@ -529,16 +568,18 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         __syncwarp();
       }
       load_x(v, j + 2);
-      if (j + 1 < steps)
-        load_w(runs, 0, j + 1);
+      if (j + 2 < steps)
+        load_w(runs, 0, j + 2);
     };
-    load_w(runs, 0, 0);
+    load_w(runs2[0], 0, 0);
     load_x(x[0], 0);
+    if (steps > 1)
+      load_w(runs2[1], 0, 1);
     load_x(x[1], 1);
     for (int j = 0; j < steps; j += 2) {
-      step(x[0], j);
+      step(x[0], runs2[0], j);
       if (j + 1 < steps)
-        step(x[1], j + 1);
+        step(x[1], runs2[1], j + 1);
     }
     // The last two steps' MMAs.
 #pragma unroll
@@ -602,11 +643,9 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         *reinterpret_cast<uint32_t *>(dst + j * h_bytes) = p[j];
     }
   }
-  cluster.sync();  // everything is fetched: a CTA may leave
+  auto fetched = cluster.barrier_arrive();  // a CTA may leave once everybody has fetched everything
 
   // B h over this CTA's slice of d, 128 outputs at a time.
-  const int d_all = parts * ctas, d_slice = ((a.d + d_all - 1) / d_all + 31) / 32 * 32;
-  const int d0 = min((part * ctas + rank) * d_slice, a.d), d1 = min(d0 + d_slice, a.d), tiles = (d1 - d0 + 127) / 128;
   const bool b_wide = aligned16(B) && w.rank % 8 == 0;
   const int b_bytes = 128 * rank_high * 2, per = rank16 / 8;
   const uint32_t idesc = umma_idesc_bf16(128, n16);
@@ -700,12 +739,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
+  cluster.barrier_wait(std::move(fetched));
 }
 
 template <typename W>
-cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned clusters, int ctas, int parts, size_t smem) {
+cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned clusters, int parts, size_t smem) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(clusters * ctas);
+  cfg.gridDim = dim3(clusters * kCtas);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = kc_stream();
@@ -713,7 +753,7 @@ cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned cl
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = kc_pdl_enabled() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = ctas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  attr[1].val.clusterDim.x = kCtas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, a, parts);
@@ -721,10 +761,9 @@ cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned cl
 
 template <typename W>
 cudaError_t run(const LoraArgs &a) {
-  constexpr int kCtas = 8;
   // Four rows an adapter make a tile worth its search (measured at d = n = 4096, rank 16).
   if (a.rows < 16 || a.rows < 4 * a.count || a.count >= kMaxBins || a.max_rank > kTileRank)
-    return launch<W>(lora_row_kernel<W>, a, (unsigned)a.rows, kCtas, 1, 0);
+    return launch<W>(lora_row_kernel<W>, a, (unsigned)a.rows, 1, 0);
   const size_t smem = TileSmem<W>(a.max_rank).total;
   cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(lora_tile_kernel<W>), TileSmem<W>(kTileRank).total);
   for (int r = 0; r < a.rows && e == cudaSuccess; r += kMaxTileRows) {
@@ -736,7 +775,7 @@ cudaError_t run(const LoraArgs &a) {
     // At most this many tiles: the full ones, and one more for each adapter and the rows without one.
     const int some = b.count + 1 < b.rows ? b.count + 1 : b.rows, tiles = (b.rows - some) / kTileRows + some;
     const int few = kc_device_sms() / (kCtas * tiles), parts = few < 1 ? 1 : few > 4 ? 4 : few;
-    e = launch<W>(lora_tile_kernel<W>, b, (unsigned)(tiles * parts), kCtas, parts, smem);
+    e = launch<W>(lora_tile_kernel<W>, b, (unsigned)(tiles * parts), parts, smem);
     if (e == cudaSuccess && r + kMaxTileRows < a.rows)
       kc_count_launch();
   }

@@ -310,6 +310,12 @@ __device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t adesc, uint64_t b
       : "memory");
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+
 // A CTA's wait for its MMAs, with one answer for a warp's lanes: false once any wait of the CTA has given up.
 __device__ __forceinline__ bool tile_wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
   bool ok = mbar_try_wait(bar, parity);
@@ -344,18 +350,19 @@ __device__ __forceinline__ uint32_t operand_at(int rows, int row, int col) {
 }
 
 // A thread's share of a weight operand: up to N runs of eight neighbouring elements in registers, read ahead of their
-// use. The operand is columns [c0, c0 + 8 per) of `rows` rows of a row-major matrix (row stride ld); zeros from column
-// `end` on.
+// use. The operand is the first `runs` runs, 1 << log a row at most, of columns from c0 on of `rows` rows of a row-major
+// matrix (row stride ld); zeros from column `end` on.
 template <typename W, int N>
 struct WeightRuns {
   uint4 v[N][sizeof(W) / 2];
 
-  __device__ __forceinline__ void load(int first, const W *w, size_t ld, int rows, int c0, int per, int end, bool wide) {
+  __device__ __forceinline__ void load(int first, const W *w, size_t ld, int rows, int c0, int runs, int log, int end,
+                                       bool wide) {
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      const int id = first + n * kThreads + threadIdx.x, row = id / per, c = c0 + (id - row * per) * 8;
-      if (row >= rows)
-        break;
+      const int id = first + n * kThreads + threadIdx.x, row = id >> log, run = id & ((1 << log) - 1), c = c0 + run * 8;
+      if (row >= rows || run >= runs)
+        continue;
       const W *src = w + row * ld + c;
       if (wide && c < end) {
 #pragma unroll
@@ -370,13 +377,13 @@ struct WeightRuns {
     }
   }
   // As operand parts of blocks of `high` rows, `bytes` apart.
-  __device__ __forceinline__ void store(int first, uint8_t *at, int bytes, int high, int rows, int per) const {
+  __device__ __forceinline__ void store(int first, uint8_t *at, int bytes, int high, int rows, int runs, int log) const {
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      const int id = first + n * kThreads + threadIdx.x, row = id / per;
-      if (row >= rows)
-        break;
-      uint8_t *dst = at + operand_at(high, row, (id - row * per) * 8);
+      const int id = first + n * kThreads + threadIdx.x, row = id >> log, run = id & ((1 << log) - 1);
+      if (row >= rows || run >= runs)
+        continue;
+      uint8_t *dst = at + operand_at(high, row, run * 8);
       if constexpr (kParts<W> == 1) {
         *reinterpret_cast<uint4 *>(dst) = v[n][0];
       } else {
@@ -521,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     // Its share of the weights: two runs a step up to 64 ranks, read two steps ahead; the others as they are needed.
     WeightRuns<W, 2> runs2[2];
     auto load_w = [&](WeightRuns<W, 2> &r, int first, int j) {
-      r.load(first, A, (size_t)a.n, w.rank, n0 + j * kStep, kStep / 8, n1, a_wide);
+      r.load(first, A, (size_t)a.n, w.rank, n0 + j * kStep, kStep / 8, 3, n1, a_wide);
     };
     const uint32_t idesc = umma_idesc_bf16(128, n16);
     auto step = [&](float4 (&v)[4], WeightRuns<W, 2> &runs, int j) {
@@ -542,15 +549,15 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
           for (int i = 0; i < 3; i++)
             *reinterpret_cast<uint2 *>(dst + i * x_bytes) = make_uint2(p0[i], p1[i]);
         }
-      runs.store(0, stage, a_bytes, rank_high, w.rank, kStep / 8);
+      runs.store(0, stage, a_bytes, rank_high, w.rank, kStep / 8, 3);
       if (w.rank > 64) {
         load_w(runs, 2 * kThreads, j);
-        runs.store(2 * kThreads, stage, a_bytes, rank_high, w.rank, kStep / 8);
+        runs.store(2 * kThreads, stage, a_bytes, rank_high, w.rank, kStep / 8, 3);
       }
       fence_proxy_async_smem();
       __syncthreads();
       if (warp == 0 && ok) {
-        if (lane == 0) {
+        if (elect_one()) {
           const uint64_t ad = umma_desc_sw128(stage), bd = umma_desc_sw128(xs);
 #pragma unroll
           for (int s2 = 2; s2 >= 0; s2--)
@@ -647,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
 
   // B h over this CTA's slice of d, 128 outputs at a time.
   const bool b_wide = aligned16(B) && w.rank % 8 == 0;
-  const int b_bytes = 128 * rank_high * 2, per = rank16 / 8;
+  const int b_bytes = 128 * rank_high * 2, per = rank16 / 8, log = rank_high == 64 ? 3 : 4;
   const uint32_t idesc = umma_idesc_bf16(128, n16);
   const int column = 32 * (warp >> 2), lane_d = 32 * (warp & 3) + lane;
   const bool base_wide = aligned16(a.base) && a.ldb % 4 == 0, out_wide = aligned16(a.out) && a.ldo % 4 == 0;
@@ -657,52 +664,59 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
   auto load_w = [&](int first, int j) {
     const int d = d0 + 128 * j;
     if (per && d < d1)
-      runs.load(first, B + (size_t)d * w.rank, (size_t)w.rank, min(128, d1 - d), 0, per, w.rank, b_wide);
+      runs.load(first, B + (size_t)d * w.rank, (size_t)w.rank, min(128, d1 - d), 0, per, log, w.rank, b_wide);
+  };
+  // A warp per row, four outputs a lane: this lane's base, read a tile ahead.
+  int r[kTileRows / kWarps];
+  float4 y[kTileRows / kWarps];
+#pragma unroll
+  for (int n = 0; n < kTileRows / kWarps; n++)
+    r[n] = t.rows[min(warp + kWarps * n, rows - 1)];
+  auto load_base = [&](int j) {
+    const int at = d0 + 128 * j + 4 * lane, left = d1 - at;
+#pragma unroll
+    for (int n = 0; n < kTileRows / kWarps; n++) {
+      y[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (a.base && warp + kWarps * n < rows)
+        y[n] = read4(a.base + r[n] * a.ldb + at, left, base_wide);
+    }
   };
   load_w(0, 0);
+  load_base(0);
   for (int j = 0; j < tiles; j++) {
     const int d = d0 + 128 * j;
     if (per) {
-      runs.store(0, smem, b_bytes, 128, min(128, d1 - d), per);
-      if (w.rank > 64) {
+      runs.store(0, smem, b_bytes, 128, min(128, d1 - d), per, log);
+      if (rank_high > 64) {
         load_w(4 * kThreads, j);
-        runs.store(4 * kThreads, smem, b_bytes, 128, min(128, d1 - d), per);
+        runs.store(4 * kThreads, smem, b_bytes, 128, min(128, d1 - d), per, log);
       }
       fence_proxy_async_smem();
       tc_fence_before();
       __syncthreads();
       if (warp == 0 && ok) {
-        if (lane == 0) {
+        if (elect_one()) {
           tc_fence_after();
           const uint64_t ad = umma_desc_sw128(smem), bd = umma_desc_sw128(operand);
-          bool more = false;
+          const int ks = rank16 / 16;
 #pragma unroll
           for (int s = 2; s >= 0; s--)
 #pragma unroll
             for (int i = 0; i < P; i++) {
               if (i > s)
                 continue;
-              for (int k = 0; k < rank16 / 16; k++) {
-                umma_bf16(tmem, ad + (i * b_bytes + (k >> 2) * 128 * 128 + 32 * (k & 3)) / 16,
-                          bd + ((s - i) * h_bytes + (k >> 2) * kTileRows * 128 + 32 * (k & 3)) / 16, idesc, more);
-                more = true;
-              }
+              const uint64_t ai = ad + i * b_bytes / 16, bi = bd + (s - i) * h_bytes / 16;
+#pragma unroll
+              for (int k = 0; k < kTileRank / 16; k++)
+                if (k < ks)
+                  umma_bf16(tmem, ai + ((k >> 2) * 128 * 128 + 32 * (k & 3)) / 16,
+                            bi + ((k >> 2) * kTileRows * 128 + 32 * (k & 3)) / 16, idesc, s < 2 || i > 0 || k > 0);
             }
           umma_commit(&t.bar[0]);
         }
         __syncwarp();
       }
       load_w(0, j + 1);
-    }
-    // Under the MMAs: this tile's base, a warp per row, four outputs a lane.
-    const int at = d + 4 * lane, left = d1 - at;
-    float4 y[kTileRows / kWarps];
-#pragma unroll
-    for (int n = 0; n < kTileRows / kWarps; n++) {
-      const int i = warp + kWarps * n;
-      y[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (a.base && i < rows)
-        y[n] = read4(a.base + t.rows[i] * a.ldb + at, left, base_wide);
     }
     if (per) {
       ok &= tile_wait(&t.bar[0], phase[0] & 1, abort_flag);
@@ -721,6 +735,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
       }
       __syncthreads();
     }
+    const int at = d + 4 * lane;
 #pragma unroll
     for (int n = 0; n < kTileRows / kWarps; n++) {
       const int i = warp + kWarps * n;
@@ -730,8 +745,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         const float4 v = *reinterpret_cast<const float4 *>(tile_out + i * 128 + 4 * lane);
         y[n].x += v.x, y[n].y += v.y, y[n].z += v.z, y[n].w += v.w;
       }
-      write4(a.out + t.rows[i] * a.ldo + at, y[n], left, out_wide);
+      write4(a.out + r[n] * a.ldo + at, y[n], d1 - at, out_wide);
     }
+    if (j + 1 < tiles)
+      load_base(j + 1);
   }
   tc_fence_before();
   __syncthreads();

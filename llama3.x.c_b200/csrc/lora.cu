@@ -89,31 +89,50 @@ __global__ void __launch_bounds__(kThreads) lora_row_kernel(const LoraArgs a, in
   const int n_slice = ((a.n + ctas - 1) / ctas + 7) & ~7;
   const int n0 = min(rank * n_slice, a.n), n1 = min(n0 + n_slice, a.n);
   const bool wide = aligned16(A) && aligned16(x) && a.n % 8 == 0;
-  for (int k = warp; k < w.rank; k += kWarps) {
-    const W *ak = A + (long long)k * a.n;
-    float s = 0.0f;
+  constexpr int R = sizeof(W) == 4 ? 2 : 4;  // rows of A at once: their reads are under way together
+  for (int k0 = warp; k0 < w.rank; k0 += R * kWarps) {
+    float s[R];
+    const W *ak[R];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+      s[r] = 0.0f, ak[r] = A + (size_t)min(k0 + r * kWarps, w.rank - 1) * a.n;
     if (wide) {
       for (int i = n0 + 8 * lane; i < n1; i += 256) {
-        float wv[8], xv[8];
-        load8(ak + i, wv);
+        float xv[8], wv[R][8];
         load8(x + i, xv);
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-          s = fmaf(wv[j], xv[j], s);
+        for (int r = 0; r < R; r++)
+          if (k0 + r * kWarps < w.rank)
+            load8(ak[r] + i, wv[r]);
+#pragma unroll
+        for (int r = 0; r < R; r++)
+          if (k0 + r * kWarps < w.rank)
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+              s[r] = fmaf(wv[r][j], xv[j], s[r]);
       }
     } else {
-      for (int i = n0 + lane; i < n1; i += 32)
-        s = fmaf(to_float(ak[i]), x[i], s);
+#pragma unroll 2
+      for (int i = n0 + lane; i < n1; i += 32) {
+        const float xi = x[i];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+          s[r] = fmaf(to_float(ak[r][i]), xi, s[r]);
+      }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1)
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0)
-      part[k] = s;
+    for (int r = 0; r < R; r++) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1)
+        s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
+      if (lane == 0 && k0 + r * kWarps < w.rank)
+        part[k0 + r * kWarps] = s[r];
+    }
   }
   cluster.sync();
   for (int k = threadIdx.x; k < w.rank; k += kThreads) {
     float s = 0.0f;
+#pragma unroll
     for (int c = 0; c < ctas; c++)
       s += *cluster.map_shared_rank(&part[k], c);
     h[k] = s * w.scale;
@@ -126,6 +145,7 @@ __global__ void __launch_bounds__(kThreads) lora_row_kernel(const LoraArgs a, in
     const W *bi = B + (long long)i * w.rank;
     float s = 0.0f;
     if (wide_b) {
+#pragma unroll 4
       for (int k = 0; k < w.rank; k += 8) {
         float wv[8];
         load8(bi + k, wv);
@@ -778,8 +798,11 @@ cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned cl
 
 template <typename W>
 cudaError_t run(const LoraArgs &a) {
-  // Four rows an adapter make a tile worth its search (measured at d = n = 4096, rank 16).
-  if (a.rows < 16 || a.rows < 4 * a.count || a.count >= kMaxBins || a.max_rank > kTileRank)
+  // The row kernel reads a row's adapter from L2 for every row, about 3.3 TB/s of it (33 rows, rank 32 fp32, 4096 to
+  // 14336: 78 MB, 24 us); a tile reads it once but takes some 40 us of steps (the same: 38 us). Tiles of fewer than four
+  // rows gain nothing.
+  const double row_bytes = (double)a.rows * a.max_rank * ((double)a.n + a.d) * sizeof(W);
+  if (row_bytes < 128e6 || a.rows < 4 * a.count || a.count >= kMaxBins || a.max_rank > kTileRank)
     return launch<W>(lora_row_kernel<W>, a, (unsigned)a.rows, 1, 0);
   const size_t smem = TileSmem<W>(a.max_rank).total;
   cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(lora_tile_kernel<W>), TileSmem<W>(kTileRank).total);

@@ -232,6 +232,18 @@ LORA = [  # rows, adapters, ranks, n, d, dtype
 ]
 
 
+# Cases large enough for tiles of rows of one adapter: ragged last steps, ranks that fill no block, three weight types,
+# tiles of few and of many rows, more adapters than the rows use.
+LORA += [
+    (400, 3, [64, 128, 100], 2056, 1100, torch.bfloat16),
+    (900, 5, [16, 24, 1, 64, 48], 1000, 1300, torch.float16),
+    (350, 2, [128, 65], 520, 904, torch.float32),
+    (2100, 90, [32] * 90, 640, 2000, torch.bfloat16),
+    (1500, 4, [20, 36, 7, 60], 1023, 777, torch.bfloat16),
+    (700, 2, [64, 64], 8, 4000, torch.float32),
+]
+
+
 def lora_inputs(case, order, seed=0):
     rows, count, ranks, n, d, dtype = case
     g = generator(rows + seed)
@@ -281,11 +293,11 @@ def test_lora(kc, case, order):
     assert ((out.double() - want).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("rows", [5, 200])
+@pytest.mark.parametrize("rows", [5, 200, 3000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_lora_strides_and_alignment(kc, rows, dtype):
     """Rows inside wider buffers (their gaps stay as they were), matrices at odd addresses."""
-    n, d, ranks = 264, 130, [16, 24]
+    n, d, ranks = (264, 130, [16, 24]) if rows < 1000 else (808, 334, [16, 24])
     a, b, scale, index, g = lora_inputs((rows, 2, ranks, n, d, dtype), "mixed")
     x, base = normal(g, rows, n + 5), normal(g, rows, d + 3)
     out = torch.full((rows, d + 7), -7.0, device="cuda")
@@ -300,9 +312,9 @@ def test_lora_strides_and_alignment(kc, rows, dtype):
         assert (out[:, d:] == -7.0).all()
 
 
-@pytest.mark.parametrize("rows", [6, 150])
+@pytest.mark.parametrize("rows", [6, 150, 4000])
 def test_lora_reports_bad_rows(kc, rows):
-    n, d = 64, 72
+    n, d = (64, 72) if rows < 1000 else (1024, 520)
     a, b, scale, index, g = lora_inputs((rows, 2, [8, 16], n, d, torch.bfloat16), "each")
     x, base = normal(g, rows, n), normal(g, rows, d)
     table = kc.lora_table(a, b, scale)
@@ -318,10 +330,10 @@ def test_lora_reports_bad_rows(kc, rows):
         assert torch.equal(out[3], base[3])
 
 
-@pytest.mark.parametrize("rows", [4, 150])
+@pytest.mark.parametrize("rows", [4, 150, 4000])
 def test_lora_nonfinite_rows_stay_their_own(kc, rows):
     """An infinity or NaN in one row, or in an adapter, shows in the rows that use it and in no other."""
-    n, d = 128, 64
+    n, d = (128, 64) if rows < 1000 else (2048, 512)
     a, b, scale, index, g = lora_inputs((rows, 3, [8, 8, 8], n, d, torch.bfloat16), "each")
     x, base = normal(g, rows, n), normal(g, rows, d)
     x[1, 5] = float("inf")
@@ -331,6 +343,19 @@ def test_lora_nonfinite_rows_stay_their_own(kc, rows):
     kc.status()
     sick = (index == 2) | (torch.arange(rows, device="cuda") == 1)
     assert not out[sick].isfinite().any() and out[~sick].isfinite().all()
+
+
+def test_lora_more_rows_than_a_launch_takes(kc):
+    """Over 16384 rows: several launches, each with its own part of the index."""
+    case = (20000, 3, [16, 8, 24], 256, 264, torch.bfloat16)
+    rows, count, ranks, n, d, dtype = case
+    a, b, scale, index, g = lora_inputs(case, "mixed")
+    x, base = normal(g, rows, n), normal(g, rows, d)
+    out = torch.full((rows, d), -7.0, device="cuda")
+    kc.k_lora_rows(out, d, base, d, x, n, index, kc.lora_table(a, b, scale), count, kc.K_BF16, 24, n, d, rows)
+    kc.status()
+    want, tol = lora_64(x, base, index, a, b, scale)
+    assert ((out.double() - want).abs() <= tol).all()
 
 
 # ---- drafts ------------------------------------------------------------------------------------------------------------

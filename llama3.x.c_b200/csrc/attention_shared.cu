@@ -335,13 +335,21 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ float abs_max(float m, float4 v) {
-  return fmaxf(fmaxf(fmaxf(m, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
+__device__ __forceinline__ float abs_max3(float a, float b, float c) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float abs_max(float m, float4 v) { return abs_max3(abs_max3(m, v.x, v.y), v.z, v.w); }
 
 // 16 bytes from global to shared memory, asynchronously; zeros without `in`.
-__device__ __forceinline__ void copy16(void *dst, const void *src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
                : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -362,20 +370,28 @@ struct Rows8 {
   static __device__ __forceinline__ void copy(float4 *slot, const float *cache, int row0, int end, int hd, int lane) {
     const int col = lane * 4 % HD, r = lane * 4 / HD;
     const float *src = cache + (size_t)(row0 + r) * hd + col;
+    const uint32_t dst = smem_u32(slot + lane);
+    if (hd == HD && row0 + 8 <= end) {  // whole rows: addresses a constant apart
+#pragma unroll
+      for (int i = 0; i < kSteps; i++)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 512 * i), "l"(src + i * kAt * HD) : "memory");
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
       const bool in = row0 + r + i * kAt < end && col < hd;
-      copy16(slot + 32 * i + lane, in ? src + (size_t)i * kAt * hd : cache, in);
+      copy16(dst + 512 * i, in ? src + (size_t)i * kAt * hd : cache, in);
     }
   }
   __device__ __forceinline__ void take(const float4 *slot, int lane) {
-    top = 0.0f;
 #pragma unroll
     for (int i = 0; i < kSteps; i++)
       x[i] = slot[32 * i + lane];
+    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < kSteps; i++)
-      top = abs_max(top, x[i]);
+      t[i & 3] = abs_max(t[i & 3], x[i]);
+    top = fmaxf(max3(t[0], t[1], t[2]), t[3]);
     // The values are here before the slot's next copy starts.
     asm volatile("" : "+f"(top)::"memory");
   }
@@ -637,11 +653,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
               r[e] = p0 + c + e < limit ? r[e] : 0xff800000u;
 #pragma unroll
           for (int e8 = 0; e8 < 32; e8 += 8) {
-            float x = __uint_as_float(r[e8]);
+            float x[8];
 #pragma unroll
-            for (int e = 1; e < 8; e++)
-              x = fmaxf(x, __uint_as_float(r[e8 + e]));
-            top = fmaxf(top, x * factor((c + e8) >> 3));
+            for (int e = 0; e < 8; e++)
+              x[e] = __uint_as_float(r[e8 + e]);
+            top = fmaxf(top, max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7])) *
+                                 factor((c + e8) >> 3));
           }
         }
         int vmin = vshift[0];
@@ -686,15 +703,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
             const float f = factor((c + e8) >> 3);
             const int grow = max(kPShift - vshift[(c + e8) >> 3] + vref, -60);
             const float from = (float)grow - base;
-            float sum = 0.0f;
+            const uint64_t f2 = f2_pack(f, f), from2 = f2_pack(from, from);
+            uint64_t sum2 = 0;
 #pragma unroll
             for (int e = e8; e < e8 + 8; e += 2) {
-              const float x = ex2(fmaf(__uint_as_float(r[e]), f, from));
-              const float y = ex2(fmaf(__uint_as_float(r[e + 1]), f, from));
-              sum += x + y;
-              split2(f2_pack(x, y), hi[e / 2], lo[e / 2]);
+              float x, y;
+              f2_unpack(f2_fma(f2_pack_bits(r[e], r[e + 1]), f2, from2), x, y);
+              const uint64_t p = f2_pack(ex2(x), ex2(y));
+              sum2 = f2_add(sum2, p);
+              split2(p, hi[e / 2], lo[e / 2]);
             }
-            l += sum * pow2(-grow);
+            float s0, s1;
+            f2_unpack(sum2, s0, s1);
+            l = fmaf(s0 + s1, pow2(-grow), l);
           }
           tmem_st16(ts + c, hi);
           tmem_st16(ts + c + 16, lo);

@@ -63,7 +63,7 @@ __device__ __forceinline__ void load8(const __half *p, float (&v)[8]) { halves<_
 __device__ __forceinline__ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename W>
-__global__ void __launch_bounds__(kThreads) lora_row_kernel(const LoraArgs a, int) {
+__global__ void __launch_bounds__(kThreads, 4) lora_row_kernel(const LoraArgs a, int) {
   __shared__ float part[kMaxRank], h[kMaxRank];
   cg::cluster_group cluster = cg::this_cluster();
   constexpr int ctas = kCtas;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads) lora_row_kernel(const LoraArgs a, in
     const W *bi = B + (long long)i * w.rank;
     float s = 0.0f;
     if (wide_b) {
-#pragma unroll 4
+#pragma unroll 2
       for (int k = 0; k < w.rank; k += 8) {
         float wv[8];
         load8(bi + k, wv);

@@ -916,21 +916,38 @@ size_t partial_floats(int n_heads, int hd, int batch, int rows) {
   return splits * each + 4;
 }
 
-// How the positions are split. In units of a tile of 64 positions against a query tile: a CTA costs about kStart units
-// before its first, so the splits are as long as an even share of the work over the SMs allows, and at most kLongest
-// tiles: the tensor cores' accumulators truncate, which over more tiles would show in the result.
-constexpr int kStart = 6, kLongest = 16;
-// `most` splits at most, two at least.
+// How the positions are split, `most` splits at most, two at least: the lengths whose CTAs are estimated to end first.
+// In units of a tile of 64 positions against a query tile (about 1.6 us): a CTA takes kStart units besides its tiles, the
+// requests' caches are taken to be half full, CTAs beyond one wave fill the gaps the longest one leaves half of, and a
+// split costs its partial results' way to memory and back. No more than kLongest tiles to a split: the tensor cores'
+// accumulators truncate, which over more tiles would show in the result.
+constexpr int kStart = 4, kLongest = 16;
 void plan_splits(SharedArgs *a, int most) {
-  const long long prefix_tiles = ceil_div(a->prefix, kTcPos), own_tiles = ceil_div(a->seq, kTcPos);
-  const long long columns = (long long)a->n_kv * a->tiles, own_columns = (long long)a->n_kv * a->batch * a->own_tiles;
-  const long long units = columns * prefix_tiles + own_columns * ((own_tiles + 1) / 2 + kStart);
-  const long long share = units / kPlanSms;
-  auto clamp = [](long long v, long long low, long long high) { return v < low ? low : v > high ? high : v; };
-  const int prefix_length = (int)clamp(share / 2, 2, kLongest), own_length = (int)clamp(share, 4, kLongest);
-  a->own_splits = (int)clamp(ceil_div((int)own_tiles, own_length), 1, kMaxSplits < most / 2 ? kMaxSplits : most / 2);
-  const int rest = most - a->own_splits;
-  a->prefix_splits = (int)clamp(ceil_div((int)prefix_tiles, prefix_length), 0, kMaxSplits < rest ? kMaxSplits : rest);
+  const int prefix_tiles = ceil_div(a->prefix, kTcPos), own_tiles = ceil_div(a->seq, kTcPos);
+  const double columns = (double)a->n_kv * a->tiles, own_columns = (double)a->n_kv * a->batch * a->own_tiles;
+  const double pass = (double)a->vectors * (a->hd + 2) * 8 / 5e12 / 1.6e-6;  // a split's partial results
+  const int most_own = most / 2 < kMaxSplits ? most / 2 : kMaxSplits;
+  double best = 0.0;
+  for (int own_length = own_tiles < kLongest ? own_tiles : kLongest; own_length >= 1; own_length -= own_length > 4 ? 2 : 1) {
+    const int own = ceil_div(own_tiles, own_length) < most_own ? ceil_div(own_tiles, own_length) : most_own;
+    const int rest = most - own < kMaxSplits ? most - own : kMaxSplits;
+    for (int length = prefix_tiles < kLongest ? prefix_tiles : kLongest; length >= (prefix_tiles ? 1 : 0); length--) {
+      int n = prefix_tiles ? ceil_div(prefix_tiles, length) : 0;
+      n = n < rest ? n : rest;
+      const double c = n ? kStart + (double)prefix_tiles / n : 0.0, c_own = kStart + 0.5 * own_tiles / own;
+      const double items = columns * n + own_columns * own, work = columns * n * c + own_columns * own * c_own;
+      const double longest = c > c_own ? c : c_own;
+      double t = items <= kPlanSms ? longest : work / kPlanSms + 0.5 * longest;
+      t = (t > longest ? t : longest) + pass * (n + own);
+      if (best == 0.0 || t < best) {
+        best = t;
+        a->prefix_splits = n;
+        a->own_splits = own;
+      }
+      if (!prefix_tiles)
+        break;
+    }
+  }
 }
 
 size_t generic_smem(int hd) { return sizeof(float) * ((size_t)kGenericPos * (2 * hd + 1) + 4 * (size_t)hd); }

@@ -36,8 +36,8 @@ struct VerifyArgs {
   long long ldt, ldd;
   const int *drafted, *counts;
   const float *uniforms, *temperature;
-  int vocab, batch, rows, loops, chunks;  // chunks of loops * kBlock logits a row
-  double *sums;              // [batch][2 rows + 1][chunks]
+  int vocab, batch, rows, slots, loops, chunks;  // slots a request; chunks of loops * kBlock logits a row
+  double *sums;              // [batch][slots][chunks]
   unsigned long long *keys;  // the same: order-preserving maximum and its first index
 };
 
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kSumThreads, 4) verify_sums_kernel(const Verif
   pdl_wait();
   pdl_launch_dependents();
   const int chunk = blockIdx.x % a.chunks, id = blockIdx.x / a.chunks;
-  const int b = id / (2 * a.rows + 1), slot = id - b * (2 * a.rows + 1);
+  const int b = id / a.slots, slot = id - b * a.slots;
   const float t = a.temperature[b];
   const float *row;
   if (!slot_row(a, b, slot, &row))
@@ -354,9 +354,9 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
     return;  // the whole cluster: a slot of the batch that is not in use
   const Weights weight{table, greedy ? 0.0 : k32_of(t)};
   int *tokens = a.tokens + (long long)b * (a.rows + 1);
-  const long long base = (long long)b * (2 * a.rows + 1) * a.chunks;
+  const long long base = (long long)b * a.slots * a.chunks;
   if (valid)
-    for (int slot = warp; slot < 2 * a.rows + 1; slot += kPickWarps) {
+    for (int slot = warp; slot < a.slots; slot += kPickWarps) {
       const float *row;
       if (!slot_row(a, b, slot, &row))
         continue;
@@ -620,8 +620,8 @@ void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt,
     kc_fail("%s: missing outputs, logits, drafts, numbers or 16-byte aligned work", name);
     return;
   }
-  // Longer chunks where they leave every SM some sixteen CTAs (half of which, or more, find nothing to do).
-  size_t blocks = verify_blocks(vocab), pairs = (size_t)batch * (2 * rows + 1) * blocks;
+  const int slots = draft && rows ? 2 * rows + 1 : rows + 1;
+  size_t blocks = verify_blocks(vocab), pairs = (size_t)batch * slots * blocks;
   if (pairs > 0x7fffffffu || (size_t)batch * kMaxCtas > 0x7fffffffu) {
     kc_fail("%s: batch %d of %d rows is too large", name, batch, rows);
     return;
@@ -630,18 +630,25 @@ void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt,
   a.accepted = accepted, a.tokens = tokens, a.target = target, a.draft = rows ? draft : nullptr;
   a.ldt = (long long)ldt, a.ldd = (long long)ldd, a.drafted = drafted, a.counts = counts;
   a.uniforms = uniforms, a.temperature = temperature, a.vocab = vocab, a.batch = batch, a.rows = rows;
-  a.loops = pairs >= (size_t)16 * kLoops * kc_device_sms() ? kLoops : 1;
+  // Longer chunks amortize a CTA's start and end, as long as those that find work (half of the drafts, say) fill the SMs
+  // four times over at four CTAs each: 64 requests of 5 drafts, 128256 tokens, 119 us with one block and 97 with four.
+  const size_t busy = (size_t)batch * (rows / 2 + 1 + (slots > rows + 1 ? rows / 2 : 0)) * blocks;
+  a.loops = 1;
+  while (a.loops < kLoops && busy / (2 * a.loops) >= (size_t)16 * kc_device_sms())
+    a.loops *= 2;
+  a.slots = slots;
   a.chunks = (int)((blocks + a.loops - 1) / a.loops);
-  pairs = (size_t)batch * (2 * rows + 1) * a.chunks;
+  pairs = (size_t)batch * slots * a.chunks;
   a.sums = static_cast<double *>(work);
   a.keys = reinterpret_cast<unsigned long long *>(a.sums + pairs);
   cudaError_t e =
       kc_launch_pdl(verify_sums_kernel, dim3((unsigned)pairs), dim3(kSumThreads), 0, kc_stream(), a);
   if (e == cudaSuccess) {
     kc_count_launch();
-    // The largest clusters that run in one wave of two CTAs per SM: a request's rows are read by more SMs at once.
+    // The largest clusters that run in about two waves of two CTAs per SM (greedy requests and accepted drafts leave
+    // early): a request's rows are read by more SMs at once.
     int ctas = kMaxCtas;
-    while (ctas > 4 && (long long)ctas * batch > 2 * kc_device_sms())
+    while (ctas > 4 && (long long)ctas * batch > 4 * kc_device_sms())
       ctas /= 2;
     e = allow_large_clusters();
     cudaLaunchConfig_t cfg = {};

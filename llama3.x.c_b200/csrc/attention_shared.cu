@@ -353,6 +353,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool in) {
                : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // All but the newest group of this thread's copies are done.
 __device__ __forceinline__ void copy_wait1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 
@@ -452,6 +453,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     tmem_alloc(&t->tmem, kTmemCols);
   const int hd = a.hd;
   const int cw = warp - kSoftWarps - 1;
+  // Softmax warps: lane n has the index of vector warp + 8 n, and whether this thread's own vector is in use.
+  const int g = warp >> 2, vec_i = 32 * (warp & 3) + lane;
+  const bool have = warp < kSoftWarps && vec_i < it.vecs, busy = 32 * (warp & 3) < it.vecs;
+  int vec = 0;
+  bool use = false;
+  if (warp < kSoftWarps) {
+    vec = vector_at(a, it.kv, it.first + min(warp + kSoftWarps * lane, it.vecs - 1));
+    const int row = (it.first + min(vec_i, it.vecs - 1)) / a.group, b = row / a.rows;
+    use = have && row - b * a.rows < request_of(a, b).count;
+  }
   float4 *kslot = reinterpret_cast<float4 *>(smem + L::raw_at) + max(cw, 0) * (4 * HD), *vslot = kslot + 2 * HD;
   if (cw >= 0) {
     Rows8<HD>::copy(kslot, it.k, it.p0 + 8 * cw, it.p1, hd, lane);
@@ -459,33 +470,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     Rows8<HD>::copy(vslot, it.v, it.p0 + 8 * cw, it.p1, hd, lane);
     copy_commit();
   } else if (warp < kSoftWarps) {
-    // The queries into the stages, a warp per row, eight rows in flight. Vectors not in use are zeros (what lies there
-    // is read, but not taken).
-    const bool wide = ((uintptr_t)a.q & 15) == 0;
-    int vec = 0, use = 0;
-    const int mine = it.first + warp + kSoftWarps * lane;
-    if (warp + kSoftWarps * lane < it.vecs) {
-      const int row = mine / a.group, b = row / a.rows;
-      vec = vector_at(a, it.kv, mine);
-      use = row - b * a.rows < request_of(a, b).count;
-    }
+    // The queries into the stages, a warp per row, all rows under way at once; what lies at vectors not in use comes
+    // too and is dropped below.
     const int e = 4 * lane;
-    for (int n0 = 0; warp + kSoftWarps * n0 < it.vecs; n0 += 8) {
-      float4 y[8];
-#pragma unroll
-      for (int n = 0; n < 8; n++) {
-        const float *src = a.q + (size_t)__shfl_sync(0xffffffffu, vec, n0 + n) * hd + e;
-        y[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (e < hd)
-          y[n] = wide ? *reinterpret_cast<const float4 *>(src) : make_float4(src[0], src[1], src[2], src[3]);
+    if (((uintptr_t)a.q & 15) == 0) {
+#pragma unroll 4
+      for (int i = warp, n = 0; i < it.vecs; i += kSoftWarps, n++) {
+        const float *src = a.q + (size_t)__shfl_sync(0xffffffffu, vec, n) * hd;
+        if (e < HD)
+          copy16(smem_u32(smem) + (i * L::row + e) * 4, e < hd ? src + e : src, e < hd);
       }
-#pragma unroll
-      for (int n = 0; n < 8; n++) {
-        const int i = warp + kSoftWarps * (n0 + n);
-        if (!__shfl_sync(0xffffffffu, use, n0 + n))
-          y[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (i < it.vecs && e < HD)
-          *reinterpret_cast<float4 *>(smem + ((size_t)i * L::row + e) * 4) = y[n];
+      copies_done();
+    } else {
+      for (int i = warp, n = 0; i < it.vecs; i += kSoftWarps, n++) {
+        const float *src = a.q + (size_t)__shfl_sync(0xffffffffu, vec, n) * hd + e;
+        if (e < HD)
+          *reinterpret_cast<float4 *>(smem + ((size_t)i * L::row + e) * 4) =
+              e < hd ? make_float4(src[0], src[1], src[2], src[3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
     }
   }
@@ -495,9 +496,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
   const uint32_t tmem = t->tmem;
 
   // The queries: group g's threads lay out half g of their vectors' elements. Vectors not in use are zeros.
-  const int g = warp >> 2, vec_i = 32 * (warp & 3) + lane;
   const uint32_t quadrant = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-  const bool have = vec_i < it.vecs, busy = 32 * (warp & 3) < it.vecs;
   int qshift = 0;
   if (warp < kSoftWarps) {
     constexpr int H = HD / 2;
@@ -507,7 +506,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       const float *src = reinterpret_cast<const float *>(smem) + (size_t)vec_i * L::row + g * H;
 #pragma unroll
       for (int e = 0; e < H; e += 4) {
-        const float4 y = have ? *reinterpret_cast<const float4 *>(src + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float4 y = use ? *reinterpret_cast<const float4 *>(src + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         x[e] = y.x, x[e + 1] = y.y, x[e + 2] = y.z, x[e + 3] = y.w;
         mx = abs_max(mx, y);
       }
@@ -767,13 +766,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       tc_fence_before();
     }
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
-    if (done)
-      for (int i = warp; i < it.vecs; i += kSoftWarps) {
-        float *dst = a.acc + ((size_t)it.split * a.vectors + vector_at(a, it.kv, it.first + i)) * hd;
-        for (int e = 4 * lane; e < hd; e += 128)
-          *reinterpret_cast<float4 *>(dst + e) =
-              *reinterpret_cast<const float4 *>(smem + ((size_t)i * L::row + e) * 4);
+    if (done) {
+      const int e = 4 * lane;
+      float *part = a.acc + (size_t)it.split * a.vectors * hd + e;
+#pragma unroll 4
+      for (int i = warp, n = 0; i < it.vecs; i += kSoftWarps, n++) {
+        float *dst = part + (size_t)__shfl_sync(0xffffffffu, vec, n) * hd;
+        if (e < hd)
+          *reinterpret_cast<float4 *>(dst) = *reinterpret_cast<const float4 *>(smem + ((size_t)i * L::row + e) * 4);
       }
+    }
   }
   __syncthreads();
   if (warp == kSoftWarps) {

@@ -44,6 +44,7 @@ struct SharedArgs {
   int vectors;                // batch * rows * n_heads
   int prefix_splits, own_splits;  // splits of the positions
   int tiles, own_tiles;           // query tiles per KV head: of the prefix part, of a request's own part
+  int extra;                      // items that a CTA with one item less of the prefix takes before the rest
 };
 
 // Rows that request b uses and the positions it has stored before them; 0 rows where they are not sound. Both loads go
@@ -68,14 +69,35 @@ struct Item {
   int p0, p1;          // positions
 };
 
+// The items of CTA `cta` of `ctas`: the prefix's in turn, so that some CTAs get one more of them than the others; of the
+// requests' own, `extra` to each of the others, then the rest in turn, the others first. -1 past the last.
+__host__ __device__ __forceinline__ int item_id(const SharedArgs &a, int cta, int ctas, int n) {
+  const int prefix = a.n_kv * a.tiles * a.prefix_splits, own = a.n_kv * a.batch * a.own_tiles * a.own_splits;
+  const int heavy = prefix % ctas, light = ctas - heavy, mine = prefix / ctas + (cta < heavy);
+  if (n < mine)
+    return cta + n * ctas;
+  n -= mine;
+  int id;
+  if (cta >= heavy && n < a.extra) {
+    id = cta - heavy + n * light;
+  } else {
+    n -= cta >= heavy ? a.extra : 0;
+    const long long rest = (long long)(cta >= heavy ? cta - heavy : cta + light) + (long long)n * ctas;
+    if (rest >= own - a.extra * light)
+      return -1;
+    id = a.extra * light + (int)rest;
+  }
+  return prefix + id;
+}
+
 // Vector i of KV head kv's flat list: index in the [batch][rows][n_heads] order.
 __device__ __forceinline__ int vector_at(const SharedArgs &a, int kv, int i) {
   return (i / a.group) * a.n_heads + kv * a.group + i % a.group;
 }
 
 // Items 0 .. n_kv * tiles * prefix_splits - 1 are the prefix's, then one per (request, KV head, query tile, split).
-// False: nothing to do.
-__device__ __forceinline__ bool item_at(const SharedArgs &a, int id, int tile, Item *it) {
+// False: nothing to do; with `report`, a request that is not sound is an error.
+__device__ __forceinline__ bool item_at(const SharedArgs &a, int id, int tile, bool report, Item *it) {
   const int prefix_items = a.n_kv * a.tiles * a.prefix_splits;
   if (id < prefix_items) {
     it->split = id % a.prefix_splits;
@@ -100,7 +122,7 @@ __device__ __forceinline__ bool item_at(const SharedArgs &a, int id, int tile, I
   it->b = id / a.n_kv;
   const Request r = request_of(a, it->b);
   if (!r.count) {
-    if (r.bad && threadIdx.x == 0)
+    if (r.bad && report)
       kc_raise(KC_ERR_BAD_ARGS);
     return false;
   }
@@ -132,7 +154,7 @@ __global__ void __launch_bounds__(kGenericThreads) shared_generic_kernel(const S
   pdl_wait();
   pdl_launch_dependents();
   Item it;
-  if (!item_at(a, blockIdx.x, kGenericVecs, &it))
+  if (!item_at(a, blockIdx.x, kGenericVecs, threadIdx.x == 0, &it))
     return;
   const int hd = a.hd, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float *ks = smem;                                 // [32][hd + 1]
@@ -208,8 +230,10 @@ __global__ void __launch_bounds__(kGenericThreads) shared_generic_kernel(const S
 
 // ---- tensor-core kernel -------------------------------------------------------------------------------------------
 
-// head_dim <= 128 in whole 16-byte units. A CTA takes one item: up to 128 query vectors of a KV head against a range of
-// positions in tiles of 64, S = Q K^T and O += P V on tcgen05 with accumulators in TMEM.
+// head_dim <= 128 in whole 16-byte units. A CTA per SM takes its items one after another: up to 128 query vectors of a KV
+// head against a range of positions in tiles of 64, S = Q K^T and O += P V on tcgen05 with accumulators in TMEM. The
+// tiles of all items run through the same stages: the next item's keys and values are under way, and its queries laid
+// out, before the last sums are done (a CTA per item took 215 us where this takes 199: 256 rows behind 8192 positions).
 //
 // fp32 products on half-precision tensor cores: x = 2^-k (hi + lo) with hi and lo fp16, 22 bits of x, and
 // x y = 2^-(k + k') (hi hi' + hi lo' + lo hi') up to 2^-22 of the product (what is dropped, lo lo', is below the
@@ -230,29 +254,36 @@ constexpr int kTcThreads = 32 * (kSoftWarps + 1 + kConvWarps);
 constexpr uint32_t kTmemQ = 0, kTmemS = 128, kTmemO = 256, kTmemCols = 512;  // S and O: two buffers each
 constexpr int kPShift = 7;  // probabilities are up to 2^8 (the lazy reference) and carry this power of two more
 
+constexpr int kMaxItems = 32;  // of a CTA: a lane of every warp finds one
+constexpr int kTailBytes = 6400;
+
 template <int HD>
 struct TcSmem {
   static constexpr int kv_bytes = kTcPos * HD * 2;  // hi or lo of K or V
   static constexpr int stage = 4 * kv_bytes;
   static constexpr int raw_at = 2 * stage;          // the next tile's keys and values as they come, a slot per converter
   static constexpr int tail_at = raw_at + 2 * kTcPos * HD * 4;
-  static constexpr int total = tail_at + 5120 + 1024;  // the tail, and room to align the start to 1 KiB
-  static constexpr int row = HD + 4;  // floats of a vector's row where queries and results pass through the stages
+  static constexpr int total = tail_at + kTailBytes + 1024;  // the tail, and room to align the start to 1 KiB
 };
-static_assert(kTcVecs * TcSmem<64>::row * 4 <= TcSmem<64>::raw_at && kTcVecs * TcSmem<128>::row * 4 <= TcSmem<128>::raw_at,
-              "the stages hold a tile of queries or results");
+
+__device__ __forceinline__ int tiles_of(const Item &it) { return (it.p1 - it.p0 + kTcPos - 1) / kTcPos; }
+
+__device__ __forceinline__ const float *shfl_ptr(const float *p, int from) {
+  return reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)p, from));
+}
 
 struct TcTail {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2];
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2], qfull;
   uint32_t tmem;
   int abort_flag;
   float kscale[4][kConvWarps];  // 2^-k of eight keys, a ring of tiles
   int vshift[4][kConvWarps];    // k of eight values
-  float qmax[2][kTcVecs];
+  int qshift[2][kTcVecs];  // of this item and the next
   float m[2][kTcVecs], l[2][kTcVecs];  // of a group's tiles, and the power of its O
   int vref[2][kTcVecs];
+  Item items[kMaxItems];
 };
-static_assert(sizeof(TcTail) <= 5120, "the tail's room");
+static_assert(sizeof(TcTail) <= kTailBytes, "the tail's room");
 
 // A whole warp's bounded wait, with one answer for all lanes: false once any wait of the CTA has given up.
 __device__ __forceinline__ bool tc_wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
@@ -296,6 +327,24 @@ __device__ __forceinline__ void umma_f16_ta(uint32_t d, uint32_t a, uint64_t bde
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+// 16 lanes x 8 N consecutive columns, four registers to 8 columns: lane t has columns 2 (t % 4) and the next of row t / 4
+// in the first two, of row t / 4 + 8 in the others.
+__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_rows(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 // Writes 32 lanes (this warp's quadrant) x 16 consecutive columns.
@@ -353,7 +402,20 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool in) {
                : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// Four elements of every 16 from src on, zeros from `left` elements on.
+template <int HD>
+__device__ __forceinline__ void load_row(float4 (&x)[HD / 16], const float *src, int left) {
+  if (((uintptr_t)src & 15) == 0) {
+#pragma unroll
+    for (int c = 0; c < HD / 16; c++)
+      x[c] = 16 * c < left ? *reinterpret_cast<const float4 *>(src + 16 * c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  } else {
+#pragma unroll
+    for (int c = 0; c < HD / 16; c++)
+      x[c] = 16 * c < left ? make_float4(src[16 * c], src[16 * c + 1], src[16 * c + 2], src[16 * c + 3])
+                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+}
 // All but the newest group of this thread's copies are done.
 __device__ __forceinline__ void copy_wait1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 
@@ -427,15 +489,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
+  // This CTA's items: every warp finds them all, a lane each, so that none has to wait for the first. Those with tiles
+  // go into the list; a split that got no positions is an empty result.
   Item it;
-  if (!item_at(a, blockIdx.x, kTcVecs, &it))
-    return;
-  const int tiles = (it.p1 - it.p0 + kTcPos - 1) / kTcPos;
-  if (tiles <= 0) {
-    for (int i = threadIdx.x; i < it.vecs; i += kTcThreads)
-      a.ml[(size_t)it.split * a.vectors + vector_at(a, it.kv, it.first + i)] = make_float2(-INFINITY, 0.0f);
-    return;
+  memset(&it, 0, sizeof(it));
+  const int id = item_id(a, blockIdx.x, gridDim.x, lane);
+  if (id >= 0 && !item_at(a, id, kTcVecs, warp == 0, &it))
+    it.vecs = 0;
+  const bool any = it.vecs > 0 && it.p1 > it.p0;
+  const unsigned mask = __ballot_sync(0xffffffffu, any);
+  const int items = __popc(mask);
+  if (warp == 0) {
+    if (any)
+      t->items[__popc(mask & ((1u << lane) - 1))] = it;
+    for (unsigned rest = __ballot_sync(0xffffffffu, it.vecs > 0 && !any); rest; rest &= rest - 1) {
+      const int from = __ffs(rest) - 1;
+      const int vecs = __shfl_sync(0xffffffffu, it.vecs, from), first = __shfl_sync(0xffffffffu, it.first, from);
+      const int kv = __shfl_sync(0xffffffffu, it.kv, from), split = __shfl_sync(0xffffffffu, it.split, from);
+      for (int i = lane; i < vecs; i += 32)
+        a.ml[(size_t)split * a.vectors + vector_at(a, kv, first + i)] = make_float2(-INFINITY, 0.0f);
+    }
   }
+  if (!items)
+    return;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; i++) {
       mbar_init(&t->kfull[i], kConvWarps);
@@ -446,6 +522,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       mbar_init(&t->pfull[i], kSoftWarps / 2);
       mbar_init(&t->pvdone[i], 1);
     }
+    mbar_init(&t->qfull, kSoftWarps);
     t->abort_flag = 0;
     fence_mbar_init();
   }
@@ -453,99 +530,49 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     tmem_alloc(&t->tmem, kTmemCols);
   const int hd = a.hd;
   const int cw = warp - kSoftWarps - 1;
-  // Softmax warps: lane n has the index of vector warp + 8 n, and whether this thread's own vector is in use.
-  const int g = warp >> 2, vec_i = 32 * (warp & 3) + lane;
-  const bool have = warp < kSoftWarps && vec_i < it.vecs, busy = 32 * (warp & 3) < it.vecs;
-  int vec = 0;
-  bool use = false;
-  if (warp < kSoftWarps) {
-    vec = vector_at(a, it.kv, it.first + min(warp + kSoftWarps * lane, it.vecs - 1));
-    const int row = (it.first + min(vec_i, it.vecs - 1)) / a.group, b = row / a.rows;
-    use = have && row - b * a.rows < request_of(a, b).count;
-  }
   float4 *kslot = reinterpret_cast<float4 *>(smem + L::raw_at) + max(cw, 0) * (4 * HD), *vslot = kslot + 2 * HD;
-  if (cw >= 0) {
-    Rows8<HD>::copy(kslot, it.k, it.p0 + 8 * cw, it.p1, hd, lane);
+  if (cw >= 0) {  // the first tile starts on its way
+    const int from = __ffs(mask) - 1;
+    const int p0 = __shfl_sync(0xffffffffu, it.p0, from) + 8 * cw, p1 = __shfl_sync(0xffffffffu, it.p1, from);
+    Rows8<HD>::copy(kslot, shfl_ptr(it.k, from), p0, p1, hd, lane);
     copy_commit();
-    Rows8<HD>::copy(vslot, it.v, it.p0 + 8 * cw, it.p1, hd, lane);
+    Rows8<HD>::copy(vslot, shfl_ptr(it.v, from), p0, p1, hd, lane);
     copy_commit();
-  } else if (warp < kSoftWarps) {
-    // The queries into the stages, a warp per row, all rows under way at once; what lies at vectors not in use comes
-    // too and is dropped below.
-    const int e = 4 * lane;
-    if (((uintptr_t)a.q & 15) == 0) {
-#pragma unroll 4
-      for (int i = warp, n = 0; i < it.vecs; i += kSoftWarps, n++) {
-        const float *src = a.q + (size_t)__shfl_sync(0xffffffffu, vec, n) * hd;
-        if (e < HD)
-          copy16(smem_u32(smem) + (i * L::row + e) * 4, e < hd ? src + e : src, e < hd);
-      }
-      copies_done();
-    } else {
-      for (int i = warp, n = 0; i < it.vecs; i += kSoftWarps, n++) {
-        const float *src = a.q + (size_t)__shfl_sync(0xffffffffu, vec, n) * hd + e;
-        if (e < HD)
-          *reinterpret_cast<float4 *>(smem + ((size_t)i * L::row + e) * 4) =
-              e < hd ? make_float4(src[0], src[1], src[2], src[3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      }
-    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = t->tmem;
 
-  // The queries: group g's threads lay out half g of their vectors' elements. Vectors not in use are zeros.
-  const uint32_t quadrant = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-  int qshift = 0;
-  if (warp < kSoftWarps) {
-    constexpr int H = HD / 2;
-    float x[H];
-    float mx = 0.0f;
-    if (busy) {
-      const float *src = reinterpret_cast<const float *>(smem) + (size_t)vec_i * L::row + g * H;
-#pragma unroll
-      for (int e = 0; e < H; e += 4) {
-        const float4 y = use ? *reinterpret_cast<const float4 *>(src + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        x[e] = y.x, x[e + 1] = y.y, x[e + 2] = y.z, x[e + 3] = y.w;
-        mx = abs_max(mx, y);
-      }
-    }
-    t->qmax[g][vec_i] = mx;
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
-    qshift = shift_for(__float_as_uint(fmaxf(t->qmax[0][vec_i], t->qmax[1][vec_i])));
-    if (busy) {
-      const uint64_t f = f2_pack(pow2(qshift), pow2(qshift));
-#pragma unroll
-      for (int c = 0; c < H; c += 32) {
-        uint32_t hi[16], lo[16];
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-          split2(f2_mul(f2_pack(x[c + 2 * e], x[c + 2 * e + 1]), f), hi[e], lo[e]);
-        tmem_st16(quadrant + kTmemQ + (g * H + c) / 2, hi);
-        tmem_st16(quadrant + kTmemQ + 64 + (g * H + c) / 2, lo);
-      }
-      tmem_wait_st();
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-
   if (warp > kSoftWarps) {
     // ---- converters ----
     // Registers hold tile j, the slots tile j + 1 as it comes. Every copy is a group of its own, empty past the last.
+    // The tiles of all items are one sequence; `ahead` is the tile that is fetched next.
     Rows8<HD> kx, vx;
-    auto next = [&](Rows8<HD> &x, float4 *slot, const float *cache, int tile) {
+    const float *ck = t->items[0].k, *cv = t->items[0].v;
+    int ahead = 0, at = t->items[0].p0 + 8 * cw, end = t->items[0].p1;
+    auto advance = [&]() {
+      at += kTcPos;
+      if (at - 8 * cw >= end && ahead < items && ++ahead < items) {
+        const Item &it = t->items[ahead];
+        ck = it.k, cv = it.v, at = it.p0 + 8 * cw, end = it.p1;
+      }
+    };
+    auto next = [&](Rows8<HD> &x, float4 *slot, const float *cache) {
       copy_wait1();
       x.take(slot, lane);
-      if (tile < tiles)
-        Rows8<HD>::copy(slot, cache, it.p0 + tile * kTcPos + 8 * cw, it.p1, hd, lane);
+      if (ahead < items)
+        Rows8<HD>::copy(slot, cache, at, end, hd, lane);
       copy_commit();
     };
-    next(kx, kslot, it.k, 1);
-    next(vx, vslot, it.v, 1);
+    int tiles = 0;
+    for (int n = 0; n < items; n++)
+      tiles += tiles_of(t->items[n]);
+    advance();
+    next(kx, kslot, ck);
+    next(vx, vslot, cv);
     for (int j = 0; j < tiles; j++) {
+      advance();
       const int s = j & 1, use = j >> 1;
       uint8_t *stage = smem + s * L::stage;
       tc_wait(&t->kempty[s], (use & 1) ^ 1, abort_flag);
@@ -556,7 +583,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&t->kfull[s]);
-      next(kx, kslot, it.k, j + 2);
+      next(kx, kslot, ck);
       tc_wait(&t->vempty[s], (use & 1) ^ 1, abort_flag);
       const int vs = vx.store(stage + 2 * L::kv_bytes, stage + 3 * L::kv_bytes, 8 * cw, lane);
       if (lane == 0)
@@ -565,11 +592,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&t->vfull[s]);
-      next(vx, vslot, it.v, j + 2);
+      next(vx, vslot, cv);
     }
   } else if (warp == kSoftWarps) {
-    // ---- MMA issue. The scores of tile j + 1 go out before the sums of tile j, so that they run under its softmax; the
-    // MMAs run in the order of issue, so the scores of tile j + 2 never overtake the sums that read their buffer. ----
+    // ---- MMA issue. The scores of tile j + 1 go out before the sums of tile j, so that they run under its softmax, or
+    // after them where they have to wait for the next item's queries. The MMAs run in the order of issue, so the scores
+    // of tile j + 2 never overtake the sums that read their buffer. ----
     const bool leader = elect_one();
     const uint32_t idesc_s = umma_idesc_f16(kTcVecs, kTcPos, false), idesc_o = umma_idesc_f16(kTcVecs, HD, true);
     const uint64_t kdesc = umma_desc_sw128(smem), vdesc = umma_desc_sw128_mn(smem + 2 * L::kv_bytes, kTcPos * 128);
@@ -593,9 +621,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       }
       __syncwarp();
     };
-    scores(0);
-    for (int j = 0; j < tiles; j++) {
-      if (j + 1 < tiles)
+    if (tc_wait(&t->qfull, 0, abort_flag))
+      scores(0);
+    int first = 0, last = tiles_of(t->items[0]) - 1;  // the item's tiles
+    for (int j = 0, n = 0;; j++) {
+      if (j < last)
         scores(j + 1);
       const int s = j & 1, use = j >> 1;
       if (!tc_wait(&t->vfull[s], use & 1, abort_flag) || !tc_wait(&t->pfull[s], use & 1, abort_flag))
@@ -609,172 +639,258 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
 #pragma unroll
           for (int c = 0; c < kTcPos / 16; c++)  // 32 positions: 16 columns of hi, 16 of lo
             umma_f16_ta(d, p + 32 * (c >> 1) + 8 * (c & 1) + (term == 0 ? 16 : 0),
-                        vd + ((term == 1 ? L::kv_bytes : 0) + 2048 * c) / 16, idesc_o, j > 1 || term || c);
+                        vd + ((term == 1 ? L::kv_bytes : 0) + 2048 * c) / 16, idesc_o, j > first + 1 || term || c);
         umma_commit(&t->pvdone[s]);
         umma_commit(&t->vempty[s]);
       }
       __syncwarp();
+      if (j == last) {
+        if (++n == items || !tc_wait(&t->qfull, n & 1, abort_flag))
+          break;
+        scores(j + 1);
+        first = j + 1, last = j + tiles_of(t->items[n]);
+      }
     }
   } else {
     // ---- softmax: a thread per query vector, group g the tiles of its parity ----
+    const int g = warp >> 2, vec_i = 32 * (warp & 3) + lane;
+    const uint32_t quadrant = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     const uint32_t ts = quadrant + kTmemS + 64 * g, to = quadrant + kTmemO + 128 * g;
-    const int limit = have ? limit_of(a, it, it.first + vec_i) : it.p0;
-    const int lowest = __reduce_min_sync(0xffffffffu, have ? limit : 0x7fffffff);
-    const float scale = rsqrtf((float)hd) * kLog2e * pow2(-qshift);
-    float m = -INFINITY, l = 0.0f;
-    int vref = 0;  // O holds sums times 2^(kPShift + vref)
-    for (int j = g; j < tiles; j += 2) {
-      const int use = j >> 1;
-      // The scores, the values' powers, and the group's previous sums: O can be rescaled. (Those are done when the
-      // scores are; the wait keeps step with the barrier's phases.)
-      if (!tc_wait(&t->sfull[g], use & 1, abort_flag) || !tc_wait(&t->vfull[g], use & 1, abort_flag) ||
-          (use > 0 && !tc_wait(&t->pvdone[g], (use - 1) & 1, abort_flag)))
-        break;
-      tc_fence_after();
-      if (busy) {
-        const int p0 = it.p0 + j * kTcPos;
-        const bool masked = p0 + kTcPos > lowest;
-        const float *kscale = t->kscale[j & 3];
-        const int *vshift = t->vshift[j & 3];
-        auto factor = [&](int c8) {  // never 0: a masked score's -infinity has to stay one
-          return fmaxf(scale * kscale[c8], FLT_MIN);
-        };
-        // Two passes over the scores in TMEM, 32 at a time: their maximum, then the probabilities.
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < 64; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(ts + c, r);
-          tmem_wait_ld();
-          if (masked)
+    // A vector's index, -1 for one that is not in use.
+    auto vector_of = [&](const Item &it) {
+      const int i = it.first + min(vec_i, it.vecs - 1), row = i / a.group, b = row / a.rows;
+      return vec_i < it.vecs && row - b * a.rows < request_of(a, b).count ? vector_at(a, it.kv, i) : -1;
+    };
+    int vec = -1, vec_ahead = vector_of(t->items[0]);
+    for (int n = 0, j0 = 0, j1 = 0;; n++) {
+      const int at = vec;
+      if (n < items) {
+        // The queries become the A operand in TMEM once the scores of the tiles before are done. Group g's warps lay out
+        // 16 of the quadrant's rows: lanes have four neighbouring elements of rows lane / 4 and lane / 4 + 8, whole
+        // sectors of global memory and the layout in which they go to TMEM. Vectors not in use are zeros.
+        vec = vec_ahead;
+        constexpr int kParts = HD / 16;
+        if (32 * (warp & 3) < t->items[n].vecs) {
+          float4 x[2][kParts];
 #pragma unroll
-            for (int e = 0; e < 32; e++)
-              r[e] = p0 + c + e < limit ? r[e] : 0xff800000u;
-#pragma unroll
-          for (int e8 = 0; e8 < 32; e8 += 8) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-              x[e] = __uint_as_float(r[e8 + e]);
-            top = fmaxf(top, max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7])) *
-                                 factor((c + e8) >> 3));
+          for (int r = 0; r < 2; r++) {
+            const int from = __shfl_sync(0xffffffffu, vec, 16 * g + (lane >> 2) + 8 * r);
+            load_row<HD>(x[r], a.q + (size_t)max(from, 0) * hd + 4 * (lane & 3), from < 0 ? 0 : hd - 4 * (lane & 3));
           }
-        }
-        int vmin = vshift[0];
+          int k[2];
 #pragma unroll
-        for (int w = 1; w < kConvWarps; w++)
-          vmin = min(vmin, vshift[w]);
-        // Move the reference when a score exceeds it by more than 8, and O's power when the values have grown.
-        const bool up = top > m + 8.0f || (m == -INFINITY && top > m);
-        const float m_new = up ? ceilf(top) : m;
-        const int vref_new = use == 0 || vmin < vref ? vmin - 1 : vref;
-        const float keep = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - m_new);
-        if (use > 0 && (vref_new != vref || __any_sync(0xffffffffu, up))) {
-          const float f = keep * pow2(vref_new - vref);
-#pragma unroll 1
-          for (int c = 0; c < HD; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(to + c, o);
-            tmem_wait_ld();
+          for (int r = 0; r < 2; r++) {
+            float mx = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-              o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st16(to + c, o);
+            for (int c = 0; c < kParts; c++)
+              mx = abs_max(mx, x[r][c]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            k[r] = shift_for(__float_as_uint(mx));
+            if ((lane & 3) == 0)
+              t->qshift[n & 1][32 * (warp & 3) + 16 * g + (lane >> 2) + 8 * r] = k[r];
           }
-        }
-        l *= keep;
-        m = m_new;
-        vref = vref_new;
-        const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll 1
-        for (int c = 0; c < 64; c += 32) {
-          uint32_t r[32], hi[16], lo[16];
-          tmem_ld32(ts + c, r);
-          tmem_wait_ld();
-          if (masked)
+          if (n)
+            tc_wait(&t->sfull[(j1 - 1) & 1], ((j1 - 1) >> 1) & 1, abort_flag);
+          tc_fence_after();
+          const uint32_t to_q = quadrant + ((uint32_t)(16 * g) << 16) + kTmemQ;
 #pragma unroll
-            for (int e = 0; e < 32; e++)
-              r[e] = p0 + c + e < limit ? r[e] : 0xff800000u;
+          for (int c0 = 0; c0 < kParts; c0 += 4) {
+            uint32_t hi[16], lo[16];
 #pragma unroll
-          for (int e8 = 0; e8 < 32; e8 += 8) {
-            // 2^(score - m) times 2^grow, the values' power in the exponent: base and grow are whole numbers. Values
-            // 2^-60 of the largest seen (zeros, mostly) count as that at most, which O does not hold.
-            const float f = factor((c + e8) >> 3);
-            const int grow = max(kPShift - vshift[(c + e8) >> 3] + vref, -60);
-            const float from = (float)grow - base;
-            const uint64_t f2 = f2_pack(f, f), from2 = f2_pack(from, from);
-            uint64_t sum2 = 0;
+            for (int r = 0; r < 2; r++) {
+              const uint64_t f = f2_pack(pow2(k[r]), pow2(k[r]));
 #pragma unroll
-            for (int e = e8; e < e8 + 8; e += 2) {
-              float x, y;
-              f2_unpack(f2_fma(f2_pack_bits(r[e], r[e + 1]), f2, from2), x, y);
-              const uint64_t p = f2_pack(ex2(x), ex2(y));
-              sum2 = f2_add(sum2, p);
-              split2(p, hi[e / 2], lo[e / 2]);
+              for (int c = 0; c < 4; c++) {
+                const float4 y = x[r][c0 + c];
+                split2(f2_mul(f2_pack(y.x, y.y), f), hi[4 * c + 2 * r], lo[4 * c + 2 * r]);
+                split2(f2_mul(f2_pack(y.z, y.w), f), hi[4 * c + 2 * r + 1], lo[4 * c + 2 * r + 1]);
+              }
             }
-            float s0, s1;
-            f2_unpack(sum2, s0, s1);
-            l = fmaf(s0 + s1, pow2(-grow), l);
+            tmem_st_rows(to_q + 8 * c0, hi);
+            tmem_st_rows(to_q + 64 + 8 * c0, lo);
           }
-          tmem_st16(ts + c, hi);
-          tmem_st16(ts + c + 16, lo);
+          tmem_wait_st();
         }
-        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&t->qfull);
+        if (n + 1 < items)
+          vec_ahead = vector_of(t->items[n + 1]);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0)
-        mbar_arrive(&t->pfull[g]);
-    }
-    // The two groups' results joined, by way of the stages (no MMA reads them any more), into the partial result.
-    t->m[g][vec_i] = m, t->l[g][vec_i] = l, t->vref[g][vec_i] = vref;
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
-    const bool done = tc_wait(&t->pvdone[0], ((tiles - 1) >> 1) & 1, abort_flag) &&
-                      (tiles < 2 || tc_wait(&t->pvdone[1], ((tiles - 2) >> 1) & 1, abort_flag));
-    // Group g joins half g of the elements.
-    if (done && busy) {
-      tc_fence_after();
-      const float m0 = t->m[0][vec_i], m1 = t->m[1][vec_i], both = fmaxf(m0, m1);
-      const float w0 = m0 == -INFINITY ? 0.0f : ex2(m0 - both), w1 = m1 == -INFINITY ? 0.0f : ex2(m1 - both);
-      if (have && g == 0)
-        a.ml[(size_t)it.split * a.vectors + vector_at(a, it.kv, it.first + vec_i)] =
-            make_float2(both, w0 * t->l[0][vec_i] + w1 * t->l[1][vec_i]);
-      const int d0 = -(kPShift + t->vref[0][vec_i]), d1 = -(kPShift + t->vref[1][vec_i]);
-      const float f0 = w0 * pow2(d0 / 2), f1 = w1 * pow2(d1 / 2);  // 2^d itself may not be a number
-      const float g0 = pow2(d0 - d0 / 2), g1 = pow2(d1 - d1 / 2);
-      float *row = reinterpret_cast<float *>(smem) + (size_t)vec_i * L::row;
-      const uint32_t from = quadrant + kTmemO;
+      if (n) {
+        // Item n - 1: the two groups' results joined into the partial result, 16 rows of the quadrant by each, in the
+        // layout of the queries.
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
+        const Item &from_it = t->items[n - 1];
+        const int last0 = j1 - 1 - ((j1 - 1) & 1), last1 = j1 - 1 - (j1 & 1);  // the groups' last tiles
+        const bool has0 = last0 >= j0, has1 = last1 >= j0;
+        bool done = !has0 || tc_wait(&t->pvdone[0], (last0 >> 1) & 1, abort_flag);
+        done = (!has1 || tc_wait(&t->pvdone[1], (last1 >> 1) & 1, abort_flag)) && done;
+        if (done && 32 * (warp & 3) < from_it.vecs) {
+          tc_fence_after();
+          const float m0 = t->m[0][vec_i], m1 = t->m[1][vec_i], both = fmaxf(m0, m1);
+          const float w0 = m0 == -INFINITY ? 0.0f : ex2(m0 - both), w1 = m1 == -INFINITY ? 0.0f : ex2(m1 - both);
+          if (at >= 0 && g == 0)
+            a.ml[(size_t)from_it.split * a.vectors + at] = make_float2(both, w0 * t->l[0][vec_i] + w1 * t->l[1][vec_i]);
+          // Powers between 2^-106 and 2^107.
+          const float f0 = w0 * pow2(-(kPShift + t->vref[0][vec_i])), f1 = w1 * pow2(-(kPShift + t->vref[1][vec_i]));
+          float *part = a.acc + (size_t)from_it.split * a.vectors * hd + 2 * (lane & 3);
+          float *dst[2];
+          uint64_t s0[2], s1[2];
+          bool in[2];
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            const int row = 16 * g + (lane >> 2) + 8 * r;
+            const float x0 = __shfl_sync(0xffffffffu, f0, row), x1 = __shfl_sync(0xffffffffu, f1, row);
+            s0[r] = f2_pack(x0, x0), s1[r] = f2_pack(x1, x1);
+            const int to_vec = __shfl_sync(0xffffffffu, at, row);
+            in[r] = to_vec >= 0;
+            dst[r] = part + (size_t)max(to_vec, 0) * hd;
+          }
+          const uint32_t from = quadrant + ((uint32_t)(16 * g) << 16) + kTmemO;
+          if (32 * (warp & 3) + 16 * g < from_it.vecs)
 #pragma unroll 1
-      for (int c = g * (HD / 2); c < (g + 1) * (HD / 2); c += 16) {
-        uint32_t o[16], p[16];
-        tmem_ld16(from + c, o);
-        if (tiles > 1)
-          tmem_ld16(from + 128 + c, p);
-        tmem_wait_ld();
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[16], p[16];
+              tmem_ld_rows(from + c, o);
+              tmem_ld_rows(from + 128 + c, p);
+              tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          float y[4];
-#pragma unroll
-          for (int n = 0; n < 4; n++) {
-            y[n] = __uint_as_float(o[e + n]) * f0 * g0;
-            if (tiles > 1)
-              y[n] += __uint_as_float(p[e + n]) * f1 * g1;
-          }
-          *reinterpret_cast<float4 *>(row + c + e) = make_float4(y[0], y[1], y[2], y[3]);
+              for (int e = 0; e < 16; e += 2) {
+                const int r = e >> 1 & 1, col = c + 2 * (e & 12);
+                const uint64_t zero = f2_pack(0.0f, 0.0f);
+                const uint64_t y0 = has0 ? f2_mul(f2_pack_bits(o[e], o[e + 1]), s0[r]) : zero;
+                const uint64_t y = has1 ? f2_fma(f2_pack_bits(p[e], p[e + 1]), s1[r], y0) : y0;
+                float2 z;
+                f2_unpack(y, z.x, z.y);
+                if (in[r] && col + 2 * (lane & 3) < hd)
+                  *reinterpret_cast<float2 *>(dst[r] + col) = z;
+              }
+            }
+          tc_fence_before();
         }
+        if (n == items)
+          break;
+        // Only now may the next item's first sums overwrite O, and its results what the other group reads here.
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
       }
-      tc_fence_before();
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
-    if (done) {
-      const int e = 4 * lane;
-      float *part = a.acc + (size_t)it.split * a.vectors * hd + e;
-#pragma unroll 4
-      for (int i = warp, n = 0; i < it.vecs; i += kSoftWarps, n++) {
-        float *dst = part + (size_t)__shfl_sync(0xffffffffu, vec, n) * hd;
-        if (e < hd)
-          *reinterpret_cast<float4 *>(dst) = *reinterpret_cast<const float4 *>(smem + ((size_t)i * L::row + e) * 4);
+      tc_wait(&t->qfull, n & 1, abort_flag);
+      const int qshift = t->qshift[n & 1][vec_i];
+      const Item &it = t->items[n];
+      j0 = j1, j1 += tiles_of(it);
+      const bool have = vec_i < it.vecs, busy = 32 * (warp & 3) < it.vecs;
+      const int limit = have ? limit_of(a, it, it.first + vec_i) : it.p0;
+      const int lowest = __reduce_min_sync(0xffffffffu, have ? limit : 0x7fffffff);
+      const float scale = rsqrtf((float)hd) * kLog2e * pow2(-qshift);
+      float m = -INFINITY, l = 0.0f;
+      int vref = 0;  // O holds sums times 2^(kPShift + vref)
+      for (int j = j0 + ((j0 ^ g) & 1); j < j1; j += 2) {
+        const int use = j >> 1;
+        const bool begin = j < j0 + 2;
+        // The scores, the values' powers, and the group's previous sums: O can be rescaled. (Those are done when the
+        // scores are; the wait keeps step with the barrier's phases.)
+        if (!tc_wait(&t->sfull[g], use & 1, abort_flag) || !tc_wait(&t->vfull[g], use & 1, abort_flag) ||
+            (use > 0 && !tc_wait(&t->pvdone[g], (use - 1) & 1, abort_flag)))
+          break;
+        tc_fence_after();
+        if (busy) {
+          const int p0 = it.p0 + (j - j0) * kTcPos;
+          const bool masked = p0 + kTcPos > lowest;
+          const float *kscale = t->kscale[j & 3];
+          const int *vshift = t->vshift[j & 3];
+          auto factor = [&](int c8) {  // never 0: a masked score's -infinity has to stay one
+            return fmaxf(scale * kscale[c8], FLT_MIN);
+          };
+          // Two passes over the scores in TMEM, 32 at a time: their maximum, then the probabilities.
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(ts + c, r);
+            tmem_wait_ld();
+            if (masked)
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                r[e] = p0 + c + e < limit ? r[e] : 0xff800000u;
+#pragma unroll
+            for (int e8 = 0; e8 < 32; e8 += 8) {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                x[e] = __uint_as_float(r[e8 + e]);
+              top = fmaxf(top, max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7])) *
+                                   factor((c + e8) >> 3));
+            }
+          }
+          int vmin = vshift[0];
+#pragma unroll
+          for (int w = 1; w < kConvWarps; w++)
+            vmin = min(vmin, vshift[w]);
+          // Move the reference when a score exceeds it by more than 8, and O's power when the values have grown.
+          const bool up = top > m + 8.0f || (m == -INFINITY && top > m);
+          const float m_new = up ? ceilf(top) : m;
+          const int vref_new = begin || vmin < vref ? vmin - 1 : vref;
+          const float keep = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - m_new);
+          if (!begin && (vref_new != vref || __any_sync(0xffffffffu, up))) {
+            const float f = keep * pow2(vref_new - vref);
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(to + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; e++)
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(to + c, o);
+            }
+          }
+          l *= keep;
+          m = m_new;
+          vref = vref_new;
+          const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t r[32], hi[16], lo[16];
+            tmem_ld32(ts + c, r);
+            tmem_wait_ld();
+            if (masked)
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                r[e] = p0 + c + e < limit ? r[e] : 0xff800000u;
+#pragma unroll
+            for (int e8 = 0; e8 < 32; e8 += 8) {
+              // 2^(score - m) times 2^grow, the values' power in the exponent: base and grow are whole numbers. Values
+              // 2^-60 of the largest seen (zeros, mostly) count as that at most, which O does not hold.
+              const float f = factor((c + e8) >> 3);
+              const int grow = max(kPShift - vshift[(c + e8) >> 3] + vref, -60);
+              const float from = (float)grow - base;
+              const uint64_t f2 = f2_pack(f, f), from2 = f2_pack(from, from);
+              uint64_t sum2 = 0;
+#pragma unroll
+              for (int e = e8; e < e8 + 8; e += 2) {
+                float x, y;
+                f2_unpack(f2_fma(f2_pack_bits(r[e], r[e + 1]), f2, from2), x, y);
+                const uint64_t p = f2_pack(ex2(x), ex2(y));
+                sum2 = f2_add(sum2, p);
+                split2(p, hi[e / 2], lo[e / 2]);
+              }
+              float s0, s1;
+              f2_unpack(sum2, s0, s1);
+              l = fmaf(s0 + s1, pow2(-grow), l);
+            }
+            tmem_st16(ts + c, hi);
+            tmem_st16(ts + c + 16, lo);
+          }
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&t->pfull[g]);
       }
+      t->m[g][vec_i] = m, t->l[g][vec_i] = l, t->vref[g][vec_i] = vref;
     }
   }
   __syncthreads();
@@ -785,11 +901,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
 }
 
 template <int HD>
-cudaError_t launch_tc(const SharedArgs &a, unsigned items) {
+cudaError_t launch_tc(const SharedArgs &a, unsigned ctas) {
   const cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(shared_tc_kernel<HD>), TcSmem<HD>::total);
   return e != cudaSuccess ? e
-                          : kc_launch_pdl(shared_tc_kernel<HD>, dim3(items), dim3(kTcThreads), TcSmem<HD>::total,
-                                          kc_stream(), a);
+                          : kc_launch_pdl(shared_tc_kernel<HD>, dim3(ctas), dim3(kTcThreads),
+                                          TcSmem<HD>::total, kc_stream(), a);
 }
 
 // Heads of whole 16-byte units at 16-byte addresses.
@@ -900,6 +1016,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs a) {
 }
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
+long long ceil_div64(long long a, long long b) { return (a + b - 1) / b; }
 
 bool shape_ok(int n_heads, int n_kv, int hd, int batch, int rows) {
   return n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && hd > 0 && hd <= kMaxHd && batch > 0 && rows > 0 &&
@@ -919,37 +1036,55 @@ size_t partial_floats(int n_heads, int hd, int batch, int rows) {
 }
 
 // How the positions are split, `most` splits at most, two at least: the lengths whose CTAs are estimated to end first.
-// In units of a tile of 64 positions against a query tile (about 1.6 us): a CTA takes kStart units besides its tiles, the
-// requests' caches are taken to be half full, CTAs beyond one wave fill the gaps the longest one leaves half of, and a
-// split costs its partial results' way to memory and back. No more than kLongest tiles to a split: the tensor cores'
-// accumulators truncate, which over more tiles would show in the result.
-constexpr int kStart = 4, kLongest = 16;
-void plan_splits(SharedArgs *a, int most) {
+// In units of a tile of 64 positions against a query tile (about 1.5 us): an item takes kItem units besides its tiles,
+// and kItemFull more with a whole tile of queries to bring and of results to write; the requests' caches are taken to be
+// half full; a split costs its partial results' way to memory and back. No more than kLongest tiles to a split: the
+// tensor cores' accumulators truncate, which over more tiles would show in the result.
+// Returns the CTAs, one per SM, or more where each would have more than kMaxItems items.
+constexpr double kItem = 2.2, kItemFull = 1.2;
+constexpr int kLongest = 16;
+int plan_splits(SharedArgs *a, int most) {
   const int prefix_tiles = ceil_div(a->prefix, kTcPos), own_tiles = ceil_div(a->seq, kTcPos);
-  const double columns = (double)a->n_kv * a->tiles, own_columns = (double)a->n_kv * a->batch * a->own_tiles;
-  const double pass = (double)a->vectors * (a->hd + 2) * 8 / 5e12 / 1.6e-6;  // a split's partial results
+  const int columns = a->n_kv * a->tiles, own_columns = a->n_kv * a->batch * a->own_tiles;
+  const int vecs = a->batch * a->rows * a->group, own_vecs = a->rows * a->group;
+  const double item = kItem + kItemFull * (vecs < kTcVecs ? vecs : kTcVecs) / kTcVecs;
+  const double own_item = kItem + kItemFull * (own_vecs < kTcVecs ? own_vecs : kTcVecs) / kTcVecs;
+  const double pass = (double)a->vectors * (a->hd + 2) * 8 / 5e12 / 1.5e-6;  // a split's partial results
   const int most_own = most / 2 < kMaxSplits ? most / 2 : kMaxSplits;
   double best = 0.0;
+  int ctas = 1;
   for (int own_length = own_tiles < kLongest ? own_tiles : kLongest; own_length >= 1; own_length -= own_length > 4 ? 2 : 1) {
     const int own = ceil_div(own_tiles, own_length) < most_own ? ceil_div(own_tiles, own_length) : most_own;
     const int rest = most - own < kMaxSplits ? most - own : kMaxSplits;
     for (int length = prefix_tiles < kLongest ? prefix_tiles : kLongest; length >= (prefix_tiles ? 1 : 0); length--) {
       int n = prefix_tiles ? ceil_div(prefix_tiles, length) : 0;
       n = n < rest ? n : rest;
-      const double c = n ? kStart + (double)prefix_tiles / n : 0.0, c_own = kStart + 0.5 * own_tiles / own;
-      const double items = columns * n + own_columns * own, work = columns * n * c + own_columns * own * c_own;
-      const double longest = c > c_own ? c : c_own;
-      double t = items <= kPlanSms ? longest : work / kPlanSms + 0.5 * longest;
-      t = (t > longest ? t : longest) + pass * (n + own);
+      const double c = n ? item + (double)prefix_tiles / n : 0.0, c_own = own_item + 0.5 * own_tiles / own;
+      const long long p = (long long)columns * n, o = (long long)own_columns * own;
+      long long g = p + o < kPlanSms ? p + o : kPlanSms;
+      if (ceil_div64(p + o, kMaxItems - 4) > g)  // fewer than kMaxItems with up to 3 extra ones
+        g = ceil_div64(p + o, kMaxItems - 4);
+      const long long heavy = p % g, light = g - heavy;
+      const int want = (int)(c / c_own + 0.5);
+      long long extra = heavy ? o / light : 0;
+      extra = extra < want ? extra : want;
+      extra = extra < 3 ? extra : 3;
+      const long long turn = o - extra * light;
+      const double end_heavy = (p / g + 1) * c + (turn / g + (turn % g > light)) * c_own;
+      const double end_light = (p / g) * c + (extra + turn / g + (turn % g > 0)) * c_own;
+      const double t = (heavy && end_heavy > end_light ? end_heavy : end_light) + pass * (n + own);
       if (best == 0.0 || t < best) {
         best = t;
         a->prefix_splits = n;
         a->own_splits = own;
+        a->extra = (int)extra;
+        ctas = (int)g;
       }
       if (!prefix_tiles)
         break;
     }
   }
+  return ctas;
 }
 
 size_t generic_smem(int hd) { return sizeof(float) * ((size_t)kGenericPos * (2 * hd + 1) + 4 * (size_t)hd); }
@@ -1028,7 +1163,7 @@ void k_attention_shared_rows(float *out, int8_t *oq, float *os, const float *q, 
   const int tile = tc ? kTcVecs : kGenericVecs;
   a.tiles = ceil_div(batch * rows * a.group, tile);
   a.own_tiles = ceil_div(rows * a.group, tile);
-  plan_splits(&a, (int)((work->capacity - 4) / ((size_t)a.vectors * (head_dim + 2))));
+  const int ctas = plan_splits(&a, (int)((work->capacity - 4) / ((size_t)a.vectors * (head_dim + 2))));
   const size_t splits = (size_t)a.prefix_splits + a.own_splits;
   a.ml = reinterpret_cast<float2 *>(work->partial);
   a.acc = work->partial + pairs_floats(splits * a.vectors);
@@ -1040,7 +1175,7 @@ void k_attention_shared_rows(float *out, int8_t *oq, float *os, const float *q, 
   }
   cudaError_t e;
   if (tc) {
-    e = head_dim > 64 ? launch_tc<128>(a, (unsigned)items) : launch_tc<64>(a, (unsigned)items);
+    e = head_dim > 64 ? launch_tc<128>(a, ctas) : launch_tc<64>(a, ctas);
   } else {
     e = kc_allow_smem(reinterpret_cast<const void *>(shared_generic_kernel), (int)generic_smem(kMaxHd));
     if (e == cudaSuccess)

@@ -30,6 +30,29 @@ constexpr int kGenericThreads = 128;
 constexpr int kGenericVecs = 32;   // query vectors per CTA
 constexpr int kGenericPos = 32;    // positions per tile
 
+// Division by a number known on the host, by multiplication (Granlund and Montgomery): exact for n < 2^31.
+struct Divisor {
+  int d;
+  unsigned m, shift;
+};
+Divisor divisor(int d) {
+  unsigned l = 0;
+  while ((1ll << l) < d)
+    l++;
+  return Divisor{d, (unsigned)(((1ull << 32) * ((1ull << l) - (unsigned)d)) / (unsigned)d + 1), l};
+}
+// n / by, and n becomes the rest.
+__host__ __device__ __forceinline__ int divide(int &n, const Divisor &by) {
+#ifdef __CUDA_ARCH__
+  const unsigned high = __umulhi((unsigned)n, by.m);
+#else
+  const unsigned high = (unsigned)(((unsigned long long)(unsigned)n * by.m) >> 32);
+#endif
+  const int q = (int)((high + (unsigned)n) >> by.shift);
+  n -= q * by.d;
+  return q;
+}
+
 struct SharedArgs {
   const float *q;             // [batch][rows][n_heads][hd]
   const float *pk, *pv;       // [n_kv][prefix_seq][hd]
@@ -44,7 +67,9 @@ struct SharedArgs {
   int vectors;                // batch * rows * n_heads
   int prefix_splits, own_splits;  // splits of the positions
   int tiles, own_tiles;           // query tiles per KV head: of the prefix part, of a request's own part
-  int extra;                      // items that a CTA with one item less of the prefix takes before the rest
+  // The items' turns: CTAs below `heavy` have per_cta + 1 of the prefix's, the others per_cta and `extra` before the rest.
+  int per_cta, heavy, extra;
+  Divisor by_prefix_splits, by_own_splits, by_kv, by_own_tiles, by_group, by_rows;
 };
 
 // Rows that request b uses and the positions it has stored before them; 0 rows where they are not sound. Both loads go
@@ -73,7 +98,7 @@ struct Item {
 // requests' own, `extra` to each of the others, then the rest in turn, the others first. -1 past the last.
 __host__ __device__ __forceinline__ int item_id(const SharedArgs &a, int cta, int ctas, int n) {
   const int prefix = a.n_kv * a.tiles * a.prefix_splits, own = a.n_kv * a.batch * a.own_tiles * a.own_splits;
-  const int heavy = prefix % ctas, light = ctas - heavy, mine = prefix / ctas + (cta < heavy);
+  const int heavy = a.heavy, light = ctas - heavy, mine = a.per_cta + (cta < heavy);
   if (n < mine)
     return cta + n * ctas;
   n -= mine;
@@ -92,7 +117,25 @@ __host__ __device__ __forceinline__ int item_id(const SharedArgs &a, int cta, in
 
 // Vector i of KV head kv's flat list: index in the [batch][rows][n_heads] order.
 __device__ __forceinline__ int vector_at(const SharedArgs &a, int kv, int i) {
-  return (i / a.group) * a.n_heads + kv * a.group + i % a.group;
+  const int row = divide(i, a.by_group);
+  return row * a.n_heads + kv * a.group + i;
+}
+
+// Index of the tile's vector i, -1 for one that is not in use.
+__device__ __forceinline__ int vector_of(const SharedArgs &a, int first, int vecs, int kv, int i) {
+  int member = first + min(i, vecs - 1);
+  int row = divide(member, a.by_group);
+  const int vec = row * a.n_heads + kv * a.group + member;
+  const int b = divide(row, a.by_rows);
+  return i < vecs && row < request_of(a, b).count ? vec : -1;
+}
+
+// The positions of one of the splits of `length`, which differ by one at most.
+__device__ __forceinline__ void split_range(int length, int split, const Divisor &by_splits, Item *it) {
+  int longer = length;
+  const int each = divide(longer, by_splits);
+  it->p0 = each * split + min(split, longer);
+  it->p1 = it->p0 + each + (split < longer);
 }
 
 // Items 0 .. n_kv * tiles * prefix_splits - 1 are the prefix's, then one per (request, KV head, query tile, split).
@@ -100,26 +143,25 @@ __device__ __forceinline__ int vector_at(const SharedArgs &a, int kv, int i) {
 __device__ __forceinline__ bool item_at(const SharedArgs &a, int id, int tile, bool report, Item *it) {
   const int prefix_items = a.n_kv * a.tiles * a.prefix_splits;
   if (id < prefix_items) {
-    it->split = id % a.prefix_splits;
-    id /= a.prefix_splits;
-    it->kv = id % a.n_kv;
+    int kv = divide(id, a.by_prefix_splits);
+    it->split = id;
+    it->first = divide(kv, a.by_kv) * tile;
+    it->kv = kv;
     it->b = -1;
-    it->first = id / a.n_kv * tile;
     it->vecs = min(tile, a.batch * a.rows * a.group - it->first);
     it->k = a.pk + (size_t)it->kv * a.prefix_seq * a.hd;
     it->v = a.pv + (size_t)it->kv * a.prefix_seq * a.hd;
-    it->p0 = (int)((long long)a.prefix * it->split / a.prefix_splits);
-    it->p1 = (int)((long long)a.prefix * (it->split + 1) / a.prefix_splits);
+    split_range(a.prefix, id, a.by_prefix_splits, it);
     return true;
   }
   id -= prefix_items;
-  const int split = id % a.own_splits;
-  id /= a.own_splits;
+  int own_tile = divide(id, a.by_own_splits);
+  const int split = id;
   it->split = a.prefix_splits + split;
-  const int own_tile = id % a.own_tiles * tile;
-  id /= a.own_tiles;
-  it->kv = id % a.n_kv;
-  it->b = id / a.n_kv;
+  int kv = divide(own_tile, a.by_own_tiles);
+  own_tile *= tile;
+  it->b = divide(kv, a.by_kv);
+  it->kv = kv;
   const Request r = request_of(a, it->b);
   if (!r.count) {
     if (r.bad && report)
@@ -134,9 +176,7 @@ __device__ __forceinline__ bool item_at(const SharedArgs &a, int id, int tile, b
   it->k = a.k + head;
   it->v = a.v + head;
   it->start = r.start;
-  const int length = r.start + r.count;
-  it->p0 = (int)((long long)length * split / a.own_splits);
-  it->p1 = (int)((long long)length * (split + 1) / a.own_splits);
+  split_range(r.start + r.count, split, a.by_own_splits, it);
   return true;
 }
 
@@ -144,7 +184,8 @@ __device__ __forceinline__ bool item_at(const SharedArgs &a, int id, int tile, b
 __device__ __forceinline__ int limit_of(const SharedArgs &a, const Item &it, int i) {
   if (it.b < 0)
     return it.p1;
-  return min(it.p1, it.start + (i - it.b * a.rows * a.group) / a.group + 1);
+  i -= it.b * a.rows * a.group;
+  return min(it.p1, it.start + divide(i, a.by_group) + 1);
 }
 
 // Any head_dim up to 256 and any alignment, in fp32 FMAs: a warp takes 8 of the tile's 32 vectors in turn, its lanes
@@ -539,6 +580,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     Rows8<HD>::copy(vslot, shfl_ptr(it.v, from), p0, p1, hd, lane);
     copy_commit();
   }
+  int vec_ahead = 0;  // softmax warps: the vector of the next item
+  if (warp < kSoftWarps) {
+    const int from = __ffs(mask) - 1;
+    const int first = __shfl_sync(0xffffffffu, it.first, from), vecs = __shfl_sync(0xffffffffu, it.vecs, from);
+    vec_ahead = vector_of(a, first, vecs, __shfl_sync(0xffffffffu, it.kv, from), 32 * (warp & 3) + lane);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -656,12 +703,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     const int g = warp >> 2, vec_i = 32 * (warp & 3) + lane;
     const uint32_t quadrant = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     const uint32_t ts = quadrant + kTmemS + 64 * g, to = quadrant + kTmemO + 128 * g;
-    // A vector's index, -1 for one that is not in use.
-    auto vector_of = [&](const Item &it) {
-      const int i = it.first + min(vec_i, it.vecs - 1), row = i / a.group, b = row / a.rows;
-      return vec_i < it.vecs && row - b * a.rows < request_of(a, b).count ? vector_at(a, it.kv, i) : -1;
-    };
-    int vec = -1, vec_ahead = vector_of(t->items[0]);
+    int vec = -1;
     for (int n = 0, j0 = 0, j1 = 0;; n++) {
       const int at = vec;
       if (n < items) {
@@ -717,7 +759,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
         if (lane == 0)
           mbar_arrive(&t->qfull);
         if (n + 1 < items)
-          vec_ahead = vector_of(t->items[n + 1]);
+          vec_ahead = vector_of(a, t->items[n + 1].first, t->items[n + 1].vecs, t->items[n + 1].kv, vec_i);
       }
       if (n) {
         // Item n - 1: the two groups' results joined into the partial result, 16 rows of the quadrant by each, in the
@@ -1077,6 +1119,8 @@ int plan_splits(SharedArgs *a, int most) {
         best = t;
         a->prefix_splits = n;
         a->own_splits = own;
+        a->per_cta = (int)(p / g);
+        a->heavy = (int)heavy;
         a->extra = (int)extra;
         ctas = (int)g;
       }
@@ -1164,6 +1208,12 @@ void k_attention_shared_rows(float *out, int8_t *oq, float *os, const float *q, 
   a.tiles = ceil_div(batch * rows * a.group, tile);
   a.own_tiles = ceil_div(rows * a.group, tile);
   const int ctas = plan_splits(&a, (int)((work->capacity - 4) / ((size_t)a.vectors * (head_dim + 2))));
+  a.by_prefix_splits = divisor(a.prefix_splits ? a.prefix_splits : 1);
+  a.by_own_splits = divisor(a.own_splits);
+  a.by_kv = divisor(a.n_kv);
+  a.by_own_tiles = divisor(a.own_tiles);
+  a.by_group = divisor(a.group);
+  a.by_rows = divisor(a.rows);
   const size_t splits = (size_t)a.prefix_splits + a.own_splits;
   a.ml = reinterpret_cast<float2 *>(work->partial);
   a.acc = work->partial + pairs_floats(splits * a.vectors);

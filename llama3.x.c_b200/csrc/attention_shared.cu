@@ -1094,13 +1094,20 @@ int plan_splits(SharedArgs *a, int most) {
   const double pass = (double)a->vectors * (a->hd + 2) * 8 / 5e12 / 1.5e-6;  // a split's partial results
   const int most_own = most / 2 < kMaxSplits ? most / 2 : kMaxSplits;
   double best = 0.0;
-  int ctas = 1;
+  int ctas = 1, tried_own = 0;
   for (int own_length = own_tiles < kLongest ? own_tiles : kLongest; own_length >= 1; own_length -= own_length > 4 ? 2 : 1) {
     const int own = ceil_div(own_tiles, own_length) < most_own ? ceil_div(own_tiles, own_length) : most_own;
+    if (own == tried_own)
+      continue;
+    tried_own = own;
     const int rest = most - own < kMaxSplits ? most - own : kMaxSplits;
+    int tried = -1;
     for (int length = prefix_tiles < kLongest ? prefix_tiles : kLongest; length >= (prefix_tiles ? 1 : 0); length--) {
       int n = prefix_tiles ? ceil_div(prefix_tiles, length) : 0;
       n = n < rest ? n : rest;
+      if (n == tried)
+        continue;
+      tried = n;
       const double c = n ? item + (double)prefix_tiles / n : 0.0, c_own = own_item + 0.5 * own_tiles / own;
       const long long p = (long long)columns * n, o = (long long)own_columns * own;
       long long g = p + o < kPlanSms ? p + o : kPlanSms;

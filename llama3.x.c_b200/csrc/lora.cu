@@ -796,13 +796,38 @@ cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned cl
   return cudaLaunchKernelEx(&cfg, kernel, a, parts);
 }
 
+// At most this many tiles: the full ones, and one more for each adapter and the rows without one.
+int most_tiles(const LoraArgs &a) {
+  const int some = a.count + 1 < a.rows ? a.count + 1 : a.rows;
+  return (a.rows - some) / kTileRows + some;
+}
+int parts_for(int tiles) {
+  const int few = kc_device_sms() / (kCtas * tiles);
+  return few < 1 ? 1 : few > 4 ? 4 : few;
+}
+
+// The two kernels' times in microseconds, fitted to 70 shapes (1 to 2048 rows, 1 to 64 adapters of rank 4 to 64, 256 to
+// 14336 columns, the three types) to 17 % on average; where the estimates choose wrongly the two are close (3 % lost on
+// average over the same shapes, 70 % at most). A row costs a cluster's start and end, its adapter comes from L2 for every
+// row, and B costs more than A (its rows are short). 33 rows, rank 32 fp32, 4096 to 14336: 20 us here, 38 as tiles.
+template <typename W>
+double row_us(const LoraArgs &a) {
+  const double mb = 1e-6 * a.rows;
+  return 4.5 + 0.034 * a.rows + mb * (0.6 * 4 * a.n + sizeof(W) * (double)a.max_rank * (0.06 * a.n + 0.23 * a.d));
+}
+// A tile reads its adapter once, in steps over the n and d columns; a wave of clusters after another. 2048 rows of rank
+// 64 bf16, 4096 to 4096: 45 us here, 509 as rows.
+template <typename W>
+double tile_us(const LoraArgs &a) {
+  const int tiles = most_tiles(a), parts = parts_for(tiles);
+  const double ctas = (double)kCtas * tiles * parts / kc_device_sms();
+  return 9.5 + (ctas > 1.0 ? ctas : 1.0) *
+                   (2.1 + 1.1e-3 * kParts<W> * a.n + (2.0e-3 + 1.44e-5 * kParts<W> * a.max_rank) * a.d / parts);
+}
+
 template <typename W>
 cudaError_t run(const LoraArgs &a) {
-  // The row kernel reads a row's adapter from L2 for every row, about 3.3 TB/s of it (33 rows, rank 32 fp32, 4096 to
-  // 14336: 78 MB, 24 us); a tile reads it once but takes some 40 us of steps (the same: 38 us). Tiles of fewer than four
-  // rows gain nothing.
-  const double row_bytes = (double)a.rows * a.max_rank * ((double)a.n + a.d) * sizeof(W);
-  if (row_bytes < 128e6 || a.rows < 4 * a.count || a.count >= kMaxBins || a.max_rank > kTileRank)
+  if (a.count >= kMaxBins || a.max_rank > kTileRank || row_us<W>(a) <= tile_us<W>(a))
     return launch<W>(lora_row_kernel<W>, a, (unsigned)a.rows, 1, 0);
   const size_t smem = TileSmem<W>(a.max_rank).total;
   cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(lora_tile_kernel<W>), TileSmem<W>(kTileRank).total);
@@ -812,9 +837,7 @@ cudaError_t run(const LoraArgs &a) {
     b.x += (long long)r * a.ldx, b.out += (long long)r * a.ldo, b.index += r;
     if (b.base)
       b.base += (long long)r * a.ldb;
-    // At most this many tiles: the full ones, and one more for each adapter and the rows without one.
-    const int some = b.count + 1 < b.rows ? b.count + 1 : b.rows, tiles = (b.rows - some) / kTileRows + some;
-    const int few = kc_device_sms() / (kCtas * tiles), parts = few < 1 ? 1 : few > 4 ? 4 : few;
+    const int tiles = most_tiles(b), parts = parts_for(tiles);
     e = launch<W>(lora_tile_kernel<W>, b, (unsigned)(tiles * parts), parts, smem);
     if (e == cudaSuccess && r + kMaxTileRows < a.rows)
       kc_count_launch();

@@ -298,7 +298,7 @@ void k_fill(float *x, size_t n, float value);
  * rows of out are left as they were, and a request that uses none needs no starts[b]. starts and counts are device
  * memory, so a captured step replays as the requests grow. starts[b] outside [0, seq_len - counts[b]] or counts[b]
  * outside [0, rows] raises an error (kc_status) and leaves the request's rows as they were. What a row sees must be
- * finite; what it does not see is never read into it. oq / os (may be NULL): out quantized for Wo as k_quantize does,
+ * finite, or that row has no result; what it does not see, finite or not, changes nothing in it. oq / os (may be NULL): out quantized for Wo as k_quantize does,
  * gs dividing head_dim. The prefix is read once for the whole batch. head_dim <= 256.
  * `work` (k_attention_shared_init, released with k_attention_free): partial results for this n_heads and head_dim and
  * up to batch * rows rows (its `workers`; its max_chunks is 0, so that neither kind of work passes for the other), which

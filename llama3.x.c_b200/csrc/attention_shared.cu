@@ -319,6 +319,8 @@ struct TcTail {
   int abort_flag;
   float kscale[4][kConvWarps];  // 2^-k of eight keys, a ring of tiles
   int vshift[4][kConvWarps];    // k of eight values
+  // A bit for each of eight positions whose keys or values hold a NaN or an infinity.
+  __align__(8) uint8_t wrong[4][kConvWarps];
   int qshift[2][kTcVecs];  // of this item and the next
   float m[2][kTcVecs], l[2][kTcVecs];  // of a group's tiles, and the power of its O
   int vref[2][kTcVecs];
@@ -432,7 +434,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ float abs_max3(float a, float b, float c) {
   float r;
-  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ float abs_max(float m, float4 v) { return abs_max3(abs_max3(m, v.x, v.y), v.z, v.w); }
@@ -495,14 +497,33 @@ struct Rows8 {
 #pragma unroll
     for (int i = 0; i < kSteps; i++)
       t[i & 3] = abs_max(t[i & 3], x[i]);
-    top = fmaxf(max3(t[0], t[1], t[2]), t[3]);
+    top = abs_max3(abs_max3(t[0], t[1], t[2]), t[3], 0.0f);
     // The values are here before the slot's next copy starts.
     asm volatile("" : "+f"(top)::"memory");
   }
   // Splits the rows and stores them as rows row .. row + 7 of the operand pair (64 rows of 128 swizzled bytes to 64
-  // columns); returns their power of two.
-  __device__ __forceinline__ int store(uint8_t *hi_at, uint8_t *lo_at, int row, int lane) const {
-    const int k = shift_for(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+  // columns); returns their power of two. Rows with a NaN or an infinity are stored as zeros and named in `wrong`: the
+  // queries that do not see them are not to notice.
+  __device__ __forceinline__ int store(uint8_t *hi_at, uint8_t *lo_at, int row, int lane, unsigned *wrong) {
+    unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    *wrong = 0;
+    if (bits >= 0x7f800000u) {
+      top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kSteps; i++) {
+        const unsigned lanes = __ballot_sync(0xffffffffu, !(abs_max(0.0f, x[i]) < INFINITY));
+#pragma unroll
+        for (int r = 0; r < kAt; r++)
+          if (lanes >> (32 / kAt * r) & (0xffffffffu >> (32 - 32 / kAt))) {
+            *wrong |= 1u << (i * kAt + r);
+            if (lane * 4 / HD == r)
+              x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+        top = abs_max(top, x[i]);
+      }
+      bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    }
+    const int k = shift_for(bits);
     const uint64_t f = f2_pack(pow2(k), pow2(k));
     const int col = lane * 4 % HD, r = lane * 4 / HD;
     const uint32_t base = (col >> 6) * (kTcPos * 128) + row * 128 + (col & 7) * 2;
@@ -623,7 +644,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       const int s = j & 1, use = j >> 1;
       uint8_t *stage = smem + s * L::stage;
       tc_wait(&t->kempty[s], (use & 1) ^ 1, abort_flag);
-      const int ks = kx.store(stage, stage + L::kv_bytes, 8 * cw, lane);
+      unsigned wrong, wrong_v;
+      const int ks = kx.store(stage, stage + L::kv_bytes, 8 * cw, lane, &wrong);
       if (lane == 0)
         t->kscale[j & 3][cw] = pow2(-ks);
       fence_proxy_async_smem();
@@ -632,9 +654,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
         mbar_arrive(&t->kfull[s]);
       next(kx, kslot, ck);
       tc_wait(&t->vempty[s], (use & 1) ^ 1, abort_flag);
-      const int vs = vx.store(stage + 2 * L::kv_bytes, stage + 3 * L::kv_bytes, 8 * cw, lane);
+      const int vs = vx.store(stage + 2 * L::kv_bytes, stage + 3 * L::kv_bytes, 8 * cw, lane, &wrong_v);
       if (lane == 0)
-        t->vshift[j & 3][cw] = vs;
+        t->vshift[j & 3][cw] = vs, t->wrong[j & 3][cw] = (uint8_t)(wrong | wrong_v);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0)
@@ -926,6 +948,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
             tmem_st16(ts + c + 16, lo);
           }
           tmem_wait_st();
+          // A vector that sees a position which is not finite has no result.
+          const unsigned long long wrong = *reinterpret_cast<const unsigned long long *>(t->wrong[j & 3]);
+          if (wrong && limit > p0 && (limit - p0 >= 64 || wrong << (64 - (limit - p0))))
+            l = NAN;
         }
         tc_fence_before();
         __syncwarp();

@@ -146,6 +146,34 @@ def test_shared_attention_peaked_and_rising_scores(kc):
         close(got, want, hd, top)
 
 
+@pytest.mark.parametrize("hd", [128, 64, 96, 256, 33])
+@pytest.mark.parametrize("wrong", [float("nan"), float("inf"), float("-inf")])
+def test_shared_attention_keeps_to_what_a_row_sees(kc, hd, wrong):
+    """Positions that are not finite, in the keys or in the values: behind the prefix and the last row, where nobody sees
+    them, and at the place of a later row of the same request, which alone has no result then; queries that are not
+    finite spoil their own row only."""
+    heads, kv, B, R, prefix, S = 8, 2, 5, 3, 130, 90
+    starts, counts = [0, 61, 66, 10, 40], [3, 3, 3, 2, 1]
+    g = generator(12)
+    q, pk, pv = normal(g, B, R, heads * hd), normal(g, kv, prefix + 9, hd), normal(g, kv, prefix + 9, hd)
+    k, v = normal(g, B, kv, S, hd), normal(g, B, kv, S, hd)
+    pk[:, prefix:], pv[:, prefix:] = wrong, wrong
+    for b in range(B):
+        k[b, :, starts[b] + counts[b]:], v[b, :, starts[b] + counts[b]:] = wrong, wrong
+    k[0, :, 1, hd // 2] = wrong
+    v[1, :, starts[1] + 2, 1] = wrong
+    k[2, :, starts[2] + 2], v[2, :, starts[2] + 1] = wrong, wrong
+    q[3, 1] = float("nan")
+    fine = torch.zeros(B, R, dtype=torch.bool, device="cuda")
+    for b, r in ((0, 0), (1, 0), (1, 1), (2, 0), (3, 0), (4, 0)):
+        fine[b, r] = True
+    got = run_attention(kc, q, pk, pv, prefix, k, v, starts, counts, heads, kv, hd)
+    want, top = attention_64(q, pk, pv, prefix, k, v, starts, [1, 2, 1, 1, 1], heads, kv, hd, got)
+    close(got[fine], want[fine], hd, top)
+    assert not got[1, 2].isfinite().all() and not got[2, 1].isfinite().all() and not got[3, 1].isfinite().any()
+    assert (got[3, 2] == -7.0).all() and (got[4, 1:] == -7.0).all()
+
+
 @pytest.mark.parametrize("hd,gs", [(128, 64), (64, 64), (64, 16), (128, 128), (96, 32)])
 def test_shared_attention_quantizes_its_output(kc, hd, gs):
     heads, kv, B, R, prefix, S = 8, 2, 3, 2, 100, 40

@@ -204,11 +204,21 @@ def _check_host():
         raise KernelError(msg.decode())
 
 
-def _stream():
+_device = _raw_stream = None  # torch's current CUDA device, and a device's current stream, once torch has them
+
+
+def _bind_torch():
+    global _device, _raw_stream
     import torch
-    if not torch.cuda.is_initialized():
+    if torch.cuda.is_available():
         torch.cuda.init()
-    _lib.kernels_set_stream(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+        _device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _stream():
+    if _device is None:
+        _bind_torch()
+    _lib.kernels_set_stream(_raw_stream(_device()))
 
 
 def _call(name, *args):
@@ -491,13 +501,16 @@ def k_random_q8(q, s, rows, cols, row0, col0, full_cols, seed, tensor, std, gs):
 
 # ---- a batch of requests over one prompt ------------------------------------------------------------------------------
 
-def _want(dtype, *tensors):
-    """The tensors (None allowed) must be contiguous ones of `dtype` on the current device: their addresses are all
-    that the library sees."""
+def _want(dtype, *tensors, strided=False):
+    """The tensors (None allowed) must be contiguous ones (`strided`: rows with strides that the call names) of `dtype`
+    on the current device: their addresses are all that the library sees."""
+    if _device is None:
+        _bind_torch()
+    device = _device() if _device else None  # None: there are no CUDA tensors
     for t in tensors:
-        if t is not None and not (t.dtype is dtype and t.is_cuda and t.is_contiguous()):
-            raise KernelError(f"needs a contiguous {dtype} CUDA tensor, got {t.dtype} on {t.device} with strides "
-                              f"{tuple(t.stride())}")
+        if t is not None and (t.dtype is not dtype or t.get_device() != device or not (strided or t.is_contiguous())):
+            raise KernelError(f"needs a contiguous {dtype} CUDA tensor on the current device, got {t.dtype} on "
+                              f"{t.device} with strides {tuple(t.stride())}")
 
 
 def shared_attention_work(n_heads, n_kv_heads, head_dim, batch, rows):
@@ -541,6 +554,11 @@ def lora_table(a, b, scale):
 
 def k_lora_rows(out, ldo, base, ldb, x, ldx, index, table, count, type, max_rank, n, d, rows):
     """out = base + scale B (A x) with the adapter each row names (include/kernels_cuda.h); table from lora_table."""
+    import torch
+    _want(torch.float32, out, base, x, strided=True)
+    _want(torch.int32, index)
+    if table is not None and count * ctypes.sizeof(LoraAdapter) > table.numel():
+        raise KernelError(f"{count} adapters of a table of {table.numel() // ctypes.sizeof(LoraAdapter)}")
     _call("k_lora_rows", _ptr(out), ldo, _ptr(base), ldb, _ptr(x), ldx, _ptr(index), _ptr(table), count, type, max_rank,
           n, d, rows)
 
@@ -555,5 +573,8 @@ def k_verify_draft(accepted, tokens, target, ldt, draft, ldd, drafted, counts, u
     import torch
     _want(torch.int32, accepted, tokens, drafted, counts)
     _want(torch.float32, uniforms, temperature)
+    _want(torch.float32, target, draft, strided=True)
+    if work is not None and work.numel() * work.element_size() < load().k_verify_bytes(vocab, batch, rows):
+        raise KernelError("k_verify_draft: the work is too small for this shape")
     _call("k_verify_draft", _ptr(accepted), _ptr(tokens), _ptr(target), ldt, _ptr(draft), ldd, _ptr(drafted),
           _ptr(counts), _ptr(uniforms), _ptr(temperature), vocab, batch, rows, _ptr(work))

@@ -125,3 +125,15 @@ def test_python_mirror_refuses_other_layouts():
         kc.k_attention_shared_rows(a, None, None, a, a, a, 4, 4, a, a, a, a, kc.AttentionWork(), 1, 1, 4, 4, 1, 4, 0)
     with pytest.raises(kc.KernelError, match="as many a and b matrices"):
         kc.lora_table([a], [], [1.0])
+
+
+def test_python_mirror_refuses_other_types_and_small_tables():
+    """Rows with strides of their own need the right type and device all the same; a table and a work have a size."""
+    import torch
+    kc = load_package()
+    a, i = torch.zeros(4, 4), torch.zeros(4, dtype=torch.int32)
+    for x in (a, a.half()):
+        with pytest.raises(kc.KernelError, match="contiguous torch.float32 CUDA tensor on the current device"):
+            kc.k_lora_rows(x, 4, None, 0, x, 4, i, None, 0, kc.K_F32, 4, 4, 4, 4)
+    with pytest.raises(kc.KernelError, match="CUDA tensor on the current device"):
+        kc.k_verify_draft(i, i, a, 4, None, 0, i, None, a, a, 4, 1, 1, a)

@@ -721,6 +721,27 @@ def test_two_works_on_two_streams(kc):
         kc.k_attention_free(w)
 
 
+def test_mirror_refuses_what_does_not_fit(kc):
+    """Tables and works that are too small for the call, types that are not the operator's: errors before any launch."""
+    g = generator(3)
+    x, out, index = normal(g, 4, 64), torch.zeros(4, 32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    table = kc.lora_table([normal(g, 8, 64)], [normal(g, 32, 8)], [1.0])
+    with pytest.raises(kc.KernelError, match="2 adapters of a table of 1"):
+        kc.k_lora_rows(out, 32, None, 0, x, 64, index, table, 2, kc.K_F32, 8, 64, 32, 4)
+    for bad in (x.half(), x.cpu()):
+        with pytest.raises(kc.KernelError, match="torch.float32 CUDA tensor on the current device"):
+            kc.k_lora_rows(out, 32, None, 0, bad, 64, index, table, 1, kc.K_F32, 8, 64, 32, 4)
+    with pytest.raises(kc.KernelError, match="torch.int32"):
+        kc.k_lora_rows(out, 32, None, 0, x, 64, index.long(), table, 1, kc.K_F32, 8, 64, 32, 4)
+    accepted, tokens = index[:1], torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    u, t, logits = torch.zeros(1, 2, device="cuda"), torch.ones(1, device="cuda"), normal(g, 2, 100)
+    work = torch.zeros(kc.k_verify_bytes(100, 1, 1), dtype=torch.uint8, device="cuda")
+    with pytest.raises(kc.KernelError, match="the work is too small"):
+        kc.k_verify_draft(accepted, tokens, logits, 100, None, 0, tokens, None, u, t, 100, 1, 1, work[:-16])
+    with pytest.raises(kc.KernelError, match="torch.float32 CUDA tensor"):
+        kc.k_verify_draft(accepted, tokens, logits.half(), 100, None, 0, tokens, None, u, t, 100, 1, 1, work)
+
+
 def test_nothing_to_do(kc):
     """A batch of none, rows of none: accepted, nothing queued."""
     before = kc.load().kc_launch_count()

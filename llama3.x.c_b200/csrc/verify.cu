@@ -25,7 +25,7 @@ constexpr int kBlock = 16 * kSumThreads;  // logits that a CTA of the sums kerne
 constexpr int kLoops = 4;                 // and how often, where there is work enough for every SM all the same
 constexpr int kPickThreads = 512;
 constexpr int kPickWarps = kPickThreads / 32;
-constexpr int kMaxCtas = 16;  // a cluster per request, of 4 to 16 CTAs
+constexpr int kMaxCtas = 16;  // a cluster per request, of 4 to 16 CTAs, or of one
 constexpr int kMaxRows = 64;
 constexpr int kMaxSlots = 2 * kMaxRows + 1;
 constexpr float kMaxTemperature = 1e30f;  // 700 T is a number
@@ -324,21 +324,29 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
   __shared__ uint2 table[32];
   __shared__ double sum_s[kMaxSlots], warp_sums[kPickWarps], slices[kMaxCtas];
   __shared__ Invert inv;
-  __shared__ int stop_s, found_s;
+  __shared__ int stop_s, found_s, drafted_s[kMaxRows];
   cg::cluster_group cluster = cg::this_cluster();
   load_table(table);
   pdl_wait();
   pdl_launch_dependents();
   const int ctas = cluster.num_blocks(), b = blockIdx.x / ctas, rank = blockIdx.x % ctas;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // What does not depend on one another is on its way at once: the drafts, the first chunks of this warp's first slot
+  // (whether they count shows later), the request's numbers.
+  const int j = threadIdx.x;
+  const int drafted = j < a.rows ? a.drafted[(long long)b * a.rows + j] : -1;
+  const long long base = (long long)b * a.slots * a.chunks;
+  const long long first_at = base + (long long)warp * a.chunks + lane;
+  const bool have_first = warp < a.slots && lane < a.chunks;
+  const unsigned long long first_key = have_first ? a.keys[first_at] : 0;
+  const double first_sum = have_first ? a.sums[first_at] : 0.0;
   const int count = count_of(a, b);
   const float t = a.temperature[b];
   const bool greedy = t == 0.0f;
   const bool valid = count >= 0 && count <= a.rows && t >= 0.0f && t <= kMaxTemperature;
   // This thread's draft, and its logits.
-  const int j = threadIdx.x;
   const bool drafts = valid && j < count;
-  const int x = drafts ? a.drafted[(long long)b * a.rows + j] : -1;
+  const int x = drafts ? drafted : -1;
   const bool x_good = x >= 0 && x < a.vocab;
   float px = 0.0f, qx = 0.0f, u = 0.0f;
   if (drafts && x_good && !greedy) {
@@ -349,28 +357,32 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
   const float u_last = a.uniforms[(long long)b * (a.rows + 1) + a.rows];
   if (threadIdx.x == 0)
     stop_s = valid ? count : 0;
+  if (j < a.rows)
+    drafted_s[j] = drafted;
   cluster.sync();  // every CTA has started before any writes into another's shared memory; the table is there
   if (count < 0)
     return;  // the whole cluster: a slot of the batch that is not in use
   const Weights weight{table, greedy ? 0.0 : k32_of(t)};
   int *tokens = a.tokens + (long long)b * (a.rows + 1);
-  const long long base = (long long)b * a.slots * a.chunks;
   if (valid)
     for (int slot = warp; slot < a.slots; slot += kPickWarps) {
       const float *row;
       if (!slot_row(a, b, slot, &row))
         continue;
       const long long at = base + (long long)slot * a.chunks;
-      unsigned long long key = 0;
-      for (int c = lane; c < a.chunks; c += 32)
+      const bool ahead = slot == warp;
+      unsigned long long key = ahead ? first_key : lane < a.chunks ? a.keys[at + lane] : 0;
+      const unsigned long long key0 = key;
+      for (int c = lane + 32; c < a.chunks; c += 32)
         key = max64(key, a.keys[at + c]);
       key = warp_max(key);
       double sum = 0.0;
       if (!greedy && key_good(key))
         for (int c = lane; c < a.chunks; c += 32) {
-          const unsigned long long k = a.keys[at + c];
+          const unsigned long long k = c == lane ? key0 : a.keys[at + c];
           if (key_good(k))
-            sum += a.sums[at + c] * weight(key_value(k), key_value(key), floor_of(key_value(key), t));
+            sum += (ahead && c == lane ? first_sum : a.sums[at + c]) *
+                   weight(key_value(k), key_value(key), floor_of(key_value(key), t));
         }
       sum = warp_sum(sum);
       if (lane == 0)
@@ -397,7 +409,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
   __syncthreads();
   const int stop = stop_s;
   const bool refused = stop < count;
-  const int at_stop = valid && refused ? a.drafted[(long long)b * a.rows + stop] : -1;
+  const int at_stop = valid && refused ? drafted_s[stop] : -1;
   // No distribution at the place where the run ends (or arguments that mean nothing): no answer.
   unsigned error = 0;
   if (!valid || (refused && (at_stop < 0 || at_stop >= a.vocab)))
@@ -645,9 +657,10 @@ void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt,
       kc_launch_pdl(verify_sums_kernel, dim3((unsigned)pairs), dim3(kSumThreads), 0, kc_stream(), a);
   if (e == cudaSuccess) {
     kc_count_launch();
-    // The largest clusters that run in about two waves of two CTAs per SM (greedy requests and accepted drafts leave
-    // early): a request's rows are read by more SMs at once.
-    int ctas = kMaxCtas;
+    // With draft logits the largest clusters that run in about two waves of two CTAs per SM (greedy requests and accepted
+    // drafts leave early): a request's rows are read by more SMs at once. Without, one CTA inverts one chunk (24 requests
+    // of 7 drafts: 13 us with one CTA a request, 16 with sixteen).
+    int ctas = a.draft ? kMaxCtas : 1;
     while (ctas > 4 && (long long)ctas * batch > 4 * kc_device_sms())
       ctas /= 2;
     e = allow_large_clusters();

@@ -86,6 +86,22 @@ cudaError_t kc_allow_smem(const void *kernel, int bytes) {
   return e;
 }
 
+cudaError_t kc_allow_clusters(const void *kernel) {
+  static std::mutex mu;
+  static std::set<std::pair<const void *, int>> done;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess)
+    return e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({kernel, dev}))
+    return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess)
+    done.insert({kernel, dev});
+  return e;
+}
+
 cudaStream_t kc_stream() { return tl_stream; }
 
 extern "C" {

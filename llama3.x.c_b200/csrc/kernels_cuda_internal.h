@@ -44,6 +44,8 @@ bool kc_pdl_enabled();
 // Raises `kernel`'s dynamic shared-memory limit to `bytes` on the current device, once per (kernel, device); safe to
 // call from several host threads at once.
 cudaError_t kc_allow_smem(const void *kernel, int bytes);
+// Clusters of more than the portable 8 CTAs, up to 16: allowed once per kernel and device.
+cudaError_t kc_allow_clusters(const void *kernel);
 
 // Launches `kernel` on `stream` with programmatic dependent launch allowed (kernels_set_pdl): it may be scheduled
 // while the previous kernel in the stream drains, so every kernel launched this way starts with griddepcontrol.wait

@@ -27,6 +27,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRank = 256;
 constexpr int kCtas = 8;  // of a cluster
+constexpr int kManyCtas = 16, kRowCtas = 4;  // of a row's cluster where so many CTAs an SM hold all rows at once
 
 struct LoraArgs {
   float *out;
@@ -62,11 +63,65 @@ __device__ __forceinline__ void load8(const __half *p, float (&v)[8]) { halves<_
 
 __device__ __forceinline__ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-template <typename W>
+// N neighbouring weights of 16 bytes.
+__device__ __forceinline__ void load16(const float *p, float (&v)[4]) {
+  const float4 a = *reinterpret_cast<const float4 *>(p);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+}
+__device__ __forceinline__ void load16(const __nv_bfloat16 *p, float (&v)[8]) { load8(p, v); }
+__device__ __forceinline__ void load16(const __half *p, float (&v)[8]) { load8(p, v); }
+
+// out = base + B h for the outputs [d0, d1) of a row, rows of B in 16-byte units: P lanes take a row together, so that a
+// warp's reads are whole lines, and keep their part of h in registers. After P steps every lane has one of the warp's 32
+// outputs.
+template <typename W, int P>
+__device__ __forceinline__ void expand_rows(const W *B, const float *h, int rank, int d0, int d1, const float *base,
+                                            float *out) {
+  constexpr int E = 16 / sizeof(W), G = 32 / P;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, p = lane % P, g = lane / P, units = rank / E;
+  float hv[E];
+#pragma unroll
+  for (int e = 0; e < E; e++)
+    hv[e] = p < units ? h[p * E + e] : 0.0f;
+  for (int i0 = d0 + 32 * warp; i0 < d1; i0 += 32 * kWarps) {
+    const int own = i0 + p * G + g;
+    const float before = base && own < d1 ? base[own] : 0.0f;
+    float mine = 0.0f;
+#pragma unroll 8
+    for (int step = 0; step < P; step++) {
+      const int i = i0 + step * G + g;
+      float s = 0.0f;
+      if (i < d1 && p < units) {
+        const W *row = B + (size_t)i * rank;
+        float wv[E];
+        load16(row + p * E, wv);
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          s = fmaf(wv[e], hv[e], s);
+        if constexpr (P == 32)
+          for (int u = p + 32; u < units; u += 32) {
+            load16(row + u * E, wv);
+#pragma unroll
+            for (int e = 0; e < E; e++)
+              s = fmaf(wv[e], h[u * E + e], s);
+          }
+      }
+#pragma unroll
+      for (int o = P / 2; o; o >>= 1)
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+      mine = p == step ? s : mine;
+    }
+    if (own < d1)
+      out[own] = before + mine;
+  }
+}
+
+// A cluster of C CTAs per row.
+template <typename W, int C>
 __global__ void __launch_bounds__(kThreads, 4) lora_row_kernel(const LoraArgs a, int) {
   __shared__ float part[kMaxRank], h[kMaxRank];
   cg::cluster_group cluster = cg::this_cluster();
-  constexpr int ctas = kCtas;
+  constexpr int ctas = C;
   const int rank = cluster.block_rank(), row = blockIdx.x / ctas;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
@@ -140,25 +195,31 @@ __global__ void __launch_bounds__(kThreads, 4) lora_row_kernel(const LoraArgs a,
   cluster.sync();  // the slices are read: a CTA may leave, and h is whole
   const int d_slice = (a.d + ctas - 1) / ctas;
   const int d0 = min(rank * d_slice, a.d), d1 = min(d0 + d_slice, a.d);
-  const bool wide_b = aligned16(B) && w.rank % 8 == 0;
+  const float *base = a.base ? a.base + (long long)row * a.ldb : nullptr;
+  float *out = a.out + (long long)row * a.ldo;
+  constexpr int E = 16 / sizeof(W);
+  if (w.rank && aligned16(B) && w.rank % E == 0) {
+    const int units = w.rank / E;
+    if (units <= 1)
+      expand_rows<W, 1>(B, h, w.rank, d0, d1, base, out);
+    else if (units <= 2)
+      expand_rows<W, 2>(B, h, w.rank, d0, d1, base, out);
+    else if (units <= 4)
+      expand_rows<W, 4>(B, h, w.rank, d0, d1, base, out);
+    else if (units <= 8)
+      expand_rows<W, 8>(B, h, w.rank, d0, d1, base, out);
+    else if (units <= 16)
+      expand_rows<W, 16>(B, h, w.rank, d0, d1, base, out);
+    else
+      expand_rows<W, 32>(B, h, w.rank, d0, d1, base, out);
+    return;
+  }
   for (int i = d0 + threadIdx.x; i < d1; i += kThreads) {
     const W *bi = B + (long long)i * w.rank;
     float s = 0.0f;
-    if (wide_b) {
-#pragma unroll 2
-      for (int k = 0; k < w.rank; k += 8) {
-        float wv[8];
-        load8(bi + k, wv);
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          s = fmaf(wv[j], h[k + j], s);
-      }
-    } else {
-      for (int k = 0; k < w.rank; k++)
-        s = fmaf(to_float(bi[k]), h[k], s);
-    }
-    const float before = a.base ? a.base[(long long)row * a.ldb + i] : 0.0f;
-    a.out[(long long)row * a.ldo + i] = before + s;
+    for (int k = 0; k < w.rank; k++)
+      s = fmaf(to_float(bi[k]), h[k], s);
+    out[i] = (base ? base[i] : 0.0f) + s;
   }
 }
 
@@ -780,9 +841,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
 }
 
 template <typename W>
-cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned clusters, int parts, size_t smem) {
+cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned clusters, int parts, size_t smem,
+                   int ctas = kCtas) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(clusters * kCtas);
+  cfg.gridDim = dim3(clusters * ctas);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = kc_stream();
@@ -790,7 +852,7 @@ cudaError_t launch(void (*kernel)(LoraArgs, int), const LoraArgs &a, unsigned cl
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = kc_pdl_enabled() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kCtas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  attr[1].val.clusterDim.x = ctas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, a, parts);
@@ -826,9 +888,18 @@ double tile_us(const LoraArgs &a) {
 }
 
 template <typename W>
+cudaError_t launch_rows(const LoraArgs &a) {
+  if ((long long)a.rows * kManyCtas <= kRowCtas * kc_device_sms()) {
+    const cudaError_t e = kc_allow_clusters(reinterpret_cast<const void *>(lora_row_kernel<W, kManyCtas>));
+    return e != cudaSuccess ? e : launch<W>(lora_row_kernel<W, kManyCtas>, a, (unsigned)a.rows, 1, 0, kManyCtas);
+  }
+  return launch<W>(lora_row_kernel<W, kCtas>, a, (unsigned)a.rows, 1, 0);
+}
+
+template <typename W>
 cudaError_t run(const LoraArgs &a) {
   if (a.count >= kMaxBins || a.max_rank > kTileRank || row_us<W>(a) <= tile_us<W>(a))
-    return launch<W>(lora_row_kernel<W>, a, (unsigned)a.rows, 1, 0);
+    return launch_rows<W>(a);
   const size_t smem = TileSmem<W>(a.max_rank).total;
   cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(lora_tile_kernel<W>), TileSmem<W>(kTileRank).total);
   for (int r = 0; r < a.rows && e == cudaSuccess; r += kMaxTileRows) {

@@ -10,8 +10,6 @@
 #include <float.h>
 #include <stdint.h>
 
-#include <mutex>
-
 #include "../../include/kernels_cuda.h"
 #include "common.cuh"
 #include "kernels_cuda_internal.h"
@@ -589,22 +587,6 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
 
 size_t verify_blocks(int vocab) { return ((size_t)vocab + kBlock - 1) / kBlock; }
 
-// Clusters of 16 CTAs are above the portable 8: allowed once per device.
-cudaError_t allow_large_clusters() {
-  static std::mutex mu;
-  static bool done[64];
-  int dev = 0;
-  const cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess || dev < 0 || dev >= 64)
-    return e != cudaSuccess ? e : cudaErrorInvalidDevice;
-  std::lock_guard<std::mutex> hold(mu);
-  if (done[dev])
-    return cudaSuccess;
-  const cudaError_t r = cudaFuncSetAttribute(verify_pick_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  done[dev] = r == cudaSuccess;
-  return r;
-}
-
 }  // namespace
 
 extern "C" {
@@ -663,7 +645,7 @@ void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt,
     int ctas = a.draft ? kMaxCtas : 1;
     while (ctas > 4 && (long long)ctas * batch > 4 * kc_device_sms())
       ctas /= 2;
-    e = allow_large_clusters();
+    e = kc_allow_clusters(reinterpret_cast<const void *>(verify_pick_kernel));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)batch * ctas);
     cfg.blockDim = dim3(kPickThreads);

@@ -26,8 +26,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRank = 256;
-constexpr int kCtas = 8;  // of a cluster
-constexpr int kManyCtas = 16, kRowCtas = 4;  // of a row's cluster where so many CTAs an SM hold all rows at once
+constexpr int kCtas = 8;  // of a tile's cluster
+constexpr int kRowCtas = 4;  // an SM's CTAs of the row kernel
 
 struct LoraArgs {
   float *out;
@@ -61,58 +61,74 @@ __device__ __forceinline__ void halves(const void *p, float (&v)[8]) {
 __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) { halves<__nv_bfloat162>(p, v); }
 __device__ __forceinline__ void load8(const __half *p, float (&v)[8]) { halves<__half2>(p, v); }
 
-__device__ __forceinline__ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+__host__ __device__ __forceinline__ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-// N neighbouring weights of 16 bytes.
-__device__ __forceinline__ void load16(const float *p, float (&v)[4]) {
+// The weights of a unit: 16 bytes, or 8.
+__device__ __forceinline__ void load_unit(const float *p, float (&v)[4]) {
   const float4 a = *reinterpret_cast<const float4 *>(p);
   v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
 }
-__device__ __forceinline__ void load16(const __nv_bfloat16 *p, float (&v)[8]) { load8(p, v); }
-__device__ __forceinline__ void load16(const __half *p, float (&v)[8]) { load8(p, v); }
+__device__ __forceinline__ void load_unit(const __nv_bfloat16 *p, float (&v)[8]) { load8(p, v); }
+__device__ __forceinline__ void load_unit(const __half *p, float (&v)[8]) { load8(p, v); }
+template <typename W>
+__device__ __forceinline__ void load_unit(const W *p, float (&v)[4]) {
+  const uint2 a = *reinterpret_cast<const uint2 *>(p);
+  const W *w = reinterpret_cast<const W *>(&a);
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    v[i] = to_float(w[i]);
+}
 
-// out = base + B h for the outputs [d0, d1) of a row, rows of B in 16-byte units: P lanes take a row together, so that a
-// warp's reads are whole lines, and keep their part of h in registers. After P steps every lane has one of the warp's 32
-// outputs.
-template <typename W, int P>
+// out = base + B h for the outputs [d0, d1) of a row, rows of B in units of E weights: P lanes take a row together, so
+// that a warp's reads are whole lines, and keep their part of h in registers. After P steps every lane has one of 32
+// outputs; K such groups are under way at once.
+template <typename W, int E, int P, int K = 1>
 __device__ __forceinline__ void expand_rows(const W *B, const float *h, int rank, int d0, int d1, const float *base,
                                             float *out) {
-  constexpr int E = 16 / sizeof(W), G = 32 / P;
+  constexpr int G = 32 / P;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, p = lane % P, g = lane / P, units = rank / E;
   float hv[E];
 #pragma unroll
   for (int e = 0; e < E; e++)
     hv[e] = p < units ? h[p * E + e] : 0.0f;
-  for (int i0 = d0 + 32 * warp; i0 < d1; i0 += 32 * kWarps) {
+  for (int i0 = d0 + 32 * K * warp; i0 < d1; i0 += 32 * K * kWarps) {
     const int own = i0 + p * G + g;
-    const float before = base && own < d1 ? base[own] : 0.0f;
-    float mine = 0.0f;
+    float before[K], mine[K];
+#pragma unroll
+    for (int k = 0; k < K; k++)
+      before[k] = base && own + 32 * k < d1 ? base[own + 32 * k] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      mine[k] = 0.0f;
 #pragma unroll 8
-    for (int step = 0; step < P; step++) {
-      const int i = i0 + step * G + g;
-      float s = 0.0f;
-      if (i < d1 && p < units) {
-        const W *row = B + (size_t)i * rank;
-        float wv[E];
-        load16(row + p * E, wv);
+      for (int step = 0; step < P; step++) {
+        const int i = i0 + 32 * k + step * G + g;
+        float s = 0.0f;
+        if (i < d1 && p < units) {
+          const W *row = B + (size_t)i * rank;
+          float wv[E];
+          load_unit(row + p * E, wv);
 #pragma unroll
-        for (int e = 0; e < E; e++)
-          s = fmaf(wv[e], hv[e], s);
-        if constexpr (P == 32)
-          for (int u = p + 32; u < units; u += 32) {
-            load16(row + u * E, wv);
+          for (int e = 0; e < E; e++)
+            s = fmaf(wv[e], hv[e], s);
+          if constexpr (P == 32)
+            for (int u = p + 32; u < units; u += 32) {
+              load_unit(row + u * E, wv);
 #pragma unroll
-            for (int e = 0; e < E; e++)
-              s = fmaf(wv[e], h[u * E + e], s);
-          }
+              for (int e = 0; e < E; e++)
+                s = fmaf(wv[e], h[u * E + e], s);
+            }
+        }
+#pragma unroll
+        for (int o = P / 2; o; o >>= 1)
+          s += __shfl_xor_sync(0xffffffffu, s, o);
+        mine[k] = p == step ? s : mine[k];
       }
-#pragma unroll
-      for (int o = P / 2; o; o >>= 1)
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-      mine = p == step ? s : mine;
     }
-    if (own < d1)
-      out[own] = before + mine;
+#pragma unroll
+    for (int k = 0; k < K; k++)
+      if (own + 32 * k < d1)
+        out[own + 32 * k] = before[k] + mine[k];
   }
 }
 
@@ -200,26 +216,46 @@ __global__ void __launch_bounds__(kThreads, 4) lora_row_kernel(const LoraArgs a,
   constexpr int E = 16 / sizeof(W);
   if (w.rank && aligned16(B) && w.rank % E == 0) {
     const int units = w.rank / E;
-    if (units <= 1)
-      expand_rows<W, 1>(B, h, w.rank, d0, d1, base, out);
+    const bool many = d1 - d0 >= 4 * kThreads;
+    if (units <= 1 && many)
+      expand_rows<W, E, 1, 4>(B, h, w.rank, d0, d1, base, out);
+    else if (units <= 1)
+      expand_rows<W, E, 1>(B, h, w.rank, d0, d1, base, out);
+    else if (units <= 2 && many)
+      expand_rows<W, E, 2, 2>(B, h, w.rank, d0, d1, base, out);
     else if (units <= 2)
-      expand_rows<W, 2>(B, h, w.rank, d0, d1, base, out);
+      expand_rows<W, E, 2>(B, h, w.rank, d0, d1, base, out);
     else if (units <= 4)
-      expand_rows<W, 4>(B, h, w.rank, d0, d1, base, out);
+      expand_rows<W, E, 4>(B, h, w.rank, d0, d1, base, out);
     else if (units <= 8)
-      expand_rows<W, 8>(B, h, w.rank, d0, d1, base, out);
+      expand_rows<W, E, 8>(B, h, w.rank, d0, d1, base, out);
     else if (units <= 16)
-      expand_rows<W, 16>(B, h, w.rank, d0, d1, base, out);
+      expand_rows<W, E, 16>(B, h, w.rank, d0, d1, base, out);
     else
-      expand_rows<W, 32>(B, h, w.rank, d0, d1, base, out);
+      expand_rows<W, E, 32>(B, h, w.rank, d0, d1, base, out);
     return;
   }
-  for (int i = d0 + threadIdx.x; i < d1; i += kThreads) {
-    const W *bi = B + (long long)i * w.rank;
-    float s = 0.0f;
+  if (sizeof(W) == 2 && w.rank == 4 && ((uintptr_t)B & 7) == 0) {
+    expand_rows<W, 4, 1, 4>(B, h, w.rank, d0, d1, base, out);
+    return;
+  }
+  constexpr int K = 4;  // outputs under way
+  for (int i0 = d0 + threadIdx.x; i0 < d1; i0 += K * kThreads) {
+    float s[K], before[K];
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+      s[j] = 0.0f;
+      before[j] = base && i0 + j * kThreads < d1 ? base[i0 + j * kThreads] : 0.0f;
+    }
+#pragma unroll 4
     for (int k = 0; k < w.rank; k++)
-      s = fmaf(to_float(bi[k]), h[k], s);
-    out[i] = (base ? base[i] : 0.0f) + s;
+#pragma unroll
+      for (int j = 0; j < K; j++)
+        s[j] = fmaf(to_float(B[(size_t)min(i0 + j * kThreads, d1 - 1) * w.rank + k]), h[k], s[j]);
+#pragma unroll
+    for (int j = 0; j < K; j++)
+      if (i0 + j * kThreads < d1)
+        out[i0 + j * kThreads] = before[j] + s[j];
   }
 }
 
@@ -869,31 +905,41 @@ int parts_for(int tiles) {
 }
 
 // The two kernels' times in microseconds, fitted to 70 shapes (1 to 2048 rows, 1 to 64 adapters of rank 4 to 64, 256 to
-// 14336 columns, the three types) to 17 % on average; where the estimates choose wrongly the two are close (3 % lost on
-// average over the same shapes, 70 % at most). A row costs a cluster's start and end, its adapter comes from L2 for every
-// row, and B costs more than A (its rows are short). 33 rows, rank 32 fp32, 4096 to 14336: 20 us here, 38 as tiles.
+// 14336 columns, the three types) to 17 % on average; where the estimates choose wrongly the two are close (1 % lost on
+// average over the same shapes, 27 % at most). A row's adapter comes from L2 for every row. 33 rows, rank 32 fp32, 4096
+// to 14336: 12 us here, 38 as tiles.
 template <typename W>
 double row_us(const LoraArgs &a) {
   const double mb = 1e-6 * a.rows;
-  return 4.5 + 0.034 * a.rows + mb * (0.6 * 4 * a.n + sizeof(W) * (double)a.max_rank * (0.06 * a.n + 0.23 * a.d));
+  return 5.7 + mb * (0.79 * 4 * a.n + 0.27 * 8 * a.d + sizeof(W) * (double)a.max_rank * (0.058 * a.n + 0.108 * a.d));
 }
 // A tile reads its adapter once, in steps over the n and d columns; a wave of clusters after another. 2048 rows of rank
-// 64 bf16, 4096 to 4096: 45 us here, 509 as rows.
+// 64 bf16, 4096 to 4096: 45 us here, 319 as rows.
 template <typename W>
 double tile_us(const LoraArgs &a) {
   const int tiles = most_tiles(a), parts = parts_for(tiles);
   const double ctas = (double)kCtas * tiles * parts / kc_device_sms();
-  return 9.5 + (ctas > 1.0 ? ctas : 1.0) *
-                   (2.1 + 1.1e-3 * kParts<W> * a.n + (2.0e-3 + 1.44e-5 * kParts<W> * a.max_rank) * a.d / parts);
+  const bool wide = aligned16(a.out) && a.ldo % 4 == 0 && aligned16(a.base) && a.ldb % 4 == 0;  // else one value at a time
+  return 9.5 + (ctas > 1.0 ? ctas : 1.0) * (2.1 + 1.1e-3 * kParts<W> * a.n +
+                                            ((wide ? 2.0e-3 : 4.6e-3) + 1.44e-5 * kParts<W> * a.max_rank) * a.d / parts);
 }
 
-template <typename W>
+// The largest cluster, 16 CTAs to one, with which all rows are resident at once, at kRowCtas CTAs an SM (291 rows of
+// rank 4: 7 us with two CTAs a row, 11 with four); with two waves where a row's adapter is large (236 rows of rank 64
+// fp16, 22 thousand columns: 76 us with four, 113 with two).
+template <typename W, int C = 16>
 cudaError_t launch_rows(const LoraArgs &a) {
-  if ((long long)a.rows * kManyCtas <= kRowCtas * kc_device_sms()) {
-    const cudaError_t e = kc_allow_clusters(reinterpret_cast<const void *>(lora_row_kernel<W, kManyCtas>));
-    return e != cudaSuccess ? e : launch<W>(lora_row_kernel<W, kManyCtas>, a, (unsigned)a.rows, 1, 0, kManyCtas);
+  if constexpr (C > 1) {
+    const bool large = C < 16 && sizeof(W) * (double)a.max_rank * ((double)a.n + a.d) > 1e6;
+    if ((long long)a.rows * C > (large ? 2 : 1) * kRowCtas * kc_device_sms())
+      return launch_rows<W, C / 2>(a);
   }
-  return launch<W>(lora_row_kernel<W, kCtas>, a, (unsigned)a.rows, 1, 0);
+  if (C > 8) {
+    const cudaError_t e = kc_allow_clusters(reinterpret_cast<const void *>(lora_row_kernel<W, C>));
+    if (e != cudaSuccess)
+      return e;
+  }
+  return launch<W>(lora_row_kernel<W, C>, a, (unsigned)a.rows, 1, 0, C);
 }
 
 template <typename W>

@@ -272,6 +272,16 @@ LORA += [
 ]
 
 
+# One CTA a row, many outputs each, at ranks of one, two and half a unit of reads; a rank of more units than lanes.
+LORA += [
+    (700, 3, [8, 4, 16], 64, 3001, torch.bfloat16),
+    (700, 3, [8, 2, 4], 64, 3001, torch.float32),
+    (620, 3, [4, 3, 1], 40, 2600, torch.float16),
+    (40, 2, [256, 132], 260, 300, torch.float32),
+    (170, 3, [24, 12, 20], 2048, 96, torch.bfloat16),
+]
+
+
 def lora_inputs(case, order, seed=0):
     rows, count, ranks, n, d, dtype = case
     g = generator(rows + seed)

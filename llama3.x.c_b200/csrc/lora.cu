@@ -36,6 +36,7 @@ struct LoraArgs {
   const int *index;
   const LoraAdapter *adapters;
   int count, max_rank, n, d, rows;
+  int from, to;  // the tile kernel's part of n
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -269,14 +270,18 @@ __global__ void __launch_bounds__(kThreads, 4) lora_row_kernel(const LoraArgs a,
 // as the N operand: D = A x' is [ranks][rows], then D = B h' [128 outputs][rows], whose lanes are neighbouring outputs
 // of one row for the epilogue's reads and writes. fp32 values are three bf16 parts (24 bits: x = x0 + x1 + x2 with no
 // scaling), fp16 weights two, fp32 weights three; a product is the sum of the parts' products up to 2^-24 of it
-// (x_i w_j with i + j <= 2). The tensor cores' sums truncate: in the first product, whose sums are long, the small
-// parts' sums have an accumulator of their own, so that the large one's is cut once for sixteen elements only.
+// (x_i w_j with i + j <= 2). The tensor cores' sums truncate, always towards zero: in the first product, whose sums are
+// long, the small parts' sums have an accumulator of their own, so that a large one is cut once for sixteen elements
+// only, and the large ones are three in turn, 48 cuts each at most (n = 10624: the result 1.2e-6 off with one, 0.4e-6
+// with three). Beyond kMaxSum elements another launch adds the product over the next ones.
 constexpr int kTileRows = 64;
 constexpr int kTileRank = 128;       // ranks the tile kernel takes
 constexpr int kMaxBins = 2048;       // adapters + 1 of the histogram
 constexpr int kMaxTileRows = 16384;  // rows of a launch: every CTA reads their indices
 constexpr int kStep = 64;            // elements of n a step: one 128-byte row of bf16
-constexpr uint32_t kTmemCols = 128;  // two accumulators of 64 rows
+constexpr uint32_t kTmemCols = 256;  // four accumulators of 64 rows
+constexpr int kTmemSmall = 192;      // the fourth takes the small parts of the first product
+constexpr int kMaxSum = 16384;       // elements of n that a launch sums in the three others
 
 // Parts of a weight.
 template <typename W>
@@ -546,8 +551,8 @@ __device__ __forceinline__ void write4(float *p, float4 v, int left, bool wide) 
     p[3] = v.w;
 }
 
-// parts clusters share a tile: each computes its vectors and takes a part of d.
-template <typename W>
+// parts clusters share a tile: each computes its vectors and takes a part of d. kPart: of n, the launch takes a part.
+template <typename W, bool kPart>
 __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a, int parts) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -601,8 +606,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
   // This CTA's slices of n and d. Its vectors' and its base's lines start on their way to L2 now.
   const int d_all = parts * ctas, d_slice = ((a.d + d_all - 1) / d_all + 31) / 32 * 32;
   const int d0 = min((part * ctas + rank) * d_slice, a.d), d1 = min(d0 + d_slice, a.d), tiles = (d1 - d0 + 127) / 128;
-  const int n_slice = ((a.n + ctas - 1) / ctas + kStep - 1) / kStep * kStep;
-  const int n0 = min(rank * n_slice, a.n), n1 = min(n0 + n_slice, a.n), steps = w.rank ? (n1 - n0 + kStep - 1) / kStep : 0;
+  const int from_n = kPart ? a.from : 0, to_n = kPart ? a.to : a.n;
+  const int n_slice = ((to_n - from_n + ctas - 1) / ctas + kStep - 1) / kStep * kStep;
+  const int n0 = min(from_n + rank * n_slice, to_n), n1 = min(n0 + n_slice, to_n);
+  const int steps = w.rank ? (n1 - n0 + kStep - 1) / kStep : 0;
   auto prefetch = [&](const float *from, long long ld, int c0, int c1) {
     const int lines = (c1 - c0 + 31) / 32;
     for (int e = threadIdx.x; e < rows * lines; e += kThreads) {
@@ -648,8 +655,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
       r.load(first, A, (size_t)a.n, w.rank, n0 + j * kStep, kStep / 8, 3, n1, a_wide);
     };
     const uint32_t idesc = umma_idesc_bf16(128, n16);
-    auto step = [&](float4 (&v)[4], WeightRuns<W, 2> &runs, int j) {
-      const int s = j & 1;
+    auto step = [&](auto odd, float4 (&v)[4], WeightRuns<W, 2> &runs, int j) {
+      constexpr int s = odd;  // j & 1
       uint8_t *stage = smem + s * L.stage, *xs = stage + P * a_bytes;
       if (j > 1) {  // the stage is free once the MMAs of two steps ago are done
         ok &= tile_wait(&t.bar[s], phase[s] & 1, abort_flag);
@@ -684,8 +691,9 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
                 continue;
 #pragma unroll
               for (int k = 0; k < kStep / 16; k++)
-                umma_bf16(tmem + (s2 ? 64 : 0), ad + (i * a_bytes + 32 * k) / 16, bd + ((s2 - i) * x_bytes + 32 * k) / 16,
-                          idesc, j > 0 || k > 0 || (s2 ? s2 < 2 || i > 0 : false));
+                umma_bf16(tmem + (s2 ? kTmemSmall : 64 * ((4 * s + k) % 3)), ad + (i * a_bytes + 32 * k) / 16,
+                          bd + ((s2 - i) * x_bytes + 32 * k) / 16, idesc,
+                          j > 0 || (s2 ? s2 < 2 || i > 0 || k > 0 : k > 2));
             }
           umma_commit(&t.bar[s]);
         }
@@ -701,9 +709,9 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
       load_w(runs2[1], 0, 1);
     load_x(x[1], 1);
     for (int j = 0; j < steps; j += 2) {
-      step(x[0], runs2[0], j);
+      step(std::integral_constant<int, 0>(), x[0], runs2[0], j);
       if (j + 1 < steps)
-        step(x[1], runs2[1], j + 1);
+        step(std::integral_constant<int, 1>(), x[1], runs2[1], j + 1);
     }
     // The last two steps' MMAs.
 #pragma unroll
@@ -720,15 +728,20 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
       const uint32_t from = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + column;
 #pragma unroll
       for (int c = 0; c < 32; c += 16) {
-        uint32_t d[16], e[16];
-        tmem_ld16(from + c, d);
-        tmem_ld16(from + 64 + c, e);
-        tmem_wait_ld();
+        float sum[16];
+#pragma unroll
+        for (int l = 0; l < 4; l++) {
+          uint32_t e[16];
+          tmem_ld16(from + 64 * l + c, e);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            sum[i] = l ? sum[i] + __uint_as_float(e[i]) : __uint_as_float(e[i]);
+        }
         if (k < rank16)
 #pragma unroll
           for (int i = 0; i < 16; i++)
-            partial[(column + c + i) * hs + k] =
-                k < w.rank ? __uint_as_float(d[i]) + __uint_as_float(e[i]) : 0.0f;
+            partial[(column + c + i) * hs + k] = k < w.rank ? sum[i] : 0.0f;
       }
     }
     tc_fence_before();
@@ -947,7 +960,8 @@ cudaError_t run(const LoraArgs &a) {
   if (a.count >= kMaxBins || a.max_rank > kTileRank || row_us<W>(a) <= tile_us<W>(a))
     return launch_rows<W>(a);
   const size_t smem = TileSmem<W>(a.max_rank).total;
-  cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(lora_tile_kernel<W>), TileSmem<W>(kTileRank).total);
+  void (*const kernel)(LoraArgs, int) = a.n > kMaxSum ? lora_tile_kernel<W, true> : lora_tile_kernel<W, false>;
+  cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(kernel), TileSmem<W>(kTileRank).total);
   for (int r = 0; r < a.rows && e == cudaSuccess; r += kMaxTileRows) {
     LoraArgs b = a;
     b.rows = a.rows - r < kMaxTileRows ? a.rows - r : kMaxTileRows;
@@ -955,9 +969,13 @@ cudaError_t run(const LoraArgs &a) {
     if (b.base)
       b.base += (long long)r * a.ldb;
     const int tiles = most_tiles(b), parts = parts_for(tiles);
-    e = launch<W>(lora_tile_kernel<W>, b, (unsigned)(tiles * parts), parts, smem);
-    if (e == cudaSuccess && r + kMaxTileRows < a.rows)
-      kc_count_launch();
+    for (int from = 0; from < a.n && e == cudaSuccess; from += kMaxSum) {
+      b.from = from, b.to = a.n - from < kMaxSum ? a.n : from + kMaxSum;
+      e = launch<W>(kernel, b, (unsigned)(tiles * parts), parts, smem);
+      if (e == cudaSuccess && (r + kMaxTileRows < a.rows || from + kMaxSum < a.n))
+        kc_count_launch();
+      b.base = b.out, b.ldb = b.ldo;
+    }
   }
   return e;
 }
@@ -986,7 +1004,7 @@ void k_lora_rows(float *out, size_t ldo, const float *base, size_t ldb, const fl
     return;
   }
   const LoraArgs a = {out, base, x, (long long)ldo, (long long)ldb, (long long)ldx, index, adapters, count, max_rank,
-                      n, d, rows};
+                      n, d, rows, 0, n};
   const cudaError_t e = type == K_F32 ? run<float>(a) : type == K_BF16 ? run<__nv_bfloat16>(a) : run<__half>(a);
   if (e == cudaSuccess)
     kc_count_launch();

@@ -282,6 +282,14 @@ LORA += [
 ]
 
 
+# Long rows: several passes over n, with a ragged last one.
+LORA += [
+    (260, 2, [64, 24], 16384 + 72, 256, torch.bfloat16),
+    (200, 1, [16], 3 * 16384 - 8, 264, torch.float32),
+    (140, 2, [100, 128], 20001, 130, torch.float16),
+]
+
+
 def lora_inputs(case, order, seed=0):
     rows, count, ranks, n, d, dtype = case
     g = generator(rows + seed)

@@ -26,7 +26,7 @@ constexpr int kMaxSplits = 64;     // of the prefix, or of a request's own posit
 
 constexpr float kLog2e = 1.44269504088896341f;
 
-constexpr int kGenericThreads = 128;
+constexpr int kGenericThreads = 256, kGenericWarps = kGenericThreads / 32;
 constexpr int kGenericVecs = 32;   // query vectors per CTA
 constexpr int kGenericPos = 32;    // positions per tile
 
@@ -188,8 +188,10 @@ __device__ __forceinline__ int limit_of(const SharedArgs &a, const Item &it, int
   return min(it.p1, it.start + divide(i, a.by_group) + 1);
 }
 
-// Any head_dim up to 256 and any alignment, in fp32 FMAs: a warp takes 8 of the tile's 32 vectors in turn, its lanes
-// the 32 positions of a tile for the scores and the head's elements for the sums.
+// Any head_dim up to 256 and any alignment, in fp32 FMAs: a warp takes a vector at a time, its lanes the 32 positions of
+// a tile for the scores and the head's elements for the sums. The shared-memory reads, two to an FMA, bound it, so the
+// positions are split finely (8 rows of 16 heads of 256 behind 2048 positions: 69 us; of 32 heads of 128 the tensor-core
+// kernel takes 18).
 __global__ void __launch_bounds__(kGenericThreads) shared_generic_kernel(const SharedArgs a) {
   extern __shared__ float smem[];
   pdl_wait();
@@ -200,10 +202,11 @@ __global__ void __launch_bounds__(kGenericThreads) shared_generic_kernel(const S
   const int hd = a.hd, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float *ks = smem;                                 // [32][hd + 1]
   float *vs = ks + kGenericPos * (hd + 1);          // [32][hd]
-  float *qs = vs + kGenericPos * hd;                // [4 warps][hd]
+  float *qs = vs + kGenericPos * hd;                // [8 warps][hd]
   const float scale = rsqrtf((float)hd) * kLog2e;
-  for (int v0 = 0; v0 < it.vecs; v0 += 4) {
-    // One vector a warp at a time; the tiles come again from the cache for the next four.
+  const bool wide = hd % 4 == 0 && (((uintptr_t)it.k | (uintptr_t)it.v) & 15) == 0;
+  for (int v0 = 0; v0 < it.vecs; v0 += kGenericWarps) {
+    // One vector a warp at a time; the tiles come again from the cache for the next eight.
     const int i = it.first + v0 + warp;
     const bool have = v0 + warp < it.vecs;
     const int vec = have ? vector_at(a, it.kv, i) : 0;
@@ -217,17 +220,40 @@ __global__ void __launch_bounds__(kGenericThreads) shared_generic_kernel(const S
     for (int t0 = it.p0; t0 < it.p1; t0 += kGenericPos) {
       const int n = min(kGenericPos, it.p1 - t0);
       __syncthreads();
-      for (int e = threadIdx.x; e < n * hd; e += kGenericThreads) {
-        const int p = e / hd, c = e - p * hd;
-        ks[p * (hd + 1) + c] = it.k[(size_t)t0 * hd + e];
-        vs[e] = it.v[(size_t)t0 * hd + e];
+#pragma unroll
+      for (int r = 0; r < kGenericPos / kGenericWarps; r++) {
+        const int p = warp + r * kGenericWarps;
+        if (p >= n)
+          break;
+        const float *kr = it.k + (size_t)(t0 + p) * hd, *vr = it.v + (size_t)(t0 + p) * hd;
+        float *kd = ks + p * (hd + 1), *vd = vs + p * hd;
+        if (wide) {
+          for (int c = 4 * lane; c < hd; c += 128) {
+            const float4 x = *reinterpret_cast<const float4 *>(kr + c);
+            *reinterpret_cast<float4 *>(vd + c) = *reinterpret_cast<const float4 *>(vr + c);
+            kd[c] = x.x, kd[c + 1] = x.y, kd[c + 2] = x.z, kd[c + 3] = x.w;
+          }
+        } else {
+          for (int c = lane; c < hd; c += 32)
+            kd[c] = kr[c], vd[c] = vr[c];
+        }
       }
       __syncthreads();
       const bool seen = t0 + lane < limit;
       float s = 0.0f;
-      if (seen)
-        for (int e = 0; e < hd; e++)
-          s = fmaf(qs[warp * hd + e], ks[lane * (hd + 1) + e], s);
+      if (seen) {
+        const float *qw = qs + warp * hd, *kl = ks + lane * (hd + 1);
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        int e = 0;
+#pragma unroll 4
+        for (; e + 4 <= hd; e += 4)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            part[j] = fmaf(qw[e + j], kl[e + j], part[j]);
+        for (; e < hd; e++)
+          part[0] = fmaf(qw[e], kl[e], part[0]);
+        s = (part[0] + part[1]) + (part[2] + part[3]);
+      }
       float top = seen ? s : -INFINITY;
 #pragma unroll
       for (int o = 16; o; o >>= 1)
@@ -275,6 +301,10 @@ __global__ void __launch_bounds__(kGenericThreads) shared_generic_kernel(const S
 // head against a range of positions in tiles of 64, S = Q K^T and O += P V on tcgen05 with accumulators in TMEM. The
 // tiles of all items run through the same stages: the next item's keys and values are under way, and its queries laid
 // out, before the last sums are done (a CTA per item took 215 us where this takes 199: 256 rows behind 8192 positions).
+// What bounds it: the conversion of keys and values, 2.7 thousand clocks a tile of 64 positions and 128 vectors, of which
+// the MMAs take 1.8. 256 rows of 32 heads of 128 behind 8192 positions: 186 us here and 12 in the join, 111 TFLOP/s of
+// fp32 products (333 of fp16), the tensor pipe 35 % busy, the shared-memory pipe 38 %, the issue slots 43 %; the rest is
+// the latency of eight converter warps, for which there are no more registers.
 //
 // fp32 products on half-precision tensor cores: x = 2^-k (hi + lo) with hi and lo fp16, 22 bits of x, and
 // x y = 2^-(k + k') (hi hi' + hi lo' + lo hi') up to 2^-22 of the product (what is dropped, lo lo', is below the
@@ -983,6 +1013,7 @@ bool tc_shape(const SharedArgs &a) {
 }
 
 // A warp per output vector: the splits joined in their order, and optionally quantized in gs-groups as k_quantize does.
+// 8192 vectors of 128 from 9 splits: 12 us, bounded by the partial results' way out of L2 (38 MB).
 __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs a) {
   __shared__ float weights[8][2 * kMaxSplits];
   __shared__ __align__(16) float outs[8][kMaxHd];
@@ -1111,13 +1142,15 @@ size_t partial_floats(int n_heads, int hd, int batch, int rows) {
 // Returns the CTAs, one per SM, or more where each would have more than kMaxItems items.
 constexpr double kItem = 2.2, kItemFull = 1.2;
 constexpr int kLongest = 16;
-int plan_splits(SharedArgs *a, int most) {
+int plan_splits(SharedArgs *a, int most, bool tc) {
   const int prefix_tiles = ceil_div(a->prefix, kTcPos), own_tiles = ceil_div(a->seq, kTcPos);
   const int columns = a->n_kv * a->tiles, own_columns = a->n_kv * a->batch * a->own_tiles;
   const int vecs = a->batch * a->rows * a->group, own_vecs = a->rows * a->group;
-  const double item = kItem + kItemFull * (vecs < kTcVecs ? vecs : kTcVecs) / kTcVecs;
-  const double own_item = kItem + kItemFull * (own_vecs < kTcVecs ? own_vecs : kTcVecs) / kTcVecs;
-  const double pass = (double)a->vectors * (a->hd + 2) * 8 / 5e12 / 1.5e-6;  // a split's partial results
+  double item = kItem + kItemFull * (vecs < kTcVecs ? vecs : kTcVecs) / kTcVecs;
+  double own_item = kItem + kItemFull * (own_vecs < kTcVecs ? own_vecs : kTcVecs) / kTcVecs;
+  double pass = (double)a->vectors * (a->hd + 2) * 8 / 5e12 / 1.5e-6;  // a split's partial results
+  if (!tc)  // a tile of the generic kernel takes ten times as long, the rest as long
+    item *= 0.1, own_item *= 0.1, pass *= 0.1;
   const int most_own = most / 2 < kMaxSplits ? most / 2 : kMaxSplits;
   double best = 0.0;
   int ctas = 1, tried_own = 0;
@@ -1164,7 +1197,7 @@ int plan_splits(SharedArgs *a, int most) {
   return ctas;
 }
 
-size_t generic_smem(int hd) { return sizeof(float) * ((size_t)kGenericPos * (2 * hd + 1) + 4 * (size_t)hd); }
+size_t generic_smem(int hd) { return sizeof(float) * ((size_t)kGenericPos * (2 * hd + 1) + kGenericWarps * (size_t)hd); }
 
 }  // namespace
 
@@ -1240,7 +1273,7 @@ void k_attention_shared_rows(float *out, int8_t *oq, float *os, const float *q, 
   const int tile = tc ? kTcVecs : kGenericVecs;
   a.tiles = ceil_div(batch * rows * a.group, tile);
   a.own_tiles = ceil_div(rows * a.group, tile);
-  const int ctas = plan_splits(&a, (int)((work->capacity - 4) / ((size_t)a.vectors * (head_dim + 2))));
+  const int ctas = plan_splits(&a, (int)((work->capacity - 4) / ((size_t)a.vectors * (head_dim + 2))), tc);
   a.by_prefix_splits = divisor(a.prefix_splits ? a.prefix_splits : 1);
   a.by_own_splits = divisor(a.own_splits);
   a.by_kv = divisor(a.n_kv);

@@ -133,7 +133,8 @@ __device__ __forceinline__ void expand_rows(const W *B, const float *h, int rank
   }
 }
 
-// A cluster of C CTAs per row.
+// A cluster of C CTAs per row. 33 rows of rank 32 fp32, 4096 to 14336: 10.4 us, 7.5 TB/s of adapters from L2, which
+// bounds it; 64 rows of rank 16 bf16, 4096 to 4096: 6.9 us, the chain index, adapter, A, cluster, B in one wave.
 template <typename W, int C>
 __global__ void __launch_bounds__(kThreads, 4) lora_row_kernel(const LoraArgs a, int) {
   __shared__ float part[kMaxRank], h[kMaxRank];
@@ -551,6 +552,9 @@ __device__ __forceinline__ void write4(float *p, float4 v, int left, bool wide) 
     p[3] = v.w;
 }
 
+// 2048 rows of 4 adapters of rank 64 bf16, 4096 to 4096: 44 us, 2.4 TB/s of the rows' own bytes, the tensor pipe 8 % and
+// the issue slots 23 % busy: the phases (rows, first product, the cluster's sum, second product) follow one another, two
+// CTAs an SM.
 // parts clusters share a tile: each computes its vectors and takes a part of d. kPart: of n, the launch takes a part.
 template <typename W, bool kPart>
 __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a, int parts) {

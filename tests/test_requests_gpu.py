@@ -204,6 +204,33 @@ def test_shared_attention_reports_bad_requests(kc, starts, counts):
     close(out, want, hd, top)
 
 
+@pytest.mark.parametrize("batch,rows,heads,kv,hd,prefix,room", [(700, 1, 8, 8, 64, 70, 40), (300, 3, 16, 8, 64, 333, 700),
+                                                                 (260, 2, 6, 2, 128, 0, 150)])
+def test_shared_attention_many_requests(kc, batch, rows, heads, kv, hd, prefix, room):
+    """Many more items than CTAs: requests of all lengths, a third of them out of use, partly used rows."""
+    g = generator(batch)
+    q = normal(g, batch, rows, heads * hd)
+    pk, pv = normal(g, kv, prefix, hd), normal(g, kv, prefix, hd)
+    k, v = normal(g, batch, kv, room, hd), normal(g, batch, kv, room, hd)
+    counts = torch.randint(-rows, rows + 1, (batch,), device="cuda", generator=g).clamp(min=0)
+    starts = (torch.rand(batch, device="cuda", generator=g) * (room - rows)).long()
+    got = run_attention(kc, q, pk if prefix else None, pv if prefix else None, prefix, k, v, starts.tolist(),
+                        counts.tolist(), heads, kv, hd)
+    row = torch.arange(rows, device="cuda")
+    q64 = q.double().view(batch, rows, kv, heads // kv, hd)
+    s = torch.cat([torch.einsum("brkgd,kpd->brkgp", q64, pk.double()), torch.einsum("brkgd,bkpd->brkgp", q64, k.double())],
+                  -1) / hd ** 0.5
+    seen = torch.arange(room, device="cuda") <= (starts[:, None] + row)[..., None]
+    seen = torch.cat([torch.ones(batch, rows, prefix, dtype=torch.bool, device="cuda"), seen], -1)
+    top = float(s.abs().max())
+    w = s.masked_fill(~seen[:, :, None, None], float("-inf")).softmax(-1)
+    want = torch.einsum("brkgp,kpd->brkgd", w[..., :prefix], pv.double()) + \
+        torch.einsum("brkgp,bkpd->brkgd", w[..., prefix:], v.double())
+    used = row < counts[:, None]
+    close(got[used], want.reshape(batch, rows, -1)[used], hd, top)
+    assert (got[~used] == -7.0).all()
+
+
 def test_shared_attention_is_the_engines_attention(kc):
     """One request whose positions are cut into a prefix and its own: k_attention_batch_kv over the whole cache."""
     heads, kv, hd, R, prefix, S = 32, 8, 128, 4, 300, 80

@@ -326,7 +326,10 @@ constexpr uint32_t kTmemQ = 0, kTmemS = 128, kTmemO = 256, kTmemCols = 512;  // 
 constexpr int kPShift = 7;  // probabilities are up to 2^8 (the lazy reference) and carry this power of two more
 
 constexpr int kMaxItems = 32;  // of a CTA: a lane of every warp finds one
-constexpr int kTailBytes = 6400;
+constexpr int kTailBytes = 8448;
+// The tensor cores' accumulators truncate: after so many tiles, half of them in each, an item's sums join its partial
+// result, in fp32, and start anew (error against 64 bits 2e-6; 4e-6 with twice as many, 15e-6 with 128).
+constexpr int kPartTiles = 16;
 
 template <int HD>
 struct TcSmem {
@@ -338,6 +341,25 @@ struct TcSmem {
 };
 
 __device__ __forceinline__ int tiles_of(const Item &it) { return (it.p1 - it.p0 + kTcPos - 1) / kTcPos; }
+
+// A CTA's work in order where items are long: of each item, one part of up to kPartTiles tiles after another.
+struct Part {
+  int n, p0, p1;
+  __device__ __forceinline__ explicit Part(const Item *items) : n(0) { begin(items[0].p0, items[0].p1); }
+  __device__ __forceinline__ void begin(int from, int end) { p0 = from, p1 = min(from + kPartTiles * kTcPos, end); }
+  // False past the last.
+  __device__ __forceinline__ bool next(const Item *items, int count) {
+    if (p1 < items[n].p1) {
+      begin(p1, items[n].p1);
+      return true;
+    }
+    if (++n >= count)
+      return false;
+    begin(items[n].p0, items[n].p1);
+    return true;
+  }
+  __device__ __forceinline__ int tiles() const { return (p1 - p0 + kTcPos - 1) / kTcPos; }
+};
 
 __device__ __forceinline__ const float *shfl_ptr(const float *p, int from) {
   return reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)p, from));
@@ -354,6 +376,7 @@ struct TcTail {
   int qshift[2][kTcVecs];  // of this item and the next
   float m[2][kTcVecs], l[2][kTcVecs];  // of a group's tiles, and the power of its O
   int vref[2][kTcVecs];
+  float2 joined[2][kTcVecs];  // (m, l) of an item's parts so far, a copy for each group
   Item items[kMaxItems];
 };
 static_assert(sizeof(TcTail) <= kTailBytes, "the tail's room");
@@ -571,7 +594,8 @@ struct Rows8 {
   }
 };
 
-template <int HD>
+// kLong: there may be items of several parts.
+template <int HD, bool kLong>
 __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedArgs a) {
   using L = TcSmem<HD>;
   extern __shared__ uint8_t smem_raw[];
@@ -695,7 +719,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     }
   } else if (warp == kSoftWarps) {
     // ---- MMA issue. The scores of tile j + 1 go out before the sums of tile j, so that they run under its softmax, or
-    // after them where they have to wait for the next item's queries. The MMAs run in the order of issue, so the scores
+    // after them where they have to wait for the next part's queries. The MMAs run in the order of issue, so the scores
     // of tile j + 2 never overtake the sums that read their buffer. ----
     const bool leader = elect_one();
     const uint32_t idesc_s = umma_idesc_f16(kTcVecs, kTcPos, false), idesc_o = umma_idesc_f16(kTcVecs, HD, true);
@@ -722,7 +746,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     };
     if (tc_wait(&t->qfull, 0, abort_flag))
       scores(0);
-    int first = 0, last = tiles_of(t->items[0]) - 1;  // the item's tiles
+    Part part(t->items);
+    int first = 0, last = (kLong ? part.tiles() : tiles_of(t->items[0])) - 1;  // the part's tiles
     for (int j = 0, n = 0;; j++) {
       if (j < last)
         scores(j + 1);
@@ -744,10 +769,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       }
       __syncwarp();
       if (j == last) {
-        if (++n == items || !tc_wait(&t->qfull, n & 1, abort_flag))
+        n++;
+        if (!(kLong ? part.next(t->items, items) : n < items) || !tc_wait(&t->qfull, n & 1, abort_flag))
           break;
         scores(j + 1);
-        first = j + 1, last = j + tiles_of(t->items[n]);
+        first = j + 1, last = j + (kLong ? part.tiles() : tiles_of(t->items[n]));
       }
     }
   } else {
@@ -756,15 +782,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     const uint32_t quadrant = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     const uint32_t ts = quadrant + kTmemS + 64 * g, to = quadrant + kTmemO + 128 * g;
     int vec = -1;
+    Part part(t->items);  // part n, and of the one before it the item and the first position
+    bool is = true;
+    int last_n = 0, last_p0 = 0;
     for (int n = 0, j0 = 0, j1 = 0;; n++) {
-      const int at = vec;
-      if (n < items) {
+      const int at = vec, item = kLong ? part.n : n;
+      const bool some = kLong ? is : n < items;
+      if (some) {
         // The queries become the A operand in TMEM once the scores of the tiles before are done. Group g's warps lay out
         // 16 of the quadrant's rows: lanes have four neighbouring elements of rows lane / 4 and lane / 4 + 8, whole
         // sectors of global memory and the layout in which they go to TMEM. Vectors not in use are zeros.
         vec = vec_ahead;
         constexpr int kParts = HD / 16;
-        if (32 * (warp & 3) < t->items[n].vecs) {
+        if (32 * (warp & 3) < t->items[item].vecs) {
           float4 x[2][kParts];
 #pragma unroll
           for (int r = 0; r < 2; r++) {
@@ -810,35 +840,47 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&t->qfull);
-        if (n + 1 < items)
-          vec_ahead = vector_of(a, t->items[n + 1].first, t->items[n + 1].vecs, t->items[n + 1].kv, vec_i);
+        Part ahead = part;
+        if (kLong ? ahead.next(t->items, items) : n + 1 < items) {
+          const Item &it = t->items[kLong ? ahead.n : n + 1];
+          vec_ahead = vector_of(a, it.first, it.vecs, it.kv, vec_i);
+        }
       }
       if (n) {
-        // Item n - 1: the two groups' results joined into the partial result, 16 rows of the quadrant by each, in the
-        // layout of the queries.
+        // Part n - 1: the two groups' results joined into the partial result, 16 rows of the quadrant by each, in the
+        // layout of the queries; a part behind the item's first adds to what its threads wrote before.
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
-        const Item &from_it = t->items[n - 1];
+        const Item &from_it = t->items[kLong ? last_n : n - 1];
+        const bool adds = kLong && last_p0 > from_it.p0;
         const int last0 = j1 - 1 - ((j1 - 1) & 1), last1 = j1 - 1 - (j1 & 1);  // the groups' last tiles
         const bool has0 = last0 >= j0, has1 = last1 >= j0;
         bool done = !has0 || tc_wait(&t->pvdone[0], (last0 >> 1) & 1, abort_flag);
         done = (!has1 || tc_wait(&t->pvdone[1], (last1 >> 1) & 1, abort_flag)) && done;
         if (done && 32 * (warp & 3) < from_it.vecs) {
           tc_fence_after();
-          const float m0 = t->m[0][vec_i], m1 = t->m[1][vec_i], both = fmaxf(m0, m1);
+          const float2 before = adds ? t->joined[g][vec_i] : make_float2(-INFINITY, 0.0f);
+          const float m0 = t->m[0][vec_i], m1 = t->m[1][vec_i], both = fmaxf(fmaxf(m0, m1), before.x);
+          const float keep = before.x == -INFINITY ? 0.0f : ex2(before.x - both);
           const float w0 = m0 == -INFINITY ? 0.0f : ex2(m0 - both), w1 = m1 == -INFINITY ? 0.0f : ex2(m1 - both);
+          float2 joined = make_float2(both, w0 * t->l[0][vec_i] + w1 * t->l[1][vec_i]);
+          if (kLong) {
+            joined.y += keep * before.y;
+            t->joined[g][vec_i] = joined;
+          }
           if (at >= 0 && g == 0)
-            a.ml[(size_t)from_it.split * a.vectors + at] = make_float2(both, w0 * t->l[0][vec_i] + w1 * t->l[1][vec_i]);
+            a.ml[(size_t)from_it.split * a.vectors + at] = joined;
           // Powers between 2^-106 and 2^107.
           const float f0 = w0 * pow2(-(kPShift + t->vref[0][vec_i])), f1 = w1 * pow2(-(kPShift + t->vref[1][vec_i]));
           float *part = a.acc + (size_t)from_it.split * a.vectors * hd + 2 * (lane & 3);
           float *dst[2];
-          uint64_t s0[2], s1[2];
+          uint64_t s0[2], s1[2], kept[2];
           bool in[2];
 #pragma unroll
           for (int r = 0; r < 2; r++) {
             const int row = 16 * g + (lane >> 2) + 8 * r;
             const float x0 = __shfl_sync(0xffffffffu, f0, row), x1 = __shfl_sync(0xffffffffu, f1, row);
-            s0[r] = f2_pack(x0, x0), s1[r] = f2_pack(x1, x1);
+            const float xk = __shfl_sync(0xffffffffu, keep, row);
+            s0[r] = f2_pack(x0, x0), s1[r] = f2_pack(x1, x1), kept[r] = f2_pack(xk, xk);
             const int to_vec = __shfl_sync(0xffffffffu, at, row);
             in[r] = to_vec >= 0;
             dst[r] = part + (size_t)max(to_vec, 0) * hd;
@@ -856,24 +898,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
                 const int r = e >> 1 & 1, col = c + 2 * (e & 12);
                 const uint64_t zero = f2_pack(0.0f, 0.0f);
                 const uint64_t y0 = has0 ? f2_mul(f2_pack_bits(o[e], o[e + 1]), s0[r]) : zero;
-                const uint64_t y = has1 ? f2_fma(f2_pack_bits(p[e], p[e + 1]), s1[r], y0) : y0;
+                uint64_t y = has1 ? f2_fma(f2_pack_bits(p[e], p[e + 1]), s1[r], y0) : y0;
                 float2 z;
-                f2_unpack(y, z.x, z.y);
-                if (in[r] && col + 2 * (lane & 3) < hd)
+                if (in[r] && col + 2 * (lane & 3) < hd) {
+                  if (adds) {
+                    z = *reinterpret_cast<const float2 *>(dst[r] + col);
+                    y = f2_fma(f2_pack(z.x, z.y), kept[r], y);
+                  }
+                  f2_unpack(y, z.x, z.y);
                   *reinterpret_cast<float2 *>(dst[r] + col) = z;
+                }
               }
             }
           tc_fence_before();
         }
-        if (n == items)
+        if (!some)
           break;
         // Only now may the next item's first sums overwrite O, and its results what the other group reads here.
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
       }
       tc_wait(&t->qfull, n & 1, abort_flag);
       const int qshift = t->qshift[n & 1][vec_i];
-      const Item &it = t->items[n];
-      j0 = j1, j1 += tiles_of(it);
+      const Item &it = t->items[item];
+      j0 = j1, j1 += kLong ? part.tiles() : tiles_of(it);
       const bool have = vec_i < it.vecs, busy = 32 * (warp & 3) < it.vecs;
       const int limit = have ? limit_of(a, it, it.first + vec_i) : it.p0;
       const int lowest = __reduce_min_sync(0xffffffffu, have ? limit : 0x7fffffff);
@@ -890,7 +937,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
           break;
         tc_fence_after();
         if (busy) {
-          const int p0 = it.p0 + (j - j0) * kTcPos;
+          const int p0 = (kLong ? part.p0 : it.p0) + (j - j0) * kTcPos;
           const bool masked = p0 + kTcPos > lowest;
           const float *kscale = t->kscale[j & 3];
           const int *vshift = t->vshift[j & 3];
@@ -989,6 +1036,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
           mbar_arrive(&t->pfull[g]);
       }
       t->m[g][vec_i] = m, t->l[g][vec_i] = l, t->vref[g][vec_i] = vref;
+      if (kLong) {
+        last_n = part.n, last_p0 = part.p0;
+        is = part.next(t->items, items);
+      }
     }
   }
   __syncthreads();
@@ -998,12 +1049,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
   }
 }
 
+template <int HD, bool kLong>
+cudaError_t launch_tc(const SharedArgs &a, unsigned ctas) {
+  const cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(shared_tc_kernel<HD, kLong>), TcSmem<HD>::total);
+  return e != cudaSuccess ? e
+                          : kc_launch_pdl(shared_tc_kernel<HD, kLong>, dim3(ctas), dim3(kTcThreads), TcSmem<HD>::total,
+                                          kc_stream(), a);
+}
+// Items of several parts only where the work's size or the longest split count leaves more than a part to a split (the
+// kernel without them is 7 % faster: 256 rows behind 8192 positions 200 us for 214).
 template <int HD>
 cudaError_t launch_tc(const SharedArgs &a, unsigned ctas) {
-  const cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(shared_tc_kernel<HD>), TcSmem<HD>::total);
-  return e != cudaSuccess ? e
-                          : kc_launch_pdl(shared_tc_kernel<HD>, dim3(ctas), dim3(kTcThreads),
-                                          TcSmem<HD>::total, kc_stream(), a);
+  const int longest = kPartTiles * kTcPos;
+  const bool parts = (a.prefix_splits && (a.prefix + a.prefix_splits - 1) / a.prefix_splits > longest) ||
+                     (a.seq + a.own_splits - 1) / a.own_splits > longest;
+  return parts ? launch_tc<HD, true>(a, ctas) : launch_tc<HD, false>(a, ctas);
 }
 
 // Heads of whole 16-byte units at 16-byte addresses.
@@ -1137,11 +1197,10 @@ size_t partial_floats(int n_heads, int hd, int batch, int rows) {
 // How the positions are split, `most` splits at most, two at least: the lengths whose CTAs are estimated to end first.
 // In units of a tile of 64 positions against a query tile (about 1.5 us): an item takes kItem units besides its tiles,
 // and kItemFull more with a whole tile of queries to bring and of results to write; the requests' caches are taken to be
-// half full; a split costs its partial results' way to memory and back. No more than kLongest tiles to a split: the
-// tensor cores' accumulators truncate, which over more tiles would show in the result.
+// half full; a split costs its partial results' way to memory and back. No more than kPartTiles tiles to a split where the
+// work's size allows it: a part more costs as much as an item.
 // Returns the CTAs, one per SM, or more where each would have more than kMaxItems items.
 constexpr double kItem = 2.2, kItemFull = 1.2;
-constexpr int kLongest = 16;
 int plan_splits(SharedArgs *a, int most, bool tc) {
   const int prefix_tiles = ceil_div(a->prefix, kTcPos), own_tiles = ceil_div(a->seq, kTcPos);
   const int columns = a->n_kv * a->tiles, own_columns = a->n_kv * a->batch * a->own_tiles;
@@ -1154,14 +1213,14 @@ int plan_splits(SharedArgs *a, int most, bool tc) {
   const int most_own = most / 2 < kMaxSplits ? most / 2 : kMaxSplits;
   double best = 0.0;
   int ctas = 1, tried_own = 0;
-  for (int own_length = own_tiles < kLongest ? own_tiles : kLongest; own_length >= 1; own_length -= own_length > 4 ? 2 : 1) {
+  for (int own_length = own_tiles < kPartTiles ? own_tiles : kPartTiles; own_length >= 1; own_length -= own_length > 4 ? 2 : 1) {
     const int own = ceil_div(own_tiles, own_length) < most_own ? ceil_div(own_tiles, own_length) : most_own;
     if (own == tried_own)
       continue;
     tried_own = own;
     const int rest = most - own < kMaxSplits ? most - own : kMaxSplits;
     int tried = -1;
-    for (int length = prefix_tiles < kLongest ? prefix_tiles : kLongest; length >= (prefix_tiles ? 1 : 0); length--) {
+    for (int length = prefix_tiles < kPartTiles ? prefix_tiles : kPartTiles; length >= (prefix_tiles ? 1 : 0); length--) {
       int n = prefix_tiles ? ceil_div(prefix_tiles, length) : 0;
       n = n < rest ? n : rest;
       if (n == tried)

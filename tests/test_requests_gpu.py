@@ -231,6 +231,23 @@ def test_shared_attention_many_requests(kc, batch, rows, heads, kv, hd, prefix, 
     assert (got[~used] == -7.0).all()
 
 
+@pytest.mark.parametrize("hd,batch,rows,prefix,room", [(64, 1, 2, 150000, 40), (128, 3, 1, 20, 70000), (128, 512, 4, 2085, 64)])
+def test_shared_attention_long_splits(kc, hd, batch, rows, prefix, room):
+    """More positions than the splits hold in one run of the accumulators: by the number of splits, and by the work's size
+    for many rows."""
+    heads, kv = (64, 2) if batch > 100 else (4, 2)
+    g = generator(hd + batch)
+    q = normal(g, batch, rows, heads * hd)
+    pk, pv = normal(g, kv, prefix, hd), normal(g, kv, prefix, hd)
+    k, v = normal(g, batch, kv, room, hd), normal(g, batch, kv, room, hd)
+    starts = [(room - rows) * (b + 1) // batch for b in range(batch)]
+    got = run_attention(kc, q, pk, pv, prefix, k, v, starts, [rows] * batch, heads, kv, hd)
+    some = sorted({0, batch // 2, batch - 1})
+    want, top = attention_64(q[some], pk, pv, prefix, k[some], v[some], [starts[b] for b in some], [rows] * len(some),
+                             heads, kv, hd, got[some])
+    close(got[some], want, hd, top)
+
+
 def test_shared_attention_is_the_engines_attention(kc):
     """One request whose positions are cut into a prefix and its own: k_attention_batch_kv over the whole cache."""
     heads, kv, hd, R, prefix, S = 32, 8, 128, 4, 300, 80

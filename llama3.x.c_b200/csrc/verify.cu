@@ -97,8 +97,10 @@ struct Weights {
     return l < floor ? 0.0 : w;
   }
 };
-// The floor: (l - m) / T is in [-760, 0] above it whatever the roundings, and finite.
-__device__ __forceinline__ float floor_of(float m, float t) { return fmaxf(fmaf(-700.0f, t, m), -FLT_MAX); }
+// The floor, the smallest float from m - 700 T on: (l - m) / T is in [-700, 0] above it, and finite. (Rounded to the
+// nearest it may lie half a step of m lower, which at a small T is far more than the 708 that a 64-bit exponent has room
+// for: at m = 20, T = 1e-8 it would be 763.)
+__device__ __forceinline__ float floor_of(float m, float t) { return fmaxf(__fmaf_ru(-700.0f, t, m), -FLT_MAX); }
 __device__ __forceinline__ double k32_of(float t) { return 46.166241308446829 / (double)t; }  // 32 / ln 2
 __device__ __forceinline__ void load_table(uint2 *table) {
   if (threadIdx.x < 32) {

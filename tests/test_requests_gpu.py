@@ -592,6 +592,29 @@ def test_verify_tiny_and_huge_temperatures(kc):
     assert (got[0] == want[0]).all() and (got[1] == want[1]).all()
 
 
+@pytest.mark.parametrize("drafts", [True, False])
+@pytest.mark.parametrize("top,t", [(20.0, 1e-8), (1500.0, 1e-6), (9.0, 1e-9), (17.0, 1.4e-9), (-20.0, 1e-8), (1e4, 3e-5),
+                                   (300.0, 2e-7)])
+def test_verify_low_temperatures(kc, top, t, drafts):
+    """Temperatures whose 700-fold is about a step of the largest logit: neighbouring numbers, ties and all the others
+    far below."""
+    vocab, B, R = 4200, 6, 2
+    rng = np.random.default_rng(15)
+    target = (top - 1.0 - abs(rng.standard_normal((B, R + 1, vocab)))).astype(np.float32)
+    top = np.float32(top)
+    target[:, :, 1234] = top
+    target[1::2, :, 4100] = top  # a tie
+    target[2::3, :, 77] = np.nextafter(top, np.float32(-np.inf))
+    draft = target[:, :R] - (rng.random((B, R, vocab)) < 0.5).astype(np.float32)
+    drafted = np.full((B, R), 1234, np.int32)
+    drafted[3:, 1] = [4100, 500, 77]
+    uniforms = rng.random((B, R + 1), dtype=np.float32)
+    args = (target, draft if drafts else None, drafted, np.full(B, R), uniforms, np.full(B, t, np.float32))
+    want = verify_64(*args, vocab)
+    got = run_verify(kc, *args, vocab, R)
+    assert (got[0] == want[0]).all() and (got[1] == want[1]).all()
+
+
 @pytest.mark.parametrize("what", ["nan", "inf", "empty", "draft_nan", "token", "negative", "count", "cold", "temp_nan"])
 def test_verify_reports(kc, what):
     """A needed row without a distribution, or arguments that mean nothing: no answer for that request, others whole."""

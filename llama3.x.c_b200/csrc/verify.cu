@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const Veri
   if (j < a.rows)
     drafted_s[j] = drafted;
   cluster.sync();  // every CTA has started before any writes into another's shared memory; the table is there
-  if (count < 0)
+  if (count == -1)
     return;  // the whole cluster: a slot of the batch that is not in use
   const Weights weight{table, greedy ? 0.0 : k32_of(t)};
   int *tokens = a.tokens + (long long)b * (a.rows + 1);

@@ -644,6 +644,25 @@ def test_verify_reports(kc, what):
         assert accepted[b] == whole[0][b] and (tokens[b] == whole[1][b]).all()
 
 
+@pytest.mark.parametrize("count", [-2, -100, -2 ** 31])
+def test_verify_reports_counts_below_the_unused_ones(kc, count):
+    """Only -1 is a slot that is not in use; a count below it is as wrong as one above the rows."""
+    B, R, vocab = 3, 2, 700
+    target, draft, drafted, counts, uniforms, temperature = verify_inputs(B, R, vocab, vocab, True, 16)
+    dev = lambda x, t: torch.tensor(np.asarray(x), dtype=t, device="cuda")  # noqa: E731
+    accepted = torch.full((B,), -9, dtype=torch.int32, device="cuda")
+    tokens = torch.full((B, R + 1), -9, dtype=torch.int32, device="cuda")
+    work = torch.empty(kc.k_verify_bytes(vocab, B, R), dtype=torch.uint8, device="cuda")
+    kc.k_verify_draft(accepted, tokens, dev(target, torch.float32), vocab, dev(draft, torch.float32), vocab,
+                      dev(drafted, torch.int32), dev([R, count, -1], torch.int32), dev(uniforms, torch.float32),
+                      dev(temperature, torch.float32), vocab, B, R, work)
+    with pytest.raises(kc.KernelError, match="rejected its arguments"):
+        kc.status()
+    want = verify_64(target, draft, drafted, [R, -1, -1], uniforms, temperature, vocab)
+    assert accepted.tolist() == [want[0][0], -1, -9]
+    assert tokens[0].tolist() == want[1][0].tolist() and (tokens[1] == -1).all() and (tokens[2] == -9).all()
+
+
 def test_verify_looks_at_no_row_behind_the_refused_draft(kc):
     B, R, vocab = 1, 3, 500
     target, draft, drafted, counts, uniforms, temperature = verify_inputs(B, R, vocab, vocab, True, 8)

@@ -501,16 +501,27 @@ def k_random_q8(q, s, rows, cols, row0, col0, full_cols, seed, tensor, std, gs):
 
 # ---- a batch of requests over one prompt ------------------------------------------------------------------------------
 
-def _want(dtype, *tensors, strided=False):
-    """The tensors (None allowed) must be contiguous ones (`strided`: rows with strides that the call names) of `dtype`
-    on the current device: their addresses are all that the library sees."""
+def _current_device():
     if _device is None:
         _bind_torch()
-    device = _device() if _device else None  # None: there are no CUDA tensors
+    return _device() if _device else None  # None: there are no CUDA tensors
+
+
+def _want(dtype, *tensors, strided=False):
+    """The tensors (None allowed) must be contiguous ones (`strided`: rows of neighbouring elements, with a row stride
+    that the call names) of `dtype` on the current device: their addresses are all that the library sees."""
+    device = _current_device()
     for t in tensors:
-        if t is not None and (t.dtype is not dtype or t.get_device() != device or not (strided or t.is_contiguous())):
+        if t is not None and (t.dtype is not dtype or t.get_device() != device or
+                              not (t.is_contiguous() or strided and (t.shape[-1] < 2 or t.stride(-1) == 1))):
             raise KernelError(f"needs a contiguous {dtype} CUDA tensor on the current device, got {t.dtype} on "
                               f"{t.device} with strides {tuple(t.stride())}")
+
+
+def _want_here(what, memory):
+    """Memory of any type (None allowed) on the current device."""
+    if memory is not None and memory.get_device() != _current_device():
+        raise KernelError(f"{what} must be on the current CUDA device, is on {memory.device}")
 
 
 def shared_attention_work(n_heads, n_kv_heads, head_dim, batch, rows):
@@ -530,6 +541,7 @@ def k_attention_shared_rows(out, oq, os_, q, prefix_key, prefix_value, prefix_se
     _want(torch.float32, out, q, prefix_key, prefix_value, kc, vc, os_)
     _want(torch.int32, starts, counts)
     _want(torch.int8, oq)
+    _want_here("the attention work", getattr(work, "_memory", None))
     _call("k_attention_shared_rows", _ptr(out), _ptr(oq), _ptr(os_), _ptr(q), _ptr(prefix_key), _ptr(prefix_value),
           prefix_seq_len, prefix, _ptr(kc), _ptr(vc), _ptr(starts), _ptr(counts), ctypes.byref(work), n_heads,
           n_kv_heads, head_dim, seq_len, batch, rows, gs)
@@ -541,6 +553,9 @@ def lora_table(a, b, scale):
     import torch
     if not (len(a) == len(b) == len(scale)) or not a:
         raise KernelError("lora_table needs as many a and b matrices as scales, at least one")
+    kinds = {torch.float32: K_F32, torch.bfloat16: K_BF16, torch.float16: K_F16}
+    if a[0].dtype not in kinds:
+        raise KernelError(f"lora_table takes float32, bfloat16 or float16 matrices, got {a[0].dtype}")
     for x, y in zip(a, b):
         _want(a[0].dtype, x, y)
         if x.shape[0] != y.shape[1] or x.shape[1] != a[0].shape[1] or y.shape[0] != b[0].shape[0]:
@@ -549,14 +564,21 @@ def lora_table(a, b, scale):
                                        for x, y, s in zip(a, b, scale)])
     table = torch.frombuffer(bytearray(entries), dtype=torch.uint8).to(a[0].device)
     table._tensors = (a, b)  # the table holds raw pointers
+    table._made_for = (kinds[a[0].dtype], a[0].shape[1], b[0].shape[0])
     return table
 
 
 def k_lora_rows(out, ldo, base, ldb, x, ldx, index, table, count, type, max_rank, n, d, rows):
-    """out = base + scale B (A x) with the adapter each row names (include/kernels_cuda.h); table from lora_table."""
+    """out = base + scale B (A x) with the adapter each row names (include/kernels_cuda.h); table from lora_table, whose
+    type and sizes have to be the call's."""
     import torch
     _want(torch.float32, out, base, x, strided=True)
     _want(torch.int32, index)
+    _want_here("the adapters' table", table)
+    made_for = getattr(table, "_made_for", (type, n, d))
+    if made_for != (type, n, d):
+        raise KernelError("a table of adapters of type %d, %d to %d, " % made_for +
+                          "for a call with type %d, %d to %d" % (type, n, d))
     if table is not None and count * ctypes.sizeof(LoraAdapter) > table.numel():
         raise KernelError(f"{count} adapters of a table of {table.numel() // ctypes.sizeof(LoraAdapter)}")
     _call("k_lora_rows", _ptr(out), ldo, _ptr(base), ldb, _ptr(x), ldx, _ptr(index), _ptr(table), count, type, max_rank,
@@ -574,6 +596,7 @@ def k_verify_draft(accepted, tokens, target, ldt, draft, ldd, drafted, counts, u
     _want(torch.int32, accepted, tokens, drafted, counts)
     _want(torch.float32, uniforms, temperature)
     _want(torch.float32, target, draft, strided=True)
+    _want_here("the work", work)
     if work is not None and work.numel() * work.element_size() < load().k_verify_bytes(vocab, batch, rows):
         raise KernelError("k_verify_draft: the work is too small for this shape")
     _call("k_verify_draft", _ptr(accepted), _ptr(tokens), _ptr(target), ldt, _ptr(draft), ldd, _ptr(drafted),

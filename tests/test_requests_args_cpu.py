@@ -137,3 +137,78 @@ def test_python_mirror_refuses_other_types_and_small_tables():
             kc.k_lora_rows(x, 4, None, 0, x, 4, i, None, 0, kc.K_F32, 4, 4, 4, 4)
     with pytest.raises(kc.KernelError, match="CUDA tensor on the current device"):
         kc.k_verify_draft(i, i, a, 4, None, 0, i, None, a, a, 4, 1, 1, a)
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """The mirror with the CPU as its device and nothing called: what passes its checks is listed."""
+    kc = load_package()
+    calls = []
+    monkeypatch.setattr(kc, "_device", lambda: -1)  # get_device() of a CPU tensor
+    monkeypatch.setattr(kc, "_call", lambda name, *args: calls.append(name))
+    return kc, calls
+
+
+@pytest.mark.parametrize("dtype,kind", [("float32", 0), ("bfloat16", 1), ("float16", 2)])
+def test_python_mirror_holds_a_table_to_its_call(on_cpu, dtype, kind):
+    """A table's adapters have a type and sizes; a call with others would read past their matrices."""
+    import torch
+    kc, calls = on_cpu
+    t = getattr(torch, dtype)
+    table = kc.lora_table([torch.zeros(8, 64, dtype=t)] * 2, [torch.zeros(32, 8, dtype=t)] * 2, [1.0, 2.0])
+    x, out, index = torch.zeros(4, 128), torch.zeros(4, 64), torch.zeros(4, dtype=torch.int32)
+    call = lambda kind=kind, n=64, d=32: kc.k_lora_rows(out, 64, None, 0, x, 128, index, table, 2, kind, 8, n, d, 4)  # noqa: E731
+    call()
+    assert calls == ["k_lora_rows"]
+    for other in ((kind + 1) % 3, (kind + 2) % 3):
+        with pytest.raises(kc.KernelError, match=f"table of adapters of type {kind}, 64 to 32, .* type {other}, 64 to 32"):
+            call(kind=other)
+    for sizes in (dict(n=128), dict(n=63), dict(d=64), dict(d=31)):
+        with pytest.raises(kc.KernelError, match="for a call with"):
+            call(**sizes)
+    assert calls == ["k_lora_rows"]
+    with pytest.raises(kc.KernelError, match="float32, bfloat16 or float16"):
+        kc.lora_table([torch.zeros(8, 64, dtype=torch.float64)], [torch.zeros(32, 8, dtype=torch.float64)], [1.0])
+
+
+def test_python_mirror_refuses_columns_apart(on_cpu):
+    """Rows may lie apart, a row's elements may not: transposed and sliced activations, outputs and logits."""
+    import torch
+    kc, calls = on_cpu
+    table = kc.lora_table([torch.zeros(8, 16)], [torch.zeros(16, 8)], [1.0])
+    index, good = torch.zeros(16, dtype=torch.int32), torch.zeros(16, 40)
+    kc.k_lora_rows(good[:, :16], 40, good[:, 16:32], 40, good[:, 20:36], 40, index, table, 1, kc.K_F32, 8, 16, 16, 16)
+    kc.k_lora_rows(good[:, :1], 40, None, 0, good[:1, :16], 40, index, table, 1, kc.K_F32, 8, 16, 16, 1)
+    assert len(calls) == 2
+    for bad in (good[:, :16].t(), good[:, ::2]):
+        for at in range(3):
+            out, base, x = [bad if i == at else good for i in range(3)]
+            with pytest.raises(kc.KernelError, match="contiguous torch.float32"):
+                kc.k_lora_rows(out, 40, base, 40, x, 40, index, table, 1, kc.K_F32, 8, 16, 16, 16)
+    i, u, t, work = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, 2), torch.ones(1), torch.zeros(1 << 16)
+    for target, draft in ((good.t(), None), (good, good.t())):
+        with pytest.raises(kc.KernelError, match="contiguous torch.float32"):
+            kc.k_verify_draft(i[:, :1], i, target, 40, draft, 40, i[:, :1], None, u, t, 16, 1, 1, work)
+    assert len(calls) == 2
+
+
+def test_python_mirror_refuses_memory_elsewhere(on_cpu):
+    """Works and tables on another device (here: one that holds nothing)."""
+    import torch
+    kc, calls = on_cpu
+    a, i = torch.zeros(4, 4), torch.zeros(4, dtype=torch.int32)
+
+    class Elsewhere:
+        device = "cuda:1"
+        get_device = staticmethod(lambda: 1)
+        numel, element_size = staticmethod(lambda: 1 << 20), staticmethod(lambda: 1)
+
+    with pytest.raises(kc.KernelError, match="the adapters' table must be on the current CUDA device, is on cuda:1"):
+        kc.k_lora_rows(a, 4, None, 0, a, 4, i, Elsewhere(), 1, kc.K_F32, 4, 4, 4, 4)
+    with pytest.raises(kc.KernelError, match="the work must be on the current CUDA device"):
+        kc.k_verify_draft(i[:1], i, a, 4, None, 0, i, None, a, a, 4, 1, 1, Elsewhere())
+    work = kc.AttentionWork()
+    work._memory = Elsewhere()
+    with pytest.raises(kc.KernelError, match="the attention work must be on the current CUDA device"):
+        kc.k_attention_shared_rows(a, None, None, a, a, a, 4, 4, a, a, i, i, work, 1, 1, 4, 4, 1, 4, 0)
+    assert not calls

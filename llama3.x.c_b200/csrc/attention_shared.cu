@@ -313,29 +313,25 @@ __global__ void __launch_bounds__(kGenericThreads) shared_generic_kernel(const S
 // into the scores' scale, k of the values into the probabilities' exponent (exact powers of two both).
 //
 // Warps: 0-3 the softmax of the even tiles and 4-7 that of the odd ones, a thread per query vector (TMEM lane), each
-// group with a reference, a sum and an O of its own (joined at the end), so that a group has two tiles' time; 8 issues
+// group with a reference and a sum of its own (joined at the end), so that a group has two tiles' time; 8 issues
 // the MMAs; 9-16 split eight keys and eight values of a tile each and store them as the MMAs' operands (keys K-major,
 // values MN-major, so neither is transposed), two stages. The queries are the A operand in TMEM (from shared memory an
 // MMA of 64 columns would wait for it), and the probabilities take the place of the scores they come from.
-// The running maximum is a whole-number reference m that moves only when a score exceeds it by 8 (a factor of 256): O
-// is seldom rescaled.
+//
+// The tensor cores' accumulators truncate, always towards zero. So P V of a tile is a product of its own (twelve MMAs,
+// the small terms first: four cuts that count), which the tile's group adds to the item's sums in fp32, rounded to
+// nearest, under the next tile's MMAs. Both lie in TMEM, each with a power of two per vector (powers are whole numbers,
+// so references move without a rounding). Accumulated over the tiles by the MMAs themselves, 16 tiles would be
+// 1.8e-6 off and a long run 15e-6, by an amount that depends on where the weight lies.
 constexpr int kTcVecs = 128, kTcPos = 64;
 constexpr int kSoftWarps = 8, kConvWarps = 8;
 constexpr int kTcThreads = 32 * (kSoftWarps + 1 + kConvWarps);
-constexpr uint32_t kTmemQ = 0, kTmemS = 128, kTmemO = 256, kTmemCols = 512;  // S and O: two buffers each
-constexpr int kPShift = 7;  // probabilities are up to 2^8 (the lazy reference) and carry this power of two more
+constexpr uint32_t kTmemQ = 0, kTmemS = 128, kTmemCols = 512;  // S: two buffers
+constexpr uint32_t kTmemSum = 256, kTmemProduct = 384;            // an item's sums so far, a tile's product
+constexpr int kPShift = 14;  // probabilities, up to 1, carry this power of two at most
 
 constexpr int kMaxItems = 32;  // of a CTA: a lane of every warp finds one
 constexpr int kTailBytes = 8448;
-// The tensor cores' accumulators truncate: after so many tiles, half of them in each, an item's sums join its partial
-// result, in fp32, and start anew (error against 64 bits 1e-6; 15e-6 with 128 and without the next line's factor).
-constexpr int kPartTiles = 16;
-// A truncation takes off half a step of 24 bits, 0.72 * 2^-24 of the accumulator on average over its mantissas, and over
-// a run the accumulator is about half of what it ends as: 2e-8 of the result for each MMA. A group's `tiles`, of which the
-// first starts with its two small terms, are given that back (error 1.8e-6 -> 1.0e-6 at 16 tiles of normal values, 3.2e-6
-// -> 1.4e-6 of positive ones).
-__device__ __forceinline__ float given_back(int tiles) { return 1.0f + 2e-8f * (12 * tiles - 8); }
-
 template <int HD>
 struct TcSmem {
   static constexpr int kv_bytes = kTcPos * HD * 2;  // hi or lo of K or V
@@ -347,44 +343,9 @@ struct TcSmem {
 
 __device__ __forceinline__ int tiles_of(const Item &it) { return (it.p1 - it.p0 + kTcPos - 1) / kTcPos; }
 
-// A CTA's work in order where items are long: of each item, one part of up to kPartTiles tiles after another.
-struct Part {
-  int n, p0, p1;
-  __device__ __forceinline__ explicit Part(const Item *items) : n(0) { begin(items[0].p0, items[0].p1); }
-  __device__ __forceinline__ void begin(int from, int end) { p0 = from, p1 = min(from + kPartTiles * kTcPos, end); }
-  // False past the last.
-  __device__ __forceinline__ bool next(const Item *items, int count) {
-    if (p1 < items[n].p1) {
-      begin(p1, items[n].p1);
-      return true;
-    }
-    if (++n >= count)
-      return false;
-    begin(items[n].p0, items[n].p1);
-    return true;
-  }
-  __device__ __forceinline__ int tiles() const { return (p1 - p0 + kTcPos - 1) / kTcPos; }
-};
-
 __device__ __forceinline__ const float *shfl_ptr(const float *p, int from) {
   return reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)p, from));
 }
-
-struct TcTail {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2], qfull;
-  uint32_t tmem;
-  int abort_flag;
-  float kscale[4][kConvWarps];  // 2^-k of eight keys, a ring of tiles
-  int vshift[4][kConvWarps];    // k of eight values
-  // A bit for each of eight positions whose keys or values hold a NaN or an infinity.
-  __align__(8) uint8_t wrong[4][kConvWarps];
-  int qshift[2][kTcVecs];  // of this item and the next
-  float m[2][kTcVecs], l[2][kTcVecs];  // of a group's tiles, and the power of its O
-  int vref[2][kTcVecs];
-  float2 joined[2][kTcVecs];  // (m, l) of an item's parts so far, a copy for each group
-  Item items[kMaxItems];
-};
-static_assert(sizeof(TcTail) <= kTailBytes, "the tail's room");
 
 // A whole warp's bounded wait, with one answer for all lanes: false once any wait of the CTA has given up.
 __device__ __forceinline__ bool tc_wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
@@ -467,6 +428,18 @@ __device__ __forceinline__ int shift_for(unsigned max_bits) {
 // 2^k for k <= 127, 0 below the normal range.
 __device__ __forceinline__ float pow2(int k) { return k < -126 ? 0.0f : __int_as_float((k + 127) << 23); }
 
+// The power of two 2^(m + rest) of a vector's values, as two whole numbers: m is a reference of the softmax (-infinity
+// where all values are zeros so far), which may be too large for the sum to be one, and rest is small.
+struct Power {
+  float m, rest;
+};
+__device__ __forceinline__ float minus(const Power &a, const Power &b) { return (a.m - b.m) + (a.rest - b.rest); }
+// 2^(a - b), 0 below the normal range; a is not above b by more than 127.
+__device__ __forceinline__ float pow2_ratio(const Power &a, const Power &b) {
+  const float e = minus(a, b);
+  return e >= -126.0f ? pow2((int)e) : 0.0f;
+}
+
 // Two values (packed) as packed fp16 high parts and the packed rest.
 __device__ __forceinline__ void split2(uint64_t xy, uint32_t &hi, uint32_t &lo) {
   float x, y;
@@ -496,6 +469,21 @@ __device__ __forceinline__ float abs_max3(float a, float b, float c) {
   return r;
 }
 __device__ __forceinline__ float abs_max(float m, float4 v) { return abs_max3(abs_max3(m, v.x, v.y), v.z, v.w); }
+
+struct TcTail {
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2], added, qfull;
+  uint32_t tmem;
+  int abort_flag;
+  float kscale[4][kConvWarps];  // 2^-k of eight keys, a ring of tiles
+  int vshift[4][kConvWarps];    // k of eight values
+  // A bit for each of eight positions whose keys or values hold a NaN or an infinity.
+  __align__(8) uint8_t wrong[4][kConvWarps];
+  int qshift[2][kTcVecs];  // of this item and the next
+  float m[2][kTcVecs], l[2][kTcVecs];  // of a group's tiles
+  Power sum[kTcVecs], last[kTcVecs];   // of the item's sums so far, and of its last tile's product where it has several
+  Item items[kMaxItems];
+};
+static_assert(sizeof(TcTail) <= kTailBytes, "the tail's room");
 
 // 16 bytes from global to shared memory, asynchronously; zeros without `in`.
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool in) {
@@ -599,8 +587,7 @@ struct Rows8 {
   }
 };
 
-// kLong: there may be items of several parts.
-template <int HD, bool kLong>
+template <int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedArgs a) {
   using L = TcSmem<HD>;
   extern __shared__ uint8_t smem_raw[];
@@ -644,6 +631,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       mbar_init(&t->pvdone[i], 1);
     }
     mbar_init(&t->qfull, kSoftWarps);
+    mbar_init(&t->added, kSoftWarps / 2);
     t->abort_flag = 0;
     fence_mbar_init();
   }
@@ -724,7 +712,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     }
   } else if (warp == kSoftWarps) {
     // ---- MMA issue. The scores of tile j + 1 go out before the sums of tile j, so that they run under its softmax, or
-    // after them where they have to wait for the next part's queries. The MMAs run in the order of issue, so the scores
+    // after them where they have to wait for the next item's queries. The MMAs run in the order of issue, so the scores
     // of tile j + 2 never overtake the sums that read their buffer. ----
     const bool leader = elect_one();
     const uint32_t idesc_s = umma_idesc_f16(kTcVecs, kTcPos, false), idesc_o = umma_idesc_f16(kTcVecs, HD, true);
@@ -751,55 +739,54 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     };
     if (tc_wait(&t->qfull, 0, abort_flag))
       scores(0);
-    Part part(t->items);
-    int first = 0, last = (kLong ? part.tiles() : tiles_of(t->items[0])) - 1;  // the part's tiles
+    int first = 0, last = tiles_of(t->items[0]) - 1;  // the item's tiles
+    int adds = 0;
     for (int j = 0, n = 0;; j++) {
       if (j < last)
         scores(j + 1);
       const int s = j & 1, use = j >> 1;
-      if (!tc_wait(&t->vfull[s], use & 1, abort_flag) || !tc_wait(&t->pfull[s], use & 1, abort_flag))
+      // An item's first product is its sums and its last one is taken at its end: those between are added to the sums
+      // before the next one takes their place.
+      if (!tc_wait(&t->vfull[s], use & 1, abort_flag) || !tc_wait(&t->pfull[s], use & 1, abort_flag) ||
+          (j > first + 1 && !tc_wait(&t->added, adds++ & 1, abort_flag)))
         break;
       tc_fence_after();
       if (leader) {
         const uint64_t vd = vdesc + (uint64_t)(s * (L::stage >> 4));
-        const uint32_t p = tmem + kTmemS + 64 * s, d = tmem + kTmemO + 128 * s;
+        const uint32_t p = tmem + kTmemS + 64 * s, d = tmem + (j == first ? kTmemSum : kTmemProduct);
 #pragma unroll
         for (int term = 0; term < 3; term++)
 #pragma unroll
           for (int c = 0; c < kTcPos / 16; c++)  // 32 positions: 16 columns of hi, 16 of lo
             umma_f16_ta(d, p + 32 * (c >> 1) + 8 * (c & 1) + (term == 0 ? 16 : 0),
-                        vd + ((term == 1 ? L::kv_bytes : 0) + 2048 * c) / 16, idesc_o, j > first + 1 || term || c);
+                        vd + ((term == 1 ? L::kv_bytes : 0) + 2048 * c) / 16, idesc_o, term || c);
         umma_commit(&t->pvdone[s]);
         umma_commit(&t->vempty[s]);
       }
       __syncwarp();
       if (j == last) {
-        n++;
-        if (!(kLong ? part.next(t->items, items) : n < items) || !tc_wait(&t->qfull, n & 1, abort_flag))
+        if (++n >= items || !tc_wait(&t->qfull, n & 1, abort_flag))
           break;
         scores(j + 1);
-        first = j + 1, last = j + (kLong ? part.tiles() : tiles_of(t->items[n]));
+        first = j + 1, last = j + tiles_of(t->items[n]);
       }
     }
   } else {
     // ---- softmax: a thread per query vector, group g the tiles of its parity ----
     const int g = warp >> 2, vec_i = 32 * (warp & 3) + lane;
     const uint32_t quadrant = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-    const uint32_t ts = quadrant + kTmemS + 64 * g, to = quadrant + kTmemO + 128 * g;
+    const uint32_t ts = quadrant + kTmemS + 64 * g;
     int vec = -1;
-    Part part(t->items);  // part n, and of the one before it the item and the first position
-    bool is = true;
-    int last_n = 0, last_p0 = 0;
     for (int n = 0, j0 = 0, j1 = 0;; n++) {
-      const int at = vec, item = kLong ? part.n : n;
-      const bool some = kLong ? is : n < items;
+      const int at = vec;
+      const bool some = n < items;
       if (some) {
         // The queries become the A operand in TMEM once the scores of the tiles before are done. Group g's warps lay out
         // 16 of the quadrant's rows: lanes have four neighbouring elements of rows lane / 4 and lane / 4 + 8, whole
         // sectors of global memory and the layout in which they go to TMEM. Vectors not in use are zeros.
         vec = vec_ahead;
         constexpr int kParts = HD / 16;
-        if (32 * (warp & 3) < t->items[item].vecs) {
+        if (32 * (warp & 3) < t->items[n].vecs) {
           float4 x[2][kParts];
 #pragma unroll
           for (int r = 0; r < 2; r++) {
@@ -845,72 +832,56 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&t->qfull);
-        Part ahead = part;
-        if (kLong ? ahead.next(t->items, items) : n + 1 < items) {
-          const Item &it = t->items[kLong ? ahead.n : n + 1];
+        if (n + 1 < items) {
+          const Item &it = t->items[n + 1];
           vec_ahead = vector_of(a, it.first, it.vecs, it.kv, vec_i);
         }
       }
       if (n) {
-        // Part n - 1: the two groups' results joined into the partial result, 16 rows of the quadrant by each, in the
-        // layout of the queries; a part behind the item's first adds to what its threads wrote before.
+        // Item n - 1: the sums, and the last tile's product with them, become the partial result, 16 rows of the quadrant
+        // by each group, in the layout of the queries.
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
-        const Item &from_it = t->items[kLong ? last_n : n - 1];
-        const bool adds = kLong && last_p0 > from_it.p0;
-        const int last0 = j1 - 1 - ((j1 - 1) & 1), last1 = j1 - 1 - (j1 & 1);  // the groups' last tiles
-        const bool has0 = last0 >= j0, has1 = last1 >= j0;
-        bool done = !has0 || tc_wait(&t->pvdone[0], (last0 >> 1) & 1, abort_flag);
-        done = (!has1 || tc_wait(&t->pvdone[1], (last1 >> 1) & 1, abort_flag)) && done;
+        const Item &from_it = t->items[n - 1];
+        const bool several = j1 - j0 > 1;
+        const bool done = tc_wait(&t->pvdone[(j1 - 1) & 1], ((j1 - 1) >> 1) & 1, abort_flag);
         if (done && 32 * (warp & 3) < from_it.vecs) {
           tc_fence_after();
-          const float2 before = adds ? t->joined[g][vec_i] : make_float2(-INFINITY, 0.0f);
-          const float m0 = t->m[0][vec_i], m1 = t->m[1][vec_i], both = fmaxf(fmaxf(m0, m1), before.x);
-          const float keep = before.x == -INFINITY ? 0.0f : ex2(before.x - both);
+          const float m0 = t->m[0][vec_i], m1 = t->m[1][vec_i], both = fmaxf(m0, m1);
           const float w0 = m0 == -INFINITY ? 0.0f : ex2(m0 - both), w1 = m1 == -INFINITY ? 0.0f : ex2(m1 - both);
-          float2 joined = make_float2(both, w0 * t->l[0][vec_i] + w1 * t->l[1][vec_i]);
-          if (kLong) {
-            joined.y += keep * before.y;
-            t->joined[g][vec_i] = joined;
-          }
           if (at >= 0 && g == 0)
-            a.ml[(size_t)from_it.split * a.vectors + at] = joined;
-          // Powers between 2^-106 and 2^107.
-          const float f0 = w0 * given_back((last0 - j0) / 2 + 1) * pow2(-(kPShift + t->vref[0][vec_i]));
-          const float f1 = w1 * given_back((last1 - j0) / 2 + 1) * pow2(-(kPShift + t->vref[1][vec_i]));
+            a.ml[(size_t)from_it.split * a.vectors + at] = make_float2(both, w0 * t->l[0][vec_i] + w1 * t->l[1][vec_i]);
+          const Power result = {both, 0.0f};
+          const float f0 = both == -INFINITY ? 0.0f : pow2_ratio(t->sum[vec_i], result);
+          const float f1 = both == -INFINITY || !several ? 0.0f : pow2_ratio(t->last[vec_i], result);
           float *part = a.acc + (size_t)from_it.split * a.vectors * hd + 2 * (lane & 3);
           float *dst[2];
-          uint64_t s0[2], s1[2], kept[2];
+          uint64_t s0[2], s1[2];
           bool in[2];
 #pragma unroll
           for (int r = 0; r < 2; r++) {
             const int row = 16 * g + (lane >> 2) + 8 * r;
             const float x0 = __shfl_sync(0xffffffffu, f0, row), x1 = __shfl_sync(0xffffffffu, f1, row);
-            const float xk = __shfl_sync(0xffffffffu, keep, row);
-            s0[r] = f2_pack(x0, x0), s1[r] = f2_pack(x1, x1), kept[r] = f2_pack(xk, xk);
+            s0[r] = f2_pack(x0, x0), s1[r] = f2_pack(x1, x1);
             const int to_vec = __shfl_sync(0xffffffffu, at, row);
             in[r] = to_vec >= 0;
             dst[r] = part + (size_t)max(to_vec, 0) * hd;
           }
-          const uint32_t from = quadrant + ((uint32_t)(16 * g) << 16) + kTmemO;
+          const uint32_t from = quadrant + ((uint32_t)(16 * g) << 16);
           if (32 * (warp & 3) + 16 * g < from_it.vecs)
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
               uint32_t o[16], p[16];
-              tmem_ld_rows(from + c, o);
-              tmem_ld_rows(from + 128 + c, p);
+              tmem_ld_rows(from + kTmemSum + c, o);
+              tmem_ld_rows(from + kTmemProduct + c, p);
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
                 const int r = e >> 1 & 1, col = c + 2 * (e & 12);
-                const uint64_t zero = f2_pack(0.0f, 0.0f);
-                const uint64_t y0 = has0 ? f2_mul(f2_pack_bits(o[e], o[e + 1]), s0[r]) : zero;
-                uint64_t y = has1 ? f2_fma(f2_pack_bits(p[e], p[e + 1]), s1[r], y0) : y0;
-                float2 z;
+                uint64_t y = f2_mul(f2_pack_bits(o[e], o[e + 1]), s0[r]);
+                if (several)
+                  y = f2_fma(f2_pack_bits(p[e], p[e + 1]), s1[r], y);
                 if (in[r] && col + 2 * (lane & 3) < hd) {
-                  if (adds) {
-                    z = *reinterpret_cast<const float2 *>(dst[r] + col);
-                    y = f2_fma(f2_pack(z.x, z.y), kept[r], y);
-                  }
+                  float2 z;
                   f2_unpack(y, z.x, z.y);
                   *reinterpret_cast<float2 *>(dst[r] + col) = z;
                 }
@@ -920,30 +891,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
         }
         if (!some)
           break;
-        // Only now may the next item's first sums overwrite O, and its results what the other group reads here.
+        // Only now may the next item's first product overwrite the sums, and its results what the other group reads here.
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory");
       }
       tc_wait(&t->qfull, n & 1, abort_flag);
       const int qshift = t->qshift[n & 1][vec_i];
-      const Item &it = t->items[item];
-      j0 = j1, j1 += kLong ? part.tiles() : tiles_of(it);
+      const Item &it = t->items[n];
+      j0 = j1, j1 += tiles_of(it);
       const bool have = vec_i < it.vecs, busy = 32 * (warp & 3) < it.vecs;
       const int limit = have ? limit_of(a, it, it.first + vec_i) : it.p0;
       const int lowest = __reduce_min_sync(0xffffffffu, have ? limit : 0x7fffffff);
       const float scale = rsqrtf((float)hd) * kLog2e * pow2(-qshift);
       float m = -INFINITY, l = 0.0f;
-      int vref = 0;  // O holds sums times 2^(kPShift + vref)
       for (int j = j0 + ((j0 ^ g) & 1); j < j1; j += 2) {
         const int use = j >> 1;
-        const bool begin = j < j0 + 2;
-        // The scores, the values' powers, and the group's previous sums: O can be rescaled. (Those are done when the
-        // scores are; the wait keeps step with the barrier's phases.)
+        // The scores and the values' powers. (The group's previous product is done when the scores are; the wait keeps
+        // step with the barrier's phases.)
         if (!tc_wait(&t->sfull[g], use & 1, abort_flag) || !tc_wait(&t->vfull[g], use & 1, abort_flag) ||
             (use > 0 && !tc_wait(&t->pvdone[g], (use - 1) & 1, abort_flag)))
           break;
         tc_fence_after();
+        Power own = {-INFINITY, 0.0f};  // of the tile's product
         if (busy) {
-          const int p0 = (kLong ? part.p0 : it.p0) + (j - j0) * kTcPos;
+          const int p0 = it.p0 + (j - j0) * kTcPos;
           const bool masked = p0 + kTcPos > lowest;
           const float *kscale = t->kscale[j & 3];
           const int *vshift = t->vshift[j & 3];
@@ -975,28 +945,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
 #pragma unroll
           for (int w = 1; w < kConvWarps; w++)
             vmin = min(vmin, vshift[w]);
-          // Move the reference when a score exceeds it by more than 8, and O's power when the values have grown.
-          const bool up = top > m + 8.0f || (m == -INFINITY && top > m);
-          const float m_new = up ? ceilf(top) : m;
-          const int vref_new = begin || vmin < vref ? vmin - 1 : vref;
-          const float keep = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - m_new);
-          if (!begin && (vref_new != vref || __any_sync(0xffffffffu, up))) {
-            const float f = keep * pow2(vref_new - vref);
-#pragma unroll 1
-            for (int c = 0; c < HD; c += 16) {
-              uint32_t o[16];
-              tmem_ld16(to + c, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 16; e++)
-                o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st16(to + c, o);
-            }
-          }
-          l *= keep;
+          const float m_new = fmaxf(m, ceilf(top));
+          l *= m == -INFINITY ? 0.0f : ex2(m - m_new);
           m = m_new;
-          vref = vref_new;
           const float base = m == -INFINITY ? 0.0f : m;
+          own = Power{m, (float)(-kPShift - vmin)};
 #pragma unroll 1
           for (int c = 0; c < 64; c += 32) {
             uint32_t r[32], hi[16], lo[16];
@@ -1011,7 +964,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
               // 2^(score - m) times 2^grow, the values' power in the exponent: base and grow are whole numbers. Values
               // 2^-60 of the largest seen (zeros, mostly) count as that at most, which O does not hold.
               const float f = factor((c + e8) >> 3);
-              const int grow = max(kPShift - vshift[(c + e8) >> 3] + vref, -60);
+              const int grow = max(kPShift - vshift[(c + e8) >> 3] + vmin, -60);
               const float from = (float)grow - base;
               const uint64_t f2 = f2_pack(f, f), from2 = f2_pack(from, from);
               uint64_t sum2 = 0;
@@ -1036,16 +989,47 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
           if (wrong && limit > p0 && (limit - p0 >= 64 || wrong << (64 - (limit - p0))))
             l = NAN;
         }
+        if (busy && j == j0)
+          t->sum[vec_i] = own;
+        if (busy && j == j1 - 1)
+          t->last[vec_i] = own;
         tc_fence_before();
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&t->pfull[g]);
+        if (j > j0 && j < j1 - 1) {
+          if (!tc_wait(&t->pvdone[g], use & 1, abort_flag))
+            break;
+          tc_fence_after();
+          if (busy) {
+            const Power before = t->sum[vec_i];
+            const Power after = minus(own, before) > 0.0f ? own : before;
+            const float keep = pow2_ratio(before, after), f = pow2_ratio(own, after);
+            const uint64_t keep2 = f2_pack(keep, keep), f2 = f2_pack(f, f);
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t o[16], p[16];
+              tmem_ld16(quadrant + kTmemSum + c, o);
+              tmem_ld16(quadrant + kTmemProduct + c, p);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                float y0, y1;
+                f2_unpack(f2_fma(f2_pack_bits(p[e], p[e + 1]), f2, f2_mul(f2_pack_bits(o[e], o[e + 1]), keep2)), y0, y1);
+                o[e] = __float_as_uint(y0), o[e + 1] = __float_as_uint(y1);
+              }
+              tmem_st16(quadrant + kTmemSum + c, o);
+            }
+            tmem_wait_st();
+            t->sum[vec_i] = after;
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive(&t->added);
+        }
       }
-      t->m[g][vec_i] = m, t->l[g][vec_i] = l, t->vref[g][vec_i] = vref;
-      if (kLong) {
-        last_n = part.n, last_p0 = part.p0;
-        is = part.next(t->items, items);
-      }
+      t->m[g][vec_i] = m, t->l[g][vec_i] = l;
     }
   }
   __syncthreads();
@@ -1055,21 +1039,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
   }
 }
 
-template <int HD, bool kLong>
-cudaError_t launch_tc(const SharedArgs &a, unsigned ctas) {
-  const cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(shared_tc_kernel<HD, kLong>), TcSmem<HD>::total);
-  return e != cudaSuccess ? e
-                          : kc_launch_pdl(shared_tc_kernel<HD, kLong>, dim3(ctas), dim3(kTcThreads), TcSmem<HD>::total,
-                                          kc_stream(), a);
-}
-// Items of several parts only where the work's size or the longest split count leaves more than a part to a split (the
-// kernel without them is 7 % faster: 256 rows behind 8192 positions 200 us for 214).
 template <int HD>
 cudaError_t launch_tc(const SharedArgs &a, unsigned ctas) {
-  const int longest = kPartTiles * kTcPos;
-  const bool parts = (a.prefix_splits && (a.prefix + a.prefix_splits - 1) / a.prefix_splits > longest) ||
-                     (a.seq + a.own_splits - 1) / a.own_splits > longest;
-  return parts ? launch_tc<HD, true>(a, ctas) : launch_tc<HD, false>(a, ctas);
+  const cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(shared_tc_kernel<HD>), TcSmem<HD>::total);
+  return e != cudaSuccess ? e
+                          : kc_launch_pdl(shared_tc_kernel<HD>, dim3(ctas), dim3(kTcThreads), TcSmem<HD>::total,
+                                          kc_stream(), a);
 }
 
 // Heads of whole 16-byte units at 16-byte addresses.
@@ -1203,10 +1178,11 @@ size_t partial_floats(int n_heads, int hd, int batch, int rows) {
 // How the positions are split, `most` splits at most, two at least: the lengths whose CTAs are estimated to end first.
 // In units of a tile of 64 positions against a query tile (about 1.5 us): an item takes kItem units besides its tiles,
 // and kItemFull more with a whole tile of queries to bring and of results to write; the requests' caches are taken to be
-// half full; a split costs its partial results' way to memory and back. No more than kPartTiles tiles to a split where the
-// work's size allows it: a part more costs as much as an item.
+// half full; a split costs its partial results' way to memory and back. No more than kSplitTiles tiles to a split where the
+// work's size allows it.
 // Returns the CTAs, one per SM, or more where each would have more than kMaxItems items.
 constexpr double kItem = 2.2, kItemFull = 1.2;
+constexpr int kSplitTiles = 16;
 int plan_splits(SharedArgs *a, int most, bool tc) {
   const int prefix_tiles = ceil_div(a->prefix, kTcPos), own_tiles = ceil_div(a->seq, kTcPos);
   const int columns = a->n_kv * a->tiles, own_columns = a->n_kv * a->batch * a->own_tiles;
@@ -1219,14 +1195,14 @@ int plan_splits(SharedArgs *a, int most, bool tc) {
   const int most_own = most / 2 < kMaxSplits ? most / 2 : kMaxSplits;
   double best = 0.0;
   int ctas = 1, tried_own = 0;
-  for (int own_length = own_tiles < kPartTiles ? own_tiles : kPartTiles; own_length >= 1; own_length -= own_length > 4 ? 2 : 1) {
+  for (int own_length = own_tiles < kSplitTiles ? own_tiles : kSplitTiles; own_length >= 1; own_length -= own_length > 4 ? 2 : 1) {
     const int own = ceil_div(own_tiles, own_length) < most_own ? ceil_div(own_tiles, own_length) : most_own;
     if (own == tried_own)
       continue;
     tried_own = own;
     const int rest = most - own < kMaxSplits ? most - own : kMaxSplits;
     int tried = -1;
-    for (int length = prefix_tiles < kPartTiles ? prefix_tiles : kPartTiles; length >= (prefix_tiles ? 1 : 0); length--) {
+    for (int length = prefix_tiles < kSplitTiles ? prefix_tiles : kSplitTiles; length >= (prefix_tiles ? 1 : 0); length--) {
       int n = prefix_tiles ? ceil_div(prefix_tiles, length) : 0;
       n = n < rest ? n : rest;
       if (n == tried)

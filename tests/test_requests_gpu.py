@@ -248,6 +248,53 @@ def test_shared_attention_long_splits(kc, hd, batch, rows, prefix, room):
     close(got[some], want, hd, top)
 
 
+# Root mean square, relative, of results in which no score's error shows: the tensor cores cut a tile's product four times
+# by up to 2^-23 of what has come together by then (5/8 of it on average over the four), a probability and a value are
+# pairs of half-precision numbers (2^-23 at most each), and the sums over tiles and splits, the weights' sum, the joins
+# and the division are some 50 roundings of 2^-24 at most: random ones, of 2^-24 sqrt(50 / 3) together.
+PRODUCTS = (4 * 5 / 8 + 2) * 2.0 ** -23 + 4 * 2.0 ** -24
+
+
+def norm_error(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+LONG = [(64, 1, 2, 150000, 40), (128, 3, 1, 20, 70000), (128, 512, 4, 2085, 64), (128, 8, 1, 2048, 40), (64, 64, 4, 1024, 30)]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "-".join(map(str, c)))
+def test_shared_attention_of_equal_values_is_the_value(kc, case):
+    """Whatever the weights, and however many tiles a split has."""
+    hd, batch, rows, prefix, room = case
+    heads, kv = (32, 2) if batch > 2 else (4, 2)
+    g = generator(hd + batch + 1)
+    q, pk, k = normal(g, batch, rows, heads * hd), normal(g, kv, prefix, hd), normal(g, batch, kv, room, hd)
+    value = normal(g, kv, 1, hd)
+    pv, v = value.expand(kv, prefix, hd).contiguous(), value.expand(batch, kv, room, hd).contiguous()
+    got = run_attention(kc, q, pk, pv, prefix, k, v, [room - rows] * batch, [rows] * batch, heads, kv, hd)
+    want = value.double().expand(kv, heads // kv, hd).reshape(-1)
+    assert norm_error(got, want.expand_as(got)) <= PRODUCTS
+
+
+@pytest.mark.parametrize("place", [0.0, 0.5, 1.0])
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "-".join(map(str, c)))
+def test_shared_attention_of_one_dominant_position(kc, case, place):
+    """A position with 0.998 of the weight, at the start, in the middle and at the end of the prefix: its value is the
+    result, with no part of it lost or added on the way."""
+    hd, batch, rows, prefix, room = case
+    heads, kv = (32, 2) if batch > 2 else (4, 2)
+    g = generator(hd + batch + 2)
+    q = torch.ones(batch, rows, heads * hd, device="cuda")
+    pk, pv = normal(g, kv, prefix, hd), normal(g, kv, prefix, hd)
+    k, v = normal(g, batch, kv, room, hd), normal(g, batch, kv, room, hd)
+    pk[:, int(place * (prefix - 1))] = (0.5 + float(np.log(500 * (prefix + room)))) / hd ** 0.5
+    got = run_attention(kc, q, pk, pv, prefix, k, v, [room - rows] * batch, [rows] * batch, heads, kv, hd)
+    some = sorted({0, batch - 1})
+    want, _ = attention_64(q[some], pk, pv, prefix, k[some], v[some], [room - rows] * len(some), [rows] * len(some), heads,
+                           kv, hd, got[some])
+    assert norm_error(got[some], want) <= PRODUCTS
+
+
 def test_shared_attention_is_the_engines_attention(kc):
     """One request whose positions are cut into a prefix and its own: k_attention_batch_kv over the whole cache."""
     heads, kv, hd, R, prefix, S = 32, 8, 128, 4, 300, 80

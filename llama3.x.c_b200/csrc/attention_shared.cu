@@ -8,10 +8,11 @@
 // out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i with M the largest m_i. Statistics and accumulators are fp32.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
-#include <float.h>
 #include <math.h>
 #include <stdint.h>
 #include <string.h>
+
+#include <type_traits>
 
 #include "../../include/kernels_cuda.h"
 #include "common.cuh"
@@ -308,9 +309,12 @@ __global__ void __launch_bounds__(kGenericThreads) shared_generic_kernel(const S
 //
 // fp32 products on half-precision tensor cores: x = 2^-k (hi + lo) with hi and lo fp16, 22 bits of x, and
 // x y = 2^-(k + k') (hi hi' + hi lo' + lo hi') up to 2^-22 of the product (what is dropped, lo lo', is below the
-// rounding of lo). The power 2^k puts the largest magnitude of a query vector, of eight keys or of eight values just
-// below 2^15, so no finite input overflows and a value 2^-17 of the largest still keeps its 22 bits. k of the keys goes
-// into the scores' scale, k of the values into the probabilities' exponent (exact powers of two both).
+// rounding of lo). The power 2^k puts the largest magnitude of one query, key or value vector just below 2^15, so no
+// finite input overflows and an element 2^-17 of its vector's largest still keeps its 22 bits. k of a key goes into its
+// scores' scale, k of a value into its probabilities (exact powers of two both). No power is shared between positions: a
+// vector that a row does not see, or that has no weight in it, takes no bits of the others. For the same reason the
+// probabilities' own power, one to a row and tile, follows the largest product of a seen probability and its value's
+// power: what is added to a row's result is off by 2^-22 of itself and 2^-39 of the largest one.
 //
 // Warps: 0-3 the softmax of the even tiles and 4-7 that of the odd ones, a thread per query vector (TMEM lane), each
 // group with a reference and a sum of its own (joined at the end), so that a group has two tiles' time; 8 issues
@@ -328,10 +332,10 @@ constexpr int kSoftWarps = 8, kConvWarps = 8;
 constexpr int kTcThreads = 32 * (kSoftWarps + 1 + kConvWarps);
 constexpr uint32_t kTmemQ = 0, kTmemS = 128, kTmemCols = 512;  // S: two buffers
 constexpr uint32_t kTmemSum = 256, kTmemProduct = 384;            // an item's sums so far, a tile's product
-constexpr int kPShift = 14;  // probabilities, up to 1, carry this power of two at most
+constexpr int kPShift = 14;  // a tile's probabilities with their values' powers are brought to 2^14 at most
 
 constexpr int kMaxItems = 32;  // of a CTA: a lane of every warp finds one
-constexpr int kTailBytes = 8448;
+constexpr int kTailBytes = 10240;
 template <int HD>
 struct TcSmem {
   static constexpr int kv_bytes = kTcPos * HD * 2;  // hi or lo of K or V
@@ -420,7 +424,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 
 // The power k for a largest magnitude (its bits): magnitudes times 2^k below 2^15. At most 100 (zeros, and maxima below
-// 2^-86, which keep fewer bits), so that a scale times 2^-k is a normal number.
+// 2^-86; those below 2^-97 keep fewer than 22 bits), so that a scale times 2^-k is a normal number.
 __device__ __forceinline__ int shift_for(unsigned max_bits) {
   const int e = (int)(max_bits >> 23) - 127;
   return min(14 - e, 100);
@@ -474,8 +478,8 @@ struct TcTail {
   uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2], added, qfull;
   uint32_t tmem;
   int abort_flag;
-  float kscale[4][kConvWarps];  // 2^-k of eight keys, a ring of tiles
-  int vshift[4][kConvWarps];    // k of eight values
+  // Of each key 2^-k, of each value 2^-k and -k: a ring of tiles.
+  __align__(16) float kscale[4][kTcPos], vscale[4][kTcPos], vlog[4][kTcPos];
   // A bit for each of eight positions whose keys or values hold a NaN or an infinity.
   __align__(8) uint8_t wrong[4][kConvWarps];
   int qshift[2][kTcVecs];  // of this item and the next
@@ -515,7 +519,6 @@ struct Rows8 {
   static constexpr int kSteps = HD / 16;    // float4 a lane: 8 or 4
   static constexpr int kAt = 128 / HD;      // rows a step
   float4 x[kSteps];
-  float top;
 
   // Starts the copy of rows [row0, row0 + 8) of cache rows of hd floats; rows from `end` on and columns from hd on are
   // zeros.
@@ -539,51 +542,51 @@ struct Rows8 {
 #pragma unroll
     for (int i = 0; i < kSteps; i++)
       x[i] = slot[32 * i + lane];
-    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < kSteps; i++)
-      t[i & 3] = abs_max(t[i & 3], x[i]);
-    top = abs_max3(abs_max3(t[0], t[1], t[2]), t[3], 0.0f);
-    // The values are here before the slot's next copy starts.
-    asm volatile("" : "+f"(top)::"memory");
+    for (int i = 0; i < kSteps; i++)  // the values are here before the slot's next copy starts
+      asm volatile("" : "+f"(x[i].x), "+f"(x[i].y), "+f"(x[i].z), "+f"(x[i].w)::"memory");
   }
-  // Splits the rows and stores them as rows row .. row + 7 of the operand pair (64 rows of 128 swizzled bytes to 64
-  // columns); returns their power of two. Rows with a NaN or an infinity are stored as zeros and named in `wrong`: the
-  // queries that do not see them are not to notice.
+  // Splits the rows, with a power of two for each (2^k with k as shift_for gives it), and stores them as rows row .. row + 7
+  // of the operand pair (64 rows of 128 swizzled bytes to 64 columns); returns the bits of 2^-k of row lane % 8. Rows with
+  // a NaN or an infinity are stored as zeros and named in `wrong`: the queries that do not see them are not to notice.
   __device__ __forceinline__ int store(uint8_t *hi_at, uint8_t *lo_at, int row, int lane, unsigned *wrong) {
-    unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-    *wrong = 0;
-    if (bits >= 0x7f800000u) {
-      top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kSteps; i++) {
-        const unsigned lanes = __ballot_sync(0xffffffffu, !(abs_max(0.0f, x[i]) < INFINITY));
-#pragma unroll
-        for (int r = 0; r < kAt; r++)
-          if (lanes >> (32 / kAt * r) & (0xffffffffu >> (32 - 32 / kAt))) {
-            *wrong |= 1u << (i * kAt + r);
-            if (lane * 4 / HD == r)
-              x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          }
-        top = abs_max(top, x[i]);
-      }
-      bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-    }
-    const int k = shift_for(bits);
-    const uint64_t f = f2_pack(pow2(k), pow2(k));
     const int col = lane * 4 % HD, r = lane * 4 / HD;
     const uint32_t base = (col >> 6) * (kTcPos * 128) + row * 128 + (col & 7) * 2;
+    auto place = [&](int i) {
+      const int rr = r + i * kAt;
+      return base + rr * 128 + ((((col & 63) >> 3) ^ (rr & 7)) << 4);
+    };
+    unsigned own = 0;
+    *wrong = 0;
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
-      const int rr = r + i * kAt;
-      const uint32_t at = base + rr * 128 + ((((col & 63) >> 3) ^ (rr & 7)) << 4);
+      const unsigned top = __float_as_uint(abs_max(0.0f, x[i]));
+      unsigned mine = 0;
+#pragma unroll
+      for (int a = 0; a < kAt; a++) {
+        const unsigned bits = __reduce_max_sync(0xffffffffu, kAt == 1 || r == a ? top : 0u);
+        *wrong |= (bits >= 0x7f800000u ? 1u : 0u) << (i * kAt + a);
+        own = (lane & 7) == i * kAt + a ? bits : own;
+        mine = kAt == 1 || r == a ? bits : mine;
+      }
+      const unsigned power = min((268u << 23) - (mine & 0x7f800000u), 227u << 23);
+      const uint64_t f = f2_pack_bits(power, power);
       uint2 hi, lo;
       split2(f2_mul(f2_pack(x[i].x, x[i].y), f), hi.x, lo.x);
       split2(f2_mul(f2_pack(x[i].z, x[i].w), f), hi.y, lo.y);
-      *reinterpret_cast<uint2 *>(hi_at + at) = hi;
-      *reinterpret_cast<uint2 *>(lo_at + at) = lo;
+      *reinterpret_cast<uint2 *>(hi_at + place(i)) = hi;
+      *reinterpret_cast<uint2 *>(lo_at + place(i)) = lo;
     }
-    return k;
+    if (*wrong) {
+#pragma unroll
+      for (int i = 0; i < kSteps; i++)
+        if (*wrong >> (r + i * kAt) & 1) {
+          *reinterpret_cast<uint2 *>(hi_at + place(i)) = make_uint2(0, 0);
+          *reinterpret_cast<uint2 *>(lo_at + place(i)) = make_uint2(0, 0);
+        }
+      own = *wrong >> (lane & 7) & 1 ? 0 : own;
+    }
+    return max((int)(own & 0x7f800000u) - (14 << 23), 27 << 23);
   }
 };
 
@@ -661,9 +664,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
 
   if (warp > kSoftWarps) {
     // ---- converters ----
-    // Registers hold tile j, the slots tile j + 1 as it comes. Every copy is a group of its own, empty past the last.
-    // The tiles of all items are one sequence; `ahead` is the tile that is fetched next.
-    Rows8<HD> kx, vx;
+    // The slots hold tile j; once its rows are in registers, the copies of tile j + 1 start. Every copy is a group of its
+    // own, empty past the last. The tiles of all items are one sequence; `ahead` is the item of the tile fetched next.
     const float *ck = t->items[0].k, *cv = t->items[0].v;
     int ahead = 0, at = t->items[0].p0 + 8 * cw, end = t->items[0].p1;
     auto advance = [&]() {
@@ -673,7 +675,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
         ck = it.k, cv = it.v, at = it.p0 + 8 * cw, end = it.p1;
       }
     };
-    auto next = [&](Rows8<HD> &x, float4 *slot, const float *cache) {
+    Rows8<HD> x;
+    auto next = [&](float4 *slot, const float *cache) {
       copy_wait1();
       x.take(slot, lane);
       if (ahead < items)
@@ -683,32 +686,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
     int tiles = 0;
     for (int n = 0; n < items; n++)
       tiles += tiles_of(t->items[n]);
-    advance();
-    next(kx, kslot, ck);
-    next(vx, vslot, cv);
     for (int j = 0; j < tiles; j++) {
       advance();
       const int s = j & 1, use = j >> 1;
       uint8_t *stage = smem + s * L::stage;
+      next(kslot, ck);
       tc_wait(&t->kempty[s], (use & 1) ^ 1, abort_flag);
       unsigned wrong, wrong_v;
-      const int ks = kx.store(stage, stage + L::kv_bytes, 8 * cw, lane, &wrong);
-      if (lane == 0)
-        t->kscale[j & 3][cw] = pow2(-ks);
+      const int ks = x.store(stage, stage + L::kv_bytes, 8 * cw, lane, &wrong);
+      if (lane < 8)
+        t->kscale[j & 3][8 * cw + lane] = __int_as_float(ks);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&t->kfull[s]);
-      next(kx, kslot, ck);
+      next(vslot, cv);
       tc_wait(&t->vempty[s], (use & 1) ^ 1, abort_flag);
-      const int vs = vx.store(stage + 2 * L::kv_bytes, stage + 3 * L::kv_bytes, 8 * cw, lane, &wrong_v);
+      const int vs = x.store(stage + 2 * L::kv_bytes, stage + 3 * L::kv_bytes, 8 * cw, lane, &wrong_v);
+      if (lane < 8)
+        t->vscale[j & 3][8 * cw + lane] = __int_as_float(vs), t->vlog[j & 3][8 * cw + lane] = (float)((vs >> 23) - 127);
       if (lane == 0)
-        t->vshift[j & 3][cw] = vs, t->wrong[j & 3][cw] = (uint8_t)(wrong | wrong_v);
+        t->wrong[j & 3][cw] = (uint8_t)(wrong | wrong_v);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0)
         mbar_arrive(&t->vfull[s]);
-      next(vx, vslot, cv);
     }
   } else if (warp == kSoftWarps) {
     // ---- MMA issue. The scores of tile j + 1 go out before the sums of tile j, so that they run under its softmax, or
@@ -902,6 +904,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
       const int limit = have ? limit_of(a, it, it.first + vec_i) : it.p0;
       const int lowest = __reduce_min_sync(0xffffffffu, have ? limit : 0x7fffffff);
       const float scale = rsqrtf((float)hd) * kLog2e * pow2(-qshift);
+      const uint64_t scale2 = f2_pack(scale, scale);
       float m = -INFINITY, l = 0.0f;
       for (int j = j0 + ((j0 ^ g) & 1); j < j1; j += 2) {
         const int use = j >> 1;
@@ -915,74 +918,118 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
         if (busy) {
           const int p0 = it.p0 + (j - j0) * kTcPos;
           const bool masked = p0 + kTcPos > lowest;
-          const float *kscale = t->kscale[j & 3];
-          const int *vshift = t->vshift[j & 3];
-          auto factor = [&](int c8) {  // never 0: a masked score's -infinity has to stay one
-            return fmaxf(scale * kscale[c8], FLT_MIN);
-          };
-          // Two passes over the scores in TMEM, 32 at a time: their maximum, then the probabilities.
-          float top = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < 64; c += 32) {
-            uint32_t r[32];
-            tmem_ld32(ts + c, r);
+          const float *kscale = t->kscale[j & 3], *vscale = t->vscale[j & 3], *vlog = t->vlog[j & 3];
+          // 32 scores from column c on, without the row's scale where `plain`, else in units of log 2 and -infinity where
+          // they are not seen.
+          auto scores = [&](auto plain, int c, uint64_t (&y)[16]) {
+            tmem_ld32_pairs(ts + c, y);
             tmem_wait_ld();
-            if (masked)
 #pragma unroll
-              for (int e = 0; e < 32; e++)
-                r[e] = p0 + c + e < limit ? r[e] : 0xff800000u;
-#pragma unroll
-            for (int e8 = 0; e8 < 32; e8 += 8) {
-              float x[8];
-#pragma unroll
-              for (int e = 0; e < 8; e++)
-                x[e] = __uint_as_float(r[e8 + e]);
-              top = fmaxf(top, max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7])) *
-                                   factor((c + e8) >> 3));
+            for (int e = 0; e < 16; e += 2) {
+              const float4 f = *reinterpret_cast<const float4 *>(kscale + c + 2 * e);
+              uint64_t f0 = f2_pack(f.x, f.y), f1 = f2_pack(f.z, f.w);
+              if (!decltype(plain)::value)
+                f0 = f2_mul(f0, scale2), f1 = f2_mul(f1, scale2);
+              y[e] = f2_mul(y[e], f0), y[e + 1] = f2_mul(y[e + 1], f1);
             }
-          }
-          int vmin = vshift[0];
+            if (!decltype(plain)::value && masked)
 #pragma unroll
-          for (int w = 1; w < kConvWarps; w++)
-            vmin = min(vmin, vshift[w]);
-          const float m_new = fmaxf(m, ceilf(top));
+              for (int e = 0; e < 16; e++) {
+                float y0, y1;
+                f2_unpack(y[e], y0, y1);
+                y[e] = f2_pack(p0 + c + 2 * e < limit ? y0 : -INFINITY, p0 + c + 2 * e + 1 < limit ? y1 : -INFINITY);
+              }
+          };
+          // Their maximum, and the maximum of score + log2 of the value's power, scores taken from `from` on.
+          auto maxima = [&](float from, float &top, float &high) {
+            top = high = -INFINITY;
+            const uint64_t from2 = f2_pack(-from, -from);
+#pragma unroll 1
+            for (int c = 0; c < 64; c += 32) {
+              uint64_t y[16];
+              scores(std::false_type(), c, y);
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                const float4 v = *reinterpret_cast<const float4 *>(vlog + c + 2 * e);
+                float y0, y1, y2, y3, z0, z1, z2, z3;
+                y[e] = f2_add(y[e], from2), y[e + 1] = f2_add(y[e + 1], from2);
+                f2_unpack(y[e], y0, y1);
+                f2_unpack(y[e + 1], y2, y3);
+                f2_unpack(f2_add(y[e], f2_pack(v.x, v.y)), z0, z1);
+                f2_unpack(f2_add(y[e + 1], f2_pack(v.z, v.w)), z2, z3);
+                top = max3(max3(top, y0, y1), y2, y3);
+                high = max3(max3(high, z0, z1), z2, z3);
+              }
+            }
+          };
+          // The plain case: every row of the warp sees the whole tile, the values' powers lie within 2^10 of one another
+          // (so that their largest will do for the row's own), no scale times a score overflows and no score is beyond
+          // 2^15 (where powers added to it are rounded away). All tiles the general way: 222 us instead of 213 at 256 rows
+          // behind 8192 positions.
+          const int v0 = (int)vlog[lane], v1 = (int)vlog[lane + 32], vmax = __reduce_max_sync(0xffffffffu, max(v0, v1));
+          bool plain = !masked && vmax - __reduce_min_sync(0xffffffffu, min(v0, v1)) <= 10 &&
+                       __all_sync(0xffffffffu, fmaxf(kscale[lane], kscale[lane + 32]) < 0x1p80f);
+          float top = -INFINITY, high = -INFINITY;
+          if (plain) {
+#pragma unroll 1
+            for (int c = 0; c < 64; c += 32) {
+              uint64_t y[16];
+              scores(std::true_type(), c, y);
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                float y0, y1, y2, y3;
+                f2_unpack(y[e], y0, y1);
+                f2_unpack(y[e + 1], y2, y3);
+                top = max3(max3(top, y0, y1), y2, y3);
+              }
+            }
+            top *= scale;
+            high = top + (float)vmax;
+            plain = __all_sync(0xffffffffu, fabsf(top) <= 0x1p15f);
+          }
+          if (!plain)
+            maxima(0.0f, top, high);
+          const float m_new = fmaxf(m, ceilf(top)), base = m_new == -INFINITY ? 0.0f : m_new;
           l *= m == -INFINITY ? 0.0f : ex2(m - m_new);
           m = m_new;
-          const float base = m == -INFINITY ? 0.0f : m;
-          own = Power{m, (float)(-kPShift - vmin)};
+          if (!plain && __any_sync(0xffffffffu, top > 0x1p15f || (top < -0x1p15f && top > -INFINITY)))
+            maxima(base, top, high);  // the differences first
+          else
+            high -= base;
+          const float rest = fmaxf(ceilf(high) - (float)kPShift, -120.0f);
+          own = Power{m, rest};
+          // Probabilities times 2^-rest and their values' powers, and their sum.
+          auto probabilities = [&](auto plain) {
+            const float raise = pow2(-(int)rest), from = decltype(plain)::value ? -base - rest : -base;
+            const uint64_t from2 = f2_pack(from, from), raise2 = f2_pack(raise, raise);
 #pragma unroll 1
-          for (int c = 0; c < 64; c += 32) {
-            uint32_t r[32], hi[16], lo[16];
-            tmem_ld32(ts + c, r);
-            tmem_wait_ld();
-            if (masked)
+            for (int c = 0; c < 64; c += 32) {
+              uint64_t y[16], sum2 = 0;
+              uint32_t hi[16], lo[16];
+              scores(plain, c, y);
 #pragma unroll
-              for (int e = 0; e < 32; e++)
-                r[e] = p0 + c + e < limit ? r[e] : 0xff800000u;
-#pragma unroll
-            for (int e8 = 0; e8 < 32; e8 += 8) {
-              // 2^(score - m) times 2^grow, the values' power in the exponent: base and grow are whole numbers. Values
-              // 2^-60 of the largest seen (zeros, mostly) count as that at most, which O does not hold.
-              const float f = factor((c + e8) >> 3);
-              const int grow = max(kPShift - vshift[(c + e8) >> 3] + vmin, -60);
-              const float from = (float)grow - base;
-              const uint64_t f2 = f2_pack(f, f), from2 = f2_pack(from, from);
-              uint64_t sum2 = 0;
-#pragma unroll
-              for (int e = e8; e < e8 + 8; e += 2) {
-                float x, y;
-                f2_unpack(f2_fma(f2_pack_bits(r[e], r[e + 1]), f2, from2), x, y);
-                const uint64_t p = f2_pack(ex2(x), ex2(y));
+              for (int e = 0; e < 16; e++) {
+                const float2 v = *reinterpret_cast<const float2 *>(vscale + c + 2 * e);
+                float x0, x1;
+                f2_unpack(decltype(plain)::value ? f2_fma(y[e], scale2, from2) : f2_add(y[e], from2), x0, x1);
+                uint64_t p = f2_pack(ex2(x0), ex2(x1));
                 sum2 = f2_add(sum2, p);
-                split2(p, hi[e / 2], lo[e / 2]);
+                p = f2_mul(p, f2_pack(v.x, v.y));
+                if (!decltype(plain)::value)
+                  p = f2_mul(p, raise2);
+                split2(p, hi[e], lo[e]);
               }
               float s0, s1;
               f2_unpack(sum2, s0, s1);
-              l = fmaf(s0 + s1, pow2(-grow), l);
+              l = fmaf(s0 + s1, decltype(plain)::value ? pow2((int)rest) : 1.0f, l);
+              tmem_st16(ts + c, hi);
+              tmem_st16(ts + c + 16, lo);
             }
-            tmem_st16(ts + c, hi);
-            tmem_st16(ts + c + 16, lo);
-          }
+          };
+          if (plain)
+            probabilities(std::true_type());
+          else
+            probabilities(std::false_type());
           tmem_wait_st();
           // A vector that sees a position which is not finite has no result.
           const unsigned long long wrong = *reinterpret_cast<const unsigned long long *>(t->wrong[j & 3]);
@@ -1007,18 +1054,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) shared_tc_kernel(const SharedAr
             const float keep = pow2_ratio(before, after), f = pow2_ratio(own, after);
             const uint64_t keep2 = f2_pack(keep, keep), f2 = f2_pack(f, f);
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 16) {
-              uint32_t o[16], p[16];
-              tmem_ld16(quadrant + kTmemSum + c, o);
-              tmem_ld16(quadrant + kTmemProduct + c, p);
+            for (int c = 0; c < HD; c += 32) {
+              uint64_t o[16], p[16];
+              tmem_ld32_pairs(quadrant + kTmemSum + c, o);
+              tmem_ld32_pairs(quadrant + kTmemProduct + c, p);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                float y0, y1;
-                f2_unpack(f2_fma(f2_pack_bits(p[e], p[e + 1]), f2, f2_mul(f2_pack_bits(o[e], o[e + 1]), keep2)), y0, y1);
-                o[e] = __float_as_uint(y0), o[e + 1] = __float_as_uint(y1);
+              for (int h = 0; h < 2; h++) {
+                uint32_t y[16];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                  float y0, y1;
+                  f2_unpack(f2_fma(p[8 * h + e], f2, f2_mul(o[8 * h + e], keep2)), y0, y1);
+                  y[2 * e] = __float_as_uint(y0), y[2 * e + 1] = __float_as_uint(y1);
+                }
+                tmem_st16(quadrant + kTmemSum + c + 16 * h, y);
               }
-              tmem_st16(quadrant + kTmemSum + c, o);
             }
             tmem_wait_st();
             t->sum[vec_i] = after;

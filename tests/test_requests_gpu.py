@@ -295,6 +295,95 @@ def test_shared_attention_of_one_dominant_position(kc, case, place):
     assert norm_error(got[some], want) <= PRODUCTS
 
 
+@pytest.mark.parametrize("hd", [128, 64, 96, 32, 256, 33])
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e10, 1e20, 3.4e38])
+def test_shared_attention_unseen_values_change_nothing(kc, hd, size):
+    """Finite keys and values of any size where a row does not see them (behind its own position, behind the prefix, behind
+    the request's last row) against zeros in their place: the same bits."""
+    heads, kv, B, R, prefix, S = 8, 2, 3, 4, 130, 90
+    starts, counts = [2, 61, 70], [4, 4, 2]
+    g = generator(17)
+    q, pk, pv = normal(g, B, R, heads * hd), normal(g, kv, prefix + 9, hd), normal(g, kv, prefix + 9, hd)
+    k, v = normal(g, B, kv, S, hd), normal(g, B, kv, S, hd)
+    for row in range(3):
+        outs = []
+        for factor in (0.0, size):
+            a = [t.clone() for t in (pk, pv, k, v)]
+            for t, sign in zip(a[:2], (1, -1)):
+                t[:, prefix:] = t[:, prefix:].sign() * sign * factor
+            for t, sign in zip(a[2:], (-1, 1)):
+                for b in range(B):
+                    t[b, :, starts[b] + row + 1:] = t[b, :, starts[b] + row + 1:].sign() * sign * factor
+            outs.append(run_attention(kc, q, a[0], a[1], prefix, a[2], a[3], starts, counts, heads, kv, hd))
+        assert torch.equal(outs[0][:, :row + 1], outs[1][:, :row + 1])
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("size", [1e2, 1e4, 1e6, 1e8, 1e12])
+def test_shared_attention_large_values_of_no_weight(kc, hd, size):
+    """Positions with next to no weight (e^-60 and less) whose values are larger than the others' by `size`, and one whose
+    key is: they cost the others nothing. Scores of the positions that count are below 6, so that a weight is off by
+    2^-24 (6 sqrt(head_dim) + 8) of itself."""
+    heads, kv, B, R, prefix, S = 8, 2, 2, 2, 1000, 70
+    g = generator(18)
+    q = 0.7 * normal(g, B, R, heads * hd)
+    q.view(B, R, heads, hd)[..., 0] = 4.0
+    pk, pv = normal(g, kv, prefix, hd), normal(g, kv, prefix, hd)
+    k, v = normal(g, B, kv, S, hd), normal(g, B, kv, S, hd)
+    pk[..., 0], k[..., 0] = 0.0, 0.0
+    for t in (5, 333, 340, 999):
+        pk[:, t, 0], pv[:, t] = -20 * hd ** 0.5, size * pv[:, t]
+    k[0, :, 3, 0], v[0, :, 3] = -20 * hd ** 0.5, size * v[0, :, 3]
+    pk[:, 777] *= 0.0
+    pk[:, 777, 0] = -20 * hd ** 0.5 * size
+    got = run_attention(kc, q, pk, pv, prefix, k, v, [S - R, 40], [R] * B, heads, kv, hd)
+    want, _ = attention_64(q, pk, pv, prefix, k, v, [S - R, 40], [R] * B, heads, kv, hd, got)
+    assert norm_error(got, want) <= U * (6 * hd ** 0.5 + 8)
+
+
+@pytest.mark.parametrize("hd", [128, 64, 32])
+@pytest.mark.parametrize("size", [1e-28, 1e-15, 1e15, 1e26])
+def test_shared_attention_keys_and_values_of_any_power(kc, hd, size):
+    """Each position's key of a power of its own between 1 / 1000 and 1000 times `size`, queries the other way; values of
+    powers 2^-40 to 2^40, those of the largest weighing most."""
+    heads, kv, B, R, prefix, S = 8, 2, 3, 2, 500, 130
+    g = generator(20)
+    power = lambda *shape: 2.0 ** torch.randint(-10, 11, shape, device="cuda", generator=g)  # noqa: E731
+    q = normal(g, B, R, heads * hd) / (1000 * size)
+    pk, k = normal(g, kv, prefix, hd) * power(kv, prefix, 1) * size, normal(g, B, kv, S, hd) * power(B, kv, S, 1) * size
+    wide = lambda *shape: 2.0 ** torch.randint(-40, 41, shape, device="cuda", generator=g)  # noqa: E731
+    pv, v = normal(g, kv, prefix, hd) * wide(kv, prefix, 1), normal(g, B, kv, S, hd) * wide(B, kv, S, 1)
+    starts = [S - R, 64, 3]
+    got = run_attention(kc, q, pk, pv, prefix, k, v, starts, [R] * B, heads, kv, hd)
+    want, top = attention_64(q, pk, pv, prefix, k, v, starts, [R] * B, heads, kv, hd, got)
+    assert norm_error(got, want) <= U * (top * hd ** 0.5 + 8)
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("size", [1e2, 1e4, 1e6, 1e9, 1e15])
+def test_shared_attention_large_scores(kc, hd, size):
+    """Scores so far apart that one position has all the weight, values of any power."""
+    heads, kv, B, R, prefix, S = 8, 2, 3, 2, 700, 66
+    g = generator(19)
+    q = size * normal(g, B, R, heads * hd).sign()
+    signs = normal(g, kv, prefix, hd).sign()
+    pk, pv = signs * 1e-4, normal(g, kv, prefix, hd) * 2.0 ** torch.randint(-30, 31, (kv, prefix, 1), device="cuda", generator=g)
+    k, v = 1e-4 * normal(g, B, kv, S, hd).sign(), normal(g, B, kv, S, hd)
+    best = torch.randint(0, prefix, (B, R, heads), device="cuda", generator=g)
+    for b in range(B):
+        for r in range(R):
+            for h in range(heads):
+                pk[h // (heads // kv), best[b, r, h]] = 1000 * q[b, r, h * hd:(h + 1) * hd].sign()
+    got = run_attention(kc, q, pk, pv, prefix, k, v, [S - R] * B, [R] * B, heads, kv, hd)
+    want, _ = attention_64(q, pk, pv, prefix, k, v, [S - R] * B, [R] * B, heads, kv, hd, got)
+    got, want = got.view(B, R, heads, hd), want.view(B, R, heads, hd)
+    # Where the two largest scores are nearer than head_dim roundings, the roundings decide.
+    top = torch.einsum("brkgd,kpd->brkgp", q.double().view(B, R, kv, heads // kv, hd), pk.double()).flatten(2, 3).topk(2).values
+    clear = top[..., 0] - top[..., 1] > 8 * U * hd * top[..., 0]
+    assert clear.sum() > clear.numel() / 2
+    assert ((got.double() - want).abs() <= PRODUCTS * want.abs().amax(-1, keepdim=True))[clear].all()
+
+
 def test_shared_attention_is_the_engines_attention(kc):
     """One request whose positions are cut into a prefix and its own: k_attention_batch_kv over the whole cache."""
     heads, kv, hd, R, prefix, S = 32, 8, 128, 4, 300, 80

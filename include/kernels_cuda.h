@@ -317,7 +317,8 @@ void k_attention_shared_rows(float *out, int8_t *oq, float *os, const float *q, 
  * entries: a [rank][n] and b [d][rank] row-major, of the type `type`. base (stride ldb) may be out itself, as after the
  * product of k_gemm_q8 or k_matmul_q8, or NULL for zeros; out must not overlap x. Ranks 0 .. max_rank <= 256; an index
  * outside [-1, count), a rank outside [0, max_rank] or a missing matrix raises an error (kc_status) and the row gets
- * its base. Sums are fp32 in a fixed order. 16-byte aligned matrices with n and rank multiples of 8 are read in 16-byte
+ * its base. Matrices are finite; activations may be any numbers: infinities and NaN, or vectors that overflow, give the
+ * infinities and NaN of the formula in their own row. Sums are fp32 in a fixed order. 16-byte aligned matrices with n and rank multiples of 8 are read in 16-byte
  * units, others one value at a time. */
 typedef enum { K_F32, K_BF16, K_F16 } KernelType;
 typedef struct {

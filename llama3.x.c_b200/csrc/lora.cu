@@ -315,6 +315,7 @@ struct LoraTile {
   int rows[kTileRows];
   int warp_sums[kWarps];
   int adapter, part, n;  // the cluster's tile: its adapter (`count`: rows without one) and its rows in order
+  bool direct[kTileRows], any_direct;  // rows whose vector is not finite
 };
 
 // False: no such tile. bins: kMaxBins words. A thread takes a run of neighbouring rows, whose adapters it keeps as long
@@ -452,13 +453,16 @@ __device__ __forceinline__ bool tile_wait(uint64_t *bar, unsigned parity, volati
   return __all_sync(0xffffffffu, ok);
 }
 
-// Two values as N packed bf16 parts.
+// Two values as N packed bf16 parts. The first part of a finite value is finite (the largest ones would round up to an
+// infinity); those of an infinity or NaN have a NaN among them where N is 3, so that none passes unseen.
 template <int N>
 __device__ __forceinline__ void parts2(float x, float y, uint32_t (&p)[N]) {
 #pragma unroll
   for (int i = 0; i < N; i++) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    p[i] = *reinterpret_cast<const uint32_t *>(&h);
+    if (i == 0)
+      asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(p[0]) : "f"(y), "f"(x));
+    else
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[i]) : "f"(y), "f"(x));
     if (i + 1 < N) {
       x -= __uint_as_float(p[i] << 16);
       y -= __uint_as_float(p[i] & 0xffff0000u);
@@ -552,6 +556,34 @@ __device__ __forceinline__ void write4(float *p, float4 v, int left, bool wide) 
     p[3] = v.w;
 }
 
+// The whole CTA: a row's product over [n0, n1) of x by fp32 FMAs, added to its outputs [d0, d1). Where a row's vector is
+// not finite its bf16 parts say nothing, and the formula decides which outputs are infinities, numbers or NaN. h: 128
+// floats of shared memory.
+template <typename W>
+__device__ __forceinline__ void row_directly(const LoraArgs &a, const W *A, const W *B, int rank, float scale, int row, int n0,
+                                             int n1, int d0, int d1, float *h) {
+  const float *x = a.x + (long long)row * a.ldx;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();
+  for (int k = warp; k < rank; k += kWarps) {
+    float s = 0.0f;
+    for (int i = n0 + lane; i < n1; i += 32)
+      s = fmaf(to_float(A[(size_t)k * a.n + i]), x[i], s);
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0)
+      h[k] = s * scale;
+  }
+  __syncthreads();
+  for (int i = d0 + threadIdx.x; i < d1; i += kThreads) {
+    float s = 0.0f;
+    for (int k = 0; k < rank; k++)
+      s = fmaf(to_float(B[(size_t)i * rank + k]), h[k], s);
+    a.out[(long long)row * a.ldo + i] += s;
+  }
+}
+
 // 2048 rows of 4 adapters of rank 64 bf16, 4096 to 4096: 44 us, 2.4 TB/s of the rows' own bytes, the tensor pipe 8 % and
 // the issue slots 23 % busy: the phases (rows, first product, the cluster's sum, second product) follow one another, two
 // CTAs an SM.
@@ -573,8 +605,11 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     mbar_init(&t.bar[0], 1);
     mbar_init(&t.bar[1], 1);
     t.abort_flag = 0;
+    t.any_direct = false;
     fence_mbar_init();
   }
+  for (int i = threadIdx.x; i < kTileRows; i += kThreads)
+    t.direct[i] = false;
   pdl_wait();
   pdl_launch_dependents();
   if (!find_tile(a, &t, reinterpret_cast<int *>(smem), id / parts))
@@ -767,6 +802,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     }
   cluster.sync();
   const int h_bytes = kTileRows * rank_high * 2;
+  unsigned direct = 0;  // a bit for each of this warp's rows that has a number which is not finite
   for (int k = 2 * lane; k < rank16; k += 64) {
 #pragma unroll
     for (int n = 0; n < kTileRows / kWarps; n++) {
@@ -776,6 +812,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
       float2 v = make_float2(0.0f, 0.0f);
       if (i < rows)
         v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&own_h[i / ctas * hs + k], i % ctas));
+      if (!(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY))
+        direct |= 1u << n;
       uint32_t p[3];
       parts2(v.x, v.y, p);
       uint8_t *dst = operand + operand_at(kTileRows, i, k);
@@ -785,6 +823,18 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     }
   }
   auto fetched = cluster.barrier_arrive();  // a CTA may leave once everybody has fetched everything
+  if (__any_sync(0xffffffffu, direct != 0)) {  // those rows get their base for now
+    direct = __reduce_or_sync(0xffffffffu, direct);
+    for (int n = 0; n < kTileRows / kWarps; n++) {
+      if (lane == 0)
+        t.direct[warp + kWarps * n] = direct >> n & 1;
+      if (direct >> n & 1)
+        for (int k = 2 * lane; k < rank16; k += 64)
+          for (int j = 0; j < 3; j++)
+            *reinterpret_cast<uint32_t *>(operand + j * h_bytes + operand_at(kTileRows, warp + kWarps * n, k)) = 0;
+    }
+    t.any_direct = true;
+  }
 
   // B h over this CTA's slice of d, 128 outputs at a time.
   const bool b_wide = aligned16(B) && w.rank % 8 == 0;
@@ -890,6 +940,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
+  if (t.any_direct)
+    for (int i = 0; i < rows; i++)
+      if (t.direct[i])
+        row_directly(a, A, B, w.rank, w.scale, t.rows[i], from_n, to_n, d0, d1, reinterpret_cast<float *>(smem));
   cluster.barrier_wait(std::move(fetched));
 }
 

@@ -571,6 +571,38 @@ def test_lora_nonfinite_rows_stay_their_own(kc, rows):
     assert not out[sick].isfinite().any() and out[~sick].isfinite().all()
 
 
+@pytest.mark.parametrize("rows", [4, 150, 4000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_lora_rows_of_any_numbers(kc, rows, dtype):
+    """Activations up to the largest finite ones, whose results are finite, and infinities, whose results are infinities or
+    NaN as the formula gives them, whichever kernel runs."""
+    n, d, ranks = (128, 64, [1, 8, 3]) if rows < 1000 else (2048, 512, [1, 8, 3])
+    a, b, scale, index, g = lora_inputs((rows, 3, ranks, n, d, dtype), "each", 3)
+    x, base = normal(g, rows, n), normal(g, rows, d)
+    for m in a:
+        m[:, 7] = m[:, 7].sign() * 2.0 ** -20
+        m[:, 8] = m[:, 8].sign() * 2.0 ** -24
+    huge = torch.finfo(torch.float32).max
+    for r in range(0, rows, 31):  # of each adapter in turn
+        x[r, 5] = float("inf")
+    for r in range(1, rows, 31):
+        x[r, 7] = huge
+    for r in range(2, rows, 31):
+        x[r, 7], x[r, 8] = -huge, 3.4e38
+    for r in range(3, rows, 31):
+        x[r, 5], x[r, 6] = float("inf"), float("-inf")
+    out = torch.empty(rows, d, device="cuda")
+    kc.k_lora_rows(out, d, base, d, x, n, index, kc.lora_table(a, b, scale), 3, kind(kc, dtype), 8, n, d, rows)
+    kc.status()
+    want, tol = lora_64(x, base, index, a, b, scale)
+    finite = want.isfinite()
+    assert finite[1::31].all() and not finite[0::31].any() and want[0::31].isinf().any()
+    assert ((out.double() - want).abs() <= tol)[finite].all()
+    assert torch.equal(out[~finite].isnan(), want[~finite].isnan())
+    inf = want.isinf()
+    assert torch.equal(out[inf].double(), want[inf])
+
+
 def test_lora_more_rows_than_a_launch_takes(kc):
     """Over 16384 rows: several launches, each with its own part of the index."""
     case = (20000, 3, [16, 8, 24], 256, 264, torch.bfloat16)

@@ -384,6 +384,26 @@ def test_shared_attention_large_scores(kc, hd, size):
     assert ((got.double() - want).abs() <= PRODUCTS * want.abs().amax(-1, keepdim=True))[clear].all()
 
 
+@pytest.mark.parametrize("case", LONG + [(128, 64, 4, 8192, 64), (256, 8, 2, 700, 60), (33, 8, 2, 700, 60)],
+                         ids=lambda c: "-".join(map(str, c)))
+def test_shared_attention_error(kc, case):
+    """The root mean square error of ordinary inputs: scores with a standard deviation of 1.5 are off by 2^-24 sqrt(head_dim)
+    of that at most (head_dim roundings, random ones), which moves the weights by as much of themselves; the products'
+    roundings join it."""
+    hd, batch, rows, prefix, room = case
+    heads, kv = (32, 2) if batch > 2 else (4, 2)
+    g = generator(hd + batch + 3)
+    q = 1.5 * normal(g, batch, rows, heads * hd)
+    pk, pv = normal(g, kv, prefix, hd), normal(g, kv, prefix, hd)
+    k, v = normal(g, batch, kv, room, hd), normal(g, batch, kv, room, hd)
+    starts = [(room - rows) * (b + 1) // batch for b in range(batch)]
+    got = run_attention(kc, q, pk, pv, prefix, k, v, starts, [rows] * batch, heads, kv, hd)
+    some = sorted({0, batch // 2, batch - 1})
+    want, _ = attention_64(q[some], pk, pv, prefix, k[some], v[some], [starts[b] for b in some], [rows] * len(some), heads,
+                           kv, hd, got[some])
+    assert norm_error(got[some], want) <= PRODUCTS + U * 1.5 * hd ** 0.5
+
+
 def test_shared_attention_is_the_engines_attention(kc):
     """One request whose positions are cut into a prefix and its own: k_attention_batch_kv over the whole cache."""
     heads, kv, hd, R, prefix, S = 32, 8, 128, 4, 300, 80
@@ -517,6 +537,38 @@ def test_lora(kc, case, order):
     kc.status()
     want, tol = lora_64(x, torch.zeros_like(base), index, a, b, scale)
     assert ((out.double() - want).abs() <= tol).all()
+
+
+def two_parts(x):
+    """To 16 bits, as two bfloat16 numbers hold it."""
+    high = x.bfloat16().double()
+    return high + (x.double() - high).bfloat16().double()
+
+
+@pytest.mark.parametrize("order", ["runs", "each"])
+@pytest.mark.parametrize("case", LORA, ids=lambda c: f"{c[0]}-{c[1]}-{max(c[2])}-{c[3]}-{c[4]}-{str(c[5])[6:]}")
+def test_lora_error(kc, case, order):
+    """The root mean square error of the products alone. The tensor cores cut a sum by half a step (0.36 * 2^-23 on average
+    over its mantissas) of what it has come to, 2/3 of its end on average over a random run: once for every 48 elements
+    of a CTA's eighth of n (16384 a launch at most), and in the second product for every 16 ranks and eight small terms.
+    Some dozen random roundings, 2^-24 sqrt(12 / 3), join it. Activations and vectors of 16 bits would not pass."""
+    rows, count, ranks, n, d, dtype = case
+    a, b, scale, index, g = lora_inputs(case, order, 2)
+    x = normal(g, rows, n)
+    out = torch.full((rows, d), -7.0, device="cuda")
+    kc.k_lora_rows(out, d, None, 0, x, n, index, kc.lora_table(a, b, scale), count, kind(kc, dtype), max(ranks), n, d, rows)
+    kc.status()
+    want, _ = lora_64(x, torch.zeros(rows, d, device="cuda"), index, a, b, scale)
+    cuts = min(n, 16384) / 8 / 48 + max(ranks) / 16 + 8
+    bound = cuts * 0.36 * 2 / 3 * 2.0 ** -23 + 2 * U
+    assert norm_error(out, want) <= bound
+    if 64 <= n <= 4096 and rows * d > 1000:
+        less = torch.zeros_like(want)
+        for i, (A, B) in enumerate(zip(a, b)):
+            at = (index == i).nonzero()[:, 0]
+            h = two_parts(two_parts(x[at]) @ A.double().T)
+            less[at] = scale[i] * (h @ B.double().T)
+        assert norm_error(less, want) > bound
 
 
 @pytest.mark.parametrize("rows", [5, 200, 3000])

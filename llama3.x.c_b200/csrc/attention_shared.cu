@@ -1210,9 +1210,11 @@ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 long long ceil_div64(long long a, long long b) { return (a + b - 1) / b; }
 
 bool shape_ok(int n_heads, int n_kv, int hd, int batch, int rows) {
+  constexpr long long most = 1 << 24;  // vectors; the product of two of the numbers does not wrap
   return n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && hd > 0 && hd <= kMaxHd && batch > 0 && rows > 0 &&
-         (long long)batch * rows * n_heads <= (1 << 24);
+         (long long)batch * rows <= most && (long long)batch * rows * n_heads <= most;
 }
+constexpr int kMaxPositions = 0x7fffffff - 1024;  // tiles are numbered past the last one
 
 // Floats of n (m, l) pairs, to a whole number of 16-byte units: the accumulators behind them stay aligned.
 size_t pairs_floats(size_t n) { return (2 * n + 3) & ~(size_t)3; }
@@ -1334,8 +1336,8 @@ void k_attention_shared_rows(float *out, int8_t *oq, float *os, const float *q, 
   const char *name = "k_attention_shared_rows";
   if (batch == 0 || rows == 0)
     return;
-  if (!shape_ok(n_heads, n_kv_heads, head_dim, batch, rows) || seq_len <= 0 || rows > seq_len || prefix < 0 ||
-      prefix > prefix_seq_len) {
+  if (!shape_ok(n_heads, n_kv_heads, head_dim, batch, rows) || seq_len <= 0 || rows > seq_len ||
+      seq_len > kMaxPositions || prefix < 0 || prefix > prefix_seq_len || prefix > kMaxPositions) {
     kc_fail("%s: invalid shape heads=%d/%d head_dim=%d batch=%d rows=%d seq_len=%d prefix=%d of %d", name, n_heads,
             n_kv_heads, head_dim, batch, rows, seq_len, prefix, prefix_seq_len);
     return;

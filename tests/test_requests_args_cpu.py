@@ -212,3 +212,21 @@ def test_python_mirror_refuses_memory_elsewhere(on_cpu):
     with pytest.raises(kc.KernelError, match="the attention work must be on the current CUDA device"):
         kc.k_attention_shared_rows(a, None, None, a, a, a, 4, 4, a, a, i, i, work, 1, 1, 4, 4, 1, 4, 0)
     assert not calls
+
+
+@pytest.mark.parametrize("bad", [dict(prefix_seq=2 ** 31 - 1, prefix=2 ** 31 - 1), dict(seq=2 ** 31 - 1),
+                                 dict(prefix_seq=2 ** 31 - 64, prefix=2 ** 31 - 64)])
+def test_shared_attention_positions_past_the_integers(lib, bad):
+    """Positions are numbered in tiles past the last one: lengths at the end of the integers would wrap."""
+    kc, L = lib
+    assert "k_attention_shared_rows: invalid shape" in shared(kc, L, made_up_work(kc, L), **bad)
+
+
+@pytest.mark.parametrize("heads,batch,rows", [(4, 2 ** 31 - 1, 2 ** 31 - 1), (8, 2 ** 30, 2 ** 31 - 1),
+                                              (2 ** 31 - 1, 2 ** 31 - 1, 4), (2 ** 16, 2 ** 24, 2 ** 24)])
+def test_shared_attention_products_of_sizes_that_wrap(lib, heads, batch, rows):
+    kc, L = lib
+    assert L.k_attention_shared_bytes(heads, 1, 64, batch, rows) == 0
+    w = kc.AttentionWork()
+    L.k_attention_shared_init(ctypes.byref(w), heads, 1, 64, batch, rows, A)
+    assert rejected(L) == "k_attention_shared_init: invalid shape"

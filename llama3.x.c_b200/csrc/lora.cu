@@ -28,6 +28,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRank = 256;
 constexpr int kCtas = 8;  // of a tile's cluster
 constexpr int kRowCtas = 4;  // an SM's CTAs of the row kernel
+constexpr int kMaxColumns = 0x7fffffff - 65536;  // slices and steps are numbered past the last one
 
 struct LoraArgs {
   float *out;
@@ -1049,8 +1050,8 @@ void k_lora_rows(float *out, size_t ldo, const float *base, size_t ldb, const fl
     kc_fail("%s: invalid weight type %d", name, type);
     return;
   }
-  if (rows < 0 || rows > (1 << 24) || n <= 0 || d <= 0 || count < 0 || max_rank <= 0 || max_rank > kMaxRank ||
-      ldx < (size_t)n || ldo < (size_t)d || (base && ldb < (size_t)d)) {
+  if (rows < 0 || rows > (1 << 24) || n <= 0 || n > kMaxColumns || d <= 0 || d > kMaxColumns || count < 0 ||
+      max_rank <= 0 || max_rank > kMaxRank || ldx < (size_t)n || ldo < (size_t)d || (base && ldb < (size_t)d)) {
     kc_fail("%s: invalid shape rows=%d n=%d d=%d count=%d max_rank=%d (at most %d)", name, rows, n, d, count, max_rank,
             kMaxRank);
     return;

@@ -230,3 +230,10 @@ def test_shared_attention_products_of_sizes_that_wrap(lib, heads, batch, rows):
     w = kc.AttentionWork()
     L.k_attention_shared_init(ctypes.byref(w), heads, 1, 64, batch, rows, A)
     assert rejected(L) == "k_attention_shared_init: invalid shape"
+
+
+@pytest.mark.parametrize("bad", [dict(n=2 ** 31 - 1, ldx=2 ** 31), dict(d=2 ** 31 - 1, ldo=2 ** 31, ldb=2 ** 31),
+                                 dict(n=2 ** 31 - 8192, ldx=2 ** 31)])
+def test_lora_columns_past_the_integers(lib, bad):
+    """Columns are numbered in slices and steps past the last one."""
+    assert "k_lora_rows: invalid shape" in lora(lib[1], **bad)

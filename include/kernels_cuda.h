@@ -291,15 +291,17 @@ void k_fill(float *x, size_t n, float value);
 
 /* ---- a batch of requests over one prompt (no counterpart in the reference, which serves one sequence) ------------ */
 /* Attention of `batch` requests that share a prefix. q and out are [batch][rows][n_heads * head_dim]; the prefix lies
- * in one head-major cache [n_kv_heads][prefix_seq_len][head_dim] (one layer of an engine's, say), positions
+ * in one head-major cache [n_kv_heads][prefix_seq_len][head_dim] (as k_rope_kv_store_rows fills one), positions
  * [0, prefix); each request's own positions in its cache of [batch][n_kv_heads][seq_len][head_dim]. Row r of request b
  * (its last token and its drafts, say) sees the prefix and own positions [0, starts[b] + r]: starts[b] positions were
  * stored before this step's rows. counts[b] (NULL: all) says how many of the rows request b uses, 0 .. rows; the other
  * rows of out are left as they were, and a request that uses none needs no starts[b]. starts and counts are device
  * memory, so a captured step replays as the requests grow. starts[b] outside [0, seq_len - counts[b]] or counts[b]
  * outside [0, rows] raises an error (kc_status) and leaves the request's rows as they were. What a row sees must be
- * finite, or that row has no result; what it does not see, finite or not, changes nothing in it. oq / os (may be NULL): out quantized for Wo as k_quantize does,
- * gs dividing head_dim. The prefix is read once for the whole batch. head_dim <= 256.
+ * finite, or that row has no result; what it does not see, finite or not, changes nothing in it. Products are fp32 ones
+ * up to 2^-22 of each (head_dim <= 128 in 16-byte units at 16-byte addresses: on the tensor cores) or 2^-24, sums fp32;
+ * vectors whose largest element is below 2^-97 keep fewer bits. oq / os (may be NULL): out quantized for Wo as k_quantize
+ * does, gs dividing head_dim. The prefix is read once for the whole batch. head_dim <= 256, up to 2^31 - 1025 positions.
  * `work` (k_attention_shared_init, released with k_attention_free): partial results for this n_heads and head_dim and
  * up to batch * rows rows (its `workers`; its max_chunks is 0, so that neither kind of work passes for the other), which
  * may split the positions differently, and so round differently, for works made for different sizes; `memory` as for
@@ -318,8 +320,10 @@ void k_attention_shared_rows(float *out, int8_t *oq, float *os, const float *q, 
  * product of k_gemm_q8 or k_matmul_q8, or NULL for zeros; out must not overlap x. Ranks 0 .. max_rank <= 256; an index
  * outside [-1, count), a rank outside [0, max_rank] or a missing matrix raises an error (kc_status) and the row gets
  * its base. Matrices are finite; activations may be any numbers: infinities and NaN, or vectors that overflow, give the
- * infinities and NaN of the formula in their own row. Sums are fp32 in a fixed order. 16-byte aligned matrices with n and rank multiples of 8 are read in 16-byte
- * units, others one value at a time. */
+ * infinities and NaN of the formula in their own row. Sums are fp32 in a fixed order. 16-byte aligned matrices with n and
+ * rank multiples of 8 are read in 16-byte units, others one value at a time. Many rows of one adapter are cheapest at
+ * ranks up to 128 with fewer than 2048 adapters in the table: only then do they share one read of it. n and d up to
+ * 2^31 - 65537. */
 typedef enum { K_F32, K_BF16, K_F16 } KernelType;
 typedef struct {
   const void *a, *b;
@@ -330,8 +334,8 @@ void k_lora_rows(float *out, size_t ldo, const float *base, size_t ldb, const fl
                  const LoraAdapter *adapters, int count, int type, int max_rank, int n, int d, int rows);
 
 /* Verification of drafted tokens (speculative sampling): request b drafted the tokens drafted[b][0 .. counts[b] - 1]
- * of drafted [batch][rows]; row j of target [batch][rows + 1] (logits, row stride ldt, as engine_forward_batch makes
- * them) is the target model's after j drafts, row j of draft [batch][rows] (stride ldd) the logits that draft j was
+ * of drafted [batch][rows]; row j of target [batch][rows + 1] (logits in device memory, row stride ldt) is the target
+ * model's after j drafts, row j of draft [batch][rows] (stride ldd) the logits that draft j was
  * drawn from, or draft is NULL when the drafts came from no distribution (a lookup in the prompt). p_j and q_j are
  * their softmax at temperature[b], 0 .. 1e30 (q_j one at the drafted token without logits). Draft j is accepted when all before
  * it are and u_j q_j(x_j) < p_j(x_j), with the given random numbers u = uniforms[b] of uniforms [batch][rows + 1], in

@@ -299,22 +299,25 @@ __global__ void __launch_bounds__(kGenericThreads) shared_generic_kernel(const S
 // ---- tensor-core kernel -------------------------------------------------------------------------------------------
 
 // head_dim <= 128 in whole 16-byte units. A CTA per SM takes its items one after another: up to 128 query vectors of a KV
-// head against a range of positions in tiles of 64, S = Q K^T and O += P V on tcgen05 with accumulators in TMEM. The
+// head against a range of positions in tiles of 64, S = Q K^T and P V on tcgen05 with accumulators in TMEM. The
 // tiles of all items run through the same stages: the next item's keys and values are under way, and its queries laid
-// out, before the last sums are done (a CTA per item took 215 us where this takes 199: 256 rows behind 8192 positions).
-// What bounds it: the conversion of keys and values, 2.7 thousand clocks a tile of 64 positions and 128 vectors, of which
-// the MMAs take 1.8. 256 rows of 32 heads of 128 behind 8192 positions: 186 us here and 12 in the join, 111 TFLOP/s of
-// fp32 products (333 of fp16), the tensor pipe 35 % busy, the shared-memory pipe 38 %, the issue slots 43 %; the rest is
-// the latency of eight converter warps, for which there are no more registers.
+// out, before the last sums are done (a CTA per item took 8 % longer at 256 rows behind 8192 positions).
+// What bounds it: two chains of dependent steps, 4.3 thousand clocks a tile of 64 positions and 128 vectors together. A
+// group of softmax warps takes 7 thousand for its tile of two (1.2 for the maximum, 2.2 for the probabilities, 1.2 until
+// the product is done, 1.3 to add it, 1.0 until the next scores), the converter warps 3.1 for a tile, the MMAs 1.8. 256
+// rows of 32 heads of 128 behind 8192 positions: 213 us with 12 in the join, 103 TFLOP/s of fp32 products (310 of fp16),
+// the tensor pipe 30 % busy, the shared-memory pipe 37 %, the issue slots 44 %; for more warps there are no registers.
 //
 // fp32 products on half-precision tensor cores: x = 2^-k (hi + lo) with hi and lo fp16, 22 bits of x, and
 // x y = 2^-(k + k') (hi hi' + hi lo' + lo hi') up to 2^-22 of the product (what is dropped, lo lo', is below the
-// rounding of lo). The power 2^k puts the largest magnitude of one query, key or value vector just below 2^15, so no
+// rounding of lo). The two bits less than fp32's cost less than the roundings of a chain of fp32 sums (0.9 to 1.0e-6 off
+// 64 bits at the sizes below, such chains 1.1 to 1.8e-6); a third part would double the MMAs, and its operands do not fit
+// into two stages. The power 2^k puts the largest magnitude of one query, key or value vector just below 2^15, so no
 // finite input overflows and an element 2^-17 of its vector's largest still keeps its 22 bits. k of a key goes into its
 // scores' scale, k of a value into its probabilities (exact powers of two both). No power is shared between positions: a
 // vector that a row does not see, or that has no weight in it, takes no bits of the others. For the same reason the
 // probabilities' own power, one to a row and tile, follows the largest product of a seen probability and its value's
-// power: what is added to a row's result is off by 2^-22 of itself and 2^-39 of the largest one.
+// power: what is added to a row's result is off by 2^-22 of itself, and by 2^-29 of the largest one of its tile at most.
 //
 // Warps: 0-3 the softmax of the even tiles and 4-7 that of the odd ones, a thread per query vector (TMEM lane), each
 // group with a reference and a sum of its own (joined at the end), so that a group has two tiles' time; 8 issues

@@ -585,8 +585,8 @@ __device__ __forceinline__ void row_directly(const LoraArgs &a, const W *A, cons
   }
 }
 
-// 2048 rows of 4 adapters of rank 64 bf16, 4096 to 4096: 44 us, 2.4 TB/s of the rows' own bytes, the tensor pipe 8 % and
-// the issue slots 23 % busy: the phases (rows, first product, the cluster's sum, second product) follow one another, two
+// 2048 rows of 4 adapters of rank 64 bf16, 4096 to 4096: 45 us, 2.4 TB/s of the rows' own bytes, the tensor pipe 8 % and
+// the issue slots 24 % busy: the phases (rows, first product, the cluster's sum, second product) follow one another, two
 // CTAs an SM.
 // parts clusters share a tile: each computes its vectors and takes a part of d. kPart: of n, the launch takes a part.
 template <typename W, bool kPart>
@@ -978,8 +978,10 @@ int parts_for(int tiles) {
 
 // The two kernels' times in microseconds, fitted to 70 shapes (1 to 2048 rows, 1 to 64 adapters of rank 4 to 64, 256 to
 // 14336 columns, the three types) to 17 % on average; where the estimates choose wrongly the two are close (1 % lost on
-// average over the same shapes, 27 % at most). A row's adapter comes from L2 for every row. 33 rows, rank 32 fp32, 4096
-// to 14336: 12 us here, 38 as tiles.
+// average over the same shapes, 27 % at most). Ranks 65 to 128 lie outside the fit: right for 8 rows and from 256 on, but
+// of 33 to 128 rows of 4 to 8 adapters many go to the row kernel where tiles take half the time (128 rows of 8 adapters of
+// rank 128 bf16, 4096 to 4096: 48 us, 29 as tiles; fp32, 2048 to 8192: 127 us, 57 as tiles). A row's adapter comes from
+// L2 for every row. 33 rows, rank 32 fp32, 4096 to 14336: 11 us here, 38 as tiles.
 template <typename W>
 double row_us(const LoraArgs &a) {
   const double mb = 1e-6 * a.rows;
@@ -1014,6 +1016,8 @@ cudaError_t launch_rows(const LoraArgs &a) {
   return launch<W>(lora_row_kernel<W, C>, a, (unsigned)a.rows, 1, 0, C);
 }
 
+// Ranks above kTileRank and kMaxBins adapters or more go to the row kernel whatever the rows (2048 rows of rank 256 bf16,
+// 4096 to 4096: 1340 us, of rank 128 as tiles 130).
 template <typename W>
 cudaError_t run(const LoraArgs &a) {
   if (a.count >= kMaxBins || a.max_rank > kTileRank || row_us<W>(a) <= tile_us<W>(a))

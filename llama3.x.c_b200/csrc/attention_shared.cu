@@ -367,12 +367,6 @@ __device__ __forceinline__ bool tc_wait(uint64_t *bar, unsigned parity, volatile
   return __all_sync(0xffffffffu, ok);
 }
 
-__device__ __forceinline__ bool elect_one() {
-  uint32_t is;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
-  return is != 0;
-}
-
 // kind::f16 instruction descriptor: fp16 A and B, A K-major, B K-major or MN-major, fp32 accumulators, M x N.
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);

@@ -435,12 +435,6 @@ __device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t adesc, uint64_t b
       : "memory");
 }
 
-__device__ __forceinline__ bool elect_one() {
-  uint32_t is;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
-  return is != 0;
-}
-
 // A CTA's wait for its MMAs, with one answer for a warp's lanes: false once any wait of the CTA has given up.
 __device__ __forceinline__ bool tile_wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
   bool ok = mbar_try_wait(bar, parity);

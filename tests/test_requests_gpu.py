@@ -655,6 +655,31 @@ def test_lora_rows_of_any_numbers(kc, rows, dtype):
     assert torch.equal(out[inf].double(), want[inf])
 
 
+@pytest.mark.parametrize("n", [1024, 16384 + 72])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_lora_rows_of_any_numbers_in_place(kc, n, dtype):
+    """Rows that are not finite, over one launch and over two parts of n, with base as the output: the same bits as beside
+    it, and every row's own result."""
+    rows, d, ranks = 700, 300, [16, 5, 128]
+    a, b, scale, index, g = lora_inputs((rows, 3, ranks, n, d, dtype), "mixed", 4)
+    x, base = normal(g, rows, n), normal(g, rows, d)
+    sick = torch.arange(0, rows, 23, device="cuda")
+    x[sick, torch.randint(0, n, (len(sick),), device="cuda", generator=g)] = float("inf")
+    x[sick[::2], n - 1] = float("nan")
+    table = kc.lora_table(a, b, scale)
+    out, again = torch.full((rows, d), -7.0, device="cuda"), base.clone()
+    kc.k_lora_rows(out, d, base, d, x, n, index, table, 3, kind(kc, dtype), 128, n, d, rows)
+    kc.k_lora_rows(again, d, again, d, x, n, index, table, 3, kind(kc, dtype), 128, n, d, rows)
+    kc.status()
+    assert torch.equal(out.isfinite(), again.isfinite())
+    assert torch.equal(out[out.isfinite()], again[out.isfinite()])
+    want, tol = lora_64(x, base, index, a, b, scale)
+    finite = want.isfinite()
+    assert torch.equal(out.isfinite(), finite) and ((out.double() - want).abs() <= tol)[finite].all()
+    with_adapter = sick[index[sick] >= 0]
+    assert len(with_adapter) > 10 and not out[with_adapter].isfinite().any()
+
+
 def test_lora_more_rows_than_a_launch_takes(kc):
     """Over 16384 rows: several launches, each with its own part of the index."""
     case = (20000, 3, [16, 8, 24], 256, 264, torch.bfloat16)

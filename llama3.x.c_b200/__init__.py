@@ -570,13 +570,13 @@ def lora_table(a, b, scale):
 
 def k_lora_rows(out, ldo, base, ldb, x, ldx, index, table, count, type, max_rank, n, d, rows):
     """out = base + scale B (A x) with the adapter each row names (include/kernels_cuda.h); table from lora_table, whose
-    type and sizes have to be the call's."""
+    type and n have to be the call's, and which has d outputs at least."""
     import torch
     _want(torch.float32, out, base, x, strided=True)
     _want(torch.int32, index)
     _want_here("the adapters' table", table)
     made_for = getattr(table, "_made_for", (type, n, d))
-    if made_for != (type, n, d):
+    if made_for[:2] != (type, n) or d > made_for[2]:  # the first d outputs alone are in order
         raise KernelError("a table of adapters of type %d, %d to %d, " % made_for +
                           "for a call with type %d, %d to %d" % (type, n, d))
     if table is not None and count * ctypes.sizeof(LoraAdapter) > table.numel():

@@ -163,10 +163,12 @@ def test_python_mirror_holds_a_table_to_its_call(on_cpu, dtype, kind):
     for other in ((kind + 1) % 3, (kind + 2) % 3):
         with pytest.raises(kc.KernelError, match=f"table of adapters of type {kind}, 64 to 32, .* type {other}, 64 to 32"):
             call(kind=other)
-    for sizes in (dict(n=128), dict(n=63), dict(d=64), dict(d=31)):
+    for sizes in (dict(n=128), dict(n=63), dict(d=64), dict(d=33)):
         with pytest.raises(kc.KernelError, match="for a call with"):
             call(**sizes)
     assert calls == ["k_lora_rows"]
+    call(d=31)  # the first outputs alone
+    assert len(calls) == 2
     with pytest.raises(kc.KernelError, match="float32, bfloat16 or float16"):
         kc.lora_table([torch.zeros(8, 64, dtype=torch.float64)], [torch.zeros(32, 8, dtype=torch.float64)], [1.0])
 

@@ -501,26 +501,24 @@ def k_random_q8(q, s, rows, cols, row0, col0, full_cols, seed, tensor, std, gs):
 
 # ---- a batch of requests over one prompt ------------------------------------------------------------------------------
 
-def _current_device():
-    if _device is None:
-        _bind_torch()
-    return _device() if _device else None  # None: there are no CUDA tensors
-
-
 def _want(dtype, *tensors, strided=False):
     """The tensors (None allowed) must be contiguous ones (`strided`: rows of neighbouring elements, with a row stride
-    that the call names) of `dtype` on the current device: their addresses are all that the library sees."""
-    device = _current_device()
+    that the call names) of `dtype` on the current device, which is returned: their addresses are all that the library
+    sees."""
+    if _device is None:
+        _bind_torch()
+    device = _device() if _device else None  # None: there are no CUDA tensors
     for t in tensors:
         if t is not None and (t.dtype is not dtype or t.get_device() != device or
                               not (t.is_contiguous() or strided and (t.shape[-1] < 2 or t.stride(-1) == 1))):
             raise KernelError(f"needs a contiguous {dtype} CUDA tensor on the current device, got {t.dtype} on "
                               f"{t.device} with strides {tuple(t.stride())}")
+    return device
 
 
-def _want_here(what, memory):
-    """Memory of any type (None allowed) on the current device."""
-    if memory is not None and memory.get_device() != _current_device():
+def _want_here(what, memory, device):
+    """Memory of any type (None allowed) on the device."""
+    if memory is not None and memory.get_device() != device:
         raise KernelError(f"{what} must be on the current CUDA device, is on {memory.device}")
 
 
@@ -540,8 +538,8 @@ def k_attention_shared_rows(out, oq, os_, q, prefix_key, prefix_value, prefix_se
     import torch
     _want(torch.float32, out, q, prefix_key, prefix_value, kc, vc, os_)
     _want(torch.int32, starts, counts)
-    _want(torch.int8, oq)
-    _want_here("the attention work", getattr(work, "_memory", None))
+    device = _want(torch.int8, oq)
+    _want_here("the attention work", getattr(work, "_memory", None), device)
     _call("k_attention_shared_rows", _ptr(out), _ptr(oq), _ptr(os_), _ptr(q), _ptr(prefix_key), _ptr(prefix_value),
           prefix_seq_len, prefix, _ptr(kc), _ptr(vc), _ptr(starts), _ptr(counts), ctypes.byref(work), n_heads,
           n_kv_heads, head_dim, seq_len, batch, rows, gs)
@@ -573,8 +571,8 @@ def k_lora_rows(out, ldo, base, ldb, x, ldx, index, table, count, type, max_rank
     type and n have to be the call's, and which has d outputs at least."""
     import torch
     _want(torch.float32, out, base, x, strided=True)
-    _want(torch.int32, index)
-    _want_here("the adapters' table", table)
+    device = _want(torch.int32, index)
+    _want_here("the adapters' table", table, device)
     made_for = getattr(table, "_made_for", (type, n, d))
     if made_for[:2] != (type, n) or d > made_for[2]:  # the first d outputs alone are in order
         raise KernelError("a table of adapters of type %d, %d to %d, " % made_for +
@@ -595,8 +593,8 @@ def k_verify_draft(accepted, tokens, target, ldt, draft, ldd, drafted, counts, u
     import torch
     _want(torch.int32, accepted, tokens, drafted, counts)
     _want(torch.float32, uniforms, temperature)
-    _want(torch.float32, target, draft, strided=True)
-    _want_here("the work", work)
+    device = _want(torch.float32, target, draft, strided=True)
+    _want_here("the work", work, device)
     if work is not None and work.numel() * work.element_size() < load().k_verify_bytes(vocab, batch, rows):
         raise KernelError("k_verify_draft: the work is too small for this shape")
     _call("k_verify_draft", _ptr(accepted), _ptr(tokens), _ptr(target), ldt, _ptr(draft), ldd, _ptr(drafted),

@@ -354,6 +354,62 @@ void k_verify_draft(int *accepted, int *tokens, const float *target, size_t ldt,
                     const int *drafted, const int *counts, const float *uniforms, const float *temperature, int vocab,
                     int batch, int rows, void *work);
 
+/* ---- serving from a paged K/V cache (no counterpart in the reference, whose cache is one sequence's) -------------- */
+/* One layer's keys and values in pages of page_size positions: key and value are [pages][n_kv_heads][page_size]
+ * [head_dim] of `type` (KernelType), head-major within a page as the contiguous cache is, page_stride elements from one
+ * page to the next (at least n_kv_heads * page_size * head_dim; more where keys and values, or layers, take turns in one
+ * pool). Position p of request b lies in row p % page_size of page table[b * max_pages + p / page_size]; the table is
+ * device memory, so a captured step replays as requests get pages. A page may be in the tables of several requests (a
+ * shared prompt). Any page_size; max_pages * page_size up to 2^31 - 1025 positions. The struct is read during the call. */
+typedef struct {
+  void *key, *value;
+  const int *table;
+  size_t page_stride;
+  int type, pages, page_size, max_pages;
+} PagedCache;
+
+/* k_rope_kv_store_rows for a batch of requests and a paged cache. q [batch][rows][n_heads * head_dim] (row stride q_ld), k
+ * and v [batch][rows][n_kv_heads * head_dim] (row stride kv_ld). Row r of request b, r < counts[b] (NULL: rows for all,
+ * 0 .. rows), stands at position starts[b] + r: its queries rotated with row starts[b] + r of `rope` [seq_len][2 *
+ * head_dim] go to q_out (row stride q_out_ld; may be q itself with q's stride, else must not overlap it), its rotated keys
+ * and its values into the cache, rounded to nearest (a value beyond fp16's range to infinity). The rotation is
+ * k_rope_kv_store_rows', bitwise. Other rows of q_out and all other cache rows stay as they were. starts and counts are
+ * device memory. A request with starts[b] outside [0, min(seq_len, max_pages * page_size) - counts[b]] or counts[b]
+ * outside [0, rows] raises an error (kc_status) and is left out whole; a row whose page is outside [0, pages) raises one
+ * and is left out. No two rows may fall on one place of the cache. */
+void k_rope_kv_store_paged(float *q_out, size_t q_out_ld, const float *q, size_t q_ld, const float *k, const float *v,
+                           size_t kv_ld, const PagedCache *cache, const float *rope, int seq_len, const int *starts,
+                           const int *counts, int n_heads, int n_kv_heads, int head_dim, int batch, int rows);
+
+/* Attention over a paged cache: q and out [batch][rows][n_heads * head_dim]; row r of request b, r < counts[b] (NULL: rows
+ * for all), sees positions [0, starts[b] + r] of its pages: starts[b] were stored before this step's rows (one row: a
+ * request's last token; more: its drafts behind it). Other rows of out stay as they were, and a request that uses none
+ * needs no starts[b] and no pages. A request with starts[b] outside [0, max_pages * page_size - counts[b]], counts[b]
+ * outside [0, rows], or a page that it sees outside [0, pages) raises an error (kc_status) and its rows stay as they were.
+ * What a row sees must be finite, or that row has no result; what it does not see, finite or not (the rest of a page,
+ * pages no one uses, later drafts), changes nothing in it. Products are fp32 ones up to 2^-22 of each, sums and statistics
+ * fp32. oq / os (may be NULL): out quantized for Wo as k_quantize does, gs dividing head_dim. head_dim <= 256.
+ * `work` (k_attention_paged_init, released with k_attention_free): partial results and tickets for this n_heads and
+ * head_dim and up to batch * rows rows (its `workers`; its max_chunks is -1, so that no other kind of work passes for it);
+ * `memory` as for k_attention_init_rows (k_attention_paged_bytes bytes, 16-byte aligned, or NULL). k_attention_paged_init
+ * zeroes the tickets on the calling thread's stream, and every call leaves them zeroed. One call in flight per work. */
+size_t k_attention_paged_bytes(int n_heads, int n_kv_heads, int head_dim, int batch, int rows);
+void k_attention_paged_init(AttentionWork *work, int n_heads, int n_kv_heads, int head_dim, int batch, int rows,
+                            void *memory);
+void k_attention_paged_rows(float *out, int8_t *oq, float *os, const float *q, const PagedCache *cache, const int *starts,
+                            const int *counts, AttentionWork *work, int n_heads, int n_kv_heads, int head_dim, int batch,
+                            int rows, int gs);
+
+/* Log probabilities from the logits of `rows` rows of `vocab` (device memory, row stride ld, a classifier's k_gemm_q8
+ * output): logprobs[r] = log softmax(logits[r])[tokens[r]], entropy[r] = -sum p log p of row r (may be NULL), and the `top`
+ * (0 .. 32, at most vocab) likeliest tokens of each row in top_tokens and top_logprobs [rows][top], in descending order,
+ * the lowest token first among equals. tokens[r] = -1: a row not in use, its outputs stay as they were. logprobs and tokens
+ * may be NULL together: every row is in use. A logit of -infinity is a token ruled out (its log probability -infinity,
+ * its share of the entropy 0). A row in use with a NaN, +infinity or no value above -infinity, or a token outside the
+ * vocabulary, raises an error (kc_status): its log probabilities and entropy are NaN, its top tokens -1. */
+void k_token_logprobs(float *logprobs, float *entropy, int *top_tokens, float *top_logprobs, const float *logits, size_t ld,
+                      const int *tokens, int vocab, int rows, int top);
+
 /* ---- test hooks (include/testing.h:67-69) ------------------------------------------------------------------------ */
 /* One named backend; returns 0 when it is not compiled in (the CPU rungs). */
 int k_gemm_q8_backend_test(Q8GemmBackend backend, const int8_t *xq, const float *xs, int m, int k, int gs,

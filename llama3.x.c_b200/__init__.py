@@ -66,6 +66,13 @@ class LoraAdapter(ctypes.Structure):
     _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("rank", ctypes.c_int), ("scale", ctypes.c_float)]
 
 
+class PagedCache(ctypes.Structure):
+    """include/kernels_cuda.h: one layer's keys and values in pages, and the requests' page table."""
+    _fields_ = [("key", ctypes.c_void_p), ("value", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("page_stride", ctypes.c_size_t), ("type", ctypes.c_int), ("pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("max_pages", ctypes.c_int)]
+
+
 # Every symbol include/kernels_cuda.h declares, with its ctypes signature (restype, argtypes).
 _c = ctypes
 _SIGNATURES = {
@@ -153,6 +160,17 @@ _SIGNATURES = {
     "k_verify_bytes": (_c.c_size_t, [_c.c_int, _c.c_int, _c.c_int]),
     "k_verify_draft": (None, [_c.c_void_p, _c.c_void_p, _f32p, _c.c_size_t, _f32p, _c.c_size_t, _c.c_void_p,
                               _c.c_void_p, _f32p, _f32p, _c.c_int, _c.c_int, _c.c_int, _c.c_void_p]),
+    "k_rope_kv_store_paged": (None, [_f32p, _c.c_size_t, _f32p, _c.c_size_t, _f32p, _f32p, _c.c_size_t,
+                                     _c.POINTER(PagedCache), _f32p, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int,
+                                     _c.c_int, _c.c_int, _c.c_int]),
+    "k_attention_paged_bytes": (_c.c_size_t, [_c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int]),
+    "k_attention_paged_init": (None, [_c.POINTER(AttentionWork), _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int,
+                                      _c.c_void_p]),
+    "k_attention_paged_rows": (None, [_f32p, _i8p, _f32p, _f32p, _c.POINTER(PagedCache), _c.c_void_p, _c.c_void_p,
+                                      _c.POINTER(AttentionWork), _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int,
+                                      _c.c_int]),
+    "k_token_logprobs": (None, [_f32p, _f32p, _c.c_void_p, _f32p, _f32p, _c.c_size_t, _c.c_void_p, _c.c_int, _c.c_int,
+                                _c.c_int]),
 }
 
 
@@ -545,13 +563,18 @@ def k_attention_shared_rows(out, oq, os_, q, prefix_key, prefix_value, prefix_se
           n_kv_heads, head_dim, seq_len, batch, rows, gs)
 
 
+def _kinds():
+    import torch
+    return {torch.float32: K_F32, torch.bfloat16: K_BF16, torch.float16: K_F16}
+
+
 def lora_table(a, b, scale):
     """k_lora_rows' device table of the adapters (a[i] [rank_i][n], b[i] [d][rank_i], scale[i]); it keeps the matrices
     alive. One dtype throughout: float32, bfloat16 or float16."""
     import torch
     if not (len(a) == len(b) == len(scale)) or not a:
         raise KernelError("lora_table needs as many a and b matrices as scales, at least one")
-    kinds = {torch.float32: K_F32, torch.bfloat16: K_BF16, torch.float16: K_F16}
+    kinds = _kinds()
     if a[0].dtype not in kinds:
         raise KernelError(f"lora_table takes float32, bfloat16 or float16 matrices, got {a[0].dtype}")
     for x, y in zip(a, b):
@@ -599,3 +622,80 @@ def k_verify_draft(accepted, tokens, target, ldt, draft, ldd, drafted, counts, u
         raise KernelError("k_verify_draft: the work is too small for this shape")
     _call("k_verify_draft", _ptr(accepted), _ptr(tokens), _ptr(target), ldt, _ptr(draft), ldd, _ptr(drafted),
           _ptr(counts), _ptr(uniforms), _ptr(temperature), vocab, batch, rows, _ptr(work))
+
+
+# ---- serving from a paged K/V cache ------------------------------------------------------------------------------------
+
+def paged_cache(key, value, table):
+    """A PagedCache of key and value [pages][n_kv_heads][page_size][head_dim] (float32, bfloat16 or float16; contiguous, or
+    slices of a larger pool along the first dimension) and table [batch][max_pages] int32; it keeps them alive."""
+    import torch
+    kinds = _kinds()
+    if key.dtype not in kinds:
+        raise KernelError(f"paged_cache takes float32, bfloat16 or float16 keys and values, got {key.dtype}")
+    device = _want(torch.int32, table)
+    for t in (key, value):
+        if (t.dim() != 4 or t.dtype is not key.dtype or t.shape != key.shape or t.get_device() != device or
+                not t[:1].is_contiguous() or t.numel() and t.stride(0) != key.stride(0)):
+            raise KernelError(f"paged_cache needs two {key.dtype} tensors of one shape [pages][n_kv_heads][page_size]"
+                              f"[head_dim] with whole pages in order on the current CUDA device, got {tuple(t.shape)} "
+                              f"{t.dtype} on {t.device} with strides {tuple(t.stride())}")
+    if table.dim() != 2:
+        raise KernelError(f"paged_cache needs a table [batch][max_pages], got {tuple(table.shape)}")
+    pages, n_kv, page_size, hd = key.shape
+    cache = PagedCache(_ptr(key), _ptr(value), _ptr(table), key.stride(0) if pages > 1 else n_kv * page_size * hd,
+                       kinds[key.dtype], pages, page_size, table.shape[1])
+    cache._tensors = (key, value, table)
+    cache._made_for = (n_kv, hd, table.shape[0], device)
+    return cache
+
+
+def _want_cache(cache, n_kv_heads, head_dim, batch, device):
+    made_for = getattr(cache, "_made_for", None)
+    if made_for and (made_for[:2] != (n_kv_heads, head_dim) or batch > made_for[2] or made_for[3] != device):
+        raise KernelError("a paged cache of %d heads of %d for %d requests on device %s, " % made_for +
+                          f"for a call with {n_kv_heads} heads of {head_dim}, {batch} requests, on device {device}")
+
+
+def k_rope_kv_store_paged(q_out, q_out_ld, q, q_ld, k, v, kv_ld, cache, rope, seq_len, starts, counts, n_heads, n_kv_heads,
+                          head_dim, batch, rows):
+    """Queries rotated, rotated keys and values into their pages (include/kernels_cuda.h); counts may be None."""
+    import torch
+    _want(torch.float32, q_out, q, k, v, strided=True)
+    _want(torch.float32, rope)
+    _want_cache(cache, n_kv_heads, head_dim, batch, _want(torch.int32, starts, counts))
+    _call("k_rope_kv_store_paged", _ptr(q_out), q_out_ld, _ptr(q), q_ld, _ptr(k), _ptr(v), kv_ld, ctypes.byref(cache),
+          _ptr(rope), seq_len, _ptr(starts), _ptr(counts), n_heads, n_kv_heads, head_dim, batch, rows)
+
+
+def paged_attention_work(n_heads, n_kv_heads, head_dim, batch, rows=1):
+    """k_attention_paged_init on torch memory, which lives as long as the work does."""
+    import torch
+    w = AttentionWork()
+    w._memory = torch.empty(max(16, load().k_attention_paged_bytes(n_heads, n_kv_heads, head_dim, batch, rows)),
+                            dtype=torch.uint8, device="cuda")
+    _call("k_attention_paged_init", ctypes.byref(w), n_heads, n_kv_heads, head_dim, batch, rows, _ptr(w._memory))
+    return w
+
+
+def k_attention_paged_rows(out, oq, os_, q, cache, starts, counts, work, n_heads, n_kv_heads, head_dim, batch, rows, gs):
+    """Attention over a paged cache (include/kernels_cuda.h); oq, os_ and counts may be None."""
+    import torch
+    _want(torch.float32, out, q, os_)
+    _want(torch.int8, oq)
+    device = _want(torch.int32, starts, counts)
+    _want_cache(cache, n_kv_heads, head_dim, batch, device)
+    _want_here("the attention work", getattr(work, "_memory", None), device)
+    _call("k_attention_paged_rows", _ptr(out), _ptr(oq), _ptr(os_), _ptr(q), ctypes.byref(cache), _ptr(starts),
+          _ptr(counts), ctypes.byref(work), n_heads, n_kv_heads, head_dim, batch, rows, gs)
+
+
+def k_token_logprobs(logprobs, entropy, top_tokens, top_logprobs, logits, ld, tokens, vocab, rows, top):
+    """Log probabilities of tokens, entropy and likeliest alternatives (include/kernels_cuda.h); logprobs with tokens,
+    entropy, and (top 0) top_tokens and top_logprobs may be None."""
+    import torch
+    _want(torch.float32, logprobs, entropy, top_logprobs)
+    _want(torch.int32, tokens, top_tokens)
+    _want(torch.float32, logits, strided=True)
+    _call("k_token_logprobs", _ptr(logprobs), _ptr(entropy), _ptr(top_tokens), _ptr(top_logprobs), _ptr(logits), ld,
+          _ptr(tokens), vocab, rows, top)

@@ -16,6 +16,7 @@
 
 #include "../../include/kernels_cuda.h"
 #include "common.cuh"
+#include "divide.cuh"
 #include "kernels_cuda_internal.h"
 #include "tcgen05.cuh"
 
@@ -30,29 +31,6 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kGenericThreads = 256, kGenericWarps = kGenericThreads / 32;
 constexpr int kGenericVecs = 32;   // query vectors per CTA
 constexpr int kGenericPos = 32;    // positions per tile
-
-// Division by a number known on the host, by multiplication (Granlund and Montgomery): exact for n < 2^31.
-struct Divisor {
-  int d;
-  unsigned m, shift;
-};
-Divisor divisor(int d) {
-  unsigned l = 0;
-  while ((1ll << l) < d)
-    l++;
-  return Divisor{d, (unsigned)(((1ull << 32) * ((1ull << l) - (unsigned)d)) / (unsigned)d + 1), l};
-}
-// n / by, and n becomes the rest.
-__host__ __device__ __forceinline__ int divide(int &n, const Divisor &by) {
-#ifdef __CUDA_ARCH__
-  const unsigned high = __umulhi((unsigned)n, by.m);
-#else
-  const unsigned high = (unsigned)(((unsigned long long)(unsigned)n * by.m) >> 32);
-#endif
-  const int q = (int)((high + (unsigned)n) >> by.shift);
-  n -= q * by.d;
-  return q;
-}
 
 struct SharedArgs {
   const float *q;             // [batch][rows][n_heads][hd]

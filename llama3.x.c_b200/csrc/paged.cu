@@ -1,0 +1,774 @@
+// Serving from a paged K/V cache: keys and values stored into their pages with the rotation of queries and keys
+// (k_rope_kv_store_paged), and attention over the pages (k_attention_paged_rows).
+//
+// A cache is [pages][n_kv][page_size][hd]; position p of request b lies in row p % page_size of page
+// table[b][p / page_size].
+//
+// Attention, per query vector q (already rotated) with scores s_p = q . k_p / sqrt(hd) over the positions that it sees:
+// out = sum_p 2^(s'_p - m) v_p / sum_p 2^(s'_p - m), s' = s log2(e), m a running maximum. The work is cut into segments,
+// a KV head of a request with up to `block` of its query vectors, and each segment's positions into tiles; the tiles of
+// all segments form one row, of which every CTA takes an equal, contiguous share, whatever the requests' lengths are. A
+// segment that lies in several shares leaves partial results (m, l = sum 2^(s' - m), o = sum 2^(s' - m) v) that the CTA
+// to finish last joins, in the order of the shares.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "../../include/kernels_cuda.h"
+#include "common.cuh"
+#include "divide.cuh"
+#include "kernels_cuda_internal.h"
+#include "tcgen05.cuh"
+
+namespace {
+
+constexpr int kMaxHd = 256;
+constexpr int kMaxPositions = 0x7fffffff - 1024;  // tiles are numbered past the last one
+constexpr float kLog2e = 1.44269504088896341f;
+
+// A request's rows in use and the positions stored before them; 0 rows where they are not sound.
+struct Request {
+  int count, start;
+  bool bad;
+};
+__device__ __forceinline__ Request request_of(const int *starts, const int *counts, int b, int rows, int positions) {
+  const int count = counts ? counts[b] : rows, start = starts[b];
+  const bool ok = count > 0 && count <= rows && start >= 0 && start <= positions - count;
+  return Request{ok ? count : 0, start, !ok && count != 0};
+}
+
+// ---- storing ------------------------------------------------------------------------------------------------------
+
+struct StoreArgs {
+  float *q_out;
+  const float *q, *k, *v, *rope;
+  void *key, *value;
+  const int *table, *starts, *counts;
+  long long q_out_ld, q_ld, kv_ld;
+  size_t page_stride;
+  int pages, page_size, max_pages, positions, n_heads, n_kv, hd, batch, rows, per_row;
+};
+
+__device__ __forceinline__ void put(float *at, float a, float b) { at[0] = a, at[1] = b; }
+__device__ __forceinline__ void put(__nv_bfloat16 *at, float a, float b) {
+  at[0] = __float2bfloat16_rn(a), at[1] = __float2bfloat16_rn(b);
+}
+__device__ __forceinline__ void put(__half *at, float a, float b) {
+  at[0] = __float2half_rn(a), at[1] = __float2half_rn(b);
+}
+
+// A thread per pair of a row's queries, keys or values.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long long row = id / a.per_row;
+  if (row >= (long long)a.batch * a.rows)
+    return;
+  int pair = (int)(id - row * a.per_row);
+  const int b = (int)(row / a.rows), r = (int)(row - (long long)b * a.rows);
+  const Request request = request_of(a.starts, a.counts, b, a.rows, a.positions);
+  if (request.bad && r == 0 && pair == 0)
+    kc_raise(KC_ERR_BAD_ARGS);
+  if (r >= request.count)
+    return;
+  const int position = request.start + r, at = position / a.page_size;
+  const int page = a.table[(size_t)b * a.max_pages + at];
+  if (page < 0 || page >= a.pages) {
+    if (pair == 0)
+      kc_raise(KC_ERR_BAD_ARGS);
+    return;
+  }
+  const int half = a.hd / 2, head = pair / half, j = 2 * (pair - head * half);
+  const float *table = a.rope + (size_t)position * 2 * a.hd;
+  const size_t place = (size_t)page * a.page_stride + (size_t)(position - at * a.page_size) * a.hd + j;
+  const size_t head_stride = (size_t)a.page_size * a.hd;
+  if (head < a.n_heads + a.n_kv) {
+    const bool is_k = head >= a.n_heads;
+    const int h = is_k ? head - a.n_heads : head;
+    const float *src = (is_k ? a.k + row * a.kv_ld : a.q + row * a.q_ld) + (size_t)h * a.hd + j;
+    const float c = table[j], s = table[a.hd + j + 1], x = src[0], y = src[1];
+    const float o0 = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s)), o1 = __fadd_rn(__fmul_rn(x, s), __fmul_rn(y, c));
+    if (is_k)
+      put(static_cast<T *>(a.key) + place + h * head_stride, o0, o1);
+    else
+      put(a.q_out + row * a.q_out_ld + (size_t)h * a.hd + j, o0, o1);
+  } else {
+    const int h = head - a.n_heads - a.n_kv;
+    const float *src = a.v + row * a.kv_ld + (size_t)h * a.hd + j;
+    put(static_cast<T *>(a.value) + place + h * head_stride, src[0], src[1]);
+  }
+}
+
+// ---- attention ----------------------------------------------------------------------------------------------------
+
+struct PagedArgs {
+  const float *q;
+  const void *key, *value;
+  const int *table, *starts, *counts;
+  float *out;
+  int8_t *oq;
+  float *os;
+  float *partial;        // [2 ctas] slots of slot_floats
+  unsigned *tickets;     // one to a segment, zero between calls
+  size_t page_stride;
+  int pages, max_pages, positions, page_size;
+  int n_heads, n_kv, group, hd, batch, rows, gs;
+  int block, blocks;     // query vectors to a segment, and segments to a KV head of a request with all rows
+  int slot_floats;
+  Divisor by_page, by_group;
+};
+
+// Slots: a flag (4 floats), m and l of each vector, then their sums.
+__host__ __device__ __forceinline__ int slot_size(int block, int hd) { return (4 + 2 * block + block * hd + 3) & ~3; }
+
+constexpr int kRangeThreads = 1024;
+struct Range {
+  long long lo, hi, total, before;  // this CTA's tiles, all tiles, those before request b
+  int b, ctas;
+  long long sums[kRangeThreads / 32];
+};
+
+// Tiles of a request's segments (of each one), and how many segments it has.
+struct Shape {
+  int tiles, segments, blocks;
+};
+__device__ __forceinline__ Shape shape_of(const PagedArgs &a, const Request &r, int tile) {
+  Shape s;
+  s.blocks = (r.count * a.group + a.block - 1) / a.block;
+  s.segments = a.n_kv * s.blocks;
+  s.tiles = r.count ? (r.start + r.count + tile - 1) / tile : 0;
+  return s;
+}
+
+// This CTA's share of the tiles, and the request in which it begins. All threads call it. False: nothing to do.
+__device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *range) {
+  const int threads = blockDim.x, t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int per = (a.batch + threads - 1) / threads, b0 = t * per, b1 = min(a.batch, b0 + per);
+  long long own = 0;
+  for (int b = b0; b < b1; b++) {
+    const Request r = request_of(a.starts, a.counts, b, a.rows, a.positions);
+    if (r.bad && blockIdx.x == 0)
+      kc_raise(KC_ERR_BAD_ARGS);
+    const Shape s = shape_of(a, r, tile);
+    own += (long long)s.tiles * s.segments;
+  }
+  long long upto = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+    upto += lane >= o ? x : 0;
+  }
+  if (lane == 31)
+    range->sums[warp] = upto;
+  __syncthreads();
+  long long total = 0;
+  for (int w = 0; w < threads / 32; w++) {
+    upto += w < warp ? range->sums[w] : 0;
+    total += range->sums[w];
+  }
+  const long long ctas = total < gridDim.x ? total : gridDim.x, cta = blockIdx.x;
+  if (cta >= ctas)
+    return false;
+  const long long lo = total * cta / ctas, hi = total * (cta + 1) / ctas;
+  if (lo >= upto - own && lo < upto) {
+    long long before = upto - own;
+    int b = b0;
+    for (;; b++) {
+      const Shape s = shape_of(a, request_of(a.starts, a.counts, b, a.rows, a.positions), tile);
+      const long long n = (long long)s.tiles * s.segments;
+      if (lo < before + n)
+        break;
+      before += n;
+    }
+    range->lo = lo, range->hi = hi, range->total = total, range->before = before, range->b = b, range->ctas = (int)ctas;
+  }
+  __syncthreads();
+  return true;
+}
+
+// The CTA whose share holds tile x.
+__device__ __forceinline__ int owner(const Range *range, long long x) {
+  return (int)(((x + 1) * range->ctas - 1) / range->total);
+}
+
+// Weights are held times 2^-guard, 2^guard above the positions that a row sees: so that the sum of as many values of the
+// type's largest size, each with the largest weight, is a number.
+__device__ __forceinline__ float guard_of(int positions) { return (float)(32 - __clz(positions)); }
+
+// One piece of work: tiles [t0, t1) of a segment.
+struct Piece {
+  int b, head, block;       // request, KV head, block of query vectors
+  int start, count, vecs;   // the request's; vectors of this block
+  int t0, t1, tiles;
+  long long first;          // the segment's first tile
+};
+
+// Walks through a CTA's pieces; every thread that walks sees the same.
+struct Walk {
+  long long at, before;
+  int b;
+  Request request;
+  Shape shape;
+  __device__ __forceinline__ Walk(const PagedArgs &a, const Range *range, int tile) {
+    at = range->lo, before = range->before, b = range->b;
+    request = request_of(a.starts, a.counts, b, a.rows, a.positions);
+    shape = shape_of(a, request, tile);
+  }
+  __device__ __forceinline__ bool next(const PagedArgs &a, const Range *range, int tile, Piece *p) {
+    if (at >= range->hi)
+      return false;
+    while (at - before >= (long long)shape.tiles * shape.segments) {
+      before += (long long)shape.tiles * shape.segments;
+      b++;
+      request = request_of(a.starts, a.counts, b, a.rows, a.positions);
+      shape = shape_of(a, request, tile);
+    }
+    const long long local = at - before;
+    const int segment = (int)(local / shape.tiles);
+    p->b = b;
+    p->head = segment / shape.blocks;
+    p->block = segment - p->head * shape.blocks;
+    p->start = request.start, p->count = request.count;
+    p->vecs = min(a.block, request.count * a.group - p->block * a.block);
+    p->tiles = shape.tiles;
+    p->first = before + (long long)segment * shape.tiles;
+    p->t0 = (int)(at - p->first);
+    p->t1 = (int)min((long long)shape.tiles, range->hi - p->first);
+    at = p->first + p->t1;
+    return true;
+  }
+};
+
+// Vector v of a piece: index in the [batch][rows][n_heads] order.
+__device__ __forceinline__ int vector_at(const PagedArgs &a, const Piece &p, int v, int *row) {
+  int member = p.block * a.block + v;
+  *row = divide(member, a.by_group);
+  return (p.b * a.rows + *row) * a.n_heads + p.head * a.group + member;
+}
+
+// The piece's vectors, with m and l of each and their sums o in shared memory, written to the output (a whole segment,
+// or the last of its pieces to be done) or to a slot. All threads call it, after a barrier behind the last write to m, l,
+// o and bad; it ends with one.
+__device__ void finish(const PagedArgs &a, const Range *range, const Piece &p, float *m, float *l, float *o,
+                       const int *bad, int *last) {
+  const int threads = blockDim.x, t = threadIdx.x, hd = a.hd;
+  bool wrong = *bad != 0;
+  if (p.t0 || p.t1 < p.tiles) {
+    const int c0 = owner(range, p.first), c1 = owner(range, p.first + p.tiles - 1);
+    const int cta = blockIdx.x;
+    float *slot = a.partial + (size_t)(2 * cta + (cta == c0)) * a.slot_floats;
+    float *slot_m = slot + 4, *slot_l = slot_m + a.block, *slot_o = slot_l + a.block;
+    if (t == 0)
+      slot[0] = wrong ? 1.0f : 0.0f;
+    for (int i = t; i < p.vecs; i += threads)
+      slot_m[i] = m[i], slot_l[i] = l[i];
+    for (int i = t; i < p.vecs * hd; i += threads)
+      slot_o[i] = o[i];
+    __threadfence();
+    __syncthreads();
+    if (t == 0) {
+      const size_t segment = ((size_t)p.b * a.n_kv + p.head) * a.blocks + p.block;
+      *last = atomicInc(&a.tickets[segment], (unsigned)(c1 - c0)) == (unsigned)(c1 - c0);
+    }
+    __syncthreads();
+    if (!*last) {
+      __syncthreads();
+      return;
+    }
+    __threadfence();
+    auto slot_of = [&](int c) { return a.partial + (size_t)(2 * c + (c == c0)) * a.slot_floats; };
+    wrong = false;
+    for (int c = c0; c <= c1; c++)
+      wrong |= __ldcg(slot_of(c)) != 0.0f;
+    for (int i = t; i < p.vecs; i += threads) {
+      float top = -INFINITY, sum = 0.0f;
+      for (int c = c0; c <= c1; c++)
+        top = fmaxf(top, __ldcg(slot_of(c) + 4 + i));
+      for (int c = c0; c <= c1; c++) {
+        const float mc = __ldcg(slot_of(c) + 4 + i);
+        sum += mc == -INFINITY ? 0.0f : exp2f(mc - top) * __ldcg(slot_of(c) + 4 + a.block + i);
+      }
+      m[i] = top, l[i] = sum;
+    }
+    __syncthreads();
+    for (int i = t; i < p.vecs * hd; i += threads) {
+      const int v = i / hd;
+      float x = 0.0f;
+      for (int c = c0; c <= c1; c++) {
+        const float mc = __ldcg(slot_of(c) + 4 + v);
+        if (mc != -INFINITY)
+          x = fmaf(exp2f(mc - m[v]), __ldcg(slot_of(c) + 4 + 2 * a.block + i), x);
+      }
+      o[i] = x;
+    }
+    __syncthreads();
+  }
+  if (wrong) {
+    if (t == 0)
+      kc_raise(KC_ERR_BAD_ARGS);
+    __syncthreads();
+    return;
+  }
+  for (int i = t; i < p.vecs * hd; i += threads) {
+    const int v = i / hd;
+    int row;
+    const size_t vec = vector_at(a, p, v, &row);
+    float x = o[i] / l[v];
+    if (fabsf(x) == INFINITY && fabsf(o[i]) < INFINITY)  // a mean of finite values, past the largest one by its rounding
+      x = copysignf(3.402823466e+38f, x);
+    o[i] = x;
+    a.out[vec * hd + (i - v * hd)] = x;
+  }
+  __syncthreads();
+  if (!a.oq)
+    return;
+  const int warp = t >> 5, lane = t & 31, groups = hd / a.gs;
+  for (int i = warp; i < p.vecs * groups; i += threads / 32) {
+    const int v = i / groups, g = (i - v * groups) * a.gs;
+    int row;
+    const size_t at = (size_t)vector_at(a, p, v, &row) * hd + g;
+    const float *x = o + v * hd + g;
+    float mx = 0.0f;
+    bool infinite = false;
+    for (int e = lane; e < a.gs; e += 32) {
+      infinite |= !(fabsf(x[e]) < INFINITY);
+      mx = fmaxf(mx, fabsf(x[e]));
+    }
+#pragma unroll
+    for (int s = 16; s; s >>= 1)
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+    if (infinite)
+      kc_raise(KC_ERR_NONFINITE);
+    const float scale = __fdiv_rn(mx, 127.0f);
+    for (int e = lane; e < a.gs; e += 32)
+      a.oq[at + e] = (int8_t)quantize_value(x[e], scale);
+    if (lane == 0)
+      a.os[at / a.gs] = scale;
+  }
+  __syncthreads();
+}
+
+// The kernel on the CUDA cores: any type, head_dim up to 256, any alignment. LANES lanes take a position, 16 of its
+// elements each, so that a score costs log2(LANES) shuffles for 16 LANES products, and its weight meets the values in the
+// same lanes without another; four query vectors in registers share each key and value.
+constexpr int kVecs = 4, kElems = 16, kPairs = kElems / 2;
+constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int kTile = 64;       // positions
+constexpr int kCtas = 148 * 3;  // the shares; a function of nothing else, so that the workspace's size is known
+
+// A pair of elements in 32 bits each.
+__device__ __forceinline__ uint64_t pair_of(uint32_t x, __nv_bfloat16) { return f2_pack_bits(x << 16, x & 0xffff0000u); }
+__device__ __forceinline__ uint64_t pair_of(uint32_t x, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x));
+  return f2_pack(f.x, f.y);
+}
+__device__ __forceinline__ float one_of(float x) { return x; }
+__device__ __forceinline__ float one_of(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float one_of(__half x) { return __half2float(x); }
+
+// This lane's 16 elements of a row: wide, 16-byte units LANES apart; else elements LANES apart, pairs of neighbours in i.
+template <typename T, int LANES, bool WIDE>
+struct Row {
+  static constexpr int kUnit = 16 / sizeof(T);
+  static constexpr int kUnits = kElems / kUnit;
+  uint4 raw[WIDE ? kUnits : 1];
+  T one[WIDE ? 1 : kElems];
+
+  // The element behind index i of the lane's 16.
+  static __device__ __forceinline__ int element(int lane, int i) {
+    return WIDE ? (lane + LANES * (i / kUnit)) * kUnit + i % kUnit : lane + LANES * i;
+  }
+  __device__ __forceinline__ void load(const T *row, bool in, int hd, int lane) {
+    if (WIDE) {
+#pragma unroll
+      for (int u = 0; u < kUnits; u++)
+        raw[u] = in && (lane + LANES * u) * kUnit < hd
+                     ? *reinterpret_cast<const uint4 *>(row + (lane + LANES * u) * kUnit)
+                     : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kElems; i++)
+        one[i] = in && lane + LANES * i < hd ? row[lane + LANES * i] : T(0.0f);
+    }
+  }
+  __device__ __forceinline__ uint64_t pair(int i) const {  // elements 2 i, 2 i + 1
+    if (!WIDE)
+      return f2_pack(one_of(one[2 * i]), one_of(one[2 * i + 1]));
+    if constexpr (sizeof(T) == 4) {
+      const uint4 x = raw[i / 2];
+      return i % 2 ? f2_pack_bits(x.z, x.w) : f2_pack_bits(x.x, x.y);
+    } else {
+      const uint4 x = raw[i / 4];
+      return pair_of(i % 4 == 0 ? x.x : i % 4 == 1 ? x.y : i % 4 == 2 ? x.z : x.w, T(0.0f));
+    }
+  }
+};
+
+template <typename T, int LANES, bool WIDE>
+__global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedArgs a) {
+  constexpr int kAt = 32 / LANES;  // positions of a warp at a time
+  __shared__ Range range;
+  __shared__ __align__(16) float sums[kWarps][kVecs][LANES * kElems];
+  __shared__ float wm[kWarps][kVecs], wl[kWarps][kVecs], m_all[kVecs], l_all[kVecs];
+  __shared__ int bad, last;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, sub = lane % LANES, at = lane / LANES;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (t == 0)
+    bad = 0;
+  if (!find_range(a, kTile, &range))
+    return;
+  const int hd = a.hd;
+  const float scale = rsqrtf((float)hd) * kLog2e;
+  Walk walk(a, &range, kTile);
+  Piece p;
+  while (walk.next(a, &range, kTile, &p)) {
+    uint64_t q[kVecs][kPairs], acc[kVecs][kPairs];
+    float m[kVecs], l[kVecs];
+    int limit[kVecs];
+#pragma unroll
+    for (int v = 0; v < kVecs; v++) {
+      int row = 0;
+      const size_t vec = v < p.vecs ? vector_at(a, p, v, &row) : 0;
+      limit[v] = v < p.vecs ? p.start + row + 1 : 0;
+      m[v] = -INFINITY, l[v] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kPairs; i++) {
+        const int e0 = Row<T, LANES, WIDE>::element(sub, 2 * i), e1 = Row<T, LANES, WIDE>::element(sub, 2 * i + 1);
+        const float x = v < p.vecs && e0 < hd ? a.q[vec * hd + e0] * scale : 0.0f;
+        const float y = v < p.vecs && e1 < hd ? a.q[vec * hd + e1] * scale : 0.0f;
+        q[v][i] = f2_pack(x, y), acc[v][i] = 0;
+      }
+    }
+    const int end = min(p.t1 * kTile, p.start + p.count);
+    const float guard = guard_of(p.start + p.count);
+    const int *pages = a.table + (size_t)p.b * a.max_pages;
+    const size_t head = (size_t)p.head * a.page_size * hd;
+    for (int p0 = p.t0 * kTile + warp * kAt; p0 < end; p0 += kWarps * kAt) {
+      const int position = p0 + at;
+      bool in = position < end;
+      int within = position;
+      const int index = in ? divide(within, a.by_page) : 0;
+      const int page = in ? pages[index] : 0;
+      if (page < 0 || page >= a.pages) {
+        bad = 1;
+        in = false;
+      }
+      const size_t place = in ? (size_t)page * a.page_stride + head + (size_t)within * hd : 0;
+      Row<T, LANES, WIDE> k, x;
+      k.load(static_cast<const T *>(a.key) + place, in, hd, sub);
+      x.load(static_cast<const T *>(a.value) + place, in, hd, sub);
+      float s[kVecs];
+      uint64_t part[kVecs];
+#pragma unroll
+      for (int v = 0; v < kVecs; v++)
+        part[v] = 0;
+#pragma unroll
+      for (int i = 0; i < kPairs; i++) {
+        const uint64_t ki = k.pair(i);
+#pragma unroll
+        for (int v = 0; v < kVecs; v++)
+          part[v] = f2_fma(q[v][i], ki, part[v]);
+      }
+      bool rises = false;
+#pragma unroll
+      for (int v = 0; v < kVecs; v++) {
+        float lo, hi;
+        f2_unpack(part[v], lo, hi);
+        s[v] = lo + hi;
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1)
+          s[v] += __shfl_xor_sync(0xffffffffu, s[v], o);
+        s[v] = in && position < limit[v] ? s[v] : -INFINITY;
+        rises |= s[v] > m[v];
+      }
+      if (rises) {
+#pragma unroll
+        for (int v = 0; v < kVecs; v++) {
+          if (!(s[v] > m[v]))
+            continue;
+          const float keep = exp2f(m[v] - s[v]);  // 0 at the first
+          m[v] = s[v];
+          l[v] *= keep;
+#pragma unroll
+          for (int i = 0; i < kPairs; i++)
+            acc[v][i] = f2_mul(acc[v][i], f2_pack(keep, keep));
+        }
+      }
+      const bool all = in && position <= p.start;  // every row sees it
+#pragma unroll
+      for (int v = 0; v < kVecs; v++) {
+        const bool seen = all || position < limit[v];
+        s[v] = s[v] == -INFINITY ? 0.0f : exp2f((s[v] - m[v]) - guard);
+        l[v] += s[v];
+        // What a row does not see may be anything: its product is left out, not made with a weight of zero.
+        if (in && seen) {
+#pragma unroll
+          for (int i = 0; i < kPairs; i++)
+            acc[v][i] = f2_fma(f2_pack(s[v], s[v]), x.pair(i), acc[v][i]);
+        }
+      }
+    }
+    // The lane groups' results, then the warps'.
+#pragma unroll
+    for (int v = 0; v < kVecs; v++) {
+      float top = m[v];
+#pragma unroll
+      for (int o = 16; o >= LANES; o >>= 1)
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float f = m[v] == -INFINITY ? 0.0f : exp2f(m[v] - top);
+      float sum = l[v] * f;
+#pragma unroll
+      for (int o = 16; o >= LANES; o >>= 1)
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0)
+        wm[warp][v] = top, wl[warp][v] = sum;
+#pragma unroll
+      for (int i = 0; i < kPairs; i++) {
+        float lo, hi;
+        f2_unpack(f2_mul(acc[v][i], f2_pack(f, f)), lo, hi);
+#pragma unroll
+        for (int o = 16; o >= LANES; o >>= 1)
+          lo += __shfl_xor_sync(0xffffffffu, lo, o), hi += __shfl_xor_sync(0xffffffffu, hi, o);
+        if (at == 0) {
+          sums[warp][v][Row<T, LANES, WIDE>::element(sub, 2 * i)] = lo;
+          sums[warp][v][Row<T, LANES, WIDE>::element(sub, 2 * i + 1)] = hi;
+        }
+      }
+    }
+    __syncthreads();
+    if (t < kVecs) {
+      float top = -INFINITY, sum = 0.0f;
+      for (int w = 0; w < kWarps; w++)
+        top = fmaxf(top, wm[w][t]);
+      for (int w = 0; w < kWarps; w++) {
+        const float f = wm[w][t] == -INFINITY ? 0.0f : exp2f(wm[w][t] - top);
+        sum += wl[w][t] * f;
+        wl[w][t] = f;
+      }
+      m_all[t] = top, l_all[t] = sum;
+    }
+    __syncthreads();
+    float *o = &sums[0][0][0];  // [vecs][hd], over the first warps' sums once they are read
+    for (int v = 0; v < p.vecs; v++) {
+      float x[kMaxHd / kThreads];
+#pragma unroll
+      for (int j = 0; j < kMaxHd / kThreads; j++) {
+        const int e = t + j * kThreads;
+        x[j] = 0.0f;
+        if (e < hd)
+          for (int w = 0; w < kWarps; w++)
+            x[j] = fmaf(wl[w][v], sums[w][v][e], x[j]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kMaxHd / kThreads; j++)
+        if (t + j * kThreads < hd)
+          o[v * hd + t + j * kThreads] = x[j];
+      __syncthreads();
+    }
+    finish(a, &range, p, m_all, l_all, o, &bad, &last);
+    if (t == 0)
+      bad = 0;
+    __syncthreads();
+  }
+}
+
+bool heads_ok(int n_heads, int n_kv, int hd, int batch, int rows) {
+  constexpr long long most = 1 << 24;  // vectors; the product of two of the numbers does not wrap
+  return n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && hd > 0 && hd <= kMaxHd && batch > 0 && rows > 0 &&
+         (long long)batch * rows <= most && (long long)batch * rows * n_heads <= most;
+}
+
+const char *cache_fault(const PagedCache *c, int n_kv, int hd) {
+  if (!c || !c->key || !c->value || !c->table)
+    return "missing keys, values or page table";
+  if (c->type != K_F32 && c->type != K_BF16 && c->type != K_F16)
+    return "invalid cache type";
+  if (c->pages <= 0 || c->page_size <= 0 || c->max_pages <= 0 ||
+      (long long)c->max_pages * c->page_size > kMaxPositions)
+    return "invalid pages";
+  if (c->page_stride / hd / n_kv < (size_t)c->page_size || c->page_stride > ((size_t)1 << 62) / c->pages)
+    return "invalid page stride";
+  return nullptr;
+}
+
+template <typename T, int LANES>
+cudaError_t launch_rows(const PagedArgs &a, bool wide) {
+  return wide ? kc_launch_pdl(paged_rows_kernel<T, LANES, true>, dim3(kCtas), dim3(kThreads), 0, kc_stream(), a)
+              : kc_launch_pdl(paged_rows_kernel<T, LANES, false>, dim3(kCtas), dim3(kThreads), 0, kc_stream(), a);
+}
+template <typename T>
+cudaError_t launch_rows_of(const PagedArgs &a) {
+  const bool wide = a.hd * sizeof(T) % 16 == 0 && a.page_stride * sizeof(T) % 16 == 0 &&
+                    !(((uintptr_t)a.key | (uintptr_t)a.value) & 15);
+  return a.hd <= 64 ? launch_rows<T, 4>(a, wide) : a.hd <= 128 ? launch_rows<T, 8>(a, wide) : launch_rows<T, 16>(a, wide);
+}
+
+int blocks_of(int n_heads, int n_kv, int rows, int block) {
+  return (int)(((long long)rows * (n_heads / n_kv) + block - 1) / block);
+}
+
+// Tickets first, to a whole number of 16 bytes, then the slots. A ticket for every query vector: enough for the segments
+// of any batch of as many rows, whatever its KV heads.
+size_t ticket_bytes(int n_heads, int batch, int rows) {
+  return ((size_t)batch * rows * n_heads * sizeof(unsigned) + 15) & ~(size_t)15;
+}
+
+}  // namespace
+
+extern "C" {
+
+void k_rope_kv_store_paged(float *q_out, size_t q_out_ld, const float *q, size_t q_ld, const float *k, const float *v,
+                           size_t kv_ld, const PagedCache *cache, const float *rope, int seq_len, const int *starts,
+                           const int *counts, int n_heads, int n_kv_heads, int head_dim, int batch, int rows) {
+  const char *name = "k_rope_kv_store_paged";
+  if (batch == 0 || rows == 0)
+    return;
+  constexpr long long most = 0x7fffffff;
+  if (n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || head_dim % 2 || batch < 0 || rows < 0 || seq_len <= 0 ||
+      (long long)batch * rows > most || ((long long)n_heads + 2 * (long long)n_kv_heads) * head_dim > most ||
+      q_ld < (size_t)n_heads * head_dim || q_out_ld < (size_t)n_heads * head_dim ||
+      kv_ld < (size_t)n_kv_heads * head_dim) {
+    kc_fail("%s: invalid shape heads=%d/%d head_dim=%d batch=%d rows=%d seq_len=%d strides %zu, %zu, %zu", name, n_heads,
+            n_kv_heads, head_dim, batch, rows, seq_len, q_out_ld, q_ld, kv_ld);
+    return;
+  }
+  if (!q_out || !q || !k || !v || !rope || !starts) {
+    kc_fail("%s: missing queries, keys, values, rotation table or starts", name);
+    return;
+  }
+  if (const char *fault = cache_fault(cache, n_kv_heads, head_dim)) {
+    kc_fail("%s: %s", name, fault);
+    return;
+  }
+  if (q_out == q && q_out_ld != q_ld) {
+    kc_fail("%s: queries rotated in place need one row stride, not %zu and %zu", name, q_out_ld, q_ld);
+    return;
+  }
+  StoreArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q_out = q_out, a.q = q, a.k = k, a.v = v, a.rope = rope, a.key = cache->key, a.value = cache->value;
+  a.table = cache->table, a.starts = starts, a.counts = counts;
+  a.q_out_ld = (long long)q_out_ld, a.q_ld = (long long)q_ld, a.kv_ld = (long long)kv_ld;
+  a.page_stride = cache->page_stride, a.pages = cache->pages, a.page_size = cache->page_size;
+  a.max_pages = cache->max_pages, a.n_heads = n_heads, a.n_kv = n_kv_heads, a.hd = head_dim;
+  const int held = cache->max_pages * cache->page_size;
+  a.positions = held < seq_len ? held : seq_len;
+  a.batch = batch, a.rows = rows, a.per_row = (n_heads + 2 * n_kv_heads) * (head_dim / 2);
+  const long long ctas = ((long long)batch * rows * a.per_row + 255) / 256;
+  if (ctas > most) {
+    kc_fail("%s: %d requests of %d rows are too many for one call", name, batch, rows);
+    return;
+  }
+  const dim3 grid((unsigned)ctas), threads(256);
+  const cudaError_t e =
+      cache->type == K_F32 ? kc_launch_pdl(paged_store_kernel<float>, grid, threads, 0, kc_stream(), a)
+      : cache->type == K_BF16
+          ? kc_launch_pdl(paged_store_kernel<__nv_bfloat16>, grid, threads, 0, kc_stream(), a)
+          : kc_launch_pdl(paged_store_kernel<__half>, grid, threads, 0, kc_stream(), a);
+  if (e == cudaSuccess)
+    kc_count_launch();
+  else
+    kc_fail("%s: CUDA launch failed: %s", name, cudaGetErrorString(cudaGetLastError()));
+}
+
+size_t k_attention_paged_bytes(int n_heads, int n_kv_heads, int head_dim, int batch, int rows) {
+  if (!heads_ok(n_heads, n_kv_heads, head_dim, batch, rows))
+    return 0;
+  return ticket_bytes(n_heads, batch, rows) + sizeof(float) * 2 * kCtas * slot_size(kVecs, head_dim);
+}
+
+void k_attention_paged_init(AttentionWork *work, int n_heads, int n_kv_heads, int head_dim, int batch, int rows,
+                            void *memory) {
+  const char *name = "k_attention_paged_init";
+  const size_t bytes = k_attention_paged_bytes(n_heads, n_kv_heads, head_dim, batch, rows);
+  memset(work, 0, sizeof(*work));
+  if (!bytes) {
+    kc_fail("%s: invalid shape", name);
+    return;
+  }
+  if ((uintptr_t)memory & 15) {
+    kc_fail("%s: the memory must be 16-byte aligned", name);
+    return;
+  }
+  void *base = memory;
+  if (!base && cudaMalloc(&base, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    kc_fail("%s: cannot allocate %zu bytes of attention work", name, bytes);
+    return;
+  }
+  const cudaError_t e = cudaMemsetAsync(base, 0, ticket_bytes(n_heads, batch, rows), kc_stream());
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    if (!memory)
+      cudaFree(base);
+    kc_fail("%s: %s", name, cudaGetErrorString(e));
+    return;
+  }
+  work->partial = static_cast<float *>(base);
+  work->max_chunks = -1;
+  work->n_heads = n_heads;
+  work->head_dim = head_dim;
+  work->workers = batch * rows;
+  work->external = memory != nullptr;
+  work->capacity = bytes / sizeof(float);
+}
+
+void k_attention_paged_rows(float *out, int8_t *oq, float *os, const float *q, const PagedCache *cache, const int *starts,
+                            const int *counts, AttentionWork *work, int n_heads, int n_kv_heads, int head_dim, int batch,
+                            int rows, int gs) {
+  const char *name = "k_attention_paged_rows";
+  if (batch == 0 || rows == 0)
+    return;
+  if (!heads_ok(n_heads, n_kv_heads, head_dim, batch, rows)) {
+    kc_fail("%s: invalid shape heads=%d/%d head_dim=%d batch=%d rows=%d", name, n_heads, n_kv_heads, head_dim, batch, rows);
+    return;
+  }
+  if (!out || !q || !starts || (oq && !os)) {
+    kc_fail("%s: missing output, queries or starts", name);
+    return;
+  }
+  if (const char *fault = cache_fault(cache, n_kv_heads, head_dim)) {
+    kc_fail("%s: %s", name, fault);
+    return;
+  }
+  if (oq && (gs <= 0 || head_dim % gs)) {
+    kc_fail("%s: group size %d does not divide the head's %d outputs", name, gs, head_dim);
+    return;
+  }
+  if (!work || !work->partial || work->max_chunks != -1 || work->n_heads != n_heads || work->head_dim != head_dim ||
+      (long long)batch * rows > work->workers ||
+      k_attention_paged_bytes(n_heads, n_kv_heads, head_dim, batch, rows) > work->capacity * sizeof(float)) {
+    kc_fail("%s: the attention work is missing or too small for this shape", name);
+    return;
+  }
+  PagedArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = q, a.key = cache->key, a.value = cache->value, a.table = cache->table, a.starts = starts, a.counts = counts;
+  a.out = out, a.oq = oq, a.os = os;
+  a.page_stride = cache->page_stride, a.pages = cache->pages, a.max_pages = cache->max_pages;
+  a.page_size = cache->page_size, a.positions = cache->max_pages * cache->page_size;
+  a.n_heads = n_heads, a.n_kv = n_kv_heads, a.group = n_heads / n_kv_heads, a.hd = head_dim;
+  a.batch = batch, a.rows = rows, a.gs = gs;
+  a.block = kVecs, a.blocks = blocks_of(n_heads, n_kv_heads, rows, kVecs);
+  a.slot_floats = slot_size(kVecs, head_dim);
+  a.by_page = divisor(a.page_size), a.by_group = divisor(a.group);
+  a.tickets = reinterpret_cast<unsigned *>(work->partial);
+  // The tickets' room is the work's own, so that it does not move between calls of different batches.
+  a.partial = work->partial + (work->capacity - (size_t)2 * kCtas * a.slot_floats);
+  const cudaError_t e = cache->type == K_F32    ? launch_rows_of<float>(a)
+                        : cache->type == K_BF16 ? launch_rows_of<__nv_bfloat16>(a)
+                                                : launch_rows_of<__half>(a);
+  if (e == cudaSuccess)
+    kc_count_launch();
+  else
+    kc_fail("%s: CUDA launch failed: %s", name, cudaGetErrorString(cudaGetLastError()));
+}
+
+}  // extern "C"

@@ -1,0 +1,663 @@
+// Attention over a paged cache on the tensor cores: 16-bit keys and values, head_dim 64 or 128, 16-byte aligned pages.
+//
+// The positions are the rows of both products, so that a decode step's few query vectors cost no padding to 128 and the
+// cache's bytes go from global memory to the tensor core as they are: for a tile of 128 positions
+//   S^T [128 positions x N] = K [128 x hd] Q^T,    O^T [hd x N] = V^T [hd x 128 positions] P^T,
+// K the K-major and V the MN-major operand A of the same row-major layout (128-byte swizzle), Q and P the operand B.
+// The 16-bit types are widened by columns: a query vector takes three of the N columns, x = x0 + x1 + x2 in three 16-bit
+// parts, and so does a vector of probabilities; the products of a 16-bit key or value with each part are exact, their sum
+// is the fp32 product up to 2^-24 of it.
+//   bf16: the parts are the leading, middle and last eight bits of the significand, cut off, not rounded: no part's
+//         rounding carries into the one before, and they add up to x exactly. bf16 has fp32's exponents.
+//   fp16: x 2^k with the largest magnitude of a query vector just below 2^15 (probabilities: 2^15 at most), then each part
+//         rounded and the rest times 2^11 for the next, so that a part of a small x is not lost below fp16's exponents; the
+//         columns are joined with 2^-11 and 2^-22.
+// A tile's sums are a product of their own, eight MMAs that start at zero; they join the running sums in fp32, in
+// registers, rounded to nearest (the tensor cores' accumulators cut towards zero).
+//
+// A CTA per SM takes its share of the tiles of all segments without a pause between segments. Warps 0-3: softmax, a
+// thread per position of a tile and per element of the head of its sums; 4: issues the MMAs; 5: lays out the next
+// segment's queries; 6-9: copy the tiles, asynchronously, through a ring of stages.
+//
+// What differs between the rows of a request's drafts, the positions behind the first row's, is not in the tiles (their
+// positions end where the block's first row's do): a later draft's key or value of any kind must not reach the rows before
+// it, not even with a weight of zero. Those few products are made in fp32 at the beginning of the segment's last piece.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+using namespace paged;
+
+constexpr int kTile = 128;  // positions
+constexpr int kSoft = 128;  // softmax threads
+constexpr int kCopyWarps = 4;
+constexpr int kThreads = kSoft + 32 + 32 + 32 * kCopyWarps;
+constexpr int kCtas = 148;
+constexpr int kMaxBlock = 32;
+constexpr int kSmem = 227 * 1024;
+
+struct Tail {
+  uint64_t full[10], empty[10], sfull[2], pfull[2], ofull[2], qfull[2], qempty[2], drained;
+  uint32_t tmem;
+  int abort_flag, bad, last;
+  Range range;
+  __align__(16) float top[2][4][kMaxBlock];  // a tile's maxima by warp
+  // Of the queries: four pieces, since the softmax may be two tiles behind the scores, and the queries two pieces ahead.
+  float qscale[4][kMaxBlock];
+};
+
+template <int HD, int BLOCK>
+struct Layout {
+  static constexpr int n = (3 * BLOCK + 15) / 16 * 16;  // columns
+  static constexpr int entry = kTile * HD * 2;
+  static constexpr int q_bytes = n * HD * 2, p_bytes = n * kTile * 2;
+  static constexpr int fit = (kSmem - 1024 - 2 * (q_bytes + p_bytes) - (int)sizeof(Tail)) / entry;
+  static constexpr int stages = fit > 10 ? 10 : HD == 128 && fit > 6 ? 6 : fit;
+  static constexpr int ahead = stages - 2;  // copies in flight: the consumer may need the two before them
+  static constexpr int q_at = stages * entry, p_at = q_at + 2 * q_bytes, tail_at = p_at + 2 * p_bytes;
+  static constexpr int total = tail_at + (int)sizeof(Tail) + 1024;
+  static constexpr int tmem = 4 * n <= 64 ? 64 : 4 * n <= 128 ? 128 : 4 * n <= 256 ? 256 : 512;
+  static_assert(ahead >= 1 && total <= kSmem, "shared memory");
+  static_assert(2 * p_bytes >= BLOCK * HD * 4, "the sums' room, over the probabilities'");
+  static_assert(2 * p_bytes >= BLOCK * BLOCK * 4 + 2 * BLOCK * HD * 2, "the drafts' room, over the probabilities'");
+};
+
+__device__ __forceinline__ bool tc_wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    ok = *abort_flag == 0;
+    if (ok && !mbar_wait_sleep_bounded(bar, parity)) {
+      *abort_flag = 1;
+      ok = false;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+// kind::f16, fp32 accumulators, fp16 or bf16 operands, A K-major or MN-major, B K-major, M x N.
+__host__ __device__ constexpr uint32_t umma_idesc(bool bf16, int m, int n, bool a_mn) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((a_mn ? 1u : 0u) << 15) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+// MN-major operand in the 128-byte swizzle: rows of 64 values along M, 8 rows (K) to an atom of 1 KiB; atoms 1 KiB apart
+// along K, `m_bytes` apart along M.
+__device__ __forceinline__ uint64_t umma_desc_sw128_mn(const void *smem_tile, uint32_t m_bytes) {
+  uint64_t d = (smem_u32(smem_tile) >> 4) & 0x3FFFull;
+  d |= (uint64_t)(m_bytes >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The largest of the warp's numbers.
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^k for -126 <= k <= 127.
+__device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) << 23); }
+
+// The 16 bits of each of a number's three parts (fp16: of a number already brought to fp16's range).
+template <typename T>
+struct Parts {
+  unsigned short part[3];
+};
+__device__ __forceinline__ Parts<__nv_bfloat16> split(float x, __nv_bfloat16) {
+  Parts<__nv_bfloat16> p;
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+    const unsigned bits = __float_as_uint(x);
+    p.part[i] = (unsigned short)(bits >> 16);
+    x -= __uint_as_float(bits & 0xffff0000u);  // exact
+  }
+  return p;
+}
+__device__ __forceinline__ Parts<__half> split(float x, __half) {
+  Parts<__half> p;
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+    const __half h = __float2half_rn(x);
+    p.part[i] = __half_as_ushort(h);
+    x = (x - __half2float(h)) * 2048.0f;  // exact
+  }
+  return p;
+}
+template <typename T>
+__device__ __forceinline__ float join(float x0, float x1, float x2) {
+  return __is_same(T, __half) ? fmaf(fmaf(x2, 0x1p-11f, x1), 0x1p-11f, x0) : (x2 + x1) + x0;
+}
+__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
+
+// 16 bytes from global to shared memory, asynchronously; zeros without `in`.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// This thread's lane of 4 or 8 columns.
+__device__ __forceinline__ void tmem_ld4(uint32_t at, float (&x)[4]) {
+  uint32_t r[4];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at));
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    x[j] = __uint_as_float(r[j]);
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t at, float *x) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(at));
+#pragma unroll
+  for (int j = 0; j < 8; j++)
+    x[j] = __uint_as_float(r[j]);
+}
+// The joined columns of this thread's lane: part p of vector v is column p * BLOCK + v. Eight
+// vectors at a time, so that three parts fit the registers.
+template <typename T, int BLOCK>
+__device__ __forceinline__ void tmem_joined(uint32_t at, float (&x)[BLOCK]) {
+  if constexpr (BLOCK == 4) {
+    float p[3][4];
+#pragma unroll
+    for (int i = 0; i < 3; i++)
+      tmem_ld4(at + 4 * i, p[i]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int v = 0; v < 4; v++)
+      x[v] = join<T>(p[0][v], p[1][v], p[2][v]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < BLOCK; c += 8) {
+      float p[3][8];
+#pragma unroll
+      for (int i = 0; i < 3; i++)
+        tmem_ld8(at + BLOCK * i + c, p[i]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int v = 0; v < 8; v++)
+        x[c + v] = join<T>(p[0][v], p[1][v], p[2][v]);
+    }
+  }
+}
+
+// The first row of a piece's block, and how many rows it has beyond that.
+struct Rows {
+  int first, more;
+};
+__device__ __forceinline__ Rows rows_of(const PagedArgs &a, const Piece &p) {
+  int lo = p.block * a.block, hi = lo + p.vecs - 1;
+  Rows r;
+  r.first = divide(lo, a.by_group);
+  r.more = divide(hi, a.by_group) - r.first;
+  return r;
+}
+
+// Row of the cache that holds a position, in elements, or -1 where its page is none.
+__device__ __forceinline__ long long place_of(const PagedArgs &a, const Piece &p, int position, int hd) {
+  int within = position;
+  const int index = divide(within, a.by_page);
+  const int page = a.table[(size_t)p.b * a.max_pages + index];
+  return page < 0 || page >= a.pages
+             ? -1
+             : (long long)((size_t)page * a.page_stride + ((size_t)p.head * a.page_size + within) * hd);
+}
+
+template <typename T, int HD, int BLOCK>
+__global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a) {
+  using L = Layout<HD, BLOCK>;
+  constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  Tail *t = reinterpret_cast<Tail *>(smem + L::tail_at);
+  volatile int *abort_flag = &t->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (!find_range(a, kTile, &t->range))
+    return;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::stages; i++) {
+      mbar_init(&t->full[i], kCopyWarps);
+      mbar_init(&t->empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&t->sfull[i], 1);
+      mbar_init(&t->pfull[i], kSoft / 32);
+      mbar_init(&t->ofull[i], 1);
+      mbar_init(&t->qfull[i], 1);
+      mbar_init(&t->qempty[i], 1);
+    }
+    mbar_init(&t->drained, 1);
+    t->abort_flag = 0;
+    t->bad = 0;
+    fence_mbar_init();
+  }
+  if (warp == kSoft / 32)
+    tmem_alloc(&t->tmem, L::tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = t->tmem;
+  const Range *range = &t->range;
+  const float scale = rsqrtf((float)HD) * kLog2e;
+  Walk walk(a, range, kTile);
+  Piece p;
+
+  if (warp >= kSoft / 32 + 2) {
+    // ---- copies: warp w of them the rows 32 w .. 32 w + 31 of every tile, keys and values in turn ----
+    constexpr int kChunks = HD / 8, kAt = 32 / kChunks;  // 16-byte units of a row, rows of a warp's instruction
+    const int w = warp - kSoft / 32 - 2;
+    const int chunk = lane % kChunks, sub = lane / kChunks;
+    const uint32_t base = smem_u32(smem) + (chunk >> 3) * (kTile * 128);
+    int slot = 0, signal = 0;
+    unsigned parity = 1, entries = 0;
+    auto done = [&]() {  // the oldest entry not yet handed over is in memory
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&t->full[signal]);
+      signal = signal + 1 == L::stages ? 0 : signal + 1;
+    };
+    while (walk.next(a, range, kTile, &p)) {
+      const int common = p.start + rows_of(a, p).first + 1;  // positions that every row of the block sees
+      int position = p.t0 * kTile + 32 * w + lane;
+      long long next = position < common ? place_of(a, p, position, HD) : -1;
+      for (int j = p.t0; j < p.t1; j++) {
+        const long long place = next;
+        position += kTile;
+        next = j + 1 < p.t1 && position < common ? place_of(a, p, position, HD) : -1;
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+          const T *from = static_cast<const T *>(kv ? a.value : a.key) + chunk * 8;
+          tc_wait(&t->empty[slot], parity, abort_flag);
+#pragma unroll
+          for (int i = 0; i < 32 / kAt; i++) {
+            const int r = i * kAt + sub;
+            const long long at = __shfl_sync(0xffffffffu, place, r);
+            const int row = 32 * w + r;
+            copy16(base + slot * L::entry + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), from + max(at, 0ll), at >= 0);
+          }
+          copy_commit();
+          slot++;
+          if (slot == L::stages)
+            slot = 0, parity ^= 1;
+          if (++entries > L::ahead) {
+            copy_wait<L::ahead>();
+            done();
+          }
+        }
+      }
+    }
+    copy_wait<0>();
+    for (int i = min(entries, (unsigned)L::ahead); i > 0; i--)
+      done();
+  } else if (warp == kSoft / 32 + 1) {
+    // ---- queries: times the scores' scale, in three parts, row part * BLOCK + v of the operand ----
+    constexpr int kEach = HD / 32;
+    for (int n = 0; walk.next(a, range, kTile, &p); n++) {
+      uint8_t *to = smem + L::q_at + (n & 1) * L::q_bytes;
+      if (n >= 2)
+        tc_wait(&t->qempty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag);
+#pragma unroll
+      for (int v0 = 0; v0 < BLOCK; v0 += 4) {
+        float x[4][kEach];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          int row;
+          const float *q = a.q + (size_t)vector_at(a, p, min(v0 + u, p.vecs - 1), &row) * HD;
+#pragma unroll
+          for (int i = 0; i < kEach; i++)
+            x[u][i] = v0 + u < p.vecs ? q[lane + 32 * i] * scale : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const int v = v0 + u;
+          if (!kBf16) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kEach; i++)
+              mx = fmaxf(mx, fabsf(x[u][i]));
+            const int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)) >> 23) - 127;
+            const int k = min(14 - e, 100);  // so that its inverse is a normal number
+#pragma unroll
+            for (int i = 0; i < kEach; i++)
+              x[u][i] *= pow2(k);
+            if (lane == 0)
+              t->qscale[n & 3][v] = pow2(-k);
+          }
+#pragma unroll
+          for (int i = 0; i < kEach; i++) {
+            const Parts<T> parts = split(x[u][i], T(0.0f));
+            const int e = lane + 32 * i;
+#pragma unroll
+            for (int part = 0; part < 3; part++) {
+              const int row = part * BLOCK + v;
+              *reinterpret_cast<unsigned short *>(to + (e >> 6) * (L::n * 128) + row * 128 +
+                                                  ((((e & 63) >> 3) ^ (row & 7)) << 4) + (e & 7) * 2) = parts.part[part];
+            }
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&t->qfull[n & 1]);
+    }
+  } else if (warp == kSoft / 32) {
+    // ---- MMA issue: the scores of tile j + 1 before the sums of tile j, so that they run under its softmax. MMAs run in
+    // the order of issue. S and O have two buffers each; that a buffer was read is known from the probabilities of a later
+    // tile (the softmax reads the scores of a tile before it writes its probabilities, and the sums of the tile before the
+    // last by then). ----
+    const bool leader = elect_one();
+    constexpr uint32_t idesc_s = umma_idesc(kBf16, kTile, L::n, false), idesc_o = umma_idesc(kBf16, HD, L::n, true);
+    const uint64_t kdesc = umma_desc_sw128(smem), vdesc = umma_desc_sw128_mn(smem, kTile * 128);
+    const uint64_t qdesc = umma_desc_sw128(smem + L::q_at), pdesc = umma_desc_sw128(smem + L::p_at);
+    const int tiles = (int)(range->hi - range->lo);
+    int piece = -1, left = 0;  // of the scores issued next: its piece, and tiles of it left
+    int kslot = 0, vslot = 1;
+    unsigned kpar = 0, vpar = 0;
+    auto scores = [&](int j) {
+      if (!left) {
+        walk.next(a, range, kTile, &p);
+        left = p.t1 - p.t0;
+        piece++;
+        if (!tc_wait(&t->qfull[piece & 1], (piece >> 1) & 1, abort_flag))
+          return false;
+      }
+      left--;
+      if (!tc_wait(&t->full[kslot], kpar, abort_flag))
+        return false;
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++)
+          umma_f16(tmem + L::n * (j & 1), kdesc + (kslot * L::entry + (c >> 2) * (kTile * 128) + 32 * (c & 3)) / 16,
+                   qdesc + ((piece & 1) * L::q_bytes + (c >> 2) * (L::n * 128) + 32 * (c & 3)) / 16, idesc_s, c);
+        umma_commit(&t->sfull[j & 1]);
+        umma_commit(&t->empty[kslot]);
+        if (!left)
+          umma_commit(&t->qempty[piece & 1]);
+      }
+      __syncwarp();
+      kslot += 2;
+      if (kslot >= L::stages)
+        kslot -= L::stages, kpar ^= 1;
+      return true;
+    };
+    bool ok = scores(0);
+    for (int j = 0; ok && j < tiles; j++) {
+      if (j + 1 < tiles && !scores(j + 1))
+        break;
+      if (!tc_wait(&t->full[vslot], vpar, abort_flag) || !tc_wait(&t->pfull[j & 1], (j >> 1) & 1, abort_flag))
+        break;
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int c = 0; c < kTile / 16; c++)
+          umma_f16(tmem + L::n * (2 + (j & 1)), vdesc + (vslot * L::entry + 2048 * c) / 16,
+                   pdesc + ((j & 1) * L::p_bytes + (c >> 2) * (L::n * 128) + 32 * (c & 3)) / 16, idesc_o, c);
+        umma_commit(&t->ofull[j & 1]);
+        umma_commit(&t->empty[vslot]);
+      }
+      __syncwarp();
+      vslot += 2;
+      if (vslot >= L::stages)
+        vslot -= L::stages, vpar ^= 1;
+    }
+    // No MMA is under way when the tensor memory is given back, whatever ended the loop.
+    if (leader)
+      umma_commit(&t->drained);
+    __syncwarp();
+    mbar_wait_sleep_bounded(&t->drained, 0);
+  } else {
+    // ---- softmax ----
+    const int tid = threadIdx.x;  // a position of the tile; of the sums, an element of the head
+    const uint32_t quadrant = tmem + ((uint32_t)(32 * warp) << 16);
+    // M = 64 keeps 16 rows in each quadrant of the tensor memory.
+    const int element = HD == 128 ? tid : 16 * warp + lane;
+    const bool has_element = HD == 128 || lane < 16;
+    uint8_t *const prow = smem + L::p_at + (tid >> 6) * (L::n * 128) + (tid & 7) * 2;
+    const int pchunk = (tid & 63) >> 3;
+    int j = 0;
+    for (int n = 0; walk.next(a, range, kTile, &p); n++) {
+      const Rows rows = rows_of(a, p);
+      const int common = p.start + rows.first + 1;
+      float m[BLOCK], l[BLOCK], acc[BLOCK];
+#pragma unroll
+      for (int v = 0; v < BLOCK; v++)
+        m[v] = -INFINITY, l[v] = 0.0f, acc[v] = 0.0f;
+      // Weights: bf16 as guard_of says, fp16 up to 2^15 (there is no value beyond 2^16).
+      const float weight = kBf16 ? guard_of(p.start + p.count) : 0x1p15f;
+      // Every page of the piece's positions is one.
+      {
+        int from = p.t0 * kTile, to = min(p.t1 * kTile, p.start + p.count) - 1;
+        from = divide(from, a.by_page), to = divide(to, a.by_page);
+        bool bad = false;
+        for (int i = from + tid; i <= to; i += kSoft) {
+          const int page = a.table[(size_t)p.b * a.max_pages + i];
+          bad |= page < 0 || page >= a.pages;
+        }
+        if (bad)
+          t->bad = 1;
+      }
+      if (rows.more && p.t1 == p.tiles) {
+        // The drafts' own positions, common .. common + more - 1; row first + r sees the first r of them.
+        T *kd = reinterpret_cast<T *>(smem + L::p_at), *vd = kd + BLOCK * HD;
+        float *sd = reinterpret_cast<float *>(vd + BLOCK * HD);  // [more][BLOCK]
+        constexpr int kUnits = HD / 8;
+        for (int i = tid; i < rows.more * kUnits; i += kSoft) {
+          const int r = i / kUnits, u = i % kUnits;
+          const long long at = place_of(a, p, common + r, HD);
+          const uint4 zero = make_uint4(0, 0, 0, 0);
+          reinterpret_cast<uint4 *>(kd)[i] =
+              at < 0 ? zero : *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.key) + at + 8 * u);
+          reinterpret_cast<uint4 *>(vd)[i] =
+              at < 0 ? zero : *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.value) + at + 8 * u);
+        }
+        meet<kSoft, 1>();
+        for (int v0 = 4 * warp; v0 < p.vecs; v0 += 16) {  // four vectors of a warp at a time
+          float q[4][HD / 32];
+          int row[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            const float *from = a.q + (size_t)vector_at(a, p, min(v0 + u, p.vecs - 1), &row[u]) * HD;
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++)
+              q[u][i] = from[lane + 32 * i] * scale;
+          }
+          for (int r = 0; r < rows.more; r++) {
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) {
+              const float k = widen(kd[r * HD + lane + 32 * i]);
+#pragma unroll
+              for (int u = 0; u < 4; u++)
+                s[u] = fmaf(q[u][i], k, s[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+#pragma unroll
+              for (int o = 16; o; o >>= 1)
+                s[u] += __shfl_xor_sync(0xffffffffu, s[u], o);
+              if (lane == 0 && v0 + u < BLOCK)
+                sd[r * BLOCK + v0 + u] = v0 + u < p.vecs && r < row[u] - rows.first ? s[u] : -INFINITY;
+            }
+          }
+        }
+        meet<kSoft, 1>();
+#pragma unroll
+        for (int v = 0; v < BLOCK; v++) {
+          if (v >= p.vecs)
+            continue;
+          int row;
+          vector_at(a, p, v, &row);
+          for (int r = 0; r < row - rows.first; r++)
+            m[v] = fmaxf(m[v], sd[r * BLOCK + v]);
+          for (int r = 0; r < row - rows.first; r++) {
+            const float w = ex2(sd[r * BLOCK + v] - m[v]) * weight;
+            l[v] += tid == 0 ? w : 0.0f;
+            if (has_element)
+              acc[v] = fmaf(w, widen(vd[r * HD + element]), acc[v]);
+          }
+        }
+        meet<kSoft, 1>();
+      }
+      for (int tile = p.t0; tile < p.t1; tile++, j++) {
+        float s[BLOCK], keep[BLOCK];
+        tc_wait(&t->sfull[j & 1], (j >> 1) & 1, abort_flag);
+        tc_fence_after();
+        tmem_joined<T, BLOCK>(quadrant + L::n * (j & 1), s);
+        tc_fence_before();
+        const bool in = tile * kTile + tid < common;
+        float (*top)[kMaxBlock] = t->top[j & 1];
+#pragma unroll
+        for (int v = 0; v < BLOCK; v++) {
+          if (!kBf16)
+            s[v] *= t->qscale[n & 3][v];
+          s[v] = in ? s[v] : -INFINITY;
+          const float x = warp_max(s[v]);
+          if (lane == 0)
+            top[warp][v] = x;
+        }
+        meet<kSoft, 1>();
+#pragma unroll
+        for (int v = 0; v < BLOCK; v++) {
+          const float x = fmaxf(fmaxf(fmaxf(top[0][v], top[1][v]), fmaxf(top[2][v], top[3][v])), m[v]);
+          keep[v] = x == -INFINITY ? 1.0f : ex2(m[v] - x);  // a tile behind the block's first row has nothing for it
+          m[v] = x;
+          const float w = in ? ex2(s[v] - x) * weight : 0.0f;
+          l[v] = fmaf(l[v], keep[v], w);
+          const Parts<T> parts = split(w, T(0.0f));
+#pragma unroll
+          for (int part = 0; part < 3; part++) {
+            const int row = part * BLOCK + v;
+            *reinterpret_cast<unsigned short *>(prow + (j & 1) * L::p_bytes + row * 128 + ((pchunk ^ (row & 7)) << 4)) =
+                parts.part[part];
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&t->pfull[j & 1]);
+        if (tile > p.t0) {
+          const int i = j - 1;
+          float o[BLOCK];
+          tc_wait(&t->ofull[i & 1], (i >> 1) & 1, abort_flag);
+          tc_fence_after();
+          tmem_joined<T, BLOCK>(quadrant + L::n * (2 + (i & 1)), o);
+          tc_fence_before();
+#pragma unroll
+          for (int v = 0; v < BLOCK; v++)
+            acc[v] += o[v];
+        }
+#pragma unroll
+        for (int v = 0; v < BLOCK; v++)
+          acc[v] *= keep[v];
+      }
+      {
+        const int i = j - 1;
+        float o[BLOCK];
+        tc_wait(&t->ofull[i & 1], (i >> 1) & 1, abort_flag);
+        tc_fence_after();
+        tmem_joined<T, BLOCK>(quadrant + L::n * (2 + (i & 1)), o);
+        tc_fence_before();
+#pragma unroll
+        for (int v = 0; v < BLOCK; v++)
+          acc[v] += o[v];
+      }
+      // The piece's result. Its last product is done, so the probabilities' room is free.
+      float *sums = reinterpret_cast<float *>(smem + L::p_at), (*part)[kMaxBlock] = t->top[j & 1];
+      float *m_all = t->top[(j & 1) ^ 1][0], *l_all = t->top[(j & 1) ^ 1][1];  // once the last tile's maxima are read
+#pragma unroll
+      for (int v = 0; v < BLOCK; v++) {
+        if (has_element && v < p.vecs)
+          sums[v * HD + element] = acc[v];
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+          l[v] += __shfl_xor_sync(0xffffffffu, l[v], o);
+        if (lane == 0)
+          part[warp][v] = l[v];
+      }
+      if (*abort_flag)
+        t->bad = 1;
+      meet<kSoft, 1>();
+      if (tid < p.vecs)
+        l_all[tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+#pragma unroll
+      for (int v = 0; v < BLOCK; v++)
+        if (tid == v)
+          m_all[v] = m[v];
+      meet<kSoft, 1>();
+      finish<kSoft, 1>(a, range, p, m_all, l_all, sums, &t->bad, &t->last);
+      if (tid == 0)
+        t->bad = 0;
+      meet<kSoft, 1>();
+    }
+  }
+  __syncthreads();
+  if (warp == kSoft / 32) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::tmem);
+  }
+}
+
+template <typename T, int HD, int BLOCK>
+cudaError_t launch(const PagedArgs &a) {
+  const auto kernel = paged_tc_kernel<T, HD, BLOCK>;
+  const cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(kernel), Layout<HD, BLOCK>::total);
+  return e != cudaSuccess
+             ? e
+             : kc_launch_pdl(kernel, dim3(kCtas), dim3(kThreads), Layout<HD, BLOCK>::total, kc_stream(), a);
+}
+template <typename T, int HD>
+cudaError_t launch_block(const PagedArgs &a) {
+  return a.block == 4    ? launch<T, HD, 4>(a)
+         : a.block == 8  ? launch<T, HD, 8>(a)
+         : a.block == 16 ? launch<T, HD, 16>(a)
+                         : launch<T, HD, kMaxBlock>(a);
+}
+
+}  // namespace
+
+bool kc_paged_tc_ok(const PagedArgs &a, int type) {
+  return (type == K_BF16 || type == K_F16) && (a.hd == 64 || a.hd == 128) && a.page_stride % 8 == 0 &&
+         !(((uintptr_t)a.key | (uintptr_t)a.value) & 15);
+}
+
+// The smallest block that holds a KV head's vectors, or the largest.
+int kc_paged_tc_block(int group, int rows) {
+  const long long vecs = (long long)group * rows;
+  return vecs <= 4 ? 4 : vecs <= 8 ? 8 : vecs <= 16 ? 16 : kMaxBlock;
+}
+
+int kc_paged_tc_slots_floats(int hd) { return 2 * kCtas * slot_size(kMaxBlock, hd); }
+
+cudaError_t kc_launch_paged_tc(const PagedArgs &a, int type) {
+  if (type == K_BF16)
+    return a.hd == 128 ? launch_block<__nv_bfloat16, 128>(a) : launch_block<__nv_bfloat16, 64>(a);
+  return a.hd == 128 ? launch_block<__half, 128>(a) : launch_block<__half, 64>(a);
+}

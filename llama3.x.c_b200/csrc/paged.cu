@@ -158,16 +158,17 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedArgs a)
   __shared__ __align__(16) float sums[kWarps][kVecs][LANES * kElems];
   __shared__ float wm[kWarps][kVecs], wl[kWarps][kVecs], m_all[kVecs], l_all[kVecs];
   __shared__ int bad, last;
+  __shared__ long long range_sums[kWarps];
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, sub = lane % LANES, at = lane / LANES;
   pdl_wait();
   pdl_launch_dependents();
   if (t == 0)
     bad = 0;
-  if (!find_range(a, kTile, &range))
+  if (!find_range(a, kTile, &range, range_sums))
     return;
   const int hd = a.hd;
   const float scale = rsqrtf((float)hd) * kLog2e;
-  Walk walk(a, &range, kTile);
+  Walk walk(&range);
   Piece p;
   while (walk.next(a, &range, kTile, &p)) {
     uint64_t q[kVecs][kPairs], acc[kVecs][kPairs];

@@ -47,13 +47,6 @@ struct PagedArgs {
 // Slots: a flag (4 floats), m and l of each vector, then their sums.
 __host__ __device__ __forceinline__ int slot_size(int block, int hd) { return (4 + 2 * block + block * hd + 3) & ~3; }
 
-constexpr int kRangeThreads = 320;  // at most
-struct Range {
-  long long lo, hi, total, before;  // this CTA's tiles, all tiles, those before request b
-  int b, ctas;
-  long long sums[kRangeThreads / 32];
-};
-
 // Tiles of a request's segments (of each one), and how many segments it has.
 struct Shape {
   int tiles, segments, blocks;
@@ -66,16 +59,40 @@ __device__ __forceinline__ Shape shape_of(const PagedArgs &a, const Request &r, 
   return s;
 }
 
-// This CTA's share of the tiles, and the request in which it begins. All threads call it. False: nothing to do.
-__device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *range) {
+// The shares of the tiles: `each` to a CTA, one more to the first `longer`. This CTA's are [lo, hi); request b, with
+// `before` tiles before its own, holds the first of them.
+struct Range {
+  long long lo, hi, each, longer, before;
+  Request request;
+  Shape shape;
+  int b;
+};
+
+// n / d where either is small more often than not.
+__device__ __forceinline__ long long quotient(long long n, long long d) {
+  return ((n | d) >> 32) == 0 ? (long long)((unsigned)n / (unsigned)d) : n / d;
+}
+
+// The CTA whose share holds tile x.
+__device__ __forceinline__ int owner(const Range *range, long long x) {
+  const long long edge = range->longer * (range->each + 1);
+  return (int)(x < edge ? quotient(x, range->each + 1) : range->longer + quotient(x - edge, range->each));
+}
+
+// This CTA's share of the tiles, and the request in which it begins. All threads call it; `sums` has room for a number a
+// warp. False: nothing to do.
+__device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *range, long long *sums) {
   const int threads = blockDim.x, t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int per = (a.batch + threads - 1) / threads, b0 = t * per, b1 = min(a.batch, b0 + per);
+  const int per = a.batch <= threads ? 1 : (a.batch + threads - 1) / threads;
+  const int b0 = min(a.batch, t * per), b1 = min(a.batch, b0 + per);
   long long own = 0;
+  Request r = {0, 0, false};
+  Shape s = {0, 0, 1};
   for (int b = b0; b < b1; b++) {
-    const Request r = request_of(a.starts, a.counts, b, a.rows, a.positions);
+    r = request_of(a.starts, a.counts, b, a.rows, a.positions);
     if (r.bad && blockIdx.x == 0)
       kc_raise(KC_ERR_BAD_ARGS);
-    const Shape s = shape_of(a, r, tile);
+    s = shape_of(a, r, tile);
     own += (long long)s.tiles * s.segments;
   }
   long long upto = own;
@@ -85,36 +102,36 @@ __device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *
     upto += lane >= o ? x : 0;
   }
   if (lane == 31)
-    range->sums[warp] = upto;
+    sums[warp] = upto;
   __syncthreads();
   long long total = 0;
   for (int w = 0; w < threads / 32; w++) {
-    upto += w < warp ? range->sums[w] : 0;
-    total += range->sums[w];
+    const long long x = sums[w];
+    upto += w < warp ? x : 0;
+    total += x;
   }
   const long long ctas = total < gridDim.x ? total : gridDim.x, cta = blockIdx.x;
   if (cta >= ctas)
     return false;
-  const long long lo = total * cta / ctas, hi = total * (cta + 1) / ctas;
-  if (lo >= upto - own && lo < upto) {
-    long long before = upto - own;
+  const long long each = quotient(total, ctas), longer = total - each * ctas;
+  const long long lo = each * cta + min(cta, longer);
+  long long before = upto - own;
+  if (lo >= before && lo < upto) {
     int b = b0;
-    for (;; b++) {
-      const Shape s = shape_of(a, request_of(a.starts, a.counts, b, a.rows, a.positions), tile);
-      const long long n = (long long)s.tiles * s.segments;
-      if (lo < before + n)
-        break;
-      before += n;
-    }
-    range->lo = lo, range->hi = hi, range->total = total, range->before = before, range->b = b, range->ctas = (int)ctas;
+    if (per > 1)
+      for (;; b++) {
+        r = request_of(a.starts, a.counts, b, a.rows, a.positions);
+        s = shape_of(a, r, tile);
+        const long long n = (long long)s.tiles * s.segments;
+        if (lo < before + n)
+          break;
+        before += n;
+      }
+    range->lo = lo, range->hi = lo + each + (cta < longer), range->each = each, range->longer = longer;
+    range->before = before, range->b = b, range->request = r, range->shape = s;
   }
   __syncthreads();
   return true;
-}
-
-// The CTA whose share holds tile x.
-__device__ __forceinline__ int owner(const Range *range, long long x) {
-  return (int)(((x + 1) * range->ctas - 1) / range->total);
 }
 
 // Weights are held times 2^-guard, 2^guard above the positions that a row sees: so that the sum of as many values of the
@@ -135,11 +152,8 @@ struct Walk {
   int b;
   Request request;
   Shape shape;
-  __device__ __forceinline__ Walk(const PagedArgs &a, const Range *range, int tile) {
-    at = range->lo, before = range->before, b = range->b;
-    request = request_of(a.starts, a.counts, b, a.rows, a.positions);
-    shape = shape_of(a, request, tile);
-  }
+  __device__ __forceinline__ explicit Walk(const Range *range)
+      : at(range->lo), before(range->before), b(range->b), request(range->request), shape(range->shape) {}
   __device__ __forceinline__ bool next(const PagedArgs &a, const Range *range, int tile, Piece *p) {
     if (at >= range->hi)
       return false;
@@ -150,7 +164,7 @@ struct Walk {
       shape = shape_of(a, request, tile);
     }
     const long long local = at - before;
-    const int segment = (int)(local / shape.tiles);
+    const int segment = (int)quotient(local, shape.tiles);
     p->b = b;
     p->head = segment / shape.blocks;
     p->block = segment - p->head * shape.blocks;
@@ -188,53 +202,79 @@ __device__ __forceinline__ void finish(const PagedArgs &a, const Range *range, c
   bool wrong = *bad != 0;
   if (p.t0 || p.t1 < p.tiles) {
     const int c0 = owner(range, p.first), c1 = owner(range, p.first + p.tiles - 1);
-    const int cta = blockIdx.x;
-    float *slot = a.partial + (size_t)(2 * cta + (cta == c0)) * a.slot_floats;
-    float *slot_m = slot + 4, *slot_l = slot_m + a.block, *slot_o = slot_l + a.block;
+    const int cta = blockIdx.x, n = p.vecs * hd;
+    const int l_at = 4 + a.block, o_at = 4 + 2 * a.block;
+    auto slot_of = [&](int c) { return a.partial + (size_t)(2 * c + (c == c0)) * a.slot_floats; };
+    float *slot = slot_of(cta);
     if (t == 0)
       slot[0] = wrong ? 1.0f : 0.0f;
     for (int i = t; i < p.vecs; i += threads)
-      slot_m[i] = m[i], slot_l[i] = l[i];
-    for (int i = t; i < p.vecs * hd; i += threads)
-      slot_o[i] = o[i];
-    __threadfence();
+      slot[4 + i] = m[i], slot[l_at + i] = l[i];
+    if (hd % 4 == 0)
+      for (int i = 4 * t; i < n; i += 4 * threads)
+        *reinterpret_cast<float4 *>(slot + o_at + i) = *reinterpret_cast<const float4 *>(o + i);
+    else
+      for (int i = t; i < n; i += threads)
+        slot[o_at + i] = o[i];
     meet<THREADS, BARRIER>();
     if (t == 0) {
       const size_t segment = ((size_t)p.b * a.n_kv + p.head) * a.blocks + p.block;
+      __threadfence();  // the barrier's and this fence's order together: the slot is in memory before the ticket
       *last = atomicInc(&a.tickets[segment], (unsigned)(c1 - c0)) == (unsigned)(c1 - c0);
+      __threadfence();
     }
     meet<THREADS, BARRIER>();
     if (!*last) {
       meet<THREADS, BARRIER>();
       return;
     }
-    __threadfence();
-    auto slot_of = [&](int c) { return a.partial + (size_t)(2 * c + (c == c0)) * a.slot_floats; };
+    // Several slots at a time on their way; those past the last are the last again, without weight.
+    constexpr int kAt = THREADS > 256 ? 4 : 8;
     wrong = false;
-    for (int c = c0; c <= c1; c++)
-      wrong |= __ldcg(slot_of(c)) != 0.0f;
-    for (int i = t; i < p.vecs; i += threads) {
-      float top = -INFINITY, sum = 0.0f;
-      for (int c = c0; c <= c1; c++)
-        top = fmaxf(top, __ldcg(slot_of(c) + 4 + i));
-      for (int c = c0; c <= c1; c++) {
-        const float mc = __ldcg(slot_of(c) + 4 + i);
-        sum += mc == -INFINITY ? 0.0f : exp2f(mc - top) * __ldcg(slot_of(c) + 4 + a.block + i);
-      }
-      m[i] = top, l[i] = sum;
-    }
-    meet<THREADS, BARRIER>();
-    for (int i = t; i < p.vecs * hd; i += threads) {
+    const int step = hd % 4 == 0 ? 4 : 1;
+    for (int i = step * t; i < n; i += step * threads) {
       const int v = i / hd;
-      float x = 0.0f;
-      for (int c = c0; c <= c1; c++) {
-        const float mc = __ldcg(slot_of(c) + 4 + v);
-        if (mc != -INFINITY)
-          x = fmaf(exp2f(mc - m[v]), __ldcg(slot_of(c) + 4 + 2 * a.block + i), x);
+      float top = -INFINITY, sum = 0.0f;
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int c = c0; c <= c1; c += kAt) {
+        float mc[kAt], lc[kAt], flag[kAt], high = top;
+        float4 oc[kAt];
+#pragma unroll
+        for (int j = 0; j < kAt; j++) {
+          const float *from = slot_of(min(c + j, c1));
+          flag[j] = __ldcg(from), mc[j] = __ldcg(from + 4 + v), lc[j] = __ldcg(from + l_at + v);
+          oc[j] = step == 4 ? __ldcg(reinterpret_cast<const float4 *>(from + o_at + i))
+                            : make_float4(__ldcg(from + o_at + i), 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int j = 0; j < kAt; j++) {
+          wrong |= flag[j] != 0.0f;
+          high = fmaxf(high, mc[j]);
+        }
+        const float keep = top == -INFINITY ? 0.0f : exp2f(top - high);
+        x.x *= keep, x.y *= keep, x.z *= keep, x.w *= keep, sum *= keep;
+        top = high;
+#pragma unroll
+        for (int j = 0; j < kAt; j++) {
+          if (c + j > c1 || mc[j] == -INFINITY)
+            continue;
+          const float w = exp2f(mc[j] - top);
+          sum = fmaf(w, lc[j], sum);
+          x.x = fmaf(w, oc[j].x, x.x), x.y = fmaf(w, oc[j].y, x.y);
+          x.z = fmaf(w, oc[j].z, x.z), x.w = fmaf(w, oc[j].w, x.w);
+        }
       }
-      o[i] = x;
+      if (step == 4)
+        *reinterpret_cast<float4 *>(o + i) = x;
+      else
+        o[i] = x.x;
+      if (i - v * hd < step)
+        l[v] = sum;
     }
+    if (wrong)
+      *last = -1;
     meet<THREADS, BARRIER>();
+    wrong = *last < 0;
   }
   if (wrong) {
     if (t == 0)

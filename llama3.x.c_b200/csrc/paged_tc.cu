@@ -15,13 +15,14 @@
 // A tile's sums are a product of their own, eight MMAs that start at zero; they join the running sums in fp32, in
 // registers, rounded to nearest (the tensor cores' accumulators cut towards zero).
 //
-// A CTA per SM takes its share of the tiles of all segments without a pause between segments. Warps 0-3: softmax, a
-// thread per position of a tile and per element of the head of its sums; 4: issues the MMAs; 5: lays out the next
-// segment's queries; 6-9: copy the tiles, asynchronously, through a ring of stages.
+// A CTA per SM takes its share of the tiles of all segments without a pause between segments. Its warps: softmax, a thread
+// per position of a tile and per element of the head of its sums, in groups of four warps that share out the query vectors
+// (4 or 8 to a thread: with all 32 of the largest block in one group, a tile took 3.9 us); one that issues the MMAs; one
+// or more that lay out the next segment's queries; four that copy the tiles, asynchronously, through a ring of stages.
 //
-// What differs between the rows of a request's drafts, the positions behind the first row's, is not in the tiles (their
-// positions end where the block's first row's do): a later draft's key or value of any kind must not reach the rows before
-// it, not even with a weight of zero. Those few products are made in fp32 at the beginning of the segment's last piece.
+// A later draft's key or value of any kind must not reach the rows before it, not even with a weight of zero: a key gives
+// scores in its own row of S^T only, which are masked; a value with an infinity or a NaN behind the block's first row is
+// zeroed by the warp that copied it, and the rows that see it get NaN for a weight there.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -32,18 +33,19 @@ namespace {
 using namespace paged;
 
 constexpr int kTile = 128;  // positions
-constexpr int kSoft = 128;  // softmax threads
 constexpr int kCopyWarps = 4;
-constexpr int kThreads = kSoft + 32 + 32 + 32 * kCopyWarps;
 constexpr int kCtas = 148;
 constexpr int kMaxBlock = 32;
+constexpr int kMaxStages = 8;
 constexpr int kSmem = 227 * 1024;
 
 struct Tail {
-  uint64_t full[10], empty[10], sfull[2], pfull[2], ofull[2], qfull[2], qempty[2], drained;
+  uint64_t full[kMaxStages], empty[kMaxStages], sfull[2], pfull[2], ofull[2], qfull[2], qempty[2], drained;
   uint32_t tmem;
   int abort_flag, bad, last;
   Range range;
+  uint8_t check[kMaxStages][kCopyWarps];   // of a stage's values: the first of a warp's rows to look at
+  uint32_t wrong[kMaxStages][kCopyWarps];  // and those of them that are not finite
   __align__(16) float top[2][4][kMaxBlock];  // a tile's maxima by warp
   // Of the queries: four pieces, since the softmax may be two tiles behind the scores, and the queries two pieces ahead.
   float qscale[4][kMaxBlock];
@@ -51,18 +53,21 @@ struct Tail {
 
 template <int HD, int BLOCK>
 struct Layout {
+  static constexpr int groups = BLOCK == 4 ? 1 : BLOCK == 8 ? 2 : 4, vecs = BLOCK / groups;  // vectors to a thread
+  static constexpr int query_warps = groups == 4 ? 3 : groups;  // (24 warps: 80 registers a thread, 25 would leave 72)
+  static constexpr int soft = 128 * groups;  // softmax threads
+  static constexpr int threads = soft + 32 + 32 * query_warps + 32 * kCopyWarps;
   static constexpr int n = (3 * BLOCK + 15) / 16 * 16;  // columns
   static constexpr int entry = kTile * HD * 2;
   static constexpr int q_bytes = n * HD * 2, p_bytes = n * kTile * 2;
   static constexpr int fit = (kSmem - 1024 - 2 * (q_bytes + p_bytes) - (int)sizeof(Tail)) / entry;
-  static constexpr int stages = fit > 10 ? 10 : HD == 128 && fit > 6 ? 6 : fit;
+  static constexpr int stages = fit > kMaxStages ? kMaxStages : fit;
   static constexpr int ahead = stages - 2;  // copies in flight: the consumer may need the two before them
   static constexpr int q_at = stages * entry, p_at = q_at + 2 * q_bytes, tail_at = p_at + 2 * p_bytes;
   static constexpr int total = tail_at + (int)sizeof(Tail) + 1024;
   static constexpr int tmem = 4 * n <= 64 ? 64 : 4 * n <= 128 ? 128 : 4 * n <= 256 ? 256 : 512;
-  static_assert(ahead >= 1 && total <= kSmem, "shared memory");
+  static_assert(ahead >= 2 && total <= kSmem, "shared memory");
   static_assert(2 * p_bytes >= BLOCK * HD * 4, "the sums' room, over the probabilities'");
-  static_assert(2 * p_bytes >= BLOCK * BLOCK * 4 + 2 * BLOCK * HD * 2, "the drafts' room, over the probabilities'");
 };
 
 __device__ __forceinline__ bool tc_wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
@@ -144,8 +149,6 @@ template <typename T>
 __device__ __forceinline__ float join(float x0, float x1, float x2) {
   return __is_same(T, __half) ? fmaf(fmaf(x2, 0x1p-11f, x1), 0x1p-11f, x0) : (x2 + x1) + x0;
 }
-__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
 
 // 16 bytes from global to shared memory, asynchronously; zeros without `in`.
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool in) {
@@ -167,7 +170,7 @@ __device__ __forceinline__ void tmem_ld4(uint32_t at, float (&x)[4]) {
   for (int j = 0; j < 4; j++)
     x[j] = __uint_as_float(r[j]);
 }
-__device__ __forceinline__ void tmem_ld8(uint32_t at, float *x) {
+__device__ __forceinline__ void tmem_ld8(uint32_t at, float (&x)[8]) {
   uint32_t r[8];
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
@@ -176,33 +179,26 @@ __device__ __forceinline__ void tmem_ld8(uint32_t at, float *x) {
   for (int j = 0; j < 8; j++)
     x[j] = __uint_as_float(r[j]);
 }
-// The joined columns of this thread's lane: part p of vector v is column p * BLOCK + v. Eight
-// vectors at a time, so that three parts fit the registers.
-template <typename T, int BLOCK>
-__device__ __forceinline__ void tmem_joined(uint32_t at, float (&x)[BLOCK]) {
-  if constexpr (BLOCK == 4) {
-    float p[3][4];
+// The joined columns of this thread's lane: part p of vector v is column p * BLOCK + v. VECS (4 or 8) vectors, `at` the
+// column of the first.
+template <typename T, int BLOCK, int VECS>
+__device__ __forceinline__ void tmem_joined(uint32_t at, float (&x)[VECS]) {
+  float p[3][VECS];
 #pragma unroll
-    for (int i = 0; i < 3; i++)
-      tmem_ld4(at + 4 * i, p[i]);
-    tmem_wait_ld();
-#pragma unroll
-    for (int v = 0; v < 4; v++)
-      x[v] = join<T>(p[0][v], p[1][v], p[2][v]);
-  } else {
-#pragma unroll
-    for (int c = 0; c < BLOCK; c += 8) {
-      float p[3][8];
-#pragma unroll
-      for (int i = 0; i < 3; i++)
-        tmem_ld8(at + BLOCK * i + c, p[i]);
-      tmem_wait_ld();
-#pragma unroll
-      for (int v = 0; v < 8; v++)
-        x[c + v] = join<T>(p[0][v], p[1][v], p[2][v]);
-    }
+  for (int i = 0; i < 3; i++) {
+    if constexpr (VECS == 4)
+      tmem_ld4(at + BLOCK * i, p[i]);
+    else
+      tmem_ld8(at + BLOCK * i, p[i]);
   }
+  tmem_wait_ld();
+#pragma unroll
+  for (int v = 0; v < VECS; v++)
+    x[v] = join<T>(p[0][v], p[1][v], p[2][v]);
 }
+
+// The four warps of a softmax group meet.
+__device__ __forceinline__ void meet_group(int group) { asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory"); }
 
 // The first row of a piece's block, and how many rows it has beyond that.
 struct Rows {
@@ -227,8 +223,9 @@ __device__ __forceinline__ long long place_of(const PagedArgs &a, const Piece &p
 }
 
 template <typename T, int HD, int BLOCK>
-__global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel(const PagedArgs a) {
   using L = Layout<HD, BLOCK>;
+  constexpr int kSoft = L::soft, kVecs = L::vecs, kMma = kSoft / 32, kQuery = kMma + 1, kCopy = kQuery + L::query_warps;
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -237,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
-  if (!find_range(a, kTile, &t->range))
+  if (!find_range(a, kTile, &t->range, reinterpret_cast<long long *>(t->top)))
     return;
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::stages; i++) {
@@ -248,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
       mbar_init(&t->sfull[i], 1);
       mbar_init(&t->pfull[i], kSoft / 32);
       mbar_init(&t->ofull[i], 1);
-      mbar_init(&t->qfull[i], 1);
+      mbar_init(&t->qfull[i], L::query_warps);
       mbar_init(&t->qempty[i], 1);
     }
     mbar_init(&t->drained, 1);
@@ -256,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
     t->bad = 0;
     fence_mbar_init();
   }
-  if (warp == kSoft / 32)
+  if (warp == kMma)
     tmem_alloc(&t->tmem, L::tmem);
   tc_fence_before();
   __syncthreads();
@@ -264,18 +261,40 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
   const uint32_t tmem = t->tmem;
   const Range *range = &t->range;
   const float scale = rsqrtf((float)HD) * kLog2e;
-  Walk walk(a, range, kTile);
+  Walk walk(range);
   Piece p;
 
-  if (warp >= kSoft / 32 + 2) {
+  if (warp >= kCopy) {
     // ---- copies: warp w of them the rows 32 w .. 32 w + 31 of every tile, keys and values in turn ----
     constexpr int kChunks = HD / 8, kAt = 32 / kChunks;  // 16-byte units of a row, rows of a warp's instruction
-    const int w = warp - kSoft / 32 - 2;
+    const int w = warp - kCopy;
     const int chunk = lane % kChunks, sub = lane / kChunks;
     const uint32_t base = smem_u32(smem) + (chunk >> 3) * (kTile * 128);
     int slot = 0, signal = 0;
     unsigned parity = 1, entries = 0;
     auto done = [&]() {  // the oldest entry not yet handed over is in memory
+      const int from = (entries - 1 - L::ahead) % 2 ? t->check[signal][w] : 32;
+      if (from < 32) {
+        // Values that some rows of the block do not see, a lane a row.
+        constexpr unsigned kExp = kBf16 ? 0x7f80u : 0x7c00u;
+        uint8_t *row = smem + signal * L::entry + (32 * w + lane) * 128;
+        bool wrong = false;
+        if (lane >= from)
+#pragma unroll 4
+          for (int i = 0; i < kChunks; i++) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(row + (i >> 3) * (kTile * 128) + (i & 7) * 16);
+            const unsigned u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              wrong |= (u[k] & kExp) == kExp || (u[k] >> 16 & kExp) == kExp;
+          }
+        if (wrong)
+          for (int i = 0; i < kChunks; i++)
+            *reinterpret_cast<uint4 *>(row + (i >> 3) * (kTile * 128) + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+        const unsigned mask = __ballot_sync(0xffffffffu, wrong);
+        if (lane == 0)
+          t->wrong[signal][w] = mask;
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0)
@@ -283,17 +302,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
       signal = signal + 1 == L::stages ? 0 : signal + 1;
     };
     while (walk.next(a, range, kTile, &p)) {
-      const int common = p.start + rows_of(a, p).first + 1;  // positions that every row of the block sees
+      const Rows rows = rows_of(a, p);
+      const int common = p.start + rows.first + 1, end = common + rows.more;  // seen by every row of the block, by any
       int position = p.t0 * kTile + 32 * w + lane;
-      long long next = position < common ? place_of(a, p, position, HD) : -1;
+      long long next = position < end ? place_of(a, p, position, HD) : -1;
       for (int j = p.t0; j < p.t1; j++) {
         const long long place = next;
         position += kTile;
-        next = j + 1 < p.t1 && position < common ? place_of(a, p, position, HD) : -1;
+        next = j + 1 < p.t1 && position < end ? place_of(a, p, position, HD) : -1;
+        const int all = min(max(common - j * kTile - 32 * w, 0), 32), any = min(max(end - j * kTile - 32 * w, 0), 32);
 #pragma unroll
         for (int kv = 0; kv < 2; kv++) {
           const T *from = static_cast<const T *>(kv ? a.value : a.key) + chunk * 8;
           tc_wait(&t->empty[slot], parity, abort_flag);
+          if (kv && lane == 0)
+            t->check[slot][w] = (uint8_t)(all < any ? all : 32);
 #pragma unroll
           for (int i = 0; i < 32 / kAt; i++) {
             const int r = i * kAt + sub;
@@ -307,15 +330,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
             slot = 0, parity ^= 1;
           if (++entries > L::ahead) {
             copy_wait<L::ahead>();
+            __syncwarp();
             done();
           }
         }
       }
     }
     copy_wait<0>();
-    for (int i = min(entries, (unsigned)L::ahead); i > 0; i--)
+    __syncwarp();
+    const unsigned issued = entries;
+    for (unsigned left = min(issued, (unsigned)L::ahead); left > 0; left--) {
+      entries = issued + L::ahead + 1 - left;  // the entry to hand over is `ahead` + 1 before
       done();
-  } else if (warp == kSoft / 32 + 1) {
+    }
+  } else if (warp >= kQuery) {
     // ---- queries: times the scores' scale, in three parts, row part * BLOCK + v of the operand ----
     constexpr int kEach = HD / 32;
     for (int n = 0; walk.next(a, range, kTile, &p); n++) {
@@ -323,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
       if (n >= 2)
         tc_wait(&t->qempty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag);
 #pragma unroll
-      for (int v0 = 0; v0 < BLOCK; v0 += 4) {
+      for (int v0 = 4 * (warp - kQuery); v0 < BLOCK; v0 += 4 * L::query_warps) {
         float x[4][kEach];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -367,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
       if (lane == 0)
         mbar_arrive(&t->qfull[n & 1]);
     }
-  } else if (warp == kSoft / 32) {
+  } else if (warp == kMma) {
     // ---- MMA issue: the scores of tile j + 1 before the sums of tile j, so that they run under its softmax. MMAs run in
     // the order of issue. S and O have two buffers each; that a buffer was read is known from the probabilities of a later
     // tile (the softmax reads the scores of a tile before it writes its probabilities, and the sums of the tile before the
@@ -435,20 +463,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
     mbar_wait_sleep_bounded(&t->drained, 0);
   } else {
     // ---- softmax ----
-    const int tid = threadIdx.x;  // a position of the tile; of the sums, an element of the head
-    const uint32_t quadrant = tmem + ((uint32_t)(32 * warp) << 16);
+    const int tid = threadIdx.x, group = warp >> 2, quad = warp & 3, v0 = group * kVecs;  // the group's first vector
+    const int row = 32 * quad + lane;  // a position of the tile; of the sums, a row of the tensor memory
+    const uint32_t quadrant = tmem + ((uint32_t)(32 * quad) << 16) + v0;
     // M = 64 keeps 16 rows in each quadrant of the tensor memory.
-    const int element = HD == 128 ? tid : 16 * warp + lane;
+    const int element = HD == 128 ? row : 16 * quad + lane;
     const bool has_element = HD == 128 || lane < 16;
-    uint8_t *const prow = smem + L::p_at + (tid >> 6) * (L::n * 128) + (tid & 7) * 2;
-    const int pchunk = (tid & 63) >> 3;
-    int j = 0;
+    uint8_t *const prow = smem + L::p_at + (row >> 6) * (L::n * 128) + (row & 7) * 2;
+    const int pchunk = (row & 63) >> 3;
+    int j = 0, vslot = 1;
+    unsigned vpar = 0;
     for (int n = 0; walk.next(a, range, kTile, &p); n++) {
       const Rows rows = rows_of(a, p);
-      const int common = p.start + rows.first + 1;
-      float m[BLOCK], l[BLOCK], acc[BLOCK];
+      const int common = p.start + rows.first + 1, end = common + rows.more;
+      float m[kVecs], l[kVecs], acc[kVecs];
 #pragma unroll
-      for (int v = 0; v < BLOCK; v++)
+      for (int v = 0; v < kVecs; v++)
         m[v] = -INFINITY, l[v] = 0.0f, acc[v] = 0.0f;
       // Weights: bf16 as guard_of says, fp16 up to 2^15 (there is no value beyond 2^16).
       const float weight = kBf16 ? guard_of(p.start + p.count) : 0x1p15f;
@@ -464,98 +494,65 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
         if (bad)
           t->bad = 1;
       }
-      if (rows.more && p.t1 == p.tiles) {
-        // The drafts' own positions, common .. common + more - 1; row first + r sees the first r of them.
-        T *kd = reinterpret_cast<T *>(smem + L::p_at), *vd = kd + BLOCK * HD;
-        float *sd = reinterpret_cast<float *>(vd + BLOCK * HD);  // [more][BLOCK]
-        constexpr int kUnits = HD / 8;
-        for (int i = tid; i < rows.more * kUnits; i += kSoft) {
-          const int r = i / kUnits, u = i % kUnits;
-          const long long at = place_of(a, p, common + r, HD);
-          const uint4 zero = make_uint4(0, 0, 0, 0);
-          reinterpret_cast<uint4 *>(kd)[i] =
-              at < 0 ? zero : *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.key) + at + 8 * u);
-          reinterpret_cast<uint4 *>(vd)[i] =
-              at < 0 ? zero : *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.value) + at + 8 * u);
-        }
-        meet<kSoft, 1>();
-        for (int v0 = 4 * warp; v0 < p.vecs; v0 += 16) {  // four vectors of a warp at a time
-          float q[4][HD / 32];
-          int row[4];
+      auto add = [&](int i) {  // the sums of tile i
+        float o[kVecs];
+        tc_wait(&t->ofull[i & 1], (i >> 1) & 1, abort_flag);
+        tc_fence_after();
+        tmem_joined<T, BLOCK, kVecs>(quadrant + L::n * (2 + (i & 1)), o);
+        tc_fence_before();
 #pragma unroll
-          for (int u = 0; u < 4; u++) {
-            const float *from = a.q + (size_t)vector_at(a, p, min(v0 + u, p.vecs - 1), &row[u]) * HD;
-#pragma unroll
-            for (int i = 0; i < HD / 32; i++)
-              q[u][i] = from[lane + 32 * i] * scale;
-          }
-          for (int r = 0; r < rows.more; r++) {
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < HD / 32; i++) {
-              const float k = widen(kd[r * HD + lane + 32 * i]);
-#pragma unroll
-              for (int u = 0; u < 4; u++)
-                s[u] = fmaf(q[u][i], k, s[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-#pragma unroll
-              for (int o = 16; o; o >>= 1)
-                s[u] += __shfl_xor_sync(0xffffffffu, s[u], o);
-              if (lane == 0 && v0 + u < BLOCK)
-                sd[r * BLOCK + v0 + u] = v0 + u < p.vecs && r < row[u] - rows.first ? s[u] : -INFINITY;
-            }
-          }
-        }
-        meet<kSoft, 1>();
-#pragma unroll
-        for (int v = 0; v < BLOCK; v++) {
-          if (v >= p.vecs)
-            continue;
-          int row;
-          vector_at(a, p, v, &row);
-          for (int r = 0; r < row - rows.first; r++)
-            m[v] = fmaxf(m[v], sd[r * BLOCK + v]);
-          for (int r = 0; r < row - rows.first; r++) {
-            const float w = ex2(sd[r * BLOCK + v] - m[v]) * weight;
-            l[v] += tid == 0 ? w : 0.0f;
-            if (has_element)
-              acc[v] = fmaf(w, widen(vd[r * HD + element]), acc[v]);
-          }
-        }
-        meet<kSoft, 1>();
-      }
+        for (int v = 0; v < kVecs; v++)
+          acc[v] += o[v];
+      };
       for (int tile = p.t0; tile < p.t1; tile++, j++) {
-        float s[BLOCK], keep[BLOCK];
+        float s[kVecs], keep[kVecs];
         tc_wait(&t->sfull[j & 1], (j >> 1) & 1, abort_flag);
         tc_fence_after();
-        tmem_joined<T, BLOCK>(quadrant + L::n * (j & 1), s);
+        tmem_joined<T, BLOCK, kVecs>(quadrant + L::n * (j & 1), s);
         tc_fence_before();
-        const bool in = tile * kTile + tid < common;
+        const int position = tile * kTile + row;
+        unsigned seen = position < common ? (1u << kVecs) - 1 : 0;  // a bit a vector
+        if (rows.more && tile * kTile + kTile > common) {
+          // The rows see different positions of this tile.
+          tc_wait(&t->full[vslot], vpar, abort_flag);
+          if (position >= common && position < end) {
+            const bool wrong = t->wrong[vslot][quad] >> lane & 1;
+#pragma unroll
+            for (int v = 0; v < kVecs; v++) {
+              int member = p.block * BLOCK + v0 + v;
+              if (v0 + v < p.vecs && position <= p.start + divide(member, a.by_group)) {
+                seen |= 1u << v;
+                s[v] = wrong ? NAN : s[v];
+              }
+            }
+          }
+        }
+        vslot += 2;
+        if (vslot >= L::stages)
+          vslot -= L::stages, vpar ^= 1;
         float (*top)[kMaxBlock] = t->top[j & 1];
 #pragma unroll
-        for (int v = 0; v < BLOCK; v++) {
+        for (int v = 0; v < kVecs; v++) {
           if (!kBf16)
-            s[v] *= t->qscale[n & 3][v];
-          s[v] = in ? s[v] : -INFINITY;
+            s[v] *= t->qscale[n & 3][v0 + v];
+          s[v] = seen >> v & 1 ? s[v] : -INFINITY;
           const float x = warp_max(s[v]);
           if (lane == 0)
-            top[warp][v] = x;
+            top[quad][v0 + v] = x;
         }
-        meet<kSoft, 1>();
+        meet_group(group);
 #pragma unroll
-        for (int v = 0; v < BLOCK; v++) {
-          const float x = fmaxf(fmaxf(fmaxf(top[0][v], top[1][v]), fmaxf(top[2][v], top[3][v])), m[v]);
-          keep[v] = x == -INFINITY ? 1.0f : ex2(m[v] - x);  // a tile behind the block's first row has nothing for it
+        for (int v = 0; v < kVecs; v++) {
+          const float x = fmaxf(fmaxf(fmaxf(top[0][v0 + v], top[1][v0 + v]), fmaxf(top[2][v0 + v], top[3][v0 + v])), m[v]);
+          keep[v] = x == -INFINITY ? 1.0f : ex2(m[v] - x);  // a row may see nothing of a piece
           m[v] = x;
-          const float w = in ? ex2(s[v] - x) * weight : 0.0f;
+          const float w = seen >> v & 1 ? ex2(s[v] - x) * weight : 0.0f;
           l[v] = fmaf(l[v], keep[v], w);
           const Parts<T> parts = split(w, T(0.0f));
 #pragma unroll
           for (int part = 0; part < 3; part++) {
-            const int row = part * BLOCK + v;
-            *reinterpret_cast<unsigned short *>(prow + (j & 1) * L::p_bytes + row * 128 + ((pchunk ^ (row & 7)) << 4)) =
+            const int r = part * BLOCK + v0 + v;
+            *reinterpret_cast<unsigned short *>(prow + (j & 1) * L::p_bytes + r * 128 + ((pchunk ^ (r & 7)) << 4)) =
                 parts.part[part];
           }
         }
@@ -563,44 +560,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&t->pfull[j & 1]);
-        if (tile > p.t0) {
-          const int i = j - 1;
-          float o[BLOCK];
-          tc_wait(&t->ofull[i & 1], (i >> 1) & 1, abort_flag);
-          tc_fence_after();
-          tmem_joined<T, BLOCK>(quadrant + L::n * (2 + (i & 1)), o);
-          tc_fence_before();
+        if (tile > p.t0)
+          add(j - 1);
 #pragma unroll
-          for (int v = 0; v < BLOCK; v++)
-            acc[v] += o[v];
-        }
-#pragma unroll
-        for (int v = 0; v < BLOCK; v++)
+        for (int v = 0; v < kVecs; v++)
           acc[v] *= keep[v];
       }
-      {
-        const int i = j - 1;
-        float o[BLOCK];
-        tc_wait(&t->ofull[i & 1], (i >> 1) & 1, abort_flag);
-        tc_fence_after();
-        tmem_joined<T, BLOCK>(quadrant + L::n * (2 + (i & 1)), o);
-        tc_fence_before();
-#pragma unroll
-        for (int v = 0; v < BLOCK; v++)
-          acc[v] += o[v];
-      }
+      add(j - 1);
       // The piece's result. Its last product is done, so the probabilities' room is free.
       float *sums = reinterpret_cast<float *>(smem + L::p_at), (*part)[kMaxBlock] = t->top[j & 1];
       float *m_all = t->top[(j & 1) ^ 1][0], *l_all = t->top[(j & 1) ^ 1][1];  // once the last tile's maxima are read
 #pragma unroll
-      for (int v = 0; v < BLOCK; v++) {
-        if (has_element && v < p.vecs)
-          sums[v * HD + element] = acc[v];
+      for (int v = 0; v < kVecs; v++) {
+        if (has_element && v0 + v < p.vecs)
+          sums[(v0 + v) * HD + element] = acc[v];
 #pragma unroll
         for (int o = 16; o; o >>= 1)
           l[v] += __shfl_xor_sync(0xffffffffu, l[v], o);
         if (lane == 0)
-          part[warp][v] = l[v];
+          part[quad][v0 + v] = l[v];
       }
       if (*abort_flag)
         t->bad = 1;
@@ -608,9 +586,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
       if (tid < p.vecs)
         l_all[tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
 #pragma unroll
-      for (int v = 0; v < BLOCK; v++)
-        if (tid == v)
-          m_all[v] = m[v];
+      for (int v = 0; v < kVecs; v++)
+        if (row == v)
+          m_all[v0 + v] = m[v];
       meet<kSoft, 1>();
       finish<kSoft, 1>(a, range, p, m_all, l_all, sums, &t->bad, &t->last);
       if (tid == 0)
@@ -619,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const PagedArgs a
     }
   }
   __syncthreads();
-  if (warp == kSoft / 32) {
+  if (warp == kMma) {
     tc_fence_after();
     tmem_dealloc(tmem, L::tmem);
   }
@@ -631,7 +609,7 @@ cudaError_t launch(const PagedArgs &a) {
   const cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(kernel), Layout<HD, BLOCK>::total);
   return e != cudaSuccess
              ? e
-             : kc_launch_pdl(kernel, dim3(kCtas), dim3(kThreads), Layout<HD, BLOCK>::total, kc_stream(), a);
+             : kc_launch_pdl(kernel, dim3(kCtas), dim3(Layout<HD, BLOCK>::threads), Layout<HD, BLOCK>::total, kc_stream(), a);
 }
 template <typename T, int HD>
 cudaError_t launch_block(const PagedArgs &a) {

@@ -154,17 +154,17 @@ struct Row {
 template <typename T, int LANES, bool WIDE>
 __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedArgs a) {
   constexpr int kAt = 32 / LANES;  // positions of a warp at a time
-  __shared__ Range range;
+  __shared__ RangeRoom room;
   __shared__ __align__(16) float sums[kWarps][kVecs][LANES * kElems];
   __shared__ float wm[kWarps][kVecs], wl[kWarps][kVecs], m_all[kVecs], l_all[kVecs];
   __shared__ int bad, last;
-  __shared__ long long range_sums[kWarps];
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, sub = lane % LANES, at = lane / LANES;
   pdl_wait();
   pdl_launch_dependents();
   if (t == 0)
     bad = 0;
-  if (!find_range(a, kTile, &range, range_sums))
+  Range range;
+  if (!find_range(a, kTile, &range, &room))
     return;
   const int hd = a.hd;
   const float scale = rsqrtf((float)hd) * kLog2e;

@@ -79,58 +79,114 @@ __device__ __forceinline__ int owner(const Range *range, long long x) {
   return (int)(x < edge ? quotient(x, range->each + 1) : range->longer + quotient(x - edge, range->each));
 }
 
-// This CTA's share of the tiles, and the request in which it begins. All threads call it; `sums` has room for a number a
-// warp. False: nothing to do.
-__device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *range, long long *sums) {
-  const int threads = blockDim.x, t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int per = a.batch <= threads ? 1 : (a.batch + threads - 1) / threads;
-  const int b0 = min(a.batch, t * per), b1 = min(a.batch, b0 + per);
-  long long own = 0;
-  Request r = {0, 0, false};
-  Shape s = {0, 0, 1};
-  for (int b = b0; b < b1; b++) {
-    r = request_of(a.starts, a.counts, b, a.rows, a.positions);
-    if (r.bad && blockIdx.x == 0)
-      kc_raise(KC_ERR_BAD_ARGS);
-    s = shape_of(a, r, tile);
-    own += (long long)s.tiles * s.segments;
-  }
-  long long upto = own;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-    upto += lane >= o ? x : 0;
-  }
-  if (lane == 31)
-    sums[warp] = upto;
-  __syncthreads();
-  long long total = 0;
-  for (int w = 0; w < threads / 32; w++) {
-    const long long x = sums[w];
-    upto += w < warp ? x : 0;
-    total += x;
-  }
+// This CTA's share of `total` tiles: false where it has none.
+__device__ __forceinline__ bool share(long long total, Range *range) {
   const long long ctas = total < gridDim.x ? total : gridDim.x, cta = blockIdx.x;
   if (cta >= ctas)
     return false;
-  const long long each = quotient(total, ctas), longer = total - each * ctas;
-  const long long lo = each * cta + min(cta, longer);
-  long long before = upto - own;
-  if (lo >= before && lo < upto) {
+  range->each = quotient(total, ctas), range->longer = total - range->each * ctas;
+  range->lo = range->each * cta + min(cta, range->longer);
+  range->hi = range->lo + range->each + (cta < range->longer);
+  return true;
+}
+
+__device__ __forceinline__ long long scan(long long x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    x += lane >= o ? y : 0;
+  }
+  return x;
+}
+
+// This CTA's share of the tiles, and the request in which it begins, in every thread's registers. All threads call it;
+// `common` is shared memory. False: nothing to do. Up to kAlone requests, every warp finds it alone, a few requests to a
+// lane: no barrier on the way to the first page (with two, a call of one request took 0.5 us longer).
+constexpr int kEachAlone = 4, kAlone = 32 * kEachAlone;
+struct RangeRoom {
+  long long sums[32];
+  Range range;
+};
+__device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *range, RangeRoom *common) {
+  const int threads = blockDim.x, t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  if (a.batch <= kAlone) {
+    const int per = (a.batch + 31) / 32, b0 = lane * per;
+    Request r[kEachAlone];
+    Shape s[kEachAlone];
+    long long own = 0;
+#pragma unroll
+    for (int i = 0; i < kEachAlone; i++)
+      if (i < per && b0 + i < a.batch)
+        r[i] = request_of(a.starts, a.counts, b0 + i, a.rows, a.positions);
+      else
+        r[i] = Request{0, 0, false};
+#pragma unroll
+    for (int i = 0; i < kEachAlone; i++) {
+      if (r[i].bad && blockIdx.x == 0 && warp == 0)
+        kc_raise(KC_ERR_BAD_ARGS);
+      s[i] = shape_of(a, r[i], tile);
+      own += (long long)s[i].tiles * s[i].segments;
+    }
+    const long long upto = scan(own, lane);
+    if (!share(__shfl_sync(0xffffffffu, upto, 31), range))
+      return false;
+    const int from = __ffs(__ballot_sync(0xffffffffu, range->lo < upto)) - 1;
+    long long before = upto - own;
+    Request at = r[0];
+    Shape shape = s[0];
     int b = b0;
-    if (per > 1)
-      for (;; b++) {
-        r = request_of(a.starts, a.counts, b, a.rows, a.positions);
-        s = shape_of(a, r, tile);
-        const long long n = (long long)s.tiles * s.segments;
-        if (lo < before + n)
-          break;
-        before += n;
+#pragma unroll
+    for (int i = 0; i + 1 < kEachAlone; i++)
+      if (b == b0 + i && lane == from && range->lo >= before + (long long)s[i].tiles * s[i].segments)
+        before += (long long)s[i].tiles * s[i].segments, b++, at = r[i + 1], shape = s[i + 1];
+    range->before = __shfl_sync(0xffffffffu, before, from);
+    range->b = __shfl_sync(0xffffffffu, b, from);
+    range->request.count = __shfl_sync(0xffffffffu, at.count, from);
+    range->request.start = __shfl_sync(0xffffffffu, at.start, from);
+    range->request.bad = false;
+    range->shape.tiles = __shfl_sync(0xffffffffu, shape.tiles, from);
+    range->shape.segments = __shfl_sync(0xffffffffu, shape.segments, from);
+    range->shape.blocks = __shfl_sync(0xffffffffu, shape.blocks, from);
+    return true;
+  }
+  const int per = (a.batch + threads - 1) / threads;
+  const int b0 = min(a.batch, t * per), b1 = min(a.batch, b0 + per);
+  long long own = 0;
+  for (int b = b0; b < b1; b++) {
+    const Request r = request_of(a.starts, a.counts, b, a.rows, a.positions);
+    if (r.bad && blockIdx.x == 0)
+      kc_raise(KC_ERR_BAD_ARGS);
+    const Shape s = shape_of(a, r, tile);
+    own += (long long)s.tiles * s.segments;
+  }
+  long long upto = scan(own, lane);
+  if (lane == 31)
+    common->sums[warp] = upto;
+  __syncthreads();
+  long long total = 0;
+  for (int w = 0; w < threads / 32; w++) {
+    const long long x = common->sums[w];
+    upto += w < warp ? x : 0;
+    total += x;
+  }
+  if (!share(total, range))
+    return false;
+  long long before = upto - own;
+  if (range->lo >= before && range->lo < upto) {
+    for (int b = b0;; b++) {
+      const Request r = request_of(a.starts, a.counts, b, a.rows, a.positions);
+      const Shape s = shape_of(a, r, tile);
+      const long long n = (long long)s.tiles * s.segments;
+      if (range->lo < before + n) {
+        range->before = before, range->b = b, range->request = r, range->shape = s;
+        common->range = *range;
+        break;
       }
-    range->lo = lo, range->hi = lo + each + (cta < longer), range->each = each, range->longer = longer;
-    range->before = before, range->b = b, range->request = r, range->shape = s;
+      before += n;
+    }
   }
   __syncthreads();
+  *range = common->range;
   return true;
 }
 

@@ -22,7 +22,7 @@
 //
 // A later draft's key or value of any kind must not reach the rows before it, not even with a weight of zero: a key gives
 // scores in its own row of S^T only, which are masked; a value with an infinity or a NaN behind the block's first row is
-// zeroed by the warp that copied it, and the rows that see it get NaN for a weight there.
+// zeroed before its product, and the rows that see it get NaN for a weight there.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -36,17 +36,14 @@ constexpr int kTile = 128;  // positions
 constexpr int kCopyWarps = 4;
 constexpr int kCtas = 148;
 constexpr int kMaxBlock = 32;
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 10;
 constexpr int kSmem = 227 * 1024;
 
 struct Tail {
   uint64_t full[kMaxStages], empty[kMaxStages], sfull[2], pfull[2], ofull[2], qfull[2], qempty[2], drained;
   uint32_t tmem;
   int abort_flag, bad, last;
-  Range range;
-  uint8_t check[kMaxStages][kCopyWarps];   // of a stage's values: the first of a warp's rows to look at
-  uint32_t wrong[kMaxStages][kCopyWarps];  // and those of them that are not finite
-  __align__(16) float top[2][4][kMaxBlock];  // a tile's maxima by warp
+  __align__(16) float top[2][4][kMaxBlock];  // a tile's maxima by warp; the warps' sums of weights
   // Of the queries: four pieces, since the softmax may be two tiles behind the scores, and the queries two pieces ahead.
   float qscale[4][kMaxBlock];
 };
@@ -62,11 +59,10 @@ struct Layout {
   static constexpr int q_bytes = n * HD * 2, p_bytes = n * kTile * 2;
   static constexpr int fit = (kSmem - 1024 - 2 * (q_bytes + p_bytes) - (int)sizeof(Tail)) / entry;
   static constexpr int stages = fit > kMaxStages ? kMaxStages : fit;
-  static constexpr int ahead = stages - 2;  // copies in flight: the consumer may need the two before them
   static constexpr int q_at = stages * entry, p_at = q_at + 2 * q_bytes, tail_at = p_at + 2 * p_bytes;
   static constexpr int total = tail_at + (int)sizeof(Tail) + 1024;
   static constexpr int tmem = 4 * n <= 64 ? 64 : 4 * n <= 128 ? 128 : 4 * n <= 256 ? 256 : 512;
-  static_assert(ahead >= 2 && total <= kSmem, "shared memory");
+  static_assert(stages >= 4 && total <= kSmem, "shared memory");
   static_assert(2 * p_bytes >= BLOCK * HD * 4, "the sums' room, over the probabilities'");
 };
 
@@ -82,10 +78,20 @@ __device__ __forceinline__ bool tc_wait(uint64_t *bar, unsigned parity, volatile
   return __all_sync(0xffffffffu, ok);
 }
 
-// kind::f16, fp32 accumulators, fp16 or bf16 operands, A K-major or MN-major, B K-major, M x N.
-__host__ __device__ constexpr uint32_t umma_idesc(bool bf16, int m, int n, bool a_mn) {
-  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((a_mn ? 1u : 0u) << 15) | ((uint32_t)(n >> 3) << 17) |
-         ((uint32_t)(m >> 4) << 24);
+// kind::f16, fp32 accumulators, fp16 or bf16 operands, both K-major or both MN-major, M x N.
+__host__ __device__ constexpr uint32_t umma_idesc(bool bf16, int m, int n, bool mn) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (mn ? (1u << 15) | (1u << 16) : 0u) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// MN-major operand in the 32-byte swizzle: rows of 16 values along N, 8 rows (K) to an atom of 256 bytes; atoms 256 bytes
+// apart along K, `n_bytes` apart along N.
+__device__ __forceinline__ uint64_t umma_desc_sw32_mn(const void *smem_tile, uint32_t n_bytes) {
+  uint64_t d = (smem_u32(smem_tile) >> 4) & 0x3FFFull;
+  d |= (uint64_t)(n_bytes >> 4) << 16;
+  d |= (uint64_t)(256 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)6 << 61;
+  return d;
 }
 // MN-major operand in the 128-byte swizzle: rows of 64 values along M, 8 rows (K) to an atom of 1 KiB; atoms 1 KiB apart
 // along K, `m_bytes` apart along M.
@@ -120,30 +126,17 @@ __device__ __forceinline__ float warp_max(float x) {
 // 2^k for -126 <= k <= 127.
 __device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) << 23); }
 
-// The 16 bits of each of a number's three parts (fp16: of a number already brought to fp16's range).
-template <typename T>
-struct Parts {
-  unsigned short part[3];
-};
-__device__ __forceinline__ Parts<__nv_bfloat16> split(float x, __nv_bfloat16) {
-  Parts<__nv_bfloat16> p;
-#pragma unroll
-  for (int i = 0; i < 3; i++) {
-    const unsigned bits = __float_as_uint(x);
-    p.part[i] = (unsigned short)(bits >> 16);
-    x -= __uint_as_float(bits & 0xffff0000u);  // exact
-  }
-  return p;
+// The next part of two numbers (fp16: already brought to fp16's range), packed, and what is left of them, exactly.
+__device__ __forceinline__ uint32_t next_part(float &x, float &y, __nv_bfloat16) {
+  const unsigned a = __float_as_uint(x), b = __float_as_uint(y);
+  x -= __uint_as_float(a & 0xffff0000u), y -= __uint_as_float(b & 0xffff0000u);
+  return __byte_perm(a, b, 0x7632);
 }
-__device__ __forceinline__ Parts<__half> split(float x, __half) {
-  Parts<__half> p;
-#pragma unroll
-  for (int i = 0; i < 3; i++) {
-    const __half h = __float2half_rn(x);
-    p.part[i] = __half_as_ushort(h);
-    x = (x - __half2float(h)) * 2048.0f;  // exact
-  }
-  return p;
+__device__ __forceinline__ uint32_t next_part(float &x, float &y, __half) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  x = (x - f.x) * 2048.0f, y = (y - f.y) * 2048.0f;
+  return *reinterpret_cast<const uint32_t *>(&h);
 }
 template <typename T>
 __device__ __forceinline__ float join(float x0, float x1, float x2) {
@@ -154,11 +147,11 @@ __device__ __forceinline__ float join(float x0, float x1, float x2) {
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+// Arrives once all copies that this thread has started are in memory.
+__device__ __forceinline__ void copy_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // This thread's lane of 4 or 8 columns.
 __device__ __forceinline__ void tmem_ld4(uint32_t at, float (&x)[4]) {
@@ -197,8 +190,22 @@ __device__ __forceinline__ void tmem_joined(uint32_t at, float (&x)[VECS]) {
     x[v] = join<T>(p[0][v], p[1][v], p[2][v]);
 }
 
-// The four warps of a softmax group meet.
+// The four warps of a softmax group meet; meet_any: and learn whether any of their threads says so.
 __device__ __forceinline__ void meet_group(int group) { asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory"); }
+__device__ __forceinline__ bool meet_any(int group, bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"((uint32_t)mine), "r"(2 + group)
+      : "memory");
+  return any != 0;
+}
+// How far a score, in powers of two, may lie above the reference before the reference moves.
+constexpr float kRise = 8.0f;
 
 // The first row of a piece's block, and how many rows it has beyond that.
 struct Rows {
@@ -234,11 +241,12 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
-  if (!find_range(a, kTile, &t->range, reinterpret_cast<long long *>(t->top)))
+  Range here;
+  if (!find_range(a, kTile, &here, reinterpret_cast<RangeRoom *>(t->top)))
     return;
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::stages; i++) {
-      mbar_init(&t->full[i], kCopyWarps);
+      mbar_init(&t->full[i], 32 * kCopyWarps);
       mbar_init(&t->empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
@@ -259,7 +267,7 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = t->tmem;
-  const Range *range = &t->range;
+  const Range *range = &here;
   const float scale = rsqrtf((float)HD) * kLog2e;
   Walk walk(range);
   Piece p;
@@ -270,53 +278,21 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
     const int w = warp - kCopy;
     const int chunk = lane % kChunks, sub = lane / kChunks;
     const uint32_t base = smem_u32(smem) + (chunk >> 3) * (kTile * 128);
-    int slot = 0, signal = 0;
-    unsigned parity = 1, entries = 0;
-    auto done = [&]() {  // the oldest entry not yet handed over is in memory
-      const int from = (entries - 1 - L::ahead) % 2 ? t->check[signal][w] : 32;
-      if (from < 32) {
-        // Values that some rows of the block do not see, a lane a row.
-        constexpr unsigned kExp = kBf16 ? 0x7f80u : 0x7c00u;
-        uint8_t *row = smem + signal * L::entry + (32 * w + lane) * 128;
-        bool wrong = false;
-        if (lane >= from)
-#pragma unroll 4
-          for (int i = 0; i < kChunks; i++) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(row + (i >> 3) * (kTile * 128) + (i & 7) * 16);
-            const unsigned u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-              wrong |= (u[k] & kExp) == kExp || (u[k] >> 16 & kExp) == kExp;
-          }
-        if (wrong)
-          for (int i = 0; i < kChunks; i++)
-            *reinterpret_cast<uint4 *>(row + (i >> 3) * (kTile * 128) + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-        const unsigned mask = __ballot_sync(0xffffffffu, wrong);
-        if (lane == 0)
-          t->wrong[signal][w] = mask;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0)
-        mbar_arrive(&t->full[signal]);
-      signal = signal + 1 == L::stages ? 0 : signal + 1;
-    };
+    int slot = 0;
+    unsigned parity = 1;
     while (walk.next(a, range, kTile, &p)) {
       const Rows rows = rows_of(a, p);
-      const int common = p.start + rows.first + 1, end = common + rows.more;  // seen by every row of the block, by any
+      const int end = p.start + rows.first + rows.more + 1;  // seen by any row of the block
       int position = p.t0 * kTile + 32 * w + lane;
       long long next = position < end ? place_of(a, p, position, HD) : -1;
       for (int j = p.t0; j < p.t1; j++) {
         const long long place = next;
         position += kTile;
         next = j + 1 < p.t1 && position < end ? place_of(a, p, position, HD) : -1;
-        const int all = min(max(common - j * kTile - 32 * w, 0), 32), any = min(max(end - j * kTile - 32 * w, 0), 32);
 #pragma unroll
         for (int kv = 0; kv < 2; kv++) {
           const T *from = static_cast<const T *>(kv ? a.value : a.key) + chunk * 8;
           tc_wait(&t->empty[slot], parity, abort_flag);
-          if (kv && lane == 0)
-            t->check[slot][w] = (uint8_t)(all < any ? all : 32);
 #pragma unroll
           for (int i = 0; i < 32 / kAt; i++) {
             const int r = i * kAt + sub;
@@ -324,25 +300,14 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
             const int row = 32 * w + r;
             copy16(base + slot * L::entry + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), from + max(at, 0ll), at >= 0);
           }
-          copy_commit();
+          copy_arrive(&t->full[slot]);
           slot++;
           if (slot == L::stages)
             slot = 0, parity ^= 1;
-          if (++entries > L::ahead) {
-            copy_wait<L::ahead>();
-            __syncwarp();
-            done();
-          }
         }
       }
     }
-    copy_wait<0>();
-    __syncwarp();
-    const unsigned issued = entries;
-    for (unsigned left = min(issued, (unsigned)L::ahead); left > 0; left--) {
-      entries = issued + L::ahead + 1 - left;  // the entry to hand over is `ahead` + 1 before
-      done();
-    }
+    copy_wait_all();
   } else if (warp >= kQuery) {
     // ---- queries: times the scores' scale, in three parts, row part * BLOCK + v of the operand ----
     constexpr int kEach = HD / 32;
@@ -359,7 +324,7 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
           const float *q = a.q + (size_t)vector_at(a, p, min(v0 + u, p.vecs - 1), &row) * HD;
 #pragma unroll
           for (int i = 0; i < kEach; i++)
-            x[u][i] = v0 + u < p.vecs ? q[lane + 32 * i] * scale : 0.0f;
+            x[u][i] = v0 + u < p.vecs ? q[2 * lane + 32 * (i & ~1) + (i & 1)] * scale : 0.0f;
         }
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -378,14 +343,13 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
               t->qscale[n & 3][v] = pow2(-k);
           }
 #pragma unroll
-          for (int i = 0; i < kEach; i++) {
-            const Parts<T> parts = split(x[u][i], T(0.0f));
-            const int e = lane + 32 * i;
+          for (int i = 0; i < kEach; i += 2) {
+            const int e = 2 * lane + 32 * i;
 #pragma unroll
             for (int part = 0; part < 3; part++) {
               const int row = part * BLOCK + v;
-              *reinterpret_cast<unsigned short *>(to + (e >> 6) * (L::n * 128) + row * 128 +
-                                                  ((((e & 63) >> 3) ^ (row & 7)) << 4) + (e & 7) * 2) = parts.part[part];
+              *reinterpret_cast<uint32_t *>(to + (e >> 6) * (L::n * 128) + row * 128 + ((((e & 63) >> 3) ^ (row & 7)) << 4) +
+                                            (e & 7) * 2) = next_part(x[u][i], x[u][i + 1], T(0.0f));
             }
           }
         }
@@ -399,11 +363,11 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
     // ---- MMA issue: the scores of tile j + 1 before the sums of tile j, so that they run under its softmax. MMAs run in
     // the order of issue. S and O have two buffers each; that a buffer was read is known from the probabilities of a later
     // tile (the softmax reads the scores of a tile before it writes its probabilities, and the sums of the tile before the
-    // last by then). ----
+    // last by then). The copies' writes come by the generic proxy, so a fence stands between their barrier and the MMAs. ----
     const bool leader = elect_one();
     constexpr uint32_t idesc_s = umma_idesc(kBf16, kTile, L::n, false), idesc_o = umma_idesc(kBf16, HD, L::n, true);
     const uint64_t kdesc = umma_desc_sw128(smem), vdesc = umma_desc_sw128_mn(smem, kTile * 128);
-    const uint64_t qdesc = umma_desc_sw128(smem + L::q_at), pdesc = umma_desc_sw128(smem + L::p_at);
+    const uint64_t qdesc = umma_desc_sw128(smem + L::q_at), pdesc = umma_desc_sw32_mn(smem + L::p_at, kTile * 32);
     const int tiles = (int)(range->hi - range->lo);
     int piece = -1, left = 0;  // of the scores issued next: its piece, and tiles of it left
     int kslot = 0, vslot = 1;
@@ -419,6 +383,7 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
       left--;
       if (!tc_wait(&t->full[kslot], kpar, abort_flag))
         return false;
+      fence_proxy_async_smem();
       tc_fence_after();
       if (leader) {
 #pragma unroll
@@ -442,12 +407,13 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
         break;
       if (!tc_wait(&t->full[vslot], vpar, abort_flag) || !tc_wait(&t->pfull[j & 1], (j >> 1) & 1, abort_flag))
         break;
+      fence_proxy_async_smem();
       tc_fence_after();
       if (leader) {
 #pragma unroll
         for (int c = 0; c < kTile / 16; c++)
           umma_f16(tmem + L::n * (2 + (j & 1)), vdesc + (vslot * L::entry + 2048 * c) / 16,
-                   pdesc + ((j & 1) * L::p_bytes + (c >> 2) * (L::n * 128) + 32 * (c & 3)) / 16, idesc_o, c);
+                   pdesc + ((j & 1) * L::p_bytes + 512 * c) / 16, idesc_o, c);
         umma_commit(&t->ofull[j & 1]);
         umma_commit(&t->empty[vslot]);
       }
@@ -469,8 +435,9 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
     // M = 64 keeps 16 rows in each quadrant of the tensor memory.
     const int element = HD == 128 ? row : 16 * quad + lane;
     const bool has_element = HD == 128 || lane < 16;
-    uint8_t *const prow = smem + L::p_at + (row >> 6) * (L::n * 128) + (row & 7) * 2;
-    const int pchunk = (row & 63) >> 3;
+    // Its row of the probabilities, and where in a row's 32 bytes its unit of 16 lies.
+    uint8_t *const prow = smem + L::p_at + row * 32;
+    const int punit = (row >> 2) & 1;
     int j = 0, vslot = 1;
     unsigned vpar = 0;
     for (int n = 0; walk.next(a, range, kTile, &p); n++) {
@@ -480,8 +447,8 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
 #pragma unroll
       for (int v = 0; v < kVecs; v++)
         m[v] = -INFINITY, l[v] = 0.0f, acc[v] = 0.0f;
-      // Weights: bf16 as guard_of says, fp16 up to 2^15 (there is no value beyond 2^16).
-      const float weight = kBf16 ? guard_of(p.start + p.count) : 0x1p15f;
+      // Weights are up to 2^kRise times this: bf16 as guard_of says, fp16 up to 2^15 (there is no value beyond 2^16).
+      const float weight = kBf16 ? guard_of(p.start + p.count) * 0x1p-8f : 0x1p7f;
       // Every page of the piece's positions is one.
       {
         int from = p.t0 * kTile, to = min(p.t1 * kTile, p.start + p.count) - 1;
@@ -515,8 +482,19 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
         if (rows.more && tile * kTile + kTile > common) {
           // The rows see different positions of this tile.
           tc_wait(&t->full[vslot], vpar, abort_flag);
-          if (position >= common && position < end) {
-            const bool wrong = t->wrong[vslot][quad] >> lane & 1;
+          const bool some = position >= common && position < end;
+          uint8_t *const values = smem + vslot * L::entry + row * 128;
+          bool wrong = false;
+          if (some) {
+            constexpr unsigned kExp = kBf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll 4
+            for (int i = 0; i < HD / 8; i++) {
+              const uint4 x = *reinterpret_cast<const uint4 *>(values + (i >> 3) * (kTile * 128) + (i & 7) * 16);
+              const unsigned u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int k = 0; k < 4; k++)
+                wrong |= (u[k] & kExp) == kExp || (u[k] >> 16 & kExp) == kExp;
+            }
 #pragma unroll
             for (int v = 0; v < kVecs; v++) {
               int member = p.block * BLOCK + v0 + v;
@@ -526,35 +504,60 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
               }
             }
           }
+          meet<kSoft, 1>();  // every group has looked
+          if (wrong && group == 0)
+            for (int i = 0; i < HD / 8; i++)
+              *reinterpret_cast<uint4 *>(values + (i >> 3) * (kTile * 128) + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         vslot += 2;
         if (vslot >= L::stages)
           vslot -= L::stages, vpar ^= 1;
-        float (*top)[kMaxBlock] = t->top[j & 1];
+        bool rises = false;
 #pragma unroll
         for (int v = 0; v < kVecs; v++) {
           if (!kBf16)
             s[v] *= t->qscale[n & 3][v0 + v];
           s[v] = seen >> v & 1 ? s[v] : -INFINITY;
-          const float x = warp_max(s[v]);
-          if (lane == 0)
-            top[quad][v0 + v] = x;
+          rises |= s[v] > m[v] + kRise;
         }
-        meet_group(group);
+        // The reference stays while no score is far above it: one barrier that tells, instead of maxima over the tile.
+        const bool moves = meet_any(group, rises);
+        if (moves) {
+          float (*top)[kMaxBlock] = t->top[0];
+#pragma unroll
+          for (int v = 0; v < kVecs; v++) {
+            const float x = warp_max(s[v]);
+            if (lane == 0)
+              top[quad][v0 + v] = x;
+          }
+          meet_group(group);
+#pragma unroll
+          for (int v = 0; v < kVecs; v++) {
+            const float x =
+                fmaxf(fmaxf(fmaxf(top[0][v0 + v], top[1][v0 + v]), fmaxf(top[2][v0 + v], top[3][v0 + v])), m[v]);
+            keep[v] = x == -INFINITY ? 1.0f : ex2(m[v] - x);  // a row may see nothing of a piece
+            m[v] = x;
+            l[v] *= keep[v];
+          }
+        }
+        float w[kVecs];
 #pragma unroll
         for (int v = 0; v < kVecs; v++) {
-          const float x = fmaxf(fmaxf(fmaxf(top[0][v0 + v], top[1][v0 + v]), fmaxf(top[2][v0 + v], top[3][v0 + v])), m[v]);
-          keep[v] = x == -INFINITY ? 1.0f : ex2(m[v] - x);  // a row may see nothing of a piece
-          m[v] = x;
-          const float w = seen >> v & 1 ? ex2(s[v] - x) * weight : 0.0f;
-          l[v] = fmaf(l[v], keep[v], w);
-          const Parts<T> parts = split(w, T(0.0f));
+          w[v] = seen >> v & 1 ? ex2(s[v] - m[v]) * weight : 0.0f;
+          l[v] += w[v];
+        }
 #pragma unroll
-          for (int part = 0; part < 3; part++) {
-            const int r = part * BLOCK + v0 + v;
-            *reinterpret_cast<unsigned short *>(prow + (j & 1) * L::p_bytes + r * 128 + ((pchunk ^ (r & 7)) << 4)) =
-                parts.part[part];
-          }
+        for (int part = 0; part < 3; part++) {
+          const int c = part * BLOCK + v0;  // the column of the first
+          uint32_t packed[kVecs / 2];
+#pragma unroll
+          for (int v = 0; v < kVecs; v += 2)
+            packed[v / 2] = next_part(w[v], w[v + 1], T(0.0f));
+          uint8_t *at = prow + (j & 1) * L::p_bytes + (c >> 4) * (kTile * 32) + (((c >> 3 & 1) ^ punit) << 4) + (c & 7) * 2;
+          if constexpr (kVecs == 4)
+            *reinterpret_cast<uint2 *>(at) = make_uint2(packed[0], packed[1]);
+          else
+            *reinterpret_cast<uint4 *>(at) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -562,14 +565,15 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
           mbar_arrive(&t->pfull[j & 1]);
         if (tile > p.t0)
           add(j - 1);
+        if (moves)
 #pragma unroll
-        for (int v = 0; v < kVecs; v++)
-          acc[v] *= keep[v];
+          for (int v = 0; v < kVecs; v++)
+            acc[v] *= keep[v];
       }
       add(j - 1);
       // The piece's result. Its last product is done, so the probabilities' room is free.
-      float *sums = reinterpret_cast<float *>(smem + L::p_at), (*part)[kMaxBlock] = t->top[j & 1];
-      float *m_all = t->top[(j & 1) ^ 1][0], *l_all = t->top[(j & 1) ^ 1][1];  // once the last tile's maxima are read
+      float *sums = reinterpret_cast<float *>(smem + L::p_at), (*part)[kMaxBlock] = t->top[1];
+      float *m_all = t->top[0][0], *l_all = t->top[0][1];  // once the last tile's maxima are read
 #pragma unroll
       for (int v = 0; v < kVecs; v++) {
         if (has_element && v0 + v < p.vecs)

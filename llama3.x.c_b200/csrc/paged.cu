@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedArgs a)
           o[v * hd + t + j * kThreads] = x[j];
       __syncthreads();
     }
-    finish<kThreads, 0>(a, &range, p, m_all, l_all, o, &bad, &last);
+    finish<kThreads, 0, 0>(a, &range, p, m_all, l_all, o, &bad, &last);
     if (t == 0)
       bad = 0;
     __syncthreads();

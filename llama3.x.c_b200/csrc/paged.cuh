@@ -249,12 +249,13 @@ __device__ __forceinline__ void meet() {
 
 // The piece's vectors, with m and l of each and their sums o in shared memory, written to the output (a whole segment,
 // or the last of its pieces to be done) or to a slot. All threads call it, after a barrier behind the last write to m, l,
-// o and bad; it ends with one. THREADS threads, numbered from 0, meet at barrier BARRIER.
-template <int THREADS, int BARRIER>
+// o and bad; it ends with one. THREADS threads, numbered from 0, meet at barrier BARRIER. HD:
+// head_dim, or 0 where it is any.
+template <int THREADS, int BARRIER, int HD>
 __device__ __forceinline__ void finish(const PagedArgs &a, const Range *range, const Piece &p, float *m, float *l, float *o,
                        const int *bad, int *last) {
   constexpr int threads = THREADS;
-  const int t = threadIdx.x, hd = a.hd;
+  const int t = threadIdx.x, hd = HD ? HD : a.hd;
   bool wrong = *bad != 0;
   if (p.t0 || p.t1 < p.tiles) {
     const int c0 = owner(range, p.first), c1 = owner(range, p.first + p.tiles - 1);
@@ -312,9 +313,9 @@ __device__ __forceinline__ void finish(const PagedArgs &a, const Range *range, c
         top = high;
 #pragma unroll
         for (int j = 0; j < kAt; j++) {
-          if (c + j > c1 || mc[j] == -INFINITY)
+          if (c + j > c1)
             continue;
-          const float w = exp2f(mc[j] - top);
+          const float w = mc[j] == -INFINITY ? 0.0f : exp2f(mc[j] - top);  // times NaN, where there is one, it is NaN
           sum = fmaf(w, lc[j], sum);
           x.x = fmaf(w, oc[j].x, x.x), x.y = fmaf(w, oc[j].y, x.y);
           x.z = fmaf(w, oc[j].z, x.z), x.w = fmaf(w, oc[j].w, x.w);
@@ -338,15 +339,27 @@ __device__ __forceinline__ void finish(const PagedArgs &a, const Range *range, c
     meet<THREADS, BARRIER>();
     return;
   }
-  for (int i = t; i < p.vecs * hd; i += threads) {
+  const bool wide = hd % 4 == 0 && ((uintptr_t)a.out & 15) == 0;
+  const int unit = wide ? 4 : 1;
+  for (int i = unit * t; i < p.vecs * hd; i += unit * threads) {
     const int v = i / hd;
     int row;
-    const size_t vec = vector_at(a, p, v, &row);
-    float x = o[i] / l[v];
-    if (fabsf(x) == INFINITY && fabsf(o[i]) < INFINITY)  // a mean of finite values, past the largest one by its rounding
-      x = copysignf(3.402823466e+38f, x);
-    o[i] = x;
-    a.out[vec * hd + (i - v * hd)] = x;
+    float *to = a.out + (size_t)vector_at(a, p, v, &row) * hd + (i - v * hd);
+    const float sum = l[v];
+    // A mean of finite values may come out past the largest one by its rounding.
+    auto mean = [&](float x) {
+      const float y = x / sum;
+      return fabsf(y) == INFINITY && fabsf(x) < INFINITY ? copysignf(3.402823466e+38f, y) : y;
+    };
+    if (wide) {
+      float4 x = *reinterpret_cast<const float4 *>(o + i);
+      x.x = mean(x.x), x.y = mean(x.y), x.z = mean(x.z), x.w = mean(x.w);
+      *reinterpret_cast<float4 *>(to) = x;
+      if (a.oq)
+        *reinterpret_cast<float4 *>(o + i) = x;
+    } else {
+      o[i] = *to = mean(o[i]);
+    }
   }
   meet<THREADS, BARRIER>();
   if (!a.oq)

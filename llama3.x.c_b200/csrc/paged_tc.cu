@@ -204,6 +204,8 @@ __device__ __forceinline__ bool meet_any(int group, bool mine) {
       : "memory");
   return any != 0;
 }
+// The reference before there is one: a number, so that the difference to a masked score (-infinity) is none.
+constexpr float kFar = 3.402823466e+38f;
 // How far a score, in powers of two, may lie above the reference before the reference moves.
 constexpr float kRise = 8.0f;
 
@@ -446,7 +448,8 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
       float m[kVecs], l[kVecs], acc[kVecs];
 #pragma unroll
       for (int v = 0; v < kVecs; v++)
-        m[v] = -INFINITY, l[v] = 0.0f, acc[v] = 0.0f;
+        m[v] = -kFar, l[v] = 0.0f, acc[v] = 0.0f;
+      const bool idle = v0 >= p.vecs;  // the group has none of the block's vectors
       // Weights are up to 2^kRise times this: bf16 as guard_of says, fp16 up to 2^15 (there is no value beyond 2^16).
       const float weight = kBf16 ? guard_of(p.start + p.count) * 0x1p-8f : 0x1p7f;
       // Every page of the piece's positions is one.
@@ -464,6 +467,8 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
       auto add = [&](int i) {  // the sums of tile i
         float o[kVecs];
         tc_wait(&t->ofull[i & 1], (i >> 1) & 1, abort_flag);
+        if (idle)
+          return;
         tc_fence_after();
         tmem_joined<T, BLOCK, kVecs>(quadrant + L::n * (2 + (i & 1)), o);
         tc_fence_before();
@@ -475,89 +480,102 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
         float s[kVecs], keep[kVecs];
         tc_wait(&t->sfull[j & 1], (j >> 1) & 1, abort_flag);
         tc_fence_after();
-        tmem_joined<T, BLOCK, kVecs>(quadrant + L::n * (j & 1), s);
+        if (!idle) {
+          tmem_joined<T, BLOCK, kVecs>(quadrant + L::n * (j & 1), s);
+          if (!kBf16)
+#pragma unroll
+            for (int v = 0; v < kVecs; v++)
+              s[v] *= t->qscale[n & 3][v0 + v];
+        }
         tc_fence_before();
         const int position = tile * kTile + row;
-        unsigned seen = position < common ? (1u << kVecs) - 1 : 0;  // a bit a vector
-        if (rows.more && tile * kTile + kTile > common) {
-          // The rows see different positions of this tile.
-          tc_wait(&t->full[vslot], vpar, abort_flag);
-          const bool some = position >= common && position < end;
-          uint8_t *const values = smem + vslot * L::entry + row * 128;
-          bool wrong = false;
-          if (some) {
-            constexpr unsigned kExp = kBf16 ? 0x7f80u : 0x7c00u;
+        if (tile * kTile + kTile > common) {
+          // Not all of the tile, or not the same of it to all rows.
+          unsigned seen = position < common ? (1u << kVecs) - 1 : 0;  // a bit a vector
+          if (rows.more) {
+            tc_wait(&t->full[vslot], vpar, abort_flag);
+            const bool some = position >= common && position < end;
+            uint8_t *const values = smem + vslot * L::entry + row * 128;
+            bool wrong = false;
+            if (some) {
+              constexpr unsigned kExp = kBf16 ? 0x7f80u : 0x7c00u;
 #pragma unroll 4
-            for (int i = 0; i < HD / 8; i++) {
-              const uint4 x = *reinterpret_cast<const uint4 *>(values + (i >> 3) * (kTile * 128) + (i & 7) * 16);
-              const unsigned u[4] = {x.x, x.y, x.z, x.w};
+              for (int i = 0; i < HD / 8; i++) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(values + (i >> 3) * (kTile * 128) + (i & 7) * 16);
+                const unsigned u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-              for (int k = 0; k < 4; k++)
-                wrong |= (u[k] & kExp) == kExp || (u[k] >> 16 & kExp) == kExp;
-            }
+                for (int k = 0; k < 4; k++)
+                  wrong |= (u[k] & kExp) == kExp || (u[k] >> 16 & kExp) == kExp;
+              }
 #pragma unroll
-            for (int v = 0; v < kVecs; v++) {
-              int member = p.block * BLOCK + v0 + v;
-              if (v0 + v < p.vecs && position <= p.start + divide(member, a.by_group)) {
-                seen |= 1u << v;
-                s[v] = wrong ? NAN : s[v];
+              for (int v = 0; v < kVecs; v++) {
+                int member = p.block * BLOCK + v0 + v;
+                if (v0 + v < p.vecs && position <= p.start + divide(member, a.by_group)) {
+                  seen |= 1u << v;
+                  s[v] = wrong ? NAN : s[v];
+                }
               }
             }
+            meet<kSoft, 1>();  // every group has looked
+            if (wrong && group == 0)
+              for (int i = 0; i < HD / 8; i++)
+                *reinterpret_cast<uint4 *>(values + (i >> 3) * (kTile * 128) + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
-          meet<kSoft, 1>();  // every group has looked
-          if (wrong && group == 0)
-            for (int i = 0; i < HD / 8; i++)
-              *reinterpret_cast<uint4 *>(values + (i >> 3) * (kTile * 128) + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int v = 0; v < kVecs; v++)
+            s[v] = seen >> v & 1 ? s[v] : -INFINITY;
         }
         vslot += 2;
         if (vslot >= L::stages)
           vslot -= L::stages, vpar ^= 1;
-        bool rises = false;
-#pragma unroll
-        for (int v = 0; v < kVecs; v++) {
-          if (!kBf16)
-            s[v] *= t->qscale[n & 3][v0 + v];
-          s[v] = seen >> v & 1 ? s[v] : -INFINITY;
-          rises |= s[v] > m[v] + kRise;
-        }
-        // The reference stays while no score is far above it: one barrier that tells, instead of maxima over the tile.
-        const bool moves = meet_any(group, rises);
-        if (moves) {
-          float (*top)[kMaxBlock] = t->top[0];
+        bool moves = false;
+        if (!idle) {
+          float d[kVecs], high = -INFINITY;
 #pragma unroll
           for (int v = 0; v < kVecs; v++) {
-            const float x = warp_max(s[v]);
-            if (lane == 0)
-              top[quad][v0 + v] = x;
+            d[v] = s[v] - m[v];
+            high = fmaxf(high, d[v]);
           }
-          meet_group(group);
+          // The reference stays while no score is far above it: one barrier that tells, instead of maxima over the tile.
+          moves = meet_any(group, high > kRise);
+          if (moves) {
+            float (*top)[kMaxBlock] = t->top[0];
+#pragma unroll
+            for (int v = 0; v < kVecs; v++) {
+              const float x = warp_max(s[v]);
+              if (lane == 0)
+                top[quad][v0 + v] = x;
+            }
+            meet_group(group);
+#pragma unroll
+            for (int v = 0; v < kVecs; v++) {
+              const float x =
+                  fmaxf(fmaxf(fmaxf(top[0][v0 + v], top[1][v0 + v]), fmaxf(top[2][v0 + v], top[3][v0 + v])), m[v]);
+              keep[v] = ex2(m[v] - x);
+              m[v] = x;
+              d[v] = s[v] - x;
+              l[v] *= keep[v];
+            }
+          }
+          float w[kVecs];
 #pragma unroll
           for (int v = 0; v < kVecs; v++) {
-            const float x =
-                fmaxf(fmaxf(fmaxf(top[0][v0 + v], top[1][v0 + v]), fmaxf(top[2][v0 + v], top[3][v0 + v])), m[v]);
-            keep[v] = x == -INFINITY ? 1.0f : ex2(m[v] - x);  // a row may see nothing of a piece
-            m[v] = x;
-            l[v] *= keep[v];
+            w[v] = ex2(d[v]) * weight;
+            l[v] += w[v];
           }
-        }
-        float w[kVecs];
 #pragma unroll
-        for (int v = 0; v < kVecs; v++) {
-          w[v] = seen >> v & 1 ? ex2(s[v] - m[v]) * weight : 0.0f;
-          l[v] += w[v];
-        }
+          for (int part = 0; part < 3; part++) {
+            const int c = part * BLOCK + v0;  // the column of the first
+            uint32_t packed[kVecs / 2];
 #pragma unroll
-        for (int part = 0; part < 3; part++) {
-          const int c = part * BLOCK + v0;  // the column of the first
-          uint32_t packed[kVecs / 2];
-#pragma unroll
-          for (int v = 0; v < kVecs; v += 2)
-            packed[v / 2] = next_part(w[v], w[v + 1], T(0.0f));
-          uint8_t *at = prow + (j & 1) * L::p_bytes + (c >> 4) * (kTile * 32) + (((c >> 3 & 1) ^ punit) << 4) + (c & 7) * 2;
-          if constexpr (kVecs == 4)
-            *reinterpret_cast<uint2 *>(at) = make_uint2(packed[0], packed[1]);
-          else
-            *reinterpret_cast<uint4 *>(at) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+            for (int v = 0; v < kVecs; v += 2)
+              packed[v / 2] = next_part(w[v], w[v + 1], T(0.0f));
+            uint8_t *at = prow + (j & 1) * L::p_bytes + (c >> 4) * (kTile * 32) + (((c >> 3 & 1) ^ punit) << 4) + (c & 7) * 2;
+            if constexpr (kVecs == 4)
+              *reinterpret_cast<uint2 *>(at) = make_uint2(packed[0], packed[1]);
+            else
+              *reinterpret_cast<uint4 *>(at) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -570,8 +588,8 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
           for (int v = 0; v < kVecs; v++)
             acc[v] *= keep[v];
       }
-      add(j - 1);
-      // The piece's result. Its last product is done, so the probabilities' room is free.
+      add(j - 1);  // idle or not: the probabilities' room is free once the last product is done
+      // The piece's result.
       float *sums = reinterpret_cast<float *>(smem + L::p_at), (*part)[kMaxBlock] = t->top[1];
       float *m_all = t->top[0][0], *l_all = t->top[0][1];  // once the last tile's maxima are read
 #pragma unroll
@@ -594,7 +612,7 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
         if (row == v)
           m_all[v0 + v] = m[v];
       meet<kSoft, 1>();
-      finish<kSoft, 1>(a, range, p, m_all, l_all, sums, &t->bad, &t->last);
+      finish<kSoft, 1, HD>(a, range, p, m_all, l_all, sums, &t->bad, &t->last);
       if (tid == 0)
         t->bad = 0;
       meet<kSoft, 1>();

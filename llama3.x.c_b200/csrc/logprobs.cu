@@ -1,6 +1,15 @@
 // Log probabilities of tokens, the entropy of their distribution and its likeliest tokens, from rows of logits
-// (k_token_logprobs). With M the row's maximum, S = sum e^(x - M) and T = sum e^(x - M) (M - x):
-// log p_i = (x_i - M) - log S, entropy = log S + T / S (two sums of terms of one sign: nothing cancels).
+// (k_token_logprobs). With M the row's maximum, taken once out of the sums, S = sum e^(x - M) and T = sum e^(x - M) (M - x)
+// over the rest: log p_i = (x_i - M) - log(1 + S), entropy = log(1 + S) + T / (1 + S). Both sums have terms of one sign and
+// neither is rounded against the 1, so that the small logarithm of a nearly certain token keeps its digits.
+//
+// The logits are read once. A CTA takes a row, or with few rows a part of one (a cluster joins them), as a stream of 16 KiB
+// stages by bulk copies, through a ring that runs on into the next row. Each thread keeps the sums of its elements relative to
+// a reference near their maximum, and that maximum with its place. At the end of the row the likeliest tokens are found by
+// way of the threads' maxima: with the threads in 64 classes, every one of the top k elements is at or above the k-th largest
+// class maximum, which about as many threads reach as there are tokens to find; only their elements, at a fixed stride,
+// are read again (from L2).
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -9,11 +18,22 @@
 #include "../../include/kernels_cuda.h"
 #include "common.cuh"
 #include "kernels_cuda_internal.h"
+#include "tcgen05.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32;  // that take logits; one more warp issues the copies
 constexpr int kMaxTop = 32;
+constexpr int kUnits = 2 * kThreads;   // 16-byte units to a stage
+constexpr int kStages = 12;
+constexpr int kClasses = 64;
+constexpr int kCandidates = 1024;
+constexpr int kMaxParts = 8;
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kRise = 3.0f;   // how far a logit may lie above a thread's reference before the reference moves
+constexpr float kLeast = -150.0f;  // e^-150 is 0 in fp32: a difference below it (-infinity) is taken for it
 
 struct LogprobArgs {
   float *logprobs, *entropy;
@@ -37,77 +57,405 @@ __device__ __forceinline__ float logit_of(unsigned long long key) {
   return __uint_as_float((b & 0x80000000u) ? b & 0x7fffffffu : ~b);
 }
 
-__device__ __forceinline__ unsigned long long block_max(unsigned long long k, unsigned long long *shared) {
+// What a part of a row gives: its maximum, the sums of the rest relative to it, and its top tokens in order (0: none).
+struct Part {
+  float max, s, t;
+  int wrong;
+  unsigned long long top[kMaxTop];
+};
+
+struct State {
+  uint64_t full[kStages], empty[kStages];
+  Part part;
+  unsigned long long keys[kThreads], least, best;  // the threads' maxima; the k-th largest class maximum, the largest
+  unsigned long long candidates[kCandidates];
+  unsigned long long merged[kMaxParts * kMaxTop];
+  float sums[2][kWarps], again[2];  // the warps' sums; the sums of the thread that has the maximum, without it
+  int marked, found, wrong, verdict;
+  unsigned short who[kThreads];  // threads whose maximum may be a top one
+};
+constexpr int kRing = kStages * kUnits * 16;
+constexpr int kSmem = kRing + (int)sizeof(State);
+
+// The larger of numbers and the first of equals: order of values, then of 16-byte units.
+__device__ __forceinline__ unsigned long long unit_key(float x, unsigned unit) { return key_of(x, (int)unit); }
+
+// A row's logits as 16-byte units from the aligned address at or before the first: `off` elements come before it.
+struct Row {
+  const float4 *units;
+  int off, count;  // count: units
+};
+__device__ __forceinline__ Row row_of(const LogprobArgs &a, int row) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.logits + (size_t)row * a.ld);
+  Row r;
+  r.units = reinterpret_cast<const float4 *>(at & ~(uintptr_t)15);
+  r.off = (int)((at & 15) / 4);
+  r.count = (int)(((long long)r.off + a.vocab + 3) / 4);
+  return r;
+}
+// Part p of n of its units.
+__device__ __forceinline__ void part_of(const Row &r, int p, int n, int *first, int *end) {
+  *first = (int)((long long)r.count * p / n);
+  *end = (int)((long long)r.count * (p + 1) / n);
+}
+// A unit's elements, -infinity for those that are not the row's.
+__device__ __forceinline__ void only_row(float (&x)[4], const Row &r, int unit, int vocab) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1)
-    k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0)
-    shared[threadIdx.x >> 5] = k;
-  __syncthreads();
-  for (int w = 0; w < kWarps; w++)
-    k = max(k, shared[w]);
-  return k;
+  for (int i = 0; i < 4; i++) {
+    const long long at = 4ll * unit + i - r.off;
+    x[i] = at >= 0 && at < vocab ? x[i] : -INFINITY;
+  }
 }
 
-// A CTA per row.
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a) {
-  __shared__ unsigned long long keys[kWarps];
-  __shared__ double sums[2][kWarps];
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN where one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long max_key(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
+__device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+
+// The weight e^d of a difference and its product with it.
+__device__ __forceinline__ void weigh(float d, float &s, float &t) {
+  d = fmaxf(d, kLeast);
+  const float w = ex2(d * kLog2e);
+  s += w;
+  t = fmaf(w, d, t);
+}
+
+// A thread's running results: the maximum and the unit it first came in, and the sums s of e^(x - ref) and t of
+// e^(x - ref) (x - ref) over its elements, in two pairs.
+struct Running {
+  float max, ref;
+  unsigned unit;
+  uint64_t s[2], t[2];
+};
+__device__ __forceinline__ void take(Running &r, const float (&x)[4], unsigned unit, bool *wrong) {
+  const float top = max3(max3(x[0], x[1], x[2]), x[3], x[3]);
+  *wrong |= !(top < INFINITY);
+  if (top > r.max)
+    r.max = top, r.unit = unit;
+  if (top > r.ref + kRise) {
+    const float by = fmaxf(r.ref - top, kLeast), f = ex2(by * kLog2e);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      r.t[i] = f2_mul(f2_fma(f2_pack(by, by), r.s[i], r.t[i]), f2_pack(f, f));
+      r.s[i] = f2_mul(r.s[i], f2_pack(f, f));
+    }
+    r.ref = top;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    float d0, d1;
+    f2_unpack(f2_add(f2_pack(x[2 * i], x[2 * i + 1]), f2_pack(-r.ref, -r.ref)), d0, d1);
+    const uint64_t d = f2_pack(fmaxf(d0, kLeast), fmaxf(d1, kLeast));
+    float e0, e1;
+    f2_unpack(f2_mul(d, f2_pack(kLog2e, kLog2e)), e0, e1);
+    const uint64_t w = f2_pack(ex2(e0), ex2(e1));
+    r.s[i] = f2_add(r.s[i], w);
+    r.t[i] = f2_fma(w, d, r.t[i]);
+  }
+}
+
+// x - max - log_s, rounded once.
+__device__ __forceinline__ float log_p(float x, float max, float log_s) {
+  return (float)(((double)x - (double)max) - (double)log_s);
+}
+
+// A CTA per row, or a cluster of `parts`; each takes rows in turn.
+__global__ void __launch_bounds__(kThreads + 32, 1) logprobs_kernel(const LogprobArgs a, int parts) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  State *t = reinterpret_cast<State *>(smem + kRing);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int part = blockIdx.x % parts, stride = gridDim.x / parts;  // parts > 1: a row to a cluster, and no more
+  cg::cluster_group cluster = cg::this_cluster();
+  if (tid == 0) {
+    for (int i = 0; i < kStages; i++) {
+      mbar_init(&t->full[i], 1);
+      mbar_init(&t->empty[i], kWarps);
+    }
+    t->marked = t->found = t->wrong = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  const int row = blockIdx.x, t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int token = a.tokens ? a.tokens[row] : 0;
-  if (token == -1)
-    return;
-  const float *x = a.logits + (size_t)row * a.ld;
-  bool wrong = token < 0 || token >= a.vocab;
-  unsigned long long best = 0;
-  for (int i = t; i < a.vocab; i += kThreads) {
-    wrong |= !(x[i] < INFINITY);
-    best = max(best, key_of(x[i], i));
-  }
-  best = block_max(best, keys);
-  const float top = logit_of(best);
-  wrong = __syncthreads_or(wrong || !(top > -INFINITY));
-  double s = 0.0, e = 0.0;
-  if (!wrong)
-    for (int i = t; i < a.vocab; i += kThreads) {
-      const float d = x[i] - top, w = expf(d);
-      s += w;
-      e -= w > 0.0f ? (double)w * d : 0.0;
+  if (parts > 1 && a.tokens && a.tokens[blockIdx.x / parts] == -1)
+    return;  // the whole cluster
+  int stage = 0;
+  unsigned parity = 0;
+
+  if (warp == kWarps) {
+    // ---- copies ----
+    if (lane == 0) {
+      bool ok = true;
+      for (int row = blockIdx.x / parts; ok && row < a.rows; row += stride) {
+        if (a.tokens && a.tokens[row] == -1)
+          continue;
+        const Row r = row_of(a, row);
+        int first, end;
+        part_of(r, part, parts, &first, &end);
+        for (int u = first; ok && u < end; u += kUnits) {
+          ok = mbar_wait_bounded(&t->empty[stage], parity ^ 1);
+          const unsigned bytes = 16u * (unsigned)min(kUnits, end - u);
+          if (ok) {
+            mbar_arrive_expect_tx(&t->full[stage], bytes);
+            bulk_g2s(smem + stage * kUnits * 16, r.units + u, bytes, &t->full[stage]);
+          }
+          if (++stage == kStages)
+            stage = 0, parity ^= 1;
+        }
+      }
     }
+    __syncwarp();
+  } else {
+    bool ok = true;  // no wait has run out
+    for (int row = blockIdx.x / parts; row < a.rows; row += stride) {
+      const int token = a.tokens ? a.tokens[row] : 0;
+      if (token == -1)
+        continue;
+      const Row r = row_of(a, row);
+      int first, end;
+      part_of(r, part, parts, &first, &end);
+      Running mine;
+      mine.max = -INFINITY, mine.ref = -3.402823466e+38f, mine.unit = first + tid;
+      mine.s[0] = mine.s[1] = mine.t[0] = mine.t[1] = 0;
+      bool wrong = token < 0 || token >= a.vocab;
+      for (int u = first; u < end; u += kUnits) {
+        ok = ok && mbar_wait_bounded(&t->full[stage], parity);
+        const float4 *from = reinterpret_cast<const float4 *>(smem + stage * kUnits * 16) + tid;
+        float4 y[2];
 #pragma unroll
-  for (int o = 16; o; o >>= 1)
-    s += __shfl_xor_sync(0xffffffffu, s, o), e += __shfl_xor_sync(0xffffffffu, e, o);
-  if (lane == 0)
-    sums[0][warp] = s, sums[1][warp] = e;
-  __syncthreads();
-  s = e = 0.0;
-  for (int w = 0; w < kWarps; w++)
-    s += sums[0][w], e += sums[1][w];
-  const double log_s = log(s);
-  if (t == 0) {
-    if (wrong)
-      kc_raise(KC_ERR_BAD_ARGS);
-    if (a.logprobs)
-      a.logprobs[row] = wrong ? NAN : (float)((double)x[token] - top - log_s);
-    if (a.entropy)
-      a.entropy[row] = wrong ? NAN : (float)(log_s + e / s);
+        for (int h = 0; h < 2; h++)
+          y[h] = u + h * kThreads + tid < end ? from[h * kThreads] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&t->empty[stage]);
+        if (++stage == kStages)
+          stage = 0, parity ^= 1;
+        const bool edge = u == 0 || u + kUnits >= r.count;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          float x[4] = {y[h].x, y[h].y, y[h].z, y[h].w};
+          const int unit = u + h * kThreads + tid;
+          if (edge)
+            only_row(x, r, unit, a.vocab);
+          take(mine, x, (unsigned)unit, &wrong);
+        }
+      }
+      wrong |= !ok;
+      // ---- the end of the part: the maximum, and the class maximum that holds the top ones ----
+      const unsigned long long key = first + tid < end ? unit_key(mine.max, mine.unit) : 0;
+      t->keys[tid] = key;
+      if (wrong)
+        t->wrong = 1;
+      meet();
+      const int wanted = a.top > 1 ? a.top : 1;
+      if (warp < 2) {
+        unsigned long long k = t->keys[tid];
+        for (int i = 1; i < kThreads / kClasses; i++)
+          k = max_key(k, t->keys[tid + i * kClasses]);
+        t->merged[tid] = k;
+        asm volatile("bar.sync 2, 64;" ::: "memory");
+        int before = 0;
+        for (int i = 0; i < kClasses; i++)
+          before += t->merged[i] > k || (t->merged[i] == k && i < tid);
+        if (before == 0)
+          t->best = k;
+        if (before == wanted - 1)
+          t->least = k;  // 0 where fewer classes have any
+      }
+      meet();
+      const unsigned long long best = t->best, least = t->least;
+      const float top = logit_of(best);
+      const bool bad = t->wrong != 0;
+      if (key != 0 && key >= least)
+        t->who[atomicAdd(&t->marked, 1)] = (unsigned short)tid;
+      // ---- the sums, relative to the maximum; the thread that has it leaves its own to the second look ----
+      float s, e;
+      {
+        float s0, s1, s2, s3, t0, t1, t2, t3;
+        f2_unpack(mine.s[0], s0, s1), f2_unpack(mine.s[1], s2, s3);
+        f2_unpack(mine.t[0], t0, t1), f2_unpack(mine.t[1], t2, t3);
+        const float by = fmaxf(mine.ref - top, kLeast), f = ex2(by * kLog2e);
+        s = (s0 + s1) + (s2 + s3);
+        e = fmaf(by, s, (t0 + t1) + (t2 + t3)) * f;
+        s *= f;
+        if (key == best || key == 0 || top == -INFINITY)
+          s = e = 0.0f;
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1)
+        s += __shfl_xor_sync(0xffffffffu, s, o), e += __shfl_xor_sync(0xffffffffu, e, o);
+      if (lane == 0)
+        t->sums[0][warp] = s, t->sums[1][warp] = e;
+      meet();
+      // ---- the second look at the marked threads' units, a warp to a thread ----
+      const int marked = bad ? 0 : t->marked;
+      for (int m = warp; m < marked; m += kWarps) {
+        const int who = t->who[m];
+        const bool owner = t->keys[who] == best;
+        const unsigned best_unit = 0xffffffffu - (unsigned)best;
+        float s2 = 0.0f, e2 = 0.0f;
+        for (int u0 = first + who; u0 < end; u0 += 32 * kThreads) {
+          const int unit = u0 + lane * kThreads;
+          float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (unit < end) {
+            const float4 y = __ldg(r.units + unit);
+            x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+            only_row(x, r, unit, a.vocab);
+          }
+          bool out = owner && (unsigned)unit == best_unit;  // the maximum is still to be left out
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const long long at = 4ll * unit + i - r.off;
+            const bool in = unit < end && at >= 0 && at < a.vocab;
+            if (in && unit_key(x[i], (unsigned)unit) >= least) {
+              const int n = atomicAdd(&t->found, 1);
+              if (n < kCandidates)
+                t->candidates[n] = key_of(x[i], (int)at);
+            }
+            if (out && x[i] == top)
+              out = false;
+            else if (owner && in)
+              weigh(x[i] - top, s2, e2);
+          }
+        }
+        if (owner) {
+#pragma unroll
+          for (int o = 16; o; o >>= 1)
+            s2 += __shfl_xor_sync(0xffffffffu, s2, o), e2 += __shfl_xor_sync(0xffffffffu, e2, o);
+          if (lane == 0)
+            t->again[0] = s2, t->again[1] = e2;
+        }
+      }
+      meet();
+      // ---- the top ones in order ----
+      const int found = t->found;
+      if (tid < kMaxTop)
+        t->part.top[tid] = 0;
+      if (tid == 0) {
+        const bool some = top > -INFINITY;
+        float s2 = some ? t->again[0] : 0.0f, e2 = some ? t->again[1] : 0.0f;
+        for (int w = 0; w < kWarps; w++)
+          s2 += t->sums[0][w], e2 += t->sums[1][w];
+        t->part.max = some ? top : -INFINITY, t->part.s = s2, t->part.t = -e2;
+        t->part.wrong = bad;
+        t->marked = t->found = t->wrong = 0;
+      }
+      meet();
+      if (!bad && found <= kCandidates) {
+        for (int i = tid; i < found; i += kThreads) {
+          const unsigned long long k = t->candidates[i];
+          int before = 0;
+          for (int j = 0; j < found; j++)
+            before += t->candidates[j] > k;
+          if (before < wanted)
+            t->part.top[before] = k;
+        }
+      } else if (!bad) {
+        // More elements above the classes' maximum than there is room for: one token after another, from the logits.
+        unsigned long long last = ~0ull;
+        for (int n = 0; n < wanted; n++) {
+          unsigned long long k = 0;
+          for (int unit = first + tid; unit < end; unit += kThreads) {
+            const float4 y = __ldg(r.units + unit);
+            const float x[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const long long at = 4ll * unit + i - r.off;
+              if (at >= 0 && at < a.vocab) {
+                const unsigned long long other = key_of(x[i], (int)at);
+                k = other < last ? max_key(k, other) : k;
+              }
+            }
+          }
+#pragma unroll
+          for (int o = 16; o; o >>= 1)
+            k = max_key(k, __shfl_xor_sync(0xffffffffu, k, o));
+          meet();
+          if (lane == 0)
+            t->merged[warp] = k;
+          meet();
+          for (int w = 0; w < kWarps; w++)
+            k = max_key(k, t->merged[w]);
+          if (tid == 0)
+            t->part.top[n] = k;
+          last = k;
+        }
+      }
+      // ---- the parts' results joined by the first of them ----
+      if (parts > 1)
+        cluster.sync();
+      else
+        meet();
+      if (part == 0) {
+        const int keys = parts * kMaxTop;
+        if (parts > 1 && tid < keys)
+          t->merged[tid] = cluster.map_shared_rank(&t->part, tid / kMaxTop)->top[tid % kMaxTop];
+        if (tid == 0) {
+          float max = -INFINITY, s3 = 0.0f, e3 = 0.0f, m[kMaxParts], n[kMaxParts], e2[kMaxParts];
+          bool any_wrong = false;
+          int of = 0;
+#pragma unroll
+          for (int i = 0; i < kMaxParts; i++) {
+            const Part *from = i == 0 || i >= parts ? &t->part : cluster.map_shared_rank(&t->part, i);
+            m[i] = i < parts ? from->max : -INFINITY, n[i] = from->s, e2[i] = from->t;
+            any_wrong |= from->wrong != 0;
+            if (m[i] > max)
+              max = m[i], of = i;
+          }
+#pragma unroll
+          for (int i = 0; i < kMaxParts; i++) {
+            if (m[i] == -INFINITY)
+              continue;
+            const float by = m[i] - max, f = ex2(fmaxf(by, kLeast) * kLog2e);
+            if (i != of)
+              n[i] += 1.0f;  // another part's maximum is one of the rest
+            if (f > 0.0f)
+              s3 = fmaf(n[i], f, s3), e3 = fmaf(fmaf(-by, n[i], e2[i]), f, e3);
+          }
+          const bool w = any_wrong || !(max > -INFINITY);
+          const float log_s = log1pf(s3);
+          if (w)
+            kc_raise(KC_ERR_BAD_ARGS);
+          if (a.logprobs)
+            a.logprobs[row] = w ? NAN : log_p(a.logits[(size_t)row * a.ld + token], max, log_s);
+          if (a.entropy)
+            a.entropy[row] = w ? NAN : log_s + e3 / (1.0f + s3);
+          t->sums[0][0] = max, t->sums[0][1] = log_s, t->verdict = w;
+        }
+        meet();
+        const bool w = t->verdict != 0;
+        const float max = t->sums[0][0], log_s = t->sums[0][1];
+        int at = -1;
+        unsigned long long k = 0;
+        if (parts == 1) {
+          at = tid, k = tid < kMaxTop ? t->part.top[tid] : 0;
+        } else if (tid < keys && (k = t->merged[tid]) != 0) {
+          at = 0;
+          for (int i = 0; i < keys; i++)
+            at += t->merged[i] > k;
+        }
+        if (w)
+          at = tid;
+        if (at >= 0 && at < a.top) {
+          a.top_tokens[(size_t)row * a.top + at] = w ? -1 : (int)(0xffffffffu - (unsigned)k);
+          a.top_logprobs[(size_t)row * a.top + at] = w ? NAN : log_p(logit_of(k), max, log_s);
+        }
+        meet();
+      }
+    }
   }
-  for (int k = 0; k < a.top; k++) {
-    if (t == 0) {
-      a.top_tokens[(size_t)row * a.top + k] = wrong ? -1 : (int)(0xffffffffu - (unsigned)best);
-      a.top_logprobs[(size_t)row * a.top + k] = wrong ? NAN : (float)((double)logit_of(best) - top - log_s);
-    }
-    if (wrong || k + 1 == a.top)
-      continue;
-    unsigned long long next = 0;
-    for (int i = t; i < a.vocab; i += kThreads) {
-      const unsigned long long key = key_of(x[i], i);
-      next = key < best ? max(next, key) : next;
-    }
-    best = block_max(next, keys);
+  if (parts > 1) {
+    if (warp == kWarps)
+      cluster.sync();  // with the consumers' above
+    cluster.sync();    // the first part has read
   }
 }
 
@@ -130,7 +478,27 @@ extern "C" void k_token_logprobs(float *logprobs, float *entropy, int *top_token
   memset(&a, 0, sizeof(a));
   a.logprobs = logprobs, a.entropy = entropy, a.top_tokens = top_tokens, a.top_logprobs = top_logprobs;
   a.logits = logits, a.ld = ld, a.tokens = tokens, a.vocab = vocab, a.rows = rows, a.top = top;
-  const cudaError_t e = kc_launch_pdl(logprobs_kernel, dim3((unsigned)rows), dim3(kThreads), 0, kc_stream(), a);
+  // With few rows a cluster of CTAs to each, as many as there are SMs for (one row of 128256: @@ us with 8 parts, @@ with
+  // one); from half as many rows as SMs on a CTA to each.
+  const int sms = kc_device_sms();
+  int parts = kMaxParts;
+  while (parts > 1 && (long long)rows * parts > sms)
+    parts /= 2;
+  cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(logprobs_kernel), kSmem);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * (long long)parts < sms ? rows * parts : parts > 1 ? rows * parts : sms));
+  cfg.blockDim = dim3(kThreads + 32);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = kc_stream();
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = kc_pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = parts, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (e == cudaSuccess)
+    e = cudaLaunchKernelEx(&cfg, logprobs_kernel, a, parts);
   if (e == cudaSuccess)
     kc_count_launch();
   else

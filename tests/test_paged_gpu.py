@@ -747,6 +747,20 @@ def test_logprobs_shapes_of_rows(kc, kind, vocab):
         check_logprobs(x, tokens, top, got)
 
 
+@pytest.mark.parametrize("period", [2048, 4096])
+@pytest.mark.parametrize("top", [1, 20, 32])
+def test_logprobs_many_candidates(kc, period, top):
+    """The likeliest tokens all at a power of two from one another, more than any list of them has room for."""
+    vocab = 128256
+    at = torch.arange(vocab, device="cuda")
+    x = torch.where(at % period < 80, 5.0 + torch.rand(vocab, device="cuda", generator=generator(1)), normal(generator(2), vocab))
+    x = torch.stack([x, x.round(), torch.where(at % period < 80, 6.0, -1.0)]).contiguous()
+    tokens = [0, 79, 128255]
+    got = run_logprobs(kc, x, tokens, top)
+    assert kc.status() == 0
+    check_logprobs(x, tokens, top, got)
+
+
 def test_logprobs_small_differences_from_certainty(kc):
     """The likeliest token's log probability -e and the entropy of a row that is nearly certain keep their own digits."""
     vocab = 2000
@@ -754,10 +768,12 @@ def test_logprobs_small_differences_from_certainty(kc):
     for r, top in enumerate((12.0, 20.0, 30.0, 50.0, 80.0)):
         x[r, 77] = top
     lp, ent, _, best = run_logprobs(kc, x, [77] * 5, 3)
-    p = torch.log_softmax(x.double(), -1)
-    h = torch.special.entr(p.exp()).sum(-1)
+    # by the sum of the rest: 64-bit log_softmax rounds it against the 1 (-0 where -log(1 + 1999 e^-50) is -3.9e-19)
+    d = torch.tensor([12.0, 20.0, 30.0, 50.0, 80.0], dtype=torch.float64, device="cuda")
+    rest = (vocab - 1) * torch.exp(-d)
+    p, h = -torch.log1p(rest), torch.log1p(rest) + rest * d / (1 + rest)
     # log(1 + s) = s - ..: no digit of s lost, s off by (d + 12) u of itself
-    for got, want, extra in ((lp, p[:, 77], 1), (best[:, 0], p[:, 77], 1), (ent, h, 2)):
+    for got, want, extra in ((lp, p, 1), (best[:, 0], p, 1), (ent, h, 2)):
         assert ((got.double() - want).abs() <= extra * 100 * U * want.abs()).all()
 
 

@@ -24,12 +24,14 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;  // that take logits; one more warp issues the copies
+constexpr int kThreads = 256, kWarps = kThreads / 32;  // that take logits; one more warp issues the copies
+constexpr int kCtas = 3;               // to an SM: one's end of a row runs under the others' streams
 constexpr int kMaxTop = 32;
-constexpr int kUnits = 2 * kThreads;   // 16-byte units to a stage
-constexpr int kStages = 12;
+constexpr int kHalf = 2 * kThreads;    // 16-byte units to a step: two neighbouring ones to a thread
+constexpr int kUnits = 2 * kHalf;      // and to a stage
+constexpr int kStages = 4;
 constexpr int kClasses = 64;
-constexpr int kCandidates = 1024;
+constexpr int kCandidates = 512;
 constexpr int kMaxParts = 8;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kRise = 3.0f;   // how far a logit may lie above a thread's reference before the reference moves
@@ -77,8 +79,8 @@ struct State {
 constexpr int kRing = kStages * kUnits * 16;
 constexpr int kSmem = kRing + (int)sizeof(State);
 
-// The larger of numbers and the first of equals: order of values, then of 16-byte units.
-__device__ __forceinline__ unsigned long long unit_key(float x, unsigned unit) { return key_of(x, (int)unit); }
+// The larger of numbers and the first of equals: order of values, then of pairs of units.
+__device__ __forceinline__ unsigned long long pair_key(float x, unsigned pair) { return key_of(x, (int)pair); }
 
 // A row's logits as 16-byte units from the aligned address at or before the first: `off` elements come before it.
 struct Row {
@@ -99,7 +101,7 @@ __device__ __forceinline__ void part_of(const Row &r, int p, int n, int *first, 
   *end = (int)((long long)r.count * (p + 1) / n);
 }
 // A unit's elements, -infinity for those that are not the row's.
-__device__ __forceinline__ void only_row(float (&x)[4], const Row &r, int unit, int vocab) {
+__device__ __forceinline__ void only_row(float *x, const Row &r, int unit, int vocab) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const long long at = 4ll * unit + i - r.off;
@@ -128,18 +130,18 @@ __device__ __forceinline__ void weigh(float d, float &s, float &t) {
   t = fmaf(w, d, t);
 }
 
-// A thread's running results: the maximum and the unit it first came in, and the sums s of e^(x - ref) and t of
-// e^(x - ref) (x - ref) over its elements, in two pairs.
+// A thread's running results: the maximum and the pair of units it first came in, and the sums s of e^(x - ref) and t of
+// e^(x - ref) (x - ref) over its elements, in four chains.
 struct Running {
   float max, ref;
-  unsigned unit;
+  unsigned pair;
   uint64_t s[2], t[2];
 };
-__device__ __forceinline__ void take(Running &r, const float (&x)[4], unsigned unit, bool *wrong) {
-  const float top = max3(max3(x[0], x[1], x[2]), x[3], x[3]);
+__device__ __forceinline__ void take(Running &r, const float (&x)[8], unsigned pair, bool *wrong) {
+  const float top = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), max3(x[5], x[6], x[7]), -INFINITY);
   *wrong |= !(top < INFINITY);
   if (top > r.max)
-    r.max = top, r.unit = unit;
+    r.max = top, r.pair = pair;
   if (top > r.ref + kRise) {
     const float by = fmaxf(r.ref - top, kLeast), f = ex2(by * kLog2e);
 #pragma unroll
@@ -149,16 +151,17 @@ __device__ __forceinline__ void take(Running &r, const float (&x)[4], unsigned u
     }
     r.ref = top;
   }
+  const uint64_t ref = f2_pack(-r.ref, -r.ref), scale = f2_pack(kLog2e, kLog2e);
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
+  for (int i = 0; i < 4; i++) {
     float d0, d1;
-    f2_unpack(f2_add(f2_pack(x[2 * i], x[2 * i + 1]), f2_pack(-r.ref, -r.ref)), d0, d1);
+    f2_unpack(f2_add(f2_pack(x[2 * i], x[2 * i + 1]), ref), d0, d1);
     const uint64_t d = f2_pack(fmaxf(d0, kLeast), fmaxf(d1, kLeast));
     float e0, e1;
-    f2_unpack(f2_mul(d, f2_pack(kLog2e, kLog2e)), e0, e1);
+    f2_unpack(f2_mul(d, scale), e0, e1);
     const uint64_t w = f2_pack(ex2(e0), ex2(e1));
-    r.s[i] = f2_add(r.s[i], w);
-    r.t[i] = f2_fma(w, d, r.t[i]);
+    r.s[i & 1] = f2_add(r.s[i & 1], w);
+    r.t[i & 1] = f2_fma(w, d, r.t[i & 1]);
   }
 }
 
@@ -168,7 +171,7 @@ __device__ __forceinline__ float log_p(float x, float max, float log_s) {
 }
 
 // A CTA per row, or a cluster of `parts`; each takes rows in turn.
-__global__ void __launch_bounds__(kThreads + 32, 1) logprobs_kernel(const LogprobArgs a, int parts) {
+__global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const LogprobArgs a, int parts) {
   extern __shared__ __align__(128) uint8_t smem[];
   State *t = reinterpret_cast<State *>(smem + kRing);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -223,34 +226,38 @@ __global__ void __launch_bounds__(kThreads + 32, 1) logprobs_kernel(const Logpro
       int first, end;
       part_of(r, part, parts, &first, &end);
       Running mine;
-      mine.max = -INFINITY, mine.ref = -3.402823466e+38f, mine.unit = first + tid;
+      mine.max = -INFINITY, mine.ref = -3.402823466e+38f, mine.pair = tid;
       mine.s[0] = mine.s[1] = mine.t[0] = mine.t[1] = 0;
       bool wrong = token < 0 || token >= a.vocab;
       for (int u = first; u < end; u += kUnits) {
         ok = ok && mbar_wait_bounded(&t->full[stage], parity);
-        const float4 *from = reinterpret_cast<const float4 *>(smem + stage * kUnits * 16) + tid;
-        float4 y[2];
+        // The two units in an order that keeps eight lanes in different banks.
+        const int swap = tid >> 2 & 1;
+        const float4 *from = reinterpret_cast<const float4 *>(smem + stage * kUnits * 16) + 2 * tid;
+        float x[2][8];
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-          y[h] = u + h * kThreads + tid < end ? from[h * kThreads] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        for (int h = 0; h < 4; h++) {
+          const int at = (h >> 1) * kHalf + ((h & 1) ^ swap);
+          const float4 y = u + 2 * tid + at < end ? from[at] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          float *to = &x[h >> 1][4 * (h & 1)];
+          to[0] = y.x, to[1] = y.y, to[2] = y.z, to[3] = y.w;
+        }
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&t->empty[stage]);
         if (++stage == kStages)
           stage = 0, parity ^= 1;
-        const bool edge = u == 0 || u + kUnits >= r.count;
+        if (u == 0 || u + kUnits >= r.count)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          float x[4] = {y[h].x, y[h].y, y[h].z, y[h].w};
-          const int unit = u + h * kThreads + tid;
-          if (edge)
-            only_row(x, r, unit, a.vocab);
-          take(mine, x, (unsigned)unit, &wrong);
-        }
+          for (int h = 0; h < 4; h++)
+            only_row(&x[h >> 1][4 * (h & 1)], r, u + 2 * tid + (h >> 1) * kHalf + ((h & 1) ^ swap), a.vocab);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          take(mine, x[h], (unsigned)(((u - first) + h * kHalf) / 2 + tid), &wrong);
       }
       wrong |= !ok;
       // ---- the end of the part: the maximum, and the class maximum that holds the top ones ----
-      const unsigned long long key = first + tid < end ? unit_key(mine.max, mine.unit) : 0;
+      const unsigned long long key = first + 2 * tid < end ? pair_key(mine.max, mine.pair) : 0;
       t->keys[tid] = key;
       if (wrong)
         t->wrong = 1;
@@ -300,22 +307,26 @@ __global__ void __launch_bounds__(kThreads + 32, 1) logprobs_kernel(const Logpro
       for (int m = warp; m < marked; m += kWarps) {
         const int who = t->who[m];
         const bool owner = t->keys[who] == best;
-        const unsigned best_unit = 0xffffffffu - (unsigned)best;
+        const unsigned best_pair = 0xffffffffu - (unsigned)best;
         float s2 = 0.0f, e2 = 0.0f;
-        for (int u0 = first + who; u0 < end; u0 += 32 * kThreads) {
-          const int unit = u0 + lane * kThreads;
+        for (int p0 = 0; first + 2 * (p0 + who) < end; p0 += 16 * kThreads) {  // 16 of its pairs at a time, a unit a lane
+          const int pair = p0 + who + (lane >> 1) * kThreads, unit = first + 2 * pair + (lane & 1);
           float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           if (unit < end) {
             const float4 y = __ldg(r.units + unit);
             x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
             only_row(x, r, unit, a.vocab);
           }
-          bool out = owner && (unsigned)unit == best_unit;  // the maximum is still to be left out
+          // The maximum is to be left out once: in the pair that it first came in, the first of it.
+          const bool here = owner && (unsigned)pair == best_pair;
+          const bool has = here && (x[0] == top || x[1] == top || x[2] == top || x[3] == top);
+          const unsigned holders = __ballot_sync(0xffffffffu, has);
+          bool out = has && lane == __ffs(holders) - 1;
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             const long long at = 4ll * unit + i - r.off;
             const bool in = unit < end && at >= 0 && at < a.vocab;
-            if (in && unit_key(x[i], (unsigned)unit) >= least) {
+            if (in && pair_key(x[i], (unsigned)pair) >= least) {
               const int n = atomicAdd(&t->found, 1);
               if (n < kCandidates)
                 t->candidates[n] = key_of(x[i], (int)at);
@@ -482,11 +493,11 @@ extern "C" void k_token_logprobs(float *logprobs, float *entropy, int *top_token
   // one); from half as many rows as SMs on a CTA to each.
   const int sms = kc_device_sms();
   int parts = kMaxParts;
-  while (parts > 1 && (long long)rows * parts > sms)
+  while (parts > 1 && (long long)rows * parts > kCtas * sms)
     parts /= 2;
   cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(logprobs_kernel), kSmem);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * (long long)parts < sms ? rows * parts : parts > 1 ? rows * parts : sms));
+  cfg.gridDim = dim3((unsigned)(parts > 1 || rows < kCtas * sms ? rows * parts : kCtas * sms));
   cfg.blockDim = dim3(kThreads + 32);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = kc_stream();

@@ -32,6 +32,7 @@ constexpr int kUnits = 2 * kHalf;      // and to a stage
 constexpr int kStages = 4;
 constexpr int kClasses = 64;
 constexpr int kCandidates = 512;
+constexpr int kLooks = 4;
 constexpr int kMaxParts = 8;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kRise = 3.0f;   // how far a logit may lie above a thread's reference before the reference moves
@@ -73,7 +74,7 @@ struct State {
   unsigned long long candidates[kCandidates];
   unsigned long long merged[kMaxParts * kMaxTop];
   float sums[2][kWarps], again[2];  // the warps' sums; the sums of the thread that has the maximum, without it
-  int marked, found, wrong, verdict;
+  int marked, found, wrong, verdict, owner;
   unsigned short who[kThreads];  // threads whose maximum may be a top one
 };
 constexpr int kRing = kStages * kUnits * 16;
@@ -119,6 +120,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN where
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ unsigned long long max_key(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
@@ -137,25 +143,33 @@ struct Running {
   unsigned pair;
   uint64_t s[2], t[2];
 };
-__device__ __forceinline__ void take(Running &r, const float (&x)[8], unsigned pair, bool *wrong) {
-  const float top = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), max3(x[5], x[6], x[7]), -INFINITY);
-  *wrong |= !(top < INFINITY);
-  if (top > r.max)
-    r.max = top, r.pair = pair;
-  if (top > r.ref + kRise) {
-    const float by = fmaxf(r.ref - top, kLeast), f = ex2(by * kLog2e);
+// Two steps' elements: of the pairs `pair` and `pair` + kThreads.
+__device__ __forceinline__ void take(Running &r, const float (&x)[2][8], unsigned pair, bool *wrong) {
+  float top[2];
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+    top[h] = max3(max3(x[h][0], x[h][1], x[h][2]), max3(x[h][3], x[h][4], x[h][5]), fmax_nan(x[h][6], x[h][7]));
+  const float high = fmax_nan(top[0], top[1]);
+  *wrong |= !(high < INFINITY);
+  if (high > r.max) {
+    r.pair = top[0] == high ? pair : pair + kThreads;
+    r.max = high;
+  }
+  if (high > r.ref + kRise) {
+    const float by = fmaxf(r.ref - high, kLeast), f = ex2(by * kLog2e);
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       r.t[i] = f2_mul(f2_fma(f2_pack(by, by), r.s[i], r.t[i]), f2_pack(f, f));
       r.s[i] = f2_mul(r.s[i], f2_pack(f, f));
     }
-    r.ref = top;
+    r.ref = high;
   }
   const uint64_t ref = f2_pack(-r.ref, -r.ref), scale = f2_pack(kLog2e, kLog2e);
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
+  for (int i = 0; i < 8; i++) {
+    const float *at = &x[i >> 2][2 * (i & 3)];
     float d0, d1;
-    f2_unpack(f2_add(f2_pack(x[2 * i], x[2 * i + 1]), ref), d0, d1);
+    f2_unpack(f2_add(f2_pack(at[0], at[1]), ref), d0, d1);
     const uint64_t d = f2_pack(fmaxf(d0, kLeast), fmaxf(d1, kLeast));
     float e0, e1;
     f2_unpack(f2_mul(d, scale), e0, e1);
@@ -229,6 +243,7 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
       mine.max = -INFINITY, mine.ref = -3.402823466e+38f, mine.pair = tid;
       mine.s[0] = mine.s[1] = mine.t[0] = mine.t[1] = 0;
       bool wrong = token < 0 || token >= a.vocab;
+      const float given = tid == 0 && part == 0 && !wrong ? __ldcg(a.logits + (size_t)row * a.ld + token) : 0.0f;
       for (int u = first; u < end; u += kUnits) {
         ok = ok && mbar_wait_bounded(&t->full[stage], parity);
         // The two units in an order that keeps eight lanes in different banks.
@@ -242,18 +257,19 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
           float *to = &x[h >> 1][4 * (h & 1)];
           to[0] = y.x, to[1] = y.y, to[2] = y.z, to[3] = y.w;
         }
+        if (u == 0 || u + kUnits >= r.count)
+#pragma unroll
+          for (int h = 0; h < 4; h++)
+            only_row(&x[h >> 1][4 * (h & 1)], r, u + 2 * tid + (h >> 1) * kHalf + ((h & 1) ^ swap), a.vocab);
+        take(mine, x, (unsigned)((u - first) / 2 + tid), &wrong);
+        // The stage is given back only now, behind the fence between this warp's reads and the next copy's writes: before it,
+        // loads still under way read what the copy brought (one row in a hundred wrong at 2048 rows of 128256).
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&t->empty[stage]);
         if (++stage == kStages)
           stage = 0, parity ^= 1;
-        if (u == 0 || u + kUnits >= r.count)
-#pragma unroll
-          for (int h = 0; h < 4; h++)
-            only_row(&x[h >> 1][4 * (h & 1)], r, u + 2 * tid + (h >> 1) * kHalf + ((h & 1) ^ swap), a.vocab);
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-          take(mine, x[h], (unsigned)(((u - first) + h * kHalf) / 2 + tid), &wrong);
       }
       wrong |= !ok;
       // ---- the end of the part: the maximum, and the class maximum that holds the top ones ----
@@ -283,6 +299,8 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
       const bool bad = t->wrong != 0;
       if (key != 0 && key >= least)
         t->who[atomicAdd(&t->marked, 1)] = (unsigned short)tid;
+      if (key == best)
+        t->owner = tid;  // the one of them that has the maximum (or any, where there is none)
       // ---- the sums, relative to the maximum; the thread that has it leaves its own to the second look ----
       float s, e;
       {
@@ -302,48 +320,66 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
       if (lane == 0)
         t->sums[0][warp] = s, t->sums[1][warp] = e;
       meet();
-      // ---- the second look at the marked threads' units, a warp to a thread ----
+      // ---- the second look at the marked threads' units: 16 of a thread's pairs, a unit a lane, kLooks times at once. The
+      // first warp looks at the thread that has the maximum, and sums the rest of it up again. ----
       const int marked = bad ? 0 : t->marked;
-      for (int m = warp; m < marked; m += kWarps) {
-        const int who = t->who[m];
-        const bool owner = t->keys[who] == best;
-        const unsigned best_pair = 0xffffffffu - (unsigned)best;
-        float s2 = 0.0f, e2 = 0.0f;
-        for (int p0 = 0; first + 2 * (p0 + who) < end; p0 += 16 * kThreads) {  // 16 of its pairs at a time, a unit a lane
-          const int pair = p0 + who + (lane >> 1) * kThreads, unit = first + 2 * pair + (lane & 1);
-          float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          if (unit < end) {
-            const float4 y = __ldg(r.units + unit);
-            x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+      const int each = (end - first + 2 * 16 * kThreads - 1) / (2 * 16 * kThreads);  // looks at a thread's pairs
+      const int looks = warp == 0 ? (marked ? each : 0) : marked * each;
+      const unsigned best_pair = 0xffffffffu - (unsigned)best;
+      const float edge = least ? logit_of(least) : -INFINITY;
+      float s2 = 0.0f, e2 = 0.0f;
+      for (int i0 = warp == 0 ? 0 : warp - 1; i0 < looks; i0 += warp == 0 ? kLooks : kLooks * (kWarps - 1)) {
+        float4 y[kLooks];
+        int pair[kLooks];
+        bool in[kLooks];
+#pragma unroll
+        for (int k = 0; k < kLooks; k++) {
+          const int i = i0 + k * (warp == 0 ? 1 : kWarps - 1), who = warp == 0 ? t->owner : t->who[min(i, looks - 1) / each];
+          const int look = warp == 0 ? i : i % each;
+          pair[k] = look * 16 * kThreads + who + (lane >> 1) * kThreads;
+          in[k] = i < looks && first + 2 * pair[k] + (lane & 1) < end && (warp == 0 || who != t->owner);
+          y[k] = in[k] ? __ldcg(r.units + first + 2 * pair[k] + (lane & 1)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < kLooks; k++) {
+          const int unit = first + 2 * pair[k] + (lane & 1);
+          float x[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
+          if (unit == 0 || unit == r.count - 1)
             only_row(x, r, unit, a.vocab);
-          }
-          // The maximum is to be left out once: in the pair that it first came in, the first of it.
-          const bool here = owner && (unsigned)pair == best_pair;
-          const bool has = here && (x[0] == top || x[1] == top || x[2] == top || x[3] == top);
-          const unsigned holders = __ballot_sync(0xffffffffu, has);
-          bool out = has && lane == __ffs(holders) - 1;
+          if (in[k] && fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= edge) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const long long at = 4ll * unit + i - r.off;
-            const bool in = unit < end && at >= 0 && at < a.vocab;
-            if (in && pair_key(x[i], (unsigned)pair) >= least) {
-              const int n = atomicAdd(&t->found, 1);
-              if (n < kCandidates)
-                t->candidates[n] = key_of(x[i], (int)at);
+            for (int j = 0; j < 4; j++) {
+              const long long at = 4ll * unit + j - r.off;
+              if (at >= 0 && at < a.vocab && pair_key(x[j], (unsigned)pair[k]) >= least) {
+                const int n = atomicAdd(&t->found, 1);
+                if (n < kCandidates)
+                  t->candidates[n] = key_of(x[j], (int)at);
+              }
             }
-            if (out && x[i] == top)
-              out = false;
-            else if (owner && in)
-              weigh(x[i] - top, s2, e2);
+          }
+          if (warp == 0) {
+            // The maximum is left out once: in the pair that it first came in, the first of it. (What is not the row's is
+            // -infinity, and adds nothing.)
+            if (!in[k])
+              x[0] = x[1] = x[2] = x[3] = -INFINITY;
+            const bool has = (unsigned)pair[k] == best_pair && fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) == top;
+            const unsigned holders = __ballot_sync(0xffffffffu, has);
+            bool out = has && lane == __ffs(holders) - 1;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              if (out && x[j] == top)
+                x[j] = -INFINITY, out = false;
+              weigh(x[j] - top, s2, e2);
+            }
           }
         }
-        if (owner) {
+      }
+      if (warp == 0) {
 #pragma unroll
-          for (int o = 16; o; o >>= 1)
-            s2 += __shfl_xor_sync(0xffffffffu, s2, o), e2 += __shfl_xor_sync(0xffffffffu, e2, o);
-          if (lane == 0)
-            t->again[0] = s2, t->again[1] = e2;
-        }
+        for (int o = 16; o; o >>= 1)
+          s2 += __shfl_xor_sync(0xffffffffu, s2, o), e2 += __shfl_xor_sync(0xffffffffu, e2, o);
+        if (lane == 0)
+          t->again[0] = s2, t->again[1] = e2;
       }
       meet();
       // ---- the top ones in order ----
@@ -352,14 +388,15 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
         t->part.top[tid] = 0;
       if (tid == 0) {
         const bool some = top > -INFINITY;
-        float s2 = some ? t->again[0] : 0.0f, e2 = some ? t->again[1] : 0.0f;
+        float s2 = some && !bad ? t->again[0] : 0.0f, e2 = some && !bad ? t->again[1] : 0.0f;
         for (int w = 0; w < kWarps; w++)
           s2 += t->sums[0][w], e2 += t->sums[1][w];
         t->part.max = some ? top : -INFINITY, t->part.s = s2, t->part.t = -e2;
         t->part.wrong = bad;
-        t->marked = t->found = t->wrong = 0;
       }
       meet();
+      if (tid == 0)
+        t->marked = t->found = t->wrong = 0;  // everybody has read them
       if (!bad && found <= kCandidates) {
         for (int i = tid; i < found; i += kThreads) {
           const unsigned long long k = t->candidates[i];
@@ -375,7 +412,7 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
         for (int n = 0; n < wanted; n++) {
           unsigned long long k = 0;
           for (int unit = first + tid; unit < end; unit += kThreads) {
-            const float4 y = __ldg(r.units + unit);
+            const float4 y = __ldcg(r.units + unit);
             const float x[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -436,7 +473,7 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
           if (w)
             kc_raise(KC_ERR_BAD_ARGS);
           if (a.logprobs)
-            a.logprobs[row] = w ? NAN : log_p(a.logits[(size_t)row * a.ld + token], max, log_s);
+            a.logprobs[row] = w ? NAN : log_p(given, max, log_s);
           if (a.entropy)
             a.entropy[row] = w ? NAN : log_s + e3 / (1.0f + s3);
           t->sums[0][0] = max, t->sums[0][1] = log_s, t->verdict = w;
@@ -489,12 +526,16 @@ extern "C" void k_token_logprobs(float *logprobs, float *entropy, int *top_token
   memset(&a, 0, sizeof(a));
   a.logprobs = logprobs, a.entropy = entropy, a.top_tokens = top_tokens, a.top_logprobs = top_logprobs;
   a.logits = logits, a.ld = ld, a.tokens = tokens, a.vocab = vocab, a.rows = rows, a.top = top;
-  // With few rows a cluster of CTAs to each, as many as there are SMs for (one row of 128256: @@ us with 8 parts, @@ with
-  // one); from half as many rows as SMs on a CTA to each.
+  // A cluster of CTAs to a row while their parts are long enough to pay for its two barriers: 2 us where every CTA has an
+  // SM to itself (8 rows of 128256: 23 us in one part, 12 in four; 64 rows of 32000: 9.9 in one, 10.6 in two), 4 to 5 us
+  // where they share them (200 rows of 128256: 30 us in one part, 27 in two; 129 rows of 50001: 12 in one, 16 in two).
   const int sms = kc_device_sms();
-  int parts = kMaxParts;
-  while (parts > 1 && (long long)rows * parts > kCtas * sms)
-    parts /= 2;
+  int parts = 1;
+  for (; parts < kMaxParts; parts *= 2) {
+    const long long ctas = (long long)rows * parts * 2;
+    if (ctas > kCtas * sms || vocab / (2 * parts) < (ctas <= sms ? 16384 : 49152))
+      break;
+  }
   cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(logprobs_kernel), kSmem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(parts > 1 || rows < kCtas * sms ? rows * parts : kCtas * sms));

@@ -761,6 +761,26 @@ def test_logprobs_many_candidates(kc, period, top):
     check_logprobs(x, tokens, top, got)
 
 
+@pytest.mark.parametrize("rows,vocab,top", [(2048, 128256, 5), (1000, 60001, 20), (64, 128256, 20)])
+def test_logprobs_many_rows_again_and_again(kc, rows, vocab, top):
+    """Every row of many, with the memory busy: the stages of the ring are read before they are written again."""
+    g = generator(vocab)
+    inputs = [3 * normal(g, rows, vocab) for _ in range(2)]
+    tokens = [int(t) for t in np.random.default_rng(rows).integers(0, vocab, rows)]
+    at = dev(tokens).long()[:, None]
+    want = []
+    for x in inputs:
+        p = torch.cat([torch.log_softmax(y.double(), -1).gather(1, t) for y, t in zip(x.split(256), at.split(256))])
+        want.append((p[:, 0], torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top].int()))
+    for i in range(12):
+        lp, _, ids, _ = run_logprobs(kc, inputs[i % 2], tokens, top)
+        p, order = want[i % 2]
+        # three standard deviations of the logits cover the mean of d: E d <= 30
+        assert ((lp.double() - p).abs() <= U * (p.abs() + 30 + 12)).all()
+        assert torch.equal(ids, order)
+    assert kc.status() == 0
+
+
 def test_logprobs_small_differences_from_certainty(kc):
     """The likeliest token's log probability -e and the entropy of a row that is nearly certain keep their own digits."""
     vocab = 2000

@@ -39,6 +39,7 @@ struct StoreArgs {
   long long q_out_ld, q_ld, kv_ld;
   size_t page_stride;
   int pages, page_size, max_pages, positions, n_heads, n_kv, hd, batch, rows, per_row;
+  Divisor by_rows, by_page, by_units;  // units: of four elements, to a head
 };
 
 __device__ __forceinline__ void put(float *at, float a, float b) { at[0] = a, at[1] = b; }
@@ -49,7 +50,88 @@ __device__ __forceinline__ void put(__half *at, float a, float b) {
   at[0] = __float2half_rn(a), at[1] = __float2half_rn(b);
 }
 
-// A thread per pair of a row's queries, keys or values.
+__device__ __forceinline__ void put4(float *at, float4 x) { *reinterpret_cast<float4 *>(at) = x; }
+__device__ __forceinline__ void put4(__nv_bfloat16 *at, float4 x) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x, x.y), hi = __floats2bfloat162_rn(x.z, x.w);
+  *reinterpret_cast<uint2 *>(at) =
+      make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+}
+__device__ __forceinline__ void put4(__half *at, float4 x) {
+  const __half2 lo = __floats2half2_rn(x.x, x.y), hi = __floats2half2_rn(x.z, x.w);
+  *reinterpret_cast<uint2 *>(at) =
+      make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+}
+
+// head_dim a multiple of four and everything aligned to four elements: a CTA, or a few with few rows, to a row; each thread
+// has kStoreUnits units of four elements on their way at once. What bounds it: memory, 2048 rows of 32/8 heads of 128 @@ us,
+// @@ TB/s; with few rows the chain starts, page and rotation, store.
+constexpr int kStoreThreads = 256, kStoreUnits = 6;
+template <typename T>
+__global__ void __launch_bounds__(kStoreThreads) paged_store4_kernel(const StoreArgs a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int row = blockIdx.x;
+  int r = row;
+  const int b = divide(r, a.by_rows);
+  const Request request = request_of(a.starts, a.counts, b, a.rows, a.positions);
+  if (request.bad && r == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+    kc_raise(KC_ERR_BAD_ARGS);
+  if (r >= request.count)
+    return;
+  const int position = request.start + r;
+  int within = position;
+  const int at = divide(within, a.by_page), page = a.table[(size_t)b * a.max_pages + at];
+  const float *table = a.rope + (size_t)position * 2 * a.hd;
+  const int units = a.per_row / 2, heads = a.n_heads + a.n_kv;
+  for (int u0 = blockIdx.y * kStoreThreads + threadIdx.x; u0 < units; u0 += gridDim.y * kStoreThreads * kStoreUnits) {
+    float4 x[kStoreUnits], c[kStoreUnits], s[kStoreUnits];
+    int head[kStoreUnits], j[kStoreUnits];
+#pragma unroll
+    for (int i = 0; i < kStoreUnits; i++) {
+      const int u = u0 + i * gridDim.y * kStoreThreads;
+      if (u >= units)
+        break;
+      j[i] = u;
+      head[i] = divide(j[i], a.by_units);
+      j[i] *= 4;
+      const float *src = head[i] < a.n_heads ? a.q + row * a.q_ld + (size_t)head[i] * a.hd
+                         : head[i] < heads   ? a.k + row * a.kv_ld + (size_t)(head[i] - a.n_heads) * a.hd
+                                             : a.v + row * a.kv_ld + (size_t)(head[i] - heads) * a.hd;
+      x[i] = *reinterpret_cast<const float4 *>(src + j[i]);
+      if (head[i] < heads) {
+        c[i] = *reinterpret_cast<const float4 *>(table + j[i]);
+        s[i] = *reinterpret_cast<const float4 *>(table + a.hd + j[i]);
+      }
+    }
+    if (page < 0 || page >= a.pages) {
+      if (threadIdx.x == 0)
+        kc_raise(KC_ERR_BAD_ARGS);
+      return;
+    }
+    const size_t place = (size_t)page * a.page_stride + (size_t)within * a.hd;
+#pragma unroll
+    for (int i = 0; i < kStoreUnits; i++) {
+      if (u0 + i * gridDim.y * kStoreThreads >= units)
+        break;
+      float4 y = x[i];
+      if (head[i] < heads) {  // (a, b) to (a cos - b sin, a sin + b cos), each product rounded
+        y.x = __fsub_rn(__fmul_rn(x[i].x, c[i].x), __fmul_rn(x[i].y, s[i].y));
+        y.y = __fadd_rn(__fmul_rn(x[i].x, s[i].y), __fmul_rn(x[i].y, c[i].x));
+        y.z = __fsub_rn(__fmul_rn(x[i].z, c[i].z), __fmul_rn(x[i].w, s[i].w));
+        y.w = __fadd_rn(__fmul_rn(x[i].z, s[i].w), __fmul_rn(x[i].w, c[i].z));
+      }
+      if (head[i] < a.n_heads) {
+        *reinterpret_cast<float4 *>(a.q_out + row * a.q_out_ld + (size_t)head[i] * a.hd + j[i]) = y;
+      } else {
+        const bool is_k = head[i] < heads;
+        T *cache = static_cast<T *>(is_k ? a.key : a.value);
+        put4(cache + place + (size_t)(head[i] - (is_k ? a.n_heads : heads)) * a.page_size * a.hd + j[i], y);
+      }
+    }
+  }
+}
+
+// A thread per pair of a row's queries, keys or values: any even head_dim and any alignment.
 template <typename T>
 __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
   pdl_wait();
@@ -328,6 +410,22 @@ bool heads_ok(int n_heads, int n_kv, int hd, int batch, int rows) {
          (long long)batch * rows <= most && (long long)batch * rows * n_heads <= most;
 }
 
+template <typename T>
+cudaError_t launch_store(const StoreArgs &a) {
+  const uintptr_t wide = (uintptr_t)a.q | (uintptr_t)a.q_out | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.rope |
+                         (a.q_ld | a.q_out_ld | a.kv_ld | a.hd) * sizeof(float);
+  const uintptr_t cache = (uintptr_t)a.key | (uintptr_t)a.value | a.page_stride * sizeof(T);
+  const long long rows = (long long)a.batch * a.rows;
+  if (wide % 16 == 0 && cache % (4 * sizeof(T)) == 0) {
+    // About two CTAs to an SM with few rows (one row of 32/8 heads of 64: three CTAs).
+    const long long most = (a.per_row / 2 + kStoreThreads - 1) / kStoreThreads, want = 2 * kc_device_sms() / rows;
+    const long long parts = want < 1 ? 1 : want < most ? want : most;
+    return kc_launch_pdl(paged_store4_kernel<T>, dim3((unsigned)rows, (unsigned)parts), dim3(kStoreThreads), 0, kc_stream(),
+                         a);
+  }
+  return kc_launch_pdl(paged_store_kernel<T>, dim3((unsigned)((rows * a.per_row + 255) / 256)), dim3(256), 0, kc_stream(), a);
+}
+
 const char *cache_fault(const PagedCache *c, int n_kv, int hd) {
   if (!c || !c->key || !c->value || !c->table)
     return "missing keys, values or page table";
@@ -415,12 +513,10 @@ void k_rope_kv_store_paged(float *q_out, size_t q_out_ld, const float *q, size_t
     kc_fail("%s: %d requests of %d rows are too many for one call", name, batch, rows);
     return;
   }
-  const dim3 grid((unsigned)ctas), threads(256);
-  const cudaError_t e =
-      cache->type == K_F32 ? kc_launch_pdl(paged_store_kernel<float>, grid, threads, 0, kc_stream(), a)
-      : cache->type == K_BF16
-          ? kc_launch_pdl(paged_store_kernel<__nv_bfloat16>, grid, threads, 0, kc_stream(), a)
-          : kc_launch_pdl(paged_store_kernel<__half>, grid, threads, 0, kc_stream(), a);
+  a.by_rows = divisor(rows), a.by_page = divisor(a.page_size), a.by_units = divisor(head_dim < 4 ? 1 : head_dim / 4);
+  const cudaError_t e = cache->type == K_F32    ? launch_store<float>(a)
+                        : cache->type == K_BF16 ? launch_store<__nv_bfloat16>(a)
+                                                : launch_store<__half>(a);
   if (e == cudaSuccess)
     kc_count_launch();
   else

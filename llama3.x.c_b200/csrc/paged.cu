@@ -177,13 +177,16 @@ __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
 
 // ---- attention ----------------------------------------------------------------------------------------------------
 
-// The kernel on the CUDA cores: any type, head_dim up to 256, any alignment. LANES lanes take a position, 16 of its
-// elements each, so that a score costs log2(LANES) shuffles for 16 LANES products, and its weight meets the values in the
-// same lanes without another; four query vectors in registers share each key and value.
-constexpr int kVecs = 4, kElems = 16, kPairs = kElems / 2;
+// The kernel on the CUDA cores: any type, head_dim up to 256, any alignment. LANES lanes take a position, ELEMS of its
+// elements each, so that a score costs log2(LANES) shuffles for ELEMS LANES products, and its weight meets the values in the
+// same lanes without another; VECS query vectors in registers share each key and value (four with 16 elements to a lane, or
+// eight with eight). Every warp has a ring of its own in shared memory, which each lane fills for itself, asynchronously, and
+// reads itself: no barrier until the end of a piece. What bounds it: @@
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kTile = 64;       // positions
 constexpr int kCtas = 148 * 3;  // the shares; a function of nothing else, so that the workspace's size is known
+constexpr int kStages = 4;
+constexpr int kRowsBlock = 8;  // query vectors to a segment at most
 
 // A pair of elements in 32 bits each.
 __device__ __forceinline__ uint64_t pair_of(uint32_t x, __nv_bfloat16) { return f2_pack_bits(x << 16, x & 0xffff0000u); }
@@ -195,30 +198,47 @@ __device__ __forceinline__ float one_of(float x) { return x; }
 __device__ __forceinline__ float one_of(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float one_of(__half x) { return __half2float(x); }
 
-// This lane's 16 elements of a row: wide, 16-byte units LANES apart; else elements LANES apart, pairs of neighbours in i.
-template <typename T, int LANES, bool WIDE>
+// 16 bytes from global to shared memory, asynchronously; zeros without `in`.
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// This lane's ELEMS elements of a row: wide, 16-byte units LANES apart; else elements LANES apart.
+template <typename T, int LANES, int ELEMS, bool WIDE>
 struct Row {
   static constexpr int kUnit = 16 / sizeof(T);
-  static constexpr int kUnits = kElems / kUnit;
+  static constexpr int kUnits = ELEMS / kUnit;
   uint4 raw[WIDE ? kUnits : 1];
-  T one[WIDE ? 1 : kElems];
+  T one[WIDE ? 1 : ELEMS];
 
-  // The element behind index i of the lane's 16.
+  // The element behind index i of the lane's.
   static __device__ __forceinline__ int element(int lane, int i) {
     return WIDE ? (lane + LANES * (i / kUnit)) * kUnit + i % kUnit : lane + LANES * i;
   }
-  __device__ __forceinline__ void load(const T *row, bool in, int hd, int lane) {
-    if (WIDE) {
+  // Starts this lane's copies to a slot of kUnits times 32 units, and reads them back.
+  static __device__ __forceinline__ void copy(uint4 *slot, const T *row, bool in, int hd, int sub, int lane) {
 #pragma unroll
-      for (int u = 0; u < kUnits; u++)
-        raw[u] = in && (lane + LANES * u) * kUnit < hd
-                     ? *reinterpret_cast<const uint4 *>(row + (lane + LANES * u) * kUnit)
-                     : make_uint4(0, 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kElems; i++)
-        one[i] = in && lane + LANES * i < hd ? row[lane + LANES * i] : T(0.0f);
+    for (int u = 0; u < kUnits; u++) {
+      const int at = (sub + LANES * u) * kUnit;
+      copy16(slot + 32 * u + lane, row + (at < hd ? at : 0), in && at < hd);
     }
+  }
+  __device__ __forceinline__ void take(const uint4 *slot, int lane) {
+#pragma unroll
+    for (int u = 0; u < kUnits; u++)
+      raw[u] = slot[32 * u + lane];
+  }
+  __device__ __forceinline__ void load(const T *row, bool in, int hd, int lane) {
+#pragma unroll
+    for (int i = 0; i < ELEMS; i++)
+      one[i] = in && lane + LANES * i < hd ? row[lane + LANES * i] : T(0.0f);
   }
   __device__ __forceinline__ uint64_t pair(int i) const {  // elements 2 i, 2 i + 1
     if (!WIDE)
@@ -233,14 +253,27 @@ struct Row {
   }
 };
 
-template <typename T, int LANES, bool WIDE>
-__global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedArgs a) {
-  constexpr int kAt = 32 / LANES;  // positions of a warp at a time
+// Shared memory: the warps' rings (nothing where they are not used), and over them their results at the end of a piece.
+template <typename T, int LANES, int ELEMS, int VECS, bool WIDE>
+struct RowsSmem {
+  using R = Row<T, LANES, ELEMS, WIDE>;
+  static constexpr int slot = 32 * R::kUnits;                            // units of a key or a value
+  static constexpr int ring = WIDE ? kStages * 2 * slot * 16 : 0;        // bytes to a warp
+  static constexpr int sums = VECS * LANES * ELEMS * (int)sizeof(float);  // of a warp
+  static constexpr int total = kWarps * (ring > sums ? ring : sums);
+};
+
+template <typename T, int LANES, int ELEMS, int VECS, bool WIDE>
+__global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs a) {
+  using S = RowsSmem<T, LANES, ELEMS, VECS, WIDE>;
+  using R = typename S::R;
+  constexpr int kAt = 32 / LANES, kStep = kWarps * kAt, kPairs = ELEMS / 2;  // positions of a warp, of all warps at a time
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ RangeRoom room;
-  __shared__ __align__(16) float sums[kWarps][kVecs][LANES * kElems];
-  __shared__ float wm[kWarps][kVecs], wl[kWarps][kVecs], m_all[kVecs], l_all[kVecs];
+  __shared__ float wm[kWarps][VECS], wl[kWarps][VECS], m_all[VECS], l_all[VECS];
   __shared__ int bad, last;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, sub = lane % LANES, at = lane / LANES;
+  uint4 *const ring = reinterpret_cast<uint4 *>(smem + warp * S::ring);
   pdl_wait();
   pdl_launch_dependents();
   if (t == 0)
@@ -253,100 +286,155 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedArgs a)
   Walk walk(&range);
   Piece p;
   while (walk.next(a, &range, kTile, &p)) {
-    uint64_t q[kVecs][kPairs], acc[kVecs][kPairs];
-    float m[kVecs], l[kVecs];
-    int limit[kVecs];
+    const int end = min(p.t1 * kTile, p.start + p.count), first = p.t0 * kTile + warp * kAt + at;
+    const int steps = (end - p.t0 * kTile + kStep - 1) / kStep;
+    const float guard = guard_of(p.start + p.count);
+    const int *pages = a.table + (size_t)p.b * a.max_pages;
+    const size_t head = (size_t)p.head * a.page_size * hd;
+    // Step i's page (-2: no position of the piece), and where its row lies.
+    auto page_of = [&](int i) {
+      int position = first + i * kStep;
+      return position < end ? pages[divide(position, a.by_page)] : -2;
+    };
+    auto row_of = [&](int i, int page, bool *in) {
+      int within = first + i * kStep;
+      *in = page >= 0 && page < a.pages;
+      if (!*in && page != -2)
+        bad = 1;
+      divide(within, a.by_page);
+      return *in ? (size_t)page * a.page_stride + head + (size_t)within * hd : 0;
+    };
+    auto fetch = [&](int i, int page) {
+      bool in;
+      const size_t place = row_of(i, page, &in);
+      uint4 *slot = ring + (i % kStages) * 2 * S::slot;
+      R::copy(slot, static_cast<const T *>(a.key) + place, in, hd, sub, lane);
+      R::copy(slot + S::slot, static_cast<const T *>(a.value) + place, in, hd, sub, lane);
+    };
+    int page = page_of(0);  // of the step fetched next
+    if (WIDE) {
 #pragma unroll
-    for (int v = 0; v < kVecs; v++) {
+      for (int i = 0; i < kStages - 1; i++) {
+        const int next = page_of(i + 1);
+        fetch(i, page);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        page = next;
+      }
+    }
+    uint64_t q[VECS][kPairs], acc[VECS][kPairs];
+    float m[VECS], l[VECS];
+    int limit[VECS];
+#pragma unroll
+    for (int v = 0; v < VECS; v++) {
       int row = 0;
       const size_t vec = v < p.vecs ? vector_at(a, p, v, &row) : 0;
       limit[v] = v < p.vecs ? p.start + row + 1 : 0;
       m[v] = -INFINITY, l[v] = 0.0f;
 #pragma unroll
       for (int i = 0; i < kPairs; i++) {
-        const int e0 = Row<T, LANES, WIDE>::element(sub, 2 * i), e1 = Row<T, LANES, WIDE>::element(sub, 2 * i + 1);
+        const int e0 = R::element(sub, 2 * i), e1 = R::element(sub, 2 * i + 1);
         const float x = v < p.vecs && e0 < hd ? a.q[vec * hd + e0] * scale : 0.0f;
         const float y = v < p.vecs && e1 < hd ? a.q[vec * hd + e1] * scale : 0.0f;
         q[v][i] = f2_pack(x, y), acc[v][i] = 0;
       }
     }
-    const int end = min(p.t1 * kTile, p.start + p.count);
-    const float guard = guard_of(p.start + p.count);
-    const int *pages = a.table + (size_t)p.b * a.max_pages;
-    const size_t head = (size_t)p.head * a.page_size * hd;
-    for (int p0 = p.t0 * kTile + warp * kAt; p0 < end; p0 += kWarps * kAt) {
-      const int position = p0 + at;
-      bool in = position < end;
-      int within = position;
-      const int index = in ? divide(within, a.by_page) : 0;
-      const int page = in ? pages[index] : 0;
-      if (page < 0 || page >= a.pages) {
-        bad = 1;
-        in = false;
+    for (int i = 0; i < steps; i++) {
+      const int position = first + i * kStep;
+      R k, x;
+      if (WIDE) {
+        const int next = page_of(i + kStages);
+        fetch(i + kStages - 1, page);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        page = next;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        const uint4 *slot = ring + (i % kStages) * 2 * S::slot;
+        k.take(slot, lane);
+        x.take(slot + S::slot, lane);
+      } else {
+        bool in;
+        const size_t place = row_of(i, page, &in);
+        page = page_of(i + 1);
+        k.load(static_cast<const T *>(a.key) + place, in, hd, sub);
+        x.load(static_cast<const T *>(a.value) + place, in, hd, sub);
       }
-      const size_t place = in ? (size_t)page * a.page_stride + head + (size_t)within * hd : 0;
-      Row<T, LANES, WIDE> k, x;
-      k.load(static_cast<const T *>(a.key) + place, in, hd, sub);
-      x.load(static_cast<const T *>(a.value) + place, in, hd, sub);
-      float s[kVecs];
-      uint64_t part[kVecs];
+      float s[VECS];
+      uint64_t part[VECS];
 #pragma unroll
-      for (int v = 0; v < kVecs; v++)
+      for (int v = 0; v < VECS; v++)
         part[v] = 0;
 #pragma unroll
-      for (int i = 0; i < kPairs; i++) {
-        const uint64_t ki = k.pair(i);
+      for (int j = 0; j < kPairs; j++) {
+        const uint64_t kj = k.pair(j);
 #pragma unroll
-        for (int v = 0; v < kVecs; v++)
-          part[v] = f2_fma(q[v][i], ki, part[v]);
+        for (int v = 0; v < VECS; v++)
+          part[v] = f2_fma(q[v][j], kj, part[v]);
       }
       bool rises = false;
 #pragma unroll
-      for (int v = 0; v < kVecs; v++) {
+      for (int v = 0; v < VECS; v++) {
         float lo, hi;
         f2_unpack(part[v], lo, hi);
         s[v] = lo + hi;
+      }
 #pragma unroll
-        for (int o = LANES / 2; o; o >>= 1)
+      for (int o = LANES / 2; o; o >>= 1)
+#pragma unroll
+        for (int v = 0; v < VECS; v++)
           s[v] += __shfl_xor_sync(0xffffffffu, s[v], o);
-        s[v] = in && position < limit[v] ? s[v] : -INFINITY;
+#pragma unroll
+      for (int v = 0; v < VECS; v++) {
+        s[v] = position < min(limit[v], end) ? s[v] : -INFINITY;
         rises |= s[v] > m[v];
       }
       if (rises) {
 #pragma unroll
-        for (int v = 0; v < kVecs; v++) {
+        for (int v = 0; v < VECS; v++) {
           if (!(s[v] > m[v]))
             continue;
-          const float keep = exp2f(m[v] - s[v]);  // 0 at the first
+          const float keep = ex2(m[v] - s[v]);  // 0 at the first
           m[v] = s[v];
           l[v] *= keep;
 #pragma unroll
-          for (int i = 0; i < kPairs; i++)
-            acc[v][i] = f2_mul(acc[v][i], f2_pack(keep, keep));
+          for (int j = 0; j < kPairs; j++)
+            acc[v][j] = f2_mul(acc[v][j], f2_pack(keep, keep));
         }
       }
-      const bool all = in && position <= p.start;  // every row sees it
 #pragma unroll
-      for (int v = 0; v < kVecs; v++) {
-        const bool seen = all || position < limit[v];
-        s[v] = s[v] == -INFINITY ? 0.0f : exp2f(s[v] - m[v]) * guard;
+      for (int v = 0; v < VECS; v++) {
+        s[v] = s[v] == -INFINITY ? 0.0f : ex2(s[v] - m[v]) * guard;
         l[v] += s[v];
-        // What a row does not see may be anything: its product is left out, not made with a weight of zero.
-        if (in && seen) {
+      }
+      if (position <= p.start) {  // every row sees it
 #pragma unroll
-          for (int i = 0; i < kPairs; i++)
-            acc[v][i] = f2_fma(f2_pack(s[v], s[v]), x.pair(i), acc[v][i]);
+        for (int j = 0; j < kPairs; j++) {
+          const uint64_t xj = x.pair(j);
+#pragma unroll
+          for (int v = 0; v < VECS; v++)
+            acc[v][j] = f2_fma(f2_pack(s[v], s[v]), xj, acc[v][j]);
         }
+      } else if (position < end) {
+        // What a row does not see may be anything: its product is left out, not made with a weight of zero.
+#pragma unroll
+        for (int v = 0; v < VECS; v++)
+          if (position < limit[v])
+#pragma unroll
+            for (int j = 0; j < kPairs; j++)
+              acc[v][j] = f2_fma(f2_pack(s[v], s[v]), x.pair(j), acc[v][j]);
       }
     }
+    if (WIDE)
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the rings' room is free
     // The lane groups' results, then the warps'.
+    float *const sums = reinterpret_cast<float *>(smem);  // [warps][VECS][LANES * ELEMS]
+    constexpr int kLine = LANES * ELEMS;
 #pragma unroll
-    for (int v = 0; v < kVecs; v++) {
+    for (int v = 0; v < VECS; v++) {
       float top = m[v];
 #pragma unroll
       for (int o = 16; o >= LANES; o >>= 1)
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float f = m[v] == -INFINITY ? 0.0f : exp2f(m[v] - top);
+      const float f = m[v] == -INFINITY ? 0.0f : ex2(m[v] - top);
       float sum = l[v] * f;
 #pragma unroll
       for (int o = 16; o >= LANES; o >>= 1)
@@ -354,50 +442,51 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const PagedArgs a)
       if (lane == 0)
         wm[warp][v] = top, wl[warp][v] = sum;
 #pragma unroll
-      for (int i = 0; i < kPairs; i++) {
+      for (int j = 0; j < kPairs; j++) {
         float lo, hi;
-        f2_unpack(f2_mul(acc[v][i], f2_pack(f, f)), lo, hi);
+        f2_unpack(f2_mul(acc[v][j], f2_pack(f, f)), lo, hi);
 #pragma unroll
         for (int o = 16; o >= LANES; o >>= 1)
           lo += __shfl_xor_sync(0xffffffffu, lo, o), hi += __shfl_xor_sync(0xffffffffu, hi, o);
         if (at == 0) {
-          sums[warp][v][Row<T, LANES, WIDE>::element(sub, 2 * i)] = lo;
-          sums[warp][v][Row<T, LANES, WIDE>::element(sub, 2 * i + 1)] = hi;
+          sums[(warp * VECS + v) * kLine + R::element(sub, 2 * j)] = lo;
+          sums[(warp * VECS + v) * kLine + R::element(sub, 2 * j + 1)] = hi;
         }
       }
     }
     __syncthreads();
-    if (t < kVecs) {
+    if (t < VECS) {
       float top = -INFINITY, sum = 0.0f;
       for (int w = 0; w < kWarps; w++)
         top = fmaxf(top, wm[w][t]);
       for (int w = 0; w < kWarps; w++) {
-        const float f = wm[w][t] == -INFINITY ? 0.0f : exp2f(wm[w][t] - top);
+        const float f = wm[w][t] == -INFINITY ? 0.0f : ex2(wm[w][t] - top);
         sum += wl[w][t] * f;
         wl[w][t] = f;
       }
       m_all[t] = top, l_all[t] = sum;
     }
     __syncthreads();
-    float *o = &sums[0][0][0];  // [vecs][hd], over the first warps' sums once they are read
-    for (int v = 0; v < p.vecs; v++) {
-      float x[kMaxHd / kThreads];
+    // Joined in place: [vecs][hd] over the first warps' results, each thread's numbers read before any is written.
+    constexpr int kEach = VECS * kLine / kThreads;
+    float y[kEach];
 #pragma unroll
-      for (int j = 0; j < kMaxHd / kThreads; j++) {
-        const int e = t + j * kThreads;
-        x[j] = 0.0f;
-        if (e < hd)
-          for (int w = 0; w < kWarps; w++)
-            x[j] = fmaf(wl[w][v], sums[w][v][e], x[j]);
-      }
-      __syncthreads();
+    for (int j = 0; j < kEach; j++) {
+      const int i = t + j * kThreads, v = i / kLine;
+      y[j] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < kMaxHd / kThreads; j++)
-        if (t + j * kThreads < hd)
-          o[v * hd + t + j * kThreads] = x[j];
-      __syncthreads();
+      for (int w = 0; w < kWarps; w++)
+        y[j] = fmaf(wl[w][v], sums[w * VECS * kLine + i], y[j]);
     }
-    finish<kThreads, 0, 0>(a, &range, p, m_all, l_all, o, &bad, &last);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kEach; j++) {
+      const int i = t + j * kThreads, v = i / kLine, e = i % kLine;
+      if (e < hd && v < p.vecs)
+        sums[v * hd + e] = y[j];
+    }
+    __syncthreads();
+    finish<kThreads, 0, 0>(a, &range, p, m_all, l_all, sums, &bad, &last);
     if (t == 0)
       bad = 0;
     __syncthreads();
@@ -439,16 +528,28 @@ const char *cache_fault(const PagedCache *c, int n_kv, int hd) {
   return nullptr;
 }
 
-template <typename T, int LANES>
-cudaError_t launch_rows(const PagedArgs &a, bool wide) {
-  return wide ? kc_launch_pdl(paged_rows_kernel<T, LANES, true>, dim3(kCtas), dim3(kThreads), 0, kc_stream(), a)
-              : kc_launch_pdl(paged_rows_kernel<T, LANES, false>, dim3(kCtas), dim3(kThreads), 0, kc_stream(), a);
+template <typename T, int LANES, int ELEMS, int VECS, bool WIDE>
+cudaError_t launch_rows(const PagedArgs &a) {
+  const auto kernel = paged_rows_kernel<T, LANES, ELEMS, VECS, WIDE>;
+  constexpr int smem = RowsSmem<T, LANES, ELEMS, VECS, WIDE>::total;
+  const cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(kernel), smem);
+  return e != cudaSuccess ? e : kc_launch_pdl(kernel, dim3(kCtas), dim3(kThreads), smem, kc_stream(), a);
+}
+template <typename T, bool WIDE>
+cudaError_t launch_rows_of(const PagedArgs &a) {
+  if (a.block == 4)
+    return a.hd <= 64    ? launch_rows<T, 4, 16, 4, WIDE>(a)
+           : a.hd <= 128 ? launch_rows<T, 8, 16, 4, WIDE>(a)
+                         : launch_rows<T, 16, 16, 4, WIDE>(a);
+  return a.hd <= 64    ? launch_rows<T, 8, 8, 8, WIDE>(a)
+         : a.hd <= 128 ? launch_rows<T, 16, 8, 8, WIDE>(a)
+                       : launch_rows<T, 32, 8, 8, WIDE>(a);
 }
 template <typename T>
 cudaError_t launch_rows_of(const PagedArgs &a) {
   const bool wide = a.hd * sizeof(T) % 16 == 0 && a.page_stride * sizeof(T) % 16 == 0 &&
                     !(((uintptr_t)a.key | (uintptr_t)a.value) & 15);
-  return a.hd <= 64 ? launch_rows<T, 4>(a, wide) : a.hd <= 128 ? launch_rows<T, 8>(a, wide) : launch_rows<T, 16>(a, wide);
+  return wide ? launch_rows_of<T, true>(a) : launch_rows_of<T, false>(a);
 }
 
 int blocks_of(int n_heads, int n_kv, int rows, int block) {
@@ -463,7 +564,7 @@ size_t ticket_bytes(int n_heads, int batch, int rows) {
 
 // The slots of whichever kernel has more.
 size_t slots_floats(int hd) {
-  const int rows = 2 * kCtas * slot_size(kVecs, hd), tc = kc_paged_tc_slots_floats(hd);
+  const int rows = 2 * kCtas * slot_size(kRowsBlock, hd), tc = kc_paged_tc_slots_floats(hd);
   return rows > tc ? rows : tc;
 }
 
@@ -602,7 +703,9 @@ void k_attention_paged_rows(float *out, int8_t *oq, float *os, const float *q, c
   a.n_heads = n_heads, a.n_kv = n_kv_heads, a.group = n_heads / n_kv_heads, a.hd = head_dim;
   a.batch = batch, a.rows = rows, a.gs = gs;
   const bool tc = kc_paged_tc_ok(a, cache->type);
-  a.block = tc ? kc_paged_tc_block(a.group, rows) : kVecs;
+  // Eight vectors to a pass over the keys and values where a KV head has more than four (24 requests of 28/4 heads of 128 up
+  // to 3001 positions in fp32: @@ us with eight, @@ with four).
+  a.block = tc ? kc_paged_tc_block(a.group, rows) : (long long)a.group * rows <= 4 ? 4 : kRowsBlock;
   a.blocks = blocks_of(n_heads, n_kv_heads, rows, a.block);
   a.slot_floats = slot_size(a.block, head_dim);
   a.by_page = divisor(a.page_size), a.by_group = divisor(a.group);

@@ -702,10 +702,13 @@ void k_attention_paged_rows(float *out, int8_t *oq, float *os, const float *q, c
   a.page_size = cache->page_size, a.positions = cache->max_pages * cache->page_size;
   a.n_heads = n_heads, a.n_kv = n_kv_heads, a.group = n_heads / n_kv_heads, a.hd = head_dim;
   a.batch = batch, a.rows = rows, a.gs = gs;
-  const bool tc = kc_paged_tc_ok(a, cache->type);
+  const bool tc = kc_paged_tc_ok(a, cache->type), f32 = kc_paged_f32_ok(a, cache->type);
   // Eight vectors to a pass over the keys and values where a KV head has more than four (24 requests of 28/4 heads of 128 up
   // to 3001 positions in fp32: @@ us with eight, @@ with four).
-  a.block = tc ? kc_paged_tc_block(a.group, rows) : (long long)a.group * rows <= 4 ? 4 : kRowsBlock;
+  a.block = tc                                 ? kc_paged_tc_block(a.group, rows)
+            : f32                              ? kPagedF32Block
+            : (long long)a.group * rows <= 4 ? 4
+                                               : kRowsBlock;
   a.blocks = blocks_of(n_heads, n_kv_heads, rows, a.block);
   a.slot_floats = slot_size(a.block, head_dim);
   a.by_page = divisor(a.page_size), a.by_group = divisor(a.group);
@@ -713,6 +716,7 @@ void k_attention_paged_rows(float *out, int8_t *oq, float *os, const float *q, c
   // The tickets' room is the work's own, so that it does not move between calls of different batches.
   a.partial = work->partial + (work->capacity - slots_floats(head_dim));
   const cudaError_t e = tc                      ? kc_launch_paged_tc(a, cache->type)
+                        : f32                   ? kc_launch_paged_f32(a)
                         : cache->type == K_F32  ? launch_rows_of<float>(a)
                         : cache->type == K_BF16 ? launch_rows_of<__nv_bfloat16>(a)
                                                 : launch_rows_of<__half>(a);

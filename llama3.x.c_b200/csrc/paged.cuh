@@ -397,3 +397,8 @@ bool kc_paged_tc_ok(const paged::PagedArgs &a, int type);
 int kc_paged_tc_block(int group, int rows);
 int kc_paged_tc_slots_floats(int hd);
 cudaError_t kc_launch_paged_tc(const paged::PagedArgs &a, int type);
+
+// The tile kernel for fp32 (paged_f32.cu): whether it takes the call, and its launch; segments of kPagedF32Block vectors.
+constexpr int kPagedF32Block = 8;
+bool kc_paged_f32_ok(const paged::PagedArgs &a, int type);
+cudaError_t kc_launch_paged_f32(const paged::PagedArgs &a);

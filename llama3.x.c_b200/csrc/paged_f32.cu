@@ -1,0 +1,337 @@
+// Attention over a paged cache in fp32, by tiles in shared memory: head_dim up to 128 in whole 16-byte units, aligned pages.
+//
+// Eight query vectors of a KV head against tiles of 64 positions, which come by asynchronous copies through a ring that runs
+// on into the next segment. What a key or value costs besides its copy is reads of shared memory, so each is read once:
+//   scores: warp w takes the w-th eighth of the head, a lane two positions, all eight vectors: a key's unit of 16 bytes
+//     meets eight vectors' (broadcasts), and two positions share each of those. No shuffles; the eighths' sums meet in
+//     shared memory;
+//   softmax: warp v takes vector v: its reference and its sum of weights are that warp's own;
+//   sums: a warp takes eight positions, a lane four elements of the head, with all vectors' sums in registers.
+// The 16-byte units of a row lie in an order that spreads eight rows over the banks.
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+using namespace paged;
+
+constexpr int kTile = 64, kVecs = 8, kThreads = 256, kWarps = 8;
+constexpr int kCtas = 148;
+constexpr float kRise = 8.0f;            // how far a score may lie above the reference before the reference moves
+constexpr float kFar = 3.402823466e+38f;  // the reference before there is one, negative
+
+template <int HD>
+struct Smem {
+  static constexpr int kStages = HD == 128 ? 3 : 5;
+  float kv[kStages][2][kTile][HD];
+  union {
+    float part[kWarps][kVecs][kTile];     // scores by eighths of the head
+    float join[kWarps / 2][kVecs][HD];    // the warps' sums at the end of a piece
+  };
+  float q[kVecs][HD], weight[kVecs][kTile], keep[kVecs], m[kVecs], l[kVecs];
+  long long place[2][kTile];              // the rows of the tile copied next, and of the one behind it
+  RangeRoom room;
+  int bad, last;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// The tiles of a share one after another, from piece to piece.
+struct Tiles {
+  Walk walk;
+  Piece p;
+  int tile;
+  bool any;
+  __device__ __forceinline__ Tiles(const PagedArgs &a, const Range *range) : walk(range) {
+    any = walk.next(a, range, kTile, &p);
+    tile = any ? p.t0 : 0;
+  }
+  __device__ __forceinline__ void next(const PagedArgs &a, const Range *range) {
+    if (any && ++tile == p.t1) {
+      any = walk.next(a, range, kTile, &p);
+      tile = any ? p.t0 : 0;
+    }
+  }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs a) {
+  using S = Smem<HD>;
+  constexpr int kStages = S::kStages, kUnits = HD / 4, kAt = kThreads / kUnits;  // 16-byte units of a row, rows at a time
+  extern __shared__ __align__(16) uint8_t raw[];
+  S *s = reinterpret_cast<S *>(raw);
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, hd = a.hd;
+  pdl_wait();
+  pdl_launch_dependents();
+  Range here;
+  if (!find_range(a, kTile, &here, &s->room))
+    return;
+  const Range *range = &here;
+  const float scale = rsqrtf((float)hd) * kLog2e;
+
+  // Row t of the tile that `ahead` has come to: its place in elements, -1 where there is none.
+  Tiles ahead(a, range);
+  auto place = [&]() -> long long {
+    int within = ahead.tile * kTile + t;
+    if (!ahead.any || t >= kTile || within >= ahead.p.start + ahead.p.count)
+      return -1;
+    const int index = divide(within, a.by_page), page = a.table[(size_t)ahead.p.b * a.max_pages + index];
+    return page < 0 || page >= a.pages
+               ? -1
+               : (long long)((size_t)page * a.page_stride + ((size_t)ahead.p.head * a.page_size + within) * hd);
+  };
+  // Copies the tile whose places are in `from` to a stage.
+  auto fetch = [&](int stage, const long long *from) {
+    const int unit = t % kUnits, row0 = t / kUnits;
+#pragma unroll
+    for (int i = 0; i < kTile / kAt; i++) {
+      const int row = row0 + i * kAt;
+      const long long at = from[row];
+      const bool in = at >= 0 && 4 * unit < hd;
+      const size_t src = in ? (size_t)at + 4 * unit : 0;
+      const int to = (unit ^ (row & 7)) * 4;
+      copy16(&s->kv[stage][0][row][to], static_cast<const float *>(a.key) + src, in);
+      copy16(&s->kv[stage][1][row][to], static_cast<const float *>(a.value) + src, in);
+    }
+  };
+
+  if (t == 0)
+    s->bad = 0;
+  // The first tiles are on their way before anything else is done; `ahead` stays one tile before the next copy.
+  for (int i = 0; i < kStages - 1; i++) {
+    if (t < kTile)
+      s->place[i & 1][t] = place();
+    ahead.next(a, range);
+    __syncthreads();
+    fetch(i, s->place[i & 1]);
+    commit();
+  }
+  if (t < kTile)
+    s->place[(kStages - 1) & 1][t] = place();
+  ahead.next(a, range);
+
+  int n = 0;  // tiles done
+  Walk walk(range);
+  Piece p;
+  while (walk.next(a, range, kTile, &p)) {
+    // The piece's queries, and whether every page of its positions is one.
+    for (int i = t; i < kVecs * HD; i += kThreads) {
+      const int v = i / HD, e = i % HD;
+      int row;
+      s->q[v][e] = v < p.vecs && e < hd ? a.q[(size_t)vector_at(a, p, v, &row) * hd + e] * scale : 0.0f;
+    }
+    {
+      int from = p.t0 * kTile, to = min(p.t1 * kTile, p.start + p.count) - 1;
+      from = divide(from, a.by_page), to = divide(to, a.by_page);
+      bool bad = false;
+      for (int i = from + t; i <= to; i += kThreads) {
+        const int page = a.table[(size_t)p.b * a.max_pages + i];
+        bad |= page < 0 || page >= a.pages;
+      }
+      if (bad)
+        s->bad = 1;
+    }
+    const float guard = guard_of(p.start + p.count);
+    int limit = 0;  // positions that this warp's vector sees
+    if (warp < p.vecs) {
+      int row;
+      vector_at(a, p, warp, &row);
+      limit = p.start + row + 1;
+    }
+    float m = -kFar, l = 0.0f;
+    uint64_t acc[kVecs][2];
+#pragma unroll
+    for (int v = 0; v < kVecs; v++)
+      acc[v][0] = acc[v][1] = 0;
+    for (int tile = p.t0; tile < p.t1; tile++, n++) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncthreads();  // the tile is there, the one before it read by all
+      const int stage = n % kStages;
+      const long long next = place();
+      fetch((n + kStages - 1) % kStages, s->place[(n + kStages - 1) & 1]);
+      commit();
+      // ---- scores ----
+      {
+        constexpr int kEach = HD / kWarps / 4;  // units of a row to a warp
+        uint64_t x[2][kVecs];
+#pragma unroll
+        for (int v = 0; v < kVecs; v++)
+          x[0][v] = x[1][v] = 0;
+#pragma unroll
+        for (int u = 0; u < kEach; u++) {
+          const int unit = warp * kEach + u, at = (unit ^ (lane & 7)) * 4;
+          const ulonglong2 k0 = *reinterpret_cast<const ulonglong2 *>(&s->kv[stage][0][lane][at]);
+          const ulonglong2 k1 = *reinterpret_cast<const ulonglong2 *>(&s->kv[stage][0][lane + 32][at]);
+#pragma unroll
+          for (int v = 0; v < kVecs; v++) {
+            const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(&s->q[v][4 * unit]);
+            x[0][v] = f2_fma(q.y, k0.y, f2_fma(q.x, k0.x, x[0][v]));
+            x[1][v] = f2_fma(q.y, k1.y, f2_fma(q.x, k1.x, x[1][v]));
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < kVecs; v++) {
+          float lo, hi;
+          f2_unpack(x[0][v], lo, hi);
+          s->part[warp][v][lane] = lo + hi;
+          f2_unpack(x[1][v], lo, hi);
+          s->part[warp][v][lane + 32] = lo + hi;
+        }
+      }
+      if (t < kTile)
+        s->place[n + kStages & 1][t] = next;
+      ahead.next(a, range);
+      __syncthreads();
+      // ---- softmax of vector `warp` ----
+      {
+        float y[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const int at = lane + 32 * i;
+          y[i] = ((s->part[0][warp][at] + s->part[1][warp][at]) + (s->part[2][warp][at] + s->part[3][warp][at])) +
+                 ((s->part[4][warp][at] + s->part[5][warp][at]) + (s->part[6][warp][at] + s->part[7][warp][at]));
+          y[i] = tile * kTile + at < limit ? y[i] : -INFINITY;
+        }
+        float keep = 1.0f;
+        if (__any_sync(0xffffffffu, y[0] > m + kRise || y[1] > m + kRise)) {
+          const float top = fmaxf(warp_max(fmaxf(y[0], y[1])), m);
+          keep = ex2(m - top);
+          m = top;
+          l *= keep;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const float w = ex2(y[i] - m) * (guard * 0x1p-8f);
+          l += w;
+          s->weight[warp][lane + 32 * i] = w;
+        }
+        if (lane == 0)
+          s->keep[warp] = keep;
+      }
+      __syncthreads();
+      // ---- sums: positions 8 warp .. 8 warp + 7 ----
+      {
+        const float4 keep[2] = {*reinterpret_cast<const float4 *>(&s->keep[0]), *reinterpret_cast<const float4 *>(&s->keep[4])};
+        const float f[kVecs] = {keep[0].x, keep[0].y, keep[0].z, keep[0].w, keep[1].x, keep[1].y, keep[1].z, keep[1].w};
+        bool moved = false;
+#pragma unroll
+        for (int v = 0; v < kVecs; v++)
+          moved |= f[v] != 1.0f;
+        if (moved)
+#pragma unroll
+          for (int v = 0; v < kVecs; v++) {
+            acc[v][0] = f2_mul(acc[v][0], f2_pack(f[v], f[v]));
+            acc[v][1] = f2_mul(acc[v][1], f2_pack(f[v], f[v]));
+          }
+        // HD 128: all lanes a row; HD 64: half a warp a row, four of the eight positions each.
+        constexpr int kSets = HD == 128 ? 2 : 1;
+        const int unit = lane % kUnits, first = 8 * warp + (HD == 128 ? 0 : 4 * (lane / kUnits));
+#pragma unroll
+        for (int g = 0; g < kSets; g++) {
+          const int p0 = first + 4 * g;
+          float4 w[kVecs];
+#pragma unroll
+          for (int v = 0; v < kVecs; v++)
+            w[v] = *reinterpret_cast<const float4 *>(&s->weight[v][p0]);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int row = p0 + i, position = tile * kTile + row;
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(&s->kv[stage][1][row][(unit ^ (row & 7)) * 4]);
+            if (position <= p.start) {  // every row sees it
+#pragma unroll
+              for (int v = 0; v < kVecs; v++) {
+                const float y = i == 0 ? w[v].x : i == 1 ? w[v].y : i == 2 ? w[v].z : w[v].w;
+                acc[v][0] = f2_fma(f2_pack(y, y), x.x, acc[v][0]);
+                acc[v][1] = f2_fma(f2_pack(y, y), x.y, acc[v][1]);
+              }
+            } else if (position < p.start + p.count) {
+              // What a row does not see may be anything: its product is left out, not made with a weight of zero.
+#pragma unroll
+              for (int v = 0; v < kVecs; v++) {
+                int member = p.block * kVecs + v;
+                if (position > p.start + divide(member, a.by_group))
+                  continue;
+                const float y = i == 0 ? w[v].x : i == 1 ? w[v].y : i == 2 ? w[v].z : w[v].w;
+                acc[v][0] = f2_fma(f2_pack(y, y), x.x, acc[v][0]);
+                acc[v][1] = f2_fma(f2_pack(y, y), x.y, acc[v][1]);
+              }
+            }
+          }
+        }
+      }
+    }
+    // ---- the end of the piece: the warps' sums joined two by two ----
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      l += __shfl_xor_sync(0xffffffffu, l, o);
+    float y[kVecs][4];
+#pragma unroll
+    for (int v = 0; v < kVecs; v++) {
+      f2_unpack(acc[v][0], y[v][0], y[v][1]);
+      f2_unpack(acc[v][1], y[v][2], y[v][3]);
+      if (HD == 64)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          y[v][i] += __shfl_xor_sync(0xffffffffu, y[v][i], 16);
+    }
+    __syncthreads();  // the scores' room is free
+    if (lane == 0)
+      s->m[warp] = m, s->l[warp] = l;
+#pragma unroll
+    for (int half = kWarps / 2; half; half >>= 1) {
+      if (warp >= half && warp < 2 * half && lane < kUnits)
+#pragma unroll
+        for (int v = 0; v < kVecs; v++)
+          *reinterpret_cast<float4 *>(&s->join[warp - half][v][4 * lane]) = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
+      __syncthreads();
+      if (warp < half && lane < kUnits)
+#pragma unroll
+        for (int v = 0; v < kVecs; v++) {
+          const float4 x = *reinterpret_cast<const float4 *>(&s->join[warp][v][4 * lane]);
+          y[v][0] += x.x, y[v][1] += x.y, y[v][2] += x.z, y[v][3] += x.w;
+        }
+      __syncthreads();
+    }
+    float *sums = &s->join[0][0][0];  // [vecs][hd]
+    if (warp == 0 && 4 * lane < hd)
+#pragma unroll
+      for (int v = 0; v < kVecs; v++)
+        if (v < p.vecs)
+          *reinterpret_cast<float4 *>(sums + v * hd + 4 * lane) = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
+    __syncthreads();
+    finish<kThreads, 0, 0>(a, range, p, s->m, s->l, sums, &s->bad, &s->last);
+    if (t == 0)
+      s->bad = 0;
+    __syncthreads();
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <int HD>
+cudaError_t launch(const PagedArgs &a) {
+  const auto kernel = paged_f32_kernel<HD>;
+  const cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(kernel), (int)sizeof(Smem<HD>));
+  return e != cudaSuccess ? e : kc_launch_pdl(kernel, dim3(kCtas), dim3(kThreads), sizeof(Smem<HD>), kc_stream(), a);
+}
+
+}  // namespace
+
+bool kc_paged_f32_ok(const PagedArgs &a, int type) {
+  return type == K_F32 && a.hd % 4 == 0 && a.hd <= 128 && a.page_stride % 4 == 0 &&
+         !(((uintptr_t)a.key | (uintptr_t)a.value) & 15);
+}
+
+cudaError_t kc_launch_paged_f32(const PagedArgs &a) { return a.hd > 64 ? launch<128>(a) : launch<64>(a); }

@@ -82,13 +82,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
   const Range *range = &here;
   const float scale = rsqrtf((float)hd) * kLog2e;
 
-  // Row t of the tile that `ahead` has come to: its place in elements, -1 where there is none.
+  // Row t of the tile that `ahead` has come to: its page (asked for some time before it is used), and with that its place
+  // in elements, -1 where there is none.
   Tiles ahead(a, range);
-  auto place = [&]() -> long long {
+  auto page_of = [&]() -> int {
     int within = ahead.tile * kTile + t;
-    if (!ahead.any || t >= kTile || within >= ahead.p.start + ahead.p.count)
-      return -1;
-    const int index = divide(within, a.by_page), page = a.table[(size_t)ahead.p.b * a.max_pages + index];
+    return ahead.any && t < kTile && within < ahead.p.start + ahead.p.count
+               ? a.table[(size_t)ahead.p.b * a.max_pages + divide(within, a.by_page)]
+               : -1;
+  };
+  auto place = [&](int page) -> long long {
+    int within = ahead.tile * kTile + t;
+    divide(within, a.by_page);
     return page < 0 || page >= a.pages
                ? -1
                : (long long)((size_t)page * a.page_stride + ((size_t)ahead.p.head * a.page_size + within) * hd);
@@ -113,14 +118,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
   // The first tiles are on their way before anything else is done; `ahead` stays one tile before the next copy.
   for (int i = 0; i < kStages - 1; i++) {
     if (t < kTile)
-      s->place[i & 1][t] = place();
+      s->place[i & 1][t] = place(page_of());
     ahead.next(a, range);
     __syncthreads();
     fetch(i, s->place[i & 1]);
     commit();
   }
   if (t < kTile)
-    s->place[(kStages - 1) & 1][t] = place();
+    s->place[(kStages - 1) & 1][t] = place(page_of());
   ahead.next(a, range);
 
   int n = 0;  // tiles done
@@ -160,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
       __syncthreads();  // the tile is there, the one before it read by all
       const int stage = n % kStages;
-      const long long next = place();
+      const int next = page_of();
       fetch((n + kStages - 1) % kStages, s->place[(n + kStages - 1) & 1]);
       commit();
       // ---- scores ----
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
         }
       }
       if (t < kTile)
-        s->place[n + kStages & 1][t] = next;
+        s->place[(n + kStages) & 1][t] = place(next);
       ahead.next(a, range);
       __syncthreads();
       // ---- softmax of vector `warp` ----
@@ -243,31 +248,34 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
         for (int g = 0; g < kSets; g++) {
           const int p0 = first + 4 * g;
           float4 w[kVecs];
+          ulonglong2 x[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            x[i] = *reinterpret_cast<const ulonglong2 *>(&s->kv[stage][1][p0 + i][(unit ^ ((p0 + i) & 7)) * 4]);
 #pragma unroll
           for (int v = 0; v < kVecs; v++)
             w[v] = *reinterpret_cast<const float4 *>(&s->weight[v][p0]);
+          auto add = [&](int v, int i) {
+            const float y = i == 0 ? w[v].x : i == 1 ? w[v].y : i == 2 ? w[v].z : w[v].w;
+            acc[v][0] = f2_fma(f2_pack(y, y), x[i].x, acc[v][0]);
+            acc[v][1] = f2_fma(f2_pack(y, y), x[i].y, acc[v][1]);
+          };
+          if (tile * kTile + kTile <= p.start + 1) {  // every row sees all of the tile
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int row = p0 + i, position = tile * kTile + row;
-            const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(&s->kv[stage][1][row][(unit ^ (row & 7)) * 4]);
-            if (position <= p.start) {  // every row sees it
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-              for (int v = 0; v < kVecs; v++) {
-                const float y = i == 0 ? w[v].x : i == 1 ? w[v].y : i == 2 ? w[v].z : w[v].w;
-                acc[v][0] = f2_fma(f2_pack(y, y), x.x, acc[v][0]);
-                acc[v][1] = f2_fma(f2_pack(y, y), x.y, acc[v][1]);
-              }
-            } else if (position < p.start + p.count) {
-              // What a row does not see may be anything: its product is left out, not made with a weight of zero.
+              for (int v = 0; v < kVecs; v++)
+                add(v, i);
+          } else {
+            // What a row does not see may be anything: its product is left out, not made with a weight of zero.
 #pragma unroll
-              for (int v = 0; v < kVecs; v++) {
-                int member = p.block * kVecs + v;
-                if (position > p.start + divide(member, a.by_group))
-                  continue;
-                const float y = i == 0 ? w[v].x : i == 1 ? w[v].y : i == 2 ? w[v].z : w[v].w;
-                acc[v][0] = f2_fma(f2_pack(y, y), x.x, acc[v][0]);
-                acc[v][1] = f2_fma(f2_pack(y, y), x.y, acc[v][1]);
-              }
+            for (int v = 0; v < kVecs; v++) {
+              int member = p.block * kVecs + v;
+              const int sees = p.start + divide(member, a.by_group) - (tile * kTile + p0);
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                if (i <= sees && v < p.vecs)
+                  add(v, i);
             }
           }
         }

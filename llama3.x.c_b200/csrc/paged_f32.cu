@@ -1,7 +1,8 @@
 // Attention over a paged cache in fp32, by tiles in shared memory: head_dim up to 128 in whole 16-byte units, aligned pages.
 //
-// Eight query vectors of a KV head against tiles of 64 positions, which come by asynchronous copies through a ring that runs
-// on into the next segment. What a key or value costs besides its copy is reads of shared memory, so each is read once:
+// Eight query vectors of a KV head against tiles of 64 positions, which four warps copy, asynchronously, through a ring that
+// runs on into the next segment. Eight warps take a tile in three steps with a barrier behind each; what a key or value costs
+// there besides its products is reads of shared memory, so each is read once:
 //   scores: warp w takes the w-th eighth of the head, a lane two positions, all eight vectors: a key's unit of 16 bytes
 //     meets eight vectors' (broadcasts), and two positions share each of those. No shuffles; the eighths' sums meet in
 //     shared memory;
@@ -14,7 +15,9 @@
 namespace {
 using namespace paged;
 
-constexpr int kTile = 64, kVecs = 8, kThreads = 256, kWarps = 8;
+constexpr int kTile = 64, kVecs = 8;
+constexpr int kWarps = 8, kSoft = 32 * kWarps;  // that compute
+constexpr int kCopyWarps = 4, kThreads = kSoft + 32 * kCopyWarps;
 constexpr int kCtas = 148;
 constexpr float kRise = 8.0f;            // how far a score may lie above the reference before the reference moves
 constexpr float kFar = 3.402823466e+38f;  // the reference before there is one, negative
@@ -28,9 +31,9 @@ struct Smem {
     float join[kWarps / 2][kVecs][HD];    // the warps' sums at the end of a piece
   };
   float q[kVecs][HD], weight[kVecs][kTile], keep[kVecs], m[kVecs], l[kVecs];
-  long long place[2][kTile];              // the rows of the tile copied next, and of the one behind it
+  uint64_t full[kStages], empty[kStages];
   RangeRoom room;
-  int bad, last;
+  int bad, last, abort_flag;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -47,30 +50,21 @@ __device__ __forceinline__ void copy16(void *dst, const void *src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
                : "memory");
 }
-__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-
-// The tiles of a share one after another, from piece to piece.
-struct Tiles {
-  Walk walk;
-  Piece p;
-  int tile;
-  bool any;
-  __device__ __forceinline__ Tiles(const PagedArgs &a, const Range *range) : walk(range) {
-    any = walk.next(a, range, kTile, &p);
-    tile = any ? p.t0 : 0;
-  }
-  __device__ __forceinline__ void next(const PagedArgs &a, const Range *range) {
-    if (any && ++tile == p.t1) {
-      any = walk.next(a, range, kTile, &p);
-      tile = any ? p.t0 : 0;
-    }
-  }
-};
+// Arrives once all copies that this thread has started are in memory.
+__device__ __forceinline__ void copy_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// A wait that gives up at once when another one of the CTA has.
+__device__ __forceinline__ void wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
+  if (!mbar_try_wait(bar, parity) && *abort_flag == 0 && !mbar_wait_sleep_bounded(bar, parity))
+    *abort_flag = 1;
+  __syncwarp();
+}
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs a) {
   using S = Smem<HD>;
-  constexpr int kStages = S::kStages, kUnits = HD / 4, kAt = kThreads / kUnits;  // 16-byte units of a row, rows at a time
+  constexpr int kStages = S::kStages, kUnits = HD / 4;  // 16-byte units of a row
   extern __shared__ __align__(16) uint8_t raw[];
   S *s = reinterpret_cast<S *>(raw);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, hd = a.hd;
@@ -81,59 +75,68 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
     return;
   const Range *range = &here;
   const float scale = rsqrtf((float)hd) * kLog2e;
-
-  // Row t of the tile that `ahead` has come to: its page (asked for some time before it is used), and with that its place
-  // in elements, -1 where there is none.
-  Tiles ahead(a, range);
-  auto page_of = [&]() -> int {
-    int within = ahead.tile * kTile + t;
-    return ahead.any && t < kTile && within < ahead.p.start + ahead.p.count
-               ? a.table[(size_t)ahead.p.b * a.max_pages + divide(within, a.by_page)]
-               : -1;
-  };
-  auto place = [&](int page) -> long long {
-    int within = ahead.tile * kTile + t;
-    divide(within, a.by_page);
-    return page < 0 || page >= a.pages
-               ? -1
-               : (long long)((size_t)page * a.page_stride + ((size_t)ahead.p.head * a.page_size + within) * hd);
-  };
-  // Copies the tile whose places are in `from` to a stage.
-  auto fetch = [&](int stage, const long long *from) {
-    const int unit = t % kUnits, row0 = t / kUnits;
-#pragma unroll
-    for (int i = 0; i < kTile / kAt; i++) {
-      const int row = row0 + i * kAt;
-      const long long at = from[row];
-      const bool in = at >= 0 && 4 * unit < hd;
-      const size_t src = in ? (size_t)at + 4 * unit : 0;
-      const int to = (unit ^ (row & 7)) * 4;
-      copy16(&s->kv[stage][0][row][to], static_cast<const float *>(a.key) + src, in);
-      copy16(&s->kv[stage][1][row][to], static_cast<const float *>(a.value) + src, in);
+  volatile int *abort_flag = &s->abort_flag;
+  if (t == 0) {
+    for (int i = 0; i < kStages; i++) {
+      mbar_init(&s->full[i], 32 * kCopyWarps);
+      mbar_init(&s->empty[i], kWarps);
     }
-  };
-
-  if (t == 0)
-    s->bad = 0;
-  // The first tiles are on their way before anything else is done; `ahead` stays one tile before the next copy.
-  for (int i = 0; i < kStages - 1; i++) {
-    if (t < kTile)
-      s->place[i & 1][t] = place(page_of());
-    ahead.next(a, range);
-    __syncthreads();
-    fetch(i, s->place[i & 1]);
-    commit();
+    s->bad = s->abort_flag = 0;
+    fence_mbar_init();
   }
-  if (t < kTile)
-    s->place[(kStages - 1) & 1][t] = place(page_of());
-  ahead.next(a, range);
-
-  int n = 0;  // tiles done
+  __syncthreads();
   Walk walk(range);
   Piece p;
+
+  if (warp >= kWarps) {
+    // ---- copies: warp w of them rows 16 w .. 16 w + 15 of every tile ----
+    constexpr int kRows = kTile / kCopyWarps, kAt = 32 / kUnits;  // rows of a warp, and of its instruction
+    const int w = warp - kWarps, unit = lane % kUnits;
+    int stage = 0;
+    unsigned parity = 1;
+    while (walk.next(a, range, kTile, &p)) {
+      const int end = p.start + p.count;
+      const int *pages = a.table + (size_t)p.b * a.max_pages;
+      // Lane r of the first 16: the page of row r, asked for a tile before it is used; -1 where there is none.
+      auto page_of = [&](int tile) -> int {
+        int within = tile * kTile + kRows * w + lane;
+        return tile < p.t1 && lane < kRows && within < end ? pages[divide(within, a.by_page)] : -1;
+      };
+      int page = page_of(p.t0);
+      for (int tile = p.t0; tile < p.t1; tile++) {
+        int within = tile * kTile + kRows * w + lane;
+        divide(within, a.by_page);
+        const long long place =
+            page < 0 || page >= a.pages
+                ? -1
+                : (long long)((size_t)page * a.page_stride + ((size_t)p.head * a.page_size + within) * hd);
+        page = page_of(tile + 1);
+        wait(&s->empty[stage], parity, abort_flag);
+#pragma unroll
+        for (int i = 0; i < kRows / kAt; i++) {
+          const int r = i * kAt + lane / kUnits, row = kRows * w + r;
+          const long long at = __shfl_sync(0xffffffffu, place, r);
+          const bool in = at >= 0 && 4 * unit < hd;
+          const size_t src = in ? (size_t)at + 4 * unit : 0;
+          const int to = (unit ^ (row & 7)) * 4;
+          copy16(&s->kv[stage][0][row][to], static_cast<const float *>(a.key) + src, in);
+          copy16(&s->kv[stage][1][row][to], static_cast<const float *>(a.value) + src, in);
+        }
+        copy_arrive(&s->full[stage]);
+        if (++stage == kStages)
+          stage = 0, parity ^= 1;
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
+
+  // ---- the computing warps ----
+  int stage = 0;
+  unsigned parity = 0;
   while (walk.next(a, range, kTile, &p)) {
     // The piece's queries, and whether every page of its positions is one.
-    for (int i = t; i < kVecs * HD; i += kThreads) {
+    for (int i = t; i < kVecs * HD; i += kSoft) {
       const int v = i / HD, e = i % HD;
       int row;
       s->q[v][e] = v < p.vecs && e < hd ? a.q[(size_t)vector_at(a, p, v, &row) * hd + e] * scale : 0.0f;
@@ -142,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
       int from = p.t0 * kTile, to = min(p.t1 * kTile, p.start + p.count) - 1;
       from = divide(from, a.by_page), to = divide(to, a.by_page);
       bool bad = false;
-      for (int i = from + t; i <= to; i += kThreads) {
+      for (int i = from + t; i <= to; i += kSoft) {
         const int page = a.table[(size_t)p.b * a.max_pages + i];
         bad |= page < 0 || page >= a.pages;
       }
@@ -161,13 +164,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
 #pragma unroll
     for (int v = 0; v < kVecs; v++)
       acc[v][0] = acc[v][1] = 0;
-    for (int tile = p.t0; tile < p.t1; tile++, n++) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-      __syncthreads();  // the tile is there, the one before it read by all
-      const int stage = n % kStages;
-      const int next = page_of();
-      fetch((n + kStages - 1) % kStages, s->place[(n + kStages - 1) & 1]);
-      commit();
+    meet<kSoft, 1>();  // the queries are there
+    for (int tile = p.t0; tile < p.t1; tile++) {
+      wait(&s->full[stage], parity, abort_flag);
       // ---- scores ----
       {
         constexpr int kEach = HD / kWarps / 4;  // units of a row to a warp
@@ -196,10 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
           s->part[warp][v][lane + 32] = lo + hi;
         }
       }
-      if (t < kTile)
-        s->place[(n + kStages) & 1][t] = place(next);
-      ahead.next(a, range);
-      __syncthreads();
+      meet<kSoft, 1>();
       // ---- softmax of vector `warp` ----
       {
         float y[2];
@@ -226,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
         if (lane == 0)
           s->keep[warp] = keep;
       }
-      __syncthreads();
+      meet<kSoft, 1>();
       // ---- sums: positions 8 warp .. 8 warp + 7 ----
       {
         const float4 keep[2] = {*reinterpret_cast<const float4 *>(&s->keep[0]), *reinterpret_cast<const float4 *>(&s->keep[4])};
@@ -280,6 +276,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
           }
         }
       }
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&s->empty[stage]);  // behind the products, which have waited for all that was read
+      if (++stage == kStages)
+        stage = 0, parity ^= 1;
     }
     // ---- the end of the piece: the warps' sums joined two by two ----
 #pragma unroll
@@ -295,23 +296,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
         for (int i = 0; i < 4; i++)
           y[v][i] += __shfl_xor_sync(0xffffffffu, y[v][i], 16);
     }
-    __syncthreads();  // the scores' room is free
+    meet<kSoft, 1>();  // the scores' room is free
     if (lane == 0)
       s->m[warp] = m, s->l[warp] = l;
+    if (*abort_flag)
+      s->bad = 1;
 #pragma unroll
     for (int half = kWarps / 2; half; half >>= 1) {
       if (warp >= half && warp < 2 * half && lane < kUnits)
 #pragma unroll
         for (int v = 0; v < kVecs; v++)
           *reinterpret_cast<float4 *>(&s->join[warp - half][v][4 * lane]) = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
-      __syncthreads();
+      meet<kSoft, 1>();
       if (warp < half && lane < kUnits)
 #pragma unroll
         for (int v = 0; v < kVecs; v++) {
           const float4 x = *reinterpret_cast<const float4 *>(&s->join[warp][v][4 * lane]);
           y[v][0] += x.x, y[v][1] += x.y, y[v][2] += x.z, y[v][3] += x.w;
         }
-      __syncthreads();
+      meet<kSoft, 1>();
     }
     float *sums = &s->join[0][0][0];  // [vecs][hd]
     if (warp == 0 && 4 * lane < hd)
@@ -319,13 +322,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
       for (int v = 0; v < kVecs; v++)
         if (v < p.vecs)
           *reinterpret_cast<float4 *>(sums + v * hd + 4 * lane) = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
-    __syncthreads();
-    finish<kThreads, 0, 0>(a, range, p, s->m, s->l, sums, &s->bad, &s->last);
+    meet<kSoft, 1>();
+    finish<kSoft, 1, 0>(a, range, p, s->m, s->l, sums, &s->bad, &s->last);
     if (t == 0)
       s->bad = 0;
-    __syncthreads();
+    meet<kSoft, 1>();
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 template <int HD>

@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
         sums[v * hd + e] = y[j];
     }
     __syncthreads();
-    finish<kThreads, 0, 0>(a, &range, p, m_all, l_all, sums, &bad, &last);
+    finish<kThreads, 0, 0>(a, &range, p, m_all, l_all, sums, &bad, &last, t);
     if (t == 0)
       bad = 0;
     __syncthreads();

@@ -249,13 +249,13 @@ __device__ __forceinline__ void meet() {
 
 // The piece's vectors, with m and l of each and their sums o in shared memory, written to the output (a whole segment,
 // or the last of its pieces to be done) or to a slot. All threads call it, after a barrier behind the last write to m, l,
-// o and bad; it ends with one. THREADS threads, numbered from 0, meet at barrier BARRIER. HD:
+// o and bad; it ends with one. THREADS threads, numbered t, meet at barrier BARRIER. HD:
 // head_dim, or 0 where it is any.
 template <int THREADS, int BARRIER, int HD>
 __device__ __forceinline__ void finish(const PagedArgs &a, const Range *range, const Piece &p, float *m, float *l, float *o,
-                       const int *bad, int *last) {
+                       const int *bad, int *last, int t) {
   constexpr int threads = THREADS;
-  const int t = threadIdx.x, hd = HD ? HD : a.hd;
+  const int hd = HD ? HD : a.hd;
   bool wrong = *bad != 0;
   if (p.t0 || p.t1 < p.tiles) {
     const int c0 = owner(range, p.first), c1 = owner(range, p.first + p.tiles - 1);

@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
         if (v < p.vecs)
           *reinterpret_cast<float4 *>(sums + v * hd + 4 * lane) = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
     meet<kSoft, 1>();
-    finish<kSoft, 1, 0>(a, range, p, s->m, s->l, sums, &s->bad, &s->last);
+    finish<kSoft, 1, 0>(a, range, p, s->m, s->l, sums, &s->bad, &s->last, t);
     if (t == 0)
       s->bad = 0;
     meet<kSoft, 1>();

@@ -17,14 +17,19 @@
 //
 // A CTA per SM takes its share of the tiles of all segments without a pause between segments. Its warps: softmax, a thread
 // per position of a tile and per element of the head of its sums, in groups of four warps that share out the query vectors
-// (4 or 8 to a thread: with all 32 of the largest block in one group, a tile took 3.9 us); one that issues the MMAs; one
-// or more that lay out the next segment's queries; four that copy the tiles, asynchronously, through a ring of stages.
+// (4 or 8 to a thread: with all 32 of the largest block in one group, a tile took 3.9 us); one that issues the MMAs; one to
+// three that lay out the next segment's queries; four that copy the tiles, asynchronously, through a ring of stages. With up
+// to eight vectors two more finish a segment (by the softmax warps themselves that takes 2 us of their time, and the shares
+// of many short segments ended last: 8 requests of up to 2048 positions 19 us with them against 22), but for a share's last,
+// for which the softmax warps are faster; with more vectors those do it all (80 requests' rows behind 4099: 58 us against 64).
 //
 // A later draft's key or value of any kind must not reach the rows before it, not even with a weight of zero: a key gives
 // scores in its own row of S^T only, which are masked; a value with an infinity or a NaN behind the block's first row is
 // zeroed before its product, and the rows that see it get NaN for a weight there.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "paged.cuh"
 #include "tcgen05.cuh"
@@ -39,11 +44,18 @@ constexpr int kMaxBlock = 32;
 constexpr int kMaxStages = 10;
 constexpr int kSmem = 227 * 1024;
 
+template <int RESULTS>
 struct Tail {
-  uint64_t full[kMaxStages], empty[kMaxStages], sfull[2], pfull[2], ofull[2], qfull[2], qempty[2], drained;
+  uint64_t full[kMaxStages], empty[kMaxStages], sfull[2], pfull[2], ofull[2], qfull[2], qempty[2], rfull[2], rempty[2];
+  uint64_t drained;
   uint32_t tmem;
-  int abort_flag, bad, last;
-  __align__(16) float top[2][4][kMaxBlock];  // a tile's maxima by warp; the warps' sums of weights
+  int abort_flag;
+  __align__(16) float top[4][kMaxBlock];  // a tile's maxima by warp
+  // A piece's results beside its sums: references, sums of weights by warp, a page that is none.
+  struct {
+    float m[kMaxBlock], l[4][kMaxBlock];
+    int bad, last;
+  } result[RESULTS];
   // Of the queries: four pieces, since the softmax may be two tiles behind the scores, and the queries two pieces ahead.
   float qscale[4][kMaxBlock];
 };
@@ -51,19 +63,25 @@ struct Tail {
 template <int HD, int BLOCK>
 struct Layout {
   static constexpr int groups = BLOCK == 4 ? 1 : BLOCK == 8 ? 2 : 4, vecs = BLOCK / groups;  // vectors to a thread
-  static constexpr int query_warps = groups == 4 ? 3 : groups;  // (24 warps: 80 registers a thread, 25 would leave 72)
+  static constexpr bool ends = groups < 4;  // warps that finish pieces
+  static constexpr int query_warps = ends ? 1 : 3, end_warps = ends ? 2 : 0;  // (12, 16 or 24 warps in all)
   static constexpr int soft = 128 * groups;  // softmax threads
-  static constexpr int threads = soft + 32 + 32 * query_warps + 32 * kCopyWarps;
+  static constexpr int threads = soft + 32 + 32 * (query_warps + end_warps) + 32 * kCopyWarps;
   static constexpr int n = (3 * BLOCK + 15) / 16 * 16;  // columns
   static constexpr int entry = kTile * HD * 2;
   static constexpr int q_bytes = n * HD * 2, p_bytes = n * kTile * 2;
-  static constexpr int fit = (kSmem - 1024 - 2 * (q_bytes + p_bytes) - (int)sizeof(Tail)) / entry;
+  static constexpr int r_bytes = BLOCK * HD * 4, r_room = ends ? 2 * r_bytes : 0;  // without, over the probabilities
+  static constexpr int results = ends ? 2 : 1;
+  using End = Tail<results>;
+  static constexpr int fit = (kSmem - 1024 - 2 * (q_bytes + p_bytes) - r_room - (int)sizeof(End)) / entry;
   static constexpr int stages = fit > kMaxStages ? kMaxStages : fit;
-  static constexpr int q_at = stages * entry, p_at = q_at + 2 * q_bytes, tail_at = p_at + 2 * p_bytes;
-  static constexpr int total = tail_at + (int)sizeof(Tail) + 1024;
+  static constexpr int q_at = stages * entry, p_at = q_at + 2 * q_bytes;
+  static constexpr int r_at = ends ? p_at + 2 * p_bytes : p_at;
+  static constexpr int tail_at = p_at + 2 * p_bytes + r_room;
+  static_assert(ends || 2 * p_bytes >= r_bytes, "the results' room");
+  static constexpr int total = tail_at + (int)sizeof(End) + 1024;
   static constexpr int tmem = 4 * n <= 64 ? 64 : 4 * n <= 128 ? 128 : 4 * n <= 256 ? 256 : 512;
   static_assert(stages >= 4 && total <= kSmem, "shared memory");
-  static_assert(2 * p_bytes >= BLOCK * HD * 4, "the sums' room, over the probabilities'");
 };
 
 __device__ __forceinline__ bool tc_wait(uint64_t *bar, unsigned parity, volatile int *abort_flag) {
@@ -234,11 +252,12 @@ __device__ __forceinline__ long long place_of(const PagedArgs &a, const Piece &p
 template <typename T, int HD, int BLOCK>
 __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel(const PagedArgs a) {
   using L = Layout<HD, BLOCK>;
-  constexpr int kSoft = L::soft, kVecs = L::vecs, kMma = kSoft / 32, kQuery = kMma + 1, kCopy = kQuery + L::query_warps;
+  constexpr int kSoft = L::soft, kVecs = L::vecs, kMma = kSoft / 32, kQuery = kMma + 1,
+                kEnd = kQuery + L::query_warps, kCopy = kEnd + L::end_warps;
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  Tail *t = reinterpret_cast<Tail *>(smem + L::tail_at);
+  auto *t = reinterpret_cast<typename L::End *>(smem + L::tail_at);
   volatile int *abort_flag = &t->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
@@ -257,10 +276,12 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
       mbar_init(&t->ofull[i], 1);
       mbar_init(&t->qfull[i], L::query_warps);
       mbar_init(&t->qempty[i], 1);
+      mbar_init(&t->rfull[i], kSoft / 32);
+      mbar_init(&t->rempty[i], 1);
+      t->result[i % L::results].bad = 0;
     }
     mbar_init(&t->drained, 1);
     t->abort_flag = 0;
-    t->bad = 0;
     fence_mbar_init();
   }
   if (warp == kMma)
@@ -273,6 +294,18 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
   const float scale = rsqrtf((float)HD) * kLog2e;
   Walk walk(range);
   Piece p;
+  // Finishes the piece whose results are in a buffer: threads numbered tid, at a barrier of their own.
+  auto end_piece = [&](int at, const Piece &p, int tid, auto threads, auto barrier) {
+    auto &result = t->result[at];
+    if (tid < p.vecs)
+      result.l[0][tid] = (result.l[0][tid] + result.l[1][tid]) + (result.l[2][tid] + result.l[3][tid]);
+    if (tid == 0 && *abort_flag)
+      result.bad = 1;
+    meet<threads(), barrier()>();
+    finish<threads(), barrier(), HD>(a, range, p, result.m, result.l[0],
+                                     reinterpret_cast<float *>(smem + L::r_at + at * L::r_bytes), &result.bad, &result.last,
+                                     tid);
+  };
 
   if (warp >= kCopy) {
     // ---- copies: warp w of them the rows 32 w .. 32 w + 31 of every tile, keys and values in turn ----
@@ -310,18 +343,29 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
       }
     }
     copy_wait_all();
+  } else if (L::ends && warp >= kEnd) {
+    // ---- the pieces' ends, but for the share's last ----
+    const int tid = threadIdx.x - 32 * kEnd;
+    for (int n = 0; walk.next(a, range, kTile, &p) && p.first + p.t1 < range->hi; n++) {
+      const int at = n & 1;
+      tc_wait(&t->rfull[at], (n >> 1) & 1, abort_flag);
+      end_piece(at, p, tid, std::integral_constant<int, L::ends ? 32 * L::end_warps : 32>(), std::integral_constant<int, 1>());
+      if (tid == 0) {
+        t->result[at].bad = 0;
+        mbar_arrive(&t->rempty[at]);
+      }
+    }
   } else if (warp >= kQuery) {
     // ---- queries: times the scores' scale, in three parts, row part * BLOCK + v of the operand ----
-    constexpr int kEach = HD / 32;
+    constexpr int kEach = HD / 32, kAt = 4;
     for (int n = 0; walk.next(a, range, kTile, &p); n++) {
       uint8_t *to = smem + L::q_at + (n & 1) * L::q_bytes;
-      if (n >= 2)
-        tc_wait(&t->qempty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag);
+      tc_wait(&t->qempty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag);
+#pragma unroll 1
+      for (int v0 = kAt * (warp - kQuery); v0 < BLOCK; v0 += kAt * L::query_warps) {
+        float x[kAt][kEach];
 #pragma unroll
-      for (int v0 = 4 * (warp - kQuery); v0 < BLOCK; v0 += 4 * L::query_warps) {
-        float x[4][kEach];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < kAt; u++) {
           int row;
           const float *q = a.q + (size_t)vector_at(a, p, min(v0 + u, p.vecs - 1), &row) * HD;
 #pragma unroll
@@ -329,7 +373,7 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
             x[u][i] = v0 + u < p.vecs ? q[2 * lane + 32 * (i & ~1) + (i & 1)] * scale : 0.0f;
         }
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < kAt; u++) {
           const int v = v0 + u;
           if (!kBf16) {
             float mx = 0.0f;
@@ -452,18 +496,11 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
       const bool idle = v0 >= p.vecs;  // the group has none of the block's vectors
       // Weights are up to 2^kRise times this: bf16 as guard_of says, fp16 up to 2^15 (there is no value beyond 2^16).
       const float weight = kBf16 ? guard_of(p.start + p.count) * 0x1p-8f : 0x1p7f;
-      // Every page of the piece's positions is one.
-      {
-        int from = p.t0 * kTile, to = min(p.t1 * kTile, p.start + p.count) - 1;
-        from = divide(from, a.by_page), to = divide(to, a.by_page);
-        bool bad = false;
-        for (int i = from + tid; i <= to; i += kSoft) {
-          const int page = a.table[(size_t)p.b * a.max_pages + i];
-          bad |= page < 0 || page >= a.pages;
-        }
-        if (bad)
-          t->bad = 1;
-      }
+      // Every page of the piece's positions is one: asked for here, looked at behind the first tile.
+      int from = p.t0 * kTile, to = min(p.t1 * kTile, p.start + p.count) - 1;
+      from = divide(from, a.by_page) + tid, to = divide(to, a.by_page);
+      const int *pages = a.table + (size_t)p.b * a.max_pages;
+      const int first_page = from <= to ? pages[from] : 0;
       auto add = [&](int i) {  // the sums of tile i
         float o[kVecs];
         tc_wait(&t->ofull[i & 1], (i >> 1) & 1, abort_flag);
@@ -516,7 +553,7 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
                 }
               }
             }
-            meet<kSoft, 1>();  // every group has looked
+            meet<kSoft, 6>();  // every group has looked
             if (wrong && group == 0)
               for (int i = 0; i < HD / 8; i++)
                 *reinterpret_cast<uint4 *>(values + (i >> 3) * (kTile * 128) + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -539,7 +576,7 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
           // The reference stays while no score is far above it: one barrier that tells, instead of maxima over the tile.
           moves = meet_any(group, high > kRise);
           if (moves) {
-            float (*top)[kMaxBlock] = t->top[0];
+            float (*top)[kMaxBlock] = t->top;
 #pragma unroll
             for (int v = 0; v < kVecs; v++) {
               const float x = warp_max(s[v]);
@@ -588,10 +625,18 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
           for (int v = 0; v < kVecs; v++)
             acc[v] *= keep[v];
       }
-      add(j - 1);  // idle or not: the probabilities' room is free once the last product is done
+      add(j - 1);
       // The piece's result.
-      float *sums = reinterpret_cast<float *>(smem + L::p_at), (*part)[kMaxBlock] = t->top[1];
-      float *m_all = t->top[0][0], *l_all = t->top[0][1];  // once the last tile's maxima are read
+      bool bad = first_page < 0 || first_page >= a.pages;
+      for (int i = from + kSoft; i <= to; i += kSoft) {
+        const int page = pages[i];
+        bad |= page < 0 || page >= a.pages;
+      }
+      const int at = L::ends ? n & 1 : 0;
+      if (L::ends)
+        tc_wait(&t->rempty[at], ((n >> 1) & 1) ^ 1, abort_flag);
+      auto &result = t->result[at];
+      float *sums = reinterpret_cast<float *>(smem + L::r_at + at * L::r_bytes);
 #pragma unroll
       for (int v = 0; v < kVecs; v++) {
         if (has_element && v0 + v < p.vecs)
@@ -600,22 +645,24 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
         for (int o = 16; o; o >>= 1)
           l[v] += __shfl_xor_sync(0xffffffffu, l[v], o);
         if (lane == 0)
-          part[quad][v0 + v] = l[v];
-      }
-      if (*abort_flag)
-        t->bad = 1;
-      meet<kSoft, 1>();
-      if (tid < p.vecs)
-        l_all[tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
-#pragma unroll
-      for (int v = 0; v < kVecs; v++)
+          result.l[quad][v0 + v] = l[v];
         if (row == v)
-          m_all[v0 + v] = m[v];
-      meet<kSoft, 1>();
-      finish<kSoft, 1, HD>(a, range, p, m_all, l_all, sums, &t->bad, &t->last);
-      if (tid == 0)
-        t->bad = 0;
-      meet<kSoft, 1>();
+          result.m[v0 + v] = m[v];
+      }
+      if (bad)
+        result.bad = 1;
+      if (L::ends && p.first + p.t1 < range->hi) {
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&t->rfull[at]);
+      } else {
+        meet<kSoft, 6>();
+        end_piece(at, p, tid, std::integral_constant<int, kSoft>(), std::integral_constant<int, 6>());
+        if (tid == 0)
+          result.bad = 0;
+        if (!L::ends)
+          meet<kSoft, 6>();
+      }
     }
   }
   __syncthreads();

@@ -47,9 +47,12 @@ struct PagedArgs {
 // Slots: a flag (4 floats), m and l of each vector, then their sums.
 __host__ __device__ __forceinline__ int slot_size(int block, int hd) { return (4 + 2 * block + block * hd + 3) & ~3; }
 
-// Tiles of a request's segments (of each one), and how many segments it has.
+// Tiles of a request's segments (of each one), and how many segments it has. The shares are cut in units: a segment's first
+// stands for its beginning and end, which take about as long as a tile, the others are its tiles (64 requests of up to 1024
+// positions: @@ us so, @@ with shares of as many tiles).
 struct Shape {
   int tiles, segments, blocks;
+  __device__ __forceinline__ long long units() const { return tiles ? (long long)(tiles + 1) * segments : 0; }
 };
 __device__ __forceinline__ Shape shape_of(const PagedArgs &a, const Request &r, int tile) {
   Shape s;
@@ -59,8 +62,8 @@ __device__ __forceinline__ Shape shape_of(const PagedArgs &a, const Request &r, 
   return s;
 }
 
-// The shares of the tiles: `each` to a CTA, one more to the first `longer`. This CTA's are [lo, hi); request b, with
-// `before` tiles before its own, holds the first of them.
+// The shares of the units: `each` to a CTA, one more to the first `longer`. This CTA's are [lo, hi); request b, with
+// `before` units before its own, holds the first of them.
 struct Range {
   long long lo, hi, each, longer, before;
   Request request;
@@ -73,13 +76,13 @@ __device__ __forceinline__ long long quotient(long long n, long long d) {
   return ((n | d) >> 32) == 0 ? (long long)((unsigned)n / (unsigned)d) : n / d;
 }
 
-// The CTA whose share holds tile x.
+// The CTA whose share holds unit x.
 __device__ __forceinline__ int owner(const Range *range, long long x) {
   const long long edge = range->longer * (range->each + 1);
   return (int)(x < edge ? quotient(x, range->each + 1) : range->longer + quotient(x - edge, range->each));
 }
 
-// This CTA's share of `total` tiles: false where it has none.
+// This CTA's share of `total` units: false where it has none.
 __device__ __forceinline__ bool share(long long total, Range *range) {
   const long long ctas = total < gridDim.x ? total : gridDim.x, cta = blockIdx.x;
   if (cta >= ctas)
@@ -99,7 +102,7 @@ __device__ __forceinline__ long long scan(long long x, int lane) {
   return x;
 }
 
-// This CTA's share of the tiles, and the request in which it begins, in every thread's registers. All threads call it;
+// This CTA's share, and the request in which it begins, in every thread's registers. All threads call it;
 // `common` is shared memory. False: nothing to do. Up to kAlone requests, every warp finds it alone, a few requests to a
 // lane: no barrier on the way to the first page (with two, a call of one request took 0.5 us longer).
 constexpr int kEachAlone = 4, kAlone = 32 * kEachAlone;
@@ -125,7 +128,7 @@ __device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *
       if (r[i].bad && blockIdx.x == 0 && warp == 0)
         kc_raise(KC_ERR_BAD_ARGS);
       s[i] = shape_of(a, r[i], tile);
-      own += (long long)s[i].tiles * s[i].segments;
+      own += s[i].units();
     }
     const long long upto = scan(own, lane);
     if (!share(__shfl_sync(0xffffffffu, upto, 31), range))
@@ -137,8 +140,8 @@ __device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *
     int b = b0;
 #pragma unroll
     for (int i = 0; i + 1 < kEachAlone; i++)
-      if (b == b0 + i && lane == from && range->lo >= before + (long long)s[i].tiles * s[i].segments)
-        before += (long long)s[i].tiles * s[i].segments, b++, at = r[i + 1], shape = s[i + 1];
+      if (b == b0 + i && lane == from && range->lo >= before + s[i].units())
+        before += s[i].units(), b++, at = r[i + 1], shape = s[i + 1];
     range->before = __shfl_sync(0xffffffffu, before, from);
     range->b = __shfl_sync(0xffffffffu, b, from);
     range->request.count = __shfl_sync(0xffffffffu, at.count, from);
@@ -157,7 +160,7 @@ __device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *
     if (r.bad && blockIdx.x == 0)
       kc_raise(KC_ERR_BAD_ARGS);
     const Shape s = shape_of(a, r, tile);
-    own += (long long)s.tiles * s.segments;
+    own += s.units();
   }
   long long upto = scan(own, lane);
   if (lane == 31)
@@ -176,7 +179,7 @@ __device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *
     for (int b = b0;; b++) {
       const Request r = request_of(a.starts, a.counts, b, a.rows, a.positions);
       const Shape s = shape_of(a, r, tile);
-      const long long n = (long long)s.tiles * s.segments;
+      const long long n = s.units();
       if (range->lo < before + n) {
         range->before = before, range->b = b, range->request = r, range->shape = s;
         common->range = *range;
@@ -199,7 +202,7 @@ struct Piece {
   int b, head, block;       // request, KV head, block of query vectors
   int start, count, vecs;   // the request's; vectors of this block
   int t0, t1, tiles;
-  long long first;          // the segment's first tile
+  long long first;          // the segment's first unit
 };
 
 // Walks through a CTA's pieces; every thread that walks sees the same.
@@ -211,27 +214,36 @@ struct Walk {
   __device__ __forceinline__ explicit Walk(const Range *range)
       : at(range->lo), before(range->before), b(range->b), request(range->request), shape(range->shape) {}
   __device__ __forceinline__ bool next(const PagedArgs &a, const Range *range, int tile, Piece *p) {
-    if (at >= range->hi)
-      return false;
-    while (at - before >= (long long)shape.tiles * shape.segments) {
-      before += (long long)shape.tiles * shape.segments;
-      b++;
-      request = request_of(a.starts, a.counts, b, a.rows, a.positions);
-      shape = shape_of(a, request, tile);
+    for (;;) {
+      if (at >= range->hi)
+        return false;
+      while (at - before >= shape.units()) {
+        before += shape.units();
+        b++;
+        request = request_of(a.starts, a.counts, b, a.rows, a.positions);
+        shape = shape_of(a, request, tile);
+      }
+      const int units = shape.tiles + 1;
+      const long long local = at - before;
+      const int segment = (int)quotient(local, units);
+      p->first = before + (long long)segment * units;
+      p->t0 = max((int)(at - p->first) - 1, 0);
+      p->t1 = (int)min((long long)units, range->hi - p->first) - 1;
+      at = p->first + p->t1 + 1;
+      if (p->t1 == p->t0)  // the share ends with the segment's first unit
+        continue;
+      p->b = b;
+      p->head = segment / shape.blocks;
+      p->block = segment - p->head * shape.blocks;
+      p->start = request.start, p->count = request.count;
+      p->vecs = min(a.block, request.count * a.group - p->block * a.block);
+      p->tiles = shape.tiles;
+      return true;
     }
-    const long long local = at - before;
-    const int segment = (int)quotient(local, shape.tiles);
-    p->b = b;
-    p->head = segment / shape.blocks;
-    p->block = segment - p->head * shape.blocks;
-    p->start = request.start, p->count = request.count;
-    p->vecs = min(a.block, request.count * a.group - p->block * a.block);
-    p->tiles = shape.tiles;
-    p->first = before + (long long)segment * shape.tiles;
-    p->t0 = (int)(at - p->first);
-    p->t1 = (int)min((long long)shape.tiles, range->hi - p->first);
-    at = p->first + p->t1;
-    return true;
+  }
+  // Whether the piece is the share's last but for a segment's first unit.
+  static __device__ __forceinline__ bool last(const Range *range, const Piece &p) {
+    return p.first + 1 + p.t1 >= range->hi;
   }
 };
 
@@ -258,7 +270,7 @@ __device__ __forceinline__ void finish(const PagedArgs &a, const Range *range, c
   const int hd = HD ? HD : a.hd;
   bool wrong = *bad != 0;
   if (p.t0 || p.t1 < p.tiles) {
-    const int c0 = owner(range, p.first), c1 = owner(range, p.first + p.tiles - 1);
+    const int c0 = owner(range, p.first + 1), c1 = owner(range, p.first + p.tiles);
     const int cta = blockIdx.x, n = p.vecs * hd;
     const int l_at = 4 + a.block, o_at = 4 + 2 * a.block;
     auto slot_of = [&](int c) { return a.partial + (size_t)(2 * c + (c == c0)) * a.slot_floats; };

@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
   } else if (L::ends && warp >= kEnd) {
     // ---- the pieces' ends, but for the share's last ----
     const int tid = threadIdx.x - 32 * kEnd;
-    for (int n = 0; walk.next(a, range, kTile, &p) && p.first + p.t1 < range->hi; n++) {
+    for (int n = 0; walk.next(a, range, kTile, &p) && !Walk::last(range, p); n++) {
       const int at = n & 1;
       tc_wait(&t->rfull[at], (n >> 1) & 1, abort_flag);
       end_piece(at, p, tid, std::integral_constant<int, L::ends ? 32 * L::end_warps : 32>(), std::integral_constant<int, 1>());
@@ -414,13 +414,15 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
     constexpr uint32_t idesc_s = umma_idesc(kBf16, kTile, L::n, false), idesc_o = umma_idesc(kBf16, HD, L::n, true);
     const uint64_t kdesc = umma_desc_sw128(smem), vdesc = umma_desc_sw128_mn(smem, kTile * 128);
     const uint64_t qdesc = umma_desc_sw128(smem + L::q_at), pdesc = umma_desc_sw32_mn(smem + L::p_at, kTile * 32);
-    const int tiles = (int)(range->hi - range->lo);
     int piece = -1, left = 0;  // of the scores issued next: its piece, and tiles of it left
     int kslot = 0, vslot = 1;
     unsigned kpar = 0, vpar = 0;
+    bool more = true;
     auto scores = [&](int j) {
       if (!left) {
-        walk.next(a, range, kTile, &p);
+        more = walk.next(a, range, kTile, &p);
+        if (!more)
+          return false;
         left = p.t1 - p.t0;
         piece++;
         if (!tc_wait(&t->qfull[piece & 1], (piece >> 1) & 1, abort_flag))
@@ -447,9 +449,10 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
         kslot -= L::stages, kpar ^= 1;
       return true;
     };
-    bool ok = scores(0);
-    for (int j = 0; ok && j < tiles; j++) {
-      if (j + 1 < tiles && !scores(j + 1))
+    bool now = scores(0);
+    for (int j = 0; now; j++) {
+      now = scores(j + 1);  // false behind the last tile, or where a wait has run out
+      if (!now && more)
         break;
       if (!tc_wait(&t->full[vslot], vpar, abort_flag) || !tc_wait(&t->pfull[j & 1], (j >> 1) & 1, abort_flag))
         break;
@@ -651,7 +654,7 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
       }
       if (bad)
         result.bad = 1;
-      if (L::ends && p.first + p.t1 < range->hi) {
+      if (L::ends && !Walk::last(range, p)) {
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&t->rfull[at]);

@@ -381,7 +381,7 @@ void k_rope_kv_store_paged(float *q_out, size_t q_out_ld, const float *q, size_t
                            size_t kv_ld, const PagedCache *cache, const float *rope, int seq_len, const int *starts,
                            const int *counts, int n_heads, int n_kv_heads, int head_dim, int batch, int rows);
 
-/* Attention over a paged cache: q and out [batch][rows][n_heads * head_dim]; row r of request b, r < counts[b] (NULL: rows
+/* Attention over a paged cache: q and out [batch][rows][n_heads * head_dim], which do not overlap; row r of request b, r < counts[b] (NULL: rows
  * for all), sees positions [0, starts[b] + r] of its pages: starts[b] were stored before this step's rows (one row: a
  * request's last token; more: its drafts behind it). Other rows of out stay as they were, and a request that uses none
  * needs no starts[b] and no pages. A request with starts[b] outside [0, max_pages * page_size - counts[b]], counts[b]

@@ -261,7 +261,6 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
   volatile int *abort_flag = &t->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  pdl_launch_dependents();
   Range here;
   if (!find_range(a, kTile, &here, reinterpret_cast<RangeRoom *>(t->top)))
     return;
@@ -289,6 +288,7 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_launch_dependents();  // behind the allocation: a kernel that waits for this one cannot hold what it still needs
   const uint32_t tmem = t->tmem;
   const Range *range = &here;
   const float scale = rsqrtf((float)HD) * kLog2e;

@@ -347,6 +347,11 @@ ATTENTION = [  # heads, kv, hd, batch, rows, longest, page
     (48, 1, 128, 2, 3, 400, 16),
     (48, 1, 64, 3, 13, 300, 64),
     (4, 4, 128, 70, 1, 300, 256),
+    (32, 8, 128, 2, 130, 400, 16),
+    (8, 8, 64, 1, 77, 100, 8),
+    (16, 2, 32, 2, 33, 90, 12),
+    (20, 4, 80, 3, 2, 333, 16),
+    (5, 1, 256, 4, 6, 150, 16),
 ]
 
 
@@ -371,6 +376,31 @@ def test_attention(kc, case, dtype):
     for b in range(B):
         assert (got[b, counts[b]:] == -7.0).all()
     close(got, want, hd, top)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 4, 8])
+@pytest.mark.parametrize("dtype", TYPES, ids=name_of)
+@pytest.mark.parametrize("heads,kv,hd,R", [(8, 2, 128, 1), (8, 2, 64, 3), (6, 3, 48, 2)])
+def test_attention_strides_and_alignment(kc, heads, kv, hd, R, dtype, offset):
+    """Queries, outputs and caches at addresses of their elements only, pages an odd stride apart, in any combination that the
+    kernels tell apart."""
+    B, page, lengths = 3, 16, [70, 200, 5]
+    shifted = lambda x, by: torch.cat([torch.zeros(by, device="cuda"), x.flatten()])[by:].view(x.shape)  # noqa: E731
+    for base, gap in ((offset, 0), (0, offset), (offset, offset)):
+        def pool(shape, dtype):
+            each = shape[1] * shape[2] * shape[3] + gap
+            return tuple(torch.full((shape[0] * each + base,), float("nan"), dtype=dtype, device="cuda")[base:]
+                         .as_strided(shape, (each, shape[2] * shape[3], shape[3], 1)) for _ in range(2))
+
+        pages = Pages(kc, 1, lengths, kv, page, hd, dtype, pool=pool)
+        g = generator(offset)
+        fill_normal(pages, g, lengths)
+        q = shifted(normal(g, B, R, heads * hd), offset % 4)
+        out = shifted(torch.full((B, R, heads * hd), -7.0, device="cuda"), base % 4)
+        starts = [n - R for n in lengths]
+        run_attention(kc, pages, q, starts, [R] * B, heads, kv, hd, out=out)
+        want, top = attention_64(pages, q, starts, [R] * B, heads, kv, hd, q)
+        close(out, want, hd, top)
 
 
 def test_attention_all_rows_without_counts(kc):

@@ -32,7 +32,7 @@ constexpr int kUnits = 2 * kHalf;      // and to a stage
 constexpr int kStages = 4;
 constexpr int kClasses = 64;
 constexpr int kCandidates = 512;
-constexpr int kLooks = 4;
+constexpr int kLooks = 2;  // (four at once took 0.4 us longer a row, eight 2: instructions that run once a row come from far)
 constexpr int kMaxParts = 8;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kRise = 3.0f;   // how far a logit may lie above a thread's reference before the reference moves

@@ -190,6 +190,7 @@ __device__ __forceinline__ bool find_range(const PagedArgs &a, int tile, Range *
   }
   __syncthreads();
   *range = common->range;
+  __syncthreads();  // the room may be used again
   return true;
 }
 

@@ -68,14 +68,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
   extern __shared__ __align__(16) uint8_t raw[];
   S *s = reinterpret_cast<S *>(raw);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, hd = a.hd;
-  pdl_wait();
-  pdl_launch_dependents();
-  Range here;
-  if (!find_range(a, kTile, &here, &s->room))
-    return;
-  const Range *range = &here;
-  const float scale = rsqrtf((float)hd) * kLog2e;
-  volatile int *abort_flag = &s->abort_flag;
   if (t == 0) {
     for (int i = 0; i < kStages; i++) {
       mbar_init(&s->full[i], 32 * kCopyWarps);
@@ -85,6 +77,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_f32_kernel(const PagedArgs 
     fence_mbar_init();
   }
   __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  Range here;
+  if (!find_range(a, kTile, &here, &s->room))
+    return;
+  const Range *range = &here;
+  const float scale = rsqrtf((float)hd) * kLog2e;
+  volatile int *abort_flag = &s->abort_flag;
   Walk walk(range);
   Piece p;
 

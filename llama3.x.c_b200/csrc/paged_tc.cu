@@ -260,10 +260,6 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
   auto *t = reinterpret_cast<typename L::End *>(smem + L::tail_at);
   volatile int *abort_flag = &t->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_wait();
-  Range here;
-  if (!find_range(a, kTile, &here, reinterpret_cast<RangeRoom *>(t->top)))
-    return;
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::stages; i++) {
       mbar_init(&t->full[i], 32 * kCopyWarps);
@@ -283,13 +279,23 @@ __global__ void __launch_bounds__(Layout<HD, BLOCK>::threads, 1) paged_tc_kernel
     t->abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == kMma)
-    tmem_alloc(&t->tmem, L::tmem);
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  pdl_launch_dependents();  // behind the allocation: a kernel that waits for this one cannot hold what it still needs
-  const uint32_t tmem = t->tmem;
+  pdl_wait();
+  Range here;
+  if (!find_range(a, kTile, &here, reinterpret_cast<RangeRoom *>(t->top)))
+    return;
+  // The copies start without the tensor memory; the MMAs' warp and the softmax meet for it. Dependents start behind its
+  // allocation: a kernel that waits for this one cannot hold what it still needs.
+  if (warp <= kMma) {
+    if (warp == kMma) {
+      tmem_alloc(&t->tmem, L::tmem);
+      pdl_launch_dependents();
+    }
+    tc_fence_before();
+    meet<kSoft + 32, 7>();
+    tc_fence_after();
+  }
+  const uint32_t tmem = t->tmem;  // for those two
   const Range *range = &here;
   const float scale = rsqrtf((float)HD) * kLog2e;
   Walk walk(range);

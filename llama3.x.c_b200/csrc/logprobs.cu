@@ -9,6 +9,9 @@
 // way of the threads' maxima: with the threads in 64 classes, every one of the top k elements is at or above the k-th largest
 // class maximum, which about as many threads reach as there are tokens to find; only their elements, at a fixed stride,
 // are read again (from L2).
+// What bounds it: many rows, memory: 2048 rows of 128256 184 us, 5.7 TB/s, with 10 us for the last rows' ends; few rows the
+// chain of a row's end, 6 us, a part's stream (12 us for 128256 logits by one CTA) and a cluster's two barriers, 2 us: 64
+// rows of 128256 with 20 alternatives 18.5 us.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>

@@ -63,8 +63,8 @@ __device__ __forceinline__ void put4(__half *at, float4 x) {
 }
 
 // head_dim a multiple of four and everything aligned to four elements: a CTA, or a few with few rows, to a row; each thread
-// has kStoreUnits units of four elements on their way at once. What bounds it: memory, 2048 rows of 32/8 heads of 128 @@ us,
-// @@ TB/s; with few rows the chain starts, page and rotation, store.
+// has kStoreUnits units of four elements on their way at once (a thread per pair of elements took 33 us for what takes 8.5).
+// What bounds it: memory, with two waves of CTAs, 2048 rows of 32/8 heads of 128 22 us, 4.3 TB/s; with few rows the chain starts, page and rotation, store (one row 1.8 us).
 constexpr int kStoreThreads = 256, kStoreUnits = 6;
 template <typename T>
 __global__ void __launch_bounds__(kStoreThreads) paged_store4_kernel(const StoreArgs a) {
@@ -177,16 +177,18 @@ __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
 
 // ---- attention ----------------------------------------------------------------------------------------------------
 
-// The kernel on the CUDA cores: any type, head_dim up to 256, any alignment. LANES lanes take a position, ELEMS of its
-// elements each, so that a score costs log2(LANES) shuffles for ELEMS LANES products, and its weight meets the values in the
-// same lanes without another; VECS query vectors in registers share each key and value (four with 16 elements to a lane, or
-// eight with eight). Every warp has a ring of its own in shared memory, which each lane fills for itself, asynchronously, and
-// reads itself: no barrier until the end of a piece. What bounds it: @@
+// The kernel on the CUDA cores: any type, head_dim up to 256, any alignment. LANES lanes take a position, 16 of its
+// elements each, so that a score costs log2(LANES) shuffles for 16 LANES products, and its weight meets the values in the
+// same lanes without another; four query vectors in registers share each key and value (eight with eight elements to a lane,
+// half the passes over the keys and values, took longer: 24 requests of 28/4 heads of 96 up to 3001 positions 108 us against
+// 75). Every warp has a ring of its own in shared memory, which each lane fills for itself, asynchronously, and reads itself:
+// no barrier until the end of a piece. What bounds it: its instructions, three warps to a scheduler that issue one every
+// 2.8 cycles (32/8 heads of 96 in bf16, 24 requests: 80 us, 1.7 TB/s).
+constexpr int kVecs = 4, kElems = 16, kPairs = kElems / 2;
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kTile = 64;       // positions
 constexpr int kCtas = 148 * 3;  // the shares; a function of nothing else, so that the workspace's size is known
 constexpr int kStages = 4;
-constexpr int kRowsBlock = 8;  // query vectors to a segment at most
 
 // A pair of elements in 32 bits each.
 __device__ __forceinline__ uint64_t pair_of(uint32_t x, __nv_bfloat16) { return f2_pack_bits(x << 16, x & 0xffff0000u); }
@@ -210,13 +212,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// This lane's ELEMS elements of a row: wide, 16-byte units LANES apart; else elements LANES apart.
-template <typename T, int LANES, int ELEMS, bool WIDE>
+// This lane's kElems elements of a row: wide, 16-byte units LANES apart; else elements LANES apart.
+template <typename T, int LANES, bool WIDE>
 struct Row {
   static constexpr int kUnit = 16 / sizeof(T);
-  static constexpr int kUnits = ELEMS / kUnit;
+  static constexpr int kUnits = kElems / kUnit;
   uint4 raw[WIDE ? kUnits : 1];
-  T one[WIDE ? 1 : ELEMS];
+  T one[WIDE ? 1 : kElems];
 
   // The element behind index i of the lane's.
   static __device__ __forceinline__ int element(int lane, int i) {
@@ -237,7 +239,7 @@ struct Row {
   }
   __device__ __forceinline__ void load(const T *row, bool in, int hd, int lane) {
 #pragma unroll
-    for (int i = 0; i < ELEMS; i++)
+    for (int i = 0; i < kElems; i++)
       one[i] = in && lane + LANES * i < hd ? row[lane + LANES * i] : T(0.0f);
   }
   __device__ __forceinline__ uint64_t pair(int i) const {  // elements 2 i, 2 i + 1
@@ -254,23 +256,23 @@ struct Row {
 };
 
 // Shared memory: the warps' rings (nothing where they are not used), and over them their results at the end of a piece.
-template <typename T, int LANES, int ELEMS, int VECS, bool WIDE>
+template <typename T, int LANES, bool WIDE>
 struct RowsSmem {
-  using R = Row<T, LANES, ELEMS, WIDE>;
+  using R = Row<T, LANES, WIDE>;
   static constexpr int slot = 32 * R::kUnits;                            // units of a key or a value
   static constexpr int ring = WIDE ? kStages * 2 * slot * 16 : 0;        // bytes to a warp
-  static constexpr int sums = VECS * LANES * ELEMS * (int)sizeof(float);  // of a warp
+  static constexpr int sums = kVecs * LANES * kElems * (int)sizeof(float);  // of a warp
   static constexpr int total = kWarps * (ring > sums ? ring : sums);
 };
 
-template <typename T, int LANES, int ELEMS, int VECS, bool WIDE>
+template <typename T, int LANES, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs a) {
-  using S = RowsSmem<T, LANES, ELEMS, VECS, WIDE>;
+  using S = RowsSmem<T, LANES, WIDE>;
   using R = typename S::R;
-  constexpr int kAt = 32 / LANES, kStep = kWarps * kAt, kPairs = ELEMS / 2;  // positions of a warp, of all warps at a time
+  constexpr int kAt = 32 / LANES, kStep = kWarps * kAt;  // positions of a warp, of all warps at a time
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ RangeRoom room;
-  __shared__ float wm[kWarps][VECS], wl[kWarps][VECS], m_all[VECS], l_all[VECS];
+  __shared__ float wm[kWarps][kVecs], wl[kWarps][kVecs], m_all[kVecs], l_all[kVecs];
   __shared__ int bad, last;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, sub = lane % LANES, at = lane / LANES;
   uint4 *const ring = reinterpret_cast<uint4 *>(smem + warp * S::ring);
@@ -321,11 +323,11 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
         page = next;
       }
     }
-    uint64_t q[VECS][kPairs], acc[VECS][kPairs];
-    float m[VECS], l[VECS];
-    int limit[VECS];
+    uint64_t q[kVecs][kPairs], acc[kVecs][kPairs];
+    float m[kVecs], l[kVecs];
+    int limit[kVecs];
 #pragma unroll
-    for (int v = 0; v < VECS; v++) {
+    for (int v = 0; v < kVecs; v++) {
       int row = 0;
       const size_t vec = v < p.vecs ? vector_at(a, p, v, &row) : 0;
       limit[v] = v < p.vecs ? p.start + row + 1 : 0;
@@ -357,21 +359,21 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
         k.load(static_cast<const T *>(a.key) + place, in, hd, sub);
         x.load(static_cast<const T *>(a.value) + place, in, hd, sub);
       }
-      float s[VECS];
-      uint64_t part[VECS];
+      float s[kVecs];
+      uint64_t part[kVecs];
 #pragma unroll
-      for (int v = 0; v < VECS; v++)
+      for (int v = 0; v < kVecs; v++)
         part[v] = 0;
 #pragma unroll
       for (int j = 0; j < kPairs; j++) {
         const uint64_t kj = k.pair(j);
 #pragma unroll
-        for (int v = 0; v < VECS; v++)
+        for (int v = 0; v < kVecs; v++)
           part[v] = f2_fma(q[v][j], kj, part[v]);
       }
       bool rises = false;
 #pragma unroll
-      for (int v = 0; v < VECS; v++) {
+      for (int v = 0; v < kVecs; v++) {
         float lo, hi;
         f2_unpack(part[v], lo, hi);
         s[v] = lo + hi;
@@ -379,16 +381,16 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
 #pragma unroll
       for (int o = LANES / 2; o; o >>= 1)
 #pragma unroll
-        for (int v = 0; v < VECS; v++)
+        for (int v = 0; v < kVecs; v++)
           s[v] += __shfl_xor_sync(0xffffffffu, s[v], o);
 #pragma unroll
-      for (int v = 0; v < VECS; v++) {
+      for (int v = 0; v < kVecs; v++) {
         s[v] = position < min(limit[v], end) ? s[v] : -INFINITY;
         rises |= s[v] > m[v];
       }
       if (rises) {
 #pragma unroll
-        for (int v = 0; v < VECS; v++) {
+        for (int v = 0; v < kVecs; v++) {
           if (!(s[v] > m[v]))
             continue;
           const float keep = ex2(m[v] - s[v]);  // 0 at the first
@@ -400,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
         }
       }
 #pragma unroll
-      for (int v = 0; v < VECS; v++) {
+      for (int v = 0; v < kVecs; v++) {
         s[v] = s[v] == -INFINITY ? 0.0f : ex2(s[v] - m[v]) * guard;
         l[v] += s[v];
       }
@@ -409,13 +411,13 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
         for (int j = 0; j < kPairs; j++) {
           const uint64_t xj = x.pair(j);
 #pragma unroll
-          for (int v = 0; v < VECS; v++)
+          for (int v = 0; v < kVecs; v++)
             acc[v][j] = f2_fma(f2_pack(s[v], s[v]), xj, acc[v][j]);
         }
       } else if (position < end) {
         // What a row does not see may be anything: its product is left out, not made with a weight of zero.
 #pragma unroll
-        for (int v = 0; v < VECS; v++)
+        for (int v = 0; v < kVecs; v++)
           if (position < limit[v])
 #pragma unroll
             for (int j = 0; j < kPairs; j++)
@@ -426,10 +428,10 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
       asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();  // the rings' room is free
     // The lane groups' results, then the warps'.
-    float *const sums = reinterpret_cast<float *>(smem);  // [warps][VECS][LANES * ELEMS]
-    constexpr int kLine = LANES * ELEMS;
+    float *const sums = reinterpret_cast<float *>(smem);  // [warps][kVecs][LANES * kElems]
+    constexpr int kLine = LANES * kElems;
 #pragma unroll
-    for (int v = 0; v < VECS; v++) {
+    for (int v = 0; v < kVecs; v++) {
       float top = m[v];
 #pragma unroll
       for (int o = 16; o >= LANES; o >>= 1)
@@ -449,13 +451,13 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
         for (int o = 16; o >= LANES; o >>= 1)
           lo += __shfl_xor_sync(0xffffffffu, lo, o), hi += __shfl_xor_sync(0xffffffffu, hi, o);
         if (at == 0) {
-          sums[(warp * VECS + v) * kLine + R::element(sub, 2 * j)] = lo;
-          sums[(warp * VECS + v) * kLine + R::element(sub, 2 * j + 1)] = hi;
+          sums[(warp * kVecs + v) * kLine + R::element(sub, 2 * j)] = lo;
+          sums[(warp * kVecs + v) * kLine + R::element(sub, 2 * j + 1)] = hi;
         }
       }
     }
     __syncthreads();
-    if (t < VECS) {
+    if (t < kVecs) {
       float top = -INFINITY, sum = 0.0f;
       for (int w = 0; w < kWarps; w++)
         top = fmaxf(top, wm[w][t]);
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
     }
     __syncthreads();
     // Joined in place: [vecs][hd] over the first warps' results, each thread's numbers read before any is written.
-    constexpr int kEach = VECS * kLine / kThreads;
+    constexpr int kEach = kVecs * kLine / kThreads;
     float y[kEach];
 #pragma unroll
     for (int j = 0; j < kEach; j++) {
@@ -476,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
       y[j] = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; w++)
-        y[j] = fmaf(wl[w][v], sums[w * VECS * kLine + i], y[j]);
+        y[j] = fmaf(wl[w][v], sums[w * kVecs * kLine + i], y[j]);
     }
     __syncthreads();
 #pragma unroll
@@ -528,22 +530,18 @@ const char *cache_fault(const PagedCache *c, int n_kv, int hd) {
   return nullptr;
 }
 
-template <typename T, int LANES, int ELEMS, int VECS, bool WIDE>
+template <typename T, int LANES, bool WIDE>
 cudaError_t launch_rows(const PagedArgs &a) {
-  const auto kernel = paged_rows_kernel<T, LANES, ELEMS, VECS, WIDE>;
-  constexpr int smem = RowsSmem<T, LANES, ELEMS, VECS, WIDE>::total;
+  const auto kernel = paged_rows_kernel<T, LANES, WIDE>;
+  constexpr int smem = RowsSmem<T, LANES, WIDE>::total;
   const cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(kernel), smem);
   return e != cudaSuccess ? e : kc_launch_pdl(kernel, dim3(kCtas), dim3(kThreads), smem, kc_stream(), a);
 }
 template <typename T, bool WIDE>
 cudaError_t launch_rows_of(const PagedArgs &a) {
-  if (a.block == 4)
-    return a.hd <= 64    ? launch_rows<T, 4, 16, 4, WIDE>(a)
-           : a.hd <= 128 ? launch_rows<T, 8, 16, 4, WIDE>(a)
-                         : launch_rows<T, 16, 16, 4, WIDE>(a);
-  return a.hd <= 64    ? launch_rows<T, 8, 8, 8, WIDE>(a)
-         : a.hd <= 128 ? launch_rows<T, 16, 8, 8, WIDE>(a)
-                       : launch_rows<T, 32, 8, 8, WIDE>(a);
+  return a.hd <= 64    ? launch_rows<T, 4, WIDE>(a)
+         : a.hd <= 128 ? launch_rows<T, 8, WIDE>(a)
+                       : launch_rows<T, 16, WIDE>(a);
 }
 template <typename T>
 cudaError_t launch_rows_of(const PagedArgs &a) {
@@ -564,7 +562,7 @@ size_t ticket_bytes(int n_heads, int batch, int rows) {
 
 // The slots of whichever kernel has more.
 size_t slots_floats(int hd) {
-  const int rows = 2 * kCtas * slot_size(kRowsBlock, hd), tc = kc_paged_tc_slots_floats(hd);
+  const int rows = 2 * kCtas * slot_size(kVecs, hd), tc = kc_paged_tc_slots_floats(hd);
   return rows > tc ? rows : tc;
 }
 
@@ -703,12 +701,7 @@ void k_attention_paged_rows(float *out, int8_t *oq, float *os, const float *q, c
   a.n_heads = n_heads, a.n_kv = n_kv_heads, a.group = n_heads / n_kv_heads, a.hd = head_dim;
   a.batch = batch, a.rows = rows, a.gs = gs;
   const bool tc = kc_paged_tc_ok(a, cache->type), f32 = kc_paged_f32_ok(a, cache->type);
-  // Eight vectors to a pass over the keys and values where a KV head has more than four (24 requests of 28/4 heads of 128 up
-  // to 3001 positions in fp32: @@ us with eight, @@ with four).
-  a.block = tc                                 ? kc_paged_tc_block(a.group, rows)
-            : f32                              ? kPagedF32Block
-            : (long long)a.group * rows <= 4 ? 4
-                                               : kRowsBlock;
+  a.block = tc ? kc_paged_tc_block(a.group, rows) : f32 ? kPagedF32Block : kVecs;
   a.blocks = blocks_of(n_heads, n_kv_heads, rows, a.block);
   a.slot_floats = slot_size(a.block, head_dim);
   a.by_page = divisor(a.page_size), a.by_group = divisor(a.group);

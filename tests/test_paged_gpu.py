@@ -1025,6 +1025,61 @@ def test_results_repeat(kc, dtype):
         assert same(run_attention(kc, pages, q, [n - 1 for n in lengths], None, heads, kv, hd, work=work), first)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=name_of)
+def test_nothing_in_use(kc, dtype):
+    """No request uses a row: nothing is written, whatever the tables, starts and inputs hold."""
+    heads, kv, hd, B, R = 8, 2, 64, 5, 3
+    pages = Pages(kc, 1, [0] * B, kv, 16, hd, dtype, width=4)
+    nan = torch.full((B, R, heads * hd), float("nan"), device="cuda")
+    out, rope = torch.full_like(nan, -7.0), rope_table(64, hd)
+    starts, counts = [-5, 1 << 30, 0, 7, -(1 << 31)], [0] * B
+    assert run_store(kc, pages, nan, nan[..., :kv * hd], nan[..., :kv * hd], rope, starts, counts, heads, kv, hd, out) == 0
+    run_attention(kc, pages, nan, starts, counts, heads, kv, hd, out=out)
+    assert (out == -7).all() and torch.isnan(pages.key.float()).all() and torch.isnan(pages.value.float()).all()
+    got = run_logprobs(kc, nan[0], [-1] * R, 4)
+    assert kc.status() == 0 and all((x == -7).all() for x in got)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name_of)
+def test_the_librarys_own_memory_and_plain_launches(kc, dtype):
+    """A work on memory that the library allocates; launches without programmatic dependence."""
+    import ctypes
+    heads, kv, hd, lengths = 8, 2, 128, [300, 5]
+    pages = Pages(kc, 1, lengths, kv, 16, hd, dtype)
+    g = generator(1)
+    fill_normal(pages, g, lengths)
+    q = normal(g, 2, 1, heads * hd)
+    work = kc.AttentionWork()
+    kc._call("k_attention_paged_init", ctypes.byref(work), heads, kv, hd, 2, 1, None)
+    assert work.external == 0
+    starts = [n - 1 for n in lengths]
+    want, top = attention_64(pages, q, starts, [1, 1], heads, kv, hd, q)
+    kc.load().kernels_set_pdl(0)
+    try:
+        for _ in range(3):
+            close(run_attention(kc, pages, q, starts, None, heads, kv, hd, work=work), want, hd, top)
+        x = 3 * normal(g, 5, 40000)
+        got = run_logprobs(kc, x, [1, 2, 3, 4, 5], 7)
+        assert kc.status() == 0
+        check_logprobs(x, [1, 2, 3, 4, 5], 7, got)
+    finally:
+        kc.load().kernels_set_pdl(1)
+        kc.k_attention_free(work)
+
+
+def test_a_product_before_and_behind(kc):
+    """Attention between tensor-core products that start while it runs: back to back, many times, the same bits."""
+    s = serving(kc, torch.bfloat16, 5)
+    step(kc, s)
+    assert kc.status() == 0
+    first = [s[n].clone() for n in ("att", "logits", "lp", "ids")]
+    for _ in range(50):
+        step(kc, s)
+    assert kc.status() == 0
+    for x, n in zip(first, ("att", "logits", "lp", "ids")):
+        assert torch.equal(x, s[n])
+
+
 def test_mirror_refuses_what_does_not_fit(kc):
     z = lambda *shape, t=torch.float32: torch.zeros(*shape, dtype=t, device="cuda")  # noqa: E731
     key, table = z(4, 2, 16, 64, t=torch.bfloat16), z(3, 4, t=torch.int32)

@@ -293,10 +293,10 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
     const float guard = guard_of(p.start + p.count);
     const int *pages = a.table + (size_t)p.b * a.max_pages;
     const size_t head = (size_t)p.head * a.page_size * hd;
-    // Step i's page (-2: no position of the piece), and where its row lies.
+    // Step i's page (-2: no position of the piece; a page below 0 is -1), and where its row lies.
     auto page_of = [&](int i) {
       int position = first + i * kStep;
-      return position < end ? pages[divide(position, a.by_page)] : -2;
+      return position < end ? max(pages[divide(position, a.by_page)], -1) : -2;
     };
     auto row_of = [&](int i, int page, bool *in) {
       int within = first + i * kStep;

@@ -1108,3 +1108,25 @@ def test_mirror_refuses_what_does_not_fit(kc):
         with pytest.raises(kc.KernelError):
             kc.k_token_logprobs(args["lp"], None, None, None, args["x"], 100, args["tokens"], 100, 3, 0)
     assert kc.status() == 0
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 256), (torch.bfloat16, 96), (torch.float16, 33), (torch.float32, 64),
+                                      (torch.bfloat16, 128)], ids=str)
+@pytest.mark.parametrize("page", [-2, -3, -128, 67])
+def test_attention_reports_every_number_that_is_no_page(kc, page, dtype, hd):
+    """Small negative numbers, and the first one past the pool, are pages as little as any other."""
+    heads, kv, n = 8, 2, 60
+    pages = Pages(kc, 3, [n, n], kv, 2, hd, dtype, spare=7)
+    assert pages.key.shape[0] == 67
+    g = generator(3)
+    fill_normal(pages, g, [n, n])
+    q = normal(g, 2, 1, heads * hd)
+    want, top = attention_64(pages, q, [n - 1] * 2, [1, 1], heads, kv, hd, q)
+    for index in (0, 11, 29):
+        pages.device_table[1, index] = page
+        out = torch.full_like(q, -7.0)
+        with pytest.raises(kc.KernelError):
+            run_attention(kc, pages, q, [n - 1] * 2, [1, 1], heads, kv, hd, out=out)
+        assert (out[1] == -7).all()
+        close(out[:1], want[:1], hd, top)
+        pages.device_table[1, index] = int(pages.table[1, index])

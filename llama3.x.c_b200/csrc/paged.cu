@@ -276,10 +276,11 @@ __global__ void __launch_bounds__(kThreads, 3) paged_rows_kernel(const PagedArgs
   __shared__ int bad, last;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, sub = lane % LANES, at = lane / LANES;
   uint4 *const ring = reinterpret_cast<uint4 *>(smem + warp * S::ring);
-  pdl_wait();
-  pdl_launch_dependents();
   if (t == 0)
     bad = 0;
+  __syncthreads();  // any warp may set it in its first fetch, and find_range need not hold a barrier
+  pdl_wait();
+  pdl_launch_dependents();
   Range range;
   if (!find_range(a, kTile, &range, &room))
     return;

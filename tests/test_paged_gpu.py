@@ -1130,3 +1130,31 @@ def test_attention_reports_every_number_that_is_no_page(kc, page, dtype, hd):
         assert (out[1] == -7).all()
         close(out[:1], want[:1], hd, top)
         pages.device_table[1, index] = int(pages.table[1, index])
+
+
+@pytest.mark.parametrize("batch", [1, 5, 128])
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 256), (torch.bfloat16, 96), (torch.float16, 33), (torch.float32, 64),
+                                      (torch.bfloat16, 128)], ids=str)
+def test_attention_bad_first_pages_every_time(kc, dtype, hd, batch):
+    """A share whose first page is none: what the first fetch of any warp finds is reported, call after call."""
+    heads, kv, n, times = 8, 2, 3, 50
+    pages = Pages(kc, 3, [n] * batch, kv, 1, hd, dtype)
+    g = generator(3)
+    fill_normal(pages, g, [n] * batch)
+    q = normal(g, batch, 1, heads * hd)
+    work, starts = kc.paged_attention_work(heads, kv, hd, batch), dev([n - 1] * batch)
+    good = pages.device_table.clone()
+    outs = torch.full((times, batch, 1, heads * hd), -7.0, device="cuda")
+    want, top = attention_64(pages, q, [n - 1] * batch, [1] * batch, heads, kv, hd, q)
+    bad = [i % batch for i in range(times)]
+    for i in range(times):
+        pages.device_table.copy_(good)
+        pages.device_table[bad[i], i % n] = -1 - i
+        kc.k_attention_paged_rows(outs[i], None, None, q, pages.cache, starts, None, work, heads, kv, hd, batch, 1, 0)
+        with pytest.raises(kc.KernelError):
+            kc.status()
+    for i in range(times):
+        others = [b for b in range(batch) if b != bad[i]]
+        assert (outs[i, bad[i]] == -7).all()
+        if others:
+            close(outs[i, others], want[others], hd, top)

@@ -406,7 +406,8 @@ void k_attention_paged_rows(float *out, int8_t *oq, float *os, const float *q, c
  * the lowest token first among equals. tokens[r] = -1: a row not in use, its outputs stay as they were. logprobs and tokens
  * may be NULL together: every row is in use. A logit of -infinity is a token ruled out (its log probability -infinity,
  * its share of the entropy 0). A row in use with a NaN, +infinity or no value above -infinity, or a token outside the
- * vocabulary, raises an error (kc_status): its log probabilities and entropy are NaN, its top tokens -1. */
+ * vocabulary, raises an error (kc_status): its log probabilities and entropy are NaN, its top tokens -1. A row may begin at
+ * any element; nothing outside the rows' logits is read. */
 void k_token_logprobs(float *logprobs, float *entropy, int *top_tokens, float *top_logprobs, const float *logits, size_t ld,
                       const int *tokens, int vocab, int rows, int top);
 

@@ -4,7 +4,8 @@
 // neither is rounded against the 1, so that the small logarithm of a nearly certain token keeps its digits.
 //
 // The logits are read once. A CTA takes a row, or with few rows a part of one (a cluster joins them), as a stream of 16 KiB
-// stages by bulk copies, through a ring that runs on into the next row. Each thread keeps the sums of its elements relative to
+// stages by bulk copies, through a ring that runs on into the next row; the ends of a row that does not begin and end at 16
+// bytes come by their elements, so that nothing outside it is read. Each thread keeps the sums of its elements relative to
 // a reference near their maximum, and that maximum with its place. At the end of the row the likeliest tokens are found by
 // way of the threads' maxima: with the threads in 64 classes, every one of the top k elements is at or above the k-th largest
 // class maximum, which about as many threads reach as there are tokens to find; only their elements, at a fixed stride,
@@ -22,6 +23,7 @@
 #include "common.cuh"
 #include "kernels_cuda_internal.h"
 #include "tcgen05.cuh"
+#include "units.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -76,6 +78,7 @@ struct State {
   unsigned long long keys[kThreads], least, best;  // the threads' maxima; the k-th largest class maximum, the largest
   unsigned long long candidates[kCandidates];
   unsigned long long merged[kMaxParts * kMaxTop];
+  __align__(16) float edges[8];  // the elements of a part's first and last unit
   float sums[2][kWarps], again[2];  // the warps' sums; the sums of the thread that has the maximum, without it
   int marked, found, wrong, verdict, owner;
   unsigned short who[kThreads];  // threads whose maximum may be a top one
@@ -86,31 +89,13 @@ constexpr int kSmem = kRing + (int)sizeof(State);
 // The larger of numbers and the first of equals: order of values, then of pairs of units.
 __device__ __forceinline__ unsigned long long pair_key(float x, unsigned pair) { return key_of(x, (int)pair); }
 
-// A row's logits as 16-byte units from the aligned address at or before the first: `off` elements come before it.
-struct Row {
-  const float4 *units;
-  int off, count;  // count: units
-};
-__device__ __forceinline__ Row row_of(const LogprobArgs &a, int row) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(a.logits + (size_t)row * a.ld);
-  Row r;
-  r.units = reinterpret_cast<const float4 *>(at & ~(uintptr_t)15);
-  r.off = (int)((at & 15) / 4);
-  r.count = (int)(((long long)r.off + a.vocab + 3) / 4);
-  return r;
+// Element i of a unit that is not whole, -infinity where it is not the row's.
+__device__ __forceinline__ float edge_element(const UnitRow &r, int unit, int i) {
+  const int at = element_of(r, unit, i);
+  return at >= 0 ? __ldcg(r.data + at) : -INFINITY;
 }
-// Part p of n of its units.
-__device__ __forceinline__ void part_of(const Row &r, int p, int n, int *first, int *end) {
-  *first = (int)((long long)r.count * p / n);
-  *end = (int)((long long)r.count * (p + 1) / n);
-}
-// A unit's elements, -infinity for those that are not the row's.
-__device__ __forceinline__ void only_row(float *x, const Row &r, int unit, int vocab) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const long long at = 4ll * unit + i - r.off;
-    x[i] = at >= 0 && at < vocab ? x[i] : -INFINITY;
-  }
+__device__ __forceinline__ float4 edge_unit(const UnitRow &r, int unit) {
+  return make_float4(edge_element(r, unit, 0), edge_element(r, unit, 1), edge_element(r, unit, 2), edge_element(r, unit, 3));
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -217,15 +202,33 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
       for (int row = blockIdx.x / parts; ok && row < a.rows; row += stride) {
         if (a.tokens && a.tokens[row] == -1)
           continue;
-        const Row r = row_of(a, row);
+        const UnitRow r = unit_row(a.logits + (size_t)row * a.ld, a.vocab);
         int first, end;
         part_of(r, part, parts, &first, &end);
+        // The part's first and last unit by their elements where not all of them are the row's.
+        int whole0, whole1;
+        whole_of(r, first, end, &whole0, &whole1);
+        float4 head, tail;
+        if (first < whole0)
+          head = edge_unit(r, first);
+        if (whole1 < end)
+          tail = edge_unit(r, whole1);
         for (int u = first; ok && u < end; u += kUnits) {
+          const int upto = min(u + kUnits, end), from = max(u, whole0), to = min(upto, whole1);
+          float4 *const slot = reinterpret_cast<float4 *>(smem + stage * kUnits * 16);
           ok = mbar_wait_bounded(&t->empty[stage], parity ^ 1);
-          const unsigned bytes = 16u * (unsigned)min(kUnits, end - u);
           if (ok) {
-            mbar_arrive_expect_tx(&t->full[stage], bytes);
-            bulk_g2s(smem + stage * kUnits * 16, r.units + u, bytes, &t->full[stage]);
+            if (from < to) {
+              mbar_expect_tx(&t->full[stage], 16u * (unsigned)(to - from));
+              bulk_g2s(slot + (from - u), unit_at(r, from), 16u * (unsigned)(to - from), &t->full[stage]);
+            }
+            if (from > u)
+              slot[0] = head;
+            if (to < upto)
+              slot[to - u] = tail;
+            if (to - from < upto - u)
+              fence_proxy_async_smem();  // before a later copy's writes
+            mbar_arrive(&t->full[stage]);
           }
           if (++stage == kStages)
             stage = 0, parity ^= 1;
@@ -239,7 +242,7 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
       const int token = a.tokens ? a.tokens[row] : 0;
       if (token == -1)
         continue;
-      const Row r = row_of(a, row);
+      const UnitRow r = unit_row(a.logits + (size_t)row * a.ld, a.vocab);
       int first, end;
       part_of(r, part, parts, &first, &end);
       Running mine;
@@ -247,6 +250,8 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
       mine.s[0] = mine.s[1] = mine.t[0] = mine.t[1] = 0;
       bool wrong = token < 0 || token >= a.vocab;
       const float given = tid == 0 && part == 0 && !wrong ? __ldcg(a.logits + (size_t)row * a.ld + token) : 0.0f;
+      // The part's first and last unit once more, for the second look: an element a thread.
+      const float edge_value = tid < 8 ? edge_element(r, tid < 4 ? first : end - 1, tid & 3) : 0.0f;
       for (int u = first; u < end; u += kUnits) {
         ok = ok && mbar_wait_bounded(&t->full[stage], parity);
         // The two units in an order that keeps eight lanes in different banks.
@@ -255,15 +260,17 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
         float x[2][8];
 #pragma unroll
         for (int h = 0; h < 4; h++) {
-          const int at = (h >> 1) * kHalf + ((h & 1) ^ swap);
-          const float4 y = u + 2 * tid + at < end ? from[at] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          const float4 y = from[(h >> 1) * kHalf + ((h & 1) ^ swap)];
           float *to = &x[h >> 1][4 * (h & 1)];
           to[0] = y.x, to[1] = y.y, to[2] = y.z, to[3] = y.w;
         }
-        if (u == 0 || u + kUnits >= r.count)
+        if (u + kUnits > end)  // the part's last stage, which others' units follow
 #pragma unroll
           for (int h = 0; h < 4; h++)
-            only_row(&x[h >> 1][4 * (h & 1)], r, u + 2 * tid + (h >> 1) * kHalf + ((h & 1) ^ swap), a.vocab);
+            if (u + 2 * tid + (h >> 1) * kHalf + ((h & 1) ^ swap) >= end)
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                x[h >> 1][4 * (h & 1) + i] = -INFINITY;
         take(mine, x, (unsigned)((u - first) / 2 + tid), &wrong);
         // The stage is given back only now, behind the fence between this warp's reads and the next copy's writes: before it,
         // loads still under way read what the copy brought (one row in a hundred wrong at 2048 rows of 128256).
@@ -278,6 +285,8 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
       // ---- the end of the part: the maximum, and the class maximum that holds the top ones ----
       const unsigned long long key = first + 2 * tid < end ? pair_key(mine.max, mine.pair) : 0;
       t->keys[tid] = key;
+      if (tid < 8)
+        t->edges[tid] = edge_value;
       if (wrong)
         t->wrong = 1;
       meet();
@@ -328,6 +337,8 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
       const int marked = bad ? 0 : t->marked;
       const int each = (end - first + 2 * 16 * kThreads - 1) / (2 * 16 * kThreads);  // looks at a thread's pairs
       const int looks = warp == 0 ? (marked ? each : 0) : marked * each;
+      int whole0, whole1;  // the part's whole units
+      whole_of(r, first, end, &whole0, &whole1);
       const unsigned best_pair = 0xffffffffu - (unsigned)best;
       const float edge = least ? logit_of(least) : -INFINITY;
       float s2 = 0.0f, e2 = 0.0f;
@@ -340,31 +351,35 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
           const int i = i0 + k * (warp == 0 ? 1 : kWarps - 1), who = warp == 0 ? t->owner : t->who[min(i, looks - 1) / each];
           const int look = warp == 0 ? i : i % each;
           pair[k] = look * 16 * kThreads + who + (lane >> 1) * kThreads;
-          in[k] = i < looks && first + 2 * pair[k] + (lane & 1) < end && (warp == 0 || who != t->owner);
-          y[k] = in[k] ? __ldcg(r.units + first + 2 * pair[k] + (lane & 1)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          const int unit = first + 2 * pair[k] + (lane & 1);
+          in[k] = i < looks && unit >= whole0 && unit < whole1 && (warp == 0 || who != t->owner);
+          y[k] = in[k] ? __ldcg(reinterpret_cast<const float4 *>(unit_at(r, unit))) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
 #pragma unroll
         for (int k = 0; k < kLooks; k++) {
           const int unit = first + 2 * pair[k] + (lane & 1);
           float x[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
-          if (unit == 0 || unit == r.count - 1)
-            only_row(x, r, unit, a.vocab);
           if (in[k] && fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= edge) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-              const long long at = 4ll * unit + j - r.off;
-              if (at >= 0 && at < a.vocab && pair_key(x[j], (unsigned)pair[k]) >= least) {
+              const int at = element_of(r, unit, j);
+              if (at >= 0 && pair_key(x[j], (unsigned)pair[k]) >= least) {
                 const int n = atomicAdd(&t->found, 1);
                 if (n < kCandidates)
-                  t->candidates[n] = key_of(x[j], (int)at);
+                  t->candidates[n] = key_of(x[j], at);
               }
             }
           }
           if (warp == 0) {
             // The maximum is left out once: in the pair that it first came in, the first of it. (What is not the row's is
             // -infinity, and adds nothing.)
-            if (!in[k])
+            if (!in[k]) {
               x[0] = x[1] = x[2] = x[3] = -INFINITY;
+              if (i0 + k < looks && unit < end)  // an edge
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                  x[j] = t->edges[(unit < whole0 ? 0 : 4) + j];
+            }
             const bool has = (unsigned)pair[k] == best_pair && fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) == top;
             const unsigned holders = __ballot_sync(0xffffffffu, has);
             bool out = has && lane == __ffs(holders) - 1;
@@ -375,6 +390,15 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
               weigh(x[j] - top, s2, e2);
             }
           }
+        }
+      }
+      // The edges' elements, which threads 0 to 7 have.
+      if (!bad && (tid < 4 ? first < whole0 : tid < 8 && whole1 < end)) {
+        const int unit = tid < 4 ? first : end - 1, at = element_of(r, unit, tid & 3);
+        if (at >= 0 && pair_key(edge_value, (unsigned)(unit - first) / 2) >= least) {
+          const int n = atomicAdd(&t->found, 1);
+          if (n < kCandidates)
+            t->candidates[n] = key_of(edge_value, at);
         }
       }
       if (warp == 0) {
@@ -415,13 +439,15 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
         for (int n = 0; n < wanted; n++) {
           unsigned long long k = 0;
           for (int unit = first + tid; unit < end; unit += kThreads) {
-            const float4 y = __ldcg(r.units + unit);
+            const float4 y = unit >= whole0 && unit < whole1
+                                 ? __ldcg(reinterpret_cast<const float4 *>(unit_at(r, unit)))
+                                 : *reinterpret_cast<const float4 *>(t->edges + (unit < whole0 ? 0 : 4));
             const float x[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              const long long at = 4ll * unit + i - r.off;
-              if (at >= 0 && at < a.vocab) {
-                const unsigned long long other = key_of(x[i], (int)at);
+              const int at = element_of(r, unit, i);
+              if (at >= 0) {
+                const unsigned long long other = key_of(x[i], at);
                 k = other < last ? max_key(k, other) : k;
               }
             }

@@ -1158,3 +1158,28 @@ def test_attention_bad_first_pages_every_time(kc, dtype, hd, batch):
         assert (outs[i, bad[i]] == -7).all()
         if others:
             close(outs[i, others], want[others], hd, top)
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+@pytest.mark.parametrize("vocab", list(range(1, 13)) + [4096, 4097, 4098, 4099, 8191, 262143, 262145])
+def test_logprobs_at_the_ends_of_rows(kc, vocab, offset):
+    """The likeliest tokens, the largest of them among equals, and the tokens asked for are a row's first and last ones, whose
+    16 bytes are not all the row's; what lies there beside them is NaN or larger than any."""
+    rows = 4
+    ld = vocab + 7
+    room = torch.full((rows * ld + offset,), float("nan"), device="cuda")
+    room[::2] = float("inf")
+    x = room[offset:].as_strided((rows, vocab), (ld, 1))
+    g = generator(vocab + offset)
+    base = normal(g, rows, vocab)
+    ends = [i for i in range(vocab) if i < 4 or i >= vocab - 4]
+    base[0, ends] = 6.0 + 0.1 * torch.rand(len(ends), device="cuda", generator=g)
+    base[1, ends] = 7.0
+    base[2, ends[-1]] = 30.0
+    base[3, ends[0]] = 30.0
+    x.copy_(base)
+    top = min(vocab, 8)
+    for tokens in ([0, vocab - 1, vocab - 1, 0], [vocab // 2] * 4):
+        got = run_logprobs(kc, x, tokens, top)
+        assert kc.status() == 0
+        check_logprobs(base, tokens, top, got)

@@ -199,6 +199,7 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
     // ---- copies ----
     if (lane == 0) {
       bool ok = true;
+      unsigned fills = 0;  // of the ring's stages
       for (int row = blockIdx.x / parts; ok && row < a.rows; row += stride) {
         if (a.tokens && a.tokens[row] == -1)
           continue;
@@ -229,11 +230,16 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
             if (to - from < upto - u)
               fence_proxy_async_smem();  // before a later copy's writes
             mbar_arrive(&t->full[stage]);
+            fills++;
           }
           if (++stage == kStages)
             stage = 0, parity ^= 1;
         }
       }
+      // No copy is under way when the CTA ends, also where a wait, here or of those who take the logits, has run out.
+#pragma unroll 1
+      for (unsigned i = fills > kStages ? fills - kStages : 0; i < fills; i++)
+        mbar_wait_sleep_bounded(&t->full[i % kStages], (i / kStages) & 1);
     }
     __syncwarp();
   } else {

@@ -1183,3 +1183,151 @@ def test_logprobs_at_the_ends_of_rows(kc, vocab, offset):
         got = run_logprobs(kc, x, tokens, top)
         assert kc.status() == 0
         check_logprobs(base, tokens, top, got)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name_of)
+def test_captured_steps_with_new_and_moved_pages(kc, dtype):
+    """A captured step replays while a request reaches a page that was none at capture and gets it only then, and while pages
+    that are in use move elsewhere in the pool."""
+    s = serving(kc, dtype, 2)
+    page = 16
+    pages = s["pages"] = Pages(kc, 2, [106, 43, 6], s["kv"], page, s["hd"], dtype, width=9, spare=8)  # the rest: no page
+    fill_normal(pages, generator(2), [100, 37, 0])
+    step(kc, s)  # sizes every buffer that a first call makes
+    assert kc.status() == 0
+    used = set(pages.table[0, :7]) | set(pages.table[1, :3]) | {pages.table[2, 0]}
+    spare = [p for p in range(pages.key.shape[0]) if p not in used]
+    none = lambda b, index: not 0 <= pages.table[b, index] < pages.key.shape[0]  # noqa: E731
+    assert none(0, 7) and none(2, 1)
+
+    def point(b, index, to):  # the table's entry, here and on the device
+        pages.table[b, index] = to
+        pages.device_table[b, index] = to
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    starts, counts = [101, 40, 6], [6, 1, 6]
+    with torch.cuda.stream(side):
+        s["starts"].copy_(torch.tensor(starts, dtype=torch.int32))
+        s["counts"].copy_(torch.tensor(counts, dtype=torch.int32))
+        with torch.cuda.graph(graph, stream=side):
+            step(kc, s)
+        for i in range(4):
+            if starts[0] + counts[0] > 7 * page and none(0, 7):
+                point(0, 7, spare.pop())
+            if starts[2] + counts[2] > page and none(2, 1):
+                point(2, 1, spare.pop())
+            if i >= 2:  # the first page of request 1 moves, and what it held is overwritten
+                old, new = int(pages.table[1, 0]), spare.pop()
+                for cache in (pages.key, pages.value):
+                    cache[new] = cache[old]
+                    cache[old] = float("nan")
+                point(1, 0, new)
+            s["starts"].copy_(torch.tensor(starts, dtype=torch.int32))
+            s["counts"].copy_(torch.tensor(counts, dtype=torch.int32))
+            s["x"].copy_(normal(generator(i), *s["x"].shape))
+            graph.replay()
+            side.synchronize()
+            assert kc.status() == 0
+            check_step(kc, s, starts, counts)
+            starts = [n + c for n, c in zip(starts, counts)]
+            counts = [5, 1, 5] if i == 0 else [1, 2, 3]
+        assert starts[0] > 7 * page and starts[2] > page
+
+
+def unsound_batch(kc, seed, batch, rows, kv, page, hd, dtype):
+    """A batch of short requests, some without rows, and of those with rows some with an unsound start or count or a page
+    that is none: (pages, starts, counts, counts of the sound ones)."""
+    rng = np.random.default_rng(seed)
+    counts = [int(c) for c in rng.integers(0, rows + 1, batch)]
+    lengths = [c + int(rng.integers(0, 70)) if c else 0 for c in counts]
+    starts = [n - c for n, c in zip(lengths, counts)]
+    pages = Pages(kc, seed, lengths, kv, page, hd, dtype)
+    g = generator(seed)
+    fill_normal(pages, g, lengths)
+    live = [b for b in range(batch) if counts[b]]
+    wrong = sorted(rng.choice(live, 24, replace=False).tolist()) + [live[0], live[-1]]
+    sound = [0 if b in wrong else c for b, c in enumerate(counts)]
+    most = pages.width * page
+    for i, b in enumerate(wrong):
+        if i % 6 == 0:
+            starts[b] = -1 - i
+        elif i % 6 == 1:
+            starts[b] = most - counts[b] + 1
+        elif i % 6 == 2:
+            counts[b] = rows + 1 + i
+        elif i % 6 == 3:
+            counts[b] = -1 - i
+        elif i % 6 == 4:
+            starts[b] = 2 ** 31 - 1
+        else:
+            pages.device_table[b, int(rng.integers(0, -(-lengths[b] // page)))] = -1 - i
+    return pages, starts, counts, sound
+
+
+@pytest.mark.parametrize("batch,rows", [(129, 3), (400, 1), (1000, 2)])
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64), (torch.float32, 128),
+                                      (torch.bfloat16, 96), (torch.float32, 256)], ids=str)
+def test_attention_many_requests_some_unsound(kc, dtype, hd, batch, rows):
+    """More requests than a warp looks at alone, unsound ones among them: an error, their rows as they were, the others'
+    right, and the work as good as new."""
+    heads, kv, page = 8, 2, 16
+    pages, starts, counts, sound = unsound_batch(kc, batch + hd, batch, rows, kv, page, hd, dtype)
+    q = normal(generator(1), batch, rows, heads * hd)
+    work = kc.paged_attention_work(heads, kv, hd, batch, rows)
+    out = torch.full_like(q, -7.0)
+    want, top = attention_64(pages, q, starts, sound, heads, kv, hd, torch.full_like(q, -7.0))
+    with pytest.raises(kc.KernelError):
+        run_attention(kc, pages, q, starts, counts, heads, kv, hd, work=work, out=out)
+    for b in range(batch):
+        assert (out[b, sound[b]:] == -7).all()
+    close(out, want, hd, top)
+    # Another batch to the kernel, whose work is shared out without them: equal results, not equal bits.
+    close(run_attention(kc, pages, q, starts, sound, heads, kv, hd, work=work), want, hd, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name_of)
+def test_store_many_requests_some_unsound(kc, dtype):
+    heads, kv, hd, batch, rows, page = 4, 2, 64, 300, 3, 16
+    pages, starts, counts, sound = unsound_batch(kc, 5, batch, rows, kv, page, hd, dtype)
+    g = generator(2)
+    q, k, v = (normal(g, batch, rows, n * hd) for n in (heads, kv, kv))
+    rope, q_out = rope_table(pages.width * page, hd), torch.full((batch, rows, heads * hd), -7.0, device="cuda")
+    # A row whose page is none is left out, and only that row; a request that is unsound whole.
+    table, most = pages.device_table.tolist(), pages.width * page
+    tried = [c if 0 <= c <= rows and 0 <= s <= most - c else 0 for s, c in zip(starts, counts)]
+    left = {(b, r) for b in range(batch) for r in range(tried[b])
+            if not 0 <= table[b][(starts[b] + r) // page] < pages.key.shape[0]}
+    want = stored(pages, q, k, v, rope, starts, tried, heads, kv, hd, q_out, skip=left)
+    with pytest.raises(kc.KernelError):
+        run_store(kc, pages, q, k, v, rope, starts, counts, heads, kv, hd, q_out)
+    check_store((q_out, pages.key, pages.value), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name_of)
+@pytest.mark.parametrize("heads,kv,hd", [(32, 8, 128), (32, 8, 64), (28, 4, 128), (8, 2, 96)])
+@pytest.mark.parametrize("rows", [5, 8, 150])
+def test_attention_prompts_drafts_and_single_tokens_together(kc, heads, kv, hd, rows, dtype):
+    """One call of a serving batch: a prompt or drafts of the longest number of rows, drafts, single tokens, and a slot out of
+    use; each request as in a call of its own."""
+    counts = [1, rows, 1, 0, 3, 1, 1, 2, 1]
+    starts = [500, 0, 1, 0, 130, 77, 1023, 64, 0]
+    lengths = [s + c if c else 0 for s, c in zip(starts, counts)]
+    pages = Pages(kc, rows, lengths, kv, 16, hd, dtype)
+    g = generator(hd + rows)
+    fill_normal(pages, g, lengths)
+    q = 1.5 * normal(g, len(counts), rows, heads * hd)
+    got = run_attention(kc, pages, q, starts, counts, heads, kv, hd)
+    want, top = attention_64(pages, q, starts, counts, heads, kv, hd, torch.full_like(q, -7.0))
+    for b, c in enumerate(counts):
+        assert (got[b, c:] == -7).all()
+    close(got, want, hd, top)
+    for b, c in enumerate(counts):
+        if c:
+            alone = Pages.__new__(Pages)
+            alone.__dict__.update(pages.__dict__)
+            alone.table, alone.device_table = pages.table[b:b + 1], pages.device_table[b:b + 1].contiguous()
+            alone.cache = kc.paged_cache(pages.key, pages.value, alone.device_table)
+            own = run_attention(kc, alone, q[b:b + 1, :c].contiguous(), [starts[b]], [c], heads, kv, hd)
+            close(own, want[b:b + 1, :c], hd, top)

@@ -710,10 +710,22 @@ bool kc_paged_tc_ok(const PagedArgs &a, int type) {
          !(((uintptr_t)a.key | (uintptr_t)a.value) & 15);
 }
 
-// The smallest block that holds a KV head's vectors, or the largest.
+// The smallest block that holds a KV head's vectors (of as many rows as the call's longest request may have) up to 16; blocks
+// of 16 up to 64 vectors, and of 32, which fetch the keys and values half as often but keep four softmax groups with eight
+// vectors to a thread and a ring of two tiles, beyond. Device time in a graph of calls, us, heads of 128 in bf16:
+//   16 requests of 32/8 heads, up to 4099 positions   blocks of 4     8    16    32
+//     4 vectors                                            39.0  38.8  38.1  50.1
+//     8                                                    43.7  39.5  39.7  52.0
+//     12                                                   54.9  45.3  41.7  54.6
+//     20                                                   76.0  56.1  48.4  58.6
+//     32                                                    105  73.7  54.9  62.2
+//     48, 64, 128                                     of 16: 66.2, 89.1, 98.7  of 32: 74.4, 83.7, 89.1
+//   4 requests of 8/8 heads, up to 1000 positions, 64, 96, 128 vectors  16.2, 20.8, 23.8    21.0, 21.0, 24.6
+//   512 rows of 32/8 heads behind 2048 positions            217                     160
+//   32 requests of 32/8 heads, up to 2048 positions: one of 8 rows, 31 of one  40.9  41.0  41.8  60.6
 int kc_paged_tc_block(int group, int rows) {
   const long long vecs = (long long)group * rows;
-  return vecs <= 4 ? 4 : vecs <= 8 ? 8 : vecs <= 16 ? 16 : kMaxBlock;
+  return vecs <= 4 ? 4 : vecs <= 8 ? 8 : vecs <= 64 ? 16 : kMaxBlock;
 }
 
 int kc_paged_tc_slots_floats(int hd) { return 2 * kCtas * slot_size(kMaxBlock, hd); }

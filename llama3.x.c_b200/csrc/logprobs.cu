@@ -561,14 +561,19 @@ extern "C" void k_token_logprobs(float *logprobs, float *entropy, int *top_token
   memset(&a, 0, sizeof(a));
   a.logprobs = logprobs, a.entropy = entropy, a.top_tokens = top_tokens, a.top_logprobs = top_logprobs;
   a.logits = logits, a.ld = ld, a.tokens = tokens, a.vocab = vocab, a.rows = rows, a.top = top;
-  // A cluster of CTAs to a row while their parts are long enough to pay for its two barriers: 2 us where every CTA has an
-  // SM to itself (8 rows of 128256: 23 us in one part, 12 in four; 64 rows of 32000: 9.9 in one, 10.6 in two), 4 to 5 us
-  // where they share them (200 rows of 128256: 30 us in one part, 27 in two; 129 rows of 50001: 12 in one, 16 in two).
+  // A cluster of CTAs to a row while their parts are long enough to pay for its two barriers, which cost more where CTAs share
+  // their SMs; and one CTA where the rows have an SM each with few left over. Device time in a graph, us, by parts (rows x
+  // vocabulary: in 1, 2, 4, 8): 1 x 32000: 9.3, 8.9, 8.6, 9.4; 8 x 32000: 9.2, 9.1, 8.7, 9.6; 64 x 32000: 9.4, 9.6, 11.2;
+  // 8 x 128256: 18.7, 13.6, 11.1, 10.8; 30 x 50001: 11.3, 10.3, 10.4, 14.1; 37 x 128256: 18.9, 13.8, 12.7, 15.5; 64 x 128256:
+  // 19.0, 15.4, 15.7; 32 x 262144: 31.9, 20.4, 16.7, 18.0; 74 x 65000: 12.3, 12.1, 12.9; 100 x 128256: 19.1, 17.0, 16.1;
+  // 110: 19.2, 17.0; 120: 19.1, 21.3; 148: 19.2, 21.3; 160: 24.8, 21.7; 200: 26.2, 23.4; 129 x 50001: 11.6, 14.4.
   const int sms = kc_device_sms();
   int parts = 1;
   for (; parts < kMaxParts; parts *= 2) {
     const long long ctas = (long long)rows * parts * 2;
     if (ctas > kCtas * sms || vocab / (2 * parts) < (ctas <= sms ? 16384 : 49152))
+      break;
+    if (parts == 1 && rows <= sms && 2 * ctas > 3 * sms)
       break;
   }
   cudaError_t e = kc_allow_smem(reinterpret_cast<const void *>(logprobs_kernel), kSmem);

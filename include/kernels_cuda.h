@@ -387,8 +387,11 @@ void k_rope_kv_store_paged(float *q_out, size_t q_out_ld, const float *q, size_t
  * needs no starts[b] and no pages. A request with starts[b] outside [0, max_pages * page_size - counts[b]], counts[b]
  * outside [0, rows], or a page that it sees outside [0, pages) raises an error (kc_status) and its rows stay as they were.
  * What a row sees must be finite, or that row has no result; what it does not see, finite or not (the rest of a page,
- * pages no one uses, later drafts), changes nothing in it. Products are fp32 ones up to 2^-22 of each, sums and statistics
- * fp32; values below 2^-80 keep fewer bits behind thousands of positions. oq / os (may be NULL): out quantized for Wo as k_quantize does, gs dividing head_dim. head_dim <= 256.
+ * pages no one uses, later drafts), changes nothing in it. Products are fp32 ones up to 2^-22 of each (an fp16 cache with
+ * head_dim 64 or 128: of a query's elements down to 2^-39 of its largest and of weights down to 2^-32 of their row's largest;
+ * smaller ones are off by up to 2^-61 and 2^-54 of the largest), sums and statistics fp32: rounded to nearest, but for the sums
+ * of 16-bit caches with head_dim 64 or 128 over the head and over 128 positions, which the tensor cores cut towards zero.
+ * Values below 2^-80 keep fewer bits behind thousands of positions. oq / os (may be NULL): out quantized for Wo as k_quantize does, gs dividing head_dim. head_dim <= 256.
  * `work` (k_attention_paged_init, released with k_attention_free): partial results and tickets for this n_heads and
  * head_dim and up to batch * rows rows (its `workers`; its max_chunks is -1, so that no other kind of work passes for it);
  * `memory` as for k_attention_init_rows (k_attention_paged_bytes bytes, 16-byte aligned, or NULL). k_attention_paged_init

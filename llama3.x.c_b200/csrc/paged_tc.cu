@@ -6,12 +6,14 @@
 // K the K-major and V the MN-major operand A of the same row-major layout (128-byte swizzle), Q and P the operand B.
 // The 16-bit types are widened by columns: a query vector takes three of the N columns, x = x0 + x1 + x2 in three 16-bit
 // parts, and so does a vector of probabilities; the products of a 16-bit key or value with each part are exact, their sum
-// is the fp32 product up to 2^-24 of it.
+// is the fp32 product up to 2^-22 of it.
 //   bf16: the parts are the leading, middle and last eight bits of the significand, cut off, not rounded: no part's
 //         rounding carries into the one before, and they add up to x exactly. bf16 has fp32's exponents.
 //   fp16: x 2^k with the largest magnitude of a query vector just below 2^15 (probabilities: 2^15 at most), then each part
 //         rounded and the rest times 2^11 for the next, so that a part of a small x is not lost below fp16's exponents; the
-//         columns are joined with 2^-11 and 2^-22.
+//         columns are joined with 2^-11 and 2^-22. The last part is a multiple of 2^-24, so x is off by up to 2^-47: 2^-22 of
+//         it down to 2^-25. A query's largest element is 2^14 at least, a row's largest probability 2^7: 2^-22 of elements
+//         down to 2^-39 and of probabilities down to 2^-32 of the largest, below that 2^-61 and 2^-54 of the largest.
 // A tile's sums are a product of their own, eight MMAs that start at zero; they join the running sums in fp32, in
 // registers, rounded to nearest (the tensor cores' accumulators cut towards zero).
 //

@@ -1331,3 +1331,24 @@ def test_attention_prompts_drafts_and_single_tokens_together(kc, heads, kv, hd, 
             alone.cache = kc.paged_cache(pages.key, pages.value, alone.device_table)
             own = run_attention(kc, alone, q[b:b + 1, :c].contiguous(), [starts[b]], [c], heads, kv, hd)
             close(own, want[b:b + 1, :c], hd, top)
+
+
+@pytest.mark.parametrize("hd", [128, 64, 96])
+@pytest.mark.parametrize("dtype", TYPES, ids=name_of)
+@pytest.mark.parametrize("bits", [20, 28, 31])
+def test_attention_small_weights_keep_their_digits(kc, dtype, hd, bits):
+    """A weight of 2^-bits of the row's largest, the only one with a value: the result is its product, to fp32's roundings."""
+    heads, kv, n = 4, 1, 300
+    pages = Pages(kc, 5, [n], kv, 16, hd, dtype)
+    keys, values = torch.zeros(kv, n, hd, device="cuda"), torch.zeros(kv, n, hd, device="cuda")
+    keys[:, :, 0] = 8.0
+    keys[:, 130, 0] = 0.0
+    values[:, 130] = 1.0 + torch.rand(hd, device="cuda", generator=generator(bits))
+    pages.fill(0, keys, values)
+    q = torch.zeros(1, 1, heads, hd, device="cuda")
+    q[..., 0] = bits * float(np.log(2.0)) / 8.0 * hd ** 0.5
+    q = q.view(1, 1, heads * hd)
+    got = run_attention(kc, pages, q, [n - 1], [1], heads, kv, hd)
+    want, top = attention_64(pages, q, [n - 1], [1], heads, kv, hd, q)
+    assert 2.0 ** -(bits + 10) < float(want.abs().min()) and float(want.abs().max()) < 2.0 ** -(bits + 6)
+    close(got, want, hd, top)

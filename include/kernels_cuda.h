@@ -381,21 +381,23 @@ void k_rope_kv_store_paged(float *q_out, size_t q_out_ld, const float *q, size_t
                            size_t kv_ld, const PagedCache *cache, const float *rope, int seq_len, const int *starts,
                            const int *counts, int n_heads, int n_kv_heads, int head_dim, int batch, int rows);
 
-/* Attention over a paged cache: q and out [batch][rows][n_heads * head_dim], which do not overlap; row r of request b, r < counts[b] (NULL: rows
- * for all), sees positions [0, starts[b] + r] of its pages: starts[b] were stored before this step's rows (one row: a
- * request's last token; more: its drafts behind it). Other rows of out stay as they were, and a request that uses none
- * needs no starts[b] and no pages. A request with starts[b] outside [0, max_pages * page_size - counts[b]], counts[b]
- * outside [0, rows], or a page that it sees outside [0, pages) raises an error (kc_status) and its rows stay as they were.
- * What a row sees must be finite, or that row has no result; what it does not see, finite or not (the rest of a page,
- * pages no one uses, later drafts), changes nothing in it. Products are fp32 ones up to 2^-22 of each (an fp16 cache with
- * head_dim 64 or 128: of a query's elements down to 2^-39 of its largest and of weights down to 2^-32 of their row's largest;
- * smaller ones are off by up to 2^-61 and 2^-54 of the largest), sums and statistics fp32: rounded to nearest, but for the sums
- * of 16-bit caches with head_dim 64 or 128 over the head and over 128 positions, which the tensor cores cut towards zero.
- * Values below 2^-80 keep fewer bits behind thousands of positions. oq / os (may be NULL): out quantized for Wo as k_quantize does, gs dividing head_dim. head_dim <= 256.
- * `work` (k_attention_paged_init, released with k_attention_free): partial results and tickets for this n_heads and
- * head_dim and up to batch * rows rows (its `workers`; its max_chunks is -1, so that no other kind of work passes for it);
- * `memory` as for k_attention_init_rows (k_attention_paged_bytes bytes, 16-byte aligned, or NULL). k_attention_paged_init
- * zeroes the tickets on the calling thread's stream, and every call leaves them zeroed. One call in flight per work. */
+/* Attention over a paged cache: q and out [batch][rows][n_heads * head_dim], which do not overlap; row r of request b,
+ * r < counts[b] (NULL: rows for all), sees positions [0, starts[b] + r] of its pages: starts[b] were stored before this
+ * step's rows (one row: a request's last token; more: its drafts behind it). Other rows of out stay as they were, and a
+ * request that uses none needs no starts[b] and no pages. A request with starts[b] outside [0, max_pages * page_size -
+ * counts[b]], counts[b] outside [0, rows], or a page that it sees outside [0, pages) raises an error (kc_status) and
+ * its rows stay as they were. What a row sees must be finite, and so must its scores in fp32, or that row has no
+ * result; what it does not see, finite or not (the rest of a page, pages no one uses, later drafts), changes nothing in
+ * it. Products are fp32 ones up to 2^-22 of each (an fp16 cache with head_dim 64 or 128: of a query's elements down to
+ * 2^-39 of its largest and of weights down to 2^-32 of their row's largest; smaller ones are off by up to 2^-61 and
+ * 2^-54 of the largest), sums and statistics fp32: rounded to nearest, but for the sums of 16-bit caches with head_dim
+ * 64 or 128 over the head and over 128 positions, which the tensor cores cut towards zero. Values below 2^-80 keep
+ * fewer bits behind thousands of positions. oq / os (may be NULL): out quantized for Wo as k_quantize does, gs dividing
+ * head_dim. head_dim <= 256. `work` (k_attention_paged_init, released with k_attention_free): partial results and
+ * tickets for this n_heads and head_dim and up to batch * rows rows (its `workers`; its max_chunks is -1, so that no
+ * other kind of work passes for it); `memory` as for k_attention_init_rows (k_attention_paged_bytes bytes, 16-byte
+ * aligned, or NULL). k_attention_paged_init zeroes the tickets on the calling thread's stream, and every call leaves
+ * them zeroed. One call in flight per work. */
 size_t k_attention_paged_bytes(int n_heads, int n_kv_heads, int head_dim, int batch, int rows);
 void k_attention_paged_init(AttentionWork *work, int n_heads, int n_kv_heads, int head_dim, int batch, int rows,
                             void *memory);

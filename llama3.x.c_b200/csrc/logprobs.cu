@@ -10,9 +10,10 @@
 // way of the threads' maxima: with the threads in 64 classes, every one of the top k elements is at or above the k-th largest
 // class maximum, which about as many threads reach as there are tokens to find; only their elements, at a fixed stride,
 // are read again (from L2).
-// What bounds it: many rows, memory: 2048 rows of 128256 184 us, 5.7 TB/s, with 10 us for the last rows' ends; few rows the
-// chain of a row's end, 6 us, a part's stream (12 us for 128256 logits by one CTA) and a cluster's two barriers, 2 us: 64
-// rows of 128256 with 20 alternatives 18.5 us.
+// What bounds it: many rows, memory: 2048 rows of 128256 181 us in a graph of calls, 5.8 TB/s, with 10 us for the last rows'
+// ends (193 to 200 call by call from Python); few rows the chain of a row's end, 6 us, a part's stream (12 us for 128256 logits
+// by one CTA) and a cluster's two barriers, 2 us: 64 rows of 128256 with 20 alternatives 18.3 us in a graph, 19.5 to 20.5 call by
+// call.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>

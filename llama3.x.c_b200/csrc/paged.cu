@@ -10,6 +10,9 @@
 // all segments form one row, of which every CTA takes an equal, contiguous share, whatever the requests' lengths are. A
 // segment that lies in several shares leaves partial results (m, l = sum 2^(s' - m), o = sum 2^(s' - m) v) that the CTA
 // to finish last joins, in the order of the shares.
+//
+// Times in these files are device times in a graph of calls, except where "back to back" stands: calls of the Python mirror one
+// after another, whose own work is 6 to 8 us each.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -63,8 +66,10 @@ __device__ __forceinline__ void put4(__half *at, float4 x) {
 }
 
 // head_dim a multiple of four and everything aligned to four elements: a CTA, or a few with few rows, to a row; each thread
-// has kStoreUnits units of four elements on their way at once (a thread per pair of elements took 33 us for what takes 8.5).
-// What bounds it: memory, with two waves of CTAs, 2048 rows of 32/8 heads of 128 22 us, 4.3 TB/s; with few rows the chain starts, page and rotation, store (one row 1.8 us).
+// has kStoreUnits units of four elements on their way at once (by the kernel for any alignment below, a thread per pair of
+// elements, 2048 rows of 32/8 heads of 128 in bf16 take 57 us instead of 22, 514 rows 33 instead of 8.6).
+// What bounds it: memory, with two waves of CTAs, 2048 rows 22 us, 4.3 TB/s; with few rows the chain starts, page and rotation,
+// store (one row 1.7 us).
 constexpr int kStoreThreads = 256, kStoreUnits = 6;
 template <typename T>
 __global__ void __launch_bounds__(kStoreThreads) paged_store4_kernel(const StoreArgs a) {
@@ -180,10 +185,10 @@ __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
 // The kernel on the CUDA cores: any type, head_dim up to 256, any alignment. LANES lanes take a position, 16 of its
 // elements each, so that a score costs log2(LANES) shuffles for 16 LANES products, and its weight meets the values in the
 // same lanes without another; four query vectors in registers share each key and value (eight with eight elements to a lane,
-// half the passes over the keys and values, took longer: 24 requests of 28/4 heads of 96 up to 3001 positions 108 us against
-// 75). Every warp has a ring of its own in shared memory, which each lane fills for itself, asynchronously, and reads itself:
+// half the passes over the keys and values, took longer: 24 requests of 28/4 heads of 96 up to 3001 positions 108 us back to
+// back against 75). Every warp has a ring of its own in shared memory, which each lane fills for itself, asynchronously, and reads itself:
 // no barrier until the end of a piece. What bounds it: its instructions, three warps to a scheduler that issue one every
-// 2.8 cycles (32/8 heads of 96 in bf16, 24 requests: 80 us, 1.7 TB/s).
+// 2.8 cycles (32/8 heads of 96 in bf16, 24 requests: 82 us, 1.7 TB/s; 28/4 heads of 96 76 us).
 constexpr int kVecs = 4, kElems = 16, kPairs = kElems / 2;
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kTile = 64;       // positions

@@ -11,8 +11,8 @@
 // The 16-byte units of a row lie in an order that spreads eight rows over the banks.
 // What bounds it: a tile's three steps take 3.0 thousand clocks (1.2 scores, 0.5 softmax, 1.2 sums; FMAs alone 1.0), its
 // copies 2.9; with eight vectors where a KV head has fewer, some of that is for nothing. 24 requests of 28/4 heads of 128 up to
-// 3001 positions: 51 us, 3.5 TB/s, of which 9 until the first tile is there and 5 for the joins (in the kernel on the CUDA
-// cores in paged.cu 125).
+// 3001 positions: 50 us, 3.6 TB/s, of which 28 are for the tiles' bytes, 9 until the first tile is there and 5 for the joins; the
+// other 8 have not been told apart.
 #include "paged.cuh"
 #include "tcgen05.cuh"
 
@@ -343,6 +343,13 @@ cudaError_t launch(const PagedArgs &a) {
 
 }  // namespace
 
+// Everything that its copies can bring goes here: the kernel on the CUDA cores in paged.cu is slower at all of it. us here and
+// there: 24 requests of one row, up to 3001 positions, heads of 32, 64, 96, 128:
+//   28/4 heads   33.9, 34.6, 48.6, 50.1    69.1, 86.4, 139, 151      32/8   57.2, 58.0, 79.0, 80.0    77.4, 98.5, 150, 160
+//   16/16        104, 104, 142, 142        140, 167, 269, 287        8/2    22.7, 22.6, 28.4, 28.8    31.5, 36.6, 48.1, 56.9
+//   48/1         46.7, 46.5, 62.8, 62.1    96.4, 112, 173, 181
+// 1 request of 512 positions, 32/8 heads of 4, 16, 128: 9.7, 9.7, 10.4    15.1, 15.3, 22.0. 2 requests of up to 64 rows, 512
+// positions, 32/8 heads of 64: 31.0    71.9.
 bool kc_paged_f32_ok(const PagedArgs &a, int type) {
   return type == K_F32 && a.hd % 4 == 0 && a.hd <= 128 && a.page_stride % 4 == 0 &&
          !(((uintptr_t)a.key | (uintptr_t)a.value) & 15);

@@ -22,14 +22,16 @@
 // (4 or 8 to a thread: with all 32 of the largest block in one group, a tile took 3.9 us); one that issues the MMAs; one to
 // three that lay out the next segment's queries; four that copy the tiles, asynchronously, through a ring of stages. With up
 // to eight vectors two more finish a segment (by the softmax warps themselves that takes 2 us of their time, and the shares
-// of many short segments ended last: 8 requests of up to 2048 positions 19 us with them against 22), but for a share's last,
-// for which the softmax warps are faster; with more vectors those do it all (80 requests' rows behind 4099: 58 us against 64).
+// of many short segments ended last: 8 requests of up to 2048 positions 19 us back to back with them against 22), but for a
+// share's last, for which the softmax warps are faster; with more vectors those do it all (16 requests of up to five rows behind
+// 4099, in blocks of 32: 58 us back to back against 64).
 //
-// What bounds it (32/8 heads of 128 in bf16): for long requests memory, 64 of up to 8192 positions 209 us, 6.4 TB/s of the
-// copy's 6.55, 1.5 us a tile; with 20 vectors the softmax warps, 2.5 thousand clocks a tile, a chain of dependent steps (the
-// tensor pipe is 12 % busy, the issue slots 39 %); for short ones the way to the first tile (5 us: the share, pages, copies)
-// and the join of the pieces (4 us: results to memory, ticket, results back), which the code of those rare steps, fetched anew
-// each time, makes longer: 8 requests of up to 2048 positions 16 us, 2.4 TB/s.
+// What bounds it (32/8 heads of 128): for long requests memory, 64 of up to 8192 positions in bf16 205 us, 6.5 TB/s of the
+// copy's 6.55, 1.5 us a tile; with 20 vectors, 16 requests of up to five rows behind 4099 48 us, nothing that is full (DRAM 41 %,
+// issue slots 46 %, tensor pipe 9 % under a profiler): chains of dependent steps in the softmax and in the joins; for short ones
+// the way to the first tile (5 us: the share, pages, copies) and the join of the pieces (4 us: results to memory, ticket, results
+// back), which the code of those rare steps, fetched anew each time, makes longer: 8 requests of up to 2048 positions in fp16
+// 16.4 us, 2.4 TB/s.
 //
 // A later draft's key or value of any kind must not reach the rows before it, not even with a weight of zero: a key gives
 // scores in its own row of S^T only, which are masked; a value with an infinity or a NaN behind the block's first row is

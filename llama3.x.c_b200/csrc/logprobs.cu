@@ -10,10 +10,9 @@
 // way of the threads' maxima: with the threads in 64 classes, every one of the top k elements is at or above the k-th largest
 // class maximum, which about as many threads reach as there are tokens to find; only their elements, at a fixed stride,
 // are read again (from L2).
-// What bounds it: many rows, memory: 2048 rows of 128256 181 us in a graph of calls, 5.8 TB/s, with 10 us for the last rows'
-// ends (193 to 200 call by call from Python); few rows the chain of a row's end, 6 us, a part's stream (12 us for 128256 logits
-// by one CTA) and a cluster's two barriers, 2 us: 64 rows of 128256 with 20 alternatives 18.3 us in a graph, 19.5 to 20.5 call by
-// call.
+// What bounds it: many rows, memory: 2048 rows of 128256 180 us in a graph of calls, 5.8 TB/s, with 10 us for the last rows'
+// ends (193 call by call from Python); few rows the chain of a row's end, 6 us, a part's stream (12 us for 128256 logits
+// by one CTA) and a cluster's two barriers, 2 us: 64 rows of 128256 with 20 alternatives 18.1 us in a graph, 18.7 call by call.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -94,9 +93,6 @@ __device__ __forceinline__ unsigned long long pair_key(float x, unsigned pair) {
 __device__ __forceinline__ float edge_element(const UnitRow &r, int unit, int i) {
   const int at = element_of(r, unit, i);
   return at >= 0 ? __ldcg(r.data + at) : -INFINITY;
-}
-__device__ __forceinline__ float4 edge_unit(const UnitRow &r, int unit) {
-  return make_float4(edge_element(r, unit, 0), edge_element(r, unit, 1), edge_element(r, unit, 2), edge_element(r, unit, 3));
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -198,50 +194,44 @@ __global__ void __launch_bounds__(kThreads + 32, kCtas) logprobs_kernel(const Lo
 
   if (warp == kWarps) {
     // ---- copies ----
-    if (lane == 0) {
-      bool ok = true;
-      unsigned fills = 0;  // of the ring's stages
-      for (int row = blockIdx.x / parts; ok && row < a.rows; row += stride) {
-        if (a.tokens && a.tokens[row] == -1)
-          continue;
-        const UnitRow r = unit_row(a.logits + (size_t)row * a.ld, a.vocab);
-        int first, end;
-        part_of(r, part, parts, &first, &end);
-        // The part's first and last unit by their elements where not all of them are the row's.
-        int whole0, whole1;
-        whole_of(r, first, end, &whole0, &whole1);
-        float4 head, tail;
-        if (first < whole0)
-          head = edge_unit(r, first);
-        if (whole1 < end)
-          tail = edge_unit(r, whole1);
-        for (int u = first; ok && u < end; u += kUnits) {
-          const int upto = min(u + kUnits, end), from = max(u, whole0), to = min(upto, whole1);
-          float4 *const slot = reinterpret_cast<float4 *>(smem + stage * kUnits * 16);
-          ok = mbar_wait_bounded(&t->empty[stage], parity ^ 1);
-          if (ok) {
-            if (from < to) {
-              mbar_expect_tx(&t->full[stage], 16u * (unsigned)(to - from));
-              bulk_g2s(slot + (from - u), unit_at(r, from), 16u * (unsigned)(to - from), &t->full[stage]);
-            }
-            if (from > u)
-              slot[0] = head;
-            if (to < upto)
-              slot[to - u] = tail;
-            if (to - from < upto - u)
-              fence_proxy_async_smem();  // before a later copy's writes
-            mbar_arrive(&t->full[stage]);
-            fills++;
-          }
-          if (++stage == kStages)
-            stage = 0, parity ^= 1;
+    bool ok = true;
+    unsigned fills = 0;  // of the ring's stages
+    for (int row = blockIdx.x / parts; ok && row < a.rows; row += stride) {
+      if (a.tokens && a.tokens[row] == -1)
+        continue;
+      const UnitRow r = unit_row(a.logits + (size_t)row * a.ld, a.vocab);
+      int first, end, whole0, whole1;
+      part_of(r, part, parts, &first, &end);
+      whole_of(r, first, end, &whole0, &whole1);
+      // The part's first and last unit where not all of them are the row's: an element each of lanes 0 to 3 and 4 to 7.
+      const float edge = lane < 8 ? edge_element(r, lane < 4 ? first : end - 1, lane & 3) : 0.0f;
+      for (int u = first; ok && u < end; u += kUnits) {
+        const int upto = min(u + kUnits, end), from = max(u, whole0), to = min(upto, whole1);
+        float4 *const slot = reinterpret_cast<float4 *>(smem + stage * kUnits * 16);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&t->empty[stage], parity ^ 1));
+        if (!ok)
+          break;
+        if (lane == 0 && from < to) {
+          mbar_expect_tx(&t->full[stage], 16u * (unsigned)(to - from));
+          bulk_g2s(slot + (from - u), unit_at(r, from), 16u * (unsigned)(to - from), &t->full[stage]);
         }
+        if (to - from < upto - u) {
+          if (lane < 4 ? from > u : lane < 8 && to < upto)
+            reinterpret_cast<float *>(slot + (lane < 4 ? 0 : to - u))[lane & 3] = edge;
+          fence_proxy_async_smem();  // before a later copy's writes
+          __syncwarp();
+        }
+        if (lane == 0)
+          mbar_arrive(&t->full[stage]);
+        fills++;
+        if (++stage == kStages)
+          stage = 0, parity ^= 1;
       }
-      // No copy is under way when the CTA ends, also where a wait, here or of those who take the logits, has run out.
-#pragma unroll 1
-      for (unsigned i = fills > kStages ? fills - kStages : 0; i < fills; i++)
-        mbar_wait_sleep_bounded(&t->full[i % kStages], (i / kStages) & 1);
     }
+    // No copy is under way when the CTA ends, also where a wait, here or of those who take the logits, has run out.
+#pragma unroll 1
+    for (unsigned i = fills > kStages ? fills - kStages : 0; i < fills; i++)
+      mbar_wait_sleep_bounded(&t->full[i % kStages], (i / kStages) & 1);
     __syncwarp();
   } else {
     bool ok = true;  // no wait has run out
@@ -564,10 +554,10 @@ extern "C" void k_token_logprobs(float *logprobs, float *entropy, int *top_token
   a.logits = logits, a.ld = ld, a.tokens = tokens, a.vocab = vocab, a.rows = rows, a.top = top;
   // A cluster of CTAs to a row while their parts are long enough to pay for its two barriers, which cost more where CTAs share
   // their SMs; and one CTA where the rows have an SM each with few left over. Device time in a graph, us, by parts (rows x
-  // vocabulary: in 1, 2, 4, 8): 1 x 32000: 9.3, 8.9, 8.6, 9.4; 8 x 32000: 9.2, 9.1, 8.7, 9.6; 64 x 32000: 9.4, 9.6, 11.2;
-  // 8 x 128256: 18.7, 13.6, 11.1, 10.8; 30 x 50001: 11.3, 10.3, 10.4, 14.1; 37 x 128256: 18.9, 13.8, 12.7, 15.5; 64 x 128256:
-  // 19.0, 15.4, 15.7; 32 x 262144: 31.9, 20.4, 16.7, 18.0; 74 x 65000: 12.3, 12.1, 12.9; 100 x 128256: 19.1, 17.0, 16.1;
-  // 110: 19.2, 17.0; 120: 19.1, 21.3; 148: 19.2, 21.3; 160: 24.8, 21.7; 200: 26.2, 23.4; 129 x 50001: 11.6, 14.4.
+  // vocabulary: in 1, 2, 4, 8): 1 x 32000: 8.8, 8.4, 8.2, 9.0; 8 x 32000: 9.0, 8.7, 8.5, 9.4; 64 x 32000: 9.2, 9.4, 11.0;
+  // 8 x 128256: 18.8, 13.4, 11.0, 10.7; 30 x 50001: 11.2, 10.2, 10.2, 13.8; 37 x 128256: 19.0, 13.8, 12.5, 15.3; 64 x 128256:
+  // 19.2, 15.2, 15.5; 32 x 262144: 32.7, 20.7, 16.6, 17.8; 74 x 65000: 12.4, 12.0, 12.7; 100 x 128256: 19.2, 16.9, 15.9;
+  // 110: 19.3, 16.8; 120: 19.4, 21.1; 148: 19.3, 21.3; 160: 24.8, 21.6; 200: 26.6, 23.4; 129 x 50001: 11.5, 14.2.
   const int sms = kc_device_sms();
   int parts = 1;
   for (; parts < kMaxParts; parts *= 2) {

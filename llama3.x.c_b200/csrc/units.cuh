@@ -26,9 +26,9 @@ __host__ __device__ __forceinline__ int element_of(const UnitRow &r, int unit, i
   const long long at = 4ll * unit + i - r.off;
   return at >= 0 && at < r.n ? (int)at : -1;
 }
-// Whether all of a unit is the row's.
+// Whether all of a unit of the row is the row's.
 __host__ __device__ __forceinline__ bool whole(const UnitRow &r, int unit) {
-  return element_of(r, unit, 0) >= 0 && element_of(r, unit, 3) >= 0;
+  return !(unit == 0 && r.off) && !(unit == r.count - 1 && (((unsigned)r.off + (unsigned)r.n) & 3));
 }
 // The whole units among [first, end), which are the row's: [*from, *to).
 __host__ __device__ __forceinline__ void whole_of(const UnitRow &r, int first, int end, int *from, int *to) {

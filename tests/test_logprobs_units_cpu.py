@@ -32,7 +32,7 @@ static void check(int off, int n, int parts, int stage) {
       const int upto = u + stage < end ? u + stage : end, from = u > whole0 ? u : whole0, to = upto < whole1 ? upto : whole1;
       for (int x = u; x < upto; x++) {
         const bool copied = x >= from && x < to;
-        if (copied != whole(r, x)) { printf("off %d n %d parts %d: unit %d\n", off, n, parts, x); exit(1); }
+        if (copied != whole(r, x) || copied != (element_of(r, x, 0) >= 0 && element_of(r, x, 3) >= 0)) { printf("off %d n %d parts %d: unit %d\n", off, n, parts, x); exit(1); }
         if (copied) {
           const float *at = unit_at(r, x);
           if (((uintptr_t)at & 15) || at < row || at + 4 > row + n) { printf("off %d n %d: unit %d outside\n", off, n, x); exit(1); }
@@ -64,6 +64,7 @@ int main() {
       check(off, n, 2, 1024);
   // The largest vocabulary: nothing wraps.
   const UnitRow r = unit_row(reinterpret_cast<const float *>((uintptr_t)28), 0x7fffffff);
+  if (whole(r, 0) || !whole(r, 1) || !whole(r, r.count - 2) || whole(r, r.count - 1)) { printf("large\n"); return 1; }
   if (r.off != 3 || r.count != 0x20000001 || element_of(r, r.count - 1, 1) != 0x7ffffffe || element_of(r, r.count - 1, 2) != -1 ||
       (uintptr_t)unit_at(r, 0x1fffffff) != 16 + 16ull * 0x1fffffff) { printf("large\n"); return 1; }
   puts("ok");
